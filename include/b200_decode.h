@@ -39,8 +39,8 @@ extern "C" {
  * b200_stack_input_conv, b200_stack_pool_attention, b200_stack_bonus_scan, b200_stack_mamba1_scan;  9: + gated linear attention
  * (b200_gla_desc), capped scores, distance biases and values that are the keys (fields appended to b200_attn_desc), short
  * convolutions and per-head norms in front of any attention (fields appended to b200_attn_prep_desc and b200_pool_attn_desc),
- * gated feed-forwards in sandwich blocks.  All additive: callers of an older version keep working once they are compiled against this header. */
-#define B200_ABI_VERSION 9
+ * gated feed-forwards in sandwich blocks;  10: + weights of 4 bits (b200_w4_*) and the paged cache of 4 bits (b200_kv4_*).  All additive: callers of an older version keep working once they are compiled against this header. */
+#define B200_ABI_VERSION 10
 
 typedef enum b200_status {
   B200_OK = 0,
@@ -167,6 +167,31 @@ int b200_attn_decode_bf16(void* out, const void* qkv, const void* q_norm_or_null
 int64_t b200_sample_workspace_bytes(void);
 int b200_sample_bf16(int64_t* token_out, const void* logits, int64_t V, float temperature, int64_t top_k, float top_p,
                      float min_p, float u, void* workspace, void* stream);
+
+/* ------------------------------------------------------------------------------------------------------------------
+ * Serving in 4 bits (nothing in the reference): Linears over 4-bit weights with group scales.
+ *   W[n, k] = scale[n, k / group]·(value − zero[n, k / group]),  value 0 … 15, group 32, 64 or 128 (the last one may be shorter);
+ *   scale and zero bf16; zero NULL: 8.
+ * q: tiles of 16 rows × 64 columns of W, [(n + 15) / 16][(k + 63) / 64][512 bytes], 16-byte aligned.  Byte 16·(4r + c) + 4·(2h + t) + 2e + p of a tile (r < 8,
+ * c < 4, h, t, e, p < 2) holds, at column 32h + 8c + 4t + 2p + e, row r in its low and row r + 8 in its high half; rows and columns
+ * past the matrix hold anything.  scale / zero: [(n + 15) / 16][groups][8][2], {row r, row r + 8}, 4-byte aligned; rows past the matrix are
+ * not read into any result.
+ * ---------------------------------------------------------------------------------------------------------------- */
+typedef struct b200_w4_weight {
+  const void* q;
+  const void* scale;
+  const void* zero;     /* or NULL */
+  int32_t n, k, group;
+} b200_w4_weight;
+
+/* y[m,n] = bf16( x[m,k]·Wᵀ + bias ), fp32 sums, one rounding.  Up to 64 rows (and any number where n is no multiple of 8) the values enter the
+ * products exactly and a group's sum is scaled in fp32; more rows take W as bf16 (each weight rounded once), laid out in `workspace`
+ * (b200_w4_workspace_bytes(m, n, k) bytes, 16-byte aligned; 0 bytes: may be NULL), through the tensor-core GEMM.
+ * Requirements: k % 8 == 0, x 16-byte aligned. */
+int64_t b200_w4_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int b200_w4_linear_bf16(void* y, const void* x, const b200_w4_weight* w, const void* bias_or_null, int64_t m, void* workspace, void* stream);
+/* out[n,k] = bf16(W), 16-byte aligned. */
+int b200_w4_dequant_bf16(void* out, const b200_w4_weight* w, void* stream);
 
 /* ------------------------------------------------------------------------------------------------------------------
  * Boundary A — the whole per-token forward behind GPTModel::forward / GPTEngine::genNextToken.

@@ -139,6 +139,10 @@ class StackDesc(C.Structure):
                 ("norm_kind", C.c_int32), ("logit_softcap", C.c_float), ("streams", C.c_int32)]
 
 
+class W4Desc(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("scale", C.c_void_p), ("zero", C.c_void_p), ("n", C.c_int32), ("k", C.c_int32), ("group", C.c_int32)]
+
+
 # name -> (restype, argtypes); every symbol include/b200_decode.h declares (tests/test_abi.py checks the two agree)
 P, I64, I32, F = C.c_void_p, C.c_int64, C.c_int, C.c_float
 PROTOTYPES = {
@@ -163,6 +167,9 @@ PROTOTYPES = {
     "b200_gemv_fused_bf16": (I32, [P, P, P, I64, I64, I32, P, F, P, P, I32, P]),
     "b200_attn_decode_workspace_bytes": (I64, [I64, I64, I64, I64]),
     "b200_attn_decode_bf16": (I32, [P, P, P, P, F, P, P, I64, P, P, I64, I64, I64, I64, P, P]),
+    "b200_w4_workspace_bytes": (I64, [I64, I64, I64]),
+    "b200_w4_linear_bf16": (I32, [P, P, C.POINTER(W4Desc), P, I64, P, P]),
+    "b200_w4_dequant_bf16": (I32, [P, C.POINTER(W4Desc), P]),
     "b200_engine_create": (I32, [C.POINTER(ModelDesc), C.POINTER(WeightTable), C.POINTER(P)]),
     "b200_engine_destroy": (None, [P]),
     "b200_engine_status": (I32, [P]),

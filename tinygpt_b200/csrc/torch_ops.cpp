@@ -12,6 +12,7 @@
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/TensorSubclassLikeUtils.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -24,7 +25,7 @@ namespace {
 
 // The C ABI of the library that _lib.py has loaded, whatever its file is called: this module is linked to none.
 #define B200_FUNCTIONS(F) \
-  F(gemv_bf16) F(gemm_bf16) F(rmsnorm_bf16) F(silu_mul_bf16) F(add_bf16) F(attn_bf16) F(gemv_fused_bf16) F(attn_decode_workspace_bytes) F(attn_decode_bf16)
+  F(gemv_bf16) F(gemm_bf16) F(rmsnorm_bf16) F(silu_mul_bf16) F(add_bf16) F(attn_bf16) F(gemv_fused_bf16) F(attn_decode_workspace_bytes) F(attn_decode_bf16) F(w4_workspace_bytes) F(w4_linear_bf16)
 struct {
 #define B200_FIELD(f) decltype(&b200_##f) f;
   B200_FUNCTIONS(B200_FIELD)
@@ -69,6 +70,14 @@ PyObject* run(const at::Tensor& x, at::IntArrayRef sizes, F call) {
     rc = call(y.data_ptr(), (void*)c10::cuda::getCurrentCUDAStream().stream());
   }
   return rc == 0 ? THPVariable_Wrap(y) : PyLong_FromLong(rc);
+}
+
+// whether a tensor lies on the current device: what runs there runs on its current stream
+bool here(const at::Tensor& t) { return t.device().index() == c10::cuda::current_device(); }
+// whether a weight's parts have the sizes of its layout
+bool w4_fits(const at::Tensor& q, const at::Tensor& scale, const at::Tensor* zero, int64_t n, int64_t k, int64_t group) {
+  const int64_t tiles = (n + 15) / 16, small = tiles * 16 * ((k + group - 1) / group);
+  return q.numel() == tiles * ((k + 63) / 64) * 512 && scale.numel() == small && (zero == nullptr || zero->numel() == small);
 }
 
 // x's sizes with another last one
@@ -180,10 +189,32 @@ PyObject* attn_decode(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+PyObject* linear_w4(PyObject*, PyObject* const* a, Py_ssize_t n_args) {   // x, q, scale, zero or None, n, k, group, bias or None
+  HANDLE_TH_ERRORS
+  const at::Tensor *x, *q, *scale, *zero, *b;
+  if (n_args != 8 || modes() || !(x = plain(a[0])) || !(q = plain(a[1], at::kByte)) || !(scale = plain(a[2])) || !plain_or_none(a[3], zero) ||
+      !PyLong_Check(a[4]) || !PyLong_Check(a[5]) || !PyLong_Check(a[6]) || !plain_or_none(a[7], b) || x->dim() < 1)
+    Py_RETURN_NONE;
+  const int64_t n = PyLong_AsLongLong(a[4]), k = PyLong_AsLongLong(a[5]), group = PyLong_AsLongLong(a[6]);
+  if (n < 1 || k < 1 || group < 1 || n > 16 * 65535 || k > 1 << 24 || x->size(-1) != k || x->numel() < 1 || !w4_fits(*q, *scale, zero, n, k, group) ||
+      (b != nullptr && b->numel() != n))
+    Py_RETURN_NONE;
+  if (!here(*x) || q->device() != x->device() || scale->device() != x->device() || (zero && zero->device() != x->device()) || (b && b->device() != x->device()))
+    Py_RETURN_NONE;
+  const b200_w4_weight w{q->data_ptr(), scale->data_ptr(), ptr(zero), (int32_t)n, (int32_t)k, (int32_t)group};
+  const int64_t m = x->numel() / k, bytes = abi.w4_workspace_bytes(m, n, k);
+  return run(*x, with_last(*x, n), [&](void* y, void* st) {
+    at::Tensor ws;
+    if (bytes > 0) ws = at::empty({bytes}, at::TensorOptions().dtype(at::kByte).device(x->device()));
+    return abi.w4_linear_bf16(y, x->data_ptr(), &w, ptr(b), m, bytes > 0 ? ws.data_ptr() : nullptr, st);
+  });
+  END_HANDLE_TH_ERRORS
+}
+
 #define B200_OP(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {{"_bind", bind, METH_O, nullptr}, B200_OP(linear),     B200_OP(gemm),        B200_OP(rms_norm),
                          B200_OP(silu_mul),                B200_OP(add),        B200_OP(flash_attention),
-                         B200_OP(gemv_fused),              B200_OP(attn_decode), {nullptr, nullptr, 0, nullptr}};
+                         B200_OP(gemv_fused),              B200_OP(attn_decode), B200_OP(linear_w4), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "b200ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -6,7 +6,7 @@ Every function raises B200Error when the CUDA library or an sm_100 device is mis
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -252,6 +252,126 @@ def sample(logits: torch.Tensor, temperature: float, top_k: int = 0, top_p: floa
     out = torch.empty(1, dtype=torch.int64, device=logits.device)
     check(lib().b200_sample_bf16(out.data_ptr(), logits.data_ptr(), logits.numel(), float(temperature), int(top_k),
                                  float(top_p), float(min_p), float(u), ws.data_ptr(), _stream()), "b200_sample_bf16")
+    return out
+
+
+# ---- weights of 4 bits (csrc/w4.cu)
+W4_GROUPS = (32, 64, 128)
+
+
+class W4Weight(NamedTuple):
+    """A Linear's weight in 4 bits, laid out by w4_pack or w4_quantize: W[n, k] = scale[n, k // group]·(value − zero[n, k // group])."""
+    q: torch.Tensor                  # uint8, tiles of 16 × 64 values (include/b200_decode.h b200_w4_weight)
+    scale: torch.Tensor              # bf16 [tiles, groups, 8, 2]
+    zero: Optional[torch.Tensor]     # the same, or None: 8
+    n: int
+    k: int
+    group: int
+
+
+def w4_pack(values: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tensor] = None, *, group: int = 64) -> W4Weight:
+    """The layout linear_w4 takes, made once per weight: values [n, k] integers 0 … 15 (uint8), scale and zero bf16 [n, ceil(k / group)]."""
+    if values.dim() != 2 or values.dtype != torch.uint8:
+        raise B200Error(f"w4_pack: values must be uint8 [n, k], got {values.dtype} {tuple(values.shape)}")
+    n, k = values.shape
+    if group not in W4_GROUPS:
+        raise B200Error(f"w4_pack: groups of {group} (one of {W4_GROUPS})")
+    if n < 1 or k < 8 or k % 8:
+        raise B200Error(f"w4_pack: W [{n}, {k}]: k must be a multiple of 8")
+    groups, tiles, blocks = -(-k // group), -(-n // 16), -(-k // 64)
+    for t, name in ((scale, "scale"), (zero, "zero")):
+        if t is not None and (t.dtype != torch.bfloat16 or tuple(t.shape) != (n, groups) or t.device != values.device):
+            raise B200Error(f"w4_pack: {name} must be bf16 [{n}, {groups}] beside the values, got {t.dtype} {tuple(t.shape)}")
+    v = torch.full((tiles * 16, blocks * 64), 8, dtype=torch.uint8, device=values.device)
+    v[:n, :k] = values & 15
+    #                 tile  hi r  block h  c  t  p  e   →  tile, block, r, c, h, t, e, p, hi
+    v = v.view(tiles, 2, 8, blocks, 2, 4, 2, 2, 2).permute(0, 3, 2, 5, 4, 6, 8, 7, 1)
+    q = (v[..., 0] | v[..., 1] << 4).contiguous().view(-1)
+
+    def rows(t):
+        p = torch.zeros(tiles * 16, groups, dtype=torch.bfloat16, device=t.device)
+        p[:n] = t
+        return p.view(tiles, 2, 8, groups).permute(0, 3, 2, 1).contiguous()
+
+    return W4Weight(q, rows(scale), None if zero is None else rows(zero), n, k, group)
+
+
+def w4_quantize(weight: torch.Tensor, *, group: int = 64, symmetric: bool = True) -> W4Weight:
+    """The nearest 4-bit weight of a matrix [n, k] (bf16 or fp32), group by group: symmetric values −7 … 7 around a zero of 8, else 0 … 15 between
+    the group's least and largest entry (0 among them) with a whole zero."""
+    if weight.dim() != 2 or not weight.dtype.is_floating_point:
+        raise B200Error(f"w4_quantize: expected a matrix, got {weight.dtype} {tuple(weight.shape)}")
+    if group not in W4_GROUPS:
+        raise B200Error(f"w4_quantize: groups of {group} (one of {W4_GROUPS})")
+    n, k = weight.shape
+    groups = -(-k // group)
+    w = torch.zeros(n, groups * group, dtype=torch.float32, device=weight.device)
+    w[:, :k] = weight
+    if not bool(torch.isfinite(w).all()):
+        raise B200Error("w4_quantize: the weight is not finite")
+    w = w.view(n, groups, group)
+    hi, lo = w.amax(-1).clamp(min=0), w.amin(-1).clamp(max=0)
+    scale = (torch.maximum(hi, -lo) / 7 if symmetric else (hi - lo) / 15).to(torch.bfloat16)
+    s = scale.float().clamp(min=torch.finfo(torch.float32).tiny)[..., None]
+    zero = None if symmetric else (-lo / s[..., 0]).round().clamp(0, 15)
+    q = ((w / s).round() + (8 if symmetric else zero[..., None])).clamp(0, 15).to(torch.uint8)
+    return w4_pack(q.view(n, -1)[:, :k], scale, None if zero is None else zero.to(torch.bfloat16), group=group)
+
+
+def _w4_desc(w: W4Weight, what: str):
+    from ._lib import W4Desc
+    if not isinstance(w, W4Weight):
+        raise B200Error(f"{what}: the weight must come from w4_pack or w4_quantize")
+    tiles, groups = -(-w.n // 16), -(-w.k // w.group)
+    q, small = _chk(w.q, f"{what}.q", torch.uint8), [None if t is None else _chk(t, f"{what}.{name}") for t, name in ((w.scale, "scale"), (w.zero, "zero"))]
+    if q.numel() != tiles * -(-w.k // 64) * 512 or any(t is not None and t.numel() != tiles * groups * 16 for t in small) or small[0] is None:
+        raise B200Error(f"{what}: the weight's parts do not fit W [{w.n}, {w.k}] in groups of {w.group}")
+    return W4Desc(q.data_ptr(), small[0].data_ptr(), _ptr(small[1]), w.n, w.k, w.group), (q, *small)
+
+
+def _same_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Kernels run on the current device's current stream: the tensors must lie there."""
+    at = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != at:
+            raise B200Error(f"{what}: a tensor on {t.device} while cuda:{at} is current")
+
+
+def linear_w4(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """linear over a weight of 4 bits: x [..., k] bf16 → bf16(x·Wᵀ + bias) [..., n], fp32 sums, rounded once.  A weight enters exactly up to 64 rows; more
+    rows multiply it as bf16 (tensor-core GEMM over a copy in a workspace)."""
+    y = _fast.linear_w4(x, weight.q, weight.scale, weight.zero, weight.n, weight.k, weight.group, bias) if weight.__class__ is W4Weight else None
+    if y.__class__ is _Tensor:
+        return y
+    if y is not None:
+        check(y, "b200_w4_linear_bf16")
+    import ctypes as C
+    x = _chk(x, "linear_w4.x")
+    d, parts = _w4_desc(weight, "linear_w4")
+    n, k = weight.n, weight.k
+    if x.dim() < 1 or x.shape[-1] != k:
+        raise B200Error(f"linear_w4: x {tuple(x.shape)} does not match W[{n}, {k}]")
+    if bias is not None:
+        bias = _chk(bias, "linear_w4.bias")
+        if bias.numel() != n:
+            raise B200Error(f"linear_w4: a bias of {bias.numel()} for W[{n}, {k}]")
+    _same_device("linear_w4", x, bias, *parts)
+    y = torch.empty(*x.shape[:-1], n, dtype=torch.bfloat16, device=x.device)
+    m = x.numel() // k
+    if m:
+        ws = torch.empty(lib().b200_w4_workspace_bytes(m, n, k), dtype=torch.uint8, device=x.device)
+        check(lib().b200_w4_linear_bf16(y.data_ptr(), x.data_ptr(), C.byref(d), _ptr(bias), m, ws.data_ptr() if ws.numel() else None, _stream()),
+              "b200_w4_linear_bf16")
+    return y
+
+
+def w4_dequantize(weight: W4Weight) -> torch.Tensor:
+    """W as bf16 [n, k]."""
+    import ctypes as C
+    d, parts = _w4_desc(weight, "w4_dequantize")
+    _same_device("w4_dequantize", *parts)
+    out = torch.empty(weight.n, weight.k, dtype=torch.bfloat16, device=weight.q.device)
+    check(lib().b200_w4_dequant_bf16(out.data_ptr(), C.byref(d), _stream()), "b200_w4_dequant_bf16")
     return out
 
 
