@@ -193,6 +193,54 @@ int b200_w4_linear_bf16(void* y, const void* x, const b200_w4_weight* w, const v
 /* out[n,k] = bf16(W), 16-byte aligned. */
 int b200_w4_dequant_bf16(void* out, const b200_w4_weight* w, void* stream);
 
+/* A cache whose keys and values are held in 4 bits, in pages of 64 tokens of all heads, `layers` pools side by side under one table.
+ * Of a row of a head, 64 entries in a row are a group: with lo and hi its least and largest entry, scale = bf16(hi / 15 − lo / 15), middle = bf16(lo + 8·scale),
+ * value = clamp(rint((x − middle) / scale), −8, 7) (0 where scale is 0; fp32), and what is read is middle + scale·value.  A group that is not finite
+ * reads as NaN.  `pages`: b200_kv4_page_bytes(kv_heads, dim) bytes a page, [layers][n_pages], 16-byte aligned; their inside is the library's.
+ * table: the pages of every sequence in order, −1 behind them; length: its tokens; refs: how many sequences list a page (0: free).  All on the
+ * device; a new cache has table −1, length and refs 0.  Calls that name sequences take `seqs` (n of them, device, at most 1 024); a number outside
+ * the cache, or one that stands in seqs before, is left out (extend, fork: refused). */
+typedef struct b200_kv4_cache {
+  void* pages;
+  int32_t* table;       /* [n_seqs][max_pages] */
+  int32_t* length;      /* [n_seqs] */
+  int32_t* refs;        /* [n_pages] */
+  int32_t layers, n_pages, n_seqs, max_pages;
+  int32_t kv_heads, dim; /* dim: 64, 128, 192 or 256 */
+} b200_kv4_cache;
+int64_t b200_kv4_page_bytes(int64_t kv_heads, int64_t dim);
+
+/* k and v [rows, kv_heads, dim] bf16, rows ld_k / ld_v elements apart → one layer of the cache.  Sequence seqs[i] of the call owns rows starts[i] … starts[i + 1] − 1,
+ * which go to its positions pos[i], pos[i] + 1, … (pos −1: nowhere).  A row whose page the sequence does not have, or shares with
+ * another one, is left out.  starts has n + 1 entries and does not fall. */
+int b200_kv4_store(const b200_kv4_cache* cache, int64_t layer, const void* k, int64_t ld_k, const void* v, int64_t ld_v, const int32_t* seqs,
+                   const int32_t* starts, const int32_t* pos, int64_t n, int64_t rows, void* stream);
+/* The reverse: what the cache holds, fp32 [rows, kv_heads, dim]; zero for a row without a place. */
+int b200_kv4_load(float* k, float* v, const b200_kv4_cache* cache, int64_t layer, const int32_t* seqs, const int32_t* starts, const int32_t* pos,
+                  int64_t n, int64_t rows, void* stream);
+/* out [rows, q_heads, dim] = softmax(scale·q·Kᵀ) V over one layer.  q's rows are ld_q elements apart and belong to the sequences as above; row j of
+ * sequence i stands at position P = pos[i] + j and sees the positions p <= P that the sequence has, with window > 0 those with P − p < window.  Query head h reads
+ * key/value head h / (q_heads / kv_heads).  A row that sees nothing, or belongs to no sequence, is zero.
+ * Scores, softmax and sums are fp32; weights of the values are rounded to bf16.  dim as in the cache; q and its rows 16-byte aligned.
+ * workspace: b200_kv4_attention_workspace_bytes() bytes, 16-byte aligned, written before it is read. */
+int64_t b200_kv4_attention_workspace_bytes(const b200_kv4_cache* cache, int64_t q_heads, int64_t n, int64_t rows);
+int b200_kv4_attention(void* out, const void* q, int64_t ld_q, const b200_kv4_cache* cache, int64_t layer, int64_t q_heads, const int32_t* seqs,
+                       const int32_t* starts, const int32_t* pos, int64_t n, int64_t rows, float scale, int64_t window, void* workspace, void* stream);
+
+/* Whose the pages are.  workspace: b200_kv4_workspace_bytes() bytes, 16-byte aligned, written before it is read; device arrays of n int32.
+ * extend: room for counts[i] more tokens of each sequence, in the order of the call, whole or not at all; new pages are the lowest free ones.
+ *   pos[i]: the first new position, −1 where refused (counts negative, more than max_pages pages, or — from the first sequence on whose pages and those
+ *   of the sequences before it in the call exceed the free ones — every one that needs a page).
+ * fork: dst[i], which must be empty, becomes a copy of src[i]: whole pages are shared, a page that is not full is copied to the lowest free page, in all
+ *   layers.  done[i]: 1, or 0 where refused (no free page, dst not empty or src itself).
+ * free: the sequences' pages lose a reference, table and length are as in a new cache.
+ * compact: the pages in use behind their number, in order, move to the free ones below it, in order, in all layers; tables follow; *live: that number. */
+int64_t b200_kv4_workspace_bytes(const b200_kv4_cache* cache);
+int b200_kv4_extend(const b200_kv4_cache* cache, const int32_t* seqs, const int32_t* counts, int32_t* pos, int64_t n, void* workspace, void* stream);
+int b200_kv4_fork(const b200_kv4_cache* cache, const int32_t* src, const int32_t* dst, int32_t* done, int64_t n, void* workspace, void* stream);
+int b200_kv4_free(const b200_kv4_cache* cache, const int32_t* seqs, int64_t n, void* stream);
+int b200_kv4_compact(const b200_kv4_cache* cache, int32_t* live, void* workspace, void* stream);
+
 /* ------------------------------------------------------------------------------------------------------------------
  * Boundary A — the whole per-token forward behind GPTModel::forward / GPTEngine::genNextToken.
  * [ref: src/model/GPTModel.h:51-58 CausalLM::forward, :80-106 GPTModel; src/layer/DecoderLayer.h:38-43;

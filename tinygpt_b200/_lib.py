@@ -143,6 +143,12 @@ class W4Desc(C.Structure):
     _fields_ = [("q", C.c_void_p), ("scale", C.c_void_p), ("zero", C.c_void_p), ("n", C.c_int32), ("k", C.c_int32), ("group", C.c_int32)]
 
 
+class KV4Desc(C.Structure):
+    _fields_ = [("pages", C.c_void_p), ("table", C.c_void_p), ("length", C.c_void_p), ("refs", C.c_void_p),
+                ("layers", C.c_int32), ("n_pages", C.c_int32), ("n_seqs", C.c_int32), ("max_pages", C.c_int32),
+                ("kv_heads", C.c_int32), ("dim", C.c_int32)]
+
+
 # name -> (restype, argtypes); every symbol include/b200_decode.h declares (tests/test_abi.py checks the two agree)
 P, I64, I32, F = C.c_void_p, C.c_int64, C.c_int, C.c_float
 PROTOTYPES = {
@@ -170,6 +176,16 @@ PROTOTYPES = {
     "b200_w4_workspace_bytes": (I64, [I64, I64, I64]),
     "b200_w4_linear_bf16": (I32, [P, P, C.POINTER(W4Desc), P, I64, P, P]),
     "b200_w4_dequant_bf16": (I32, [P, C.POINTER(W4Desc), P]),
+    "b200_kv4_page_bytes": (I64, [I64, I64]),
+    "b200_kv4_store": (I32, [C.POINTER(KV4Desc), I64, P, I64, P, I64, P, P, P, I64, I64, P]),
+    "b200_kv4_load": (I32, [P, P, C.POINTER(KV4Desc), I64, P, P, P, I64, I64, P]),
+    "b200_kv4_attention_workspace_bytes": (I64, [C.POINTER(KV4Desc), I64, I64, I64]),
+    "b200_kv4_attention": (I32, [P, P, I64, C.POINTER(KV4Desc), I64, I64, P, P, P, I64, I64, F, I64, P, P]),
+    "b200_kv4_extend": (I32, [C.POINTER(KV4Desc), P, P, P, I64, P, P]),
+    "b200_kv4_fork": (I32, [C.POINTER(KV4Desc), P, P, P, I64, P, P]),
+    "b200_kv4_free": (I32, [C.POINTER(KV4Desc), P, I64, P]),
+    "b200_kv4_compact": (I32, [C.POINTER(KV4Desc), P, P, P]),
+    "b200_kv4_workspace_bytes": (I64, [C.POINTER(KV4Desc)]),
     "b200_engine_create": (I32, [C.POINTER(ModelDesc), C.POINTER(WeightTable), C.POINTER(P)]),
     "b200_engine_destroy": (None, [P]),
     "b200_engine_status": (I32, [P]),

@@ -25,7 +25,8 @@ namespace {
 
 // The C ABI of the library that _lib.py has loaded, whatever its file is called: this module is linked to none.
 #define B200_FUNCTIONS(F) \
-  F(gemv_bf16) F(gemm_bf16) F(rmsnorm_bf16) F(silu_mul_bf16) F(add_bf16) F(attn_bf16) F(gemv_fused_bf16) F(attn_decode_workspace_bytes) F(attn_decode_bf16) F(w4_workspace_bytes) F(w4_linear_bf16)
+  F(gemv_bf16) F(gemm_bf16) F(rmsnorm_bf16) F(silu_mul_bf16) F(add_bf16) F(attn_bf16) F(gemv_fused_bf16) F(attn_decode_workspace_bytes) F(attn_decode_bf16) F(w4_workspace_bytes) F(w4_linear_bf16) \
+  F(kv4_store) F(kv4_load) F(kv4_attention_workspace_bytes) F(kv4_attention) F(kv4_extend) F(kv4_fork) F(kv4_free) F(kv4_compact) F(kv4_workspace_bytes)
 struct {
 #define B200_FIELD(f) decltype(&b200_##f) f;
   B200_FUNCTIONS(B200_FIELD)
@@ -42,11 +43,11 @@ PyObject* bind(PyObject*, PyObject* handle) {   // what dlopen gave; before any 
 }
 
 // an ordinary contiguous CUDA tensor of this type, or null
-const at::Tensor* plain(PyObject* o, at::ScalarType type = at::kBFloat16) {
+const at::Tensor* plain(PyObject* o, at::ScalarType type = at::kBFloat16, bool contiguous = true) {
   if (!THPVariable_CheckExact(o)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
   if (!t.defined() || t.layout() != at::kStrided || !t.is_cuda() || t.scalar_type() != type || !t.unsafeGetTensorImpl()->has_storage() ||
-      at::isTensorSubclassLike(t) || t.key_set().has(c10::DispatchKey::Functionalize) || t._is_zerotensor() || !t.is_contiguous() || t.is_neg() ||
+      at::isTensorSubclassLike(t) || t.key_set().has(c10::DispatchKey::Functionalize) || t._is_zerotensor() || (contiguous && !t.is_contiguous()) || t.is_neg() ||
       t.is_conj())
     return nullptr;
   return &t;
@@ -211,10 +212,179 @@ PyObject* linear_w4(PyObject*, PyObject* const* a, Py_ssize_t n_args) {   // x, 
   END_HANDLE_TH_ERRORS
 }
 
+// ---- the paged cache of 4 bits.  A call starts with the cache's descriptor (its address, as KV4Cache keeps it) and its device.
+struct Kv4 {
+  const b200_kv4_cache* c;
+  int64_t device;
+  bool take(PyObject* const* a) {
+    if (modes() || !PyLong_Check(a[0]) || !PyLong_Check(a[1])) return false;
+    c = static_cast<const b200_kv4_cache*>(PyLong_AsVoidPtr(a[0]));
+    device = PyLong_AsLongLong(a[1]);
+    return c != nullptr && device == c10::cuda::current_device();
+  }
+  bool with(const at::Tensor& t) const { return t.device().index() == device; }
+  at::TensorOptions options(at::ScalarType type) const { return at::TensorOptions().dtype(type).device(at::kCUDA, (int8_t)device); }
+};
+// n whole numbers beside the cache
+const at::Tensor* numbers(const Kv4& kv, PyObject* o, int64_t n = -1) {
+  const at::Tensor* t = plain(o, at::kInt);
+  return t != nullptr && t->dim() == 1 && kv.with(*t) && (n < 0 || t->size(0) == n) ? t : nullptr;
+}
+// rows [any number, heads, dim] whose heads lie side by side
+const at::Tensor* head_rows(const Kv4& kv, PyObject* o) {
+  const at::Tensor* t = plain(o, at::kBFloat16, false);
+  return t != nullptr && t->dim() == 3 && kv.with(*t) && t->size(0) > 0 && t->size(2) == kv.c->dim && t->stride(2) == 1 && t->stride(1) == t->size(2) &&
+                 (t->size(0) == 1 || t->stride(0) >= t->size(1) * t->size(2))
+             ? t : nullptr;
+}
+int64_t row_stride(const at::Tensor& t) { return t.size(0) == 1 ? t.size(1) * t.size(2) : t.stride(0); }
+struct Kv4Where {
+  const at::Tensor *seqs, *starts, *pos;
+  int64_t n;
+  bool take(const Kv4& kv, PyObject* const* a) {
+    if (!(seqs = numbers(kv, a[0]))) return false;
+    n = seqs->size(0);
+    return (starts = numbers(kv, a[1], n + 1)) && (pos = numbers(kv, a[2], n));
+  }
+  static const int32_t* at(const at::Tensor* t) { return static_cast<const int32_t*>(t->data_ptr()); }
+};
+template <typename F>
+PyObject* status(F call) {   // of a call without a result: None was not for it, so True or the status
+  int rc;
+  {
+    pybind11::gil_scoped_release free;
+    rc = call((void*)c10::cuda::getCurrentCUDAStream().stream());
+  }
+  if (rc == 0) Py_RETURN_TRUE;
+  return PyLong_FromLong(rc);
+}
+
+int64_t whole_number(PyObject* o) {   // −1, which nothing here takes, for one that no int64 holds
+  const int64_t v = PyLong_AsLongLong(o);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return -1;
+  }
+  return v;
+}
+
+PyObject* kv4_store(PyObject*, PyObject* const* a, Py_ssize_t n_args) {   // cache, device, layer, k, v, seqs, starts, pos
+  HANDLE_TH_ERRORS
+  Kv4 kv;
+  Kv4Where w;
+  const at::Tensor *k, *v;
+  if (n_args != 8 || !kv.take(a) || !PyLong_Check(a[2]) || !(k = head_rows(kv, a[3])) || !(v = head_rows(kv, a[4])) || !w.take(kv, a + 5) ||
+      k->sizes() != v->sizes() || k->size(1) != kv.c->kv_heads)
+    Py_RETURN_NONE;
+  const int64_t layer = whole_number(a[2]);
+  return status([&](void* st) {
+    return abi.kv4_store(kv.c, layer, k->data_ptr(), row_stride(*k), v->data_ptr(), row_stride(*v), w.at(w.seqs), w.at(w.starts), w.at(w.pos), w.n, k->size(0), st);
+  });
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* kv4_load(PyObject*, PyObject* const* a, Py_ssize_t n_args) {   // cache, device, layer, seqs, starts, pos, rows
+  HANDLE_TH_ERRORS
+  Kv4 kv;
+  Kv4Where w;
+  if (n_args != 7 || !kv.take(a) || !PyLong_Check(a[2]) || !w.take(kv, a + 3) || !PyLong_Check(a[6])) Py_RETURN_NONE;
+  const int64_t layer = whole_number(a[2]), rows = whole_number(a[6]);
+  if (rows < 1 || rows > 1 << 24) Py_RETURN_NONE;
+  at::Tensor k, v;
+  int rc;
+  {
+    pybind11::gil_scoped_release free;
+    k = at::empty({rows, kv.c->kv_heads, kv.c->dim}, kv.options(at::kFloat));
+    v = at::empty_like(k);
+    rc = abi.kv4_load(static_cast<float*>(k.data_ptr()), static_cast<float*>(v.data_ptr()), kv.c, layer, w.at(w.seqs), w.at(w.starts), w.at(w.pos), w.n, rows,
+                      (void*)c10::cuda::getCurrentCUDAStream().stream());
+  }
+  if (rc != 0) return PyLong_FromLong(rc);
+  PyObject *pk = THPVariable_Wrap(k), *pv = THPVariable_Wrap(v);
+  PyObject* both = pk && pv ? PyTuple_Pack(2, pk, pv) : nullptr;
+  Py_XDECREF(pk);
+  Py_XDECREF(pv);
+  return both;
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* kv4_attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {   // cache, device, layer, q, seqs, starts, pos, scale, window
+  HANDLE_TH_ERRORS
+  Kv4 kv;
+  Kv4Where w;
+  const at::Tensor* q;
+  if (n_args != 9 || !kv.take(a) || !PyLong_Check(a[2]) || !(q = head_rows(kv, a[3])) || !w.take(kv, a + 4) || !PyFloat_Check(a[7]) || !PyLong_Check(a[8]))
+    Py_RETURN_NONE;
+  const int64_t layer = whole_number(a[2]), window = whole_number(a[8]), heads = q->size(1), rows = q->size(0);
+  const float scale = (float)PyFloat_AS_DOUBLE(a[7]);
+  const int64_t bytes = abi.kv4_attention_workspace_bytes(kv.c, heads, w.n, rows);
+  if (bytes < 0) Py_RETURN_NONE;
+  return run(*q, q->sizes(), [&](void* y, void* st) {
+    at::Tensor ws;
+    if (bytes > 0) ws = at::empty({bytes}, kv.options(at::kByte));
+    return abi.kv4_attention(y, q->data_ptr(), row_stride(*q), kv.c, layer, heads, w.at(w.seqs), w.at(w.starts), w.at(w.pos), w.n, rows, scale, window,
+                             bytes > 0 ? ws.data_ptr() : nullptr, st);
+  });
+  END_HANDLE_TH_ERRORS
+}
+
+// Bookkeeping: `first` and `second` lists of n numbers → n numbers
+template <typename F>
+PyObject* kv4_lists(PyObject* const* a, Py_ssize_t n_args, F call) {   // cache, device, first, second
+  Kv4 kv;
+  const at::Tensor *x, *y;
+  if (n_args != 4 || !kv.take(a) || !(x = numbers(kv, a[2])) || !(y = numbers(kv, a[3], x->size(0))) || x->size(0) < 1) Py_RETURN_NONE;
+  at::Tensor out;
+  int rc;
+  {
+    pybind11::gil_scoped_release free;
+    out = at::empty({x->size(0)}, kv.options(at::kInt));
+    const at::Tensor ws = at::empty({abi.kv4_workspace_bytes(kv.c)}, kv.options(at::kByte));
+    rc = call(kv.c, Kv4Where::at(x), Kv4Where::at(y), static_cast<int32_t*>(out.data_ptr()), x->size(0), ws.data_ptr(),
+              (void*)c10::cuda::getCurrentCUDAStream().stream());
+  }
+  return rc == 0 ? THPVariable_Wrap(out) : PyLong_FromLong(rc);
+}
+PyObject* kv4_extend(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  return kv4_lists(a, n_args, abi.kv4_extend);
+  END_HANDLE_TH_ERRORS
+}
+PyObject* kv4_fork(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  return kv4_lists(a, n_args, abi.kv4_fork);
+  END_HANDLE_TH_ERRORS
+}
+PyObject* kv4_free(PyObject*, PyObject* const* a, Py_ssize_t n_args) {   // cache, device, seqs
+  HANDLE_TH_ERRORS
+  Kv4 kv;
+  const at::Tensor* s;
+  if (n_args != 3 || !kv.take(a) || !(s = numbers(kv, a[2])) || s->size(0) < 1) Py_RETURN_NONE;
+  return status([&](void* st) { return abi.kv4_free(kv.c, Kv4Where::at(s), s->size(0), st); });
+  END_HANDLE_TH_ERRORS
+}
+PyObject* kv4_compact(PyObject*, PyObject* const* a, Py_ssize_t n_args) {   // cache, device
+  HANDLE_TH_ERRORS
+  Kv4 kv;
+  if (n_args != 2 || !kv.take(a)) Py_RETURN_NONE;
+  at::Tensor out;
+  int rc;
+  {
+    pybind11::gil_scoped_release free;
+    out = at::empty({1}, kv.options(at::kInt));
+    const at::Tensor ws = at::empty({abi.kv4_workspace_bytes(kv.c)}, kv.options(at::kByte));
+    rc = abi.kv4_compact(kv.c, static_cast<int32_t*>(out.data_ptr()), ws.data_ptr(), (void*)c10::cuda::getCurrentCUDAStream().stream());
+  }
+  return rc == 0 ? THPVariable_Wrap(out) : PyLong_FromLong(rc);
+  END_HANDLE_TH_ERRORS
+}
+
 #define B200_OP(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {{"_bind", bind, METH_O, nullptr}, B200_OP(linear),     B200_OP(gemm),        B200_OP(rms_norm),
                          B200_OP(silu_mul),                B200_OP(add),        B200_OP(flash_attention),
-                         B200_OP(gemv_fused),              B200_OP(attn_decode), B200_OP(linear_w4), {nullptr, nullptr, 0, nullptr}};
+                         B200_OP(gemv_fused),              B200_OP(attn_decode), B200_OP(linear_w4),
+                         B200_OP(kv4_store), B200_OP(kv4_load), B200_OP(kv4_attention), B200_OP(kv4_extend), B200_OP(kv4_fork), B200_OP(kv4_free),
+                         B200_OP(kv4_compact), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "b200ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

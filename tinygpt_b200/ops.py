@@ -375,6 +375,197 @@ def w4_dequantize(weight: W4Weight) -> torch.Tensor:
     return out
 
 
+# ---- the paged cache of 4-bit keys and values (csrc/kv4.cu, kv4_attn.cu, kv4_pages.cu)
+KV4_PAGE, KV4_GROUP, KV4_MAX_SEQS = 64, 64, 1024
+
+
+class KV4Cache:
+    """Keys and values of many sequences and layers in 4 bits, in pages of 64 tokens (include/b200_decode.h b200_kv4_cache), made by kv4_cache.  pages
+    uint8 [layers, n_pages, bytes]; table int32 [n_seqs, max_pages], length int32 [n_seqs], refs int32 [n_pages]: read them as you like."""
+    __slots__ = ("pages", "table", "length", "refs", "layers", "n_pages", "n_seqs", "max_pages", "kv_heads", "head_dim", "_desc", "_at")
+
+    def __init__(self, pages, table, length, refs, kv_heads, head_dim):
+        import ctypes as C
+        from ._lib import KV4Desc
+        put = lambda **kw: [object.__setattr__(self, name, value) for name, value in kw.items()]
+        put(pages=pages, table=table, length=length, refs=refs, layers=pages.shape[0], n_pages=pages.shape[1], n_seqs=table.shape[0],
+            max_pages=table.shape[1], kv_heads=kv_heads, head_dim=head_dim)
+        put(_desc=KV4Desc(pages.data_ptr(), table.data_ptr(), length.data_ptr(), refs.data_ptr(), self.layers, self.n_pages, self.n_seqs, self.max_pages,
+                          kv_heads, head_dim))
+        put(_at=(C.addressof(self._desc), pages.device.index))
+
+    def __setattr__(self, name, value):   # kernels hold the tensors' addresses
+        raise AttributeError(f"KV4Cache.{name} cannot be replaced; write into it")
+
+
+def kv4_cache(layers: int, n_pages: int, n_seqs: int, max_pages: int, kv_heads: int, head_dim: int, device=None) -> KV4Cache:
+    """An empty cache: n_pages pages of 64 tokens a layer, for n_seqs sequences of up to max_pages pages; head_dim 64, 128, 192 or 256."""
+    for v, name in ((layers, "layers"), (n_pages, "n_pages"), (n_seqs, "n_seqs"), (max_pages, "max_pages"), (kv_heads, "kv_heads")):
+        if int(v) < 1 or int(v) >= 1 << 24:
+            raise B200Error(f"kv4_cache: {name} = {v}")
+    page = lib().b200_kv4_page_bytes(kv_heads, head_dim)
+    if page < 0:
+        raise B200Error(f"kv4_cache: {kv_heads} heads of {head_dim} (64, 128, 192 or 256)")
+    check(lib().b200_device_check(), "kv4_cache")
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    if device.type != "cuda":
+        raise B200Error("kv4_cache: the cache must live on a CUDA device (there is no CPU path)")
+    return KV4Cache(torch.empty(layers, n_pages, page, dtype=torch.uint8, device=device),
+                    torch.full((n_seqs, max_pages), -1, dtype=torch.int32, device=device), torch.zeros(n_seqs, dtype=torch.int32, device=device),
+                    torch.zeros(n_pages, dtype=torch.int32, device=device), int(kv_heads), int(head_dim))
+
+
+def _kv4(cache: KV4Cache, what: str, **numbers: torch.Tensor):
+    """The cache's descriptor and lists of whole numbers beside it, checked."""
+    import ctypes as C
+    if cache.__class__ is not KV4Cache:
+        raise B200Error(f"{what}: expected a KV4Cache")
+    got = [_chk(t, f"{what}.{name}", torch.int32) for name, t in numbers.items()]
+    for t, name in zip(got, numbers):
+        if t.dim() != 1:
+            raise B200Error(f"{what}.{name}: expected a list of numbers, got {tuple(t.shape)}")
+    _same_device(what, cache.pages, *got)
+    return (C.byref(cache._desc), *got)
+
+
+def _kv4_where(cache, what, seqs, starts, pos):
+    got = _kv4(cache, what, seqs=seqs, starts=starts, pos=pos)
+    n = got[1].shape[0]
+    if got[2].shape[0] != n + 1 or got[3].shape[0] != n:
+        raise B200Error(f"{what}: {n} sequences take {n + 1} starts and {n} positions, got {got[2].shape[0]} and {got[3].shape[0]}")
+    if n > KV4_MAX_SEQS:
+        raise B200Error(f"{what}: {n} sequences in a call (at most {KV4_MAX_SEQS})")
+    return got
+
+
+def _kv4_rows(t: torch.Tensor, what: str, heads: Optional[int], dim: int):
+    if not t.is_cuda:
+        raise B200Error(f"{what}: tensor must live on a CUDA device (there is no CPU path)")
+    if t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
+        raise B200Error(f"{what}: expected bf16 [rows, {heads or 'heads'}, {dim}], got {t.dtype} {tuple(t.shape)}")
+    _same_device(what, t)
+    if t.stride(2) != 1 or t.stride(1) != dim or (t.shape[0] > 1 and t.stride(0) < t.shape[1] * dim):
+        t = t.contiguous()
+    return t, t.shape[1] * dim if t.shape[0] <= 1 else t.stride(0)
+
+
+def kv4_store(cache: KV4Cache, layer: int, k: torch.Tensor, v: torch.Tensor, seqs: torch.Tensor, starts: torch.Tensor, pos: torch.Tensor) -> None:
+    """Rows of k and v bf16 [rows, kv_heads, head_dim] (row strides may differ: slices of one projection) → the cache, in 4 bits.  Sequence seqs[i] owns
+    rows starts[i] … starts[i + 1] − 1, for its positions pos[i], pos[i] + 1, … (what kv4_extend answered; −1: nowhere).  A row whose page the
+    sequence does not have, or shares, is left out.  seqs, starts (one more), pos: int32 on the device."""
+    y = _fast.kv4_store(*cache._at, layer, k, v, seqs, starts, pos) if cache.__class__ is KV4Cache else None
+    if y is True:
+        return
+    if y is not None:
+        check(y, "b200_kv4_store")
+    d, seqs, starts, pos = _kv4_where(cache, "kv4_store", seqs, starts, pos)
+    k, ld_k = _kv4_rows(k, "kv4_store.k", cache.kv_heads, cache.head_dim)
+    v, ld_v = _kv4_rows(v, "kv4_store.v", cache.kv_heads, cache.head_dim)
+    if k.shape != v.shape:
+        raise B200Error("kv4_store: k and v differ in rows")
+    if k.shape[0] and seqs.shape[0]:
+        check(lib().b200_kv4_store(d, int(layer), k.data_ptr(), ld_k, v.data_ptr(), ld_v, seqs.data_ptr(), starts.data_ptr(), pos.data_ptr(), seqs.shape[0],
+                                   k.shape[0], _stream()), "b200_kv4_store")
+
+
+def kv4_load(cache: KV4Cache, layer: int, seqs: torch.Tensor, starts: torch.Tensor, pos: torch.Tensor, rows: int):
+    """What the cache holds at the places that kv4_store would write: (k, v) fp32 [rows, kv_heads, head_dim], zero for a row without a place."""
+    y = _fast.kv4_load(*cache._at, layer, seqs, starts, pos, rows) if cache.__class__ is KV4Cache else None
+    if y.__class__ is tuple:
+        return y
+    if y is not None:
+        check(y, "b200_kv4_load")
+    d, seqs, starts, pos = _kv4_where(cache, "kv4_load", seqs, starts, pos)
+    if rows < 0:
+        raise B200Error(f"kv4_load: {rows} rows")
+    k, v = (torch.zeros(rows, cache.kv_heads, cache.head_dim, dtype=torch.float32, device=cache.pages.device) for _ in range(2))
+    if rows and seqs.shape[0]:
+        check(lib().b200_kv4_load(k.data_ptr(), v.data_ptr(), d, int(layer), seqs.data_ptr(), starts.data_ptr(), pos.data_ptr(), seqs.shape[0], rows,
+                                  _stream()), "b200_kv4_load")
+    return k, v
+
+
+def kv4_attention(cache: KV4Cache, layer: int, q: torch.Tensor, seqs: torch.Tensor, starts: torch.Tensor, pos: torch.Tensor, *,
+                  scale: Optional[float] = None, window: int = 0) -> torch.Tensor:
+    """Causal attention of q bf16 [rows, q_heads, head_dim] over the cache → the same shape.  Rows belong to sequences as in kv4_store; the row at position
+    P sees the sequence's positions p ≤ P, with a window those with P − p < window.  scale: head_dim^(−1/2) unless given.  A row that sees nothing is zero."""
+    if cache.__class__ is KV4Cache:
+        if scale is None:
+            scale = cache.head_dim ** -0.5
+        y = _fast.kv4_attention(*cache._at, layer, q, seqs, starts, pos, scale, window)
+        if y.__class__ is _Tensor:
+            return y
+        if y is not None:
+            check(y, "b200_kv4_attention")
+    d, seqs, starts, pos = _kv4_where(cache, "kv4_attention", seqs, starts, pos)
+    q, ld_q = _kv4_rows(q, "kv4_attention.q", None, cache.head_dim)
+    rows, heads, n = q.shape[0], q.shape[1], seqs.shape[0]
+    if heads < 1 or heads % cache.kv_heads:
+        raise B200Error(f"kv4_attention: {heads} query heads over {cache.kv_heads} key/value heads")
+    if not rows or not n:
+        return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ws = torch.empty(lib().b200_kv4_attention_workspace_bytes(d, heads, n, rows), dtype=torch.uint8, device=q.device)
+    check(lib().b200_kv4_attention(out.data_ptr(), q.data_ptr(), ld_q, d, int(layer), heads, seqs.data_ptr(), starts.data_ptr(), pos.data_ptr(), n, rows,
+                                   float(scale), int(window), ws.data_ptr() if ws.numel() else None, _stream()), "b200_kv4_attention")
+    return out
+
+
+def _kv4_lists(cache, name, a, b, names):
+    y = getattr(_fast, name)(*cache._at, a, b) if cache.__class__ is KV4Cache else None
+    if y.__class__ is _Tensor:
+        return y
+    if y is not None:
+        check(y, f"b200_{name}")
+    d, a, b = _kv4(cache, name, **dict(zip(names, (a, b))))
+    n = a.shape[0]
+    if b.shape[0] != n or n > KV4_MAX_SEQS:
+        raise B200Error(f"{name}: {n} {names[0]} and {b.shape[0]} {names[1]} (as many, at most {KV4_MAX_SEQS})")
+    out = torch.empty(n, dtype=torch.int32, device=a.device)
+    if n:
+        ws = torch.empty(lib().b200_kv4_workspace_bytes(d), dtype=torch.uint8, device=a.device)
+        check(getattr(lib(), f"b200_{name}")(d, a.data_ptr(), b.data_ptr(), out.data_ptr(), n, ws.data_ptr(), _stream()), f"b200_{name}")
+    return out
+
+
+def kv4_extend(cache: KV4Cache, seqs: torch.Tensor, counts: torch.Tensor) -> torch.Tensor:
+    """Room for counts[i] more tokens of sequence seqs[i], in order, whole or not at all → the first new position of each, −1 where there are not enough free
+    pages or places in the table.  New pages are the lowest free ones.  A sequence that stands in seqs twice is refused the second time."""
+    return _kv4_lists(cache, "kv4_extend", seqs, counts, ("seqs", "counts"))
+
+
+def kv4_fork(cache: KV4Cache, src: torch.Tensor, dst: torch.Tensor) -> torch.Tensor:
+    """dst[i] (empty) becomes a copy of src[i]: whole pages are shared until they are freed, a page that is not full is copied, in all layers → 1, or 0 where
+    there is no free page or dst[i] is not empty."""
+    return _kv4_lists(cache, "kv4_fork", src, dst, ("src", "dst"))
+
+
+def kv4_free(cache: KV4Cache, seqs: torch.Tensor) -> None:
+    """The sequences become empty; pages that no other one shares are free."""
+    y = _fast.kv4_free(*cache._at, seqs) if cache.__class__ is KV4Cache else None
+    if y is True:
+        return
+    if y is not None:
+        check(y, "b200_kv4_free")
+    d, seqs = _kv4(cache, "kv4_free", seqs=seqs)
+    if seqs.shape[0]:
+        check(lib().b200_kv4_free(d, seqs.data_ptr(), seqs.shape[0], _stream()), "b200_kv4_free")
+
+
+def kv4_compact(cache: KV4Cache) -> torch.Tensor:
+    """The pages in use move to the front of the pool, those that lie there already stay → int32 [1]: their number."""
+    y = _fast.kv4_compact(*cache._at) if cache.__class__ is KV4Cache else None
+    if y.__class__ is _Tensor:
+        return y
+    if y is not None:
+        check(y, "b200_kv4_compact")
+    d, = _kv4(cache, "kv4_compact")
+    out = torch.empty(1, dtype=torch.int32, device=cache.pages.device)
+    ws = torch.empty(lib().b200_kv4_workspace_bytes(d), dtype=torch.uint8, device=cache.pages.device)
+    check(lib().b200_kv4_compact(d, out.data_ptr(), ws.data_ptr(), _stream()), "b200_kv4_compact")
+    return out
+
+
 # ------------------------------------------------------------------------------- mechanisms of the layer-stack engine
 # T = bf16 or fp32 storage (taken from the tensors); norms, softmax, gates and accumulation are fp32 in both.
 def _sdt(t: torch.Tensor) -> int:
