@@ -212,7 +212,7 @@ int64_t b200_kv4_page_bytes(int64_t kv_heads, int64_t dim);
 
 /* k and v [rows, kv_heads, dim] bf16, rows ld_k / ld_v elements apart → one layer of the cache.  Sequence seqs[i] of the call owns rows starts[i] … starts[i + 1] − 1,
  * which go to its positions pos[i], pos[i] + 1, … (pos −1: nowhere).  A row whose page the sequence does not have, or shares with
- * another one, is left out.  starts has n + 1 entries and does not fall. */
+ * another one, is left out.  starts has n + 1 entries and does not fall.  k, v and their rows 16-byte aligned. */
 int b200_kv4_store(const b200_kv4_cache* cache, int64_t layer, const void* k, int64_t ld_k, const void* v, int64_t ld_v, const int32_t* seqs,
                    const int32_t* starts, const int32_t* pos, int64_t n, int64_t rows, void* stream);
 /* The reverse: what the cache holds, fp32 [rows, kv_heads, dim]; zero for a row without a place. */

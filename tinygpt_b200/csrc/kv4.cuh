@@ -1,11 +1,12 @@
 // kv4.cuh — the paged cache of keys and values in 4 bits: its layout, and what its kernels share.
 //
 // A page holds kPage tokens of every key/value head; of a head, four tiles of 16 tokens lie one behind the other, each
-//   keys    [group of 64 entries][512 bytes]     lane 4r + c, word 2h + t, byte 2e + hi:  token r + 8·hi, entries 32h + 8c + 4t + {e, e + 2}
+//   keys    [group of 64 entries][512 bytes]     lane 4r + c, word 2h + t, byte 2e + hi:  token r + 8·hi, entries 32h + 8c + 4t + 2e + {0, 1}
 //   their scale | middle << 16                    [group][r][hi]
-//   values  [group][512 bytes]                    lane 4r + c, word j, byte 2e + p:        token 2c + 8p + e, entries 16j + r + {0, 8}
-//   their scale | middle << 16                    [group][r][hi]
-// so that a lane's 16 bytes are its A operands of four m16n8k16 products (tokens × entries of K, entries × tokens of Vᵀ), and no two tokens share a byte.
+//   values  [group][512 bytes]                    lane 4r + c, word j, byte 2e + p:        token 2c + 8p + e, entries 16j + 2r + {0, 1}
+//   their scale | middle << 16                    [group][token % 8][token / 8]
+// so that a lane's 16 bytes are its A operands of four m16n8k16 products (tokens × entries of K, entries × tokens of Vᵀ), no two tokens share a byte, and
+// a byte holds two neighbouring entries.
 #pragma once
 #include "lowbit.cuh"
 
@@ -21,22 +22,23 @@ int check_kv4_rows(const b200_kv4_cache* c, int64_t layer, const int32_t* seqs, 
                    const char* what);
 
 #ifdef __CUDACC__
-// Row → (sequence of the call, page, token in it); page < 0: the row has no place.
+// Where a row goes.  page < 0: nowhere; else its token of the page, and how many rows from it on lie in its tile of 16 (0: an earlier row's run has it).
 struct Kv4Place {
-  int page, token;
+  int page, token, run;
 };
-__device__ __forceinline__ Kv4Place kv4_place(const b200_kv4_cache& c, const int32_t* seqs, const int32_t* starts, const int32_t* pos, int n, int row) {
+__device__ __forceinline__ Kv4Place kv4_place(const b200_kv4_cache& c, const int32_t* seqs, const int32_t* starts, const int32_t* pos, int n, int rows, int row) {
   int lo = 0, hi = n;   // the last i with starts[i] <= row
   while (hi - lo > 1) {
     const int mid = (lo + hi) / 2;
     if (starts[mid] <= row) lo = mid;
     else hi = mid;
   }
-  const int slot = seqs[lo], p = pos[lo], first = starts[lo];
+  const int slot = seqs[lo], p = pos[lo], first = starts[lo], end = min(starts[lo + 1], rows);
   const int64_t at = (int64_t)p + row - first;
-  if (first > row || row >= starts[lo + 1] || p < 0 || slot < 0 || slot >= c.n_seqs || at >= (int64_t)c.max_pages * kPage) return {-1, 0};
-  const int page = c.table[(int64_t)slot * c.max_pages + at / kPage];
-  return {page < c.n_pages ? page : -1, (int)(at % kPage)};
+  if (first > row || row >= end || p < 0 || slot < 0 || slot >= c.n_seqs || at >= (int64_t)c.max_pages * kPage) return {-1, 0, 0};
+  const int page = c.table[(int64_t)slot * c.max_pages + at / kPage], in_tile = (int)(at % kKvTile);
+  const bool leads = in_tile == 0 || row == max(first, 0);
+  return {page < c.n_pages ? page : -1, (int)(at % kPage), leads ? min(kKvTile - in_tile, end - row) : 0};
 }
 __device__ __forceinline__ uint8_t* kv4_head(const b200_kv4_cache& c, int layer, int page, int head) {
   const int64_t block = 4 * kv4_tile_bytes(c.dim / kKvGroup);

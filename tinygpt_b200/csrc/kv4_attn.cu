@@ -7,9 +7,10 @@
 //   output   Oᵀ += Vᵀ·P  a value's scale goes into its weight (rounded to bf16), Σ weight·middle is kept in fp32 beside the products
 // Everything between memory and the products is in registers; a transposing move turns the weights of a score tile into the operand that Vᵀ meets.
 //
-// Work is cut evenly over the CTAs whatever the sequences' lengths: (sequence, column block, head, page) in this order is one line of units,
-// of which every CTA takes an equal piece.  A CTA that holds all of an item's pages writes its rows; parts of an item go to the workspace and a
-// second kernel joins them in their order.
+// Work is cut evenly over the warps of the GPU whatever the sequences' lengths: the items (sequence, column block, head) form one line, each as
+// long as its steps of 32 tokens and kAhead more for what an item costs before its first token, and every warp takes an equal piece of the line.  A warp
+// that holds all of an item writes its rows; parts go to the workspace (one for a CTA whose warps are all inside an item) and a second
+// kernel joins them in their order.
 #include "kv4.cuh"
 
 #include <algorithm>
@@ -18,7 +19,8 @@ namespace b200 {
 
 namespace {
 
-constexpr int kWarps = 8, kThreads = kWarps * 32;
+constexpr int kStep = 32, kAhead = 2;
+constexpr int kGrid = 148;
 
 struct Kv4Attn {
   b200_kv4_cache cache;
@@ -27,6 +29,7 @@ struct Kv4Attn {
   int64_t ld_q;
   const int32_t *seqs, *starts, *pos;
   float* parts;
+  struct Kv4Split* splits;   // of every warp
   int layer, q_heads, group, n, rows, window;
   float scale_log2;
 };
@@ -50,9 +53,18 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// A sequence of the call: its rows, the tokens they may see, its work.
+__device__ __forceinline__ long long warp_scan(long long v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long b = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += b;
+  }
+  return v;
+}
+
+// A sequence of the call: its rows, the tokens they may see, its items.
 struct Kv4Seq {
-  int row0, count, pos, slot, last, page0, pages, blocks;   // tokens below `last`; pages page0 … page0 + pages − 1 (one at least)
+  int row0, count, pos, slot, last, step0, steps, blocks;   // tokens below `last`; steps step0 … step0 + steps − 1 (one at least)
 };
 __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4Attn& p, int i, int columns) {
   Kv4Seq s;
@@ -62,112 +74,130 @@ __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4Attn& p, int i, int columns) 
   s.slot = p.seqs[i];
   s.blocks = (int)(((int64_t)s.count * p.group + columns - 1) / columns);
   s.last = 0;
-  s.page0 = 0;
+  s.step0 = 0;
   if (s.pos >= 0 && s.slot >= 0 && s.slot < p.cache.n_seqs)
     s.last = (int)min(min((int64_t)p.cache.length[s.slot], (int64_t)s.pos + s.count), min((int64_t)p.cache.max_pages * kPage, (int64_t)(1 << 30)));
   s.last = max(s.last, 0);
-  if (p.window > 0 && s.pos >= p.window) s.page0 = min((s.pos - p.window + 1) / kPage, s.last / kPage);
-  s.pages = max((s.last + kPage - 1) / kPage - s.page0, 1);
+  if (p.window > 0 && s.pos >= p.window) s.step0 = min((s.pos - p.window + 1) / kStep, s.last / kStep);
+  s.steps = max((s.last + kStep - 1) / kStep - s.step0, 1);
   return s;
 }
-// ends[i]: units of the sequences up to i; the longest item's pages come back.  All threads of the CTA.
-__device__ int kv4_plan(const Kv4Attn& p, int columns, long long* ends) {
-  __shared__ long long carry[kWarps];
-  __shared__ int longest[kWarps];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  constexpr int kEach = kKvMaxSeqs / kThreads;
-  long long mine[kEach], sum = 0;
-  int most = 1;
-#pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    const int i = threadIdx.x * kEach + e;
-    if (i < p.n) {
-      const Kv4Seq s = kv4_seq(p, i, columns);
-      sum += (long long)s.blocks * p.cache.kv_heads * s.pages;
-      if (s.blocks > 0) most = max(most, s.pages);
-    }
-    mine[e] = sum;
-  }
-  long long before = sum;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, before, o);
-    if (lane >= o) before += v;
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-  }
-  if (lane == 31) {
-    carry[warp] = before;
-    longest[warp] = most;
-  }
+__device__ __forceinline__ long long kv4_line(const Kv4Attn& p, const Kv4Seq& s) { return (long long)s.blocks * p.cache.kv_heads * (s.steps + kAhead); }
+// ends[i]: the line up to the end of sequence i.  All threads of a CTA of THREADS.
+template <int THREADS>
+__device__ void kv4_plan(const Kv4Attn& p, int columns, long long* ends) {
+  __shared__ long long carry[THREADS / 32];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, each = (p.n + THREADS - 1) / THREADS, first = threadIdx.x * each;
+  long long sum = 0;
+  for (int i = first; i < min(first + each, p.n); ++i) ends[i] = sum += kv4_line(p, kv4_seq(p, i, columns));
+  const long long upto = warp_scan(sum, lane);
+  if (lane == 31) carry[warp] = upto;
   __syncthreads();
-  before -= sum;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += carry[w];
-    most = max(most, longest[w]);
-  }
-#pragma unroll
-  for (int e = 0; e < kEach; ++e)
-    if (threadIdx.x * kEach + e < p.n) ends[threadIdx.x * kEach + e] = before + mine[e];
+  long long before = upto - sum;
+  for (int w = 0; w < warp; ++w) before += carry[w];
+  for (int i = first; i < min(first + each, p.n); ++i) ends[i] += before;
   __syncthreads();
-  return most;
 }
-// units of a CTA: an equal share, but at least a page to each warp where items have as many
-__device__ __forceinline__ long long kv4_share(long long units, int ctas, int longest) { return max((units + ctas - 1) / ctas, (long long)min(longest, kWarps)); }
-__device__ __forceinline__ int kv4_find(const long long* ends, int n, long long unit) {   // the first i with ends[i] > unit
+__device__ __forceinline__ int kv4_find(const long long* ends, int n, long long at) {   // the first i with ends[i] > at
   int lo = 0, hi = n - 1;
   while (lo < hi) {
     const int mid = (lo + hi) / 2;
-    if (ends[mid] > unit) hi = mid;
+    if (ends[mid] > at) hi = mid;
     else lo = mid + 1;
   }
   return lo;
 }
-__device__ __forceinline__ float* kv4_part(const Kv4Attn& p, int cta, int which, int columns) {
-  return p.parts + ((int64_t)cta * 2 + which) * columns * (p.cache.dim + 2);
+// How the line is cut: `warps` pieces, `each` CTA having so many of them; piece w starts at line·w / warps.  A piece is no shorter than a step and what
+// comes before it, and short lines are spread over the CTAs first.
+struct Cut {
+  long long line;
+  int warps, each;
+  __device__ Cut(long long line_, int ctas, int most) : line(line_) {
+    const int want = (int)min(max(line / (kAhead + 1), 1ll), (long long)ctas * most);
+    each = (want + ctas - 1) / ctas;
+    warps = want;
+  }
+  __device__ __forceinline__ long long start(int w) const { return line * min(w, warps) / warps; }
+};
+// a warp's parts: of an item that came before it (0) and of one that goes on behind it (1).  [column][dim], maxima, sums
+__device__ __forceinline__ float* kv4_part(const Kv4Attn& p, int64_t warp, int which, int columns) {
+  return p.parts + (warp * 2 + which) * columns * (p.cache.dim + 2);
 }
+// An item that its first warp does not finish, for the kernel that joins the parts: the warps that hold it, of those the ones that left one part for their CTA.
+struct Kv4Split {
+  int from, to, in0, in1;   // warps from … to; CTAs in0 … in1 − 1 (none: in0 >= in1)
+  int row0, col0, n_cols, head, each;   // from < 0: none
+};
 
 template <int NG, int NT>
 struct Shape {
   static constexpr int kTile = kv4_tile_bytes(NG);
-  static constexpr int kStageTiles = NG <= 2 ? 4 : 2;
-  static constexpr int kStage = kStageTiles * kTile;
+  static constexpr int kTiles = kStep / kKvTile;                // of a step
+  static constexpr int kStage = kTiles * kTile;
+  static constexpr int kWarps = NG * NT <= 2 ? 16 : 8;
+  static constexpr int kThreads = kWarps * 32;
   static constexpr bool kQInRegs = NG * NT <= 4;
   static constexpr int kQBytes = kQInRegs ? 0 : NT * NG * 2 * 512;
-  static constexpr int kSmem = kWarps * 2 * kStage + kQBytes + kKvMaxSeqs * 8;
-  static_assert(8 * NT * (NG * 64 + 2) * 4 <= 2 * kStage, "a warp's output fits its ring");
+  static constexpr int kRoom = 232448 - 1024 - kKvMaxSeqs * 8;
+  static constexpr int kStages = kWarps * (3 * kStage + kQBytes) <= kRoom ? 3 : 2;
+  static constexpr int kRing = kStages * kStage > 8 * NT * (NG * 64 + 2) * 4 ? kStages * kStage : (8 * NT * (NG * 64 + 2) * 4 + 15) / 16 * 16;
+  static constexpr int kOwn = kRing + kQBytes;                  // shared memory of a warp
+  static constexpr int kSmem = kWarps * kOwn + kKvMaxSeqs * 8;
+  static_assert(kWarps * kOwn <= kRoom, "shared memory of an SM");
 };
 
 template <int NG, int NT>
-__global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Kv4Attn p) {
+__global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(const Kv4Attn p) {
   using S = Shape<NG, NT>;
-  constexpr int kCols = 8 * NT, kDim = NG * 64, kPer = 4 / S::kStageTiles;   // stages of a page
+  constexpr int kCols = 8 * NT, kDim = NG * 64;
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
-  uint8_t* const ring = smem + warp * 2 * S::kStage;
-  uint4* const q_smem = reinterpret_cast<uint4*>(smem + kWarps * 2 * S::kStage);
-  long long* const ends = reinterpret_cast<long long*>(smem + kWarps * 2 * S::kStage + S::kQBytes);
+  uint8_t* const ring = smem + warp * S::kOwn;
+  uint4* const q_smem = reinterpret_cast<uint4*>(ring + S::kRing);
+  long long* const ends = reinterpret_cast<long long*>(smem + S::kWarps * S::kOwn);
   pdl_wait();
   pdl_trigger();
 
   // rows of no sequence
   {
     const int head = min(max(p.starts[0], 0), p.rows), tail = min(max(p.starts[p.n], head), p.rows), width = p.q_heads * kDim;
-    for (int64_t row = blockIdx.x; row < head + p.rows - tail; row += gridDim.x)
-      for (int d = threadIdx.x; d < width; d += kThreads) p.out[(row < head ? row : row - head + tail) * width + d] = f_to_bf16(0.f);
+    for (int row = blockIdx.x; row < head + p.rows - tail; row += gridDim.x)
+      for (int d = threadIdx.x; d < width; d += S::kThreads) p.out[(int64_t)(row < head ? row : row - head + tail) * width + d] = f_to_bf16(0.f);
   }
-  const int longest = kv4_plan(p, kCols, ends);
-  const long long units = ends[p.n - 1], share = kv4_share(units, gridDim.x, longest);
-  long long unit = share * blockIdx.x;
-  const long long stop = min(unit + share, units);
-  int i = unit < stop ? kv4_find(ends, p.n, unit) : 0;
-  while (unit < stop) {
-    while (ends[i] <= unit) ++i;
+  // Up to 32 sequences: every warp has them all in its lanes, and nobody waits for anybody.
+  const bool few = p.n <= 32;
+  long long mine_end = 0, line;
+  if (few) {
+    mine_end = warp_scan(lane < p.n ? kv4_line(p, kv4_seq(p, lane, kCols)) : 0, lane);
+    line = __shfl_sync(0xffffffffu, mine_end, 31);
+  } else {
+    kv4_plan<S::kThreads>(p, kCols, ends);
+    line = ends[p.n - 1];
+  }
+  const Cut cut(line, gridDim.x, S::kWarps);
+  const int me = blockIdx.x * cut.each + warp;
+  const int64_t own = (int64_t)blockIdx.x * S::kWarps + warp;   // of the workspace's places
+  long long at_line = cut.start(me);
+  const long long stop = warp < cut.each ? cut.start(me + 1) : at_line, cta = cut.start(blockIdx.x * cut.each), cta_end = cut.start((blockIdx.x + 1) * cut.each);
+  if (lane == 0) p.splits[own].from = -1;
+  int i = !few && at_line < stop ? kv4_find(ends, p.n, at_line) : 0;
+  while (at_line < stop) {
+    long long base = 0;
+    if (few) {
+      i = __popc(__ballot_sync(0xffffffffu, mine_end <= at_line));
+      if (i > 0) base = __shfl_sync(0xffffffffu, mine_end, i - 1);
+    } else {
+      while (ends[i] <= at_line) ++i;
+      if (i > 0) base = ends[i - 1];
+    }
     const Kv4Seq s = kv4_seq(p, i, kCols);
-    const long long in_seq = unit - (i > 0 ? ends[i - 1] : 0);
-    const int item = (int)(in_seq / s.pages), first = (int)(in_seq % s.pages), head = item % p.cache.kv_heads, block = item / p.cache.kv_heads;
-    const int many = (int)min((long long)(s.pages - first), stop - unit);
-    unit += many;
+    const int length = s.steps + kAhead, item = (int)((at_line - base) / length), head = item % p.cache.kv_heads, block = item / p.cache.kv_heads;
+    const long long begin = base + (long long)item * length + kAhead, end = begin + s.steps;   // of its steps
+    const int first = (int)max(at_line - begin, 0ll), many = (int)(min(stop, end) - begin) - first;
+    // all the CTA's warps have a piece, and of this item alone
+    const bool inside = cut.each > 1 && cta >= begin && cta_end <= end && ((int)blockIdx.x + 1) * cut.each <= cut.warps;
+    at_line = min(stop, end);
+    if (many <= 0) continue;
 
     // the block's queries, as the B operands of K·qᵀ, and their sums over each group
     const int col0 = block * kCols, n_cols = s.count * p.group;
@@ -182,9 +212,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Kv4Attn p) 
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint4 v = col < n_cols ? *reinterpret_cast<const uint4*>(src + g * 64 + h * 32) : make_uint4(0, 0, 0, 0);
+          const uint4 u = col < n_cols ? *reinterpret_cast<const uint4*>(src + g * 64 + h * 32) : make_uint4(0, 0, 0, 0);
+          // entries {0, 2}, {1, 3}, {4, 6}, {5, 7}
+          const uint4 v = make_uint4(__byte_perm(u.x, u.y, 0x5410), __byte_perm(u.x, u.y, 0x7632), __byte_perm(u.z, u.w, 0x5410), __byte_perm(u.z, u.w, 0x7632));
           if constexpr (S::kQInRegs) qf[t][g][h] = v;
-          else if (warp == 0) q_smem[((t * NG + g) * 2 + h) * 32 + lane] = v;
+          else q_smem[((t * NG + g) * 2 + h) * 32 + lane] = v;
           mma16816(sum, kBf16Ones, kBf16Ones, kBf16Ones, kBf16Ones, v.x, v.y);
           mma16816(sum, kBf16Ones, kBf16Ones, kBf16Ones, kBf16Ones, v.z, v.w);
         }
@@ -192,7 +224,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Kv4Attn p) 
         qsum[g][t][1] = sum[1];
       }
     }
-    if constexpr (!S::kQInRegs) __syncthreads();
     int at[NT][2];   // positions of this lane's columns (2c, 2c + 1); −1: no column
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -203,48 +234,53 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Kv4Attn p) 
       }
     const int at_low = s.pos + col0 / p.group, at_high = s.pos + (min(col0 + kCols, n_cols) - 1) / p.group;
 
-    float o[NG * 4][NT][4] = {};
+    float o[NG * 4][NT][4] = {}, wsum[NG][NT][4] = {};   // wsum: Σ of the rounded weights, in every row
     float top[NT][2], sum[NT][2] = {}, mid[NG][NT][2] = {};
 #pragma unroll
     for (int t = 0; t < NT; ++t) top[t][0] = top[t][1] = -INFINITY;
 
-    const int32_t* table = p.cache.table + (int64_t)max(s.slot, 0) * p.cache.max_pages + s.page0 + first;
-    const int n_stages = s.last > 0 ? many * kPer : 0;
+    const int step0 = s.step0 + first, n_steps = s.last > 0 ? many : 0;
+    const int32_t* table = p.cache.table + (int64_t)max(s.slot, 0) * p.cache.max_pages;
     auto page_of = [&](int u) {
-      if (u >= n_stages) return -1;
-      const int page = table[u / kPer];
+      if (u >= n_steps) return -1;
+      const int page = table[(step0 + u) / (kPage / kStep)];
       return page < p.cache.n_pages ? page : -1;
     };
     auto fetch = [&](int u, int page, int slot) {
       if (page >= 0) {
-        const uint8_t* src = kv4_head(p.cache, p.layer, page, head) + u % kPer * S::kStage;
+        const uint8_t* src = kv4_head(p.cache, p.layer, page, head) + (step0 + u) % (kPage / kStep) * S::kStage + lane * 16;
+        uint8_t* dst = ring + slot * S::kStage + lane * 16;
 #pragma unroll
         for (int b = 0; b < S::kStage; b += 512)
-          if (S::kStage % 512 == 0 || b + lane * 16 < S::kStage) cp_async16(ring + slot * S::kStage + b + lane * 16, src + b + lane * 16);
+          if (S::kStage % 512 == 0 || b + lane * 16 < S::kStage) cp_async16(dst + b, src + b);
       }
       cp_async_commit();
     };
-    int page = page_of(warp), next = page_of(warp + kWarps), slot = 0;
-    fetch(warp, page, 0);
-    for (int u = warp; u < n_stages; u += kWarps, slot ^= 1) {
-      fetch(u + kWarps, next, slot ^ 1);
-      const int now = page;
-      page = next;
-      next = page_of(u + 2 * kWarps);
-      cp_async_wait<1>();
+    uint32_t have = 0;   // bit u % 32: step u has a page
+    int next;
+#pragma unroll
+    for (int u = 0; u < S::kStages - 1; ++u) {
+      const int page = page_of(u);
+      have |= (uint32_t)(page >= 0) << u;
+      fetch(u, page, u);
+    }
+    next = page_of(S::kStages - 1);
+    int slot = 0;
+    for (int u = 0; u < n_steps; ++u) {
+      const int ahead = u + S::kStages - 1, into = slot == 0 ? S::kStages - 1 : slot - 1;
+      have = (have & ~(1u << (ahead % 32))) | (uint32_t)(next >= 0) << (ahead % 32);
+      fetch(ahead, next, into);
+      next = page_of(ahead + 1);
+      cp_async_wait<S::kStages - 1>();
       __syncwarp();
-      if (now >= 0) {
+      if (have >> (u % 32) & 1) {
         const uint8_t* stage = ring + slot * S::kStage;
-        const int key0 = (s.page0 + first) * kPage + u * (S::kStageTiles * kKvTile);
-        const bool whole = key0 + S::kStageTiles * kKvTile <= min(s.last, at_low + 1) && (p.window == 0 || at_high - key0 < p.window);
-        float sc[S::kStageTiles][NT][4];
+        const int key0 = (step0 + u) * kStep;
+        const bool whole = key0 + kStep <= min(s.last, at_low + 1) && (p.window == 0 || at_high - key0 < p.window);
+        float sc[S::kTiles][NT][4] = {};
 #pragma unroll
-        for (int k = 0; k < S::kStageTiles; ++k) {
+        for (int k = 0; k < S::kTiles; ++k) {
           const uint8_t* tile = stage + k * S::kTile;
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sc[k][t][e] = 0.f;
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
             const uint4 w = *reinterpret_cast<const uint4*>(tile + g * 512 + lane * 16);
@@ -254,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Kv4Attn p) 
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               uint32_t a[4];
-              nibbles_bf16(words[j], a);
+              nibbles_128(words[j], a);
 #pragma unroll
               for (int t = 0; t < NT; ++t) {
                 uint4 b;
@@ -263,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Kv4Attn p) 
                 mma16816(acc[t], a[0], a[2], a[1], a[3], j % 2 ? b.z : b.x, j % 2 ? b.w : b.y);
               }
             }
-            const float s0 = bf16_lo(small.x), m0 = bf16_hi(small.x), s1 = bf16_lo(small.y), m1 = bf16_hi(small.y);
+            const float s0 = bf16_lo(small.x), m0 = fmaf(-kNibbleOff, s0, bf16_hi(small.x)), s1 = bf16_lo(small.y), m1 = fmaf(-kNibbleOff, s1, bf16_hi(small.y));
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
               sc[k][t][0] = fmaf(s0, acc[t][0], fmaf(m0, qsum[g][t][0], sc[k][t][0]));
@@ -275,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Kv4Attn p) 
         }
         if (!whole) {
 #pragma unroll
-          for (int k = 0; k < S::kStageTiles; ++k)
+          for (int k = 0; k < S::kTiles; ++k)
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -285,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Kv4Attn p) 
                 if (!seen) sc[k][t][e] = -INFINITY;
               }
         }
-        float now_top[NT][2], shift[NT][2];
+        float now[NT][2], shift[NT][2];
         bool moved = false;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -293,11 +329,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Kv4Attn p) 
           for (int e = 0; e < 2; ++e) {
             float m = -INFINITY;
 #pragma unroll
-            for (int k = 0; k < S::kStageTiles; ++k) m = fmaxf(m, fmaxf(sc[k][t][e], sc[k][t][e + 2]));
+            for (int k = 0; k < S::kTiles; ++k) m = fmaxf(m, fmaxf(sc[k][t][e], sc[k][t][e + 2]));
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
             m = fmaxf(top[t][e], m * p.scale_log2);
-            now_top[t][e] = m;
+            now[t][e] = m;
             shift[t][e] = m == -INFINITY ? 0.f : m;
             moved |= m != top[t][e];
           }
@@ -307,10 +343,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Kv4Attn p) 
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const float f = exp2_fast(top[t][e] - shift[t][e]);   // 0 where there was none
-              top[t][e] = now_top[t][e];
+              top[t][e] = now[t][e];
               sum[t][e] *= f;
 #pragma unroll
-              for (int g = 0; g < NG; ++g) mid[g][t][e] *= f;
+              for (int g = 0; g < NG; ++g) {
+                mid[g][t][e] *= f;
+                wsum[g][t][e] *= f;
+              }
 #pragma unroll
               for (int d = 0; d < NG * 4; ++d) {
                 o[d][t][e] *= f;
@@ -319,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Kv4Attn p) 
             }
         }
 #pragma unroll
-        for (int k = 0; k < S::kStageTiles; ++k) {
+        for (int k = 0; k < S::kTiles; ++k) {
           const uint8_t* tile = stage + k * S::kTile + NG * (512 + 64);
 #pragma unroll
           for (int t = 0; t < NT; ++t)
@@ -337,23 +376,24 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Kv4Attn p) 
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
               float w[4] = {sc[k][t][0] * s0, sc[k][t][1] * s0, sc[k][t][2] * s1, sc[k][t][3] * s1};
-              float y[4] = {sc[k][t][0] * m0, sc[k][t][1] * m0, sc[k][t][2] * m1, sc[k][t][3] * m1};
+              float y[4] = {m0, m0, m1, m1};
               if (!whole) {   // what is not seen may hold anything
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                   if (sc[k][t][e] == 0.f) w[e] = y[e] = 0.f;
               }
-              mid[g][t][0] += y[0] + y[2];
-              mid[g][t][1] += y[1] + y[3];
+              mid[g][t][0] = fmaf(sc[k][t][2], y[2], fmaf(sc[k][t][0], y[0], mid[g][t][0]));
+              mid[g][t][1] = fmaf(sc[k][t][3], y[3], fmaf(sc[k][t][1], y[1], mid[g][t][1]));
               b[t][0] = transpose8x8(pack2(w[0], w[1]));
               b[t][1] = transpose8x8(pack2(w[2], w[3]));
+              mma16816(wsum[g][t], kBf16Ones, kBf16Ones, kBf16Ones, kBf16Ones, b[t][0], b[t][1]);
             }
             const uint4 v = *reinterpret_cast<const uint4*>(tile + g * 512 + lane * 16);
             const uint32_t words[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               uint32_t a[4];
-              nibbles_bf16(words[j], a);
+              nibbles_128(words[j], a);
 #pragma unroll
               for (int t = 0; t < NT; ++t) mma16816(o[g * 4 + j][t], a[0], a[1], a[2], a[3], b[t][0], b[t][1]);
             }
@@ -361,108 +401,170 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_kernel(const Kv4Attn p) 
         }
       }
       __syncwarp();   // the stage is free
+      slot = slot + 1 == S::kStages ? 0 : slot + 1;
     }
     cp_async_wait<0>();
     __syncwarp();
 
-    // the warps' parts meet in shared memory: [column][dim], then the maxima and the sums
-    float* const own = reinterpret_cast<float*>(ring);
+    // Σ over the tokens is whole but for what the lanes of a column keep apart
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float l = sum[t][e];
 #pragma unroll
-        for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-        const int col = t * 8 + 2 * c + e;
-        if (r == 0) {
-          own[kCols * kDim + col] = top[t][e];
-          own[kCols * kDim + kCols + col] = l;
-        }
+        for (int x = 4; x < 32; x <<= 1) sum[t][e] += __shfl_xor_sync(0xffffffffu, sum[t][e], x);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
           float y = mid[g][t][e];
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) y += __shfl_xor_sync(0xffffffffu, y, x);
+          y = fmaf(-kNibbleOff, wsum[g][t][e], y);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            own[col * kDim + g * 64 + j * 16 + r] = o[g * 4 + j][t][e] + y;
-            own[col * kDim + g * 64 + j * 16 + r + 8] = o[g * 4 + j][t][e + 2] + y;
+            o[g * 4 + j][t][e] += y;
+            o[g * 4 + j][t][e + 2] += y;
           }
         }
       }
-    __syncthreads();
-    const bool all = many == s.pages;
-    float* const part = all ? nullptr : kv4_part(p, blockIdx.x, first == 0, kCols);
-    for (int x = threadIdx.x; x < kCols * kDim; x += kThreads) {
-      const int col = x / kDim, d = x % kDim;
-      float m = -INFINITY;
+    if (many == s.steps) {
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, reinterpret_cast<const float*>(smem + w * 2 * S::kStage)[kCols * kDim + col]);
-      float l = 0.f, v = 0.f;
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float* from = reinterpret_cast<const float*>(smem + w * 2 * S::kStage);
-        const float lw = from[kCols * kDim + kCols + col];
-        if (lw != 0.f) {   // what has seen a token (one that is no number too)
-          const float f = exp2_fast(from[kCols * kDim + col] - m);
-          l = fmaf(f, lw, l);
-          v = fmaf(f, from[x], v);
+        for (int e = 0; e < 2; ++e) {
+          const int col = col0 + t * 8 + 2 * c + e;
+          if (col >= n_cols) continue;
+          const float f = sum[t][e] == 0.f ? 0.f : 1.f / sum[t][e];
+          __nv_bfloat16* dst = p.out + ((int64_t)(s.row0 + col / p.group) * p.q_heads + head * p.group + col % p.group) * kDim + 2 * r;
+#pragma unroll
+          for (int d = 0; d < NG * 4; ++d) *reinterpret_cast<uint32_t*>(dst + 16 * d) = pack2(o[d][t][e] * f, o[d][t][e + 2] * f);
         }
+    } else {
+      float* const part = inside ? reinterpret_cast<float*>(ring) : kv4_part(p, own, first == 0, kCols);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int col = t * 8 + 2 * c + e;
+#pragma unroll
+          for (int d = 0; d < NG * 4; ++d) *reinterpret_cast<float2*>(part + col * kDim + 16 * d + 2 * r) = make_float2(o[d][t][e], o[d][t][e + 2]);
+          if (r == 0) {
+            part[kCols * kDim + col] = top[t][e];
+            part[kCols * kDim + kCols + col] = sum[t][e];
+          }
+        }
+      if (first == 0 && lane == 0) {
+        Kv4Split split;
+        auto warp_at = [&](long long x) {   // whose piece of the line x is
+          int w = (int)(x * cut.warps / cut.line);
+          while (cut.start(w) > x) --w;
+          while (cut.start(w + 1) <= x) ++w;
+          return w;
+        };
+        split.from = me;
+        split.to = warp_at(end - 1);
+        split.in0 = cta == begin ? blockIdx.x : blockIdx.x + 1;
+        split.in1 = cut.start(split.to + 1) == end && (split.to + 1) % cut.each == 0 ? (split.to + 1) / cut.each : split.to / cut.each;
+        if (cut.each == 1) split.in1 = split.in0;
+        split.row0 = s.row0;
+        split.col0 = col0;
+        split.n_cols = n_cols;
+        split.head = head;
+        split.each = cut.each;
+        p.splits[own] = split;
       }
-      if (all) {
-        if (col0 + col < n_cols)
-          p.out[((int64_t)(s.row0 + (col0 + col) / p.group) * p.q_heads + head * p.group + (col0 + col) % p.group) * kDim + d] =
-              f_to_bf16(l == 0.f ? 0.f : v / l);
-      } else {
-        part[x] = v;
-        if (d == 0) {
-          part[kCols * kDim + col] = m;
-          part[kCols * kDim + kCols + col] = l;
+      if (inside) {   // every warp of the CTA that has a piece comes here, once
+        named_bar_sync(1, cut.each * 32);
+        float* const joined = kv4_part(p, (int64_t)blockIdx.x * S::kWarps, 0, kCols);
+        for (int x = threadIdx.x; x < kCols * kDim; x += cut.each * 32) {
+          const int col = x / kDim;
+          float m = -INFINITY;
+          for (int w = 0; w < cut.each; ++w) m = fmaxf(m, reinterpret_cast<const float*>(smem + w * S::kOwn)[kCols * kDim + col]);
+          float l = 0.f, v = 0.f;
+#pragma unroll 4
+          for (int w = 0; w < cut.each; ++w) {
+            const float* from = reinterpret_cast<const float*>(smem + w * S::kOwn);
+            const float lw = from[kCols * kDim + kCols + col];
+            if (lw != 0.f) {   // what has seen a token (one that is no number too)
+              const float f = exp2_fast(from[kCols * kDim + col] - m);
+              l = fmaf(f, lw, l);
+              v = fmaf(f, from[x], v);
+            }
+          }
+          joined[x] = v;
+          if (x % kDim == 0) {
+            joined[kCols * kDim + col] = m;
+            joined[kCols * kDim + kCols + col] = l;
+          }
         }
       }
     }
-    __syncthreads();
   }
 }
 
-// One CTA (of a row of the grid) for every border between two CTAs of the kernel above: it joins the item that lies across the border, if no border before
-// lies in it too.  The item's parts are taken in their order.
-__global__ void __launch_bounds__(kThreads) kv4_join_kernel(const Kv4Attn p, int columns, int ctas) {
-  __shared__ long long ends[kKvMaxSeqs];
+// The items that lie in more than one warp's piece of the line.  CTA (c, column) takes those that begin in CTA c's pieces: its warps every eighth part in
+// order, then the warps meet.
+constexpr int kJoinWarps = 8;
+template <int NG>
+__global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn p, int columns, int warps) {
+  __shared__ float part_m[kJoinWarps], part_l[kJoinWarps], part_o[kJoinWarps][NG * 64];
+  constexpr int kDim = NG * 64;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, col = blockIdx.y;
   pdl_wait();
   pdl_trigger();
-  const int longest = kv4_plan(p, columns, ends);
-  const long long units = ends[p.n - 1], share = kv4_share(units, ctas, longest), border = share * (blockIdx.x + 1);
-  if (border >= units) return;
-  const int i = kv4_find(ends, p.n, border);
-  const Kv4Seq s = kv4_seq(p, i, columns);
-  const long long base = i > 0 ? ends[i - 1] : 0;
-  const int item = (int)((border - base) / s.pages);
-  const long long begin = base + (long long)item * s.pages, end = begin + s.pages;
-  if (begin == border || begin / share != blockIdx.x) return;
-  const int head = item % p.cache.kv_heads, col0 = item / p.cache.kv_heads * columns, n_cols = s.count * p.group, dim = p.cache.dim;
-  const int from = (int)(begin / share), to = (int)((end - 1) / share);
-  for (int x = blockIdx.y * kThreads + threadIdx.x; x < columns * dim; x += gridDim.y * kThreads) {
-    const int col = x / dim, d = x % dim;
-    if (col0 + col >= n_cols) break;
-    float m = -INFINITY, l = 0.f, v = 0.f;
-    for (int c = from; c <= to; ++c) m = fmaxf(m, kv4_part(p, c, c == from, columns)[columns * dim + col]);
-    for (int c = from; c <= to; ++c) {
-      const float* part = kv4_part(p, c, c == from, columns);
-      const float lw = part[columns * dim + columns + col];
+  const Kv4Split* splits = p.splits + blockIdx.x * warps;
+  uint32_t left = __ballot_sync(0xffffffffu, lane < warps && splits[lane].from >= 0);
+  for (; left != 0; left &= left - 1) {
+    const Kv4Split s = splits[__ffs(left) - 1];
+    const int at = s.col0 + col;
+    if (at >= s.n_cols) continue;
+    const bool some = s.in0 < s.in1;
+    const int before = some ? s.in0 * s.each - s.from : s.to - s.from + 1, whole = some ? s.in1 - s.in0 : 0;
+    const int parts = before + whole + (some ? s.to - s.in1 * s.each + 1 : 0);
+    float m = -INFINITY, l = 0.f;
+    float2 v[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) v[g] = make_float2(0.f, 0.f);
+#pragma unroll 4
+    for (int k = warp; k < parts; k += kJoinWarps) {
+      const int w = k < before ? s.from + k : k < before + whole ? (s.in0 + k - before) * s.each : s.in1 * s.each + k - before - whole;
+      const float* part = kv4_part(p, (int64_t)(w / s.each) * warps + w % s.each, k < before && k == 0, columns);
+      const float mw = part[columns * kDim + col], lw = part[columns * kDim + columns + col];
+      float2 x[NG];
+#pragma unroll
+      for (int g = 0; g < NG; ++g) x[g] = *reinterpret_cast<const float2*>(part + col * kDim + g * 64 + 2 * lane);
       if (lw == 0.f) continue;
-      const float f = exp2_fast(part[columns * dim + col] - m);
-      l = fmaf(f, lw, l);
-      v = fmaf(f, part[x], v);
+      const float top = fmaxf(m, mw), f = exp2_fast(mw - top), keep = l == 0.f ? 0.f : exp2_fast(m - top);
+      m = top;
+      l = fmaf(f, lw, l * keep);
+#pragma unroll
+      for (int g = 0; g < NG; ++g) v[g] = make_float2(fmaf(f, x[g].x, v[g].x * keep), fmaf(f, x[g].y, v[g].y * keep));
     }
-    p.out[((int64_t)(s.row0 + (col0 + col) / p.group) * p.q_heads + head * p.group + (col0 + col) % p.group) * dim + d] = f_to_bf16(l == 0.f ? 0.f : v / l);
+    if (lane == 0) {
+      part_m[warp] = m;
+      part_l[warp] = l;
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) *reinterpret_cast<float2*>(part_o[warp] + g * 64 + 2 * lane) = v[g];
+    __syncthreads();
+    for (int d = threadIdx.x; d < kDim; d += kJoinWarps * 32) {
+      float top = -INFINITY, sum = 0.f, y = 0.f;
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, part_m[w]);
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) {
+        if (part_l[w] == 0.f) continue;
+        const float f = exp2_fast(part_m[w] - top);
+        sum = fmaf(f, part_l[w], sum);
+        y = fmaf(f, part_o[w][d], y);
+      }
+      p.out[((int64_t)(s.row0 + at / p.group) * p.q_heads + s.head * p.group + at % p.group) * kDim + d] = f_to_bf16(sum == 0.f ? 0.f : y / sum);
+    }
+    __syncthreads();
   }
 }
 
 // Column tiles of a block: what an average sequence brings.
 int column_tiles(int64_t group, int64_t n, int64_t rows) { return group * ((rows + n - 1) / n) <= 8 ? 1 : 2; }
-int grid_of() { return 148; }
 
 template <int NG, int NT>
 int launch(const Kv4Attn& p, cudaStream_t st) {
@@ -470,9 +572,21 @@ int launch(const Kv4Attn& p, cudaStream_t st) {
   static PerDevice attrs;
   B200_CUDA(attrs([] { return cudaFuncSetAttribute(kv4_attn_kernel<NG, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem); }));
   const bool pdl = op_pdl(st);
-  B200_CUDA(launch_pdl(kv4_attn_kernel<NG, NT>, dim3(grid_of()), dim3(kThreads), S::kSmem, st, pdl, p));
-  B200_CUDA(launch_pdl(kv4_join_kernel, dim3(grid_of() - 1, 8 * NT * NG * 64 / kThreads), dim3(kThreads), 0, st, pdl, p, 8 * NT, grid_of()));
+  B200_CUDA(launch_pdl(kv4_attn_kernel<NG, NT>, dim3(kGrid), dim3(S::kThreads), S::kSmem, st, pdl, p));
+  B200_CUDA(launch_pdl(kv4_join_kernel<NG>, dim3(kGrid, 8 * NT), dim3(kJoinWarps * 32), 0, st, pdl, p, 8 * NT, S::kWarps));
   return B200_OK;
+}
+int warps_of(int groups, int tiles) {
+  switch (groups * 2 + tiles - 3) {
+    case 0: return Shape<1, 1>::kWarps;
+    case 1: return Shape<1, 2>::kWarps;
+    case 2: return Shape<2, 1>::kWarps;
+    case 3: return Shape<2, 2>::kWarps;
+    case 4: return Shape<3, 1>::kWarps;
+    case 5: return Shape<3, 2>::kWarps;
+    case 6: return Shape<4, 1>::kWarps;
+    default: return Shape<4, 2>::kWarps;
+  }
 }
 
 }  // namespace
@@ -484,8 +598,9 @@ extern "C" {
 int64_t b200_kv4_attention_workspace_bytes(const b200_kv4_cache* cache, int64_t q_heads, int64_t n, int64_t rows) {
   using namespace b200;
   if (cache == nullptr || cache->kv_heads < 1 || q_heads < 1 || q_heads % cache->kv_heads != 0 || n < 1 || rows < 1) return -1;
+  if (cache->dim % kKvGroup != 0 || cache->dim < 64 || cache->dim > 256) return -1;
   const int tiles = column_tiles(q_heads / cache->kv_heads, n, rows);
-  return (int64_t)grid_of() * 2 * 8 * tiles * (cache->dim + 2) * 4;
+  return (int64_t)kGrid * warps_of(cache->dim / kKvGroup, tiles) * (2 * 8 * tiles * (cache->dim + 2) * 4 + (int64_t)sizeof(Kv4Split));
 }
 
 int b200_kv4_attention(void* out, const void* q, int64_t ld_q, const b200_kv4_cache* cache, int64_t layer, int64_t q_heads, const int32_t* seqs,
@@ -508,6 +623,8 @@ int b200_kv4_attention(void* out, const void* q, int64_t ld_q, const b200_kv4_ca
   p.starts = starts;
   p.pos = pos;
   p.parts = (float*)workspace;
+  const int tiles = column_tiles(q_heads / cache->kv_heads, n, rows);
+  p.splits = (Kv4Split*)(p.parts + (int64_t)kGrid * warps_of(cache->dim / kKvGroup, tiles) * 2 * 8 * tiles * (cache->dim + 2));
   p.layer = (int)layer;
   p.q_heads = (int)q_heads;
   p.group = (int)(q_heads / cache->kv_heads);
@@ -516,7 +633,7 @@ int b200_kv4_attention(void* out, const void* q, int64_t ld_q, const b200_kv4_ca
   p.window = (int)std::min<int64_t>(window, INT32_MAX);
   p.scale_log2 = scale * 1.44269504f;
   const cudaStream_t st = (cudaStream_t)stream;
-  const bool two = column_tiles(p.group, n, rows) == 2;
+  const bool two = tiles == 2;
   switch (cache->dim / kKvGroup) {
     case 1: return two ? launch<1, 2>(p, st) : launch<1, 1>(p, st);
     case 2: return two ? launch<2, 2>(p, st) : launch<2, 1>(p, st);

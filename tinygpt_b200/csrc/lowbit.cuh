@@ -15,15 +15,21 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
 }
 constexpr uint32_t kBf16Ones = 0x3f803f80u;
 
-// Eight nibbles → (nibble − 8) as four pairs of bf16: pair i is {bits 4i, bits 16 + 4i}.  0x4300 | v is 128 + v in bf16 (a step of 128 … 255 is 1), and
-// taking 136 away is exact.
+// Eight nibbles → 128 + nibble as four pairs of bf16: pair i is {bits 4i, bits 16 + 4i}.  0x4300 | v is 128 + v in bf16 (from 128 to 255 a step is 1).  The
+// 128, and the 8 that makes a nibble a value, are taken off the sums: Σ (128 + nibble)·x − 136·Σ x, which costs one more product where a subtraction here
+// would cost one instruction a pair; in fp32 the detour moves a sum by some 2^-17 of it.
+constexpr float kNibbleOff = 136.f;
+__device__ __forceinline__ void nibbles_128(uint32_t w, uint32_t (&a)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;" : "=r"(a[i]) : "r"(w >> (4 * i)));   // (w & mask) | 128
+}
+// the same, less 136: exact
 __device__ __forceinline__ void nibbles_bf16(uint32_t w, uint32_t (&a)[4]) {
-  const uint32_t kOff = 0x43084308u;   // 136
+  const uint32_t kOff = 0x43084308u;
+  nibbles_128(w, a);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    uint32_t v;
-    asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;" : "=r"(v) : "r"(w >> (4 * i)));   // (w & mask) | 128
-    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&kOff));
+    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a[i]), *reinterpret_cast<const __nv_bfloat162*>(&kOff));
     a[i] = *reinterpret_cast<const uint32_t*>(&d);
   }
 }

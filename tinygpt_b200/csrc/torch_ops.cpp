@@ -234,7 +234,8 @@ const at::Tensor* numbers(const Kv4& kv, PyObject* o, int64_t n = -1) {
 const at::Tensor* head_rows(const Kv4& kv, PyObject* o) {
   const at::Tensor* t = plain(o, at::kBFloat16, false);
   return t != nullptr && t->dim() == 3 && kv.with(*t) && t->size(0) > 0 && t->size(2) == kv.c->dim && t->stride(2) == 1 && t->stride(1) == t->size(2) &&
-                 (t->size(0) == 1 || t->stride(0) >= t->size(1) * t->size(2))
+                 (t->size(0) == 1 || (t->stride(0) >= t->size(1) * t->size(2) && t->stride(0) % 8 == 0)) &&
+                 reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0
              ? t : nullptr;
 }
 int64_t row_stride(const at::Tensor& t) { return t.size(0) == 1 ? t.size(1) * t.size(2) : t.stride(0); }

@@ -444,8 +444,8 @@ def _kv4_rows(t: torch.Tensor, what: str, heads: Optional[int], dim: int):
     if t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
         raise B200Error(f"{what}: expected bf16 [rows, {heads or 'heads'}, {dim}], got {t.dtype} {tuple(t.shape)}")
     _same_device(what, t)
-    if t.stride(2) != 1 or t.stride(1) != dim or (t.shape[0] > 1 and t.stride(0) < t.shape[1] * dim):
-        t = t.contiguous()
+    if t.stride(2) != 1 or t.stride(1) != dim or (t.shape[0] > 1 and (t.stride(0) < t.shape[1] * dim or t.stride(0) % 8)) or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
     return t, t.shape[1] * dim if t.shape[0] <= 1 else t.stride(0)
 
 
