@@ -12,172 +12,183 @@ constexpr int kStoreWarps = 8;
 
 struct Job {
   int row, head, group, values;
-  Kv4Place at;        // of lane's row row + lane
+  Kv4Place place;     // of row row + lane
   uint32_t leads, nowhere;
 };
-// starts go through shared memory: the search would wait for memory with every step
+// Up to 32 sequences: a lane has each, so that all a row needs is there after one wait for memory.  More: starts go through shared memory, where the search is.
 template <int ROWS>
-__device__ Job find_job(const b200_kv4_cache& cache, const int32_t* seqs, const int32_t* starts, const int32_t* pos, int n, int rows, int32_t* shared, bool owned) {
-  for (int i = threadIdx.x; i <= n; i += kStoreWarps * 32) shared[i] = starts[i];
-  __syncthreads();
-  const int groups = cache.dim / kKvGroup, lane = threadIdx.x % 32;
-  int job = blockIdx.y * kStoreWarps + threadIdx.x / 32;
+__device__ Job find_job(const b200_kv4_cache& cache, const int32_t* seqs, const int32_t* starts, const int32_t* pos, int n, int rows, int32_t* shared) {
+  const int groups = cache.dim / kKvGroup, lane = threadIdx.x % 32, job = blockIdx.y * kStoreWarps + threadIdx.x / 32;
   Job j{};
   j.row = blockIdx.x * ROWS;
   j.values = job % 2;
   j.group = job / 2 % groups;
   j.head = job / (2 * groups);
-  j.at = {-1, 0, 0};
-  const bool in = j.head < cache.kv_heads && lane < ROWS && j.row + lane < rows;
-  if (in) j.at = kv4_place(cache, seqs, shared, pos, n, rows, j.row + lane);
-  if (owned && j.at.page >= 0 && cache.refs[j.at.page] != 1) j.at.page = -1;
-  j.leads = __ballot_sync(0xffffffffu, j.at.page >= 0 && j.at.run > 0);
-  j.nowhere = __ballot_sync(0xffffffffu, in && j.at.page < 0);
+  j.place = {-1, 0, 0};
+  const int row = j.row + lane;
+  const bool in = j.head < cache.kv_heads && lane < ROWS && row < rows;
+  int i = 0, slot, at, first, end;   // the last i with starts[i] <= row
+  if (n <= 32) {
+    const int my_start = lane < n ? starts[lane] : INT32_MAX, my_slot = lane < n ? seqs[lane] : -1, my_pos = lane < n ? pos[lane] : -1, last = starts[n];
+    for (int s = 1; s < n; ++s) i = __shfl_sync(0xffffffffu, my_start, s) <= row ? s : i;
+    slot = __shfl_sync(0xffffffffu, my_slot, i);
+    at = __shfl_sync(0xffffffffu, my_pos, i);
+    first = __shfl_sync(0xffffffffu, my_start, i);
+    end = __shfl_sync(0xffffffffu, my_start, min(i + 1, 31));
+    if (i + 1 == n) end = last;
+  } else {
+    for (int s = threadIdx.x; s <= n; s += kStoreWarps * 32) shared[s] = starts[s];
+    __syncthreads();
+    int hi = n;
+    while (hi - i > 1) {
+      const int mid = (i + hi) / 2;
+      if (shared[mid] <= row) i = mid;
+      else hi = mid;
+    }
+    slot = seqs[i];
+    at = pos[i];
+    first = shared[i];
+    end = shared[i + 1];
+  }
+  if (in) j.place = kv4_place(cache, slot, at, first, min(end, rows), row);
+  j.leads = __ballot_sync(0xffffffffu, j.place.slot >= 0 && j.place.run > 0);
+  j.nowhere = __ballot_sync(0xffffffffu, in && j.place.slot < 0);
   return j;
 }
 
-// Scale and middle of what `lo`, `hi` bound, and a value's nibble.
+// The greatest of a token's entries and of their negatives, two bf16 side by side: lanes' words first, then the lanes' halves.  NaN stays.
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+constexpr uint32_t kNegate = 0x80008000u;
+template <int N>
+__device__ __forceinline__ uint32_t extremes(const uint32_t* two) {   // {greatest, greatest negative} of N words
+  uint32_t top = two[0], low = two[0] ^ kNegate;
+#pragma unroll
+  for (int i = 1; i < N; ++i) {
+    top = max2(top, two[i]);
+    low = max2(low, two[i] ^ kNegate);
+  }
+  return max2(__byte_perm(top, low, 0x5410), __byte_perm(top, low, 0x7632));
+}
+
+// Scale and middle of a group with these extremes.
 struct Scale {
   float s, m, inverse;
   uint32_t both;
 };
-__device__ __forceinline__ Scale make_scale(float lo, float hi, bool finite) {
+__device__ __forceinline__ Scale make_scale(uint32_t ends) {
+  const float hi = bf16_lo(ends), lo = -bf16_hi(ends);
   const __nv_bfloat16 s = f_to_bf16(hi / 15.f - lo / 15.f), m = f_to_bf16(fmaf(8.f, bf16_to_f(s), lo));
-  if (!finite) return {0.f, 0.f, __uint_as_float(0x7fffffffu), 0x7fff7fffu};   // reads as NaN
-  return {bf16_to_f(s), bf16_to_f(m), 1.f / bf16_to_f(s), (uint32_t)__bfloat16_as_ushort(s) | (uint32_t)__bfloat16_as_ushort(m) << 16};
+  if (!isfinite(hi) || !isfinite(lo)) return {0.f, 0.f, 0.f, 0x7fff7fffu};   // reads as NaN
+  return {bf16_to_f(s), bf16_to_f(m), bf16_to_f(s) > 0.f ? 1.f / bf16_to_f(s) : 0.f, (uint32_t)__bfloat16_as_ushort(s) | (uint32_t)__bfloat16_as_ushort(m) << 16};
 }
-// Eight values of a token in fp32, −8 … 7.  The quotient decides, rounded as a division rounds it; a product with the inverse is within 2^-20 of it, so that only
-// what comes nearer than that to the middle between two values (or has an inverse that is none) is divided.
-__device__ __noinline__ float exact_value(float d, float scale) { return scale > 0.f ? rintf(fminf(fmaxf(d / scale, -8.f), 7.f)) : 0.f; }
+
+// N words of two entries → 2N nibbles (value + 8), each in the low bits of a whole number whose next bits up to 16 are zero.  The quotient by the scale decides,
+// rounded as a division rounds it: the product with the (rounded) inverse and one step of Markstein's correction by the exact remainder give just that
+// as long as nothing underflows, in three instructions; ties are common, since entries, middles and scales have eight bits each.  Scales that are next to
+// nothing are divided by.
+constexpr float kRound = 12582912.f + 8.f;   // 1.5·2^23: a sum with it is rounded to a whole number
+__device__ __noinline__ float exact_value(float d, float scale) { return fminf(fmaxf(d / scale, -8.f), 7.f); }
 template <int N>
-__device__ __forceinline__ void to_values(float (&x)[N], const Scale& sc) {
-  constexpr float kMagic = 12582912.f;   // 1.5·2^23: a sum with it is rounded to a whole number
-  bool close = !(sc.inverse < INFINITY);
-  float d[N];
+__device__ __forceinline__ void to_nibbles(uint32_t (&out)[2 * N], const uint32_t* two, const Scale& sc) {
+  const bool tiny = sc.s > 0.f && sc.s < 0x1p-100f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    d[i] = x[i] - sc.m;
-    const float q = fminf(fmaxf(d[i] * sc.inverse, -8.f), 7.f);
-    x[i] = (q + kMagic) - kMagic;
-    close |= !(fabsf(q - x[i]) < 0.499998f);
+  for (int i = 0; i < 2 * N; ++i) {
+    const float d = (i % 2 ? bf16_hi(two[i / 2]) : bf16_lo(two[i / 2])) - sc.m, q = d * sc.inverse;
+    out[i] = __float_as_uint(fminf(fmaxf(fmaf(fmaf(-q, sc.s, d), sc.inverse, q), -8.f), 7.f) + kRound);
   }
-  if (close)
+  if (tiny)
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = exact_value(d[i], sc.s);
+    for (int i = 0; i < 2 * N; ++i) out[i] = __float_as_uint(exact_value((i % 2 ? bf16_hi(two[i / 2]) : bf16_lo(two[i / 2])) - sc.m, sc.s) + kRound);
 }
-// a byte's two values, and a whole number below 65 536 from fp32
-__device__ __forceinline__ float two_values(float first, float second) { return fmaf(16.f, second, first); }
-__device__ __forceinline__ uint32_t halves(float lo, float hi) {
-  constexpr float kMagic = 8388608.f + 8 * 4369;   // 2^23, and 8 for each of four values
-  return __byte_perm(__float_as_uint(lo + kMagic), __float_as_uint(hi + kMagic), 0x5410);
-}
-__device__ __forceinline__ bool is_finite(uint32_t two) { return (two & 0x7f80u) != 0x7f80u && (two & 0x7f800000u) != 0x7f800000u; }
 
 template <int ROWS>
-__global__ void __launch_bounds__(kStoreWarps * 32) kv4_store_kernel(const b200_kv4_cache cache, int layer, const __nv_bfloat16* k, int64_t ld_k,
+__global__ void __launch_bounds__(kStoreWarps * 32, 4) kv4_store_kernel(const b200_kv4_cache cache, int layer, const __nv_bfloat16* k, int64_t ld_k,
                                                                      const __nv_bfloat16* v, int64_t ld_v, const int32_t* seqs, const int32_t* starts,
                                                                      const int32_t* pos, int n, int rows) {
   __shared__ int32_t shared[kKvMaxSeqs + 1];
   pdl_wait();
   pdl_trigger();
-  const Job job = find_job<ROWS>(cache, seqs, starts, pos, n, rows, shared, true);
+  const Job job = find_job<ROWS>(cache, seqs, starts, pos, n, rows, shared);
   const int lane = threadIdx.x % 32, r = lane / 4, c = lane % 4, g = job.group, head = job.head, groups = cache.dim / kKvGroup;
   for (uint32_t left = job.leads; left != 0; left &= left - 1) {
     const int lead = __ffs(left) - 1, row = job.row + lead;
-    const Kv4Place at{__shfl_sync(0xffffffffu, job.at.page, lead), __shfl_sync(0xffffffffu, job.at.token, lead), __shfl_sync(0xffffffffu, job.at.run, lead)};
-    const int first = at.token % kKvTile;
-    uint8_t* tile = kv4_head(cache, layer, at.page, head) + at.token / kKvTile * kv4_tile_bytes(groups) + job.values * groups * (512 + 64);
-    uint32_t* small = reinterpret_cast<uint32_t*>(tile + groups * 512) + g * 16;
-    uint8_t* mine = tile + g * 512 + lane * 16;
-    float half[8];   // of the lane's four words
-    if (job.values == 0) {   // keys: tokens r and r + 8, 16 entries of each
+    const Kv4Place to{__shfl_sync(0xffffffffu, job.place.slot, lead), __shfl_sync(0xffffffffu, job.place.at, lead), __shfl_sync(0xffffffffu, job.place.run, lead)};
+    const int first = to.at % kKvTile;
+    auto here = [&](int token) { return token >= first && token < first + to.run; };
+    // the rows, while the page is looked up
+    uint32_t x[16];
+    if (job.values == 0) {   // keys: of tokens r and r + 8 the entries {0 … 7, 32 … 39} + 8c
       const __nv_bfloat16* src = k + (int64_t)(row - first) * ld_k + head * cache.dim + g * kKvGroup + 8 * c;
 #pragma unroll
-      for (int hi = 0; hi < 2; ++hi) {
-        const int token = r + 8 * hi;
-        const bool here = token >= first && token < first + at.run;
-        uint4 x[2];
-        x[0] = x[1] = make_uint4(0, 0, 0, 0);
-        if (here) {
-          x[0] = *reinterpret_cast<const uint4*>(src + token * ld_k);
-          x[1] = *reinterpret_cast<const uint4*>(src + token * ld_k + 32);
-        }
-        float f[16], lo, top;
-        bool finite = true;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t two[4] = {x[h].x, x[h].y, x[h].z, x[h].w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            f[8 * h + 2 * e] = bf16_lo(two[e]);
-            f[8 * h + 2 * e + 1] = bf16_hi(two[e]);
-            finite &= is_finite(two[e]);
-          }
-        }
-        lo = top = f[0];
-#pragma unroll
-        for (int e = 1; e < 16; ++e) {
-          lo = fminf(lo, f[e]);
-          top = fmaxf(top, f[e]);
-        }
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-          lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          finite &= __shfl_xor_sync(0xffffffffu, (int)finite, o) != 0;
-        }
-        const Scale sc = make_scale(lo, top, finite);
-        to_values(f, sc);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) half[e] = hi == 0 ? two_values(f[2 * e], f[2 * e + 1]) : fmaf(256.f, two_values(f[2 * e], f[2 * e + 1]), half[e]);
-        if (here && c == 0) small[r * 2 + hi] = sc.both;
+      for (int e = 0; e < 4; ++e) {
+        const int token = r + e / 2 * 8;
+        const uint4 w = here(token) ? *reinterpret_cast<const uint4*>(src + token * ld_k + e % 2 * 32) : make_uint4(0, 0, 0, 0);
+        x[4 * e] = w.x;
+        x[4 * e + 1] = w.y;
+        x[4 * e + 2] = w.z;
+        x[4 * e + 3] = w.w;
       }
-    } else {              // values: four tokens, eight entries of each
+    } else {                 // values: of tokens 2c + {0, 8, 1, 9} the entries 16j + 2r + {0, 1}
       const __nv_bfloat16* src = v + (int64_t)(row - first) * ld_v + head * cache.dim + g * kKvGroup + 2 * r;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int token = 2 * c + b % 2 * 8 + b / 2;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[4 * b + j] = here(token) ? *reinterpret_cast<const uint32_t*>(src + token * ld_v + 16 * j) : 0;
+      }
+    }
+    const int page = kv4_page(cache, to.slot, to.at);
+    if (page < 0 || cache.refs[page] != 1) continue;
+    uint8_t* tile = kv4_head(cache, layer, page, head) + to.at % kPage / kKvTile * kv4_tile_bytes(groups) + job.values * groups * (512 + 64);
+    uint32_t* small = reinterpret_cast<uint32_t*>(tile + groups * 512) + g * 16;
+    uint8_t* mine = tile + g * 512 + lane * 16;
+    uint32_t half[8];   // the lane's four words, 16 bits each
+    if (job.values == 0) {
+#pragma unroll
+      for (int hi = 0; hi < 2; ++hi) {
+        uint32_t ends = extremes<8>(x + 8 * hi), q[16];
+        ends = max2(ends, __shfl_xor_sync(0xffffffffu, ends, 1));
+        ends = max2(ends, __shfl_xor_sync(0xffffffffu, ends, 2));
+        const Scale sc = make_scale(ends);
+        to_nibbles<8>(q, x + 8 * hi, sc);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t byte = q[2 * e] + 16 * q[2 * e + 1];
+          half[e] = hi == 0 ? byte : half[e] + 256 * byte;
+        }
+        if (here(r + 8 * hi) && c == 0) small[r * 2 + hi] = sc.both;
+      }
+    } else {
 #pragma unroll
       for (int b = 0; b < 4; ++b) {   // byte 2e + p of every word
         const int e = b / 2, p = b % 2, token = 2 * c + 8 * p + e;
-        const bool here = token >= first && token < first + at.run;
-        uint32_t two[4];
-        bool finite = true;
-        float lo = INFINITY, top = -INFINITY;
+        uint32_t ends = extremes<4>(x + 4 * b), q[8];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) ends = max2(ends, __shfl_xor_sync(0xffffffffu, ends, o));
+        const Scale sc = make_scale(ends);
+        to_nibbles<4>(q, x + 4 * b, sc);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          two[j] = here ? *reinterpret_cast<const uint32_t*>(src + token * ld_v + 16 * j) : 0;
-          finite &= is_finite(two[j]);
-          lo = fminf(lo, fminf(bf16_lo(two[j]), bf16_hi(two[j])));
-          top = fmaxf(top, fmaxf(bf16_lo(two[j]), bf16_hi(two[j])));
+          const uint32_t byte = q[2 * j] + 16 * q[2 * j + 1];
+          half[2 * j + e] = p == 0 ? byte : half[2 * j + e] + 256 * byte;
         }
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-          lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          finite &= __shfl_xor_sync(0xffffffffu, (int)finite, o) != 0;
-        }
-        const Scale sc = make_scale(lo, top, finite);
-        float f[8];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          f[2 * j] = bf16_lo(two[j]);
-          f[2 * j + 1] = bf16_hi(two[j]);
-        }
-        to_values(f, sc);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) half[2 * j + e] = p == 0 ? two_values(f[2 * j], f[2 * j + 1]) : fmaf(256.f, two_values(f[2 * j], f[2 * j + 1]), half[2 * j + e]);
-        if (here && r == 0) small[token % 8 * 2 + token / 8] = sc.both;
+        if (here(token) && r == 0) small[token % 8 * 2 + token / 8] = sc.both;
       }
     }
-    const uint32_t words[4] = {halves(half[0], half[1]), halves(half[2], half[3]), halves(half[4], half[5]), halves(half[6], half[7])};
-    if (at.run == kKvTile) {
+    uint32_t words[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) words[j] = __byte_perm(half[2 * j], half[2 * j + 1], 0x5410);
+    if (to.run == kKvTile) {
       *reinterpret_cast<uint4*>(mine) = make_uint4(words[0], words[1], words[2], words[3]);
     } else {   // the bytes of the tokens that come
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const int token = job.values == 0 ? r + 8 * (b % 2) : 2 * c + 8 * (b % 2) + b / 2;
-        if (token >= first && token < first + at.run)
+      for (int b = 0; b < 4; ++b)
+        if (here(job.values == 0 ? r + 8 * (b % 2) : 2 * c + 8 * (b % 2) + b / 2))
 #pragma unroll
           for (int j = 0; j < 4; ++j) mine[4 * j + b] = (uint8_t)(words[j] >> (8 * b));
-      }
     }
   }
 }
@@ -188,45 +199,50 @@ __global__ void __launch_bounds__(kStoreWarps * 32) kv4_load_kernel(float* k, fl
   __shared__ int32_t shared[kKvMaxSeqs + 1];
   pdl_wait();
   pdl_trigger();
-  const Job job = find_job<ROWS>(cache, seqs, starts, pos, n, rows, shared, false);
+  const Job job = find_job<ROWS>(cache, seqs, starts, pos, n, rows, shared);
   const int lane = threadIdx.x % 32, r = lane / 4, c = lane % 4, g = job.group, head = job.head, groups = cache.dim / kKvGroup;
   const int64_t ld = (int64_t)cache.kv_heads * cache.dim;
+  float* const out = (job.values ? v : k) + head * cache.dim + g * kKvGroup;
   for (uint32_t left = job.nowhere; left != 0; left &= left - 1)
-    *reinterpret_cast<float2*>((job.values ? v : k) + (job.row + __ffs(left) - 1) * ld + head * cache.dim + g * kKvGroup + 2 * lane) = make_float2(0.f, 0.f);
+    *reinterpret_cast<float2*>(out + (job.row + __ffs(left) - 1) * ld + 2 * lane) = make_float2(0.f, 0.f);
   for (uint32_t left = job.leads; left != 0; left &= left - 1) {
     const int lead = __ffs(left) - 1, row = job.row + lead;
-    const Kv4Place at{__shfl_sync(0xffffffffu, job.at.page, lead), __shfl_sync(0xffffffffu, job.at.token, lead), __shfl_sync(0xffffffffu, job.at.run, lead)};
-    const int first = at.token % kKvTile;
-    const uint8_t* tile = kv4_head(cache, layer, at.page, head) + at.token / kKvTile * kv4_tile_bytes(groups) + job.values * groups * (512 + 64);
+    const Kv4Place from{__shfl_sync(0xffffffffu, job.place.slot, lead), __shfl_sync(0xffffffffu, job.place.at, lead), __shfl_sync(0xffffffffu, job.place.run, lead)};
+    const int first = from.at % kKvTile, page = kv4_page(cache, from.slot, from.at);
+    if (page < 0) {
+      for (int t = 0; t < from.run; ++t) *reinterpret_cast<float2*>(out + (row + t) * ld + 2 * lane) = make_float2(0.f, 0.f);
+      continue;
+    }
+    float* const dst = out + (int64_t)(row - first) * ld;
+    const uint8_t* tile = kv4_head(cache, layer, page, head) + from.at % kPage / kKvTile * kv4_tile_bytes(groups) + job.values * groups * (512 + 64);
     const uint32_t* small = reinterpret_cast<const uint32_t*>(tile + groups * 512) + g * 16;
     const uint4 w = *reinterpret_cast<const uint4*>(tile + g * 512 + lane * 16);
     const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-    const int64_t from = (int64_t)(row - first) * ld + head * cache.dim + g * kKvGroup;
     if (job.values == 0) {
 #pragma unroll
       for (int hi = 0; hi < 2; ++hi) {
         const int token = r + 8 * hi;
-        if (token < first || token >= first + at.run) continue;
+        if (token < first || token >= first + from.run) continue;
         const float s = bf16_lo(small[r * 2 + hi]), m = bf16_hi(small[r * 2 + hi]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {   // word 2h + t: four entries
           float o[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[e] = fmaf(s, (float)(int)(words[j] >> (16 * (e / 2) + 8 * hi + 4 * (e % 2)) & 15) - 8.f, m);
-          *reinterpret_cast<float4*>(k + from + token * ld + j / 2 * 32 + 8 * c + j % 2 * 4) = make_float4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<float4*>(dst + token * ld + j / 2 * 32 + 8 * c + j % 2 * 4) = make_float4(o[0], o[1], o[2], o[3]);
         }
       }
     } else {
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         const int token = 2 * c + b % 2 * 8 + b / 2;
-        if (token < first || token >= first + at.run) continue;
+        if (token < first || token >= first + from.run) continue;
         const uint32_t both = small[token % 8 * 2 + token / 8];
         const float s = bf16_lo(both), m = bf16_hi(both);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t byte = words[j] >> (8 * b);
-          *reinterpret_cast<float2*>(v + from + token * ld + 16 * j + 2 * r) =
+          *reinterpret_cast<float2*>(dst + token * ld + 16 * j + 2 * r) =
               make_float2(fmaf(s, (float)(int)(byte & 15) - 8.f, m), fmaf(s, (float)(int)(byte >> 4 & 15) - 8.f, m));
         }
       }

@@ -22,23 +22,19 @@ int check_kv4_rows(const b200_kv4_cache* c, int64_t layer, const int32_t* seqs, 
                    const char* what);
 
 #ifdef __CUDACC__
-// Where a row goes.  page < 0: nowhere; else its token of the page, and how many rows from it on lie in its tile of 16 (0: an earlier row's run has it).
+// Where a row goes: its slot and position (slot < 0: nowhere), and how many rows from it on lie in its tile of 16 (0: an earlier row's run has it).
 struct Kv4Place {
-  int page, token, run;
+  int slot, at, run;
 };
-__device__ __forceinline__ Kv4Place kv4_place(const b200_kv4_cache& c, const int32_t* seqs, const int32_t* starts, const int32_t* pos, int n, int rows, int row) {
-  int lo = 0, hi = n;   // the last i with starts[i] <= row
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (starts[mid] <= row) lo = mid;
-    else hi = mid;
-  }
-  const int slot = seqs[lo], p = pos[lo], first = starts[lo], end = min(starts[lo + 1], rows);
-  const int64_t at = (int64_t)p + row - first;
-  if (first > row || row >= end || p < 0 || slot < 0 || slot >= c.n_seqs || at >= (int64_t)c.max_pages * kPage) return {-1, 0, 0};
-  const int page = c.table[(int64_t)slot * c.max_pages + at / kPage], in_tile = (int)(at % kKvTile);
-  const bool leads = in_tile == 0 || row == max(first, 0);
-  return {page < c.n_pages ? page : -1, (int)(at % kPage), leads ? min(kKvTile - in_tile, end - row) : 0};
+__device__ __forceinline__ Kv4Place kv4_place(const b200_kv4_cache& c, int slot, int pos, int first, int end, int row) {   // of a sequence with rows first … end − 1
+  const int64_t at = (int64_t)pos + row - first;
+  if (first > row || row >= end || pos < 0 || slot < 0 || slot >= c.n_seqs || at >= (int64_t)c.max_pages * kPage) return {-1, 0, 0};
+  const int in_tile = (int)(at % kKvTile);
+  return {slot, (int)at, in_tile == 0 || row == max(first, 0) ? min(kKvTile - in_tile, end - row) : 0};
+}
+__device__ __forceinline__ int kv4_page(const b200_kv4_cache& c, int slot, int at) {   // −1: none
+  const int page = c.table[(int64_t)slot * c.max_pages + at / kPage];
+  return page < c.n_pages ? page : -1;
 }
 __device__ __forceinline__ uint8_t* kv4_head(const b200_kv4_cache& c, int layer, int page, int head) {
   const int64_t block = 4 * kv4_tile_bytes(c.dim / kKvGroup);

@@ -44,15 +44,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(o) : "r"(v));
   return o;
 }
-__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 __device__ __forceinline__ long long warp_scan(long long v, int lane) {
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -117,7 +108,10 @@ struct Cut {
     each = (want + ctas - 1) / ctas;
     warps = want;
   }
-  __device__ __forceinline__ long long start(int w) const { return line * min(w, warps) / warps; }
+  __device__ __forceinline__ long long start(int w) const {
+    w = min(w, warps);
+    return line < 1 << 19 ? (long long)((uint32_t)line * (uint32_t)w / (uint32_t)warps) : line * w / warps;   // (64-bit divisions take a quarter of a µs)
+  }
 };
 // a warp's parts: of an item that came before it (0) and of one that goes on behind it (1).  [column][dim], maxima, sums
 __device__ __forceinline__ float* kv4_part(const Kv4Attn& p, int64_t warp, int which, int columns) {
@@ -134,7 +128,7 @@ struct Shape {
   static constexpr int kTile = kv4_tile_bytes(NG);
   static constexpr int kTiles = kStep / kKvTile;                // of a step
   static constexpr int kStage = kTiles * kTile;
-  static constexpr int kWarps = NG * NT <= 2 ? 16 : 8;
+  static constexpr int kWarps = 8;
   static constexpr int kThreads = kWarps * 32;
   static constexpr bool kQInRegs = NG * NT <= 4;
   static constexpr int kQBytes = kQInRegs ? 0 : NT * NG * 2 * 512;
@@ -199,31 +193,7 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
     at_line = min(stop, end);
     if (many <= 0) continue;
 
-    // the block's queries, as the B operands of K·qᵀ, and their sums over each group
     const int col0 = block * kCols, n_cols = s.count * p.group;
-    uint4 qf[S::kQInRegs ? NT : 1][NG][2];
-    float qsum[NG][NT][2];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int col = col0 + t * 8 + r;
-      const __nv_bfloat16* src = p.q + (int64_t)(s.row0 + col / p.group) * p.ld_q + (int64_t)(head * p.group + col % p.group) * kDim + 8 * c;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint4 u = col < n_cols ? *reinterpret_cast<const uint4*>(src + g * 64 + h * 32) : make_uint4(0, 0, 0, 0);
-          // entries {0, 2}, {1, 3}, {4, 6}, {5, 7}
-          const uint4 v = make_uint4(__byte_perm(u.x, u.y, 0x5410), __byte_perm(u.x, u.y, 0x7632), __byte_perm(u.z, u.w, 0x5410), __byte_perm(u.z, u.w, 0x7632));
-          if constexpr (S::kQInRegs) qf[t][g][h] = v;
-          else q_smem[((t * NG + g) * 2 + h) * 32 + lane] = v;
-          mma16816(sum, kBf16Ones, kBf16Ones, kBf16Ones, kBf16Ones, v.x, v.y);
-          mma16816(sum, kBf16Ones, kBf16Ones, kBf16Ones, kBf16Ones, v.z, v.w);
-        }
-        qsum[g][t][0] = sum[0];
-        qsum[g][t][1] = sum[1];
-      }
-    }
     int at[NT][2];   // positions of this lane's columns (2c, 2c + 1); −1: no column
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -266,6 +236,31 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
     }
     next = page_of(S::kStages - 1);
     int slot = 0;
+
+    // the block's queries, as the B operands of K·qᵀ, and their sums over each group
+    uint4 qf[S::kQInRegs ? NT : 1][NG][2];
+    float qsum[NG][NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int col = col0 + t * 8 + r;
+      const __nv_bfloat16* src = p.q + (int64_t)(s.row0 + col / p.group) * p.ld_q + (int64_t)(head * p.group + col % p.group) * kDim + 8 * c;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint4 u = col < n_cols ? *reinterpret_cast<const uint4*>(src + g * 64 + h * 32) : make_uint4(0, 0, 0, 0);
+          // entries {0, 2}, {1, 3}, {4, 6}, {5, 7}
+          const uint4 v = make_uint4(__byte_perm(u.x, u.y, 0x5410), __byte_perm(u.x, u.y, 0x7632), __byte_perm(u.z, u.w, 0x5410), __byte_perm(u.z, u.w, 0x7632));
+          if constexpr (S::kQInRegs) qf[t][g][h] = v;
+          else q_smem[((t * NG + g) * 2 + h) * 32 + lane] = v;
+          mma16816(sum, kBf16Ones, kBf16Ones, kBf16Ones, kBf16Ones, v.x, v.y);
+          mma16816(sum, kBf16Ones, kBf16Ones, kBf16Ones, kBf16Ones, v.z, v.w);
+        }
+        qsum[g][t][0] = sum[0];
+        qsum[g][t][1] = sum[1];
+      }
+    }
     for (int u = 0; u < n_steps; ++u) {
       const int ahead = u + S::kStages - 1, into = slot == 0 ? S::kStages - 1 : slot - 1;
       have = (have & ~(1u << (ahead % 32))) | (uint32_t)(next >= 0) << (ahead % 32);
@@ -501,65 +496,88 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
   }
 }
 
-// The items that lie in more than one warp's piece of the line.  CTA (c, column) takes those that begin in CTA c's pieces: its warps every eighth part in
-// order, then the warps meet.
+// The items that lie in more than one warp's piece of the line.  CTA (c, column) takes those that begin in CTA c's pieces: a warp each while their parts are few,
+// else all warps, every eighth part in order, and then the warps meet.
 constexpr int kJoinWarps = 8;
 template <int NG>
+struct Joined {
+  float m = -INFINITY, l = 0.f;
+  float2 v[NG];
+  __device__ Joined() {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) v[g] = make_float2(0.f, 0.f);
+  }
+  __device__ __forceinline__ void take(float mw, float lw, const float2 (&x)[NG]) {
+    if (lw == 0.f) return;   // has seen no token
+    const float top = fmaxf(m, mw), f = exp2_fast(mw - top), keep = l == 0.f ? 0.f : exp2_fast(m - top);
+    m = top;
+    l = fmaf(f, lw, l * keep);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) v[g] = make_float2(fmaf(f, x[g].x, v[g].x * keep), fmaf(f, x[g].y, v[g].y * keep));
+  }
+};
+template <int NG>
 __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn p, int columns, int warps) {
-  __shared__ float part_m[kJoinWarps], part_l[kJoinWarps], part_o[kJoinWarps][NG * 64];
-  constexpr int kDim = NG * 64;
+  __shared__ float part_m[kJoinWarps], part_l[kJoinWarps];
+  __shared__ float2 part_v[kJoinWarps][NG * 32];
+  constexpr int kDim = NG * 64, kAtOnce = 4;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, col = blockIdx.y;
   pdl_wait();
   pdl_trigger();
   const Kv4Split* splits = p.splits + blockIdx.x * warps;
-  uint32_t left = __ballot_sync(0xffffffffu, lane < warps && splits[lane].from >= 0);
-  for (; left != 0; left &= left - 1) {
-    const Kv4Split s = splits[__ffs(left) - 1];
-    const int at = s.col0 + col;
-    if (at >= s.n_cols) continue;
-    const bool some = s.in0 < s.in1;
-    const int before = some ? s.in0 * s.each - s.from : s.to - s.from + 1, whole = some ? s.in1 - s.in0 : 0;
-    const int parts = before + whole + (some ? s.to - s.in1 * s.each + 1 : 0);
-    float m = -INFINITY, l = 0.f;
-    float2 v[NG];
+  const Kv4Split mine = lane < warps ? splits[lane] : Kv4Split{-1};
+  auto of = [&](int v, int from) { return __shfl_sync(0xffffffffu, v, from); };
+  int number = 0;
+  for (uint32_t left = __ballot_sync(0xffffffffu, mine.from >= 0 && mine.col0 + col < mine.n_cols); left != 0; left &= left - 1) {
+    const int i = __ffs(left) - 1, from = of(mine.from, i), to = of(mine.to, i), in0 = of(mine.in0, i), in1 = of(mine.in1, i), each = of(mine.each, i);
+    const bool some = in0 < in1;
+    const int before = some ? in0 * each - from : to - from + 1, whole = some ? in1 - in0 : 0, parts = before + whole + (some ? to - in1 * each + 1 : 0);
+    const bool alone = parts <= 2 * kAtOnce;
+    if (alone && number++ % kJoinWarps != warp) continue;
+    const int first = alone ? 0 : warp, step = alone ? 1 : kJoinWarps;
+    Joined<NG> o;
+    for (int k0 = first; k0 < parts; k0 += kAtOnce * step) {
+      float m[kAtOnce], l[kAtOnce];
+      float2 x[kAtOnce][NG];
 #pragma unroll
-    for (int g = 0; g < NG; ++g) v[g] = make_float2(0.f, 0.f);
-#pragma unroll 4
-    for (int k = warp; k < parts; k += kJoinWarps) {
-      const int w = k < before ? s.from + k : k < before + whole ? (s.in0 + k - before) * s.each : s.in1 * s.each + k - before - whole;
-      const float* part = kv4_part(p, (int64_t)(w / s.each) * warps + w % s.each, k < before && k == 0, columns);
-      const float mw = part[columns * kDim + col], lw = part[columns * kDim + columns + col];
-      float2 x[NG];
+      for (int e = 0; e < kAtOnce; ++e) {
+        const int k = min(k0 + e * step, parts - 1);
+        const int w = k < before ? from + k : k < before + whole ? (in0 + k - before) * each : in1 * each + k - before - whole;
+        const float* part = kv4_part(p, (int64_t)(w / each) * warps + w % each, k < before && k == 0, columns);
+        m[e] = part[columns * kDim + col];
+        l[e] = k0 + e * step < parts ? part[columns * kDim + columns + col] : 0.f;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) x[g] = *reinterpret_cast<const float2*>(part + col * kDim + g * 64 + 2 * lane);
-      if (lw == 0.f) continue;
-      const float top = fmaxf(m, mw), f = exp2_fast(mw - top), keep = l == 0.f ? 0.f : exp2_fast(m - top);
-      m = top;
-      l = fmaf(f, lw, l * keep);
-#pragma unroll
-      for (int g = 0; g < NG; ++g) v[g] = make_float2(fmaf(f, x[g].x, v[g].x * keep), fmaf(f, x[g].y, v[g].y * keep));
-    }
-    if (lane == 0) {
-      part_m[warp] = m;
-      part_l[warp] = l;
-    }
-#pragma unroll
-    for (int g = 0; g < NG; ++g) *reinterpret_cast<float2*>(part_o[warp] + g * 64 + 2 * lane) = v[g];
-    __syncthreads();
-    for (int d = threadIdx.x; d < kDim; d += kJoinWarps * 32) {
-      float top = -INFINITY, sum = 0.f, y = 0.f;
-#pragma unroll
-      for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, part_m[w]);
-#pragma unroll
-      for (int w = 0; w < kJoinWarps; ++w) {
-        if (part_l[w] == 0.f) continue;
-        const float f = exp2_fast(part_m[w] - top);
-        sum = fmaf(f, part_l[w], sum);
-        y = fmaf(f, part_o[w][d], y);
+        for (int g = 0; g < NG; ++g) x[e][g] = *reinterpret_cast<const float2*>(part + col * kDim + g * 64 + 2 * lane);
       }
-      p.out[((int64_t)(s.row0 + at / p.group) * p.q_heads + s.head * p.group + at % p.group) * kDim + d] = f_to_bf16(sum == 0.f ? 0.f : y / sum);
+#pragma unroll
+      for (int e = 0; e < kAtOnce; ++e) o.take(m[e], l[e], x[e]);
     }
-    __syncthreads();
+    const int at = of(mine.col0, i) + col;
+    __nv_bfloat16* out = p.out + ((int64_t)(of(mine.row0, i) + at / p.group) * p.q_heads + of(mine.head, i) * p.group + at % p.group) * kDim;
+    if (!alone) {
+      if (lane == 0) {
+        part_m[warp] = o.m;
+        part_l[warp] = o.l;
+      }
+#pragma unroll
+      for (int g = 0; g < NG; ++g) part_v[warp][g * 32 + lane] = o.v[g];
+      __syncthreads();
+      if (warp == 0) {
+        o = Joined<NG>();
+        for (int w = 0; w < kJoinWarps; ++w) {
+          float2 x[NG];
+#pragma unroll
+          for (int g = 0; g < NG; ++g) x[g] = part_v[w][g * 32 + lane];
+          o.take(part_m[w], part_l[w], x);
+        }
+      }
+      __syncthreads();
+    }
+    if (alone || warp == 0) {
+      const float f = o.l == 0.f ? 0.f : 1.f / o.l;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) *reinterpret_cast<uint32_t*>(out + g * 64 + 2 * lane) = pack2(o.v[g].x * f, o.v[g].y * f);
+    }
   }
 }
 

@@ -14,11 +14,9 @@ namespace b200 {
 
 namespace {
 
-constexpr int kWarps = 8;
-
 __device__ __forceinline__ uint4 ld_once(const uint4* p) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
 
@@ -32,116 +30,153 @@ struct W4Params {
   int m, n, k, blocks, groups;
 };
 
-// A warp takes every kWarps-th column block of RT row tiles; the CTA's warps are summed in shared memory in their order.  Values enter the
-// products as value − 8, exact in bf16, and a group's sums are scaled in fp32: nothing is rounded to fewer bits before the result.
-template <int NT, int RT, int GROUP, bool ZERO>
-__global__ void __launch_bounds__(kWarps * 32) w4_linear_kernel(const W4Params p) {
-  constexpr int kParts = GROUP == 32 ? 2 : 1;   // groups of a column block (of 128: one for two blocks)
-  constexpr int kUnroll = NT * RT <= 2 ? 4 : NT * RT <= 4 ? 2 : 1;
-  constexpr int kSums = RT * NT * 4;
-  __shared__ float red[kWarps][kSums][32];
+// A CTA takes RT row tiles, a warp one of WARPS equal pieces of their columns, which come through a ring of its own in shared memory, 128 columns a stage; the
+// pieces are summed in shared memory in their order.  Values enter the products exactly and a group's sums are scaled in fp32, so nothing is rounded to
+// fewer bits before the result: as 128 + nibble, with Σ x of the group from a product with ones (kSums: with one tile of columns that costs less than
+// the subtraction, and a zero needs the sum anyway), or as nibble − 8.  What bounds it is the unpacking: seven instructions of half rate for eight values.
+template <int NT, int RT, int WARPS, int GROUP, bool ZERO>
+struct W4Shape {
+  static constexpr int kStages = 2;   // (four take the room of a third and a fourth CTA: 28 672 × 4 096 18.1 → 20.0 µs)
+  static constexpr bool kSums = ZERO || NT == 1;
+  static constexpr int kParts = 128 / GROUP;   // groups of a stage
+  static constexpr int kSmall = RT * kParts * (ZERO ? 2 : 1) * 32;   // bytes of scales and zeros
+  static constexpr int kStage = RT * 1024 + kSmall;
+  static constexpr int kTotals = RT * NT * 4;
+  static constexpr int kRing = kStages * kStage > kTotals * 128 ? kStages * kStage : kTotals * 128;
+  static constexpr int kSmem = WARPS * kRing;
+};
+template <int NT, int RT, int WARPS, int GROUP, bool ZERO>
+__global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 32 / WARPS : 1) w4_linear_kernel(const W4Params p) {
+  using S = W4Shape<NT, RT, WARPS, GROUP, ZERO>;
+  constexpr int kSteps = 8 / S::kParts;   // products of a group
+  extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
-  const int tile0 = blockIdx.x * RT, tiles = (p.n + 15) / 16;
+  const int tiles = (p.n + 15) / 16, tile0 = blockIdx.x * RT;
+  const int all = (p.blocks + 1) / 2, from = all * warp / WARPS, to = all * (warp + 1) / WARPS;
+  uint8_t* const ring = smem + warp * S::kRing;
   pdl_wait();
   pdl_trigger();
+
   const uint4* q[RT];
-  const uint32_t *scale[RT], *zero[RT];
 #pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    const int64_t tile = min(tile0 + t, tiles - 1);
-    q[t] = p.q + tile * p.blocks * 32 + lane;
-    scale[t] = p.scale + tile * p.groups * 8 + r;
-    zero[t] = p.zero + tile * p.groups * 8 + r;
+  for (int t = 0; t < RT; ++t) q[t] = p.q + ((int64_t)min(tile0 + t, tiles - 1) * p.blocks + 2 * from) * 32 + lane;
+  // this lane's part of the small numbers: of row tile and group of the stage j / 8, the scale or the zero of rows lane % 8, + 8
+  constexpr int kEach = RT * S::kParts * (ZERO ? 2 : 1) * 8;
+  const uint32_t* small[(kEach + 31) / 32];
+#pragma unroll
+  for (int e = 0; e < (kEach + 31) / 32; ++e) {
+    const int j = (lane + 32 * e) / 8, t = j / S::kParts % RT;
+    small[e] = (j >= RT * S::kParts ? p.zero : p.scale) + (int64_t)min(tile0 + t, tiles - 1) * p.groups * 8 + lane % 8;
   }
+  auto fetch = [&](int i) {
+    if (i < to) {
+      uint8_t* dst = ring + i % S::kStages * S::kStage;
+      const bool both = 2 * i + 1 < p.blocks;   // (an odd last block's neighbour meets zeros of x)
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        cp_async16(dst + t * 1024 + lane * 16, q[t]);
+        if (both) cp_async16(dst + t * 1024 + 512 + lane * 16, q[t] + 32);
+        q[t] += 64;
+      }
+#pragma unroll
+      for (int e = 0; e < (kEach + 31) / 32; ++e) {
+        const int g = min(i * S::kParts + (lane + 32 * e) / 8 % S::kParts, p.groups - 1);
+        if (kEach % 32 == 0 || lane + 32 * e < kEach) cp_async4(dst + RT * 1024 + (lane + 32 * e) * 4, small[e] + g * 8);
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int a = 0; a < S::kStages - 1; ++a) fetch(from + a);
+  // rows past m have the last row's numbers: their columns of the products go nowhere
   const __nv_bfloat16* x[NT];
-  bool has[NT];
 #pragma unroll
-  for (int i = 0; i < NT; ++i) {
-    has[i] = i * 8 + r < p.m;
-    x[i] = p.x + (int64_t)(i * 8 + r) * p.k + 8 * c;
-  }
+  for (int t = 0; t < NT; ++t) x[t] = p.x + (int64_t)min(t * 8 + r, p.m - 1) * p.k + 8 * c;
   float total[RT][NT][4] = {};
-#pragma unroll kUnroll
-  for (int b = warp; b < p.blocks; b += kWarps) {
-    uint4 w[RT], xb[NT][2];
-    uint32_t s[RT][kParts], z[RT][kParts];
+  for (int i = from; i < to; ++i) {
+    uint4 xb[NT][4];
+    const bool full = (i + 1) * 128 <= p.k;
 #pragma unroll
-    for (int t = 0; t < RT; ++t) w[t] = ld_once(q[t] + (int64_t)b * 32);
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        xb[i][h] = has[i] && b * 64 + h * 32 + c * 8 < p.k ? __ldg(reinterpret_cast<const uint4*>(x[i] + b * 64 + h * 32)) : make_uint4(0, 0, 0, 0);
+      for (int h = 0; h < 4; ++h) {
+        if (full) xb[t][h] = *reinterpret_cast<const uint4*>(x[t] + i * 128 + h * 32);
+        else xb[t][h] = i * 128 + h * 32 + c * 8 < p.k ? *reinterpret_cast<const uint4*>(x[t] + i * 128 + h * 32) : make_uint4(0, 0, 0, 0);
+      }
+    fetch(i + S::kStages - 1);
+    cp_async_wait<S::kStages - 1>();
+    __syncwarp();
+    const uint8_t* stage = ring + i % S::kStages * S::kStage;
+    const uint32_t* nums = reinterpret_cast<const uint32_t*>(stage + RT * 1024);
+    uint4 w[RT][2];
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
-      for (int h = 0; h < kParts; ++h) {
-        const int g = GROUP == 32 ? min(2 * b + h, p.groups - 1) : GROUP == 64 ? b : b / 2;
-        s[t][h] = __ldg(scale[t] + (int64_t)g * 8);
-        z[t][h] = ZERO ? __ldg(zero[t] + (int64_t)g * 8) : 0;
-      }
+      for (int h = 0; h < 2; ++h) w[t][h] = *reinterpret_cast<const uint4*>(stage + t * 1024 + h * 512 + lane * 16);
 #pragma unroll
-    for (int h = 0; h < kParts; ++h) {
-      constexpr int kHalves = 2 / kParts;
-      float sum[NT][4];   // Σ x of the group, the same for every row
-      if constexpr (ZERO) {
+    for (int h = 0; h < S::kParts; ++h) {
+      float sum[NT][4] = {};
+      if constexpr (S::kSums) {
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          sum[i][0] = sum[i][1] = sum[i][2] = sum[i][3] = 0.f;
+        for (int j = h * kSteps; j < (h + 1) * kSteps; ++j)
 #pragma unroll
-          for (int e = 0; e < kHalves; ++e) {
-            const uint4 v = xb[i][h + e];
-            mma16816(sum[i], kBf16Ones, kBf16Ones, kBf16Ones, kBf16Ones, v.x, v.y);
-            mma16816(sum[i], kBf16Ones, kBf16Ones, kBf16Ones, kBf16Ones, v.z, v.w);
-          }
-        }
+          for (int n = 0; n < NT; ++n)
+            mma16816(sum[n], kBf16Ones, kBf16Ones, kBf16Ones, kBf16Ones, j % 2 ? xb[n][j / 2].z : xb[n][j / 2].x, j % 2 ? xb[n][j / 2].w : xb[n][j / 2].y);
       }
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
         float acc[NT][4] = {};
 #pragma unroll
-        for (int e = 0; e < kHalves; ++e) {
-          uint32_t a[4];
-          nibbles_bf16(h + e == 0 ? w[t].x : w[t].z, a);
+        for (int j = h * kSteps; j < (h + 1) * kSteps; ++j) {
+          const uint4 v = w[t][j / 4];
+          const uint32_t word = j % 4 == 0 ? v.x : j % 4 == 1 ? v.y : j % 4 == 2 ? v.z : v.w;
+          uint32_t f[4];
+          if constexpr (S::kSums) nibbles_128(word, f);
+          else nibbles_bf16(word, f);
 #pragma unroll
-          for (int i = 0; i < NT; ++i) mma16816(acc[i], a[0], a[1], a[2], a[3], xb[i][h + e].x, xb[i][h + e].y);
-          nibbles_bf16(h + e == 0 ? w[t].y : w[t].w, a);
-#pragma unroll
-          for (int i = 0; i < NT; ++i) mma16816(acc[i], a[0], a[1], a[2], a[3], xb[i][h + e].z, xb[i][h + e].w);
+          for (int n = 0; n < NT; ++n)
+            mma16816(acc[n], f[0], f[1], f[2], f[3], j % 2 ? xb[n][j / 2].z : xb[n][j / 2].x, j % 2 ? xb[n][j / 2].w : xb[n][j / 2].y);
         }
-        const float s0 = bf16_lo(s[t][h]), s1 = bf16_hi(s[t][h]);
-        const float z0 = 8.f - bf16_lo(z[t][h]), z1 = 8.f - bf16_hi(z[t][h]);
+        const uint32_t s = nums[(t * S::kParts + h) * 8 + r], z = ZERO ? nums[((RT + t) * S::kParts + h) * 8 + r] : 0;
+        const float s0 = bf16_lo(s), s1 = bf16_hi(s);
+        const float z0 = ZERO ? -128.f - bf16_lo(z) : -kNibbleOff, z1 = ZERO ? -128.f - bf16_hi(z) : -kNibbleOff;
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          if constexpr (ZERO) {
-            acc[i][0] = fmaf(z0, sum[i][0], acc[i][0]);
-            acc[i][1] = fmaf(z0, sum[i][1], acc[i][1]);
-            acc[i][2] = fmaf(z1, sum[i][2], acc[i][2]);
-            acc[i][3] = fmaf(z1, sum[i][3], acc[i][3]);
+        for (int n = 0; n < NT; ++n) {
+          if constexpr (S::kSums) {
+            acc[n][0] = fmaf(z0, sum[n][0], acc[n][0]);
+            acc[n][1] = fmaf(z0, sum[n][1], acc[n][1]);
+            acc[n][2] = fmaf(z1, sum[n][0], acc[n][2]);
+            acc[n][3] = fmaf(z1, sum[n][1], acc[n][3]);
           }
-          total[t][i][0] = fmaf(s0, acc[i][0], total[t][i][0]);
-          total[t][i][1] = fmaf(s0, acc[i][1], total[t][i][1]);
-          total[t][i][2] = fmaf(s1, acc[i][2], total[t][i][2]);
-          total[t][i][3] = fmaf(s1, acc[i][3], total[t][i][3]);
+          total[t][n][0] = fmaf(s0, acc[n][0], total[t][n][0]);
+          total[t][n][1] = fmaf(s0, acc[n][1], total[t][n][1]);
+          total[t][n][2] = fmaf(s1, acc[n][2], total[t][n][2]);
+          total[t][n][3] = fmaf(s1, acc[n][3], total[t][n][3]);
         }
       }
     }
+    __syncwarp();   // the stage is free
   }
+  cp_async_wait<0>();
+  __syncwarp();
+  float* const own = reinterpret_cast<float*>(ring);
 #pragma unroll
   for (int t = 0; t < RT; ++t)
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) red[warp][(t * NT + i) * 4 + e][lane] = total[t][i][e];
+      for (int e = 0; e < 4; ++e) own[((t * NT + n) * 4 + e) * 32 + lane] = total[t][n][e];
   __syncthreads();
-  for (int o = threadIdx.x; o < kSums * 32; o += kWarps * 32) {   // rows of W fastest
-    const int row = o % (16 * RT), col = o / (16 * RT);
-    const int from = ((row / 16) * NT + col / 8) * 4 + (row % 16 / 8) * 2 + col % 2, at = row % 8 * 4 + col % 8 / 2;
+  constexpr int kRows = RT * 16;
+  for (int o = threadIdx.x; o < kRows * NT * 8; o += WARPS * 32) {   // rows of W fastest
+    const int row = o % kRows, col = o / kRows, n = blockIdx.x * kRows + row;
+    if (col >= p.m) break;
+    if (n >= p.n) continue;
+    const int of = ((row / 16 * NT + col / 8) * 4 + row % 16 / 8 * 2 + col % 2) * 32 + row % 8 * 4 + col % 8 / 2;
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) v += red[w][from][at];
-    const int n = tile0 * 16 + row;
-    if (n < p.n && col < p.m) p.y[(int64_t)col * p.n + n] = f_to_bf16(p.bias != nullptr ? v + bf16_to_f(p.bias[n]) : v);
+    for (int w = 0; w < WARPS; ++w) v += reinterpret_cast<const float*>(smem + w * S::kRing)[of];
+    p.y[(int64_t)col * p.n + n] = f_to_bf16(p.bias != nullptr ? v + bf16_to_f(p.bias[n]) : v);
   }
 }
 
@@ -197,15 +232,21 @@ W4Params params(const b200_w4_weight& w) {
   return p;
 }
 
-template <int NT, int RT>
-int launch_rows(const W4Params& p, int group, cudaStream_t st) {
-  const dim3 grid((unsigned)(((p.n + 15) / 16 + RT - 1) / RT));
-  const bool pdl = op_pdl(st), zero = p.zero != nullptr;
-  const auto k = group == 32 ? (zero ? w4_linear_kernel<NT, RT, 32, true> : w4_linear_kernel<NT, RT, 32, false>)
-                 : group == 64 ? (zero ? w4_linear_kernel<NT, RT, 64, true> : w4_linear_kernel<NT, RT, 64, false>)
-                               : (zero ? w4_linear_kernel<NT, RT, 128, true> : w4_linear_kernel<NT, RT, 128, false>);
-  B200_CUDA(launch_pdl(k, grid, dim3(kWarps * 32), 0, st, pdl, p));
+template <int NT, int RT, int WARPS, int GROUP, bool ZERO>
+int launch_kernel(const W4Params& p, cudaStream_t st) {
+  using S = W4Shape<NT, RT, WARPS, GROUP, ZERO>;
+  static PerDevice attrs;
+  B200_CUDA(attrs([] { return cudaFuncSetAttribute(w4_linear_kernel<NT, RT, WARPS, GROUP, ZERO>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem); }));
+  const int rows = RT * 16;
+  B200_CUDA(launch_pdl(w4_linear_kernel<NT, RT, WARPS, GROUP, ZERO>, dim3((unsigned)((p.n + rows - 1) / rows)), dim3(WARPS * 32), S::kSmem, st, op_pdl(st), p));
   return B200_OK;
+}
+template <int NT, int RT, int WARPS>
+int launch_rows(const W4Params& p, int group, cudaStream_t st) {
+  const bool zero = p.zero != nullptr;
+  if (group == 32) return zero ? launch_kernel<NT, RT, WARPS, 32, true>(p, st) : launch_kernel<NT, RT, WARPS, 32, false>(p, st);
+  if (group == 64) return zero ? launch_kernel<NT, RT, WARPS, 64, true>(p, st) : launch_kernel<NT, RT, WARPS, 64, false>(p, st);
+  return zero ? launch_kernel<NT, RT, WARPS, 128, true>(p, st) : launch_kernel<NT, RT, WARPS, 128, false>(p, st);
 }
 
 int launch_dequant(void* out, const W4Params& p, int group, float* bias_out, cudaStream_t st) {
@@ -214,18 +255,19 @@ int launch_dequant(void* out, const W4Params& p, int group, float* bias_out, cud
   return B200_OK;
 }
 
-// Rows of x for which W is laid out as bf16 for the tcgen05 GEMM.
-bool as_gemm(int64_t m, int64_t n) { return m > 64 && n % 8 == 0; }
+// Rows of x for which W is laid out as bf16 for the tcgen05 GEMM: more than 64, and more than 32 over a large W, where eight tiles of columns cost the
+// mma.sync kernel more than the copy of W (µs at 64 rows, here / there: 4 096 × 4 096 16.8 / 17.7, 14 336 × 4 096 56 / 47).
+bool as_gemm(int64_t m, int64_t n, int64_t k) { return n % 8 == 0 && (m > 64 || (m > 32 && n * k > 20 * 1000 * 1000)); }
 int64_t bf16_bytes(int64_t n, int64_t k) { return (n * k * 2 + 15) / 16 * 16; }
 
 }  // namespace
 
-int64_t w4_linear_workspace_bytes(int64_t m, int64_t n, int64_t k) { return as_gemm(m, n) ? bf16_bytes(n, k) + n * 4 : 0; }
+int64_t w4_linear_workspace_bytes(int64_t m, int64_t n, int64_t k) { return as_gemm(m, n, k) ? bf16_bytes(n, k) + n * 4 : 0; }
 
 int launch_w4_linear(void* y, const void* x, const b200_w4_weight& w, const void* bias, int64_t m, void* workspace, cudaStream_t st) {
   W4Params p = params(w);
   p.bias = (const __nv_bfloat16*)bias;
-  if (as_gemm(m, w.n)) {
+  if (as_gemm(m, w.n, w.k)) {
     float* b = bias != nullptr ? (float*)((char*)workspace + bf16_bytes(w.n, w.k)) : nullptr;
     const int rc = launch_dequant(workspace, p, w.group, b, st);
     if (rc != B200_OK) return rc;
@@ -236,8 +278,14 @@ int launch_w4_linear(void* y, const void* x, const b200_w4_weight& w, const void
     p.m = (int)std::min<int64_t>(m - r, 64);
     p.x = (const __nv_bfloat16*)x + r * w.k;
     p.y = (__nv_bfloat16*)y + r * w.n;
-    const int rc = p.m <= 8 ? launch_rows<1, 1>(p, w.group, st) : p.m <= 16 ? launch_rows<2, 1>(p, w.group, st)
-                 : p.m <= 32 ? launch_rows<4, 1>(p, w.group, st) : launch_rows<8, 1>(p, w.group, st);
+    // Two row tiles to a warp share the loads of x and its sums, where CTAs are left for all SMs (µs, one / two: 1 × 4 096 × 4 096 4.9 / 4.7, 8 × 8 192 × 4 096
+    // 8.1 / 7.2, 32 × 4 096 × 4 096 12.8 / 9.7; 8 × 2 048 × 4 896 4.9 / 5.7, 32 × 1 024 × 4 096 6.9 / 9.1).  All warps of a CTA share a row tile's
+    // columns: fewer warps to a tile are fewer sums, and lost at every size (28 672 × 4 096: 17.7, four warps a tile 19.3).
+    const bool two = (p.n + 15) / 16 >= 256;
+    const int rc = p.m <= 8 ? (two ? launch_rows<1, 2, 8>(p, w.group, st) : launch_rows<1, 1, 8>(p, w.group, st))
+                 : p.m <= 16 ? (two ? launch_rows<2, 2, 8>(p, w.group, st) : launch_rows<2, 1, 8>(p, w.group, st))
+                 : p.m <= 32 ? (two ? launch_rows<4, 2, 8>(p, w.group, st) : launch_rows<4, 1, 8>(p, w.group, st))
+                             : (two ? launch_rows<8, 2, 8>(p, w.group, st) : launch_rows<8, 1, 8>(p, w.group, st));
     if (rc != B200_OK) return rc;
   }
   return B200_OK;
