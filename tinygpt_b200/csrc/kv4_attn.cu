@@ -22,6 +22,25 @@ namespace {
 constexpr int kStep = 32, kAhead = 2;
 constexpr int kGrid = 148;
 
+// Division by a number that the host knows (Granlund and Montgomery): a multiplication and two shifts
+struct Divisor {
+  uint32_t d, m;
+  int s1, s2;
+  explicit Divisor(uint32_t d_ = 1) : d(d_) {
+    int s = 0;
+    while ((1ull << s) < d) ++s;
+    m = (uint32_t)((((1ull << s) - d) << 32) / d + 1);
+    s1 = std::min(s, 1);
+    s2 = std::max(s - 1, 0);
+  }
+#ifdef __CUDACC__
+  __device__ __forceinline__ int of(int n) const {
+    const uint32_t t = __umulhi(m, (uint32_t)n);
+    return (int)((t + (((uint32_t)n - t) >> s1)) >> s2);
+  }
+#endif
+};
+
 struct Kv4Attn {
   b200_kv4_cache cache;
   __nv_bfloat16* out;
@@ -30,7 +49,8 @@ struct Kv4Attn {
   const int32_t *seqs, *starts, *pos;
   float* parts;
   struct Kv4Split* splits;   // of every warp
-  int layer, q_heads, group, n, rows, window;
+  Divisor group, kv_heads;   // query heads of a key/value head
+  int layer, q_heads, n, rows, window;
   float scale_log2;
 };
 
@@ -63,7 +83,7 @@ __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4Attn& p, int i, int columns) 
   s.count = max(min(p.starts[i + 1], p.rows) - s.row0, 0);
   s.pos = min(p.pos[i], 1 << 30);
   s.slot = p.seqs[i];
-  s.blocks = (int)(((int64_t)s.count * p.group + columns - 1) / columns);
+  s.blocks = (int)(((int64_t)s.count * p.group.d + columns - 1) / columns);
   s.last = 0;
   s.step0 = 0;
   if (s.pos >= 0 && s.slot >= 0 && s.slot < p.cache.n_seqs)
@@ -74,22 +94,40 @@ __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4Attn& p, int i, int columns) 
   return s;
 }
 __device__ __forceinline__ long long kv4_line(const Kv4Attn& p, const Kv4Seq& s) { return (long long)s.blocks * p.cache.kv_heads * (s.steps + kAhead); }
-// ends[i]: the line up to the end of sequence i.  All threads of a CTA of THREADS.
+__device__ __forceinline__ Kv4Seq kv4_from(const Kv4Seq& s, int lane) {   // another lane's
+  Kv4Seq o;
+  o.row0 = __shfl_sync(0xffffffffu, s.row0, lane);
+  o.count = __shfl_sync(0xffffffffu, s.count, lane);
+  o.pos = __shfl_sync(0xffffffffu, s.pos, lane);
+  o.slot = __shfl_sync(0xffffffffu, s.slot, lane);
+  o.last = __shfl_sync(0xffffffffu, s.last, lane);
+  o.step0 = __shfl_sync(0xffffffffu, s.step0, lane);
+  o.steps = __shfl_sync(0xffffffffu, s.steps, lane);
+  o.blocks = __shfl_sync(0xffffffffu, s.blocks, lane);
+  return o;
+}
+// ends[i]: the line up to the end of sequence i; all of it comes back.  The call has checked that it is below 2^31 for starts that do not fall; for others it may not
+// be, and nothing is done.  All threads of a CTA of THREADS.
+__device__ __forceinline__ int kv4_whole(long long line) { return line <= INT32_MAX ? (int)line : 0; }
 template <int THREADS>
-__device__ void kv4_plan(const Kv4Attn& p, int columns, long long* ends) {
+__device__ int kv4_plan(const Kv4Attn& p, int columns, int* ends) {
   __shared__ long long carry[THREADS / 32];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, each = (p.n + THREADS - 1) / THREADS, first = threadIdx.x * each;
   long long sum = 0;
-  for (int i = first; i < min(first + each, p.n); ++i) ends[i] = sum += kv4_line(p, kv4_seq(p, i, columns));
+  for (int i = first; i < min(first + each, p.n); ++i) sum += kv4_line(p, kv4_seq(p, i, columns));
   const long long upto = warp_scan(sum, lane);
   if (lane == 31) carry[warp] = upto;
   __syncthreads();
-  long long before = upto - sum;
-  for (int w = 0; w < warp; ++w) before += carry[w];
-  for (int i = first; i < min(first + each, p.n); ++i) ends[i] += before;
+  long long before = upto - sum, all = 0;
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += carry[w];
+    all += carry[w];
+  }
+  for (int i = first; i < min(first + each, p.n); ++i) ends[i] = (int)(before += kv4_line(p, kv4_seq(p, i, columns)));
   __syncthreads();
+  return kv4_whole(all);
 }
-__device__ __forceinline__ int kv4_find(const long long* ends, int n, long long at) {   // the first i with ends[i] > at
+__device__ __forceinline__ int kv4_find(const int* ends, int n, int at) {   // the first i with ends[i] > at
   int lo = 0, hi = n - 1;
   while (lo < hi) {
     const int mid = (lo + hi) / 2;
@@ -98,20 +136,19 @@ __device__ __forceinline__ int kv4_find(const long long* ends, int n, long long 
   }
   return lo;
 }
-// How the line is cut: `warps` pieces, `each` CTA having so many of them; piece w starts at line·w / warps.  A piece is no shorter than a step and what
+// How the line is cut: `warps` pieces, `each` CTA having so many of them; piece w starts at about line·w / warps (as fp32 has it: the same for everyone).  A piece is no shorter than a step and what
 // comes before it, and short lines are spread over the CTAs first.
 struct Cut {
-  long long line;
-  int warps, each;
-  __device__ Cut(long long line_, int ctas, int most) : line(line_) {
-    const int want = (int)min(max(line / (kAhead + 1), 1ll), (long long)ctas * most);
-    each = (want + ctas - 1) / ctas;
-    warps = want;
+  int line, warps, each, whole, rest;   // line = whole·warps + rest
+  float inverse;
+  __device__ Cut(int line_, int most) : line(line_) {
+    warps = min(max(line / (kAhead + 1), 1), kGrid * most);
+    each = (warps + kGrid - 1) / kGrid;
+    inverse = __frcp_rn((float)warps);
+    whole = line / warps;
+    rest = line - whole * warps;
   }
-  __device__ __forceinline__ long long start(int w) const {
-    w = min(w, warps);
-    return line < 1 << 19 ? (long long)((uint32_t)line * (uint32_t)w / (uint32_t)warps) : line * w / warps;   // (64-bit divisions take a quarter of a µs)
-  }
+  __device__ __forceinline__ int start(int w) const { return w < warps ? w * whole + (int)((float)(w * rest) * inverse) : line; }
 };
 // a warp's parts: of an item that came before it (0) and of one that goes on behind it (1).  [column][dim], maxima, sums
 __device__ __forceinline__ float* kv4_part(const Kv4Attn& p, int64_t warp, int which, int columns) {
@@ -132,11 +169,11 @@ struct Shape {
   static constexpr int kThreads = kWarps * 32;
   static constexpr bool kQInRegs = NG * NT <= 4;
   static constexpr int kQBytes = kQInRegs ? 0 : NT * NG * 2 * 512;
-  static constexpr int kRoom = 232448 - 1024 - kKvMaxSeqs * 8;
+  static constexpr int kRoom = 232448 - 1024 - kKvMaxSeqs * 4;
   static constexpr int kStages = kWarps * (3 * kStage + kQBytes) <= kRoom ? 3 : 2;
-  static constexpr int kRing = kStages * kStage > 8 * NT * (NG * 64 + 2) * 4 ? kStages * kStage : (8 * NT * (NG * 64 + 2) * 4 + 15) / 16 * 16;
+  static constexpr int kRing = kStages * kStage > 8 * NT * (NG * 64 + 6) * 4 ? kStages * kStage : (8 * NT * (NG * 64 + 6) * 4 + 15) / 16 * 16;
   static constexpr int kOwn = kRing + kQBytes;                  // shared memory of a warp
-  static constexpr int kSmem = kWarps * kOwn + kKvMaxSeqs * 8;
+  static constexpr int kSmem = kWarps * kOwn + kKvMaxSeqs * 4;
   static_assert(kWarps * kOwn <= kRoom, "shared memory of an SM");
 };
 
@@ -148,61 +185,78 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
   uint8_t* const ring = smem + warp * S::kOwn;
   uint4* const q_smem = reinterpret_cast<uint4*>(ring + S::kRing);
-  long long* const ends = reinterpret_cast<long long*>(smem + S::kWarps * S::kOwn);
+  int* const ends = reinterpret_cast<int*>(smem + S::kWarps * S::kOwn);
   pdl_wait();
   pdl_trigger();
 
   // rows of no sequence
   {
     const int head = min(max(p.starts[0], 0), p.rows), tail = min(max(p.starts[p.n], head), p.rows), width = p.q_heads * kDim;
-    for (int row = blockIdx.x; row < head + p.rows - tail; row += gridDim.x)
+    for (int row = blockIdx.x; row < head + p.rows - tail; row += kGrid)
       for (int d = threadIdx.x; d < width; d += S::kThreads) p.out[(int64_t)(row < head ? row : row - head + tail) * width + d] = f_to_bf16(0.f);
   }
   // Up to 32 sequences: every warp has them all in its lanes, and nobody waits for anybody.
   const bool few = p.n <= 32;
-  long long mine_end = 0, line;
+  Kv4Seq mine{};
+  int mine_end = 0, line;
   if (few) {
-    mine_end = warp_scan(lane < p.n ? kv4_line(p, kv4_seq(p, lane, kCols)) : 0, lane);
-    line = __shfl_sync(0xffffffffu, mine_end, 31);
+    if (lane < p.n) mine = kv4_seq(p, lane, kCols);
+    const long long end = warp_scan(lane < p.n ? kv4_line(p, mine) : 0, lane);
+    mine_end = (int)end;
+    line = kv4_whole(__shfl_sync(0xffffffffu, end, 31));
   } else {
-    kv4_plan<S::kThreads>(p, kCols, ends);
-    line = ends[p.n - 1];
+    line = kv4_plan<S::kThreads>(p, kCols, ends);
   }
-  const Cut cut(line, gridDim.x, S::kWarps);
+  const Cut cut(line, S::kWarps);
   const int me = blockIdx.x * cut.each + warp;
   const int64_t own = (int64_t)blockIdx.x * S::kWarps + warp;   // of the workspace's places
-  long long at_line = cut.start(me);
-  const long long stop = warp < cut.each ? cut.start(me + 1) : at_line, cta = cut.start(blockIdx.x * cut.each), cta_end = cut.start((blockIdx.x + 1) * cut.each);
+  int at_line = cut.start(me);
+  const int stop = warp < cut.each ? cut.start(me + 1) : at_line;
   if (lane == 0) p.splits[own].from = -1;
   int i = !few && at_line < stop ? kv4_find(ends, p.n, at_line) : 0;
   while (at_line < stop) {
-    long long base = 0;
+    int base = 0;
+    Kv4Seq s;
     if (few) {
       i = __popc(__ballot_sync(0xffffffffu, mine_end <= at_line));
       if (i > 0) base = __shfl_sync(0xffffffffu, mine_end, i - 1);
+      s = kv4_from(mine, i);
     } else {
       while (ends[i] <= at_line) ++i;
       if (i > 0) base = ends[i - 1];
+      s = kv4_seq(p, i, kCols);
     }
-    const Kv4Seq s = kv4_seq(p, i, kCols);
-    const int length = s.steps + kAhead, item = (int)((at_line - base) / length), head = item % p.cache.kv_heads, block = item / p.cache.kv_heads;
-    const long long begin = base + (long long)item * length + kAhead, end = begin + s.steps;   // of its steps
-    const int first = (int)max(at_line - begin, 0ll), many = (int)(min(stop, end) - begin) - first;
-    // all the CTA's warps have a piece, and of this item alone
-    const bool inside = cut.each > 1 && cta >= begin && cta_end <= end && ((int)blockIdx.x + 1) * cut.each <= cut.warps;
+    const int length = s.steps + kAhead;
+    int item = (int)((float)(at_line - base) * __frcp_rn((float)length));   // (a division costs more than these)
+    while (item * length > at_line - base) --item;
+    while ((item + 1) * length <= at_line - base) ++item;
+    const int block = p.kv_heads.of(item), head = item - block * p.kv_heads.d;
+    const int begin = base + item * length + kAhead, end = begin + s.steps;   // of its steps
+    const int first = max(at_line - begin, 0), many = min(stop, end) - begin - first;
     at_line = min(stop, end);
     if (many <= 0) continue;
 
-    const int col0 = block * kCols, n_cols = s.count * p.group;
+    const int col0 = block * kCols, n_cols = s.count * p.group.d;
+    uint4 raw[NT][NG][2];   // the block's queries
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int col = col0 + t * 8 + r;
+      const int token = p.group.of(col);
+      const __nv_bfloat16* src = p.q + (int64_t)(s.row0 + token) * p.ld_q + (int64_t)(head * p.group.d + col - token * p.group.d) * kDim + 8 * c;
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) raw[t][g][h] = col < n_cols ? *reinterpret_cast<const uint4*>(src + g * 64 + h * 32) : make_uint4(0, 0, 0, 0);
+    }
     int at[NT][2];   // positions of this lane's columns (2c, 2c + 1); −1: no column
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int col = col0 + t * 8 + 2 * c + e;
-        at[t][e] = col < n_cols ? s.pos + col / p.group : -1;
+        at[t][e] = col < n_cols ? s.pos + p.group.of(col) : -1;
       }
-    const int at_low = s.pos + col0 / p.group, at_high = s.pos + (min(col0 + kCols, n_cols) - 1) / p.group;
+    const int at_low = s.pos + p.group.of(col0), at_high = s.pos + p.group.of(min(col0 + kCols, n_cols) - 1);
 
     float o[NG * 4][NT][4] = {}, wsum[NG][NT][4] = {};   // wsum: Σ of the rounded weights, in every row
     float top[NT][2], sum[NT][2] = {}, mid[NG][NT][2] = {};
@@ -237,19 +291,17 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
     next = page_of(S::kStages - 1);
     int slot = 0;
 
-    // the block's queries, as the B operands of K·qᵀ, and their sums over each group
+    // as the B operands of K·qᵀ, and their sums over each group
     uint4 qf[S::kQInRegs ? NT : 1][NG][2];
     float qsum[NG][NT][2];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int col = col0 + t * 8 + r;
-      const __nv_bfloat16* src = p.q + (int64_t)(s.row0 + col / p.group) * p.ld_q + (int64_t)(head * p.group + col % p.group) * kDim + 8 * c;
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint4 u = col < n_cols ? *reinterpret_cast<const uint4*>(src + g * 64 + h * 32) : make_uint4(0, 0, 0, 0);
+          const uint4 u = raw[t][g][h];
           // entries {0, 2}, {1, 3}, {4, 6}, {5, 7}
           const uint4 v = make_uint4(__byte_perm(u.x, u.y, 0x5410), __byte_perm(u.x, u.y, 0x7632), __byte_perm(u.z, u.w, 0x5410), __byte_perm(u.z, u.w, 0x7632));
           if constexpr (S::kQInRegs) qf[t][g][h] = v;
@@ -260,7 +312,6 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
         qsum[g][t][0] = sum[0];
         qsum[g][t][1] = sum[1];
       }
-    }
     for (int u = 0; u < n_steps; ++u) {
       const int ahead = u + S::kStages - 1, into = slot == 0 ? S::kStages - 1 : slot - 1;
       have = (have & ~(1u << (ahead % 32))) | (uint32_t)(next >= 0) << (ahead % 32);
@@ -429,11 +480,16 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
           const int col = col0 + t * 8 + 2 * c + e;
           if (col >= n_cols) continue;
           const float f = sum[t][e] == 0.f ? 0.f : 1.f / sum[t][e];
-          __nv_bfloat16* dst = p.out + ((int64_t)(s.row0 + col / p.group) * p.q_heads + head * p.group + col % p.group) * kDim + 2 * r;
+          const int token = p.group.of(col);
+          __nv_bfloat16* dst = p.out + ((int64_t)(s.row0 + token) * p.q_heads + head * p.group.d + col - token * p.group.d) * kDim + 2 * r;
 #pragma unroll
           for (int d = 0; d < NG * 4; ++d) *reinterpret_cast<uint32_t*>(dst + 16 * d) = pack2(o[d][t][e] * f, o[d][t][e + 2] * f);
         }
     } else {
+      // all the CTA's warps have a piece, and of this item alone
+      const int cta = cut.start(blockIdx.x * cut.each), cta_end = cut.start((blockIdx.x + 1) * cut.each);
+      const bool inside = cut.each > 1 && cta >= begin && cta_end <= end && ((int)blockIdx.x + 1) * cut.each <= cut.warps;
+      const int wide = inside ? kDim + 4 : kDim;   // (shared memory: columns on other banks)
       float* const part = inside ? reinterpret_cast<float*>(ring) : kv4_part(p, own, first == 0, kCols);
 #pragma unroll
       for (int t = 0; t < NT; ++t)
@@ -441,16 +497,16 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
         for (int e = 0; e < 2; ++e) {
           const int col = t * 8 + 2 * c + e;
 #pragma unroll
-          for (int d = 0; d < NG * 4; ++d) *reinterpret_cast<float2*>(part + col * kDim + 16 * d + 2 * r) = make_float2(o[d][t][e], o[d][t][e + 2]);
+          for (int d = 0; d < NG * 4; ++d) *reinterpret_cast<float2*>(part + col * wide + 16 * d + 2 * r) = make_float2(o[d][t][e], o[d][t][e + 2]);
           if (r == 0) {
-            part[kCols * kDim + col] = top[t][e];
-            part[kCols * kDim + kCols + col] = sum[t][e];
+            part[kCols * wide + col] = top[t][e];
+            part[kCols * wide + kCols + col] = sum[t][e];
           }
         }
       if (first == 0 && lane == 0) {
         Kv4Split split;
-        auto warp_at = [&](long long x) {   // whose piece of the line x is
-          int w = (int)(x * cut.warps / cut.line);
+        auto warp_at = [&](int x) {   // whose piece of the line x is
+          int w = min(x / cut.whole, cut.warps - 1);
           while (cut.start(w) > x) --w;
           while (cut.start(w + 1) <= x) ++w;
           return w;
@@ -470,24 +526,34 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
       if (inside) {   // every warp of the CTA that has a piece comes here, once
         named_bar_sync(1, cut.each * 32);
         float* const joined = kv4_part(p, (int64_t)blockIdx.x * S::kWarps, 0, kCols);
-        for (int x = threadIdx.x; x < kCols * kDim; x += cut.each * 32) {
-          const int col = x / kDim;
-          float m = -INFINITY;
-          for (int w = 0; w < cut.each; ++w) m = fmaxf(m, reinterpret_cast<const float*>(smem + w * S::kOwn)[kCols * kDim + col]);
-          float l = 0.f, v = 0.f;
+        for (int col = warp; col < kCols; col += cut.each) {   // a warp takes a column, a lane a warp's maximum and sum
+          const float* of = reinterpret_cast<const float*>(smem + min(lane, cut.each - 1) * S::kOwn) + kCols * (kDim + 4) + col;
+          float l = lane < cut.each ? of[kCols] : 0.f, m = l != 0.f ? of[0] : -INFINITY;   // (a sum that is no number has seen a token)
+          float all = m;
+#pragma unroll
+          for (int x = 1; x < 32; x <<= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, x));
+          const float f = l != 0.f ? exp2_fast(m - all) : 0.f;
+          l *= f;
+#pragma unroll
+          for (int x = 1; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+          float2 v[NG];
+#pragma unroll
+          for (int g = 0; g < NG; ++g) v[g] = make_float2(0.f, 0.f);
 #pragma unroll 4
           for (int w = 0; w < cut.each; ++w) {
-            const float* from = reinterpret_cast<const float*>(smem + w * S::kOwn);
-            const float lw = from[kCols * kDim + kCols + col];
-            if (lw != 0.f) {   // what has seen a token (one that is no number too)
-              const float f = exp2_fast(from[kCols * kDim + col] - m);
-              l = fmaf(f, lw, l);
-              v = fmaf(f, from[x], v);
+            const float fw = __shfl_sync(0xffffffffu, f, w);
+            if (fw == 0.f) continue;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+              const float2 o2 = *reinterpret_cast<const float2*>(smem + w * S::kOwn + (col * (kDim + 4) + g * 64 + 2 * lane) * 4);
+              v[g].x = fmaf(fw, o2.x, v[g].x);
+              v[g].y = fmaf(fw, o2.y, v[g].y);
             }
           }
-          joined[x] = v;
-          if (x % kDim == 0) {
-            joined[kCols * kDim + col] = m;
+#pragma unroll
+          for (int g = 0; g < NG; ++g) *reinterpret_cast<float2*>(joined + col * kDim + g * 64 + 2 * lane) = v[g];
+          if (lane == 0) {
+            joined[kCols * kDim + col] = all;
             joined[kCols * kDim + kCols + col] = l;
           }
         }
@@ -553,7 +619,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn
       for (int e = 0; e < kAtOnce; ++e) o.take(m[e], l[e], x[e]);
     }
     const int at = of(mine.col0, i) + col;
-    __nv_bfloat16* out = p.out + ((int64_t)(of(mine.row0, i) + at / p.group) * p.q_heads + of(mine.head, i) * p.group + at % p.group) * kDim;
+    const int token = p.group.of(at);
+    __nv_bfloat16* out = p.out + ((int64_t)(of(mine.row0, i) + token) * p.q_heads + of(mine.head, i) * p.group.d + at - token * p.group.d) * kDim;
     if (!alone) {
       if (lane == 0) {
         part_m[warp] = o.m;
@@ -631,7 +698,11 @@ int b200_kv4_attention(void* out, const void* q, int64_t ld_q, const b200_kv4_ca
                  cache->kv_heads);
   B200_CHECK_ARG(aligned16(q, workspace, out) && ld_q % 8 == 0 && ld_q >= q_heads * cache->dim, "kv4_attention: q's rows must be 16-byte aligned and apart");
   B200_CHECK_ARG(scale > 0.f && scale < 1e30f && window >= 0, "kv4_attention: scale %g, window %lld", (double)scale, (long long)window);
-  B200_CHECK_ARG(rows * q_heads < 1ll << 31, "kv4_attention: %lld rows of %lld heads", (long long)rows, (long long)q_heads);
+  // the line of all work is counted in 32 bits: 1 M rows of 32 heads over 64 K tokens, or 64 K over 1 M
+  const int64_t group = q_heads / cache->kv_heads, columns = 8 * column_tiles(group, n, rows);
+  const int64_t items = cache->kv_heads * std::min(rows * ((group + columns - 1) / columns), rows * group / columns + n);
+  B200_CHECK_ARG(items * ((int64_t)cache->max_pages * (kPage / kStep) + kAhead) < 1ll << 31 && rows * q_heads < 1ll << 31,
+                 "kv4_attention: %lld rows of %lld heads over %d pages are too many for one call", (long long)rows, (long long)q_heads, cache->max_pages);
   Kv4Attn p{};
   p.cache = *cache;
   p.out = (__nv_bfloat16*)out;
@@ -645,7 +716,8 @@ int b200_kv4_attention(void* out, const void* q, int64_t ld_q, const b200_kv4_ca
   p.splits = (Kv4Split*)(p.parts + (int64_t)kGrid * warps_of(cache->dim / kKvGroup, tiles) * 2 * 8 * tiles * (cache->dim + 2));
   p.layer = (int)layer;
   p.q_heads = (int)q_heads;
-  p.group = (int)(q_heads / cache->kv_heads);
+  p.group = Divisor((uint32_t)(q_heads / cache->kv_heads));
+  p.kv_heads = Divisor((uint32_t)cache->kv_heads);
   p.n = (int)n;
   p.rows = (int)rows;
   p.window = (int)std::min<int64_t>(window, INT32_MAX);
