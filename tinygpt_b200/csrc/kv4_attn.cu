@@ -14,19 +14,21 @@
 #include "kv4.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace b200 {
 
 namespace {
 
 constexpr int kStep = 32, kAhead = 2;
+constexpr float kSlack = 8.f;
 constexpr int kGrid = 148;
 
 // Division by a number that the host knows (Granlund and Montgomery): a multiplication and two shifts
 struct Divisor {
   uint32_t d, m;
   int s1, s2;
-  explicit Divisor(uint32_t d_ = 1) : d(d_) {
+  Divisor(uint32_t d_ = 1) : d(d_) {
     int s = 0;
     while ((1ull << s) < d) ++s;
     m = (uint32_t)((((1ull << s) - d) << 32) / d + 1);
@@ -258,7 +260,7 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
       }
     const int at_low = s.pos + p.group.of(col0), at_high = s.pos + p.group.of(min(col0 + kCols, n_cols) - 1);
 
-    float o[NG * 4][NT][4] = {}, wsum[NG][NT][4] = {};   // wsum: Σ of the rounded weights, in every row
+    float o[NG * 4][NT][4] = {};
     float top[NT][2], sum[NT][2] = {}, mid[NG][NT][2] = {};
 #pragma unroll
     for (int t = 0; t < NT; ++t) top[t][0] = top[t][1] = -INFINITY;
@@ -312,6 +314,89 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
         qsum[g][t][0] = sum[0];
         qsum[g][t][1] = sum[1];
       }
+    // scores of a step, as the products leave them
+    auto scores = [&](const uint8_t* stage, float (&sc)[S::kTiles][NT][4]) {
+#pragma unroll
+      for (int k = 0; k < S::kTiles; ++k) {
+        const uint8_t* tile = stage + k * S::kTile;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const uint4 w = *reinterpret_cast<const uint4*>(tile + g * 512 + lane * 16);
+          const uint2 small = *reinterpret_cast<const uint2*>(tile + NG * 512 + g * 64 + r * 8);
+          const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+          float acc[NT][4] = {};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t a[4];
+            nibbles_128(words[j], a);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              uint4 b;
+              if constexpr (S::kQInRegs) b = qf[t][g][j / 2];
+              else b = q_smem[((t * NG + g) * 2 + j / 2) * 32 + lane];
+              mma16816(acc[t], a[0], a[2], a[1], a[3], j % 2 ? b.z : b.x, j % 2 ? b.w : b.y);
+            }
+          }
+          const float s0 = bf16_lo(small.x), m0 = fmaf(-kNibbleOff, s0, bf16_hi(small.x)), s1 = bf16_lo(small.y), m1 = fmaf(-kNibbleOff, s1, bf16_hi(small.y));
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            sc[k][t][0] = fmaf(s0, acc[t][0], fmaf(m0, qsum[g][t][0], g ? sc[k][t][0] : 0.f));
+            sc[k][t][1] = fmaf(s0, acc[t][1], fmaf(m0, qsum[g][t][1], g ? sc[k][t][1] : 0.f));
+            sc[k][t][2] = fmaf(s1, acc[t][2], fmaf(m1, qsum[g][t][0], g ? sc[k][t][2] : 0.f));
+            sc[k][t][3] = fmaf(s1, acc[t][3], fmaf(m1, qsum[g][t][1], g ? sc[k][t][3] : 0.f));
+          }
+        }
+      }
+    };
+    // weights and values of a step; `whole`: every column sees all of it
+    auto values = [&](const uint8_t* stage, const float (&sc)[S::kTiles][NT][4], auto whole) {
+      float shift[NT][2];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) shift[t][e] = whole || top[t][e] != -INFINITY ? -top[t][e] : 0.f;
+#pragma unroll
+      for (int k = 0; k < S::kTiles; ++k) {
+        const uint8_t* tile = stage + k * S::kTile + NG * (512 + 64);
+        float weight[NT][4];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            weight[t][e] = exp2_fast(fmaf(sc[k][t][e], p.scale_log2, shift[t][e % 2]));
+            sum[t][e % 2] += weight[t][e];
+          }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const uint2 small = *reinterpret_cast<const uint2*>(tile + NG * 512 + g * 64 + r * 8);
+          const float s0 = bf16_lo(small.x), m0 = bf16_hi(small.x), s1 = bf16_lo(small.y), m1 = bf16_hi(small.y);
+          uint32_t b[NT][2];
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            float w[4] = {weight[t][0] * s0, weight[t][1] * s0, weight[t][2] * s1, weight[t][3] * s1};
+            float y[4] = {m0, m0, m1, m1};
+            if constexpr (!whole) {   // what is not seen may hold anything
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (weight[t][e] == 0.f) w[e] = y[e] = 0.f;
+            }
+            mid[g][t][0] = fmaf(weight[t][2], y[2], fmaf(weight[t][0], y[0], mid[g][t][0]));
+            mid[g][t][1] = fmaf(weight[t][3], y[3], fmaf(weight[t][1], y[1], mid[g][t][1]));
+            b[t][0] = transpose8x8(pack2(w[0], w[1]));
+            b[t][1] = transpose8x8(pack2(w[2], w[3]));
+          }
+          const uint4 v = *reinterpret_cast<const uint4*>(tile + g * 512 + lane * 16);
+          const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t a[4];
+            nibbles_bf16(words[j], a);   // exact: what is taken off afterwards would be rounded off the sums over all tokens
+#pragma unroll
+            for (int t = 0; t < NT; ++t) mma16816(o[g * 4 + j][t], a[0], a[1], a[2], a[3], b[t][0], b[t][1]);
+          }
+        }
+      }
+    };
     for (int u = 0; u < n_steps; ++u) {
       const int ahead = u + S::kStages - 1, into = slot == 0 ? S::kStages - 1 : slot - 1;
       have = (have & ~(1u << (ahead % 32))) | (uint32_t)(next >= 0) << (ahead % 32);
@@ -319,133 +404,63 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
       next = page_of(ahead + 1);
       cp_async_wait<S::kStages - 1>();
       __syncwarp();
-      if (have >> (u % 32) & 1) {
-        const uint8_t* stage = ring + slot * S::kStage;
-        const int key0 = (step0 + u) * kStep;
-        const bool whole = key0 + kStep <= min(s.last, at_low + 1) && (p.window == 0 || at_high - key0 < p.window);
-        float sc[S::kTiles][NT][4] = {};
+      const uint8_t* stage = ring + slot * S::kStage;
+      float sc[S::kTiles][NT][4];
+      scores(stage, sc);
+      // a page that is not there counts as not seen, whatever the stage holds
+      const int key0 = (step0 + u) * kStep, last = have >> (u % 32) & 1 ? s.last : 0;
+      const bool whole = key0 + kStep <= min(last, at_low + 1) && (p.window == 0 || at_high - key0 < p.window);
+      if (!whole) {
 #pragma unroll
-        for (int k = 0; k < S::kTiles; ++k) {
-          const uint8_t* tile = stage + k * S::kTile;
-#pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            const uint4 w = *reinterpret_cast<const uint4*>(tile + g * 512 + lane * 16);
-            const uint2 small = *reinterpret_cast<const uint2*>(tile + NG * 512 + g * 64 + r * 8);
-            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-            float acc[NT][4] = {};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              uint32_t a[4];
-              nibbles_128(words[j], a);
-#pragma unroll
-              for (int t = 0; t < NT; ++t) {
-                uint4 b;
-                if constexpr (S::kQInRegs) b = qf[t][g][j / 2];
-                else b = q_smem[((t * NG + g) * 2 + j / 2) * 32 + lane];
-                mma16816(acc[t], a[0], a[2], a[1], a[3], j % 2 ? b.z : b.x, j % 2 ? b.w : b.y);
-              }
-            }
-            const float s0 = bf16_lo(small.x), m0 = fmaf(-kNibbleOff, s0, bf16_hi(small.x)), s1 = bf16_lo(small.y), m1 = fmaf(-kNibbleOff, s1, bf16_hi(small.y));
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              sc[k][t][0] = fmaf(s0, acc[t][0], fmaf(m0, qsum[g][t][0], sc[k][t][0]));
-              sc[k][t][1] = fmaf(s0, acc[t][1], fmaf(m0, qsum[g][t][1], sc[k][t][1]));
-              sc[k][t][2] = fmaf(s1, acc[t][2], fmaf(m1, qsum[g][t][0], sc[k][t][2]));
-              sc[k][t][3] = fmaf(s1, acc[t][3], fmaf(m1, qsum[g][t][1], sc[k][t][3]));
-            }
-          }
-        }
-        if (!whole) {
-#pragma unroll
-          for (int k = 0; k < S::kTiles; ++k)
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int key = key0 + k * kKvTile + r + 8 * (e / 2), from = at[t][e % 2];
-                const bool seen = key <= from && key < s.last && (p.window == 0 || from - key < p.window);
-                if (!seen) sc[k][t][e] = -INFINITY;
-              }
-        }
-        float now[NT][2], shift[NT][2];
-        bool moved = false;
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float m = -INFINITY;
-#pragma unroll
-            for (int k = 0; k < S::kTiles; ++k) m = fmaxf(m, fmaxf(sc[k][t][e], sc[k][t][e + 2]));
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-            m = fmaxf(top[t][e], m * p.scale_log2);
-            now[t][e] = m;
-            shift[t][e] = m == -INFINITY ? 0.f : m;
-            moved |= m != top[t][e];
-          }
-        if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float f = exp2_fast(top[t][e] - shift[t][e]);   // 0 where there was none
-              top[t][e] = now[t][e];
-              sum[t][e] *= f;
-#pragma unroll
-              for (int g = 0; g < NG; ++g) {
-                mid[g][t][e] *= f;
-                wsum[g][t][e] *= f;
-              }
-#pragma unroll
-              for (int d = 0; d < NG * 4; ++d) {
-                o[d][t][e] *= f;
-                o[d][t][e + 2] *= f;
-              }
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < S::kTiles; ++k) {
-          const uint8_t* tile = stage + k * S::kTile + NG * (512 + 64);
+        for (int k = 0; k < S::kTiles; ++k)
 #pragma unroll
           for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float v = exp2_fast(fmaf(sc[k][t][e], p.scale_log2, -shift[t][e % 2]));
-              sum[t][e % 2] += v;
-              sc[k][t][e] = v;
+              const int key = key0 + k * kKvTile + r + 8 * (e / 2), from = at[t][e % 2];
+              const bool seen = key <= from && key < last && (p.window == 0 || from - key < p.window);
+              if (!seen) sc[k][t][e] = -INFINITY;
             }
+      }
+      float m[NT][2];
 #pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            const uint2 small = *reinterpret_cast<const uint2*>(tile + NG * 512 + g * 64 + r * 8);
-            const float s0 = bf16_lo(small.x), m0 = bf16_hi(small.x), s1 = bf16_lo(small.y), m1 = bf16_hi(small.y);
-            uint32_t b[NT][2];
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              float w[4] = {sc[k][t][0] * s0, sc[k][t][1] * s0, sc[k][t][2] * s1, sc[k][t][3] * s1};
-              float y[4] = {m0, m0, m1, m1};
-              if (!whole) {   // what is not seen may hold anything
+        for (int e = 0; e < 2; ++e) {
+          m[t][e] = -INFINITY;
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (sc[k][t][e] == 0.f) w[e] = y[e] = 0.f;
-              }
-              mid[g][t][0] = fmaf(sc[k][t][2], y[2], fmaf(sc[k][t][0], y[0], mid[g][t][0]));
-              mid[g][t][1] = fmaf(sc[k][t][3], y[3], fmaf(sc[k][t][1], y[1], mid[g][t][1]));
-              b[t][0] = transpose8x8(pack2(w[0], w[1]));
-              b[t][1] = transpose8x8(pack2(w[2], w[3]));
-              mma16816(wsum[g][t], kBf16Ones, kBf16Ones, kBf16Ones, kBf16Ones, b[t][0], b[t][1]);
-            }
-            const uint4 v = *reinterpret_cast<const uint4*>(tile + g * 512 + lane * 16);
-            const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+          for (int k = 0; k < S::kTiles; ++k) m[t][e] = fmaxf(m[t][e], fmaxf(sc[k][t][e], sc[k][t][e + 2]));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              uint32_t a[4];
-              nibbles_128(words[j], a);
+          for (int x = 4; x < 32; x <<= 1) m[t][e] = fmaxf(m[t][e], __shfl_xor_sync(0xffffffffu, m[t][e], x));
+        }
+      // The running maximum moves only where it would be passed by more than 2^8: up to there weights and sums are as exact with the old one
+      bool moved = false;
 #pragma unroll
-              for (int t = 0; t < NT; ++t) mma16816(o[g * 4 + j][t], a[0], a[1], a[2], a[3], b[t][0], b[t][1]);
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          m[t][e] *= p.scale_log2;
+          moved |= m[t][e] > top[t][e] + kSlack;
+        }
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float now = fmaxf(top[t][e], m[t][e]), f = now == -INFINITY ? 1.f : exp2_fast(top[t][e] - now);   // 0 where there was none
+            top[t][e] = now;
+            sum[t][e] *= f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) mid[g][t][e] *= f;
+#pragma unroll
+            for (int d = 0; d < NG * 4; ++d) {
+              o[d][t][e] *= f;
+              o[d][t][e + 2] *= f;
             }
           }
-        }
       }
+      if (whole) values(stage, sc, std::true_type());
+      else values(stage, sc, std::false_type());
       __syncwarp();   // the stage is free
       slot = slot + 1 == S::kStages ? 0 : slot + 1;
     }
@@ -464,7 +479,6 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
           float y = mid[g][t][e];
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) y += __shfl_xor_sync(0xffffffffu, y, x);
-          y = fmaf(-kNibbleOff, wsum[g][t][e], y);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             o[g * 4 + j][t][e] += y;
