@@ -146,7 +146,7 @@ def test_rows_without_a_place(built_lib):
 
 # ------------------------------------------------------------------------------------------------- attention
 @pytest.mark.gpu
-@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 64), (14, 2, 64), (4, 2, 128), (16, 2, 128), (9, 1, 128), (6, 2, 192), (8, 4, 256), (20, 2, 256)])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 64), (14, 2, 64), (4, 2, 128), (16, 2, 128), (9, 1, 128), (6, 2, 192), (10, 1, 192), (8, 4, 256), (20, 2, 256)])
 def test_single_tokens(built_lib, heads, kv_heads, dim):
     lengths = [1, 15, 16, 17, 0, 63, 64, 65, 130, 511, 700]
     run_case(Rand(3), lengths, [1 if l else 1 for l in lengths], heads, kv_heads, dim)

@@ -14,7 +14,6 @@
 #include "kv4.cuh"
 
 #include <algorithm>
-#include <type_traits>
 
 namespace b200 {
 
@@ -162,6 +161,326 @@ struct Kv4Split {
   int row0, col0, n_cols, head, each;   // from < 0: none
 };
 
+// What a warp keeps of its 8·NT columns while it goes over the tokens: lane 4r + c has columns 2c, 2c + 1 of every tile.
+template <int NG, int NT>
+struct Columns {
+  static constexpr int kDim = NG * 64, kTiles = kStep / kKvTile;
+  float o[NG * 4][NT][4], mid[NG][NT][2], top[NT][2], sum[NT][2], qsum[NG][NT][2];
+  int at[NT][2];          // positions; −1: no column
+  int at_low, at_high;    // of the block
+
+  __device__ __forceinline__ void start(const Kv4Attn& p, const Kv4Seq& s, int col0, int n_cols, int c) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int col = col0 + t * 8 + 2 * c + e;
+        at[t][e] = col < n_cols ? s.pos + p.group.of(col) : -1;
+        top[t][e] = -INFINITY;
+        sum[t][e] = 0.f;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) mid[g][t][e] = 0.f;
+#pragma unroll
+        for (int d = 0; d < NG * 4; ++d) o[d][t][e] = o[d][t][e + 2] = 0.f;
+      }
+    at_low = s.pos + p.group.of(col0);
+    at_high = s.pos + p.group.of(min(col0 + 8 * NT, n_cols) - 1);
+  }
+  // q's rows of the columns → the B operands of K·qᵀ (entries {0, 2}, {1, 3}, {4, 6}, {5, 7} of eight) and their sums over each group
+  __device__ __forceinline__ void take(int g, int t, uint4 (&q)[2]) {
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint4 u = q[h];
+      q[h] = make_uint4(__byte_perm(u.x, u.y, 0x5410), __byte_perm(u.x, u.y, 0x7632), __byte_perm(u.z, u.w, 0x5410), __byte_perm(u.z, u.w, 0x7632));
+      mma16816(s, kBf16Ones, kBf16Ones, kBf16Ones, kBf16Ones, q[h].x, q[h].y);
+      mma16816(s, kBf16Ones, kBf16Ones, kBf16Ones, kBf16Ones, q[h].z, q[h].w);
+    }
+    qsum[g][t][0] = s[0];
+    qsum[g][t][1] = s[1];
+  }
+  // scores of a step, as the products leave them: `words` gives the A operands of a tile and group, `small` its scales and middles, `query` the B operands
+  template <typename Words, typename Small, typename Query>
+  __device__ __forceinline__ void scores(float (&sc)[kTiles][NT][4], const Words& words, const Small& small, const Query& query) const {
+#pragma unroll
+    for (int k = 0; k < kTiles; ++k)
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const auto w = words(k, g);
+        const uint2 two = small(k, g);
+        float acc[NT][4] = {};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t a[4];
+          w.keys(j, a);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            const uint4 b = query(t, g, j / 2);
+            mma16816(acc[t], a[0], a[2], a[1], a[3], j % 2 ? b.z : b.x, j % 2 ? b.w : b.y);
+          }
+        }
+        const float s0 = bf16_lo(two.x), m0 = fmaf(-w.kOff, s0, bf16_hi(two.x)), s1 = bf16_lo(two.y), m1 = fmaf(-w.kOff, s1, bf16_hi(two.y));
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          sc[k][t][0] = fmaf(s0, acc[t][0], fmaf(m0, qsum[g][t][0], g ? sc[k][t][0] : 0.f));
+          sc[k][t][1] = fmaf(s0, acc[t][1], fmaf(m0, qsum[g][t][1], g ? sc[k][t][1] : 0.f));
+          sc[k][t][2] = fmaf(s1, acc[t][2], fmaf(m1, qsum[g][t][0], g ? sc[k][t][2] : 0.f));
+          sc[k][t][3] = fmaf(s1, acc[t][3], fmaf(m1, qsum[g][t][1], g ? sc[k][t][3] : 0.f));
+        }
+      }
+  }
+  // whether every column sees all tokens of the step at key0; where not, the scores of the others are −∞
+  __device__ __forceinline__ bool mask(float (&sc)[kTiles][NT][4], int key0, int last, int window, int r) const {
+    const bool whole = key0 + kStep <= min(last, at_low + 1) && (window == 0 || at_high - key0 < window);
+    if (!whole) {
+#pragma unroll
+      for (int k = 0; k < kTiles; ++k)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = key0 + k * kKvTile + r + 8 * (e / 2), from = at[t][e % 2];
+            const bool seen = key <= from && key < last && (window == 0 || from - key < window);
+            if (!seen) sc[k][t][e] = -INFINITY;
+          }
+    }
+    return whole;
+  }
+  // The running maximum moves only where it would be passed by more than 2^8: up to there weights and sums are as exact with the old one.
+  __device__ __forceinline__ void settle(const float (&sc)[kTiles][NT][4], float scale_log2) {
+    float m[NT][2];
+    bool moved = false;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[t][e] = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < kTiles; ++k) m[t][e] = fmaxf(m[t][e], fmaxf(sc[k][t][e], sc[k][t][e + 2]));
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) m[t][e] = fmaxf(m[t][e], __shfl_xor_sync(0xffffffffu, m[t][e], x));
+        m[t][e] *= scale_log2;
+        moved |= m[t][e] > top[t][e] + kSlack;
+      }
+    if (!__any_sync(0xffffffffu, moved)) return;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float now = fmaxf(top[t][e], m[t][e]), f = now == -INFINITY ? 1.f : exp2_fast(top[t][e] - now);   // 0 where there was none
+        top[t][e] = now;
+        sum[t][e] *= f;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) mid[g][t][e] *= f;
+#pragma unroll
+        for (int d = 0; d < NG * 4; ++d) {
+          o[d][t][e] *= f;
+          o[d][t][e + 2] *= f;
+        }
+      }
+  }
+  // weights and values of a step
+  template <bool WHOLE, typename Words, typename Small>
+  __device__ __forceinline__ void values(const float (&sc)[kTiles][NT][4], float scale_log2, const Words& words, const Small& small) {
+    float shift[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) shift[t][e] = WHOLE || top[t][e] != -INFINITY ? -top[t][e] : 0.f;
+#pragma unroll
+    for (int k = 0; k < kTiles; ++k) {
+      float weight[NT][4];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          weight[t][e] = exp2_fast(fmaf(sc[k][t][e], scale_log2, shift[t][e % 2]));
+          sum[t][e % 2] += weight[t][e];
+        }
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const uint2 two = small(k, g);
+        const float s0 = bf16_lo(two.x), m0 = bf16_hi(two.x), s1 = bf16_lo(two.y), m1 = bf16_hi(two.y);
+        uint32_t b[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          float w[4] = {weight[t][0] * s0, weight[t][1] * s0, weight[t][2] * s1, weight[t][3] * s1};
+          float y[4] = {m0, m0, m1, m1};
+          if constexpr (!WHOLE) {   // what is not seen may hold anything
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (weight[t][e] == 0.f) w[e] = y[e] = 0.f;
+          }
+          mid[g][t][0] = fmaf(weight[t][2], y[2], fmaf(weight[t][0], y[0], mid[g][t][0]));
+          mid[g][t][1] = fmaf(weight[t][3], y[3], fmaf(weight[t][1], y[1], mid[g][t][1]));
+          b[t][0] = transpose8x8(pack2(w[0], w[1]));
+          b[t][1] = transpose8x8(pack2(w[2], w[3]));
+        }
+        const auto v = words(k, g);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t a[4];
+          v.values(j, a);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma16816(o[g * 4 + j][t], a[0], a[1], a[2], a[3], b[t][0], b[t][1]);
+        }
+      }
+    }
+  }
+  // Σ over the tokens is whole then, but for what the lanes of a column have kept apart
+  __device__ __forceinline__ void finish() {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) sum[t][e] += __shfl_xor_sync(0xffffffffu, sum[t][e], x);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          float y = mid[g][t][e];
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) y += __shfl_xor_sync(0xffffffffu, y, x);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            o[g * 4 + j][t][e] += y;
+            o[g * 4 + j][t][e + 2] += y;
+          }
+        }
+      }
+  }
+  __device__ __forceinline__ void write(const Kv4Attn& p, const Kv4Seq& s, int head, int col0, int n_cols, int r, int c) const {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int col = col0 + t * 8 + 2 * c + e;
+        if (col >= n_cols) continue;
+        const float f = sum[t][e] == 0.f ? 0.f : 1.f / sum[t][e];
+        const int token = p.group.of(col);
+        __nv_bfloat16* dst = p.out + ((int64_t)(s.row0 + token) * p.q_heads + head * p.group.d + col - token * p.group.d) * kDim + 2 * r;
+#pragma unroll
+        for (int d = 0; d < NG * 4; ++d) *reinterpret_cast<uint32_t*>(dst + 16 * d) = pack2(o[d][t][e] * f, o[d][t][e + 2] * f);
+      }
+  }
+  // as a part: columns first … of `columns`, `wide` floats from one to the next, behind them all maxima and all sums
+  __device__ __forceinline__ void leave(float* part, int first, int columns, int wide, int r, int c) const {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int col = first + t * 8 + 2 * c + e;
+#pragma unroll
+        for (int d = 0; d < NG * 4; ++d) *reinterpret_cast<float2*>(part + col * wide + 16 * d + 2 * r) = make_float2(o[d][t][e], o[d][t][e + 2]);
+        if (r == 0) {
+          part[columns * wide + col] = top[t][e];
+          part[columns * wide + columns + col] = sum[t][e];
+        }
+      }
+  }
+};
+// the query that column `col` of the block belongs to, eight entries from 8c on
+template <int NG>
+__device__ __forceinline__ const __nv_bfloat16* kv4_query(const Kv4Attn& p, const Kv4Seq& s, int head, int col, int c) {
+  const int token = p.group.of(col);
+  return p.q + (int64_t)(s.row0 + token) * p.ld_q + (int64_t)(head * p.group.d + col - token * p.group.d) * (NG * 64) + 8 * c;
+}
+// A operands from a tile's nibbles
+struct Nibbles {
+  static constexpr float kOff = kNibbleOff;
+  uint4 w;
+  __device__ __forceinline__ uint32_t word(int j) const { return j == 0 ? w.x : j == 1 ? w.y : j == 2 ? w.z : w.w; }
+  __device__ __forceinline__ void keys(int j, uint32_t (&a)[4]) const { nibbles_128(word(j), a); }
+  __device__ __forceinline__ void values(int j, uint32_t (&a)[4]) const { nibbles_bf16(word(j), a); }   // exact: 136 taken off later would be rounded off the sums over all tokens
+};
+// the same, unpacked in shared memory
+struct Unpacked {
+  static constexpr float kOff = 0.f;
+  const uint4* of;   // this lane's, of word 0
+  __device__ __forceinline__ void keys(int j, uint32_t (&a)[4]) const {
+    const uint4 v = of[j * 32];
+    a[0] = v.x;
+    a[1] = v.y;
+    a[2] = v.z;
+    a[3] = v.w;
+  }
+  __device__ __forceinline__ void values(int j, uint32_t (&a)[4]) const { keys(j, a); }
+};
+
+// A CTA's or a warp's way along the line: the sequences' ends, and one item after the other.
+struct Walk {
+  Kv4Seq mine;      // up to 32 sequences: every warp has them all in its lanes, and nobody waits for anybody
+  int mine_end, line, i;
+  const int* ends;  // more: in shared memory
+  bool few;
+  template <int THREADS>
+  __device__ __forceinline__ void plan(const Kv4Attn& p, int columns, int* room) {
+    const int lane = threadIdx.x % 32;
+    few = p.n <= 32;
+    ends = room;
+    mine = Kv4Seq{};
+    mine_end = 0;
+    if (few) {
+      if (lane < p.n) mine = kv4_seq(p, lane, columns);
+      const long long end = warp_scan(lane < p.n ? kv4_line(p, mine) : 0, lane);
+      mine_end = (int)end;
+      line = kv4_whole(__shfl_sync(0xffffffffu, end, 31));
+    } else {
+      line = kv4_plan<THREADS>(p, columns, room);
+    }
+  }
+  __device__ __forceinline__ void seek(int n, int at, int stop) { i = !few && at < stop ? kv4_find(ends, n, at) : 0; }
+  // the item at this place of the line: its sequence, key/value head, block of columns; its steps lie at begin … end − 1
+  Kv4Seq s;
+  int head, block, begin, end;
+  __device__ __forceinline__ void item(const Kv4Attn& p, int columns, int at) {
+    int base = 0;
+    if (few) {
+      i = __popc(__ballot_sync(0xffffffffu, mine_end <= at));
+      if (i > 0) base = __shfl_sync(0xffffffffu, mine_end, i - 1);
+      s = kv4_from(mine, i);
+    } else {
+      while (ends[i] <= at) ++i;
+      if (i > 0) base = ends[i - 1];
+      s = kv4_seq(p, i, columns);
+    }
+    const int length = s.steps + kAhead;
+    int number = (int)((float)(at - base) * __frcp_rn((float)length));   // (a division costs more than these)
+    while (number * length > at - base) --number;
+    while ((number + 1) * length <= at - base) ++number;
+    block = p.kv_heads.of(number);
+    head = number - block * p.kv_heads.d;
+    begin = base + number * length + kAhead;
+    end = begin + s.steps;
+  }
+};
+__device__ __forceinline__ void kv4_split(const Kv4Attn& p, const Walk& w, const Cut& cut, int64_t own, int me, int col0, int n_cols) {
+  auto warp_at = [&](int x) {   // whose piece of the line x is
+    int v = min(x / cut.whole, cut.warps - 1);
+    while (cut.start(v) > x) --v;
+    while (cut.start(v + 1) <= x) ++v;
+    return v;
+  };
+  Kv4Split split;
+  split.from = me;
+  split.to = warp_at(w.end - 1);
+  split.in0 = cut.start(blockIdx.x * cut.each) == w.begin ? blockIdx.x : blockIdx.x + 1;
+  split.in1 = cut.start(split.to + 1) == w.end && (split.to + 1) % cut.each == 0 ? (split.to + 1) / cut.each : split.to / cut.each;
+  if (cut.each == 1) split.in1 = split.in0;
+  split.row0 = w.s.row0;
+  split.col0 = col0;
+  split.n_cols = n_cols;
+  split.head = w.head;
+  split.each = cut.each;
+  p.splits[own] = split;
+}
+// rows of no sequence are zero
+__device__ __forceinline__ void kv4_others(const Kv4Attn& p) {
+  const int head = min(max(p.starts[0], 0), p.rows), tail = min(max(p.starts[p.n], head), p.rows), width = p.q_heads * p.cache.dim;
+  for (int row = blockIdx.x; row < head + p.rows - tail; row += kGrid)
+    for (int d = threadIdx.x; d < width; d += blockDim.x) p.out[(int64_t)(row < head ? row : row - head + tail) * width + d] = f_to_bf16(0.f);
+}
+
+// ---- few columns to a sequence: every warp for itself
 template <int NG, int NT>
 struct Shape {
   static constexpr int kTile = kv4_tile_bytes(NG);
@@ -187,85 +506,42 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
   uint8_t* const ring = smem + warp * S::kOwn;
   uint4* const q_smem = reinterpret_cast<uint4*>(ring + S::kRing);
-  int* const ends = reinterpret_cast<int*>(smem + S::kWarps * S::kOwn);
   pdl_wait();
   pdl_trigger();
 
-  // rows of no sequence
-  {
-    const int head = min(max(p.starts[0], 0), p.rows), tail = min(max(p.starts[p.n], head), p.rows), width = p.q_heads * kDim;
-    for (int row = blockIdx.x; row < head + p.rows - tail; row += kGrid)
-      for (int d = threadIdx.x; d < width; d += S::kThreads) p.out[(int64_t)(row < head ? row : row - head + tail) * width + d] = f_to_bf16(0.f);
-  }
-  // Up to 32 sequences: every warp has them all in its lanes, and nobody waits for anybody.
-  const bool few = p.n <= 32;
-  Kv4Seq mine{};
-  int mine_end = 0, line;
-  if (few) {
-    if (lane < p.n) mine = kv4_seq(p, lane, kCols);
-    const long long end = warp_scan(lane < p.n ? kv4_line(p, mine) : 0, lane);
-    mine_end = (int)end;
-    line = kv4_whole(__shfl_sync(0xffffffffu, end, 31));
-  } else {
-    line = kv4_plan<S::kThreads>(p, kCols, ends);
-  }
-  const Cut cut(line, S::kWarps);
+  kv4_others(p);
+  Walk w{};
+  w.plan<S::kThreads>(p, kCols, reinterpret_cast<int*>(smem + S::kWarps * S::kOwn));
+  const Cut cut(w.line, S::kWarps);
   const int me = blockIdx.x * cut.each + warp;
   const int64_t own = (int64_t)blockIdx.x * S::kWarps + warp;   // of the workspace's places
   int at_line = cut.start(me);
   const int stop = warp < cut.each ? cut.start(me + 1) : at_line;
   if (lane == 0) p.splits[own].from = -1;
-  int i = !few && at_line < stop ? kv4_find(ends, p.n, at_line) : 0;
+  w.seek(p.n, at_line, stop);
   while (at_line < stop) {
-    int base = 0;
-    Kv4Seq s;
-    if (few) {
-      i = __popc(__ballot_sync(0xffffffffu, mine_end <= at_line));
-      if (i > 0) base = __shfl_sync(0xffffffffu, mine_end, i - 1);
-      s = kv4_from(mine, i);
-    } else {
-      while (ends[i] <= at_line) ++i;
-      if (i > 0) base = ends[i - 1];
-      s = kv4_seq(p, i, kCols);
-    }
-    const int length = s.steps + kAhead;
-    int item = (int)((float)(at_line - base) * __frcp_rn((float)length));   // (a division costs more than these)
-    while (item * length > at_line - base) --item;
-    while ((item + 1) * length <= at_line - base) ++item;
-    const int block = p.kv_heads.of(item), head = item - block * p.kv_heads.d;
-    const int begin = base + item * length + kAhead, end = begin + s.steps;   // of its steps
-    const int first = max(at_line - begin, 0), many = min(stop, end) - begin - first;
-    at_line = min(stop, end);
+    w.item(p, kCols, at_line);
+    const Kv4Seq& s = w.s;
+    const int first = max(at_line - w.begin, 0), many = min(stop, w.end) - w.begin - first;
+    at_line = min(stop, w.end);
     if (many <= 0) continue;
 
-    const int col0 = block * kCols, n_cols = s.count * p.group.d;
-    uint4 raw[NT][NG][2];   // the block's queries
+    const int col0 = w.block * kCols, n_cols = s.count * p.group.d;
+    uint4 q[NT][NG][2];   // the block's queries
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int col = col0 + t * 8 + r;
-      const int token = p.group.of(col);
-      const __nv_bfloat16* src = p.q + (int64_t)(s.row0 + token) * p.ld_q + (int64_t)(head * p.group.d + col - token * p.group.d) * kDim + 8 * c;
+      const __nv_bfloat16* src = kv4_query<NG>(p, s, w.head, col, c);
 #pragma unroll
       for (int g = 0; g < NG; ++g)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) raw[t][g][h] = col < n_cols ? *reinterpret_cast<const uint4*>(src + g * 64 + h * 32) : make_uint4(0, 0, 0, 0);
+        for (int h = 0; h < 2; ++h) q[t][g][h] = col < n_cols ? *reinterpret_cast<const uint4*>(src + g * 64 + h * 32) : make_uint4(0, 0, 0, 0);
     }
-    int at[NT][2];   // positions of this lane's columns (2c, 2c + 1); −1: no column
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int col = col0 + t * 8 + 2 * c + e;
-        at[t][e] = col < n_cols ? s.pos + p.group.of(col) : -1;
-      }
-    const int at_low = s.pos + p.group.of(col0), at_high = s.pos + p.group.of(min(col0 + kCols, n_cols) - 1);
+    Columns<NG, NT> cols;
+    cols.start(p, s, col0, n_cols, c);
 
-    float o[NG * 4][NT][4] = {};
-    float top[NT][2], sum[NT][2] = {}, mid[NG][NT][2] = {};
-#pragma unroll
-    for (int t = 0; t < NT; ++t) top[t][0] = top[t][1] = -INFINITY;
-
-    const int step0 = s.step0 + first, n_steps = s.last > 0 ? many : 0;
+    // (steps that no column sees, in a block whose columns stand far apart from the sequence's others, are not gone over)
+    const int step0 = s.step0 + first, n_steps = s.last > 0 ? min(many, cols.at_high / kStep + 1 - step0) : 0;
     const int32_t* table = p.cache.table + (int64_t)max(s.slot, 0) * p.cache.max_pages;
     auto page_of = [&](int u) {
       if (u >= n_steps) return -1;
@@ -274,7 +550,7 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
     };
     auto fetch = [&](int u, int page, int slot) {
       if (page >= 0) {
-        const uint8_t* src = kv4_head(p.cache, p.layer, page, head) + (step0 + u) % (kPage / kStep) * S::kStage + lane * 16;
+        const uint8_t* src = kv4_head(p.cache, p.layer, page, w.head) + (step0 + u) % (kPage / kStep) * S::kStage + lane * 16;
         uint8_t* dst = ring + slot * S::kStage + lane * 16;
 #pragma unroll
         for (int b = 0; b < S::kStage; b += 512)
@@ -292,111 +568,16 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
     }
     next = page_of(S::kStages - 1);
     int slot = 0;
-
-    // as the B operands of K·qᵀ, and their sums over each group
-    uint4 qf[S::kQInRegs ? NT : 1][NG][2];
-    float qsum[NG][NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint4 u = raw[t][g][h];
-          // entries {0, 2}, {1, 3}, {4, 6}, {5, 7}
-          const uint4 v = make_uint4(__byte_perm(u.x, u.y, 0x5410), __byte_perm(u.x, u.y, 0x7632), __byte_perm(u.z, u.w, 0x5410), __byte_perm(u.z, u.w, 0x7632));
-          if constexpr (S::kQInRegs) qf[t][g][h] = v;
-          else q_smem[((t * NG + g) * 2 + h) * 32 + lane] = v;
-          mma16816(sum, kBf16Ones, kBf16Ones, kBf16Ones, kBf16Ones, v.x, v.y);
-          mma16816(sum, kBf16Ones, kBf16Ones, kBf16Ones, kBf16Ones, v.z, v.w);
-        }
-        qsum[g][t][0] = sum[0];
-        qsum[g][t][1] = sum[1];
-      }
-    // scores of a step, as the products leave them
-    auto scores = [&](const uint8_t* stage, float (&sc)[S::kTiles][NT][4]) {
-#pragma unroll
-      for (int k = 0; k < S::kTiles; ++k) {
-        const uint8_t* tile = stage + k * S::kTile;
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          const uint4 w = *reinterpret_cast<const uint4*>(tile + g * 512 + lane * 16);
-          const uint2 small = *reinterpret_cast<const uint2*>(tile + NG * 512 + g * 64 + r * 8);
-          const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-          float acc[NT][4] = {};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t a[4];
-            nibbles_128(words[j], a);
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              uint4 b;
-              if constexpr (S::kQInRegs) b = qf[t][g][j / 2];
-              else b = q_smem[((t * NG + g) * 2 + j / 2) * 32 + lane];
-              mma16816(acc[t], a[0], a[2], a[1], a[3], j % 2 ? b.z : b.x, j % 2 ? b.w : b.y);
-            }
-          }
-          const float s0 = bf16_lo(small.x), m0 = fmaf(-kNibbleOff, s0, bf16_hi(small.x)), s1 = bf16_lo(small.y), m1 = fmaf(-kNibbleOff, s1, bf16_hi(small.y));
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            sc[k][t][0] = fmaf(s0, acc[t][0], fmaf(m0, qsum[g][t][0], g ? sc[k][t][0] : 0.f));
-            sc[k][t][1] = fmaf(s0, acc[t][1], fmaf(m0, qsum[g][t][1], g ? sc[k][t][1] : 0.f));
-            sc[k][t][2] = fmaf(s1, acc[t][2], fmaf(m1, qsum[g][t][0], g ? sc[k][t][2] : 0.f));
-            sc[k][t][3] = fmaf(s1, acc[t][3], fmaf(m1, qsum[g][t][1], g ? sc[k][t][3] : 0.f));
-          }
+        cols.take(g, t, q[t][g]);
+        if constexpr (!S::kQInRegs) {
+          q_smem[((t * NG + g) * 2) * 32 + lane] = q[t][g][0];
+          q_smem[((t * NG + g) * 2 + 1) * 32 + lane] = q[t][g][1];
         }
       }
-    };
-    // weights and values of a step; `whole`: every column sees all of it
-    auto values = [&](const uint8_t* stage, const float (&sc)[S::kTiles][NT][4], auto whole) {
-      float shift[NT][2];
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) shift[t][e] = whole || top[t][e] != -INFINITY ? -top[t][e] : 0.f;
-#pragma unroll
-      for (int k = 0; k < S::kTiles; ++k) {
-        const uint8_t* tile = stage + k * S::kTile + NG * (512 + 64);
-        float weight[NT][4];
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            weight[t][e] = exp2_fast(fmaf(sc[k][t][e], p.scale_log2, shift[t][e % 2]));
-            sum[t][e % 2] += weight[t][e];
-          }
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          const uint2 small = *reinterpret_cast<const uint2*>(tile + NG * 512 + g * 64 + r * 8);
-          const float s0 = bf16_lo(small.x), m0 = bf16_hi(small.x), s1 = bf16_lo(small.y), m1 = bf16_hi(small.y);
-          uint32_t b[NT][2];
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            float w[4] = {weight[t][0] * s0, weight[t][1] * s0, weight[t][2] * s1, weight[t][3] * s1};
-            float y[4] = {m0, m0, m1, m1};
-            if constexpr (!whole) {   // what is not seen may hold anything
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (weight[t][e] == 0.f) w[e] = y[e] = 0.f;
-            }
-            mid[g][t][0] = fmaf(weight[t][2], y[2], fmaf(weight[t][0], y[0], mid[g][t][0]));
-            mid[g][t][1] = fmaf(weight[t][3], y[3], fmaf(weight[t][1], y[1], mid[g][t][1]));
-            b[t][0] = transpose8x8(pack2(w[0], w[1]));
-            b[t][1] = transpose8x8(pack2(w[2], w[3]));
-          }
-          const uint4 v = *reinterpret_cast<const uint4*>(tile + g * 512 + lane * 16);
-          const uint32_t words[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t a[4];
-            nibbles_bf16(words[j], a);   // exact: what is taken off afterwards would be rounded off the sums over all tokens
-#pragma unroll
-            for (int t = 0; t < NT; ++t) mma16816(o[g * 4 + j][t], a[0], a[1], a[2], a[3], b[t][0], b[t][1]);
-          }
-        }
-      }
-    };
     for (int u = 0; u < n_steps; ++u) {
       const int ahead = u + S::kStages - 1, into = slot == 0 ? S::kStages - 1 : slot - 1;
       have = (have & ~(1u << (ahead % 32))) | (uint32_t)(next >= 0) << (ahead % 32);
@@ -405,180 +586,219 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
       cp_async_wait<S::kStages - 1>();
       __syncwarp();
       const uint8_t* stage = ring + slot * S::kStage;
+      auto keys = [&](int k, int g) { return Nibbles{*reinterpret_cast<const uint4*>(stage + k * S::kTile + g * 512 + lane * 16)}; };
+      auto key_small = [&](int k, int g) { return *reinterpret_cast<const uint2*>(stage + k * S::kTile + NG * 512 + g * 64 + r * 8); };
+      auto values = [&](int k, int g) { return Nibbles{*reinterpret_cast<const uint4*>(stage + k * S::kTile + NG * (512 + 64) + g * 512 + lane * 16)}; };
+      auto value_small = [&](int k, int g) { return *reinterpret_cast<const uint2*>(stage + k * S::kTile + NG * (512 + 64 + 512) + g * 64 + r * 8); };
+      auto query = [&](int t, int g, int h) {
+        if constexpr (S::kQInRegs) return q[t][g][h];
+        else return q_smem[((t * NG + g) * 2 + h) * 32 + lane];
+      };
       float sc[S::kTiles][NT][4];
-      scores(stage, sc);
+      cols.scores(sc, keys, key_small, query);
       // a page that is not there counts as not seen, whatever the stage holds
-      const int key0 = (step0 + u) * kStep, last = have >> (u % 32) & 1 ? s.last : 0;
-      const bool whole = key0 + kStep <= min(last, at_low + 1) && (p.window == 0 || at_high - key0 < p.window);
-      if (!whole) {
-#pragma unroll
-        for (int k = 0; k < S::kTiles; ++k)
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int key = key0 + k * kKvTile + r + 8 * (e / 2), from = at[t][e % 2];
-              const bool seen = key <= from && key < last && (p.window == 0 || from - key < p.window);
-              if (!seen) sc[k][t][e] = -INFINITY;
-            }
-      }
-      float m[NT][2];
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          m[t][e] = -INFINITY;
-#pragma unroll
-          for (int k = 0; k < S::kTiles; ++k) m[t][e] = fmaxf(m[t][e], fmaxf(sc[k][t][e], sc[k][t][e + 2]));
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) m[t][e] = fmaxf(m[t][e], __shfl_xor_sync(0xffffffffu, m[t][e], x));
-        }
-      // The running maximum moves only where it would be passed by more than 2^8: up to there weights and sums are as exact with the old one
-      bool moved = false;
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          m[t][e] *= p.scale_log2;
-          moved |= m[t][e] > top[t][e] + kSlack;
-        }
-      if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float now = fmaxf(top[t][e], m[t][e]), f = now == -INFINITY ? 1.f : exp2_fast(top[t][e] - now);   // 0 where there was none
-            top[t][e] = now;
-            sum[t][e] *= f;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) mid[g][t][e] *= f;
-#pragma unroll
-            for (int d = 0; d < NG * 4; ++d) {
-              o[d][t][e] *= f;
-              o[d][t][e + 2] *= f;
-            }
-          }
-      }
-      if (whole) values(stage, sc, std::true_type());
-      else values(stage, sc, std::false_type());
+      const bool whole = cols.mask(sc, (step0 + u) * kStep, have >> (u % 32) & 1 ? s.last : 0, p.window, r);
+      cols.settle(sc, p.scale_log2);
+      if (whole) cols.template values<true>(sc, p.scale_log2, values, value_small);
+      else cols.template values<false>(sc, p.scale_log2, values, value_small);
       __syncwarp();   // the stage is free
       slot = slot + 1 == S::kStages ? 0 : slot + 1;
     }
     cp_async_wait<0>();
     __syncwarp();
-
-    // Σ over the tokens is whole but for what the lanes of a column keep apart
+    cols.finish();
+    if (many == s.steps) {
+      cols.write(p, s, w.head, col0, n_cols, r, c);
+      continue;
+    }
+    if (first == 0 && lane == 0) kv4_split(p, w, cut, own, me, col0, n_cols);
+    // all the CTA's warps have a piece, and of this item alone
+    const int cta = cut.start(blockIdx.x * cut.each), cta_end = cut.start((blockIdx.x + 1) * cut.each);
+    if (cut.each == 1 || cta < w.begin || cta_end > w.end || ((int)blockIdx.x + 1) * cut.each > cut.warps) {
+      cols.leave(kv4_part(p, own, first == 0, kCols), 0, kCols, kDim, r, c);
+      continue;
+    }
+    constexpr int kWide = kDim + 4;   // (columns on other banks)
+    cols.leave(reinterpret_cast<float*>(ring), 0, kCols, kWide, r, c);
+    named_bar_sync(1, cut.each * 32);   // every warp of the CTA that has a piece comes here, once
+    float* const joined = kv4_part(p, (int64_t)blockIdx.x * S::kWarps, 0, kCols);
+    for (int col = warp; col < kCols; col += cut.each) {   // a warp takes a column, a lane a warp's maximum and sum
+      const float* of = reinterpret_cast<const float*>(smem + min(lane, cut.each - 1) * S::kOwn) + kCols * kWide + col;
+      float l = lane < cut.each ? of[kCols] : 0.f, m = l != 0.f ? of[0] : -INFINITY;   // (a sum that is no number has seen a token)
+      float all = m;
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+      for (int x = 1; x < 32; x <<= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, x));
+      const float f = l != 0.f ? exp2_fast(m - all) : 0.f;
+      l *= f;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
+      for (int x = 1; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+      float2 v[NG];
 #pragma unroll
-        for (int x = 4; x < 32; x <<= 1) sum[t][e] += __shfl_xor_sync(0xffffffffu, sum[t][e], x);
+      for (int g = 0; g < NG; ++g) v[g] = make_float2(0.f, 0.f);
+#pragma unroll 4
+      for (int k = 0; k < cut.each; ++k) {
+        const float fk = __shfl_sync(0xffffffffu, f, k);
+        if (fk == 0.f) continue;
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-          float y = mid[g][t][e];
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) y += __shfl_xor_sync(0xffffffffu, y, x);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            o[g * 4 + j][t][e] += y;
-            o[g * 4 + j][t][e + 2] += y;
-          }
+          const float2 o2 = *reinterpret_cast<const float2*>(smem + k * S::kOwn + (col * kWide + g * 64 + 2 * lane) * 4);
+          v[g].x = fmaf(fk, o2.x, v[g].x);
+          v[g].y = fmaf(fk, o2.y, v[g].y);
         }
       }
-    if (many == s.steps) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int col = col0 + t * 8 + 2 * c + e;
-          if (col >= n_cols) continue;
-          const float f = sum[t][e] == 0.f ? 0.f : 1.f / sum[t][e];
-          const int token = p.group.of(col);
-          __nv_bfloat16* dst = p.out + ((int64_t)(s.row0 + token) * p.q_heads + head * p.group.d + col - token * p.group.d) * kDim + 2 * r;
-#pragma unroll
-          for (int d = 0; d < NG * 4; ++d) *reinterpret_cast<uint32_t*>(dst + 16 * d) = pack2(o[d][t][e] * f, o[d][t][e + 2] * f);
-        }
-    } else {
-      // all the CTA's warps have a piece, and of this item alone
-      const int cta = cut.start(blockIdx.x * cut.each), cta_end = cut.start((blockIdx.x + 1) * cut.each);
-      const bool inside = cut.each > 1 && cta >= begin && cta_end <= end && ((int)blockIdx.x + 1) * cut.each <= cut.warps;
-      const int wide = inside ? kDim + 4 : kDim;   // (shared memory: columns on other banks)
-      float* const part = inside ? reinterpret_cast<float*>(ring) : kv4_part(p, own, first == 0, kCols);
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int col = t * 8 + 2 * c + e;
-#pragma unroll
-          for (int d = 0; d < NG * 4; ++d) *reinterpret_cast<float2*>(part + col * wide + 16 * d + 2 * r) = make_float2(o[d][t][e], o[d][t][e + 2]);
-          if (r == 0) {
-            part[kCols * wide + col] = top[t][e];
-            part[kCols * wide + kCols + col] = sum[t][e];
-          }
-        }
-      if (first == 0 && lane == 0) {
-        Kv4Split split;
-        auto warp_at = [&](int x) {   // whose piece of the line x is
-          int w = min(x / cut.whole, cut.warps - 1);
-          while (cut.start(w) > x) --w;
-          while (cut.start(w + 1) <= x) ++w;
-          return w;
-        };
-        split.from = me;
-        split.to = warp_at(end - 1);
-        split.in0 = cta == begin ? blockIdx.x : blockIdx.x + 1;
-        split.in1 = cut.start(split.to + 1) == end && (split.to + 1) % cut.each == 0 ? (split.to + 1) / cut.each : split.to / cut.each;
-        if (cut.each == 1) split.in1 = split.in0;
-        split.row0 = s.row0;
-        split.col0 = col0;
-        split.n_cols = n_cols;
-        split.head = head;
-        split.each = cut.each;
-        p.splits[own] = split;
-      }
-      if (inside) {   // every warp of the CTA that has a piece comes here, once
-        named_bar_sync(1, cut.each * 32);
-        float* const joined = kv4_part(p, (int64_t)blockIdx.x * S::kWarps, 0, kCols);
-        for (int col = warp; col < kCols; col += cut.each) {   // a warp takes a column, a lane a warp's maximum and sum
-          const float* of = reinterpret_cast<const float*>(smem + min(lane, cut.each - 1) * S::kOwn) + kCols * (kDim + 4) + col;
-          float l = lane < cut.each ? of[kCols] : 0.f, m = l != 0.f ? of[0] : -INFINITY;   // (a sum that is no number has seen a token)
-          float all = m;
-#pragma unroll
-          for (int x = 1; x < 32; x <<= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, x));
-          const float f = l != 0.f ? exp2_fast(m - all) : 0.f;
-          l *= f;
-#pragma unroll
-          for (int x = 1; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-          float2 v[NG];
-#pragma unroll
-          for (int g = 0; g < NG; ++g) v[g] = make_float2(0.f, 0.f);
-#pragma unroll 4
-          for (int w = 0; w < cut.each; ++w) {
-            const float fw = __shfl_sync(0xffffffffu, f, w);
-            if (fw == 0.f) continue;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-              const float2 o2 = *reinterpret_cast<const float2*>(smem + w * S::kOwn + (col * (kDim + 4) + g * 64 + 2 * lane) * 4);
-              v[g].x = fmaf(fw, o2.x, v[g].x);
-              v[g].y = fmaf(fw, o2.y, v[g].y);
-            }
-          }
-#pragma unroll
-          for (int g = 0; g < NG; ++g) *reinterpret_cast<float2*>(joined + col * kDim + g * 64 + 2 * lane) = v[g];
-          if (lane == 0) {
-            joined[kCols * kDim + col] = all;
-            joined[kCols * kDim + kCols + col] = l;
-          }
-        }
+      for (int g = 0; g < NG; ++g) *reinterpret_cast<float2*>(joined + col * kDim + g * 64 + 2 * lane) = v[g];
+      if (lane == 0) {
+        joined[kCols * kDim + col] = all;
+        joined[kCols * kDim + kCols + col] = l;
       }
     }
   }
 }
 
-// The items that lie in more than one warp's piece of the line.  CTA (c, column) takes those that begin in CTA c's pieces: a warp each while their parts are few,
-// else all warps, every eighth part in order, and then the warps meet.
-constexpr int kJoinWarps = 8;
+// ---- many columns to a sequence: a CTA takes 8·NT of them to a warp, all warps unpack a step's tokens once for all
+template <int NG>
+struct Prompt {
+  static constexpr int kTile = kv4_tile_bytes(NG);
+  static constexpr int kTiles = kStep / kKvTile;
+  static constexpr int kStage = kTiles * kTile;
+  static constexpr int kStages = 4;
+  static constexpr int kNT = NG <= 2 ? 2 : 1;
+  static constexpr int kWarps = 8;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kCols = kWarps * 8 * kNT;
+  static constexpr int kUnpacked = kTiles * 2 * NG * 4 * 512;   // of a step
+  static constexpr bool kQInRegs = NG * kNT <= 4;
+  static constexpr int kSmem = kStages * kStage + 2 * kUnpacked + kKvMaxSeqs * 4;
+};
+template <int NG>
+__global__ void __launch_bounds__(Prompt<NG>::kThreads, 1) kv4_prompt_kernel(const Kv4Attn p) {
+  using S = Prompt<NG>;
+  constexpr int NT = S::kNT, kDim = NG * 64;
+  static_assert(S::kQInRegs, "queries in registers");
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
+  uint8_t* const ring = smem;
+  uint4* const unpacked = reinterpret_cast<uint4*>(smem + S::kStages * S::kStage);
+  pdl_wait();
+  pdl_trigger();
+
+  kv4_others(p);
+  Walk w{};
+  w.plan<S::kThreads>(p, S::kCols, reinterpret_cast<int*>(smem + S::kStages * S::kStage + 2 * S::kUnpacked));
+  const Cut cut(w.line, 1);
+  int at_line = cut.start(blockIdx.x);
+  const int stop = cut.start(blockIdx.x + 1);
+  if (threadIdx.x == 0) p.splits[blockIdx.x].from = -1;
+  w.seek(p.n, at_line, stop);
+  while (at_line < stop) {
+    w.item(p, S::kCols, at_line);
+    const Kv4Seq& s = w.s;
+    const int first = max(at_line - w.begin, 0), many = min(stop, w.end) - w.begin - first;
+    at_line = min(stop, w.end);
+    if (many <= 0) continue;
+
+    const int block0 = w.block * S::kCols, col0 = block0 + warp * 8 * NT, n_cols = s.count * p.group.d;
+    uint4 q[NT][NG][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int col = col0 + t * 8 + r;
+      const __nv_bfloat16* src = kv4_query<NG>(p, s, w.head, col, c);
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) q[t][g][h] = col < n_cols ? *reinterpret_cast<const uint4*>(src + g * 64 + h * 32) : make_uint4(0, 0, 0, 0);
+    }
+    Columns<NG, NT> cols;
+    cols.start(p, s, col0, n_cols, c);
+    const bool some = col0 < n_cols;
+
+    // steps that a column of the block sees
+    const int step0 = s.step0 + first, high = s.pos + p.group.of(min(block0 + S::kCols, n_cols) - 1), low = s.pos + p.group.of(block0);
+    const int begin = p.window > 0 && low >= p.window ? max((low - p.window + 1) / kStep - step0, 0) : 0;
+    const int end = s.last > 0 ? min(many, high / kStep + 1 - step0) : 0;
+    const int32_t* table = p.cache.table + (int64_t)max(s.slot, 0) * p.cache.max_pages;
+    auto page_of = [&](int u) {
+      if (u >= end) return -1;
+      const int page = table[(step0 + u) / (kPage / kStep)];
+      return page < p.cache.n_pages ? page : -1;
+    };
+    auto fetch = [&](int u, int page) {
+      if (page >= 0) {
+        const uint8_t* src = kv4_head(p.cache, p.layer, page, w.head) + (step0 + u) % (kPage / kStep) * S::kStage;
+        uint8_t* dst = ring + u % S::kStages * S::kStage;
+        for (int b = threadIdx.x * 16; b < S::kStage; b += S::kThreads * 16) cp_async16(dst + b, src + b);
+      }
+      cp_async_commit();
+    };
+    // a warp unpacks whole groups of a tile's keys or values: the operands in the order in which a product takes them
+    auto unpack = [&](int u) {
+      const uint8_t* stage = ring + u % S::kStages * S::kStage;
+      uint4* to = unpacked + u % 2 * (S::kUnpacked / 16);
+      for (int e = warp; e < S::kTiles * 2 * NG; e += S::kWarps) {   // (tile, keys | values, group)
+        const int k = e / (2 * NG), v = e / NG % 2, g = e % NG;
+        const Nibbles n{*reinterpret_cast<const uint4*>(stage + k * S::kTile + v * NG * (512 + 64) + g * 512 + lane * 16)};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t a[4];
+          n.values(j, a);
+          to[(e * 4 + j) * 32 + lane] = make_uint4(a[0], a[1], a[2], a[3]);
+        }
+      }
+    };
+    uint32_t have = 0;   // bit u % 32: step u has a page
+    for (int u = begin; u < begin + S::kStages - 2; ++u) {
+      const int page = page_of(u);
+      have |= (uint32_t)(page >= 0) << (u % 32);
+      fetch(u, page);
+    }
+    int next = page_of(begin + S::kStages - 2);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int g = 0; g < NG; ++g) cols.take(g, t, q[t][g]);
+    // Step u is unpacked one turn of the loop before its products, so that one barrier a turn does: behind it step u's raw bytes are there, the products of
+    // u − 2 are done and the operands of u − 1 lie ready.
+    for (int u = begin; u <= end; ++u) {
+      const int ahead = u + S::kStages - 2;
+      have = (have & ~(1u << (ahead % 32))) | (uint32_t)(next >= 0) << (ahead % 32);
+      cp_async_wait<S::kStages - 3>();
+      __syncthreads();
+      fetch(ahead, next);
+      next = page_of(ahead + 1);
+      if (u < end) unpack(u);
+      if (u == begin || !some) continue;
+      const int v = u - 1, key0 = (step0 + v) * kStep;
+      if (key0 > cols.at_high || (p.window > 0 && cols.at_low - key0 >= p.window + kStep - 1)) continue;   // nothing that this warp's columns see
+      const uint8_t* stage = ring + v % S::kStages * S::kStage;
+      const uint4* from = unpacked + v % 2 * (S::kUnpacked / 16) + lane;
+      auto keys = [&](int k, int g) { return Unpacked{from + (k * 2 * NG + g) * 4 * 32}; };
+      auto key_small = [&](int k, int g) { return *reinterpret_cast<const uint2*>(stage + k * S::kTile + NG * 512 + g * 64 + r * 8); };
+      auto values = [&](int k, int g) { return Unpacked{from + (k * 2 * NG + NG + g) * 4 * 32}; };
+      auto value_small = [&](int k, int g) { return *reinterpret_cast<const uint2*>(stage + k * S::kTile + NG * (512 + 64 + 512) + g * 64 + r * 8); };
+      auto query = [&](int t, int g, int h) { return q[t][g][h]; };
+      float sc[S::kTiles][NT][4];
+      cols.scores(sc, keys, key_small, query);
+      const bool whole = cols.mask(sc, key0, have >> (v % 32) & 1 ? s.last : 0, p.window, r);
+      cols.settle(sc, p.scale_log2);
+      if (whole) cols.template values<true>(sc, p.scale_log2, values, value_small);
+      else cols.template values<false>(sc, p.scale_log2, values, value_small);
+    }
+    cp_async_wait<0>();
+    __syncthreads();   // the ring and the operands are free
+    cols.finish();
+    if (many == s.steps) {
+      cols.write(p, s, w.head, col0, n_cols, r, c);
+    } else {
+      if (first == 0 && threadIdx.x == 0) kv4_split(p, w, cut, blockIdx.x, blockIdx.x, block0, n_cols);
+      if (some) cols.leave(kv4_part(p, blockIdx.x, first == 0, S::kCols), warp * 8 * NT, S::kCols, kDim, r, c);
+    }
+  }
+}
+
+// The items that lie in more than one piece of the line.  CTA (c, y) joins parts of those that begin in CTA c's pieces: a column to a warp while an item's parts are
+// few, else a column to the CTA, its warps every eighth part in order, and then the warps meet.
+constexpr int kJoinWarps = 8, kJoinRows = 16;
 template <int NG>
 struct Joined {
   float m = -INFINITY, l = 0.f;
@@ -601,20 +821,24 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn
   __shared__ float part_m[kJoinWarps], part_l[kJoinWarps];
   __shared__ float2 part_v[kJoinWarps][NG * 32];
   constexpr int kDim = NG * 64, kAtOnce = 4;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, col = blockIdx.y;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, turns = gridDim.y * kJoinWarps;
   pdl_wait();
   pdl_trigger();
   const Kv4Split* splits = p.splits + blockIdx.x * warps;
   const Kv4Split mine = lane < warps ? splits[lane] : Kv4Split{-1};
   auto of = [&](int v, int from) { return __shfl_sync(0xffffffffu, v, from); };
-  int number = 0;
-  for (uint32_t left = __ballot_sync(0xffffffffu, mine.from >= 0 && mine.col0 + col < mine.n_cols); left != 0; left &= left - 1) {
+  int number = 0;   // of items that are joined a column to a warp
+  for (uint32_t left = __ballot_sync(0xffffffffu, mine.from >= 0); left != 0; left &= left - 1) {
     const int i = __ffs(left) - 1, from = of(mine.from, i), to = of(mine.to, i), in0 = of(mine.in0, i), in1 = of(mine.in1, i), each = of(mine.each, i);
+    const int many = min(of(mine.n_cols, i) - of(mine.col0, i), columns);
     const bool some = in0 < in1;
     const int before = some ? in0 * each - from : to - from + 1, whole = some ? in1 - in0 : 0, parts = before + whole + (some ? to - in1 * each + 1 : 0);
     const bool alone = parts <= 2 * kAtOnce;
-    if (alone && number++ % kJoinWarps != warp) continue;
     const int first = alone ? 0 : warp, step = alone ? 1 : kJoinWarps;
+    // columns are dealt out in turn, over the items that a warp joins alone
+    const int start = alone ? (blockIdx.y * kJoinWarps + warp + turns - number * columns % turns) % turns : blockIdx.y;
+    if (alone) ++number;
+    for (int col = start; col < many; col += alone ? turns : gridDim.y) {
     Joined<NG> o;
     for (int k0 = first; k0 < parts; k0 += kAtOnce * step) {
       float m[kAtOnce], l[kAtOnce];
@@ -659,34 +883,37 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn
 #pragma unroll
       for (int g = 0; g < NG; ++g) *reinterpret_cast<uint32_t*>(out + g * 64 + 2 * lane) = pack2(o.v[g].x * f, o.v[g].y * f);
     }
+    }
   }
 }
 
-// Column tiles of a block: what an average sequence brings.
-int column_tiles(int64_t group, int64_t n, int64_t rows) { return group * ((rows + n - 1) / n) <= 8 ? 1 : 2; }
+// How a call's rows are taken: by the columns that an average sequence brings.  Up to 8: a tile of columns to a warp; up to 32: two; more: a CTA for 128 (64 of heads
+// of 192 and 256), which unpacks for all of them (257 rows of 16 / 8 heads of 128 under a window of 1 024: KVPROMPT µs, two tiles to a warp 36.7).
+struct Way {
+  int tiles, columns, warps;   // tiles of a warp (0: the CTA's way), columns of a block, pieces of the line to a CTA
+};
+Way kv4_way(int64_t group, int64_t n, int64_t rows, int groups) {
+  const int64_t columns = group * ((rows + n - 1) / n);
+  if (columns > 32) return {0, groups <= 2 ? 128 : 64, 1};
+  return columns > 8 ? Way{2, 16, 8} : Way{1, 8, 8};
+}
 
-template <int NG, int NT>
-int launch(const Kv4Attn& p, cudaStream_t st) {
-  using S = Shape<NG, NT>;
-  static PerDevice attrs;
-  B200_CUDA(attrs([] { return cudaFuncSetAttribute(kv4_attn_kernel<NG, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem); }));
+template <typename Shape>
+int launch(const Kv4Attn& p, void (*kernel)(Kv4Attn), void (*join)(Kv4Attn, int, int), const Way& way, PerDevice& attrs, cudaStream_t st) {
+  B200_CUDA(attrs([kernel] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem); }));
   const bool pdl = op_pdl(st);
-  B200_CUDA(launch_pdl(kv4_attn_kernel<NG, NT>, dim3(kGrid), dim3(S::kThreads), S::kSmem, st, pdl, p));
-  B200_CUDA(launch_pdl(kv4_join_kernel<NG>, dim3(kGrid, 8 * NT), dim3(kJoinWarps * 32), 0, st, pdl, p, 8 * NT, S::kWarps));
+  B200_CUDA(launch_pdl(kernel, dim3(kGrid), dim3(Shape::kThreads), Shape::kSmem, st, pdl, p));
+  B200_CUDA(launch_pdl(join, dim3(kGrid, std::min(way.columns, kJoinRows)), dim3(kJoinWarps * 32), 0, st, pdl, p, way.columns, way.warps));
   return B200_OK;
 }
-int warps_of(int groups, int tiles) {
-  switch (groups * 2 + tiles - 3) {
-    case 0: return Shape<1, 1>::kWarps;
-    case 1: return Shape<1, 2>::kWarps;
-    case 2: return Shape<2, 1>::kWarps;
-    case 3: return Shape<2, 2>::kWarps;
-    case 4: return Shape<3, 1>::kWarps;
-    case 5: return Shape<3, 2>::kWarps;
-    case 6: return Shape<4, 1>::kWarps;
-    default: return Shape<4, 2>::kWarps;
-  }
+template <int NG>
+int launch_groups(const Kv4Attn& p, const Way& way, cudaStream_t st) {
+  static PerDevice one, two, many;
+  if (way.tiles == 1) return launch<Shape<NG, 1>>(p, kv4_attn_kernel<NG, 1>, kv4_join_kernel<NG>, way, one, st);
+  if (way.tiles == 2) return launch<Shape<NG, 2>>(p, kv4_attn_kernel<NG, 2>, kv4_join_kernel<NG>, way, two, st);
+  return launch<Prompt<NG>>(p, kv4_prompt_kernel<NG>, kv4_join_kernel<NG>, way, many, st);
 }
+int64_t part_floats(const Way& way, int dim) { return (int64_t)kGrid * way.warps * 2 * way.columns * (dim + 2); }
 
 }  // namespace
 
@@ -698,8 +925,8 @@ int64_t b200_kv4_attention_workspace_bytes(const b200_kv4_cache* cache, int64_t 
   using namespace b200;
   if (cache == nullptr || cache->kv_heads < 1 || q_heads < 1 || q_heads % cache->kv_heads != 0 || n < 1 || rows < 1) return -1;
   if (cache->dim % kKvGroup != 0 || cache->dim < 64 || cache->dim > 256) return -1;
-  const int tiles = column_tiles(q_heads / cache->kv_heads, n, rows);
-  return (int64_t)kGrid * warps_of(cache->dim / kKvGroup, tiles) * (2 * 8 * tiles * (cache->dim + 2) * 4 + (int64_t)sizeof(Kv4Split));
+  const Way way = kv4_way(q_heads / cache->kv_heads, n, rows, cache->dim / kKvGroup);
+  return part_floats(way, cache->dim) * 4 + (int64_t)kGrid * way.warps * sizeof(Kv4Split);
 }
 
 int b200_kv4_attention(void* out, const void* q, int64_t ld_q, const b200_kv4_cache* cache, int64_t layer, int64_t q_heads, const int32_t* seqs,
@@ -713,7 +940,9 @@ int b200_kv4_attention(void* out, const void* q, int64_t ld_q, const b200_kv4_ca
   B200_CHECK_ARG(aligned16(q, workspace, out) && ld_q % 8 == 0 && ld_q >= q_heads * cache->dim, "kv4_attention: q's rows must be 16-byte aligned and apart");
   B200_CHECK_ARG(scale > 0.f && scale < 1e30f && window >= 0, "kv4_attention: scale %g, window %lld", (double)scale, (long long)window);
   // the line of all work is counted in 32 bits: 1 M rows of 32 heads over 64 K tokens, or 64 K over 1 M
-  const int64_t group = q_heads / cache->kv_heads, columns = 8 * column_tiles(group, n, rows);
+  const int64_t group = q_heads / cache->kv_heads;
+  const Way way = kv4_way(group, n, rows, cache->dim / kKvGroup);
+  const int64_t columns = way.columns;
   const int64_t items = cache->kv_heads * std::min(rows * ((group + columns - 1) / columns), rows * group / columns + n);
   B200_CHECK_ARG(items * ((int64_t)cache->max_pages * (kPage / kStep) + kAhead) < 1ll << 31 && rows * q_heads < 1ll << 31,
                  "kv4_attention: %lld rows of %lld heads over %d pages are too many for one call", (long long)rows, (long long)q_heads, cache->max_pages);
@@ -726,8 +955,7 @@ int b200_kv4_attention(void* out, const void* q, int64_t ld_q, const b200_kv4_ca
   p.starts = starts;
   p.pos = pos;
   p.parts = (float*)workspace;
-  const int tiles = column_tiles(q_heads / cache->kv_heads, n, rows);
-  p.splits = (Kv4Split*)(p.parts + (int64_t)kGrid * warps_of(cache->dim / kKvGroup, tiles) * 2 * 8 * tiles * (cache->dim + 2));
+  p.splits = (Kv4Split*)(p.parts + part_floats(way, cache->dim));
   p.layer = (int)layer;
   p.q_heads = (int)q_heads;
   p.group = Divisor((uint32_t)(q_heads / cache->kv_heads));
@@ -737,12 +965,11 @@ int b200_kv4_attention(void* out, const void* q, int64_t ld_q, const b200_kv4_ca
   p.window = (int)std::min<int64_t>(window, INT32_MAX);
   p.scale_log2 = scale * 1.44269504f;
   const cudaStream_t st = (cudaStream_t)stream;
-  const bool two = tiles == 2;
   switch (cache->dim / kKvGroup) {
-    case 1: return two ? launch<1, 2>(p, st) : launch<1, 1>(p, st);
-    case 2: return two ? launch<2, 2>(p, st) : launch<2, 1>(p, st);
-    case 3: return two ? launch<3, 2>(p, st) : launch<3, 1>(p, st);
-    default: return two ? launch<4, 2>(p, st) : launch<4, 1>(p, st);
+    case 1: return launch_groups<1>(p, way, st);
+    case 2: return launch_groups<2>(p, way, st);
+    case 3: return launch_groups<3>(p, way, st);
+    default: return launch_groups<4>(p, way, st);
   }
 }
 
