@@ -481,12 +481,14 @@ __device__ __forceinline__ void kv4_others(const Kv4Attn& p) {
 }
 
 // ---- few columns to a sequence: every warp for itself
+// (the workspace is sized by this)
+constexpr int kPieceWarps = 8;
 template <int NG, int NT>
 struct Shape {
   static constexpr int kTile = kv4_tile_bytes(NG);
   static constexpr int kTiles = kStep / kKvTile;                // of a step
   static constexpr int kStage = kTiles * kTile;
-  static constexpr int kWarps = 8;
+  static constexpr int kWarps = kPieceWarps, kPieces = kWarps, kCols = 8 * NT;   // pieces of the line to a CTA, columns of a block
   static constexpr int kThreads = kWarps * 32;
   static constexpr bool kQInRegs = NG * NT <= 4;
   static constexpr int kQBytes = kQInRegs ? 0 : NT * NG * 2 * 512;
@@ -509,7 +511,6 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
   pdl_wait();
   pdl_trigger();
 
-  kv4_others(p);
   Walk w{};
   w.plan<S::kThreads>(p, kCols, reinterpret_cast<int*>(smem + S::kWarps * S::kOwn));
   const Cut cut(w.line, S::kWarps);
@@ -654,6 +655,7 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
       }
     }
   }
+  kv4_others(p);
 }
 
 // ---- many columns to a sequence: a CTA takes 8·NT of them to a warp, all warps unpack a step's tokens once for all
@@ -664,7 +666,7 @@ struct Prompt {
   static constexpr int kStage = kTiles * kTile;
   static constexpr int kStages = 4;
   static constexpr int kNT = NG <= 2 ? 2 : 1;
-  static constexpr int kWarps = 8;
+  static constexpr int kWarps = 8, kPieces = 1;
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kCols = kWarps * 8 * kNT;
   static constexpr int kUnpacked = kTiles * 2 * NG * 4 * 512;   // of a step
@@ -683,7 +685,6 @@ __global__ void __launch_bounds__(Prompt<NG>::kThreads, 1) kv4_prompt_kernel(con
   pdl_wait();
   pdl_trigger();
 
-  kv4_others(p);
   Walk w{};
   w.plan<S::kThreads>(p, S::kCols, reinterpret_cast<int*>(smem + S::kStages * S::kStage + 2 * S::kUnpacked));
   const Cut cut(w.line, 1);
@@ -794,6 +795,7 @@ __global__ void __launch_bounds__(Prompt<NG>::kThreads, 1) kv4_prompt_kernel(con
       if (some) cols.leave(kv4_part(p, blockIdx.x, first == 0, S::kCols), warp * 8 * NT, S::kCols, kDim, r, c);
     }
   }
+  kv4_others(p);
 }
 
 // The items that lie in more than one piece of the line.  CTA (c, y) joins parts of those that begin in CTA c's pieces: a column to a warp while an item's parts are
@@ -895,23 +897,24 @@ struct Way {
 Way kv4_way(int64_t group, int64_t n, int64_t rows, int groups) {
   const int64_t columns = group * ((rows + n - 1) / n);
   if (columns > 32) return {0, groups <= 2 ? 128 : 64, 1};
-  return columns > 8 ? Way{2, 16, 8} : Way{1, 8, 8};
+  return columns > 8 ? Way{2, 16, kPieceWarps} : Way{1, 8, kPieceWarps};
 }
 
-template <typename Shape>
-int launch(const Kv4Attn& p, void (*kernel)(Kv4Attn), void (*join)(Kv4Attn, int, int), const Way& way, PerDevice& attrs, cudaStream_t st) {
-  B200_CUDA(attrs([kernel] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem); }));
+template <typename Shape, void (*kKernel)(Kv4Attn), void (*kJoin)(Kv4Attn, int, int)>
+int launch(const Kv4Attn& p, const Way& way, cudaStream_t st) {
+  B200_CHECK_ARG(way.warps == Shape::kPieces && way.columns == Shape::kCols, "kv4_attention: the workspace is not this kernel's");
+  static PerDevice attrs;
+  B200_CUDA(attrs([] { return cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem); }));
   const bool pdl = op_pdl(st);
-  B200_CUDA(launch_pdl(kernel, dim3(kGrid), dim3(Shape::kThreads), Shape::kSmem, st, pdl, p));
-  B200_CUDA(launch_pdl(join, dim3(kGrid, std::min(way.columns, kJoinRows)), dim3(kJoinWarps * 32), 0, st, pdl, p, way.columns, way.warps));
+  B200_CUDA(launch_pdl(kKernel, dim3(kGrid), dim3(Shape::kThreads), Shape::kSmem, st, pdl, p));
+  B200_CUDA(launch_pdl(kJoin, dim3(kGrid, std::min(way.columns, kJoinRows)), dim3(kJoinWarps * 32), 0, st, pdl, p, way.columns, way.warps));
   return B200_OK;
 }
 template <int NG>
 int launch_groups(const Kv4Attn& p, const Way& way, cudaStream_t st) {
-  static PerDevice one, two, many;
-  if (way.tiles == 1) return launch<Shape<NG, 1>>(p, kv4_attn_kernel<NG, 1>, kv4_join_kernel<NG>, way, one, st);
-  if (way.tiles == 2) return launch<Shape<NG, 2>>(p, kv4_attn_kernel<NG, 2>, kv4_join_kernel<NG>, way, two, st);
-  return launch<Prompt<NG>>(p, kv4_prompt_kernel<NG>, kv4_join_kernel<NG>, way, many, st);
+  if (way.tiles == 1) return launch<Shape<NG, 1>, kv4_attn_kernel<NG, 1>, kv4_join_kernel<NG>>(p, way, st);
+  if (way.tiles == 2) return launch<Shape<NG, 2>, kv4_attn_kernel<NG, 2>, kv4_join_kernel<NG>>(p, way, st);
+  return launch<Prompt<NG>, kv4_prompt_kernel<NG>, kv4_join_kernel<NG>>(p, way, st);
 }
 int64_t part_floats(const Way& way, int dim) { return (int64_t)kGrid * way.warps * 2 * way.columns * (dim + 2); }
 
