@@ -202,16 +202,17 @@ __global__ void __launch_bounds__(256) w4_dequant_kernel(__nv_bfloat16* out, con
     const uint32_t s = __ldg(p.scale + at), z = p.zero != nullptr ? __ldg(p.zero + at) : 0x41004100u;   // 8, 8
 #pragma unroll
     for (int hi = 0; hi < 2; ++hi) {
-      const float sc = hi ? bf16_hi(s) : bf16_lo(s), off = 8.f - (hi ? bf16_hi(z) : bf16_lo(z));
+      // scale·value − scale·zero: the second product has 16 bits, so that one rounding is left to fp32
+      const float sc = hi ? bf16_hi(s) : bf16_lo(s), off = -sc * (hi ? bf16_hi(z) : bf16_lo(z));
       uint32_t o[4];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         uint32_t a[4];
-        nibbles_bf16(words[2 * h + t], a);
+        nibbles_128(words[2 * h + t], a);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const uint32_t v = a[2 * e + hi];
-          o[2 * t + e] = pack2((bf16_lo(v) + off) * sc, (bf16_hi(v) + off) * sc);
+          o[2 * t + e] = pack2(fmaf(sc, bf16_lo(v) - 128.f, off), fmaf(sc, bf16_hi(v) - 128.f, off));
         }
       }
       const int64_t n = tile * 16 + r + 8 * hi;
