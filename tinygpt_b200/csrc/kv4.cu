@@ -141,11 +141,11 @@ __global__ void __launch_bounds__(kStoreWarps * 32, 4) kv4_store_kernel(const b2
       }
     }
     const int page = kv4_page(cache, to.slot, to.at);
-    if (page < 0 || cache.refs[page] != 1) continue;
-    uint8_t* tile = kv4_head(cache, layer, page, head) + to.at % kPage / kKvTile * kv4_tile_bytes(groups) + job.values * groups * (512 + 64);
+    const int owners = page >= 0 ? cache.refs[page] : 0;   // (asked for here, looked at when there is something to store)
+    uint8_t* tile = kv4_head(cache, layer, max(page, 0), head) + to.at % kPage / kKvTile * kv4_tile_bytes(groups) + job.values * groups * (512 + 64);
     uint32_t* small = reinterpret_cast<uint32_t*>(tile + groups * 512) + g * 16;
     uint8_t* mine = tile + g * 512 + lane * 16;
-    uint32_t half[8];   // the lane's four words, 16 bits each
+    uint32_t half[8], both[4];   // the lane's four words, 16 bits each; its tokens' scales and middles
     if (job.values == 0) {
 #pragma unroll
       for (int hi = 0; hi < 2; ++hi) {
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kStoreWarps * 32, 4) kv4_store_kernel(const b2
           const uint32_t byte = q[2 * e] + 16 * q[2 * e + 1];
           half[e] = hi == 0 ? byte : half[e] + 256 * byte;
         }
-        if (here(r + 8 * hi) && c == 0) small[r * 2 + hi] = sc.both;
+        both[hi] = sc.both;
       }
     } else {
 #pragma unroll
@@ -175,7 +175,19 @@ __global__ void __launch_bounds__(kStoreWarps * 32, 4) kv4_store_kernel(const b2
           const uint32_t byte = q[2 * j] + 16 * q[2 * j + 1];
           half[2 * j + e] = p == 0 ? byte : half[2 * j + e] + 256 * byte;
         }
-        if (here(token) && r == 0) small[token % 8 * 2 + token / 8] = sc.both;
+        both[b] = sc.both;
+      }
+    }
+    if (owners != 1) continue;
+    if (job.values == 0) {
+#pragma unroll
+      for (int hi = 0; hi < 2; ++hi)
+        if (here(r + 8 * hi) && c == 0) small[r * 2 + hi] = both[hi];
+    } else {
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int token = 2 * c + 8 * (b % 2) + b / 2;
+        if (here(token) && r == 0) small[token % 8 * 2 + token / 8] = both[b];
       }
     }
     uint32_t words[4];

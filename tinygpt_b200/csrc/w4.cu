@@ -180,7 +180,9 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 32 / WARPS : 1) w4_linea
   }
 }
 
-// W as bf16 [n, k], each value rounded once; with `bias`, that as fp32 behind it.  A warp takes a tile: eight values in a row to a lane, four times.
+// W as bf16 [n, k], each value rounded once; with `bias_out`, the bias as fp32 too.  A warp takes kDequantBlocks tiles in a row: eight values in a row to a lane, four
+// times a tile.
+constexpr int kDequantBlocks = 2;
 __global__ void __launch_bounds__(256) w4_dequant_kernel(__nv_bfloat16* out, const W4Params p, int group, float* bias_out) {
   pdl_wait();
   pdl_trigger();
@@ -190,33 +192,40 @@ __global__ void __launch_bounds__(256) w4_dequant_kernel(__nv_bfloat16* out, con
     const int n = (int)tile * 16 + threadIdx.x;
     if (n < p.n) bias_out[n] = bf16_to_f(p.bias[n]);
   }
-  const int b = blockIdx.x * 8 + threadIdx.x / 32;
-  if (b >= p.blocks) return;
-  const uint4 w = ld_once(p.q + (tile * p.blocks + b) * 32 + lane);
-  const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+  const int b0 = (blockIdx.x * 8 + threadIdx.x / 32) * kDequantBlocks;
+  if (b0 >= p.blocks) return;
+  uint4 w[kDequantBlocks];
+  uint32_t s[kDequantBlocks][2], z[kDequantBlocks][2];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int k0 = b * 64 + h * 32 + c * 8;
-    if (k0 >= p.k) break;
-    const int64_t at = (tile * p.groups + k0 / group) * 8 + r;
-    const uint32_t s = __ldg(p.scale + at), z = p.zero != nullptr ? __ldg(p.zero + at) : 0x41004100u;   // 8, 8
+  for (int b = 0; b < kDequantBlocks; ++b) {
+    w[b] = ld_once(p.q + (tile * p.blocks + min(b0 + b, p.blocks - 1)) * 32 + lane);
 #pragma unroll
-    for (int hi = 0; hi < 2; ++hi) {
-      // scale·value − scale·zero: the second product has 16 bits, so that one rounding is left to fp32
-      const float sc = hi ? bf16_hi(s) : bf16_lo(s), off = -sc * (hi ? bf16_hi(z) : bf16_lo(z));
-      uint32_t o[4];
+    for (int h = 0; h < 2; ++h) {
+      const int64_t at = (tile * p.groups + min(((b0 + b) * 64 + h * 32) / group, p.groups - 1)) * 8 + r;
+      s[b][h] = __ldg(p.scale + at);
+      z[b][h] = p.zero != nullptr ? __ldg(p.zero + at) : 0x41004100u;   // 8, 8
+    }
+  }
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        uint32_t a[4];
-        nibbles_128(words[2 * h + t], a);
+  for (int b = 0; b < kDequantBlocks; ++b) {
+    const uint32_t words[4] = {w[b].x, w[b].y, w[b].z, w[b].w};
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint32_t v = a[2 * e + hi];
-          o[2 * t + e] = pack2(fmaf(sc, bf16_lo(v) - 128.f, off), fmaf(sc, bf16_hi(v) - 128.f, off));
-        }
+    for (int h = 0; h < 2; ++h) {
+      const int k0 = (b0 + b) * 64 + h * 32 + c * 8;
+      if (k0 >= p.k) continue;
+      uint32_t v[2][4];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) nibbles_128(words[2 * h + t], v[t]);
+#pragma unroll
+      for (int hi = 0; hi < 2; ++hi) {
+        // scale·value − scale·zero: the second product has 16 bits, so that one rounding is left to fp32
+        const float sc = hi ? bf16_hi(s[b][h]) : bf16_lo(s[b][h]), off = -sc * (hi ? bf16_hi(z[b][h]) : bf16_lo(z[b][h]));
+        uint32_t o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = pack2(fmaf(sc, bf16_lo(v[e / 2][2 * (e % 2) + hi]) - 128.f, off), fmaf(sc, bf16_hi(v[e / 2][2 * (e % 2) + hi]) - 128.f, off));
+        const int64_t n = tile * 16 + r + 8 * hi;
+        if (n < p.n) *reinterpret_cast<uint4*>(out + n * p.k + k0) = make_uint4(o[0], o[1], o[2], o[3]);
       }
-      const int64_t n = tile * 16 + r + 8 * hi;
-      if (n < p.n) *reinterpret_cast<uint4*>(out + n * p.k + k0) = make_uint4(o[0], o[1], o[2], o[3]);
     }
   }
 }
@@ -251,7 +260,7 @@ int launch_rows(const W4Params& p, int group, cudaStream_t st) {
 }
 
 int launch_dequant(void* out, const W4Params& p, int group, float* bias_out, cudaStream_t st) {
-  const dim3 grid((unsigned)((p.blocks + 7) / 8), (unsigned)((p.n + 15) / 16));
+  const dim3 grid((unsigned)((p.blocks + 8 * kDequantBlocks - 1) / (8 * kDequantBlocks)), (unsigned)((p.n + 15) / 16));
   B200_CUDA(launch_pdl(w4_dequant_kernel, grid, dim3(256), 0, st, op_pdl(st), (__nv_bfloat16*)out, p, group, bias_out));
   return B200_OK;
 }

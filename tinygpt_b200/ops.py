@@ -512,11 +512,6 @@ def kv4_attention(cache: KV4Cache, layer: int, q: torch.Tensor, seqs: torch.Tens
 
 
 def _kv4_lists(cache, name, a, b, names):
-    y = getattr(_fast, name)(*cache._at, a, b) if cache.__class__ is KV4Cache else None
-    if y.__class__ is _Tensor:
-        return y
-    if y is not None:
-        check(y, f"b200_{name}")
     d, a, b = _kv4(cache, name, **dict(zip(names, (a, b))))
     n = a.shape[0]
     if b.shape[0] != n or n > KV4_MAX_SEQS:
@@ -531,12 +526,24 @@ def _kv4_lists(cache, name, a, b, names):
 def kv4_extend(cache: KV4Cache, seqs: torch.Tensor, counts: torch.Tensor) -> torch.Tensor:
     """Room for counts[i] more tokens of sequence seqs[i], in order, whole or not at all → the first new position of each, −1 where there are not enough free
     pages or places in the table.  New pages are the lowest free ones.  A sequence that stands in seqs twice is refused the second time."""
+    if cache.__class__ is KV4Cache:
+        y = _fast.kv4_extend(*cache._at, seqs, counts)
+        if y.__class__ is _Tensor:
+            return y
+        if y is not None:
+            check(y, "b200_kv4_extend")
     return _kv4_lists(cache, "kv4_extend", seqs, counts, ("seqs", "counts"))
 
 
 def kv4_fork(cache: KV4Cache, src: torch.Tensor, dst: torch.Tensor) -> torch.Tensor:
     """dst[i] (empty) becomes a copy of src[i]: whole pages are shared until they are freed, a page that is not full is copied, in all layers → 1, or 0 where
     there is no free page or dst[i] is not empty."""
+    if cache.__class__ is KV4Cache:
+        y = _fast.kv4_fork(*cache._at, src, dst)
+        if y.__class__ is _Tensor:
+            return y
+        if y is not None:
+            check(y, "b200_kv4_fork")
     return _kv4_lists(cache, "kv4_fork", src, dst, ("src", "dst"))
 
 
