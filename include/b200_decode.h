@@ -222,7 +222,7 @@ int b200_kv4_load(float* k, float* v, const b200_kv4_cache* cache, int64_t layer
  * sequence i stands at position P = pos[i] + j and sees the positions p <= P that the sequence has, with window > 0 those with P − p < window.  Query head h reads
  * key/value head h / (q_heads / kv_heads).  A row that sees nothing, or belongs to no sequence, is zero.
  * Scores, softmax and sums are fp32; weights of the values are rounded to bf16.  dim as in the cache; q and its rows 16-byte aligned.
- * workspace: b200_kv4_attention_workspace_bytes() bytes, 16-byte aligned, written before it is read. */
+ * workspace: b200_kv4_attention_workspace_bytes() bytes (0: may be NULL), 16-byte aligned, written before it is read. */
 int64_t b200_kv4_attention_workspace_bytes(const b200_kv4_cache* cache, int64_t q_heads, int64_t n, int64_t rows);
 int b200_kv4_attention(void* out, const void* q, int64_t ld_q, const b200_kv4_cache* cache, int64_t layer, int64_t q_heads, const int32_t* seqs,
                        const int32_t* starts, const int32_t* pos, int64_t n, int64_t rows, float scale, int64_t window, void* workspace, void* stream);

@@ -31,11 +31,11 @@ class Rand:
         return (torch.randn(*shape, generator=self.g, device="cuda") * spread + mean).to(BF16)
 
 
-def filled(rand, lengths, kv_heads, dim, layers=1, layer=0, spare=2, seqs=None):
+def filled(rand, lengths, kv_heads, dim, layers=1, layer=0, spare=2, seqs=None, room=1):
     """A cache whose sequences came in two steps, so that their pages lie mixed; k and v as given."""
     n = len(lengths)
     pages = sum(-(-l // 64) for l in lengths) + spare
-    cache = ops.kv4_cache(layers, pages, n, max(max(-(-l // 64) for l in lengths), 1) + 1, kv_heads, dim)
+    cache = ops.kv4_cache(layers, pages, n, max(max(-(-l // 64) for l in lengths), 1) + room, kv_heads, dim)
     cache.pages.fill_(255)   # values 15, scale and middle NaN: what is not written must not be seen
     k, v = rand(sum(lengths), kv_heads, dim, spread=1.5, mean=0.7), rand(sum(lengths), kv_heads, dim)
     order = dev(list(range(n)) if seqs is None else seqs)
@@ -46,8 +46,8 @@ def filled(rand, lengths, kv_heads, dim, layers=1, layer=0, spare=2, seqs=None):
     return cache, order, k, v
 
 
-def run_case(rand, lengths, counts, heads, kv_heads, dim, window=0, scale=None, layers=1, layer=0):
-    cache, seqs, k, v = filled(rand, lengths, kv_heads, dim, layers, layer)
+def run_case(rand, lengths, counts, heads, kv_heads, dim, window=0, scale=None, layers=1, layer=0, room=1):
+    cache, seqs, k, v = filled(rand, lengths, kv_heads, dim, layers, layer, room=room)
     q = rand(max(sum(counts), 1), heads, dim)
     pos = [l - c if l else -1 for l, c in zip(lengths, counts)]
     out = ops.kv4_attention(cache, layer, q, seqs, starts_of(counts), dev(pos), window=window, scale=scale)
@@ -145,25 +145,44 @@ def test_rows_without_a_place(built_lib):
 
 
 # ------------------------------------------------------------------------------------------------- attention
+# room: pages that a sequence could still take.  Calls over small caches go to clusters, others are cut evenly over the GPU's warps.
 @pytest.mark.gpu
+@pytest.mark.parametrize("room", [1, 9000])
 @pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 64), (14, 2, 64), (4, 2, 128), (16, 2, 128), (9, 1, 128), (6, 2, 192), (10, 1, 192), (8, 4, 256), (20, 2, 256)])
-def test_single_tokens(built_lib, heads, kv_heads, dim):
+def test_single_tokens(built_lib, heads, kv_heads, dim, room):
     lengths = [1, 15, 16, 17, 0, 63, 64, 65, 130, 511, 700]
-    run_case(Rand(3), lengths, [1 if l else 1 for l in lengths], heads, kv_heads, dim)
+    run_case(Rand(3), lengths, [1] * len(lengths), heads, kv_heads, dim, room=room)
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,heads,kv_heads,dim", [(1, 4, 1, 64), (8, 4, 2, 128), (9, 8, 4, 64), (35, 3, 1, 128), (18, 32, 4, 64), (74, 2, 2, 64), (2, 24, 2, 256)])
+def test_clusters_of_all_sizes(built_lib, n, heads, kv_heads, dim):
+    """One to eight CTAs to a sequence's head, sequences of which most have fewer steps than the cluster has warps."""
+    lengths = [(37 * i) % 400 + (i % 3 > 0) for i in range(n)]
+    run_case(Rand(12), lengths, [1] * n, heads, kv_heads, dim, window=0 if n % 2 else 70)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("room", [1, 9000])
+def test_unequal_counts_of_few_columns(built_lib, room):
+    """Sequences that bring several blocks of columns where the average brings one; the last rows are nobody's."""
+    run_case(Rand(13), [100, 300, 5, 64, 1], [3, 11, 0, 1, 0], 4, 2, 64, room=room)
+    run_case(Rand(13), [100, 300, 5, 64, 90], [0, 50, 0, 1, 0], 2, 2, 128, room=room)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("room", [1, 9000])
 @pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 64), (7, 1, 64), (8, 2, 128), (4, 2, 192), (4, 1, 256)])
 @pytest.mark.parametrize("window", [0, 1, 40, 200])
-def test_several_tokens(built_lib, heads, kv_heads, dim, window):
-    run_case(Rand(4), [3, 64, 200, 90, 330], [3, 2, 70, 0, 33], heads, kv_heads, dim, window=window)
+def test_several_tokens(built_lib, heads, kv_heads, dim, window, room):
+    run_case(Rand(4), [3, 64, 200, 90, 330], [3, 2, 70, 0, 33], heads, kv_heads, dim, window=window, room=room)
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("lengths", [[6000], [5000, 64, 2000], [700] * 40])
 def test_work_cut_over_ctas(built_lib, lengths):
     rand = Rand(5)
-    cache, q, seqs, pos, out = run_case(rand, lengths, [1] * len(lengths), 4, 2, 64, layers=2, layer=1, scale=0.05)
+    cache, q, seqs, pos, out = run_case(rand, lengths, [1] * len(lengths), 4, 2, 64, layers=2, layer=1, scale=0.05, room=9000)
     again = ops.kv4_attention(cache, 1, q, seqs, starts_of([1] * len(lengths)), dev(pos), scale=0.05)
     assert torch.equal(out, again)
 

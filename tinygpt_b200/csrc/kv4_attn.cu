@@ -12,6 +12,7 @@
 // that holds all of an item writes its rows; parts go to the workspace (one for a CTA whose warps are all inside an item) and a second
 // kernel joins them in their order.
 #include "kv4.cuh"
+#include "tc.cuh"
 
 #include <algorithm>
 
@@ -476,7 +477,7 @@ __device__ __forceinline__ void kv4_split(const Kv4Attn& p, const Walk& w, const
 // rows of no sequence are zero
 __device__ __forceinline__ void kv4_others(const Kv4Attn& p) {
   const int head = min(max(p.starts[0], 0), p.rows), tail = min(max(p.starts[p.n], head), p.rows), width = p.q_heads * p.cache.dim;
-  for (int row = blockIdx.x; row < head + p.rows - tail; row += kGrid)
+  for (int row = blockIdx.x; row < head + p.rows - tail; row += gridDim.x)
     for (int d = threadIdx.x; d < width; d += blockDim.x) p.out[(int64_t)(row < head ? row : row - head + tail) * width + d] = f_to_bf16(0.f);
 }
 
@@ -500,6 +501,134 @@ struct Shape {
   static_assert(kWarps * kOwn <= kRoom, "shared memory of an SM");
 };
 
+// A warp goes over steps first … first + many − 1 of a sequence's with the columns of a block.
+template <int NG, int NT>
+__device__ __forceinline__ void kv4_run(const Kv4Attn& p, const Kv4Seq& s, int head, int col0, int n_cols, int first, int many, uint8_t* own, Columns<NG, NT>& cols) {
+  using S = Shape<NG, NT>;
+  const int lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
+  uint8_t* const ring = own;
+  uint4* const q_smem = reinterpret_cast<uint4*>(own + S::kRing);
+  uint4 q[NT][NG][2];   // the block's queries
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int col = col0 + t * 8 + r;
+    const __nv_bfloat16* src = kv4_query<NG>(p, s, head, col, c);
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) q[t][g][h] = col < n_cols ? *reinterpret_cast<const uint4*>(src + g * 64 + h * 32) : make_uint4(0, 0, 0, 0);
+  }
+  cols.start(p, s, col0, n_cols, c);
+
+  // (steps that no column sees, in a block whose columns stand far apart from the sequence's others, are not gone over)
+  const int step0 = s.step0 + first, n_steps = s.last > 0 ? min(many, cols.at_high / kStep + 1 - step0) : 0;
+  const int32_t* table = p.cache.table + (int64_t)max(s.slot, 0) * p.cache.max_pages;
+  auto page_of = [&](int u) {
+    if (u >= n_steps) return -1;
+    const int page = table[(step0 + u) / (kPage / kStep)];
+    return page < p.cache.n_pages ? page : -1;
+  };
+  auto fetch = [&](int u, int page, int slot) {
+    if (page >= 0) {
+      const uint8_t* src = kv4_head(p.cache, p.layer, page, head) + (step0 + u) % (kPage / kStep) * S::kStage + lane * 16;
+      uint8_t* dst = ring + slot * S::kStage + lane * 16;
+#pragma unroll
+      for (int b = 0; b < S::kStage; b += 512)
+        if (S::kStage % 512 == 0 || b + lane * 16 < S::kStage) cp_async16(dst + b, src + b);
+    }
+    cp_async_commit();
+  };
+  uint32_t have = 0;   // bit u % 32: step u has a page
+  int next;
+#pragma unroll
+  for (int u = 0; u < S::kStages - 1; ++u) {
+    const int page = page_of(u);
+    have |= (uint32_t)(page >= 0) << u;
+    fetch(u, page, u);
+  }
+  next = page_of(S::kStages - 1);
+  int slot = 0;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      cols.take(g, t, q[t][g]);
+      if constexpr (!S::kQInRegs) {
+        q_smem[((t * NG + g) * 2) * 32 + lane] = q[t][g][0];
+        q_smem[((t * NG + g) * 2 + 1) * 32 + lane] = q[t][g][1];
+      }
+    }
+  for (int u = 0; u < n_steps; ++u) {
+    const int ahead = u + S::kStages - 1, into = slot == 0 ? S::kStages - 1 : slot - 1;
+    have = (have & ~(1u << (ahead % 32))) | (uint32_t)(next >= 0) << (ahead % 32);
+    fetch(ahead, next, into);
+    next = page_of(ahead + 1);
+    cp_async_wait<S::kStages - 1>();
+    __syncwarp();
+    const uint8_t* stage = ring + slot * S::kStage;
+    auto keys = [&](int k, int g) { return Nibbles{*reinterpret_cast<const uint4*>(stage + k * S::kTile + g * 512 + lane * 16)}; };
+    auto key_small = [&](int k, int g) { return *reinterpret_cast<const uint2*>(stage + k * S::kTile + NG * 512 + g * 64 + r * 8); };
+    auto values = [&](int k, int g) { return Nibbles{*reinterpret_cast<const uint4*>(stage + k * S::kTile + NG * (512 + 64) + g * 512 + lane * 16)}; };
+    auto value_small = [&](int k, int g) { return *reinterpret_cast<const uint2*>(stage + k * S::kTile + NG * (512 + 64 + 512) + g * 64 + r * 8); };
+    auto query = [&](int t, int g, int h) {
+      if constexpr (S::kQInRegs) return q[t][g][h];
+      else return q_smem[((t * NG + g) * 2 + h) * 32 + lane];
+    };
+    float sc[S::kTiles][NT][4];
+    cols.scores(sc, keys, key_small, query);
+    // a page that is not there counts as not seen, whatever the stage holds
+    const bool whole = cols.mask(sc, (step0 + u) * kStep, have >> (u % 32) & 1 ? s.last : 0, p.window, r);
+    cols.settle(sc, p.scale_log2);
+    if (whole) cols.template values<true>(sc, p.scale_log2, values, value_small);
+    else cols.template values<false>(sc, p.scale_log2, values, value_small);
+    __syncwarp();   // the stage is free
+    slot = slot + 1 == S::kStages ? 0 : slot + 1;
+  }
+  cp_async_wait<0>();
+  __syncwarp();
+  cols.finish();
+}
+
+// The parts of a CTA's first `each` warps, left in their shared memory, become one at `joined`, `wide` floats from a column to the next: a warp takes a column, a lane a
+// warp's maximum and sum.
+template <int NG, int NT>
+__device__ __forceinline__ void kv4_meet(const uint8_t* smem, int each, float* joined, int wide) {
+  using S = Shape<NG, NT>;
+  constexpr int kCols = S::kCols, kWide = NG * 64 + 4;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  for (int col = warp; col < kCols; col += each) {
+    const float* of = reinterpret_cast<const float*>(smem + min(lane, each - 1) * S::kOwn) + kCols * kWide + col;
+    float l = lane < each ? of[kCols] : 0.f, m = l != 0.f ? of[0] : -INFINITY;   // (a sum that is no number has seen a token)
+    float all = m;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, x));
+    const float f = l != 0.f ? exp2_fast(m - all) : 0.f;
+    l *= f;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+    float2 v[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) v[g] = make_float2(0.f, 0.f);
+#pragma unroll 4
+    for (int k = 0; k < each; ++k) {
+      const float fk = __shfl_sync(0xffffffffu, f, k);
+      if (fk == 0.f) continue;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const float2 o2 = *reinterpret_cast<const float2*>(smem + k * S::kOwn + (col * kWide + g * 64 + 2 * lane) * 4);
+        v[g].x = fmaf(fk, o2.x, v[g].x);
+        v[g].y = fmaf(fk, o2.y, v[g].y);
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) *reinterpret_cast<float2*>(joined + col * wide + g * 64 + 2 * lane) = v[g];
+    if (lane == 0) {
+      joined[kCols * wide + col] = all;
+      joined[kCols * wide + kCols + col] = l;
+    }
+  }
+}
+
 template <int NG, int NT>
 __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(const Kv4Attn p) {
   using S = Shape<NG, NT>;
@@ -507,7 +636,6 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
   uint8_t* const ring = smem + warp * S::kOwn;
-  uint4* const q_smem = reinterpret_cast<uint4*>(ring + S::kRing);
   pdl_wait();
   pdl_trigger();
 
@@ -528,86 +656,8 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
     if (many <= 0) continue;
 
     const int col0 = w.block * kCols, n_cols = s.count * p.group.d;
-    uint4 q[NT][NG][2];   // the block's queries
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int col = col0 + t * 8 + r;
-      const __nv_bfloat16* src = kv4_query<NG>(p, s, w.head, col, c);
-#pragma unroll
-      for (int g = 0; g < NG; ++g)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) q[t][g][h] = col < n_cols ? *reinterpret_cast<const uint4*>(src + g * 64 + h * 32) : make_uint4(0, 0, 0, 0);
-    }
     Columns<NG, NT> cols;
-    cols.start(p, s, col0, n_cols, c);
-
-    // (steps that no column sees, in a block whose columns stand far apart from the sequence's others, are not gone over)
-    const int step0 = s.step0 + first, n_steps = s.last > 0 ? min(many, cols.at_high / kStep + 1 - step0) : 0;
-    const int32_t* table = p.cache.table + (int64_t)max(s.slot, 0) * p.cache.max_pages;
-    auto page_of = [&](int u) {
-      if (u >= n_steps) return -1;
-      const int page = table[(step0 + u) / (kPage / kStep)];
-      return page < p.cache.n_pages ? page : -1;
-    };
-    auto fetch = [&](int u, int page, int slot) {
-      if (page >= 0) {
-        const uint8_t* src = kv4_head(p.cache, p.layer, page, w.head) + (step0 + u) % (kPage / kStep) * S::kStage + lane * 16;
-        uint8_t* dst = ring + slot * S::kStage + lane * 16;
-#pragma unroll
-        for (int b = 0; b < S::kStage; b += 512)
-          if (S::kStage % 512 == 0 || b + lane * 16 < S::kStage) cp_async16(dst + b, src + b);
-      }
-      cp_async_commit();
-    };
-    uint32_t have = 0;   // bit u % 32: step u has a page
-    int next;
-#pragma unroll
-    for (int u = 0; u < S::kStages - 1; ++u) {
-      const int page = page_of(u);
-      have |= (uint32_t)(page >= 0) << u;
-      fetch(u, page, u);
-    }
-    next = page_of(S::kStages - 1);
-    int slot = 0;
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        cols.take(g, t, q[t][g]);
-        if constexpr (!S::kQInRegs) {
-          q_smem[((t * NG + g) * 2) * 32 + lane] = q[t][g][0];
-          q_smem[((t * NG + g) * 2 + 1) * 32 + lane] = q[t][g][1];
-        }
-      }
-    for (int u = 0; u < n_steps; ++u) {
-      const int ahead = u + S::kStages - 1, into = slot == 0 ? S::kStages - 1 : slot - 1;
-      have = (have & ~(1u << (ahead % 32))) | (uint32_t)(next >= 0) << (ahead % 32);
-      fetch(ahead, next, into);
-      next = page_of(ahead + 1);
-      cp_async_wait<S::kStages - 1>();
-      __syncwarp();
-      const uint8_t* stage = ring + slot * S::kStage;
-      auto keys = [&](int k, int g) { return Nibbles{*reinterpret_cast<const uint4*>(stage + k * S::kTile + g * 512 + lane * 16)}; };
-      auto key_small = [&](int k, int g) { return *reinterpret_cast<const uint2*>(stage + k * S::kTile + NG * 512 + g * 64 + r * 8); };
-      auto values = [&](int k, int g) { return Nibbles{*reinterpret_cast<const uint4*>(stage + k * S::kTile + NG * (512 + 64) + g * 512 + lane * 16)}; };
-      auto value_small = [&](int k, int g) { return *reinterpret_cast<const uint2*>(stage + k * S::kTile + NG * (512 + 64 + 512) + g * 64 + r * 8); };
-      auto query = [&](int t, int g, int h) {
-        if constexpr (S::kQInRegs) return q[t][g][h];
-        else return q_smem[((t * NG + g) * 2 + h) * 32 + lane];
-      };
-      float sc[S::kTiles][NT][4];
-      cols.scores(sc, keys, key_small, query);
-      // a page that is not there counts as not seen, whatever the stage holds
-      const bool whole = cols.mask(sc, (step0 + u) * kStep, have >> (u % 32) & 1 ? s.last : 0, p.window, r);
-      cols.settle(sc, p.scale_log2);
-      if (whole) cols.template values<true>(sc, p.scale_log2, values, value_small);
-      else cols.template values<false>(sc, p.scale_log2, values, value_small);
-      __syncwarp();   // the stage is free
-      slot = slot + 1 == S::kStages ? 0 : slot + 1;
-    }
-    cp_async_wait<0>();
-    __syncwarp();
-    cols.finish();
+    kv4_run(p, s, w.head, col0, n_cols, first, many, ring, cols);
     if (many == s.steps) {
       cols.write(p, s, w.head, col0, n_cols, r, c);
       continue;
@@ -622,11 +672,55 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
     constexpr int kWide = kDim + 4;   // (columns on other banks)
     cols.leave(reinterpret_cast<float*>(ring), 0, kCols, kWide, r, c);
     named_bar_sync(1, cut.each * 32);   // every warp of the CTA that has a piece comes here, once
-    float* const joined = kv4_part(p, (int64_t)blockIdx.x * S::kWarps, 0, kCols);
-    for (int col = warp; col < kCols; col += cut.each) {   // a warp takes a column, a lane a warp's maximum and sum
-      const float* of = reinterpret_cast<const float*>(smem + min(lane, cut.each - 1) * S::kOwn) + kCols * kWide + col;
-      float l = lane < cut.each ? of[kCols] : 0.f, m = l != 0.f ? of[0] : -INFINITY;   // (a sum that is no number has seen a token)
-      float all = m;
+    kv4_meet<NG, NT>(smem, cut.each, kv4_part(p, (int64_t)blockIdx.x * S::kWarps, 0, kCols), kDim);
+  }
+  kv4_others(p);
+}
+
+// ---- few columns to a sequence of a small cache: a cluster takes a sequence's head, its warps equal pieces of the steps; the parts meet in shared memory, first the
+// CTA's, then over the cluster's.  One launch, no workspace.
+template <int NG, int NT>
+struct Cluster : Shape<NG, NT> {
+  using S = Shape<NG, NT>;
+  static constexpr int kWide = NG * 64 + 4, kJoined = S::kWarps * S::kOwn;      // the CTA's part, behind the warps' rings
+  static constexpr int kSmem = kJoined + S::kCols * (kWide + 2) * 4;
+};
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float ld_cluster_f1(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+template <int NG, int NT>
+__global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_cluster_kernel(const Kv4Attn p, int ctas) {
+  using S = Cluster<NG, NT>;
+  constexpr int kCols = S::kCols, kDim = NG * 64;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = lane / 4, c = lane % 4, rank = (int)cluster_rank();
+  uint8_t* const ring = smem + warp * S::kOwn;
+  float* const joined = reinterpret_cast<float*>(smem + S::kJoined);
+  pdl_wait();
+  pdl_trigger();
+  const int number = blockIdx.x / ctas, i = p.kv_heads.of(number), head = number - i * p.kv_heads.d;
+  const Kv4Seq s = kv4_seq(p, i, kCols);
+  const int n_cols = s.count * p.group.d, piece = rank * S::kWarps + warp, pieces = ctas * S::kWarps;
+  const int first = (int)((int64_t)s.steps * piece / pieces), many = (int)((int64_t)s.steps * (piece + 1) / pieces) - first;
+  for (int col0 = 0; col0 < n_cols; col0 += kCols) {
+    Columns<NG, NT> cols;
+    kv4_run(p, s, head, col0, n_cols, first, many, ring, cols);
+    cols.leave(reinterpret_cast<float*>(ring), 0, kCols, S::kWide, r, c);
+    __syncthreads();
+    kv4_meet<NG, NT>(smem, S::kWarps, joined, S::kWide);
+    cluster_sync_all();
+    for (int col = rank + ctas * warp; col < kCols; col += ctas * S::kWarps) {
+      if (col0 + col >= n_cols) break;
+      const uint32_t at = smem_u32(joined + S::kCols * S::kWide + col);
+      const uint32_t from = mapa_u32(at, min(lane, ctas - 1));
+      float l = lane < ctas ? ld_cluster_f1(from + kCols * 4) : 0.f, m = l != 0.f ? ld_cluster_f1(from) : -INFINITY, all = m;
 #pragma unroll
       for (int x = 1; x < 32; x <<= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, x));
       const float f = l != 0.f ? exp2_fast(m - all) : 0.f;
@@ -637,23 +731,24 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
 #pragma unroll
       for (int g = 0; g < NG; ++g) v[g] = make_float2(0.f, 0.f);
 #pragma unroll 4
-      for (int k = 0; k < cut.each; ++k) {
+      for (int k = 0; k < ctas; ++k) {
         const float fk = __shfl_sync(0xffffffffu, f, k);
         if (fk == 0.f) continue;
+        const uint32_t part = mapa_u32(smem_u32(joined + col * S::kWide + 2 * lane), k);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-          const float2 o2 = *reinterpret_cast<const float2*>(smem + k * S::kOwn + (col * kWide + g * 64 + 2 * lane) * 4);
+          const float2 o2 = ld_cluster_f2(part + g * 256);
           v[g].x = fmaf(fk, o2.x, v[g].x);
           v[g].y = fmaf(fk, o2.y, v[g].y);
         }
       }
+      const float inverse = l == 0.f ? 0.f : 1.f / l;
+      const int token = p.group.of(col0 + col);
+      __nv_bfloat16* out = p.out + ((int64_t)(s.row0 + token) * p.q_heads + head * p.group.d + col0 + col - token * p.group.d) * kDim;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) *reinterpret_cast<float2*>(joined + col * kDim + g * 64 + 2 * lane) = v[g];
-      if (lane == 0) {
-        joined[kCols * kDim + col] = all;
-        joined[kCols * kDim + kCols + col] = l;
-      }
+      for (int g = 0; g < NG; ++g) *reinterpret_cast<uint32_t*>(out + g * 64 + 2 * lane) = pack2(v[g].x * inverse, v[g].y * inverse);
     }
+    cluster_sync_all();   // nobody reads this CTA's part any more
   }
   kv4_others(p);
 }
@@ -890,16 +985,45 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn
 }
 
 // How a call's rows are taken: by the columns that an average sequence brings.  Up to 8: a tile of columns to a warp; up to 32: two; more: a CTA for 128 (64 of heads
-// of 192 and 256), which unpacks for all of them (257 rows of 16 / 8 heads of 128 under a window of 1 024: KVPROMPT µs, two tiles to a warp 36.7).
+// of 192 and 256), which unpacks for all of them (257 rows of 16 / 8 heads of 128 under a window of 1 024: 34.1 µs, two tiles to a warp 36.7).
+// Few columns over a small cache go to clusters: they save the second launch, and are worth it while a warp's share of the longest sequence that the cache can
+// hold is no more than some 2.5 steps above what the even cut would give it (µs, clusters / even cut, one sequence of 24 / 8 heads of 128: 1 000 tokens
+// 7.2 / 10.5, 4 000 9.0 / 11.4, 12 000 14.1 / 13.4; 14 / 2 heads of 64: 1 000 6.8 / 9.3, 4 000 7.7 / 10.6).
 struct Way {
-  int tiles, columns, warps;   // tiles of a warp (0: the CTA's way), columns of a block, pieces of the line to a CTA
+  int tiles, columns, warps, cluster;   // tiles of a warp (0: the CTA's way), columns of a block, pieces of the line to a CTA; CTAs of a cluster (0: none)
 };
-Way kv4_way(int64_t group, int64_t n, int64_t rows, int groups) {
-  const int64_t columns = group * ((rows + n - 1) / n);
-  if (columns > 32) return {0, groups <= 2 ? 128 : 64, 1};
-  return columns > 8 ? Way{2, 16, kPieceWarps} : Way{1, 8, kPieceWarps};
+Way kv4_way(int64_t group, int64_t n, int64_t rows, const b200_kv4_cache& cache) {
+  const int64_t columns = group * ((rows + n - 1) / n), items = n * cache.kv_heads;
+  if (columns > 32) return {0, cache.dim <= 128 ? 128 : 64, 1, 0};
+  const int tiles = columns > 8 ? 2 : 1;
+  int ctas = items <= 16 ? 8 : items <= 35 ? 4 : items <= 74 ? 2 : items <= kGrid ? 1 : 0;   // (that the SMs hold at once)
+  const double steps = (double)cache.max_pages * (kPage / kStep);
+  while (ctas > 1 && ctas / 2 * kPieceWarps >= steps) ctas /= 2;   // no more than a warp for every step
+  if (ctas > 0 && steps * (1.0 / (ctas * kPieceWarps) - (double)cache.kv_heads / (kGrid * kPieceWarps)) <= 2.5) return {tiles, 8 * tiles, 0, ctas};
+  return {tiles, 8 * tiles, kPieceWarps, 0};
 }
 
+template <typename Shape, void (*kKernel)(Kv4Attn, int)>
+int launch_cluster(const Kv4Attn& p, const Way& way, cudaStream_t st) {
+  static PerDevice attrs;
+  B200_CUDA(attrs([] { return cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem); }));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(p.n * p.kv_heads.d * way.cluster));
+  cfg.blockDim = dim3(Shape::kThreads);
+  cfg.dynamicSmemBytes = Shape::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)way.cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = op_pdl(st) ? 1 : 0;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  B200_CUDA(cudaLaunchKernelEx(&cfg, kKernel, p, way.cluster));
+  return B200_OK;
+}
 template <typename Shape, void (*kKernel)(Kv4Attn), void (*kJoin)(Kv4Attn, int, int)>
 int launch(const Kv4Attn& p, const Way& way, cudaStream_t st) {
   B200_CHECK_ARG(way.warps == Shape::kPieces && way.columns == Shape::kCols, "kv4_attention: the workspace is not this kernel's");
@@ -912,6 +1036,8 @@ int launch(const Kv4Attn& p, const Way& way, cudaStream_t st) {
 }
 template <int NG>
 int launch_groups(const Kv4Attn& p, const Way& way, cudaStream_t st) {
+  if (way.cluster > 0)
+    return way.tiles == 1 ? launch_cluster<Cluster<NG, 1>, kv4_cluster_kernel<NG, 1>>(p, way, st) : launch_cluster<Cluster<NG, 2>, kv4_cluster_kernel<NG, 2>>(p, way, st);
   if (way.tiles == 1) return launch<Shape<NG, 1>, kv4_attn_kernel<NG, 1>, kv4_join_kernel<NG>>(p, way, st);
   if (way.tiles == 2) return launch<Shape<NG, 2>, kv4_attn_kernel<NG, 2>, kv4_join_kernel<NG>>(p, way, st);
   return launch<Prompt<NG>, kv4_prompt_kernel<NG>, kv4_join_kernel<NG>>(p, way, st);
@@ -928,7 +1054,7 @@ int64_t b200_kv4_attention_workspace_bytes(const b200_kv4_cache* cache, int64_t 
   using namespace b200;
   if (cache == nullptr || cache->kv_heads < 1 || q_heads < 1 || q_heads % cache->kv_heads != 0 || n < 1 || rows < 1) return -1;
   if (cache->dim % kKvGroup != 0 || cache->dim < 64 || cache->dim > 256) return -1;
-  const Way way = kv4_way(q_heads / cache->kv_heads, n, rows, cache->dim / kKvGroup);
+  const Way way = kv4_way(q_heads / cache->kv_heads, n, rows, *cache);
   return part_floats(way, cache->dim) * 4 + (int64_t)kGrid * way.warps * sizeof(Kv4Split);
 }
 
@@ -937,18 +1063,19 @@ int b200_kv4_attention(void* out, const void* q, int64_t ld_q, const b200_kv4_ca
   using namespace b200;
   int rc = op_check();
   if (rc != B200_OK || (rc = check_kv4_rows(cache, layer, seqs, starts, pos, n, rows, "kv4_attention")) != B200_OK) return rc;
-  B200_CHECK_ARG(out && q && workspace, "kv4_attention: null pointer");
+  B200_CHECK_ARG(out && q, "kv4_attention: null pointer");
   B200_CHECK_ARG(q_heads >= 1 && q_heads <= 1 << 16 && q_heads % cache->kv_heads == 0, "kv4_attention: %lld query heads over %d", (long long)q_heads,
                  cache->kv_heads);
   B200_CHECK_ARG(aligned16(q, workspace, out) && ld_q % 8 == 0 && ld_q >= q_heads * cache->dim, "kv4_attention: q's rows must be 16-byte aligned and apart");
   B200_CHECK_ARG(scale > 0.f && scale < 1e30f && window >= 0, "kv4_attention: scale %g, window %lld", (double)scale, (long long)window);
   // the line of all work is counted in 32 bits: 1 M rows of 32 heads over 64 K tokens, or 64 K over 1 M
   const int64_t group = q_heads / cache->kv_heads;
-  const Way way = kv4_way(group, n, rows, cache->dim / kKvGroup);
+  const Way way = kv4_way(group, n, rows, *cache);
   const int64_t columns = way.columns;
   const int64_t items = cache->kv_heads * std::min(rows * ((group + columns - 1) / columns), rows * group / columns + n);
   B200_CHECK_ARG(items * ((int64_t)cache->max_pages * (kPage / kStep) + kAhead) < 1ll << 31 && rows * q_heads < 1ll << 31,
                  "kv4_attention: %lld rows of %lld heads over %d pages are too many for one call", (long long)rows, (long long)q_heads, cache->max_pages);
+  B200_CHECK_ARG(workspace || way.warps == 0, "kv4_attention: null workspace");
   Kv4Attn p{};
   p.cache = *cache;
   p.out = (__nv_bfloat16*)out;
