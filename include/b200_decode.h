@@ -187,7 +187,7 @@ typedef struct b200_w4_weight {
 /* y[m,n] = bf16( x[m,k]·Wᵀ + bias ), fp32 sums, one rounding.  Up to 32 rows, 64 over a small W (and any number where n is no multiple of 8), the values
  * enter the products exactly and a group's sum is scaled in fp32; more rows take W as bf16 (each weight rounded once), laid out in `workspace`
  * (b200_w4_workspace_bytes(m, n, k) bytes, 16-byte aligned; 0 bytes: may be NULL), through the tensor-core GEMM.
- * Requirements: k % 8 == 0, x 16-byte aligned. */
+ * Requirements: k % 8 == 0, x 16-byte aligned.  x is below 2^120 in magnitude; a row of x that is not finite gives results that are not. */
 int64_t b200_w4_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int b200_w4_linear_bf16(void* y, const void* x, const b200_w4_weight* w, const void* bias_or_null, int64_t m, void* workspace, void* stream);
 /* out[n,k] = bf16(W), 16-byte aligned. */
@@ -199,7 +199,7 @@ int b200_w4_dequant_bf16(void* out, const b200_w4_weight* w, void* stream);
  * reads as NaN.  `pages`: b200_kv4_page_bytes(kv_heads, dim) bytes a page, [layers][n_pages], 16-byte aligned; their inside is the library's.
  * table: the pages of every sequence in order, −1 behind them; length: its tokens; refs: how many sequences list a page (0: free).  All on the
  * device; a new cache has table −1, length and refs 0.  Calls that name sequences take `seqs` (n of them, device, at most 1 024); a number outside
- * the cache, or one that stands in seqs before, is left out (extend, fork: refused). */
+ * the cache is left out, and in extend, fork and free one that stands in the list before (extend, fork: refused). */
 typedef struct b200_kv4_cache {
   void* pages;
   int32_t* table;       /* [n_seqs][max_pages] */
@@ -212,7 +212,7 @@ int64_t b200_kv4_page_bytes(int64_t kv_heads, int64_t dim);
 
 /* k and v [rows, kv_heads, dim] bf16, rows ld_k / ld_v elements apart → one layer of the cache.  Sequence seqs[i] of the call owns rows starts[i] … starts[i + 1] − 1,
  * which go to its positions pos[i], pos[i] + 1, … (pos −1: nowhere).  A row whose page the sequence does not have, or shares with
- * another one, is left out.  starts has n + 1 entries and does not fall.  k, v and their rows 16-byte aligned. */
+ * another one, is left out.  starts has n + 1 entries and does not fall; no position is named twice.  k, v and their rows 16-byte aligned. */
 int b200_kv4_store(const b200_kv4_cache* cache, int64_t layer, const void* k, int64_t ld_k, const void* v, int64_t ld_v, const int32_t* seqs,
                    const int32_t* starts, const int32_t* pos, int64_t n, int64_t rows, void* stream);
 /* The reverse: what the cache holds, fp32 [rows, kv_heads, dim]; zero for a row without a place. */
@@ -221,7 +221,7 @@ int b200_kv4_load(float* k, float* v, const b200_kv4_cache* cache, int64_t layer
 /* out [rows, q_heads, dim] = softmax(scale·q·Kᵀ) V over one layer.  q's rows are ld_q elements apart and belong to the sequences as above; row j of
  * sequence i stands at position P = pos[i] + j and sees the positions p <= P that the sequence has, with window > 0 those with P − p < window.  Query head h reads
  * key/value head h / (q_heads / kv_heads).  A row that sees nothing, or belongs to no sequence, is zero.
- * Scores, softmax and sums are fp32; weights of the values are rounded to bf16.  dim as in the cache; q and its rows 16-byte aligned.
+ * Scores, softmax and sums are fp32; weights of the values are rounded to bf16.  dim as in the cache; q and its rows 16-byte aligned, q below 2^120; scale > 0.
  * workspace: b200_kv4_attention_workspace_bytes() bytes (0: may be NULL), 16-byte aligned, written before it is read. */
 int64_t b200_kv4_attention_workspace_bytes(const b200_kv4_cache* cache, int64_t q_heads, int64_t n, int64_t rows);
 int b200_kv4_attention(void* out, const void* q, int64_t ld_q, const b200_kv4_cache* cache, int64_t layer, int64_t q_heads, const int32_t* seqs,

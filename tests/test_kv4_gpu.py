@@ -77,6 +77,19 @@ def test_refusals_without_a_device():
             ops.kv4_cache(1, 4, 2, 2, 2, 64)
 
 
+def test_descriptors_match_the_compiler(tmp_path):
+    import ctypes as C
+    import subprocess
+    from pathlib import Path
+    from tinygpt_b200._lib import KV4Desc, W4Desc
+    (tmp_path / "sz.c").write_text('#include <stdio.h>\n#include <stddef.h>\n#include "b200_decode.h"\nint main(void) { printf("%zu %zu %zu %zu %zu %zu\\n", '
+                                   'sizeof(b200_w4_weight), offsetof(b200_w4_weight, group), sizeof(b200_kv4_cache), offsetof(b200_kv4_cache, refs), '
+                                   'offsetof(b200_kv4_cache, layers), offsetof(b200_kv4_cache, dim)); return 0; }\n')
+    subprocess.run(["gcc", "-I", str(Path(__file__).resolve().parent.parent / "include"), str(tmp_path / "sz.c"), "-o", str(tmp_path / "sz")], check=True)
+    got = [int(v) for v in subprocess.run([str(tmp_path / "sz")], capture_output=True, text=True, check=True).stdout.split()]
+    assert got == [C.sizeof(W4Desc), W4Desc.group.offset, C.sizeof(KV4Desc), KV4Desc.refs.offset, KV4Desc.layers.offset, KV4Desc.dim.offset]
+
+
 def test_page_bytes(built_lib):
     from tinygpt_b200._lib import lib
     assert [lib().b200_kv4_page_bytes(8, d) for d in (64, 128, 192, 256)] == [2 * 8 * 64 * (d // 2 + d // 64 * 4) for d in (64, 128, 192, 256)]
@@ -253,9 +266,10 @@ def test_rows_that_see_nothing(built_lib):
 
 
 @pytest.mark.gpu
-def test_strides_streams_capture_and_refusals(built_lib):
+@pytest.mark.parametrize("room", [1, 9000])
+def test_strides_streams_capture_and_refusals(built_lib, room):
     rand = Rand(9)
-    cache, seqs, k, v = filled(rand, [150, 40], 2, 128)
+    cache, seqs, k, v = filled(rand, [150, 40], 2, 128, room=room)
     wide = rand(2, 3 * 4 * 128)
     q = wide[:, 512:1024].unflatten(1, (4, 128))
     where = (seqs, dev([0, 1, 2]), dev([149, 39]))
@@ -301,12 +315,70 @@ def test_strides_streams_capture_and_refusals(built_lib):
     assert ops.kv4_attention(cache, 0, q[:0], *where).shape == (0, 4, 128) and ops.kv4_load(cache, 0, *where, 0)[0].shape == (0, 2, 128)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("room", [1, 9000])
+def test_places_past_32_bits(built_lib, room):
+    """A pool of 7 GB: pages and layers whose places no 32 bits hold."""
+    rand = Rand(14)
+    cache = ops.kv4_cache(3, 16000, 3, 3 + room, 8, 256)
+    assert cache.pages[0].numel() * 2 > 2 ** 32
+    cache.table[:, :3] = dev([[15999, 3, 15000], [15998, -1, -1], [7, 15997, -1]])
+    cache.length.copy_(dev([150, 20, 100]))
+    cache.refs[dev([15999, 3, 15000, 15998, 7, 15997]).long()] = 1
+    lengths, seqs = [150, 20, 100], dev([0, 1, 2])
+    k, v, q = rand(270, 8, 256), rand(270, 8, 256), rand(3, 16, 256)
+    ops.kv4_store(cache, 2, k, v, seqs, starts_of(lengths), dev([0, 0, 0]))
+    assert torch.equal(ops.kv4_load(cache, 2, seqs, starts_of(lengths), dev([0, 0, 0]), 270)[1].cpu(), orc.held(v))
+    out, first = ops.kv4_attention(cache, 2, q, seqs, dev([0, 1, 2, 3]), dev([l - 1 for l in lengths])), 0
+    for i, l in enumerate(lengths):
+        want, bound = orc.attention(q[i:i + 1], orc.held(k[first:first + l]), orc.held(v[first:first + l]), l - 1, 1 / 16, 0)
+        assert bool(((out[i:i + 1].cpu().double() - want).abs() <= bound).all())
+        first += l
+    before = cache.pages[2, 15999].clone()
+    assert ops.kv4_compact(cache).tolist() == [6]
+    assert torch.equal(cache.pages[2, cache.table[0, 0]], before) and int(cache.table.max()) < 6
+    assert torch.equal(ops.kv4_attention(cache, 2, q, seqs, dev([0, 1, 2, 3]), dev([l - 1 for l in lengths])), out)
+
+
+@pytest.mark.gpu
+def test_a_chain_beside_the_ends_of_kernels(built_lib):
+    """Launches that begin while the one in front ends read what it wrote: a decode loop without a synchronisation against the same with one after every call."""
+    def chain(sync, room):
+        rand = Rand(15)
+        s = (lambda t: (torch.cuda.synchronize(), t)[1]) if sync else (lambda t: t)
+        hidden, heads, kv_heads, dim, n = 256, 4, 2, 64, 5
+        w_in, w_out = ops.w4_quantize(rand((heads + 2 * kv_heads) * dim, hidden, spread=0.06)), ops.w4_quantize(rand(hidden, heads * dim, spread=0.06), group=128)
+        cache, seqs, starts = ops.kv4_cache(1, 60, n + 1, 4 + room, kv_heads, dim), dev(list(range(n))), dev(list(range(n + 1)))
+        cache.pages.zero_()
+        x, out = rand(n, hidden), []
+        for step in range(70):
+            pos = s(ops.kv4_extend(cache, seqs, dev([1] * n)))
+            q, k, v = (t.unflatten(1, (-1, dim)) for t in s(ops.linear_w4(x, w_in)).split([heads * dim, kv_heads * dim, kv_heads * dim], 1))
+            ops.kv4_store(cache, 0, k, v, seqs, starts, pos)
+            x = s(ops.add(x, s(ops.linear_w4(s(ops.kv4_attention(cache, 0, q, seqs, starts, pos)).flatten(1), w_out))))
+            x = s(ops.rms_norm(x, None, 1e-6))
+            if step % 20 == 10:
+                s(ops.kv4_fork(cache, dev([2]), dev([n])))
+                ops.kv4_free(cache, dev([0]))
+                s(ops.kv4_compact(cache))
+                s(ops.kv4_fork(cache, dev([n]), dev([0])))
+                ops.kv4_free(cache, dev([n]))
+            out.append(x)
+        return torch.stack(out), cache
+    for room in (1, 9000):
+        want, ref = chain(True, room)
+        assert bool(torch.isfinite(want.float()).all())
+        for _ in range(5):
+            got, cache = chain(False, room)
+            assert torch.equal(got, want) and torch.equal(cache.table, ref.table) and torch.equal(cache.refs, ref.refs) and torch.equal(cache.length, ref.length)
+
+
 # ------------------------------------------------------------------------------------------------- pages
 @pytest.mark.gpu
-@pytest.mark.parametrize("seed", range(4))
+@pytest.mark.parametrize("seed", range(8))
 def test_bookkeeping_against_lists(built_lib, seed):
     rng = random.Random(seed)
-    n_pages, n_seqs, max_pages = rng.choice([(40, 6, 9), (5000, 40, 300), (9000, 200, 64), (17, 3, 17)])
+    n_pages, n_seqs, max_pages = rng.choice([(40, 6, 9), (5000, 40, 300), (9000, 200, 64), (17, 3, 17), (4096, 60, 90)])
     cache, model = ops.kv4_cache(2, n_pages, n_seqs, max_pages, 1, 64), orc.Pages(n_pages, n_seqs, max_pages)
     g = torch.Generator(device="cuda").manual_seed(seed)
     cache.pages.random_(0, 256, generator=g)

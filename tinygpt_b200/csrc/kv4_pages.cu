@@ -11,7 +11,7 @@ namespace b200 {
 namespace {
 
 // Threads of a planning CTA: a sequence of the call each, and kEach pages at a time.  Small calls over small pools take the small one, whose barriers and
-// launch cost less (µs, 1 024 / 256 threads, 8 sequences over 384 pages: fork 7.2 / FORK256, extend 4.3 / EXT256).
+// launch cost less (µs, 1 024 / 256 threads, 8 sequences over 384 pages: fork 7.3 / 5.8, extend 4.4 / 3.3).
 constexpr int kMany = kKvMaxSeqs, kFew = 256, kEach = 8;
 inline bool few(int64_t n, int n_pages) { return n <= kFew && n_pages <= 2 * kFew * kEach; }
 constexpr int kCopy = 4 * 256 * 16;   // bytes of a page that a CTA copies at a time
