@@ -176,6 +176,13 @@ def test_clusters_of_all_sizes(built_lib, n, heads, kv_heads, dim):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lengths,heads,kv_heads,dim", [([4500], 8, 1, 64), ([9000, 1, 4097], 6, 2, 128), ([8200], 12, 6, 64), ([4200, 4099], 16, 2, 192)])
+def test_clusters_of_sixteen(built_lib, lengths, heads, kv_heads, dim):
+    """Few heads over long caches: 128 warps to a sequence's head, of which a short neighbour needs one."""
+    run_case(Rand(14), lengths, [1] * len(lengths), heads, kv_heads, dim, window=0)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("room", [1, 9000])
 def test_unequal_counts_of_few_columns(built_lib, room):
     """Sequences that bring several blocks of columns where the average brings one; the last rows are nobody's."""

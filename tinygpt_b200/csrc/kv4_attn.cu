@@ -987,8 +987,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn
 // How a call's rows are taken: by the columns that an average sequence brings.  Up to 8: a tile of columns to a warp; up to 32: two; more: a CTA for 128 (64 of heads
 // of 192 and 256), which unpacks for all of them (257 rows of 16 / 8 heads of 128 under a window of 1 024: 34.1 µs, two tiles to a warp 36.7).
 // Few columns over a small cache go to clusters: they save the second launch, and are worth it while a warp's share of the longest sequence that the cache can
-// hold is no more than some 2.5 steps above what the even cut would give it (µs, clusters / even cut, one sequence of 24 / 8 heads of 128: 1 000 tokens
-// 7.2 / 10.5, 4 000 9.0 / 11.4, 12 000 14.1 / 13.4; 14 / 2 heads of 64: 1 000 6.8 / 9.3, 4 000 7.7 / 10.6).
+// hold is no more than some three steps above what the even cut would give it (µs, clusters / even cut, one sequence of 24 / 8 heads of 128: 1 000 tokens
+// 7.2 / 10.5, 4 000 9.0 / 11.4, 12 000 14.0 / 13.2; 14 / 2 heads of 64: 1 000 6.5 / 8.8, 4 000 7.5 / 10.2, 16 000 9.9 / 11.8; 32 / 4 heads of 128: 8 000 9.9 / 12.3,
+// 32 768 18.4 / 18.7).  As large a cluster as the SMs hold all of at once: of 16 CTAs 7, of 8 15, of 4 33 (36 / 6 heads of 128, 12 000
+// tokens: clusters of 16 11.0, of 10 13.0; 24 / 8 heads, 4 000 tokens, where eight clusters of 16 are two rounds: 15.9).
 struct Way {
   int tiles, columns, warps, cluster;   // tiles of a warp (0: the CTA's way), columns of a block, pieces of the line to a CTA; CTAs of a cluster (0: none)
 };
@@ -996,17 +998,20 @@ Way kv4_way(int64_t group, int64_t n, int64_t rows, const b200_kv4_cache& cache)
   const int64_t columns = group * ((rows + n - 1) / n), items = n * cache.kv_heads;
   if (columns > 32) return {0, cache.dim <= 128 ? 128 : 64, 1, 0};
   const int tiles = columns > 8 ? 2 : 1;
-  int ctas = items <= 16 ? 8 : items <= 35 ? 4 : items <= 74 ? 2 : items <= kGrid ? 1 : 0;   // (that the SMs hold at once)
+  int ctas = items <= 6 ? 16 : items <= 15 ? 8 : items <= 33 ? 4 : items <= 74 ? 2 : items <= kGrid ? 1 : 0;   // (that the SMs hold at once)
   const double steps = (double)cache.max_pages * (kPage / kStep);
   while (ctas > 1 && ctas / 2 * kPieceWarps >= steps) ctas /= 2;   // no more than a warp for every step
-  if (ctas > 0 && steps * (1.0 / (ctas * kPieceWarps) - (double)cache.kv_heads / (kGrid * kPieceWarps)) <= 2.5) return {tiles, 8 * tiles, 0, ctas};
+  if (ctas > 0 && steps * (1.0 / (ctas * kPieceWarps) - (double)cache.kv_heads / (kGrid * kPieceWarps)) <= 3.2) return {tiles, 8 * tiles, 0, ctas};
   return {tiles, 8 * tiles, kPieceWarps, 0};
 }
 
 template <typename Shape, void (*kKernel)(Kv4Attn, int)>
 int launch_cluster(const Kv4Attn& p, const Way& way, cudaStream_t st) {
   static PerDevice attrs;
-  B200_CUDA(attrs([] { return cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem); }));
+  B200_CUDA(attrs([] {
+    const cudaError_t e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem);
+    return e != cudaSuccess ? e : cudaFuncSetAttribute(kKernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  }));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(p.n * p.kv_heads.d * way.cluster));
   cfg.blockDim = dim3(Shape::kThreads);
