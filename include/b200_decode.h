@@ -185,8 +185,8 @@ typedef struct b200_w4_weight {
 } b200_w4_weight;
 
 /* y[m,n] = bf16( x[m,k]·Wᵀ + bias ), fp32 sums, one rounding.  Up to 32 rows, 64 over a small W (and any number where n is no multiple of 8), the values
- * enter the products exactly and a group's sum is scaled in fp32; more rows take W as bf16 (each weight rounded once), laid out in `workspace`
- * (b200_w4_workspace_bytes(m, n, k) bytes, 16-byte aligned; 0 bytes: may be NULL), through the tensor-core GEMM.
+ * enter the products exactly and a group's sum is scaled in fp32; more rows take W as bf16 (each weight rounded once): up to 256 rows unpacked on the way into the
+ * tensor cores, more laid out in `workspace` (b200_w4_workspace_bytes(m, n, k) bytes, 16-byte aligned; 0 bytes: may be NULL) for the general GEMM.
  * Requirements: k % 8 == 0, x 16-byte aligned.  x is below 2^120 in magnitude; a row of x that is not finite gives results that are not. */
 int64_t b200_w4_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int b200_w4_linear_bf16(void* y, const void* x, const b200_w4_weight* w, const void* bias_or_null, int64_t m, void* workspace, void* stream);

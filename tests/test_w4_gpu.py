@@ -91,6 +91,27 @@ def test_linear_w4(built_lib, n, k, group, zero):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("group,zero", [(32, False), (32, True), (64, True), (128, False), (128, True)])
+@pytest.mark.parametrize("n,k", [(1032, 8200), (4104, 2056), (8200, 1000), (20008, 512), (24, 4096), (1000, 136)])
+def test_many_rows(built_lib, n, k, group, zero):
+    """From 33 rows over large weights and 65 over all: tiles of 128 channels that one to eight CTAs share, zeros between the whole numbers and on them, rows past a
+    tile's and past what is unpacked into the products."""
+    v, s, z = parts(n, k, group, zero)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    if zero:
+        z[: n // 2] = z[: n // 2].round()
+    w, full = ops.w4_pack(v, s, z, group=group), dense(v, s, z, group)
+    for m in (40, 65, 80, 128, 129, 256, 257):
+        x, b = torch.randn(m, k, generator=g, device="cuda").to(BF16), torch.randn(n, generator=g, device="cuda").to(BF16)
+        y = ops.linear_w4(x, w)
+        close(y, x, full, None, 2.0 ** -8 if m > 64 or n * k > 6_000_000 else 0.0)
+        close(ops.linear_w4(x, w, b), x, full, b, 2.0 ** -8 if m > 64 or n * k > 6_000_000 else 0.0)
+        x[3, k - 1] = float("inf")
+        got = ops.linear_w4(x, w)
+        assert not bool(got[3].isfinite().any()) and torch.equal(got[:3], y[:3]) and torch.equal(got[4:], y[4:])   # a row's values reach that row alone
+
+
+@pytest.mark.gpu
 def test_calls_of_all_kinds(built_lib):
     v, s, z = parts(48, 128, 64, True)
     w, full = ops.w4_pack(v, s, z), dense(v, s, z, 64)

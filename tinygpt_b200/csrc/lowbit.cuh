@@ -46,7 +46,8 @@ __device__ __forceinline__ void nibbles_bf16(uint32_t w, uint32_t (&a)[4]) {
 }
 #endif
 
-// ---- Linears over weights of 4 bits (w4.cu)
+// ---- Linears over weights of 4 bits (w4.cu; w4_gemm.cu: any number of rows, on tcgen05)
+int launch_w4_gemm(void* y, const void* x, const b200_w4_weight& w, const void* bias, int64_t m, cudaStream_t st);
 int64_t w4_linear_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int launch_w4_linear(void* y, const void* x, const b200_w4_weight& w, const void* bias, int64_t m, void* workspace, cudaStream_t st);
 int launch_w4_dequant(void* out, const b200_w4_weight& w, cudaStream_t st);

@@ -265,19 +265,27 @@ int launch_dequant(void* out, const W4Params& p, int group, float* bias_out, cud
   return B200_OK;
 }
 
-// Rows of x for which W is laid out as bf16 for the tcgen05 GEMM: more than 64, and more than 32 over a large W, where eight tiles of columns cost the
-// mma.sync kernel more than the copy of W (µs at 64 rows, here / there: 4 096 × 4 096 16.8 / 17.7, 14 336 × 4 096 56 / 47).
-bool as_gemm(int64_t m, int64_t n, int64_t k) { return n % 8 == 0 && (m > 64 || (m > 32 && n * k > 20 * 1000 * 1000)); }
+// Which way rows of x go.  Values exact (w4_linear_kernel): up to 32 rows, and up to 64 over a W whose unpacking for each eight of them costs little (µs at 64 rows,
+// exact / on tcgen05: 4 096 × 4 096 17.7 / 11.2, 14 336 × 4 096 45.8 / 22.0).  W as bf16, unpacked into the products of 128 rows (w4_gemm.cu), up to 256.  More: W laid out
+// as bf16 once, which costs its writing, and the general GEMM (µs, unpacked / laid out: 128 × 1 024 × 1 024 8.8 / 13.0, 128 × 4 096 × 4 096 12.9 / 18.8, 256 × 4 096 × 4 096
+// 17.1 / 22.4, 256 × 4 096 × 14 336 37.7 / 62, 256 × 28 672 × 4 096 96 / 104; 300 × 896 × 896 9.9 / 8.8, 512 × 4 096 × 4 096 25.9 / 25.3, 512 × 14 336 × 4 096 94 / 72).
+enum class W4Way { exact, unpacked, laid_out };
+W4Way w4_way(int64_t m, int64_t n, int64_t k) {
+  if (n % 8 != 0 || m <= 32 || (m <= 64 && n * k <= 6 * 1000 * 1000)) return W4Way::exact;
+  return m <= 256 ? W4Way::unpacked : W4Way::laid_out;
+}
 int64_t bf16_bytes(int64_t n, int64_t k) { return (n * k * 2 + 15) / 16 * 16; }
 
 }  // namespace
 
-int64_t w4_linear_workspace_bytes(int64_t m, int64_t n, int64_t k) { return as_gemm(m, n, k) ? bf16_bytes(n, k) + n * 4 : 0; }
+int64_t w4_linear_workspace_bytes(int64_t m, int64_t n, int64_t k) { return w4_way(m, n, k) == W4Way::laid_out ? bf16_bytes(n, k) + n * 4 : 0; }
 
 int launch_w4_linear(void* y, const void* x, const b200_w4_weight& w, const void* bias, int64_t m, void* workspace, cudaStream_t st) {
   W4Params p = params(w);
   p.bias = (const __nv_bfloat16*)bias;
-  if (as_gemm(m, w.n, w.k)) {
+  const W4Way way = w4_way(m, w.n, w.k);
+  if (way == W4Way::unpacked) return launch_w4_gemm(y, x, w, bias, m, st);
+  if (way == W4Way::laid_out) {
     float* b = bias != nullptr ? (float*)((char*)workspace + bf16_bytes(w.n, w.k)) : nullptr;
     const int rc = launch_dequant(workspace, p, w.group, b, st);
     if (rc != B200_OK) return rc;

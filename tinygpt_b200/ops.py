@@ -339,7 +339,7 @@ def _same_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
 
 def linear_w4(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """linear over a weight of 4 bits: x [..., k] bf16 → bf16(x·Wᵀ + bias) [..., n], fp32 sums, rounded once.  Up to 32 rows (64 over a small
-    weight) the weight enters exactly; more rows multiply it as bf16 (tensor-core GEMM over a copy in a workspace)."""
+    weight) the weight enters exactly; more rows multiply it as bf16 (beyond 256 as a copy in a workspace)."""
     y = _fast.linear_w4(x, weight.q, weight.scale, weight.zero, weight.n, weight.k, weight.group, bias) if weight.__class__ is W4Weight else None
     if y.__class__ is _Tensor:
         return y
