@@ -199,6 +199,15 @@ def test_several_tokens(built_lib, heads, kv_heads, dim, window, room):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lengths,counts,heads,kv_heads,dim", [([700], [700], 8, 1, 64), ([520, 900, 1], [520, 333, 1], 6, 2, 128), ([40 + i for i in range(40)], [40] * 40, 8, 2, 64),
+                                                               ([300], [300], 4, 2, 256)])
+@pytest.mark.parametrize("window", [0, 1, 90])
+def test_prompts(built_lib, lengths, counts, heads, kv_heads, dim, window):
+    """Rows from a sequence's first token on: blocks of columns that see from one step to all, more of them than a warp has lanes, empty ones under a window."""
+    run_case(Rand(15), lengths, counts, heads, kv_heads, dim, window=window)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("lengths", [[6000], [5000, 64, 2000], [700] * 40])
 def test_work_cut_over_ctas(built_lib, lengths):
     rand = Rand(5)

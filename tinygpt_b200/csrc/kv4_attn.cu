@@ -95,7 +95,22 @@ __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4Attn& p, int i, int columns) 
   s.steps = max((s.last + kStep - 1) / kStep - s.step0, 1);
   return s;
 }
-__device__ __forceinline__ long long kv4_line(const Kv4Attn& p, const Kv4Seq& s) { return (long long)s.blocks * p.cache.kv_heads * (s.steps + kAhead); }
+// The steps that a block of columns sees, from s.step0 on: the first of them, and how many (one at least).
+__device__ __forceinline__ int2 kv4_block_steps(const Kv4Attn& p, const Kv4Seq& s, int block, int columns) {
+  const int low = s.pos + p.group.of(block * columns), high = s.pos + p.group.of(min((block + 1) * columns, s.count * (int)p.group.d) - 1);
+  const int end = s.last > 0 ? min(s.steps, high / kStep + 1 - s.step0) : 1;
+  const int begin = p.window > 0 && low >= p.window ? max((low - p.window + 1) / kStep - s.step0, 0) : 0;
+  return make_int2(min(begin, max(end - 1, 0)), max(end - begin, 1));
+}
+// What a sequence takes of the line.  EXACT: every block what its own columns see (a prompt's first rows see little of it, and under a window none sees all: 2 048
+// rows of 16 / 8 heads of 128 from the first token on 194 → 114 µs); else all that the sequence's rows see.
+template <bool EXACT>
+__device__ __forceinline__ long long kv4_line(const Kv4Attn& p, const Kv4Seq& s, int columns) {
+  if constexpr (!EXACT) return (long long)s.blocks * p.cache.kv_heads * (s.steps + kAhead);
+  long long sum = 0;
+  for (int b = 0; b < s.blocks; ++b) sum += kv4_block_steps(p, s, b, columns).y + kAhead;
+  return sum * p.cache.kv_heads;
+}
 __device__ __forceinline__ Kv4Seq kv4_from(const Kv4Seq& s, int lane) {   // another lane's
   Kv4Seq o;
   o.row0 = __shfl_sync(0xffffffffu, s.row0, lane);
@@ -111,12 +126,12 @@ __device__ __forceinline__ Kv4Seq kv4_from(const Kv4Seq& s, int lane) {   // ano
 // ends[i]: the line up to the end of sequence i; all of it comes back.  The call has checked that it is below 2^31 for starts that do not fall; for others it may not
 // be, and nothing is done.  All threads of a CTA of THREADS.
 __device__ __forceinline__ int kv4_whole(long long line) { return line <= INT32_MAX ? (int)line : 0; }
-template <int THREADS>
+template <int THREADS, bool EXACT>
 __device__ int kv4_plan(const Kv4Attn& p, int columns, int* ends) {
   __shared__ long long carry[THREADS / 32];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, each = (p.n + THREADS - 1) / THREADS, first = threadIdx.x * each;
   long long sum = 0;
-  for (int i = first; i < min(first + each, p.n); ++i) sum += kv4_line(p, kv4_seq(p, i, columns));
+  for (int i = first; i < min(first + each, p.n); ++i) sum += kv4_line<EXACT>(p, kv4_seq(p, i, columns), columns);
   const long long upto = warp_scan(sum, lane);
   if (lane == 31) carry[warp] = upto;
   __syncthreads();
@@ -125,7 +140,7 @@ __device__ int kv4_plan(const Kv4Attn& p, int columns, int* ends) {
     if (w < warp) before += carry[w];
     all += carry[w];
   }
-  for (int i = first; i < min(first + each, p.n); ++i) ends[i] = (int)(before += kv4_line(p, kv4_seq(p, i, columns)));
+  for (int i = first; i < min(first + each, p.n); ++i) ends[i] = (int)(before += kv4_line<EXACT>(p, kv4_seq(p, i, columns), columns));
   __syncthreads();
   return kv4_whole(all);
 }
@@ -408,6 +423,7 @@ struct Unpacked {
 };
 
 // A CTA's or a warp's way along the line: the sequences' ends, and one item after the other.
+template <bool EXACT>
 struct Walk {
   Kv4Seq mine;      // up to 32 sequences: every warp has them all in its lanes, and nobody waits for anybody
   int mine_end, line, i;
@@ -422,11 +438,22 @@ struct Walk {
     mine_end = 0;
     if (few) {
       if (lane < p.n) mine = kv4_seq(p, lane, columns);
-      const long long end = warp_scan(lane < p.n ? kv4_line(p, mine) : 0, lane);
+      constexpr int kAlone = EXACT ? 2 : INT32_MAX;   // blocks that a lane goes through by itself
+      long long length = lane < p.n && mine.blocks <= kAlone ? kv4_line<EXACT>(p, mine, columns) : 0;
+      for (uint32_t left = __ballot_sync(0xffffffffu, mine.blocks > kAlone); left != 0; left &= left - 1) {
+        const int of = __ffs(left) - 1;
+        const Kv4Seq s = kv4_from(mine, of);
+        long long sum = 0;
+        for (int b = lane; b < s.blocks; b += 32) sum += kv4_block_steps(p, s, b, columns).y + kAhead;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        if (lane == of) length = sum * p.cache.kv_heads;
+      }
+      const long long end = warp_scan(length, lane);
       mine_end = (int)end;
       line = kv4_whole(__shfl_sync(0xffffffffu, end, 31));
     } else {
-      line = kv4_plan<THREADS>(p, columns, room);
+      line = kv4_plan<THREADS, EXACT>(p, columns, room);
     }
   }
   __device__ __forceinline__ void seek(int n, int at, int stop) { i = !few && at < stop ? kv4_find(ends, n, at) : 0; }
@@ -444,17 +471,40 @@ struct Walk {
       if (i > 0) base = ends[i - 1];
       s = kv4_seq(p, i, columns);
     }
+    if constexpr (EXACT) {
+      const int lane = threadIdx.x % 32;
+      for (int first = 0;; first += 32) {   // (`at` lies in a block of the sequence)
+        const int2 steps = first + lane < s.blocks ? kv4_block_steps(p, s, first + lane, columns) : make_int2(0, -kAhead);
+        const int upto = (int)warp_scan((long long)(steps.y + kAhead) * (int)p.kv_heads.d, lane);
+        const uint32_t before = __ballot_sync(0xffffffffu, base + upto <= at);
+        if (before == 0xffffffffu) {
+          base += __shfl_sync(0xffffffffu, upto, 31);
+          continue;
+        }
+        const int k = __popc(before);
+        if (k > 0) base += __shfl_sync(0xffffffffu, upto, k - 1);
+        block = first + k;
+        s.step0 += __shfl_sync(0xffffffffu, steps.x, k);
+        s.steps = __shfl_sync(0xffffffffu, steps.y, k);
+        break;
+      }
+    }
     const int length = s.steps + kAhead;
     int number = (int)((float)(at - base) * __frcp_rn((float)length));   // (a division costs more than these)
     while (number * length > at - base) --number;
     while ((number + 1) * length <= at - base) ++number;
-    block = p.kv_heads.of(number);
-    head = number - block * p.kv_heads.d;
+    if constexpr (EXACT) {
+      head = number;
+    } else {
+      block = p.kv_heads.of(number);
+      head = number - block * p.kv_heads.d;
+    }
     begin = base + number * length + kAhead;
     end = begin + s.steps;
   }
 };
-__device__ __forceinline__ void kv4_split(const Kv4Attn& p, const Walk& w, const Cut& cut, int64_t own, int me, int col0, int n_cols) {
+template <bool EXACT>
+__device__ __forceinline__ void kv4_split(const Kv4Attn& p, const Walk<EXACT>& w, const Cut& cut, int64_t own, int me, int col0, int n_cols) {
   auto warp_at = [&](int x) {   // whose piece of the line x is
     int v = min(x / cut.whole, cut.warps - 1);
     while (cut.start(v) > x) --v;
@@ -639,8 +689,8 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
   pdl_wait();
   pdl_trigger();
 
-  Walk w{};
-  w.plan<S::kThreads>(p, kCols, reinterpret_cast<int*>(smem + S::kWarps * S::kOwn));
+  Walk<false> w{};
+  w.template plan<S::kThreads>(p, kCols, reinterpret_cast<int*>(smem + S::kWarps * S::kOwn));
   const Cut cut(w.line, S::kWarps);
   const int me = blockIdx.x * cut.each + warp;
   const int64_t own = (int64_t)blockIdx.x * S::kWarps + warp;   // of the workspace's places
@@ -780,8 +830,8 @@ __global__ void __launch_bounds__(Prompt<NG>::kThreads, 1) kv4_prompt_kernel(con
   pdl_wait();
   pdl_trigger();
 
-  Walk w{};
-  w.plan<S::kThreads>(p, S::kCols, reinterpret_cast<int*>(smem + S::kStages * S::kStage + 2 * S::kUnpacked));
+  Walk<true> w{};
+  w.template plan<S::kThreads>(p, S::kCols, reinterpret_cast<int*>(smem + S::kStages * S::kStage + 2 * S::kUnpacked));
   const Cut cut(w.line, 1);
   int at_line = cut.start(blockIdx.x);
   const int stop = cut.start(blockIdx.x + 1);
@@ -985,7 +1035,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn
 }
 
 // How a call's rows are taken: by the columns that an average sequence brings.  Up to 8: a tile of columns to a warp; up to 32: two; more: a CTA for 128 (64 of heads
-// of 192 and 256), which unpacks for all of them (257 rows of 16 / 8 heads of 128 under a window of 1 024: 34.1 µs, two tiles to a warp 36.7).
+// of 192 and 256), which unpacks for all of them (257 rows of 16 / 8 heads of 128 under a window of 1 024: 32.0 µs, two tiles to a warp 36.7).
 // Few columns over a small cache go to clusters: they save the second launch, and are worth it while a warp's share of the longest sequence that the cache can
 // hold is no more than some three steps above what the even cut would give it (µs, clusters / even cut, one sequence of 24 / 8 heads of 128: 1 000 tokens
 // 7.2 / 10.5, 4 000 9.0 / 11.4, 12 000 14.0 / 13.2; 14 / 2 heads of 64: 1 000 6.5 / 8.8, 4 000 7.5 / 10.2, 16 000 9.9 / 11.8; 32 / 4 heads of 128: 8 000 9.9 / 12.3,
