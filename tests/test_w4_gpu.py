@@ -92,7 +92,7 @@ def test_linear_w4(built_lib, n, k, group, zero):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("group,zero", [(32, False), (32, True), (64, True), (128, False), (128, True)])
-@pytest.mark.parametrize("n,k", [(1032, 8200), (4104, 2056), (8200, 1000), (20008, 512), (24, 4096), (1000, 136)])
+@pytest.mark.parametrize("n,k", [(1032, 8200), (4104, 2056), (8200, 1000), (20008, 512), (24, 4096), (1000, 136), (24, 8)])
 def test_many_rows(built_lib, n, k, group, zero):
     """From 33 rows over large weights and 65 over all: tiles of 128 channels that one to eight CTAs share, zeros between the whole numbers and on them, rows past a
     tile's and past what is unpacked into the products."""
@@ -142,7 +142,7 @@ def test_calls_of_all_kinds(built_lib):
         assert torch.equal(out, want)
     for bad in (lambda: ops.linear_w4(x.float(), w), lambda: ops.linear_w4(x[..., :64], w), lambda: ops.linear_w4(x, v), lambda: ops.linear_w4(x.cpu(), w),
                 lambda: ops.linear_w4(x, w, torch.zeros(47, device="cuda", dtype=BF16)), lambda: ops.linear_w4(x, w._replace(n=64)),
-                lambda: ops.linear_w4(x, w._replace(q=w.q[:512])), lambda: ops.linear_w4(x, w._replace(group=48)),
+                lambda: ops.linear_w4(x, w._replace(q=w.q[:512])), lambda: ops.linear_w4(x, w._replace(group=48)), lambda: ops.linear_w4(x, w._replace(n=2 ** 70)),
                 lambda: ops.linear_w4(torch.zeros(129, device="cuda", dtype=BF16)[1:], w)):
         with pytest.raises(B200Error):
             bad()

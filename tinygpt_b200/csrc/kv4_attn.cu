@@ -473,7 +473,8 @@ struct Walk {
     }
     if constexpr (EXACT) {
       const int lane = threadIdx.x % 32;
-      for (int first = 0;; first += 32) {   // (`at` lies in a block of the sequence)
+      block = 0;
+      for (int first = 0; first < s.blocks; first += 32) {   // (`at` lies in a block of the sequence, unless someone writes to its length meanwhile)
         const int2 steps = first + lane < s.blocks ? kv4_block_steps(p, s, first + lane, columns) : make_int2(0, -kAhead);
         const int upto = (int)warp_scan((long long)(steps.y + kAhead) * (int)p.kv_heads.d, lane);
         const uint32_t before = __ballot_sync(0xffffffffu, base + upto <= at);
@@ -494,7 +495,7 @@ struct Walk {
     while (number * length > at - base) --number;
     while ((number + 1) * length <= at - base) ++number;
     if constexpr (EXACT) {
-      head = number;
+      head = min(number, (int)p.kv_heads.d - 1);
     } else {
       block = p.kv_heads.of(number);
       head = number - block * p.kv_heads.d;

@@ -193,13 +193,22 @@ PyObject* attn_decode(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+int64_t whole_number(PyObject* o) {   // −1, which nothing here takes, for one that no int64 holds
+  const int64_t v = PyLong_AsLongLong(o);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return -1;
+  }
+  return v;
+}
+
 PyObject* linear_w4(PyObject*, PyObject* const* a, Py_ssize_t n_args) {   // x, q, scale, zero or None, n, k, group, bias or None
   HANDLE_TH_ERRORS
   const at::Tensor *x, *q, *scale, *zero, *b;
   if (n_args != 8 || modes() || !(x = plain(a[0])) || !(q = plain(a[1], at::kByte)) || !(scale = plain(a[2])) || !plain_or_none(a[3], zero) ||
       !PyLong_Check(a[4]) || !PyLong_Check(a[5]) || !PyLong_Check(a[6]) || !plain_or_none(a[7], b) || x->dim() < 1)
     Py_RETURN_NONE;
-  const int64_t n = PyLong_AsLongLong(a[4]), k = PyLong_AsLongLong(a[5]), group = PyLong_AsLongLong(a[6]);
+  const int64_t n = whole_number(a[4]), k = whole_number(a[5]), group = whole_number(a[6]);
   if (n < 1 || k < 1 || group < 1 || n > 16 * 65535 || k > 1 << 24 || x->size(-1) != k || x->numel() < 1 || !w4_fits(*q, *scale, zero, n, k, group) ||
       (b != nullptr && b->numel() != n))
     Py_RETURN_NONE;
@@ -261,15 +270,6 @@ PyObject* status(F call) {   // of a call without a result: None was not for it,
   }
   if (rc == 0) Py_RETURN_TRUE;
   return PyLong_FromLong(rc);
-}
-
-int64_t whole_number(PyObject* o) {   // −1, which nothing here takes, for one that no int64 holds
-  const int64_t v = PyLong_AsLongLong(o);
-  if (PyErr_Occurred()) {
-    PyErr_Clear();
-    return -1;
-  }
-  return v;
 }
 
 PyObject* kv4_store(PyObject*, PyObject* const* a, Py_ssize_t n_args) {   // cache, device, layer, k, v, seqs, starts, pos
