@@ -76,7 +76,7 @@ def test_quantize_is_within_half_a_step(symmetric, group):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("group,zero", [(32, False), (32, True), (64, False), (64, True), (128, False), (128, True)])
-@pytest.mark.parametrize("n,k", [(1, 8), (16, 64), (40, 200), (33, 1000), (264, 1096), (4104, 328)])
+@pytest.mark.parametrize("n,k", [(1, 8), (16, 64), (40, 200), (33, 1000), (264, 1096), (4104, 328), (8200, 264)])
 def test_linear_w4(built_lib, n, k, group, zero):
     v, s, z = parts(n, k, group, zero)
     w, full = ops.w4_pack(v, s, z, group=group), dense(v, s, z, group)

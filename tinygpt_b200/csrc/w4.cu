@@ -299,10 +299,17 @@ int launch_w4_linear(void* y, const void* x, const b200_w4_weight& w, const void
     // Two row tiles to a warp share the loads of x and its sums, where CTAs are left for all SMs (µs, one / two: 1 × 4 096 × 4 096 4.9 / 4.7, 8 × 8 192 × 4 096
     // 8.1 / 7.2, 32 × 4 096 × 4 096 12.8 / 9.7; 8 × 2 048 × 4 896 4.9 / 5.7, 32 × 1 024 × 4 096 6.9 / 9.1).  All warps of a CTA share a row tile's
     // columns: fewer warps to a tile are fewer sums, and lost at every size (28 672 × 4 096: 17.7, four warps a tile 19.3).
-    const bool two = (p.n + 15) / 16 >= 256;
+    // Four where the loads of x weigh more, at 17 to 32 rows, or its sums, at 9 to 16 with zeros of many groups, and a CTA is left for most SMs (two / four: 32 × 28 672 ×
+    // 4 096 51 / 45, 24 × 8 192 × 4 096 17.8 / 14.8, 12 × 8 192 × 4 096 with zeros of 64 columns 12.1 / 9.5; with zeros of 128, 16 × 28 672 × 4 096 26.4 / 29.6, without
+    // 24.5 / 28.3, one row of it 16.5 / 16.6).
+    const int tiles = (p.n + 15) / 16;
+    const bool two = tiles >= 256, four = tiles >= 512;
     const int rc = p.m <= 8 ? (two ? launch_rows<1, 2, 8>(p, w.group, st) : launch_rows<1, 1, 8>(p, w.group, st))
-                 : p.m <= 16 ? (two ? launch_rows<2, 2, 8>(p, w.group, st) : launch_rows<2, 1, 8>(p, w.group, st))
-                 : p.m <= 32 ? (two ? launch_rows<4, 2, 8>(p, w.group, st) : launch_rows<4, 1, 8>(p, w.group, st))
+                 : p.m <= 16 ? (four && p.zero != nullptr && w.group == 32 ? launch_kernel<2, 4, 8, 32, true>(p, st)
+                                : four && p.zero != nullptr && w.group == 64 ? launch_kernel<2, 4, 8, 64, true>(p, st)
+                                : two ? launch_rows<2, 2, 8>(p, w.group, st) : launch_rows<2, 1, 8>(p, w.group, st))
+                 : p.m <= 32 ? (four ? launch_rows<4, 4, 8>(p, w.group, st)
+                                : two ? launch_rows<4, 2, 8>(p, w.group, st) : launch_rows<4, 1, 8>(p, w.group, st))
                              : (two ? launch_rows<8, 2, 8>(p, w.group, st) : launch_rows<8, 1, 8>(p, w.group, st));
     if (rc != B200_OK) return rc;
   }
