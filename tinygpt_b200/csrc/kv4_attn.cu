@@ -12,6 +12,7 @@
 // that holds all of an item writes its rows; parts go to the workspace (one for a CTA whose warps are all inside an item) and a second
 // kernel joins them in their order.
 #include "kv4.cuh"
+#include "kv4_steps.cuh"
 #include "tc.cuh"
 
 #include <algorithm>
@@ -20,7 +21,7 @@ namespace b200 {
 
 namespace {
 
-constexpr int kStep = 32, kAhead = 2;
+constexpr int kAhead = 2;
 constexpr float kSlack = 8.f;
 constexpr int kGrid = 148;
 
@@ -87,20 +88,18 @@ __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4Attn& p, int i, int columns) 
   s.slot = p.seqs[i];
   s.blocks = (int)(((int64_t)s.count * p.group.d + columns - 1) / columns);
   s.last = 0;
-  s.step0 = 0;
   if (s.pos >= 0 && s.slot >= 0 && s.slot < p.cache.n_seqs)
     s.last = (int)min(min((int64_t)p.cache.length[s.slot], (int64_t)s.pos + s.count), min((int64_t)p.cache.max_pages * kPage, (int64_t)(1 << 30)));
   s.last = max(s.last, 0);
-  if (p.window > 0 && s.pos >= p.window) s.step0 = min((s.pos - p.window + 1) / kStep, s.last / kStep);
-  s.steps = max((s.last + kStep - 1) / kStep - s.step0, 1);
+  const Kv4Steps steps = kv4_seq_steps(s.pos, s.last, p.window);
+  s.step0 = steps.first;
+  s.steps = steps.n;
   return s;
 }
 // The steps that a block of columns sees, from s.step0 on: the first of them, and how many (one at least).
-__device__ __forceinline__ int2 kv4_block_steps(const Kv4Attn& p, const Kv4Seq& s, int block, int columns) {
+__device__ __forceinline__ Kv4Steps kv4_block_steps(const Kv4Attn& p, const Kv4Seq& s, int block, int columns) {
   const int low = s.pos + p.group.of(block * columns), high = s.pos + p.group.of(min((block + 1) * columns, s.count * (int)p.group.d) - 1);
-  const int end = s.last > 0 ? min(s.steps, high / kStep + 1 - s.step0) : 1;
-  const int begin = p.window > 0 && low >= p.window ? max((low - p.window + 1) / kStep - s.step0, 0) : 0;
-  return make_int2(min(begin, max(end - 1, 0)), max(end - begin, 1));
+  return kv4_rows_steps(low, high, s.last, p.window, {s.step0, s.steps});
 }
 // What a sequence takes of the line.  EXACT: every block what its own columns see (a prompt's first rows see little of it, and under a window none sees all: 2 048
 // rows of 16 / 8 heads of 128 from the first token on 194 → 114 µs); else all that the sequence's rows see.
@@ -108,7 +107,7 @@ template <bool EXACT>
 __device__ __forceinline__ long long kv4_line(const Kv4Attn& p, const Kv4Seq& s, int columns) {
   if constexpr (!EXACT) return (long long)s.blocks * p.cache.kv_heads * (s.steps + kAhead);
   long long sum = 0;
-  for (int b = 0; b < s.blocks; ++b) sum += kv4_block_steps(p, s, b, columns).y + kAhead;
+  for (int b = 0; b < s.blocks; ++b) sum += kv4_block_steps(p, s, b, columns).n + kAhead;
   return sum * p.cache.kv_heads;
 }
 __device__ __forceinline__ Kv4Seq kv4_from(const Kv4Seq& s, int lane) {   // another lane's
@@ -444,7 +443,7 @@ struct Walk {
         const int of = __ffs(left) - 1;
         const Kv4Seq s = kv4_from(mine, of);
         long long sum = 0;
-        for (int b = lane; b < s.blocks; b += 32) sum += kv4_block_steps(p, s, b, columns).y + kAhead;
+        for (int b = lane; b < s.blocks; b += 32) sum += kv4_block_steps(p, s, b, columns).n + kAhead;
 #pragma unroll
         for (int x = 1; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
         if (lane == of) length = sum * p.cache.kv_heads;
@@ -475,8 +474,8 @@ struct Walk {
       const int lane = threadIdx.x % 32;
       block = 0;
       for (int first = 0; first < s.blocks; first += 32) {   // (`at` lies in a block of the sequence, unless someone writes to its length meanwhile)
-        const int2 steps = first + lane < s.blocks ? kv4_block_steps(p, s, first + lane, columns) : make_int2(0, -kAhead);
-        const int upto = (int)warp_scan((long long)(steps.y + kAhead) * (int)p.kv_heads.d, lane);
+        const Kv4Steps steps = first + lane < s.blocks ? kv4_block_steps(p, s, first + lane, columns) : Kv4Steps{0, -kAhead};
+        const int upto = (int)warp_scan((long long)(steps.n + kAhead) * (int)p.kv_heads.d, lane);
         const uint32_t before = __ballot_sync(0xffffffffu, base + upto <= at);
         if (before == 0xffffffffu) {
           base += __shfl_sync(0xffffffffu, upto, 31);
@@ -485,8 +484,8 @@ struct Walk {
         const int k = __popc(before);
         if (k > 0) base += __shfl_sync(0xffffffffu, upto, k - 1);
         block = first + k;
-        s.step0 += __shfl_sync(0xffffffffu, steps.x, k);
-        s.steps = __shfl_sync(0xffffffffu, steps.y, k);
+        s.step0 += __shfl_sync(0xffffffffu, steps.first, k);
+        s.steps = __shfl_sync(0xffffffffu, steps.n, k);
         break;
       }
     }
@@ -572,7 +571,7 @@ __device__ __forceinline__ void kv4_run(const Kv4Attn& p, const Kv4Seq& s, int h
   cols.start(p, s, col0, n_cols, c);
 
   // (steps that no column sees, in a block whose columns stand far apart from the sequence's others, are not gone over)
-  const int step0 = s.step0 + first, n_steps = s.last > 0 ? min(many, cols.at_high / kStep + 1 - step0) : 0;
+  const int step0 = s.step0 + first, n_steps = kv4_steps_end(cols.at_high, s.last, step0, many);
   const int32_t* table = p.cache.table + (int64_t)max(s.slot, 0) * p.cache.max_pages;
   auto page_of = [&](int u) {
     if (u >= n_steps) return -1;
@@ -862,8 +861,7 @@ __global__ void __launch_bounds__(Prompt<NG>::kThreads, 1) kv4_prompt_kernel(con
 
     // steps that a column of the block sees
     const int step0 = s.step0 + first, high = s.pos + p.group.of(min(block0 + S::kCols, n_cols) - 1), low = s.pos + p.group.of(block0);
-    const int begin = p.window > 0 && low >= p.window ? max((low - p.window + 1) / kStep - step0, 0) : 0;
-    const int end = s.last > 0 ? min(many, high / kStep + 1 - step0) : 0;
+    const int begin = kv4_steps_begin(low, p.window, step0), end = kv4_steps_end(high, s.last, step0, many);
     const int32_t* table = p.cache.table + (int64_t)max(s.slot, 0) * p.cache.max_pages;
     auto page_of = [&](int u) {
       if (u >= end) return -1;
