@@ -199,7 +199,8 @@ int b200_w4_dequant_bf16(void* out, const b200_w4_weight* w, void* stream);
  * reads as NaN.  `pages`: b200_kv4_page_bytes(kv_heads, dim) bytes a page, [layers][n_pages], 16-byte aligned; their inside is the library's.
  * table: the pages of every sequence in order, −1 behind them; length: its tokens; refs: how many sequences list a page (0: free).  All on the
  * device; a new cache has table −1, length and refs 0.  Calls that name sequences take `seqs` (n of them, device, at most 1 024); a number outside
- * the cache is left out, and in extend, fork and free one that stands in the list before (extend, fork: refused). */
+ * the cache is left out, and in extend, fork and free one that stands in the list before (extend, fork: refused).  What a call reads is not to be written while it
+ * runs, by calls on another stream either: the sequences' results are undefined then (but every access stays within the arrays, and every call ends). */
 typedef struct b200_kv4_cache {
   void* pages;
   int32_t* table;       /* [n_seqs][max_pages] */

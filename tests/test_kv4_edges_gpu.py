@@ -1,10 +1,13 @@
-"""The paged cache of 4-bit keys and values where it can go wrong: windows behind all of a sequence whose row of the table is full."""
+"""The paged cache of 4-bit keys and values where it can go wrong: windows behind all of a sequence whose row of the table is full, lengths that change while a
+call runs."""
+import re
+
 import pytest
 import torch
 
 import kv4_oracle as orc
 from test_kv4_gpu import Rand, dev, filled, starts_of
-from tinygpt_b200 import ops
+from tinygpt_b200 import build, ops
 
 BF16 = torch.bfloat16
 
@@ -35,3 +38,41 @@ def test_windows_behind_a_full_row(built_lib, pages, rows):
                 assert bool(((got - want).abs() <= bound).all()), (window, at, s)
                 blind = max(0, min(rows, at + rows - (length + window - 1)))
                 assert blind == 0 or not got[rows - blind:].any()
+
+
+# ------------------------------------------------------------------------------------------------- lengths that change
+def test_what_warps_meet_by_is_read_once():
+    """Another stream may write to a length while a call runs, and a warp that waits at a barrier for one that went by another length waits for good.  So the lists and
+    the lengths are read in one place, the kernel whose warps go together goes by one reading, and no barrier's threads are counted by what was read."""
+    text = (build.CSRC / "kv4_attn.cu").read_text()
+    body = text[text.index("kv4_read(const Kv4Attn& p, int i) {"):]
+    body = body[:body.index("\n}\n")]
+    for what in ("p.cache.length[", "p.pos[", "p.seqs["):
+        assert text.count(what) == body.count(what) == 1, what
+    assert text.count("kv4_seq(p, kv4_read(p, i)") == 2 and text.count("kv4_from(kv4_seq(p, kv4_read(p, i)") == 2   # of a warp: lane 0's
+    assert "EXACT ? rows[i] : kv4_read(p, i)" in text and "EXACT ? rows[lane] : kv4_read(p, lane)" in text
+    assert "bar_sync" not in text and "barrier" not in re.sub(r"//.*", "", text)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,rows,pages,heads", [(1, 1, 40, 4), (1, 1, 300, 4), (3, 1, 300, 4), (40, 1, 300, 4), (2, 60, 40, 4), (40, 60, 12, 4)])
+def test_lengths_that_change_under_a_call(built_lib, n, rows, pages, heads):
+    """Lengths that another stream writes meanwhile spoil at most what is computed: every call ends, and the next one is right."""
+    rand, dim = Rand(22), 64
+    lengths = [64 * pages - (37 * i) % 300 for i in range(n)]
+    cache, seqs, k, v = filled(rand, lengths, 1, dim, room=0)
+    q, starts, pos = rand(n * rows, heads, dim), starts_of([rows] * n), dev([l - rows for l in lengths])
+    want = ops.kv4_attention(cache, 0, q, seqs, starts, pos)
+    torch.cuda.synchronize()
+    length, other = cache.length.clone(), dev([(l * 5) // 7 for l in lengths])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(100):
+        with torch.cuda.stream(side):
+            for _ in range(4):
+                cache.length.copy_(other)
+                cache.length.copy_(length)
+        for _ in range(2):
+            ops.kv4_attention(cache, 0, q, seqs, starts, pos)
+    torch.cuda.synchronize()
+    assert torch.equal(ops.kv4_attention(cache, 0, q, seqs, starts, pos), want)

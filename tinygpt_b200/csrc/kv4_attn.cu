@@ -76,21 +76,31 @@ __device__ __forceinline__ long long warp_scan(long long v, int lane) {
   return v;
 }
 
-// A sequence of the call: its rows, the tokens they may see, its items.
-struct Kv4Seq {
-  int row0, count, pos, slot, last, step0, steps, blocks;   // tokens below `last`; steps step0 … step0 + steps − 1 (one at least)
+// A sequence of the call: its rows and the tokens below `last` that they may see.  Nothing else reads the call's lists and the lengths; who writes to them meanwhile
+// spoils results, but no two threads that meet at a barrier may go by different ones.
+struct Kv4Rows {
+  int row0, count, pos, slot, last;
 };
-__device__ __forceinline__ Kv4Seq kv4_seq(const Kv4Attn& p, int i, int columns) {
-  Kv4Seq s;
+__device__ __forceinline__ Kv4Rows kv4_read(const Kv4Attn& p, int i) {
+  Kv4Rows s;
   s.row0 = min(max(p.starts[i], 0), p.rows);
   s.count = max(min(p.starts[i + 1], p.rows) - s.row0, 0);
   s.pos = min(p.pos[i], 1 << 30);
   s.slot = p.seqs[i];
-  s.blocks = (int)(((int64_t)s.count * p.group.d + columns - 1) / columns);
   s.last = 0;
   if (s.pos >= 0 && s.slot >= 0 && s.slot < p.cache.n_seqs)
     s.last = (int)min(min((int64_t)p.cache.length[s.slot], (int64_t)s.pos + s.count), min((int64_t)p.cache.max_pages * kPage, (int64_t)(1 << 30)));
   s.last = max(s.last, 0);
+  return s;
+}
+// The same with its items: steps step0 … step0 + steps − 1 (one at least), blocks of columns.
+struct Kv4Seq : Kv4Rows {
+  int step0, steps, blocks;
+};
+__device__ __forceinline__ Kv4Seq kv4_seq(const Kv4Attn& p, const Kv4Rows& rows, int columns) {
+  Kv4Seq s;
+  static_cast<Kv4Rows&>(s) = rows;
+  s.blocks = (int)(((int64_t)s.count * p.group.d + columns - 1) / columns);
   const Kv4Steps steps = kv4_seq_steps(s.pos, s.last, p.window);
   s.step0 = steps.first;
   s.steps = steps.n;
@@ -123,14 +133,18 @@ __device__ __forceinline__ Kv4Seq kv4_from(const Kv4Seq& s, int lane) {   // ano
   return o;
 }
 // ends[i]: the line up to the end of sequence i; all of it comes back.  The call has checked that it is below 2^31 for starts that do not fall; for others it may not
-// be, and nothing is done.  All threads of a CTA of THREADS.
+// be, and nothing is done.  `rows`: the sequences, where they have been read (EXACT).  All threads of a CTA of THREADS.
 __device__ __forceinline__ int kv4_whole(long long line) { return line <= INT32_MAX ? (int)line : 0; }
 template <int THREADS, bool EXACT>
-__device__ int kv4_plan(const Kv4Attn& p, int columns, int* ends) {
+__device__ int kv4_plan(const Kv4Attn& p, int columns, int* ends, const Kv4Rows* rows) {
   __shared__ long long carry[THREADS / 32];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, each = (p.n + THREADS - 1) / THREADS, first = threadIdx.x * each;
   long long sum = 0;
-  for (int i = first; i < min(first + each, p.n); ++i) sum += kv4_line<EXACT>(p, kv4_seq(p, i, columns), columns);
+  for (int i = first; i < min(first + each, p.n); ++i) {
+    const long long length = kv4_line<EXACT>(p, kv4_seq(p, EXACT ? rows[i] : kv4_read(p, i), columns), columns);
+    ends[i] = (int)min(length, (long long)INT32_MAX);
+    sum += length;
+  }
   const long long upto = warp_scan(sum, lane);
   if (lane == 31) carry[warp] = upto;
   __syncthreads();
@@ -139,7 +153,7 @@ __device__ int kv4_plan(const Kv4Attn& p, int columns, int* ends) {
     if (w < warp) before += carry[w];
     all += carry[w];
   }
-  for (int i = first; i < min(first + each, p.n); ++i) ends[i] = (int)(before += kv4_line<EXACT>(p, kv4_seq(p, i, columns), columns));
+  for (int i = first; i < min(first + each, p.n); ++i) ends[i] = (int)(before += ends[i]);
   __syncthreads();
   return kv4_whole(all);
 }
@@ -421,22 +435,30 @@ struct Unpacked {
   __device__ __forceinline__ void values(int j, uint32_t (&a)[4]) const { keys(j, a); }
 };
 
-// A CTA's or a warp's way along the line: the sequences' ends, and one item after the other.
+// A CTA's (EXACT) or a warp's way along the line: the sequences' ends, and one item after the other.  Warps that go their way together have the sequences from one
+// reading in shared memory; those that go alone read them for themselves, and meet at no barrier that depends on what they read.
+constexpr int walk_room(bool exact) { return kKvMaxSeqs * (4 + (exact ? (int)sizeof(Kv4Rows) : 0)); }   // bytes of shared memory
 template <bool EXACT>
 struct Walk {
-  Kv4Seq mine;      // up to 32 sequences: every warp has them all in its lanes, and nobody waits for anybody
+  Kv4Seq mine;      // up to 32 sequences: every warp has them all in its lanes
   int mine_end, line, i;
   const int* ends;  // more: in shared memory
+  const Kv4Rows* rows;
   bool few;
   template <int THREADS>
   __device__ __forceinline__ void plan(const Kv4Attn& p, int columns, int* room) {
     const int lane = threadIdx.x % 32;
     few = p.n <= 32;
     ends = room;
+    rows = reinterpret_cast<const Kv4Rows*>(room + kKvMaxSeqs);
     mine = Kv4Seq{};
     mine_end = 0;
+    if constexpr (EXACT) {
+      for (int k = threadIdx.x; k < p.n; k += THREADS) reinterpret_cast<Kv4Rows*>(room + kKvMaxSeqs)[k] = kv4_read(p, k);
+      __syncthreads();
+    }
     if (few) {
-      if (lane < p.n) mine = kv4_seq(p, lane, columns);
+      if (lane < p.n) mine = kv4_seq(p, EXACT ? rows[lane] : kv4_read(p, lane), columns);
       constexpr int kAlone = EXACT ? 2 : INT32_MAX;   // blocks that a lane goes through by itself
       long long length = lane < p.n && mine.blocks <= kAlone ? kv4_line<EXACT>(p, mine, columns) : 0;
       for (uint32_t left = __ballot_sync(0xffffffffu, mine.blocks > kAlone); left != 0; left &= left - 1) {
@@ -452,7 +474,7 @@ struct Walk {
       mine_end = (int)end;
       line = kv4_whole(__shfl_sync(0xffffffffu, end, 31));
     } else {
-      line = kv4_plan<THREADS, EXACT>(p, columns, room);
+      line = kv4_plan<THREADS, EXACT>(p, columns, room, rows);
     }
   }
   __device__ __forceinline__ void seek(int n, int at, int stop) { i = !few && at < stop ? kv4_find(ends, n, at) : 0; }
@@ -468,7 +490,7 @@ struct Walk {
     } else {
       while (ends[i] <= at) ++i;
       if (i > 0) base = ends[i - 1];
-      s = kv4_seq(p, i, columns);
+      s = EXACT ? kv4_seq(p, rows[i], columns) : kv4_from(kv4_seq(p, kv4_read(p, i), columns), 0);
     }
     if constexpr (EXACT) {
       const int lane = threadIdx.x % 32;
@@ -543,11 +565,11 @@ struct Shape {
   static constexpr int kThreads = kWarps * 32;
   static constexpr bool kQInRegs = NG * NT <= 4;
   static constexpr int kQBytes = kQInRegs ? 0 : NT * NG * 2 * 512;
-  static constexpr int kRoom = 232448 - 1024 - kKvMaxSeqs * 4;
+  static constexpr int kRoom = 232448 - 1024 - walk_room(false);
   static constexpr int kStages = kWarps * (3 * kStage + kQBytes) <= kRoom ? 3 : 2;
   static constexpr int kRing = kStages * kStage > 8 * NT * (NG * 64 + 6) * 4 ? kStages * kStage : (8 * NT * (NG * 64 + 6) * 4 + 15) / 16 * 16;
   static constexpr int kOwn = kRing + kQBytes;                  // shared memory of a warp
-  static constexpr int kSmem = kWarps * kOwn + kKvMaxSeqs * 4;
+  static constexpr int kSmem = kWarps * kOwn + walk_room(false);
   static_assert(kWarps * kOwn <= kRoom, "shared memory of an SM");
 };
 
@@ -571,7 +593,7 @@ __device__ __forceinline__ void kv4_run(const Kv4Attn& p, const Kv4Seq& s, int h
   cols.start(p, s, col0, n_cols, c);
 
   // (steps that no column sees, in a block whose columns stand far apart from the sequence's others, are not gone over)
-  const int step0 = s.step0 + first, n_steps = kv4_steps_end(cols.at_high, s.last, step0, many);
+  const int step0 = s.step0 + first, n_steps = col0 < n_cols ? kv4_steps_end(cols.at_high, s.last, step0, many) : 0;
   const int32_t* table = p.cache.table + (int64_t)max(s.slot, 0) * p.cache.max_pages;
   auto page_of = [&](int u) {
     if (u >= n_steps) return -1;
@@ -641,10 +663,12 @@ __device__ __forceinline__ void kv4_run(const Kv4Attn& p, const Kv4Seq& s, int h
 
 // The parts of a CTA's first `each` warps, left in their shared memory, become one at `joined`, `wide` floats from a column to the next: a warp takes a column, a lane a
 // warp's maximum and sum.
+template <int NG>
+constexpr int kMeetWide = NG * 64 + 4;   // floats of a column there (columns on other banks)
 template <int NG, int NT>
 __device__ __forceinline__ void kv4_meet(const uint8_t* smem, int each, float* joined, int wide) {
   using S = Shape<NG, NT>;
-  constexpr int kCols = S::kCols, kWide = NG * 64 + 4;
+  constexpr int kCols = S::kCols, kWide = kMeetWide<NG>;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   for (int col = warp; col < kCols; col += each) {
     const float* of = reinterpret_cast<const float*>(smem + min(lane, each - 1) * S::kOwn) + kCols * kWide + col;
@@ -698,6 +722,8 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
   const int stop = warp < cut.each ? cut.start(me + 1) : at_line;
   if (lane == 0) p.splits[own].from = -1;
   w.seek(p.n, at_line, stop);
+  __shared__ int inside[S::kWarps];   // whether a warp has left its part here: all the CTA's warps that have a piece do, of one item, or none
+  bool left_here = false;
   while (at_line < stop) {
     w.item(p, kCols, at_line);
     const Kv4Seq& s = w.s;
@@ -719,11 +745,14 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
       cols.leave(kv4_part(p, own, first == 0, kCols), 0, kCols, kDim, r, c);
       continue;
     }
-    constexpr int kWide = kDim + 4;   // (columns on other banks)
-    cols.leave(reinterpret_cast<float*>(ring), 0, kCols, kWide, r, c);
-    named_bar_sync(1, cut.each * 32);   // every warp of the CTA that has a piece comes here, once
-    kv4_meet<NG, NT>(smem, cut.each, kv4_part(p, (int64_t)blockIdx.x * S::kWarps, 0, kCols), kDim);
+    cols.leave(reinterpret_cast<float*>(ring), 0, kCols, kMeetWide<NG>, r, c);
+    left_here = true;   // (its last item)
   }
+  if (lane == 0) inside[warp] = left_here;
+  __syncthreads();
+  bool all = warp < cut.each;
+  for (int k = 0; k < cut.each; ++k) all = all && inside[k] != 0;
+  if (all) kv4_meet<NG, NT>(smem, cut.each, kv4_part(p, (int64_t)blockIdx.x * S::kWarps, 0, kCols), kDim);
   kv4_others(p);
 }
 
@@ -732,7 +761,7 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
 template <int NG, int NT>
 struct Cluster : Shape<NG, NT> {
   using S = Shape<NG, NT>;
-  static constexpr int kWide = NG * 64 + 4, kJoined = S::kWarps * S::kOwn;      // the CTA's part, behind the warps' rings
+  static constexpr int kWide = kMeetWide<NG>, kJoined = S::kWarps * S::kOwn;      // the CTA's part, behind the warps' rings
   static constexpr int kSmem = kJoined + S::kCols * (kWide + 2) * 4;
 };
 __device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
@@ -756,16 +785,20 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_cluster_kernel
   pdl_wait();
   pdl_trigger();
   const int number = blockIdx.x / ctas, i = p.kv_heads.of(number), head = number - i * p.kv_heads.d;
-  const Kv4Seq s = kv4_seq(p, i, kCols);
+  const Kv4Seq s = kv4_from(kv4_seq(p, kv4_read(p, i), kCols), 0);
   const int n_cols = s.count * p.group.d, piece = rank * S::kWarps + warp, pieces = ctas * S::kWarps;
   const int first = (int)((int64_t)s.steps * piece / pieces), many = (int)((int64_t)s.steps * (piece + 1) / pieces) - first;
-  for (int col0 = 0; col0 < n_cols; col0 += kCols) {
+  __shared__ int blocks_here;   // of the first CTA: all of the cluster go over so many
+  int blocks = 1;
+  if (threadIdx.x == 0) blocks_here = s.blocks;
+  for (int col0 = 0, block = 0; block < blocks; ++block, col0 += kCols) {
     Columns<NG, NT> cols;
     kv4_run(p, s, head, col0, n_cols, first, many, ring, cols);
     cols.leave(reinterpret_cast<float*>(ring), 0, kCols, S::kWide, r, c);
     __syncthreads();
     kv4_meet<NG, NT>(smem, S::kWarps, joined, S::kWide);
     cluster_sync_all();
+    if (block == 0) blocks = ld_cluster_i32(mapa_u32(smem_u32(&blocks_here), 0));
     for (int col = rank + ctas * warp; col < kCols; col += ctas * S::kWarps) {
       if (col0 + col >= n_cols) break;
       const uint32_t at = smem_u32(joined + S::kCols * S::kWide + col);
@@ -816,7 +849,7 @@ struct Prompt {
   static constexpr int kCols = kWarps * 8 * kNT;
   static constexpr int kUnpacked = kTiles * 2 * NG * 4 * 512;   // of a step
   static constexpr bool kQInRegs = NG * kNT <= 4;
-  static constexpr int kSmem = kStages * kStage + 2 * kUnpacked + kKvMaxSeqs * 4;
+  static constexpr int kSmem = kStages * kStage + 2 * kUnpacked + walk_room(true);
 };
 template <int NG>
 __global__ void __launch_bounds__(Prompt<NG>::kThreads, 1) kv4_prompt_kernel(const Kv4Attn p) {
