@@ -1,5 +1,5 @@
 """The paged cache of 4-bit keys and values where it can go wrong: windows behind all of a sequence whose row of the table is full, lengths that change while a
-call runs."""
+call runs, values that are no numbers behind weights of nothing."""
 import re
 
 import pytest
@@ -76,3 +76,24 @@ def test_lengths_that_change_under_a_call(built_lib, n, rows, pages, heads):
             ops.kv4_attention(cache, 0, q, seqs, starts, pos)
     torch.cuda.synchronize()
     assert torch.equal(ops.kv4_attention(cache, 0, q, seqs, starts, pos), want)
+
+
+# ------------------------------------------------------------------------------------------------- values that are no numbers
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,room", [(1, 1), (1, 9000), (7, 1), (7, 9000), (60, 1)])   # clusters, the even cut, one and two tiles; a CTA's block
+@pytest.mark.parametrize("low", [(10, 11), (0, 32), (138, 139), (128, 160), (0, 160)])   # tokens with next to no weight: one of a step, a step, all that is in a piece
+def test_a_value_that_is_seen_counts_whatever_its_weight(built_lib, rows, room, low):
+    """A weight that is rounded to nothing makes nothing of a value that is not a number, whether the step is seen whole or in part and wherever it is joined."""
+    rand, dim, length = Rand(23), 128, 161 + rows
+    cache, seqs, k, v = filled(rand, [length], 2, dim, room=room)
+    k.zero_()
+    k[low[0]:low[1]] = -40.0
+    v[low[0], 0, 5] = float("nan")
+    ops.kv4_store(cache, 0, k, v, seqs, dev([0, length]), dev([0]))
+    q = torch.ones(rows, 4, dim, device="cuda", dtype=BF16)
+    for at in (length - rows, max(low[0] - rows // 2, 0)):
+        out = ops.kv4_attention(cache, 0, q, seqs, dev([0, rows]), dev([at])).cpu().double()
+        want, bound = orc.attention(q, orc.held(k), orc.held(v), at, dim ** -0.5, 0)
+        assert torch.equal(out.isnan(), want.isnan()) and bool(want[-1, :2, :64].isnan().all())
+        rest = ~want.isnan()
+        assert bool(((out - want).abs() <= bound)[rest].all())

@@ -335,10 +335,10 @@ struct Columns {
         for (int t = 0; t < NT; ++t) {
           float w[4] = {weight[t][0] * s0, weight[t][1] * s0, weight[t][2] * s1, weight[t][3] * s1};
           float y[4] = {m0, m0, m1, m1};
-          if constexpr (!WHOLE) {   // what is not seen may hold anything
+          if constexpr (!WHOLE) {   // what is not seen may hold anything (and what is seen counts, however small its weight)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (weight[t][e] == 0.f) w[e] = y[e] = 0.f;
+              if (sc[k][t][e] == -INFINITY) w[e] = y[e] = 0.f;
           }
           mid[g][t][0] = fmaf(weight[t][2], y[2], fmaf(weight[t][0], y[0], mid[g][t][0]));
           mid[g][t][1] = fmaf(weight[t][3], y[3], fmaf(weight[t][1], y[1], mid[g][t][1]));
@@ -677,6 +677,7 @@ __device__ __forceinline__ void kv4_meet(const uint8_t* smem, int each, float* j
 #pragma unroll
     for (int x = 1; x < 32; x <<= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, x));
     const float f = l != 0.f ? exp2_fast(m - all) : 0.f;
+    const uint32_t some = __ballot_sync(0xffffffffu, l != 0.f);   // warps that have seen a token
     l *= f;
 #pragma unroll
     for (int x = 1; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
@@ -686,7 +687,7 @@ __device__ __forceinline__ void kv4_meet(const uint8_t* smem, int each, float* j
 #pragma unroll 4
     for (int k = 0; k < each; ++k) {
       const float fk = __shfl_sync(0xffffffffu, f, k);
-      if (fk == 0.f) continue;
+      if (!(some >> k & 1)) continue;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         const float2 o2 = *reinterpret_cast<const float2*>(smem + k * S::kOwn + (col * kWide + g * 64 + 2 * lane) * 4);
@@ -807,6 +808,7 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_cluster_kernel
 #pragma unroll
       for (int x = 1; x < 32; x <<= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, x));
       const float f = l != 0.f ? exp2_fast(m - all) : 0.f;
+      const uint32_t some = __ballot_sync(0xffffffffu, l != 0.f);
       l *= f;
 #pragma unroll
       for (int x = 1; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
@@ -816,7 +818,7 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_cluster_kernel
 #pragma unroll 4
       for (int k = 0; k < ctas; ++k) {
         const float fk = __shfl_sync(0xffffffffu, f, k);
-        if (fk == 0.f) continue;
+        if (!(some >> k & 1)) continue;
         const uint32_t part = mapa_u32(smem_u32(joined + col * S::kWide + 2 * lane), k);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
