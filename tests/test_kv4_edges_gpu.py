@@ -97,3 +97,21 @@ def test_a_value_that_is_seen_counts_whatever_its_weight(built_lib, rows, room, 
         assert torch.equal(out.isnan(), want.isnan()) and bool(want[-1, :2, :64].isnan().all())
         rest = ~want.isnan()
         assert bool(((out - want).abs() <= bound)[rest].all())
+
+
+# ------------------------------------------------------------------------------------------------- calls of all kinds
+@pytest.mark.gpu
+def test_calls_without_a_sequence(built_lib):
+    """A server's step in which no sequence lives: rows belong to nobody, whichever way the call goes (contiguous tensors, others)."""
+    rand, none, start = Rand(24), dev([]), dev([0])
+    cache, seqs, k, v = filled(rand, [70, 3], 2, 64)
+    was = [t.clone() for t in (cache.pages, cache.table, cache.length, cache.refs)]
+    wide = rand(5, 4, 64)
+    for x in (wide[:, :2].contiguous(), wide[:, :2], wide.transpose(0, 1)[:2].transpose(0, 1)):
+        assert ops.kv4_store(cache, 0, x, x, none, start, none) is None
+        assert not ops.kv4_attention(cache, 0, x, none, start, none).any()
+    for rows in (0, 5):
+        got = ops.kv4_load(cache, 0, none, start, none, rows)
+        assert all(t.shape == (rows, 2, 64) and t.dtype == torch.float32 and not t.any() for t in got)
+    assert ops.kv4_extend(cache, none, none).shape == ops.kv4_fork(cache, none, none).shape == (0,) and ops.kv4_free(cache, none) is None
+    assert all(torch.equal(a, b) for a, b in zip(was, (cache.pages, cache.table, cache.length, cache.refs)))

@@ -256,8 +256,8 @@ struct Kv4Where {
   int64_t n;
   bool take(const Kv4& kv, PyObject* const* a) {
     if (!(seqs = numbers(kv, a[0]))) return false;
-    n = seqs->size(0);
-    return (starts = numbers(kv, a[1], n + 1)) && (pos = numbers(kv, a[2], n));
+    n = seqs->size(0);   // (a call without sequences launches nothing: ops.py's)
+    return n > 0 && (starts = numbers(kv, a[1], n + 1)) && (pos = numbers(kv, a[2], n));
   }
   static const int32_t* at(const at::Tensor* t) { return static_cast<const int32_t*>(t->data_ptr()); }
 };
