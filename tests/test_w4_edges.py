@@ -1,0 +1,29 @@
+"""Weights of 4 bits where they can go wrong: matrices next to the largest number."""
+import pytest
+import torch
+
+from tinygpt_b200 import ops
+from tinygpt_b200._lib import B200Error
+
+
+def unpacked(w):
+    """W of a W4Weight, in 64 bits (CPU)."""
+    tiles, blocks, groups = -(-w.n // 16), -(-w.k // 64), -(-w.k // w.group)
+    v = torch.stack((w.q & 15, w.q >> 4), -1).view(tiles, blocks, 8, 4, 2, 2, 2, 2, 2).permute(0, 8, 2, 1, 4, 3, 5, 7, 6).reshape(tiles * 16, blocks * 64)[:w.n, :w.k]
+    back = lambda t: t.permute(0, 3, 2, 1).reshape(-1, groups)[:w.n].double().repeat_interleave(w.group, 1)[:, :w.k]
+    return back(w.scale) * (v.double() - (8 if w.zero is None else back(w.zero))), back(w.scale)
+
+
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("group", [32, 128])
+def test_quantize_to_the_ends_of_fp32(symmetric, group):
+    """A group's range may pass the largest fp32 number though its entries do not."""
+    g = torch.Generator().manual_seed(5)
+    w = (torch.rand(4, 200, generator=g) * 2 - 1) * 3e38
+    w[1, :7] = 3.3e38
+    w[2] = w[2].abs()
+    w[3] = -w[3].abs()
+    got, s = unpacked(ops.w4_quantize(w, group=group, symmetric=symmetric))
+    assert bool(torch.isfinite(got).all())
+    # half a step; the range's ends lose what the scale's rounding (2^-8 of up to 15 steps) and the zero's to a whole number take: half a step more
+    assert bool(((got - w.double()).abs() <= s * (0.5 + 15 * 2.0 ** -8 + (0 if symmetric else 0.5))).all())

@@ -311,7 +311,8 @@ def w4_quantize(weight: torch.Tensor, *, group: int = 64, symmetric: bool = True
         raise B200Error("w4_quantize: the weight is not finite")
     w = w.view(n, groups, group)
     hi, lo = w.amax(-1).clamp(min=0), w.amin(-1).clamp(max=0)
-    scale = (torch.maximum(hi, -lo) / 7 if symmetric else (hi - lo) / 15).to(torch.bfloat16)
+    span = (hi - lo) / 15   # (hi − lo may pass the largest fp32 number)
+    scale = (torch.maximum(hi, -lo) / 7 if symmetric else torch.where(torch.isfinite(span), span, hi / 15 - lo / 15)).to(torch.bfloat16)
     s = scale.float().clamp(min=torch.finfo(torch.float32).tiny)[..., None]
     zero = None if symmetric else (-lo / s[..., 0]).round().clamp(0, 15)
     q = ((w / s).round() + (8 if symmetric else zero[..., None])).clamp(0, 15).to(torch.uint8)
