@@ -1,4 +1,4 @@
-"""Weights of 4 bits where they can go wrong: matrices next to the largest number."""
+"""Weights of 4 bits where they can go wrong: matrices next to the largest number, values and sizes of more bits than a layout holds."""
 import pytest
 import torch
 
@@ -27,3 +27,12 @@ def test_quantize_to_the_ends_of_fp32(symmetric, group):
     assert bool(torch.isfinite(got).all())
     # half a step; the range's ends lose what the scale's rounding (2^-8 of up to 15 steps) and the zero's to a whole number take: half a step more
     assert bool(((got - w.double()).abs() <= s * (0.5 + 15 * 2.0 ** -8 + (0 if symmetric else 0.5))).all())
+
+
+def test_pack_refuses_values_of_more_bits():
+    v, s = torch.full((16, 64), 15, dtype=torch.uint8), torch.ones(16, 1).to(torch.bfloat16)
+    assert bool((ops.w4_pack(v, s).q == 255).all())
+    for bad in (16, 255):
+        v[15, 63] = bad
+        with pytest.raises(B200Error, match="0 … 15"):
+            ops.w4_pack(v, s)

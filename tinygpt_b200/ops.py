@@ -282,8 +282,10 @@ def w4_pack(values: torch.Tensor, scale: torch.Tensor, zero: Optional[torch.Tens
     for t, name in ((scale, "scale"), (zero, "zero")):
         if t is not None and (t.dtype != torch.bfloat16 or tuple(t.shape) != (n, groups) or t.device != values.device):
             raise B200Error(f"w4_pack: {name} must be bf16 [{n}, {groups}] beside the values, got {t.dtype} {tuple(t.shape)}")
+    if int(values.max()) > 15:
+        raise B200Error(f"w4_pack: values must be 0 … 15, got {int(values.max())}")
     v = torch.full((tiles * 16, blocks * 64), 8, dtype=torch.uint8, device=values.device)
-    v[:n, :k] = values & 15
+    v[:n, :k] = values
     #                 tile  hi r  block h  c  t  p  e   →  tile, block, r, c, h, t, e, p, hi
     v = v.view(tiles, 2, 8, blocks, 2, 4, 2, 2, 2).permute(0, 3, 2, 5, 4, 6, 8, 7, 1)
     q = (v[..., 0] | v[..., 1] << 4).contiguous().view(-1)
