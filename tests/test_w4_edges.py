@@ -36,3 +36,25 @@ def test_pack_refuses_values_of_more_bits():
         v[15, 63] = bad
         with pytest.raises(B200Error, match="0 … 15"):
             ops.w4_pack(v, s)
+
+
+def test_sizes_that_a_descriptor_does_not_hold_are_refused():
+    """n, k and the group reach the library in 32 bits; a W4Weight made by hand may hold more, which must not come out as others."""
+    w = ops.w4_pack(torch.zeros(16, 128, dtype=torch.uint8), torch.ones(16, 1).to(torch.bfloat16), group=128)
+    for bad, what in ((w._replace(group=2 ** 32 + 64), "groups of"), (w._replace(group=48), "groups of"), (w._replace(group=0), "groups of"),
+                      (w._replace(n=2 ** 32 + 16), "out of range"), (w._replace(k=2 ** 32 + 128), "out of range"), (w._replace(k=-128), "out of range"),
+                      (w._replace(n=0), "out of range")):
+        for call in (ops.w4_dequantize, lambda w: ops.linear_w4(torch.zeros(1, 128, dtype=torch.bfloat16), w)):
+            with pytest.raises(B200Error, match=what):
+                call(bad)
+
+
+@pytest.mark.gpu
+def test_sizes_that_a_descriptor_does_not_hold_are_refused_on_the_device(built_lib):
+    w = ops.w4_pack(torch.zeros(16, 128, dtype=torch.uint8, device="cuda"), torch.ones(16, 1, device="cuda").to(torch.bfloat16), group=128)
+    x = torch.ones(3, 128, device="cuda", dtype=torch.bfloat16)
+    assert bool((ops.linear_w4(x, w) == -8 * 128).all())
+    for bad in (w._replace(group=2 ** 32 + 64), w._replace(group=2 ** 32 + 128), w._replace(n=2 ** 32 + 16), w._replace(k=2 ** 32 + 128)):
+        for call in (lambda: ops.linear_w4(x, bad), lambda: ops.w4_dequantize(bad)):
+            with pytest.raises(B200Error):
+                call()

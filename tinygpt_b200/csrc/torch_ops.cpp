@@ -209,7 +209,7 @@ PyObject* linear_w4(PyObject*, PyObject* const* a, Py_ssize_t n_args) {   // x, 
       !PyLong_Check(a[4]) || !PyLong_Check(a[5]) || !PyLong_Check(a[6]) || !plain_or_none(a[7], b) || x->dim() < 1)
     Py_RETURN_NONE;
   const int64_t n = whole_number(a[4]), k = whole_number(a[5]), group = whole_number(a[6]);
-  if (n < 1 || k < 1 || group < 1 || n > 16 * 65535 || k > 1 << 24 || x->size(-1) != k || x->numel() < 1 || !w4_fits(*q, *scale, zero, n, k, group) ||
+  if (n < 1 || k < 1 || (group != 32 && group != 64 && group != 128) || n > 16 * 65535 || k > 1 << 24 || x->size(-1) != k || x->numel() < 1 || !w4_fits(*q, *scale, zero, n, k, group) ||
       (b != nullptr && b->numel() != n))
     Py_RETURN_NONE;
   if (!here(*x) || q->device() != x->device() || scale->device() != x->device() || (zero && zero->device() != x->device()) || (b && b->device() != x->device()))

@@ -325,6 +325,10 @@ def _w4_desc(w: W4Weight, what: str):
     from ._lib import W4Desc
     if not isinstance(w, W4Weight):
         raise B200Error(f"{what}: the weight must come from w4_pack or w4_quantize")
+    if w.group not in W4_GROUPS:   # (the descriptor has 32 bits for each number)
+        raise B200Error(f"{what}: groups of {w.group} (one of {W4_GROUPS})")
+    if not (1 <= w.n <= 16 * 65535 and 8 <= w.k <= 1 << 24):
+        raise B200Error(f"{what}: W [{w.n}, {w.k}] out of range")
     tiles, groups = -(-w.n // 16), -(-w.k // w.group)
     q, small = _chk(w.q, f"{what}.q", torch.uint8), [None if t is None else _chk(t, f"{what}.{name}") for t, name in ((w.scale, "scale"), (w.zero, "zero"))]
     if q.numel() != tiles * -(-w.k // 64) * 512 or any(t is not None and t.numel() != tiles * groups * 16 for t in small) or small[0] is None:
@@ -349,8 +353,8 @@ def linear_w4(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = 
     if y is not None:
         check(y, "b200_w4_linear_bf16")
     import ctypes as C
-    x = _chk(x, "linear_w4.x")
     d, parts = _w4_desc(weight, "linear_w4")
+    x = _chk(x, "linear_w4.x")
     n, k = weight.n, weight.k
     if x.dim() < 1 or x.shape[-1] != k:
         raise B200Error(f"linear_w4: x {tuple(x.shape)} does not match W[{n}, {k}]")
