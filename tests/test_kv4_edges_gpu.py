@@ -8,6 +8,7 @@ import torch
 import kv4_oracle as orc
 from test_kv4_gpu import Rand, dev, filled, starts_of
 from tinygpt_b200 import build, ops
+from tinygpt_b200._lib import B200Error
 
 BF16 = torch.bfloat16
 
@@ -115,3 +116,18 @@ def test_calls_without_a_sequence(built_lib):
         assert all(t.shape == (rows, 2, 64) and t.dtype == torch.float32 and not t.any() for t in got)
     assert ops.kv4_extend(cache, none, none).shape == ops.kv4_fork(cache, none, none).shape == (0,) and ops.kv4_free(cache, none) is None
     assert all(torch.equal(a, b) for a, b in zip(was, (cache.pages, cache.table, cache.length, cache.refs)))
+
+
+@pytest.mark.gpu
+def test_numbers_past_64_bits_are_refused(built_lib):
+    """On both ways, the native one and the one that other tensors take: none of them comes out as another layer or window."""
+    rand = Rand(25)
+    cache, seqs, k, v = filled(rand, [70, 3], 2, 64)
+    where, wide = (seqs, dev([0, 1, 2]), dev([69, 2])), rand(2, 2, 64)
+    for x in (wide, wide.transpose(1, 2).contiguous().transpose(1, 2)):
+        assert ops.kv4_attention(cache, 0, x, *where, window=2 ** 62).isfinite().all()
+        for bad in (2 ** 64, 2 ** 63, -1, 2 ** 64 + 1, -2 ** 64):
+            for call in (lambda: ops.kv4_attention(cache, bad, x, *where), lambda: ops.kv4_attention(cache, 0, x, *where, window=bad),
+                         lambda: ops.kv4_store(cache, bad, x, x, *where), lambda: ops.kv4_load(cache, bad, *where, 2)):
+                with pytest.raises(B200Error):
+                    call()

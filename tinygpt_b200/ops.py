@@ -435,13 +435,15 @@ def _kv4(cache: KV4Cache, what: str, **numbers: torch.Tensor):
     return (C.byref(cache._desc), *got)
 
 
-def _kv4_where(cache, what, seqs, starts, pos):
+def _kv4_where(cache, what, layer, seqs, starts, pos):
     got = _kv4(cache, what, seqs=seqs, starts=starts, pos=pos)
     n = got[1].shape[0]
     if got[2].shape[0] != n + 1 or got[3].shape[0] != n:
         raise B200Error(f"{what}: {n} sequences take {n + 1} starts and {n} positions, got {got[2].shape[0]} and {got[3].shape[0]}")
     if n > KV4_MAX_SEQS:
         raise B200Error(f"{what}: {n} sequences in a call (at most {KV4_MAX_SEQS})")
+    if not 0 <= int(layer) < cache.layers:
+        raise B200Error(f"{what}: layer {layer} of {cache.layers}")
     return got
 
 
@@ -465,7 +467,7 @@ def kv4_store(cache: KV4Cache, layer: int, k: torch.Tensor, v: torch.Tensor, seq
         return
     if y is not None:
         check(y, "b200_kv4_store")
-    d, seqs, starts, pos = _kv4_where(cache, "kv4_store", seqs, starts, pos)
+    d, seqs, starts, pos = _kv4_where(cache, "kv4_store", layer, seqs, starts, pos)
     k, ld_k = _kv4_rows(k, "kv4_store.k", cache.kv_heads, cache.head_dim)
     v, ld_v = _kv4_rows(v, "kv4_store.v", cache.kv_heads, cache.head_dim)
     if k.shape != v.shape:
@@ -482,7 +484,7 @@ def kv4_load(cache: KV4Cache, layer: int, seqs: torch.Tensor, starts: torch.Tens
         return y
     if y is not None:
         check(y, "b200_kv4_load")
-    d, seqs, starts, pos = _kv4_where(cache, "kv4_load", seqs, starts, pos)
+    d, seqs, starts, pos = _kv4_where(cache, "kv4_load", layer, seqs, starts, pos)
     if rows < 0:
         raise B200Error(f"kv4_load: {rows} rows")
     k, v = (torch.zeros(rows, cache.kv_heads, cache.head_dim, dtype=torch.float32, device=cache.pages.device) for _ in range(2))
@@ -504,11 +506,13 @@ def kv4_attention(cache: KV4Cache, layer: int, q: torch.Tensor, seqs: torch.Tens
             return y
         if y is not None:
             check(y, "b200_kv4_attention")
-    d, seqs, starts, pos = _kv4_where(cache, "kv4_attention", seqs, starts, pos)
+    d, seqs, starts, pos = _kv4_where(cache, "kv4_attention", layer, seqs, starts, pos)
     q, ld_q = _kv4_rows(q, "kv4_attention.q", None, cache.head_dim)
     rows, heads, n = q.shape[0], q.shape[1], seqs.shape[0]
     if heads < 1 or heads % cache.kv_heads:
         raise B200Error(f"kv4_attention: {heads} query heads over {cache.kv_heads} key/value heads")
+    if not 0 <= int(window) < 1 << 63:
+        raise B200Error(f"kv4_attention: window {window}")
     if not rows or not n:
         return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
