@@ -187,7 +187,8 @@ typedef struct b200_w4_weight {
 /* y[m,n] = bf16( x[m,k]·Wᵀ + bias ), fp32 sums, one rounding.  Up to 32 rows, 64 over a small W (and any number where n is no multiple of 8), the values
  * enter the products exactly and a group's sum is scaled in fp32; more rows take W as bf16 (each weight rounded once): up to 256 rows unpacked on the way into the
  * tensor cores, more laid out in `workspace` (b200_w4_workspace_bytes(m, n, k) bytes, 16-byte aligned; 0 bytes: may be NULL) for the general GEMM.
- * Requirements: k % 8 == 0, x 16-byte aligned.  x is below 2^120 in magnitude; a row of x that is not finite gives results that are not. */
+ * Requirements: k % 8 == 0, x 16-byte aligned.  x is below 2^112 in magnitude and a zero no more than 128 (a group's 128 + value are summed before the scale and
+ * the zero meet them), the sums of |W|·|x| below 2^127; a row of x that is not finite gives results that are not. */
 int64_t b200_w4_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int b200_w4_linear_bf16(void* y, const void* x, const b200_w4_weight* w, const void* bias_or_null, int64_t m, void* workspace, void* stream);
 /* out[n,k] = bf16(W), 16-byte aligned. */
@@ -222,7 +223,9 @@ int b200_kv4_load(float* k, float* v, const b200_kv4_cache* cache, int64_t layer
 /* out [rows, q_heads, dim] = softmax(scale·q·Kᵀ) V over one layer.  q's rows are ld_q elements apart and belong to the sequences as above; row j of
  * sequence i stands at position P = pos[i] + j and sees the positions p <= P that the sequence has, with window > 0 those with P − p < window.  Query head h reads
  * key/value head h / (q_heads / kv_heads).  A row that sees nothing, or belongs to no sequence, is zero.
- * Scores, softmax and sums are fp32; weights of the values are rounded to bf16.  dim as in the cache; q and its rows 16-byte aligned, q below 2^120; scale > 0.
+ * Scores, softmax and sums are fp32; weights of the values are rounded to bf16.  dim as in the cache; q and its rows 16-byte aligned; scale > 0.  In magnitude q is below
+ * 2^112, and so is the largest |q|·|k|, with scale and without; a value times the number of tokens that a row sees is below 2^118 (weights grow to 2^8 before the
+ * running maximum moves).
  * workspace: b200_kv4_attention_workspace_bytes() bytes (0: may be NULL), 16-byte aligned, written before it is read. */
 int64_t b200_kv4_attention_workspace_bytes(const b200_kv4_cache* cache, int64_t q_heads, int64_t n, int64_t rows);
 int b200_kv4_attention(void* out, const void* q, int64_t ld_q, const b200_kv4_cache* cache, int64_t layer, int64_t q_heads, const int32_t* seqs,

@@ -131,3 +131,28 @@ def test_numbers_past_64_bits_are_refused(built_lib):
                          lambda: ops.kv4_store(cache, bad, x, x, *where), lambda: ops.kv4_load(cache, bad, *where, 2)):
                 with pytest.raises(B200Error):
                     call()
+
+
+# ------------------------------------------------------------------------------------------------- numbers up to the stated bounds
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,room", [(1, 1), (1, 9000), (7, 9000), (60, 1)])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_numbers_up_to_the_stated_bounds(built_lib, rows, room, dim):
+    """Queries of one sign just below 2^112 over keys of one sign, values of one sign whose sum over the tokens comes to 2^118 and weights that rise to almost 2^8
+    above the running maximum: everything stays finite, and right."""
+    rand, length = Rand(26), 1023
+    cache, seqs, k, v = filled(rand, [length], 1, dim, room=room)
+    up = torch.linspace(0.5, 0.96, length, device="cuda")[:, None, None] * (1 + 0.02 * torch.rand(length, 1, dim, generator=rand.g, device="cuda"))
+    k = up.to(BF16)
+    v = ((1 - 0.5 * torch.rand(length, 1, dim, generator=rand.g, device="cuda")) * 2.0 ** 108).to(BF16).clamp(max=2.0 ** 108 * (1 - 2.0 ** -8))
+    v[::2, :, :64] = v[0, :, :1]   # groups of one number beside others
+    ops.kv4_store(cache, 0, k, v, seqs, dev([0, length]), dev([0]))
+    q = torch.full((rows, 4, dim), 2.0 ** 112 * (1 - 2.0 ** -8), device="cuda").to(BF16)
+    scale = 12.0 / dim * 2.0 ** -112   # scores from 6 to some 11.6: 2^8 in weight
+    out = ops.kv4_attention(cache, 0, q, seqs, dev([0, rows]), dev([length - rows]), scale=scale).cpu().double()
+    want, bound = orc.attention(q, orc.held(k), orc.held(v), length - rows, scale, 0)
+    assert bool(torch.isfinite(out).all()) and bool(((out - want).abs() <= bound).all())
+    # and with queries of the other sign, whose scores fall
+    out = ops.kv4_attention(cache, 0, -q, seqs, dev([0, rows]), dev([length - rows]), scale=scale).cpu().double()
+    want, bound = orc.attention(-q, orc.held(k), orc.held(v), length - rows, scale, 0)
+    assert bool(torch.isfinite(out).all()) and bool(((out - want).abs() <= bound).all())

@@ -58,3 +58,24 @@ def test_sizes_that_a_descriptor_does_not_hold_are_refused_on_the_device(built_l
         for call in (lambda: ops.linear_w4(x, bad), lambda: ops.w4_dequantize(bad)):
             with pytest.raises(B200Error):
                 call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group,zero", [(32, None), (64, 128.0), (128, None), (128, 128.0), (128, -128.0), (128, 7.5)])
+@pytest.mark.parametrize("m", [1, 8, 20, 60, 100, 300])
+def test_inputs_up_to_the_stated_bound(built_lib, m, group, zero):
+    """Entries of x of one sign just below 2^112: the sums in front of a group's scale are as large as they come, the result is not."""
+    n, k = 264, 520
+    g = torch.Generator(device="cuda").manual_seed(7)
+    v = torch.randint(0, 16, (n, k), generator=g, device="cuda", dtype=torch.uint8)
+    v[:8], v[8:16] = 15, 8
+    s = ((torch.rand(n, -(-k // group), generator=g, device="cuda") + 0.5) * 2.0 ** -10).to(torch.bfloat16)
+    z = None if zero is None else torch.full_like(s, zero)
+    x = ((1 - torch.rand(m, k, generator=g, device="cuda") * 0.25) * 2.0 ** 112).to(torch.bfloat16).clamp(max=2.0 ** 112 * (1 - 2.0 ** -8))
+    x[m // 2] = -x[m // 2]
+    y = ops.linear_w4(x, ops.w4_pack(v, s, z, group=group)).double()
+    full = s.double().repeat_interleave(group, 1)[:, :k] * (v.double() - (8 if zero is None else zero))
+    # half a step of the result; fp32 sums of k terms, each no more than (128 + 15 + |zero|) scales; beyond the exact way a weight's rounding
+    size = x.double().abs() @ (s.double().repeat_interleave(group, 1)[:, :k] * (143 + abs(zero or 8))).t()
+    bound = (x.double() @ full.t()).abs() * 2.0 ** -8 + size * k * 2.0 ** -23 + (x.double().abs() @ full.abs().t() * 2.0 ** -9 if m > 64 else 0)
+    assert bool(torch.isfinite(y).all()) and bool(((y - x.double() @ full.t()).abs() <= bound).all())
