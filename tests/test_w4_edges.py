@@ -79,3 +79,56 @@ def test_inputs_up_to_the_stated_bound(built_lib, m, group, zero):
     size = x.double().abs() @ (s.double().repeat_interleave(group, 1)[:, :k] * (143 + abs(zero or 8))).t()
     bound = (x.double() @ full.t()).abs() * 2.0 ** -8 + size * k * 2.0 ** -23 + (x.double().abs() @ full.abs().t() * 2.0 ** -9 if m > 64 else 0)
     assert bool(torch.isfinite(y).all()) and bool(((y - x.double() @ full.t()).abs() <= bound).all())
+
+
+# ------------------------------------------------------------------------------------------------- sums that are exact
+def whole_numbers(n, k, group, zero, seed=9, device="cuda"):
+    """A weight of values times powers of two from 1/2 to 2, zeros whole and halves: exact as bf16, and so is every sum over it of whole numbers x in fp32 (8 200 columns of
+    at most 3·(128 + 15)·2, and 3·(128 + 15)·2 beside them for the zeros, in halves: below 2^24 by far, and so in every order)."""
+    g = torch.Generator(device=device).manual_seed(seed)
+    v = torch.randint(0, 16, (n, k), generator=g, device=device, dtype=torch.uint8)
+    shape = (n, -(-k // group))
+    s = torch.exp2(torch.randint(-1, 2, shape, generator=g, device=device).float()).to(torch.bfloat16)
+    z = None
+    if zero:
+        z = torch.randint(0, 16, shape, generator=g, device=device).float()
+        z[n // 2:] += 0.5 * torch.randint(0, 2, (n - n // 2, shape[1]), generator=g, device=device)
+        z = z.to(torch.bfloat16)
+    full = s.double().repeat_interleave(group, 1)[:, :k] * (v.double() - (8 if z is None else z.double().repeat_interleave(group, 1)[:, :k]))
+    return ops.w4_pack(v, s, z, group=group), full, g
+
+
+def rows_of(m, k, g):
+    return torch.randint(-3, 4, (m, k), generator=g, device=g.device).to(torch.bfloat16)
+
+
+SIZES = [(1032, 8200), (24, 4096), (4104, 2056), (8200, 1000), (20008, 512), (28672, 264), (999, 520), (40, 8)]
+
+
+@pytest.mark.parametrize("n,k", [(1032, 8200), (24, 4096), (200, 2056)])
+@pytest.mark.parametrize("zero", [False, True])
+def test_no_lost_columns_pass(n, k, zero):
+    """Eight columns, a stage of 128 or the share of one of eight CTAs, lost or counted twice, move results that have to be equal, of every row."""
+    _, full, g = whole_numbers(n, k, 64, zero, device="cpu")
+    x = rows_of(40, k, g).double()
+    want = (x @ full.t()).to(torch.bfloat16)
+    for first, many in ((0, 8), (k - 8, 8), (0, 128), (k // 256 * 128, 128), (k - k % 128 if k % 128 else k - 128, 128), (k // 8 * 3, k // 8)):
+        lost = x.clone()
+        lost[:, first:first + many] = 0
+        for bad in (lost, 2 * x - lost):
+            assert bool(((bad @ full.t()).to(torch.bfloat16) != want).any(1).all()), (first, many)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group,zero", [(32, False), (32, True), (64, False), (64, True), (128, False), (128, True)])
+@pytest.mark.parametrize("n,k", SIZES)
+def test_whole_numbers_are_exact(built_lib, n, k, group, zero):
+    """Every way, at every number of rows around its ends: nothing but the result is rounded, so that every column counts once."""
+    w, full, g = whole_numbers(n, k, group, zero)
+    bias = torch.randint(-64, 65, (n,), generator=g, device="cuda").to(torch.bfloat16)
+    assert torch.equal(ops.w4_dequantize(w).double(), full)
+    for m in (1, 2, 8, 9, 16, 17, 24, 32, 33, 40, 64, 65, 80, 100, 128, 129, 200, 256, 257, 300):
+        x = rows_of(m, k, g)
+        want = x.double() @ full.t()
+        assert torch.equal(ops.linear_w4(x, w), want.to(torch.bfloat16)), m
+        assert torch.equal(ops.linear_w4(x, w, bias), (want + bias.double()).to(torch.bfloat16)), m
