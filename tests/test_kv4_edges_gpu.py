@@ -156,3 +156,16 @@ def test_numbers_up_to_the_stated_bounds(built_lib, rows, room, dim):
     out = ops.kv4_attention(cache, 0, -q, seqs, dev([0, rows]), dev([length - rows]), scale=scale).cpu().double()
     want, bound = orc.attention(-q, orc.held(k), orc.held(v), length - rows, scale, 0)
     assert bool(torch.isfinite(out).all()) and bool(((out - want).abs() <= bound).all())
+
+
+def test_parts_of_a_cache_are_checked(built_lib):
+    """A cache put together from tensors at hand: kernels take its sizes from them, so what does not fit is refused."""
+    page = 2 * 64 * (64 // 2 + 4)
+    ok = dict(pages=torch.empty(1, 4, page, dtype=torch.uint8), table=torch.zeros(2, 3, dtype=torch.int32), length=torch.zeros(2, dtype=torch.int32),
+              refs=torch.zeros(4, dtype=torch.int32), kv_heads=1, head_dim=64)
+    for bad, what in ((dict(pages=ok["pages"].float()), "pages"), (dict(pages=ok["pages"][0]), "pages"), (dict(pages=ok["pages"][..., :-1]), "pages"),
+                      (dict(table=ok["table"].long()), "table"), (dict(table=ok["table"].t()), "table"), (dict(table=ok["table"][0]), "table"),
+                      (dict(length=ok["length"][:1]), "length"), (dict(refs=ok["refs"][:3]), "refs"), (dict(refs=ok["refs"].float()), "refs"),
+                      (dict(head_dim=128), "pages"), (dict(head_dim=32), "heads"), (dict(kv_heads=0), "heads"), ({}, "CUDA device")):
+        with pytest.raises(B200Error, match=what):
+            ops.KV4Cache(**{**ok, **bad})

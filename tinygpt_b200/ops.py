@@ -394,11 +394,22 @@ class KV4Cache:
     def __init__(self, pages, table, length, refs, kv_heads, head_dim):
         import ctypes as C
         from ._lib import KV4Desc
+        page = lib().b200_kv4_page_bytes(kv_heads, head_dim)
+        if page < 0:
+            raise B200Error(f"KV4Cache: {kv_heads} heads of {head_dim} (64, 128, 192 or 256)")
+        layers, n_pages = pages.shape[:2] if pages.dim() == 3 else (1, 1)
+        n_seqs, max_pages = table.shape if table.dim() == 2 else (1, 1)
+        for t, name, dtype, shape in ((pages, "pages", torch.uint8, (layers, n_pages, page)),
+                                      (table, "table", torch.int32, (n_seqs, max_pages)),
+                                      (length, "length", torch.int32, (n_seqs,)), (refs, "refs", torch.int32, (n_pages,))):
+            if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device != pages.device or t.numel() == 0:
+                raise B200Error(f"KV4Cache: {name} must be contiguous {dtype} {shape} beside the pages, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        if not pages.is_cuda:
+            raise B200Error("KV4Cache: the cache must live on a CUDA device (there is no CPU path)")
         put = lambda **kw: [object.__setattr__(self, name, value) for name, value in kw.items()]
-        put(pages=pages, table=table, length=length, refs=refs, layers=pages.shape[0], n_pages=pages.shape[1], n_seqs=table.shape[0],
-            max_pages=table.shape[1], kv_heads=kv_heads, head_dim=head_dim)
-        put(_desc=KV4Desc(pages.data_ptr(), table.data_ptr(), length.data_ptr(), refs.data_ptr(), self.layers, self.n_pages, self.n_seqs, self.max_pages,
-                          kv_heads, head_dim))
+        put(pages=pages, table=table, length=length, refs=refs, layers=layers, n_pages=n_pages, n_seqs=n_seqs, max_pages=max_pages, kv_heads=kv_heads,
+            head_dim=head_dim)
+        put(_desc=KV4Desc(pages.data_ptr(), table.data_ptr(), length.data_ptr(), refs.data_ptr(), layers, n_pages, n_seqs, max_pages, kv_heads, head_dim))
         put(_at=(C.addressof(self._desc), pages.device.index))
 
     def __setattr__(self, name, value):   # kernels hold the tensors' addresses
