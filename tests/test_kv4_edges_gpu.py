@@ -50,8 +50,10 @@ def test_what_warps_meet_by_is_read_once():
     body = body[:body.index("\n}\n")]
     for what in ("p.cache.length[", "p.pos[", "p.seqs["):
         assert text.count(what) == body.count(what) == 1, what
-    assert text.count("kv4_seq(p, kv4_read(p, i)") == 2 and text.count("kv4_from(kv4_seq(p, kv4_read(p, i)") == 2   # of a warp: lane 0's
-    assert "EXACT ? rows[i] : kv4_read(p, i)" in text and "EXACT ? rows[lane] : kv4_read(p, lane)" in text
+    # kv4_read by a thread of the plan, into shared memory, by a lane for its warp, and of lane 0 for a warp
+    for what in ("EXACT ? rows[i] : kv4_read(p, i)", "[k] = kv4_read(p, k)", "EXACT ? rows[lane] : kv4_read(p, lane)", "kv4_read_warp(const Kv4Attn& p, int i) {"):
+        assert text.count(what) == 1, what
+    assert text.count("kv4_read(p, ") == 4 and text.count("kv4_read_warp(p, ") == 2
     assert "bar_sync" not in text and "barrier" not in re.sub(r"//.*", "", text)
 
 

@@ -93,6 +93,16 @@ __device__ __forceinline__ Kv4Rows kv4_read(const Kv4Attn& p, int i) {
   s.last = max(s.last, 0);
   return s;
 }
+__device__ __forceinline__ Kv4Rows kv4_read_warp(const Kv4Attn& p, int i) {   // lane 0's reading, for a warp
+  const Kv4Rows s = kv4_read(p, i);
+  Kv4Rows o;
+  o.row0 = __shfl_sync(0xffffffffu, s.row0, 0);
+  o.count = __shfl_sync(0xffffffffu, s.count, 0);
+  o.pos = __shfl_sync(0xffffffffu, s.pos, 0);
+  o.slot = __shfl_sync(0xffffffffu, s.slot, 0);
+  o.last = __shfl_sync(0xffffffffu, s.last, 0);
+  return o;
+}
 // The same with its items: steps step0 … step0 + steps − 1 (one at least), blocks of columns.
 struct Kv4Seq : Kv4Rows {
   int step0, steps, blocks;
@@ -490,7 +500,7 @@ struct Walk {
     } else {
       while (ends[i] <= at) ++i;
       if (i > 0) base = ends[i - 1];
-      s = EXACT ? kv4_seq(p, rows[i], columns) : kv4_from(kv4_seq(p, kv4_read(p, i), columns), 0);
+      s = kv4_seq(p, EXACT ? rows[i] : kv4_read_warp(p, i), columns);
     }
     if constexpr (EXACT) {
       const int lane = threadIdx.x % 32;
@@ -723,8 +733,7 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
   const int stop = warp < cut.each ? cut.start(me + 1) : at_line;
   if (lane == 0) p.splits[own].from = -1;
   w.seek(p.n, at_line, stop);
-  __shared__ int inside[S::kWarps];   // whether a warp has left its part here: all the CTA's warps that have a piece do, of one item, or none
-  bool left_here = false;
+  bool left_here = false;   // all the CTA's warps that have a piece leave their part here, of one item, or none does
   while (at_line < stop) {
     w.item(p, kCols, at_line);
     const Kv4Seq& s = w.s;
@@ -749,11 +758,7 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
     cols.leave(reinterpret_cast<float*>(ring), 0, kCols, kMeetWide<NG>, r, c);
     left_here = true;   // (its last item)
   }
-  if (lane == 0) inside[warp] = left_here;
-  __syncthreads();
-  bool all = warp < cut.each;
-  for (int k = 0; k < cut.each; ++k) all = all && inside[k] != 0;
-  if (all) kv4_meet<NG, NT>(smem, cut.each, kv4_part(p, (int64_t)blockIdx.x * S::kWarps, 0, kCols), kDim);
+  if (__syncthreads_and(left_here || warp >= cut.each) && warp < cut.each) kv4_meet<NG, NT>(smem, cut.each, kv4_part(p, (int64_t)blockIdx.x * S::kWarps, 0, kCols), kDim);
   kv4_others(p);
 }
 
@@ -786,7 +791,7 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_cluster_kernel
   pdl_wait();
   pdl_trigger();
   const int number = blockIdx.x / ctas, i = p.kv_heads.of(number), head = number - i * p.kv_heads.d;
-  const Kv4Seq s = kv4_from(kv4_seq(p, kv4_read(p, i), kCols), 0);
+  const Kv4Seq s = kv4_seq(p, kv4_read_warp(p, i), kCols);
   const int n_cols = s.count * p.group.d, piece = rank * S::kWarps + warp, pieces = ctas * S::kWarps;
   const int first = (int)((int64_t)s.steps * piece / pieces), many = (int)((int64_t)s.steps * (piece + 1) / pieces) - first;
   __shared__ int blocks_here;   // of the first CTA: all of the cluster go over so many
