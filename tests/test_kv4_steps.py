@@ -63,3 +63,22 @@ def test_steps_stay_within_the_table(tmp_path):
     subprocess.run(["g++", "-std=c++17", "-O1", "-I", str(build.CSRC), str(tmp_path / "main.cpp"), "-o", str(exe)], check=True)
     r = subprocess.run([str(exe)], capture_output=True, text=True)
     assert r.returncode == 0 and int(r.stdout) > 100000, r.stdout
+
+
+def test_a_cluster_does_not_take_many_blocks_in_turn(built_lib):
+    """A cluster goes over a sequence's blocks one after the other, so a call goes to clusters (no workspace) only where the one that may bring most rows has few."""
+    import ctypes as C
+
+    from tinygpt_b200._lib import KV4Desc, lib
+
+    def clusters(heads, kv_heads, dim, max_pages, n, rows):
+        cache = KV4Desc(None, None, None, None, 1, 4096, n, max_pages, kv_heads, dim)
+        return lib().b200_kv4_attention_workspace_bytes(C.byref(cache), heads, n, rows) == 0
+
+    # one token a sequence, small caches: as many columns as the group has
+    assert clusters(14, 2, 64, 1, 2, 2) and clusters(4, 4, 128, 13, 32, 32) and clusters(24, 8, 128, 63, 1, 1) and clusters(32, 4, 64, 7, 18, 18)
+    assert clusters(4, 2, 64, 6, 5, 8)
+    # 32 tokens beside a piece of 800 rows, and of 500 beside four, whose average is few columns
+    assert not clusters(4, 4, 128, 13, 33, 832) and not clusters(2, 2, 64, 13, 20, 519)
+    # larger tables are cut evenly
+    assert not clusters(24, 8, 128, 512, 1, 1)

@@ -1079,7 +1079,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn
 // hold is no more than some three steps above what the even cut would give it (µs, clusters / even cut, one sequence of 24 / 8 heads of 128: 1 000 tokens
 // 7.2 / 10.5, 4 000 9.0 / 11.4, 12 000 14.0 / 13.2; 14 / 2 heads of 64: 1 000 6.5 / 8.8, 4 000 7.5 / 10.2, 16 000 9.9 / 11.8; 32 / 4 heads of 128: 8 000 9.9 / 12.3,
 // 32 768 18.4 / 18.7).  As large a cluster as the SMs hold all of at once: of 16 CTAs 7, of 8 15, of 4 33 (36 / 6 heads of 128, 12 000
-// tokens: clusters of 16 11.0, of 10 13.0; 24 / 8 heads, 4 000 tokens, where eight clusters of 16 are two rounds: 15.9).
+// tokens: clusters of 16 11.0, of 10 13.0; 24 / 8 heads, 4 000 tokens, where eight clusters of 16 are two rounds: 15.9).  A cluster goes over its sequence's blocks of columns
+// in turn, so both shares count once for every block of the sequence that may bring most rows, the others bringing one each (32 tokens beside a piece of 800 rows, 4 / 4 heads
+// of 128 over 832 tokens: clusters 434, even cut 31).
 struct Way {
   int tiles, columns, warps, cluster;   // tiles of a warp (0: the CTA's way), columns of a block, pieces of the line to a CTA; CTAs of a cluster (0: none)
 };
@@ -1090,7 +1092,8 @@ Way kv4_way(int64_t group, int64_t n, int64_t rows, const b200_kv4_cache& cache)
   int ctas = items <= 6 ? 16 : items <= 15 ? 8 : items <= 33 ? 4 : items <= 74 ? 2 : items <= kGrid ? 1 : 0;   // (that the SMs hold at once)
   const double steps = (double)cache.max_pages * (kPage / kStep);
   while (ctas > 1 && ctas / 2 * kPieceWarps >= steps) ctas /= 2;   // no more than a warp for every step
-  if (ctas > 0 && steps * (1.0 / (ctas * kPieceWarps) - (double)cache.kv_heads / (kGrid * kPieceWarps)) <= 3.2) return {tiles, 8 * tiles, 0, ctas};
+  const int64_t blocks = (group * std::max<int64_t>(rows - n + 1, 1) + 8 * tiles - 1) / (8 * tiles);
+  if (ctas > 0 && (double)blocks * steps * (1.0 / (ctas * kPieceWarps) - (double)cache.kv_heads / (kGrid * kPieceWarps)) <= 3.2) return {tiles, 8 * tiles, 0, ctas};
   return {tiles, 8 * tiles, kPieceWarps, 0};
 }
 
