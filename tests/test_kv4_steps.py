@@ -1,5 +1,6 @@
-"""Which steps of 32 tokens the attention over the paged 4-bit cache goes over (csrc/kv4_steps.cuh, compiled for the host): none lies behind what a sequence has, also
-where a window lies behind all of it and the table's row is full, and every token that a row sees is in one of them."""
+"""Which steps of 32 tokens the attention over the paged 4-bit cache goes over and how the line of them is cut (csrc/kv4_steps.cuh, compiled for the host): no step lies behind
+what a sequence has, also where a window lies behind all of it and the table's row is full, every token that a row sees is in one of them, every step is gone over once, and
+every search ends."""
 import subprocess
 
 from tinygpt_b200 import build
@@ -82,3 +83,127 @@ def test_a_cluster_does_not_take_many_blocks_in_turn(built_lib):
     assert not clusters(4, 4, 128, 13, 33, 832) and not clusters(2, 2, 64, 13, 20, 519)
     # larger tables are cut evenly
     assert not clusters(24, 8, 128, 512, 1, 1)
+
+
+CUT = """
+#include <algorithm>
+#include <cstdio>
+#include <map>
+#include <random>
+#include <vector>
+#include "kv4_steps.cuh"
+using namespace b200;
+struct Seq { int blocks, steps[2]; };   // steps as one reading or another finds them
+#define NEED(cond) do { if (!(cond)) { printf("line %d: %s\\\\n", __LINE__, #cond); return 1; } } while (0)
+static int walk(std::mt19937& rng, const std::vector<Seq>& seqs, int heads, int most, bool same) {
+  const int n = (int)seqs.size();
+  auto reading = [&] { return same ? 0 : (int)(rng() % 2); };
+  std::map<long long, int> left;             // place of a part -> item
+  std::map<int, std::vector<int>> covered;   // item -> how often each step
+  std::map<int, int> many_left;
+  struct Join { Kv4Pieces p; int item; };
+  std::vector<Join> joins;
+  auto id = [&](int i, int number) { int k = number; for (int j = 0; j < i; ++j) k += seqs[j].blocks * heads; return k; };
+  for (int cta = 0; cta < kGrid; ++cta) {
+    std::vector<int> ends(n);
+    int line = 0;
+    for (int i = 0; i < n; ++i) ends[i] = line += seqs[i].blocks * heads * (seqs[i].steps[reading()] + kAhead);
+    const Kv4Cut cut(line, most);
+    NEED(cut.each >= 1 && cut.each <= most && cut.start(0) == 0 && cut.start(cut.warps) == line);
+    int here = 0, inside_item = -1;
+    for (int warp = 0; warp < most; ++warp) {
+      const int me = cta * cut.each + warp;
+      int at = cut.start(me);
+      const int stop = warp < cut.each ? cut.start(me + 1) : at;
+      NEED(at <= stop && stop <= line);
+      for (int i = 0; at < stop;) {
+        while (ends[i] <= at) ++i;
+        const int base = i > 0 ? ends[i - 1] : 0, steps = seqs[i].steps[reading()];
+        const Kv4Item item = kv4_item(at, base, ends[i], steps);
+        NEED(item.number >= 0 && item.end > at && item.end <= line);
+        const int first = std::max(at - item.begin, 0), many = std::min(stop, item.end) - item.begin - first;
+        at = std::min(stop, item.end);
+        if (many <= 0) continue;
+        NEED(first >= 0 && first + many <= steps);
+        const int which = same ? id(i, item.number) : 0;
+        if (same) {
+          auto& c = covered[which];
+          c.resize(steps);
+          for (int s = first; s < first + many; ++s) ++c[s];
+        }
+        if (many == steps) continue;
+        if (first == 0) {
+          const Kv4Pieces p = kv4_pieces(cut, cta, me, item.begin, item.end);
+          NEED(p.from >= 0 && p.from <= p.to && p.to < cut.warps && p.before >= 0 && p.whole >= 0 && p.parts >= 1 && p.parts <= cut.warps);
+          for (int k = 0; k < p.parts; ++k) NEED(p.piece(k) >= p.from && p.piece(k) <= p.to && p.piece(k) / p.each < kGrid && p.piece(k) % p.each < most);
+          joins.push_back({p, which});
+        }
+        if (!kv4_inside(cut, cta, item.begin, item.end)) {
+          if (same) {
+            const long long place = ((long long)cta * most + warp) * 2 + (first == 0);
+            NEED(!left.count(place));
+            left[place] = which;
+            ++many_left[which];
+          }
+          continue;
+        }
+        NEED(at == stop);   // its last item
+        ++here;
+        if (same) {
+          NEED(inside_item < 0 || inside_item == which);
+          inside_item = which;
+        }
+      }
+    }
+    if (same) {
+      NEED(here == 0 || here == cut.each);   // all of them meet or none
+      if (here > 0) {
+        left[(long long)cta * most * 2] = inside_item;
+        ++many_left[inside_item];
+      }
+    }
+  }
+  if (!same) return 0;
+  int items = 0;
+  for (const Seq& s : seqs) items += s.blocks * heads;
+  NEED((int)covered.size() == items);
+  for (auto& c : covered)
+    for (int v : c.second) NEED(v == 1);
+  NEED(joins.size() == many_left.size());
+  for (const Join& j : joins) {   // the parts that are joined are those that were left
+    NEED(j.p.parts == many_left[j.item]);
+    for (int k = 0; k < j.p.parts; ++k) {
+      const int w = j.p.piece(k);
+      const long long place = ((long long)(w / j.p.each) * most + w % j.p.each) * 2 + (k < j.p.before && k == 0);
+      NEED(left.count(place) && left[place] == j.item);
+      left.erase(place);
+    }
+  }
+  NEED(left.empty());
+  return 0;
+}
+int main() {
+  std::mt19937 rng(1);
+  for (int round = 0; round < 400; ++round) {
+    const int n = 1 + rng() % (round % 3 ? 5 : 70), heads = 1 + rng() % 8, top = 1 << rng() % 11;
+    std::vector<Seq> seqs(n);
+    for (Seq& s : seqs) s = {(int)(rng() % (round % 4 ? 2 : 20) + (round % 5 > 0)), {(int)(1 + rng() % top), (int)(1 + rng() % top)}};
+    for (int most : {1, 8}) {
+      if (walk(rng, seqs, heads, most, true)) return printf("round %d, one reading\\\\n", round), 1;
+      for (int k = 0; k < 3; ++k)
+        if (walk(rng, seqs, heads, most, false)) return printf("round %d, changing lengths\\\\n", round), 1;
+    }
+  }
+  return 0;
+}
+"""
+
+
+def test_the_line_is_cut_and_joined(tmp_path):
+    """Every step of every item is gone over once and every part that is left is joined, in one part a CTA or a warp; and where every reading of a sequence finds another
+    length, as it may if another stream writes to it meanwhile, all searches end and all places lie where they may."""
+    (tmp_path / "main.cpp").write_text(CUT.replace("\\\\n", "\\n"))
+    exe = tmp_path / "main"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-I", str(build.CSRC), str(tmp_path / "main.cpp"), "-o", str(exe)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0, r.stdout

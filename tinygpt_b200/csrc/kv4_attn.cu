@@ -21,9 +21,7 @@ namespace b200 {
 
 namespace {
 
-constexpr int kAhead = 2;
 constexpr float kSlack = 8.f;
-constexpr int kGrid = 148;
 
 // Division by a number that the host knows (Granlund and Montgomery): a multiplication and two shifts
 struct Divisor {
@@ -176,28 +174,13 @@ __device__ __forceinline__ int kv4_find(const int* ends, int n, int at) {   // t
   }
   return lo;
 }
-// How the line is cut: `warps` pieces, `each` CTA having so many of them; piece w starts at about line·w / warps (as fp32 has it: the same for everyone).  A piece is no shorter than a step and what
-// comes before it, and short lines are spread over the CTAs first.
-struct Cut {
-  int line, warps, each, whole, rest;   // line = whole·warps + rest
-  float inverse;
-  __device__ Cut(int line_, int most) : line(line_) {
-    warps = min(max(line / (kAhead + 1), 1), kGrid * most);
-    each = (warps + kGrid - 1) / kGrid;
-    inverse = __frcp_rn((float)warps);
-    whole = line / warps;
-    rest = line - whole * warps;
-  }
-  __device__ __forceinline__ int start(int w) const { return w < warps ? w * whole + (int)((float)(w * rest) * inverse) : line; }
-};
 // a warp's parts: of an item that came before it (0) and of one that goes on behind it (1).  [column][dim], maxima, sums
 __device__ __forceinline__ float* kv4_part(const Kv4Attn& p, int64_t warp, int which, int columns) {
   return p.parts + (warp * 2 + which) * columns * (p.cache.dim + 2);
 }
-// An item that its first warp does not finish, for the kernel that joins the parts: the warps that hold it, of those the ones that left one part for their CTA.
-struct Kv4Split {
-  int from, to, in0, in1;   // warps from … to; CTAs in0 … in1 − 1 (none: in0 >= in1)
-  int row0, col0, n_cols, head, each;   // from < 0: none
+// An item that its first warp does not finish, for the kernel that joins the parts: the pieces that hold it, its columns.
+struct Kv4Split : Kv4Pieces {
+  int row0, col0, n_cols, head;
 };
 
 // What a warp keeps of its 8·NT columns while it goes over the tokens: lane 4r + c has columns 2c, 2c + 1 of every tile.
@@ -492,14 +475,16 @@ struct Walk {
   Kv4Seq s;
   int head, block, begin, end;
   __device__ __forceinline__ void item(const Kv4Attn& p, int columns, int at) {
-    int base = 0;
+    int base = 0, limit;
     if (few) {
       i = __popc(__ballot_sync(0xffffffffu, mine_end <= at));
       if (i > 0) base = __shfl_sync(0xffffffffu, mine_end, i - 1);
+      limit = __shfl_sync(0xffffffffu, mine_end, i);
       s = kv4_from(mine, i);
     } else {
       while (ends[i] <= at) ++i;
       if (i > 0) base = ends[i - 1];
+      limit = ends[i];
       s = kv4_seq(p, EXACT ? rows[i] : kv4_read_warp(p, i), columns);
     }
     if constexpr (EXACT) {
@@ -521,39 +506,25 @@ struct Walk {
         break;
       }
     }
-    const int length = s.steps + kAhead;
-    int number = (int)((float)(at - base) * __frcp_rn((float)length));   // (a division costs more than these)
-    while (number * length > at - base) --number;
-    while ((number + 1) * length <= at - base) ++number;
+    const Kv4Item item = kv4_item(at, base, limit, s.steps);
     if constexpr (EXACT) {
-      head = min(number, (int)p.kv_heads.d - 1);
+      head = min(item.number, (int)p.kv_heads.d - 1);
     } else {
-      block = p.kv_heads.of(number);
-      head = number - block * p.kv_heads.d;
+      block = p.kv_heads.of(item.number);
+      head = item.number - block * p.kv_heads.d;
     }
-    begin = base + number * length + kAhead;
-    end = begin + s.steps;
+    begin = item.begin;
+    end = item.end;
   }
 };
 template <bool EXACT>
-__device__ __forceinline__ void kv4_split(const Kv4Attn& p, const Walk<EXACT>& w, const Cut& cut, int64_t own, int me, int col0, int n_cols) {
-  auto warp_at = [&](int x) {   // whose piece of the line x is
-    int v = min(x / cut.whole, cut.warps - 1);
-    while (cut.start(v) > x) --v;
-    while (cut.start(v + 1) <= x) ++v;
-    return v;
-  };
+__device__ __forceinline__ void kv4_split(const Kv4Attn& p, const Walk<EXACT>& w, const Kv4Cut& cut, int64_t own, int me, int col0, int n_cols) {
   Kv4Split split;
-  split.from = me;
-  split.to = warp_at(w.end - 1);
-  split.in0 = cut.start(blockIdx.x * cut.each) == w.begin ? blockIdx.x : blockIdx.x + 1;
-  split.in1 = cut.start(split.to + 1) == w.end && (split.to + 1) % cut.each == 0 ? (split.to + 1) / cut.each : split.to / cut.each;
-  if (cut.each == 1) split.in1 = split.in0;
+  static_cast<Kv4Pieces&>(split) = kv4_pieces(cut, blockIdx.x, me, w.begin, w.end);
   split.row0 = w.s.row0;
   split.col0 = col0;
   split.n_cols = n_cols;
   split.head = w.head;
-  split.each = cut.each;
   p.splits[own] = split;
 }
 // rows of no sequence are zero
@@ -726,7 +697,7 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
 
   Walk<false> w{};
   w.template plan<S::kThreads>(p, kCols, reinterpret_cast<int*>(smem + S::kWarps * S::kOwn));
-  const Cut cut(w.line, S::kWarps);
+  const Kv4Cut cut(w.line, S::kWarps);
   const int me = blockIdx.x * cut.each + warp;
   const int64_t own = (int64_t)blockIdx.x * S::kWarps + warp;   // of the workspace's places
   int at_line = cut.start(me);
@@ -750,8 +721,7 @@ __global__ void __launch_bounds__(Shape<NG, NT>::kThreads, 1) kv4_attn_kernel(co
     }
     if (first == 0 && lane == 0) kv4_split(p, w, cut, own, me, col0, n_cols);
     // all the CTA's warps have a piece, and of this item alone
-    const int cta = cut.start(blockIdx.x * cut.each), cta_end = cut.start((blockIdx.x + 1) * cut.each);
-    if (cut.each == 1 || cta < w.begin || cta_end > w.end || ((int)blockIdx.x + 1) * cut.each > cut.warps) {
+    if (!kv4_inside(cut, blockIdx.x, w.begin, w.end)) {
       cols.leave(kv4_part(p, own, first == 0, kCols), 0, kCols, kDim, r, c);
       continue;
     }
@@ -872,7 +842,7 @@ __global__ void __launch_bounds__(Prompt<NG>::kThreads, 1) kv4_prompt_kernel(con
 
   Walk<true> w{};
   w.template plan<S::kThreads>(p, S::kCols, reinterpret_cast<int*>(smem + S::kStages * S::kStage + 2 * S::kUnpacked));
-  const Cut cut(w.line, 1);
+  const Kv4Cut cut(w.line, 1);
   int at_line = cut.start(blockIdx.x);
   const int stop = cut.start(blockIdx.x + 1);
   if (threadIdx.x == 0) p.splits[blockIdx.x].from = -1;
@@ -1011,14 +981,16 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn
   pdl_wait();
   pdl_trigger();
   const Kv4Split* splits = p.splits + blockIdx.x * warps;
-  const Kv4Split mine = lane < warps ? splits[lane] : Kv4Split{-1};
+  Kv4Split mine{};
+  mine.from = -1;
+  if (lane < warps) mine = splits[lane];
   auto of = [&](int v, int from) { return __shfl_sync(0xffffffffu, v, from); };
   int number = 0;   // of items that are joined a column to a warp
   for (uint32_t left = __ballot_sync(0xffffffffu, mine.from >= 0); left != 0; left &= left - 1) {
-    const int i = __ffs(left) - 1, from = of(mine.from, i), to = of(mine.to, i), in0 = of(mine.in0, i), in1 = of(mine.in1, i), each = of(mine.each, i);
+    const int i = __ffs(left) - 1;
+    const Kv4Pieces pieces{of(mine.from, i), 0, of(mine.in0, i), of(mine.in1, i), of(mine.each, i), of(mine.before, i), of(mine.whole, i), 0};
     const int many = min(of(mine.n_cols, i) - of(mine.col0, i), columns);
-    const bool some = in0 < in1;
-    const int before = some ? in0 * each - from : to - from + 1, whole = some ? in1 - in0 : 0, parts = before + whole + (some ? to - in1 * each + 1 : 0);
+    const int parts = of(mine.parts, i);
     const bool alone = parts <= 2 * kAtOnce;
     const int first = alone ? 0 : warp, step = alone ? 1 : kJoinWarps;
     // columns are dealt out in turn, over the items that a warp joins alone
@@ -1031,9 +1003,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn
       float2 x[kAtOnce][NG];
 #pragma unroll
       for (int e = 0; e < kAtOnce; ++e) {
-        const int k = min(k0 + e * step, parts - 1);
-        const int w = k < before ? from + k : k < before + whole ? (in0 + k - before) * each : in1 * each + k - before - whole;
-        const float* part = kv4_part(p, (int64_t)(w / each) * warps + w % each, k < before && k == 0, columns);
+        const int k = min(k0 + e * step, parts - 1), w = pieces.piece(k);
+        const float* part = kv4_part(p, (int64_t)(w / pieces.each) * warps + w % pieces.each, k < pieces.before && k == 0, columns);
         m[e] = part[columns * kDim + col];
         l[e] = k0 + e * step < parts ? part[columns * kDim + columns + col] : 0.f;
 #pragma unroll
