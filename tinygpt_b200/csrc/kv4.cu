@@ -104,7 +104,8 @@ __device__ __forceinline__ void to_nibbles(uint32_t (&out)[2 * N], const uint32_
     for (int i = 0; i < 2 * N; ++i) out[i] = __float_as_uint(exact_value((i % 2 ? bf16_hi(two[i / 2]) : bf16_lo(two[i / 2])) - sc.m, sc.s) + kRound);
 }
 
-// (Five CTAs to an SM: 3 049 rows of 8 heads of 128, stored and read back, 18.8 µs; four 19.7, six, which spill, 19.3.)
+// Five CTAs to an SM, in 48 registers, which spills 132 bytes: 3 049 rows of 8 heads of 128 are stored in 10.7 µs and stored and read back in 18.8; four (64 registers, 56 bytes) take 11.1
+// and 19.7, six (40, 264) 12.0 and 20.4.  There the issue slots are busy for 64 % of the cycles and the ALU for 47; 32 768 rows take 73 µs (79 and 60 %): instructions, then.
 template <int ROWS>
 __global__ void __launch_bounds__(kStoreWarps * 32, 5) kv4_store_kernel(const b200_kv4_cache cache, int layer, const __nv_bfloat16* k, int64_t ld_k,
                                                                      const __nv_bfloat16* v, int64_t ld_v, const int32_t* seqs, const int32_t* starts,

@@ -534,7 +534,8 @@ __device__ __forceinline__ void kv4_others(const Kv4Attn& p) {
     for (int d = threadIdx.x; d < width; d += blockDim.x) p.out[(int64_t)(row < head ? row : row - head + tail) * width + d] = f_to_bf16(0.f);
 }
 
-// ---- few columns to a sequence: every warp for itself
+// ---- few columns to a sequence: every warp for itself.  Two tiles of columns of heads of 192 and 256 take more than 255 registers (some 70 and 450 bytes of spills): 2 × 8 rows of 8 / 4
+// heads of 256 over 8 000 and 3 000 tokens 22.6 µs.
 // (the workspace is sized by this)
 constexpr int kPieceWarps = 8;
 template <int NG, int NT>
@@ -1048,11 +1049,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn
 // of 192 and 256), which unpacks for all of them (257 rows of 16 / 8 heads of 128 under a window of 1 024: 32.0 µs, two tiles to a warp 36.7).
 // Few columns over a small cache go to clusters: they save the second launch, and are worth it while a warp's share of the longest sequence that the cache can
 // hold is no more than some three steps above what the even cut would give it (µs, clusters / even cut, one sequence of 24 / 8 heads of 128: 1 000 tokens
-// 7.2 / 10.5, 4 000 9.0 / 11.4, 12 000 14.0 / 13.2; 14 / 2 heads of 64: 1 000 6.5 / 8.8, 4 000 7.5 / 10.2, 16 000 9.9 / 11.8; 32 / 4 heads of 128: 8 000 9.9 / 12.3,
-// 32 768 18.4 / 18.7).  As large a cluster as the SMs hold all of at once: of 16 CTAs 7, of 8 15, of 4 33 (36 / 6 heads of 128, 12 000
+// 7.5 / 10.2, 4 000 9.0 / 10.9, 12 000 14.1 / 12.2; 14 / 2 heads of 64: 1 000 6.4 / 9.3, 4 000 7.0 / 10.2, 16 000 9.6 / 11.4; 32 / 4 heads of 128: 8 000 9.5 / 12.0,
+// 32 768 17.2 / 15.0).  As large a cluster as the SMs hold all of at once: of 16 CTAs 7, of 8 15, of 4 33 (36 / 6 heads of 128, 12 000
 // tokens: clusters of 16 11.0, of 10 13.0; 24 / 8 heads, 4 000 tokens, where eight clusters of 16 are two rounds: 15.9).  A cluster goes over its sequence's blocks of columns
 // in turn, so both shares count once for every block of the sequence that may bring most rows, the others bringing one each (32 tokens beside a piece of 800 rows, 4 / 4 heads
 // of 128 over 832 tokens: clusters 434, even cut 31).
+// One way is taken for a whole call, by its average: a prompt's piece beside many single tokens is faster as two calls (µs, 32 / 8 heads of 128 over 4 000 tokens each: 512 rows beside 63
+// tokens 850, apart 184 + 81).
 struct Way {
   int tiles, columns, warps, cluster;   // tiles of a warp (0: the CTA's way), columns of a block, pieces of the line to a CTA; CTAs of a cluster (0: none)
 };

@@ -33,10 +33,12 @@ struct W4Params {
 // A CTA takes RT row tiles, a warp one of WARPS equal pieces of their columns, which come through a ring of its own in shared memory, 128 columns a stage; the
 // pieces are summed in shared memory in their order.  Values enter the products exactly and a group's sums are scaled in fp32, so nothing is rounded to
 // fewer bits before the result: as 128 + nibble, with Σ x of the group from a product with ones (kSums: with one tile of columns that costs less than
-// the subtraction, and a zero needs the sum anyway), or as nibble − 8.  What bounds it is the unpacking: seven instructions of half rate for eight values.
+// the subtraction, and a zero needs the sum anyway), or as nibble − 8.  Nothing is saturated: one row × 28 672 × 4 096 with zeros takes 16.5 µs (3.8 TB/s), in which the ALU, which
+// unpacks eight values in seven instructions of half rate, is busy for 53 % of the cycles, the issue slots for 55 and DRAM for 37; its 896 CTAs are two rounds on the SMs' 592
+// places, and each fills rings of its own and sums over its warps.  32 rows (448 CTAs, one to an SM, 44.7 µs): tensor cores 39 %, issue 33, DRAM 15.
 template <int NT, int RT, int WARPS, int GROUP, bool ZERO>
 struct W4Shape {
-  static constexpr int kStages = 2;   // (four take the room of a third and a fourth CTA: 28 672 × 4 096 18.1 → 20.0 µs)
+  static constexpr int kStages = 2;   // (more take the room of a third and a fourth CTA: 1 / 16 / 32 rows × 28 672 × 4 096 with two 16.8 / 24.7 / 45.0 µs, three 17.8 / 25.5 / 46.8, four 19.1 / 27.4 / 47.9)
   static constexpr bool kSums = ZERO || NT == 1;
   static constexpr int kParts = 128 / GROUP;   // groups of a stage
   static constexpr int kSmall = RT * kParts * (ZERO ? 2 : 1) * 32;   // bytes of scales and zeros
@@ -266,9 +268,12 @@ int launch_dequant(void* out, const W4Params& p, int group, float* bias_out, cud
 }
 
 // Which way rows of x go.  Values exact (w4_linear_kernel): up to 32 rows, and up to 64 over a W whose unpacking for each eight of them costs little (µs at 64 rows,
-// exact / on tcgen05: 4 096 × 4 096 17.7 / 11.2, 14 336 × 4 096 45.8 / 22.0).  W as bf16, unpacked into the products of 128 rows (w4_gemm.cu), up to 256.  More: W laid out
+// exact / on tcgen05: 4 096 × 4 096 17.7 / 11.2, 14 336 × 4 096 45.8 / 22.0).  That 32 rows are exact is a choice for exactness and not for speed: the widest weights would be as fast or
+// faster on tcgen05 from some 20 rows on (28 672 × 4 096: 16 rows 24.3 / 38.7, 24 42.0 / 39.9, 32 44.7 / 40.2, with zeros of 32 columns 71 / 48; 32 × 14 336 × 4 096 24.5 / 20.8; 32 × 8 192 ×
+// 4 096 12.6 / 13.6, 32 × 4 096 × 4 096 8.8 / 9.9).  W as bf16, unpacked into the products of 128 rows (w4_gemm.cu), up to 256.  More: W laid out
 // as bf16 once, which costs its writing, and the general GEMM (µs, unpacked / laid out: 128 × 1 024 × 1 024 8.8 / 13.0, 128 × 4 096 × 4 096 12.9 / 18.8, 256 × 4 096 × 4 096
-// 17.1 / 22.4, 256 × 4 096 × 14 336 37.7 / 62, 256 × 28 672 × 4 096 96 / 104; 300 × 896 × 896 9.9 / 8.8, 512 × 4 096 × 4 096 25.9 / 25.3, 512 × 14 336 × 4 096 94 / 72).
+// 17.1 / 22.4, 256 × 4 096 × 14 336 37.7 / 62, 256 × 28 672 × 4 096 96 / 104; 300 × 896 × 896 9.9 / 8.8, 512 × 4 096 × 4 096 25.9 / 25.3, 512 × 14 336 × 4 096 94 / 72).  Both want n to be a
+// multiple of 8; other widths go the exact way, 64 rows a launch, each of which reads W (128 × 50 257 × 1 024 118 µs, 50 264 channels 36).
 enum class W4Way { exact, unpacked, laid_out };
 W4Way w4_way(int64_t m, int64_t n, int64_t k) {
   if (n % 8 != 0 || m <= 32 || (m <= 64 && n * k <= 6 * 1000 * 1000)) return W4Way::exact;
@@ -296,12 +301,13 @@ int launch_w4_linear(void* y, const void* x, const b200_w4_weight& w, const void
     p.m = (int)std::min<int64_t>(m - r, 64);
     p.x = (const __nv_bfloat16*)x + r * w.k;
     p.y = (__nv_bfloat16*)y + r * w.n;
-    // Two row tiles to a warp share the loads of x and its sums, where CTAs are left for all SMs (µs, one / two: 1 × 4 096 × 4 096 4.9 / 4.7, 8 × 8 192 × 4 096
-    // 8.1 / 7.2, 32 × 4 096 × 4 096 12.8 / 9.7; 8 × 2 048 × 4 896 4.9 / 5.7, 32 × 1 024 × 4 096 6.9 / 9.1).  All warps of a CTA share a row tile's
+    // Two row tiles to a warp share the loads of x and its sums, where CTAs are left for all SMs (µs, one / two: 1 × 28 672 × 4 096 19.1 / 16.9, 8 × 8 192 × 4 096
+    // 7.2 / 6.6, 32 × 4 096 × 4 096 11.8 / 8.8, but 1 × 4 096 × 4 096 4.3 / 4.5; 8 × 2 048 × 4 896 4.4 / 6.0, 32 × 1 024 × 4 096 6.2 / 8.1).  All warps of a CTA share a row tile's
     // columns: fewer warps to a tile are fewer sums, and lost at every size (28 672 × 4 096: 17.7, four warps a tile 19.3).
     // Four where the loads of x weigh more, at 17 to 32 rows, or its sums, at 9 to 16 with zeros of many groups, and a CTA is left for most SMs (two / four: 32 × 28 672 ×
-    // 4 096 51 / 45, 24 × 8 192 × 4 096 17.8 / 14.8, 12 × 8 192 × 4 096 with zeros of 64 columns 12.1 / 9.5; with zeros of 128, 16 × 28 672 × 4 096 26.4 / 29.6, without
-    // 24.5 / 28.3, one row of it 16.5 / 16.6).
+    // 4 096 51.4 / 44.8, 24 × 8 192 × 4 096 14.6 / 11.8, 12 × 8 192 × 4 096 with zeros of 64 columns 10.7 / 8.6; with zeros of 128, 16 × 28 672 × 4 096 26.4 / 29.6, without
+    // 24.5 / 28.3, one row of it 16.5 / 16.6).  What they hold does not always fit 255 registers: four tiles spill 8 to 256 bytes (all but those of 128 columns without zeros), two
+    // with eight tiles of x 28 to 308, one with eight up to 156; one tile of x, kept to 64 registers for four CTAs to an SM, up to 32.
     const int tiles = (p.n + 15) / 16;
     const bool two = tiles >= 256, four = tiles >= 512;
     const int rc = p.m <= 8 ? (two ? launch_rows<1, 2, 8>(p, w.group, st) : launch_rows<1, 1, 8>(p, w.group, st))

@@ -472,7 +472,7 @@ def _kv4_rows(t: torch.Tensor, what: str, heads: Optional[int], dim: int):
 def kv4_store(cache: KV4Cache, layer: int, k: torch.Tensor, v: torch.Tensor, seqs: torch.Tensor, starts: torch.Tensor, pos: torch.Tensor) -> None:
     """Rows of k and v bf16 [rows, kv_heads, head_dim] (row strides may differ: slices of one projection) → the cache, in 4 bits.  Sequence seqs[i] owns
     rows starts[i] … starts[i + 1] − 1, for its positions pos[i], pos[i] + 1, … (what kv4_extend answered; −1: nowhere).  A row whose page the
-    sequence does not have, or shares, is left out.  seqs, starts (one more), pos: int32 on the device."""
+    sequence does not have, or shares, is left out.  Keys are stored as they come: a model that rotates them by position does so before.  seqs, starts (one more), pos: int32 on the device."""
     y = _fast.kv4_store(*cache._at, layer, k, v, seqs, starts, pos) if cache.__class__ is KV4Cache else None
     if y is True:
         return
