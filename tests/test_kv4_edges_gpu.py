@@ -148,3 +148,15 @@ def test_parts_of_a_cache_are_checked(built_lib):
                       (dict(head_dim=128), "pages"), (dict(head_dim=32), "heads"), (dict(kv_heads=0), "heads"), ({}, "CUDA device")):
         with pytest.raises(B200Error, match=what):
             ops.KV4Cache(**{**ok, **bad})
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,room", [(1, 1), (1, 9000), (7, 9000), (60, 1)])
+def test_a_window_over_everything_masks_nothing(built_lib, rows, room):
+    rand, length = Rand(27), 300
+    cache, seqs, k, v = filled(rand, [length], 2, 64, room=room)
+    q = rand(rows, 4, 64)
+    args = (cache, 0, q, seqs, dev([0, rows]), dev([length - rows]))
+    want = ops.kv4_attention(*args)
+    for window in (length, 2 ** 30, 2 ** 31 - 65, 2 ** 31 - 32, 2 ** 31 - 1, 2 ** 31, 2 ** 62):
+        assert torch.equal(ops.kv4_attention(*args, window=window), want), window

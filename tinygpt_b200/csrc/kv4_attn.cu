@@ -1163,7 +1163,7 @@ int b200_kv4_attention(void* out, const void* q, int64_t ld_q, const b200_kv4_ca
   p.kv_heads = Divisor((uint32_t)cache->kv_heads);
   p.n = (int)n;
   p.rows = (int)rows;
-  p.window = (int)std::min<int64_t>(window, INT32_MAX);
+  p.window = window > INT32_MAX - 64 ? 0 : (int)window;   // positions end below 2^30 + 2^24, so such a window masks nothing; and a step added to it stays in 32 bits
   p.scale_log2 = scale * 1.44269504f;
   const cudaStream_t st = (cudaStream_t)stream;
   switch (cache->dim / kKvGroup) {
