@@ -160,3 +160,26 @@ def test_a_window_over_everything_masks_nothing(built_lib, rows, room):
     want = ops.kv4_attention(*args)
     for window in (length, 2 ** 30, 2 ** 31 - 65, 2 ** 31 - 32, 2 ** 31 - 1, 2 ** 31, 2 ** 62):
         assert torch.equal(ops.kv4_attention(*args, window=window), want), window
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,room", [(5, 1), (5, 9000), (12, 9000), (60, 1), (150, 1)])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_masked_numbers_that_are_none(built_lib, rows, room, dim):
+    """Keys and values that are not finite, behind a row's own position and in front of its window, change nothing for that row, in every way; for rows that see them
+    they count."""
+    rand, length, window = Rand(28), 333, 90
+    cache, seqs, k, v = filled(rand, [length], 2, dim, room=room)
+    q, first = rand(rows, 4, dim), length - rows
+    args = (cache, 0, q, seqs, dev([0, rows]), dev([first]))
+    plain, windowed = ops.kv4_attention(*args), ops.kv4_attention(*args, window=window)
+    for t in (first + rows // 2, first, length - 1, first - 10, max(first + rows // 2 - window, 0)):
+        for which in (0, 1):
+            bad = [x[t:t + 1].clone() for x in (k, v)]
+            bad[which][0, :, 3::64] = (float("nan"), float("inf"))[t % 2]
+            ops.kv4_store(cache, 0, *bad, seqs, dev([0, 1]), dev([t]))
+            for got, want, w in ((ops.kv4_attention(*args), plain, 0), (ops.kv4_attention(*args, window=window), windowed, window)):
+                at = first + torch.arange(rows)
+                sees = (at >= t) & ((at - t < w) | (w == 0))
+                assert torch.equal(got.cpu()[~sees], want.cpu()[~sees]) and bool(got.cpu()[sees].isnan().all()), (t, which, w)
+            ops.kv4_store(cache, 0, k[t:t + 1], v[t:t + 1], seqs, dev([0, 1]), dev([t]))
