@@ -183,3 +183,18 @@ def test_masked_numbers_that_are_none(built_lib, rows, room, dim):
                 sees = (at >= t) & ((at - t < w) | (w == 0))
                 assert torch.equal(got.cpu()[~sees], want.cpu()[~sees]) and bool(got.cpu()[sees].isnan().all()), (t, which, w)
             ops.kv4_store(cache, 0, k[t:t + 1], v[t:t + 1], seqs, dev([0, 1]), dev([t]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,room", [(1, 1), (1, 9000), (7, 9000), (60, 1)])
+def test_positions_to_the_end_of_32_bits(built_lib, rows, room):
+    """Rows far behind what the sequence holds see of it what their window reaches."""
+    rand, length = Rand(29), 300
+    cache, seqs, k, v = filled(rand, [length], 2, 64, room=room)
+    q, hk, hv = rand(rows, 4, 64), orc.held(k), orc.held(v)
+    for at in (2 ** 30 - 1, 2 ** 30 + 7, 2 ** 31 - 300, 2 ** 31 - 70 - rows):
+        for back in (1, 31, 200, length - 1 + rows, length + 500):   # the first row's window ends so far behind the first token
+            window = at - back
+            want, bound = orc.attention(q, hk, hv, at, 64 ** -0.5, window)
+            got = ops.kv4_attention(cache, 0, q, seqs, dev([0, rows]), dev([at]), window=window).cpu().double()
+            assert bool(((got - want).abs() <= bound).all()), (at, back)

@@ -43,7 +43,7 @@ int main() {
   long n = 0;
   for (int max_pages : {1, 2, 3})
     for (int length = 0; length <= max_pages * 64; ++length)
-      for (int pos : {0, 1, 30, 31, 32, 33, 63, 64, 65, 95, 96, 127, 128, 129, 160, 191, 192, 193, 500, 1 << 30})
+      for (int pos : {0, 1, 30, 31, 32, 33, 63, 64, 65, 95, 96, 127, 128, 129, 160, 191, 192, 193, 500, 1 << 30, 2147483647 - 64 - 70})
         for (int rows : {1, 2, 33, 70})
           for (int window : {0, 1, 2, 10, 31, 32, 33, 64, 65, 150, 2147483647})
             for (int columns : {1, 8, 64}) {

@@ -83,7 +83,7 @@ __device__ __forceinline__ Kv4Rows kv4_read(const Kv4Attn& p, int i) {
   Kv4Rows s;
   s.row0 = min(max(p.starts[i], 0), p.rows);
   s.count = max(min(p.starts[i + 1], p.rows) - s.row0, 0);
-  s.pos = min(p.pos[i], 1 << 30);
+  s.pos = min(p.pos[i], INT32_MAX - 64 - s.count);   // (so that positions, and a step behind them, stay in 32 bits)
   s.slot = p.seqs[i];
   s.last = 0;
   if (s.pos >= 0 && s.slot >= 0 && s.slot < p.cache.n_seqs)
@@ -1163,7 +1163,7 @@ int b200_kv4_attention(void* out, const void* q, int64_t ld_q, const b200_kv4_ca
   p.kv_heads = Divisor((uint32_t)cache->kv_heads);
   p.n = (int)n;
   p.rows = (int)rows;
-  p.window = window > INT32_MAX - 64 ? 0 : (int)window;   // positions end below 2^30 + 2^24, so such a window masks nothing; and a step added to it stays in 32 bits
+  p.window = window > INT32_MAX - 64 ? 0 : (int)window;   // positions end before that, so such a window masks nothing; and a step added to it stays in 32 bits
   p.scale_log2 = scale * 1.44269504f;
   const cudaStream_t st = (cudaStream_t)stream;
   switch (cache->dim / kKvGroup) {
