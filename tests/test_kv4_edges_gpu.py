@@ -198,3 +198,104 @@ def test_positions_to_the_end_of_32_bits(built_lib, rows, room):
             want, bound = orc.attention(q, hk, hv, at, 64 ** -0.5, window)
             got = ops.kv4_attention(cache, 0, q, seqs, dev([0, rows]), dev([at]), window=window).cpu().double()
             assert bool(((got - want).abs() <= bound).all()), (at, back)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("room", [0, 9000])
+def test_a_sequence_twice_in_a_call(built_lib, room):
+    """Two pieces of one sequence, stored and attended in one call: places in one tile of 16 and apart."""
+    rand, heads, dim = Rand(30), 4, 64
+    cache = ops.kv4_cache(1, 8, 2, 4 + room, 2, dim)
+    cache.pages.fill_(255)
+    assert ops.kv4_extend(cache, dev([1, 0]), dev([200, 70])).tolist() == [0, 0]
+    k, v, q = rand(270, 2, dim), rand(270, 2, dim), rand(270, heads, dim)
+    # rows: of sequence 1 positions 0 … 7, of it 8 … 99, of sequence 0 all, of sequence 1 100 … 199
+    seqs, starts, pos = dev([1, 1, 0, 1]), dev([0, 8, 100, 170, 270]), dev([0, 8, 0, 100])
+    ops.kv4_store(cache, 0, k, v, seqs, starts, pos)
+    for got, x in zip(ops.kv4_load(cache, 0, seqs, starts, pos, 270), (k, v)):
+        assert torch.equal(got.cpu(), orc.held(x))
+    hk, hv = ({1: torch.cat((orc.held(x)[:100], orc.held(x)[170:])), 0: orc.held(x)[100:170]} for x in (k, v))
+    for rows, at in ([(0, 8), (8, 100), (100, 170), (170, 270)], [0, 8, 0, 100]), ([(7, 8), (99, 100), (169, 170), (269, 270)], [7, 99, 69, 199]):
+        x = torch.cat([q[a:b] for a, b in rows])
+        counts = [b - a for a, b in rows]
+        out, row = ops.kv4_attention(cache, 0, x, seqs, starts_of(counts), dev(at)).cpu().double(), 0
+        for s, c, p in zip((1, 1, 0, 1), counts, at):
+            want, bound = orc.attention(x[row:row + c], hk[s], hv[s], p, dim ** -0.5, 0)
+            assert bool(((out[row:row + c] - want).abs() <= bound).all()), (s, c, p)
+            row += c
+
+
+@pytest.mark.gpu
+def test_calls_on_several_streams(built_lib):
+    """Calls of every way at once, each with its own workspace, over one cache that none of them writes, beside Linears of every way."""
+    rand, dim = Rand(31), 128
+    lengths = [3000, 64, 700, 1111]
+    big, seqs, _, _ = filled(rand, lengths, 2, dim, room=9000)
+    small, few, _, _ = filled(rand, [900, 33], 2, dim)
+    w = ops.w4_quantize(rand(512, 1024, spread=0.03))
+    jobs = []
+    for cache, s, ls in ((big, seqs, lengths), (small, few, [900, 33])):
+        for rows in (1, 6, 60):
+            counts = [min(rows, l) for l in ls]
+            q, st, pos = rand(sum(counts), 4, dim), starts_of(counts), dev([l - c for l, c in zip(ls, counts)])
+            jobs.append(lambda cache=cache, q=q, s=s, st=st, pos=pos: ops.kv4_attention(cache, 0, q, s, st, pos))
+    for m in (1, 20, 100, 300):
+        x = rand(m, 1024)
+        jobs.append(lambda x=x: ops.linear_w4(x, w))
+    want = [job() for job in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for turn in range(20):
+        for n, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                for i in range(len(jobs)):
+                    j = (i * (2 * n + 1) + turn) % len(jobs)
+                    got.append((j, jobs[j]()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[j]) for j, y in got)
+
+
+class Guarded:
+    """Device memory between two guards; what it held before is numbers that are none."""
+
+    def __init__(self, nbytes):
+        self.all = torch.full((4096 + -(-nbytes // 256) * 256 + 4096,), 255, dtype=torch.uint8, device="cuda")
+        self.at, self.nbytes = self.all.data_ptr() + 4096, nbytes
+
+    def view(self, dtype, *shape):
+        return self.all[4096:4096 + self.nbytes].view(dtype).view(shape)
+
+    def intact(self):
+        return bool((self.all[:4096] == 255).all()) and bool((self.all[4096 + self.nbytes:] == 255).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lengths,counts,heads,kv_heads,dim,room", [([900, 33], [1, 1], 14, 2, 64, 0), ([3000, 64, 700], [1, 1, 1], 24, 8, 128, 9000), ([700] * 40, [1] * 40, 4, 2, 64, 9000),
+                                                                    ([3000, 300], [6, 20], 4, 2, 256, 9000), ([900, 300], [257, 1], 16, 8, 128, 0), ([500], [200], 4, 1, 192, 0),
+                                                                    ([60] * 40, [50] * 40, 4, 2, 64, 0)])
+def test_calls_of_the_library_stay_within_their_memory(built_lib, lengths, counts, heads, kv_heads, dim, room):
+    """The C entry points with workspaces and results of just the bytes they ask for, whatever those held before."""
+    import ctypes as C
+    from tinygpt_b200._lib import lib
+    rand, n, rows = Rand(32), len(lengths), sum(counts)
+    cache, seqs, k, v = filled(rand, lengths, kv_heads, dim, room=room)
+    d, stream = C.byref(cache._desc), torch.cuda.current_stream().cuda_stream
+    q, st, pos = rand(rows, heads, dim), starts_of(counts), dev([l - c for l, c in zip(lengths, counts)])
+    want = ops.kv4_attention(cache, 0, q, seqs, st, pos)
+    out, ws = Guarded(2 * q.numel()), Guarded(lib().b200_kv4_attention_workspace_bytes(d, heads, n, rows))
+    assert lib().b200_kv4_attention(out.at, q.data_ptr(), heads * dim, d, 0, heads, seqs.data_ptr(), st.data_ptr(), pos.data_ptr(), n, rows, dim ** -0.5, 0,
+                                    ws.at if ws.nbytes else None, stream) == 0
+    assert torch.equal(out.view(BF16, *q.shape), want) and out.intact() and ws.intact()
+    total = sum(lengths)
+    keys, vals = Guarded(4 * k.numel()), Guarded(4 * v.numel())
+    assert lib().b200_kv4_load(keys.at, vals.at, d, 0, seqs.data_ptr(), starts_of(lengths).data_ptr(), dev([0] * n).data_ptr(), n, total, stream) == 0
+    assert torch.equal(vals.view(torch.float32, *v.shape).cpu(), orc.held(v)) and keys.intact() and vals.intact()
+    ws = Guarded(lib().b200_kv4_workspace_bytes(d))
+    for call, other in (("extend", [64] * n), ("fork", [n] * n)):
+        got, others = Guarded(4 * n), dev(other)
+        assert getattr(lib(), f"b200_kv4_{call}")(d, seqs.data_ptr(), others.data_ptr(), got.at, n, ws.at, stream) == 0
+        assert got.intact() and ws.intact()
+    live = Guarded(4)
+    assert lib().b200_kv4_free(d, seqs.data_ptr(), n // 2 + 1, stream) == 0 and lib().b200_kv4_compact(d, live.at, ws.at, stream) == 0
+    assert int(live.view(torch.int32, 1)) == int((cache.refs > 0).sum()) and live.intact() and ws.intact()

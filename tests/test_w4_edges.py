@@ -132,3 +132,23 @@ def test_whole_numbers_are_exact(built_lib, n, k, group, zero):
         want = x.double() @ full.t()
         assert torch.equal(ops.linear_w4(x, w), want.to(torch.bfloat16)), m
         assert torch.equal(ops.linear_w4(x, w, bias), (want + bias.double()).to(torch.bfloat16)), m
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,k,m", [(24, 72, 1), (4104, 520, 20), (999, 520, 70), (264, 1096, 60), (4104, 520, 129), (1032, 72, 300)])
+def test_calls_of_the_library_stay_within_their_memory(built_lib, n, k, m):
+    """The C entry points with a workspace and results of just the bytes they ask for, whatever those held before."""
+    import ctypes as C
+    from test_kv4_edges_gpu import Guarded
+    from tinygpt_b200._lib import W4Desc, lib
+    w, full, g = whole_numbers(n, k, 64, True)
+    x, bias, stream = rows_of(m, k, g), torch.randint(-64, 65, (n,), generator=g, device="cuda").to(torch.bfloat16), torch.cuda.current_stream().cuda_stream
+    d = W4Desc(w.q.data_ptr(), w.scale.data_ptr(), w.zero.data_ptr(), n, k, 64)
+    for b in (None, bias):
+        y, ws = Guarded(2 * m * n), Guarded(lib().b200_w4_workspace_bytes(m, n, k))
+        assert lib().b200_w4_linear_bf16(y.at, x.data_ptr(), C.byref(d), None if b is None else b.data_ptr(), m, ws.at if ws.nbytes else None, stream) == 0
+        want = x.double() @ full.t() + (0 if b is None else b.double())
+        assert torch.equal(y.view(torch.bfloat16, m, n), want.to(torch.bfloat16)) and y.intact() and ws.intact()
+    out = Guarded(2 * n * k)
+    assert lib().b200_w4_dequant_bf16(out.at, C.byref(d), stream) == 0
+    assert torch.equal(out.view(torch.bfloat16, n, k).double(), full) and out.intact()
