@@ -490,7 +490,7 @@ struct Walk {
     if constexpr (EXACT) {
       const int lane = threadIdx.x % 32;
       block = 0;
-      for (int first = 0; first < s.blocks; first += 32) {   // (`at` lies in a block of the sequence, unless someone writes to its length meanwhile)
+      for (int first = 0; first < s.blocks; first += 32) {   // (`at` lies in a block of the sequence)
         const Kv4Steps steps = first + lane < s.blocks ? kv4_block_steps(p, s, first + lane, columns) : Kv4Steps{0, -kAhead};
         const int upto = (int)warp_scan((long long)(steps.n + kAhead) * (int)p.kv_heads.d, lane);
         const uint32_t before = __ballot_sync(0xffffffffu, base + upto <= at);
