@@ -39,8 +39,10 @@ extern "C" {
  * b200_stack_input_conv, b200_stack_pool_attention, b200_stack_bonus_scan, b200_stack_mamba1_scan;  9: + gated linear attention
  * (b200_gla_desc), capped scores, distance biases and values that are the keys (fields appended to b200_attn_desc), short
  * convolutions and per-head norms in front of any attention (fields appended to b200_attn_prep_desc and b200_pool_attn_desc),
- * gated feed-forwards in sandwich blocks;  10: + weights of 4 bits (b200_w4_*) and the paged cache of 4 bits (b200_kv4_*).  All additive: callers of an older version keep working once they are compiled against this header. */
-#define B200_ABI_VERSION 10
+ * gated feed-forwards in sandwich blocks;  10: + weights of 4 bits (b200_w4_*) and the paged cache of 4 bits (b200_kv4_*);
+ * 11: + rows and weights of 8 bits (b200_f8_*, b200_rmsnorm_f8, b200_silu_mul_f8), products grouped by expert (b200_grouped_bf16) and routed experts
+ * (b200_expert_*, b200_experts_f8_*).  All additive: callers of an older version keep working once they are compiled against this header. */
+#define B200_ABI_VERSION 11
 
 typedef enum b200_status {
   B200_OK = 0,
@@ -193,6 +195,51 @@ int64_t b200_w4_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int b200_w4_linear_bf16(void* y, const void* x, const b200_w4_weight* w, const void* bias_or_null, int64_t m, void* workspace, void* stream);
 /* out[n,k] = bf16(W), 16-byte aligned. */
 int b200_w4_dequant_bf16(void* out, const b200_w4_weight* w, void* stream);
+
+/* ------------------------------------------------------------------------------------------------------------------
+ * Serving in 8 bits (nothing in the reference): e4m3 with fp32 scales, and products of rows grouped by expert.
+ * Rows in 8 bits: q [rows][ld] bytes, ld = k rounded up to 16 (bytes behind k are 0), 16-byte aligned; scale fp32 [(k + 127) / 128][rows].  A number is value·scale of
+ * its block of 128 entries.  Of a block of numbers t:  s = max(fp32(max|t| / 448), 2^-126),  value = e4m3(fp32(t / s)), ties to even.  A block with an
+ * entry that is not finite reads as NaN where that entry is, and makes results of its row that are not finite.
+ * ---------------------------------------------------------------------------------------------------------------- */
+/* t = row index[i] of x (bf16 [x_rows], ld_x entries apart; index NULL: row i), zeros where the index is none of x_rows; scale = s. */
+int b200_f8_rows_bf16(void* q, float* scale, const void* x, int64_t ld_x, int64_t x_rows, const int32_t* index_or_null, int64_t rows, int64_t k, void* stream);
+/* z = x, or bf16(x + residual), which goes to `sum` (it may lie where x or the residual does); t = z·w (fp32; w NULL: 1); scale = s·rsqrt(mean(z²) + eps). */
+int b200_rmsnorm_f8(void* q, float* scale, void* sum_or_null, const void* x, const void* residual_or_null, const void* w_or_null, int64_t rows, int64_t dim,
+                    float eps, void* stream);
+/* gate_up rows are [gate(n) | up(n)], bf16; t = silu(gate)·up in fp32; scale = s. */
+int b200_silu_mul_f8(void* q, float* scale, const void* gate_up, int64_t rows, int64_t n, void* stream);
+/* out[rows, k] = value·scale, fp32. */
+int b200_f8_rows_dequant(float* out, const void* q, const float* scale, int64_t rows, int64_t k, void* stream);
+
+/* W[e][i][j] = value·scale[e][i / 128][j / 128]: q bytes [experts][n][ld], ld = k rounded up to 16, 16-byte aligned; scale fp32 [experts][(n + 127) / 128][(k + 127) / 128].
+ * One matrix: experts 1. */
+typedef struct b200_f8_weight {
+  const void* q;
+  const float* scale;
+  int32_t n, k, experts;
+} b200_f8_weight;
+
+/* y[rows, n] = bf16( x·Wᵀ + bias ) of rows in 8 bits: the products of 128 entries are summed in the tensor cores, scaled and added in fp32, rounded once.  The
+ * magnitude of value sums · scales stays below 2^127.  How a sum is cut over CTAs depends on the number of rows. */
+int b200_f8_linear_bf16(void* y, const void* q, const float* scale, const b200_f8_weight* w, const void* bias_or_null, int64_t rows, void* stream);
+/* Rows starts[e] … starts[e + 1] − 1 meet W[e] (starts int32 [experts + 1] on the device, not falling; none, or any number of rows to an expert); rows in front of the first
+ * group and behind the last are zeros in y.  Up to 1 024 experts. */
+int b200_f8_grouped_bf16(void* y, const void* q, const float* scale, const b200_f8_weight* w, const int32_t* starts, int64_t rows, void* stream);
+/* The same over x bf16 [rows, k] and w bf16 [experts, n, k], k % 8 == 0, 16-byte aligned. */
+int b200_grouped_bf16(void* y, const void* x, const void* w, const int32_t* starts, int64_t rows, int64_t experts, int64_t n, int64_t k, void* stream);
+
+/* chosen int32 [rows, top] → the pairs in the order of their experts, an expert's in the order of the rows: starts [experts + 1], source [rows·top] (the row of every
+ * pair; −1 behind the last), place [rows, top] (where a pair went).  A choice outside 0 … experts − 1 is no pair: place −1. */
+int b200_expert_order(int32_t* starts, int32_t* source, int32_t* place, const int32_t* chosen, int64_t rows, int64_t top, int64_t experts, void* stream);
+/* out[r] = bf16( Σ_t weights[r, t]·y[place[r, t]] ), y bf16 [rows·top, n], fp32 in the order of t; a place outside y adds nothing. */
+int b200_expert_combine_bf16(void* out, const void* y, const int32_t* place, const float* weights, int64_t rows, int64_t top, int64_t n, void* stream);
+/* A layer of routed experts: w_in [experts, 2·ff, width] = [gate | up], w_out [experts, width, ff]; x bf16 [rows, width] → out bf16 [rows, width] =
+ * Σ_t weights[r, t]·W_out[e]·(silu(gate)·up), e = chosen[r, t]: the rows in 8 bits, [gate | up] rounded to bf16, silu(gate)·up in 8 bits, an expert's result rounded to
+ * bf16, as the calls above one behind the other make them.  workspace: b200_experts_f8_workspace_bytes bytes, 16-byte aligned. */
+int64_t b200_experts_f8_workspace_bytes(int64_t rows, int64_t top, int64_t experts, int64_t width, int64_t ff);
+int b200_experts_f8_bf16(void* out, const void* x, const int32_t* chosen, const float* weights, const b200_f8_weight* w_in, const b200_f8_weight* w_out, int64_t rows,
+                         int64_t top, void* workspace, void* stream);
 
 /* A cache whose keys and values are held in 4 bits, in pages of 64 tokens of all heads, `layers` pools side by side under one table.
  * Of a row of a head, 64 entries in a row are a group: with lo and hi its least and largest entry, scale = bf16(hi / 15 − lo / 15), middle = bf16(lo + 8·scale),

@@ -139,6 +139,10 @@ class StackDesc(C.Structure):
                 ("norm_kind", C.c_int32), ("logit_softcap", C.c_float), ("streams", C.c_int32)]
 
 
+class F8Desc(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("scale", C.c_void_p), ("n", C.c_int32), ("k", C.c_int32), ("experts", C.c_int32)]
+
+
 class W4Desc(C.Structure):
     _fields_ = [("q", C.c_void_p), ("scale", C.c_void_p), ("zero", C.c_void_p), ("n", C.c_int32), ("k", C.c_int32), ("group", C.c_int32)]
 
@@ -173,6 +177,17 @@ PROTOTYPES = {
     "b200_gemv_fused_bf16": (I32, [P, P, P, I64, I64, I32, P, F, P, P, I32, P]),
     "b200_attn_decode_workspace_bytes": (I64, [I64, I64, I64, I64]),
     "b200_attn_decode_bf16": (I32, [P, P, P, P, F, P, P, I64, P, P, I64, I64, I64, I64, P, P]),
+    "b200_f8_rows_bf16": (I32, [P, P, P, I64, I64, P, I64, I64, P]),
+    "b200_rmsnorm_f8": (I32, [P, P, P, P, P, P, I64, I64, F, P]),
+    "b200_silu_mul_f8": (I32, [P, P, P, I64, I64, P]),
+    "b200_f8_rows_dequant": (I32, [P, P, P, I64, I64, P]),
+    "b200_f8_linear_bf16": (I32, [P, P, P, C.POINTER(F8Desc), P, I64, P]),
+    "b200_f8_grouped_bf16": (I32, [P, P, P, C.POINTER(F8Desc), P, I64, P]),
+    "b200_grouped_bf16": (I32, [P, P, P, P, I64, I64, I64, I64, P]),
+    "b200_expert_order": (I32, [P, P, P, P, I64, I64, I64, P]),
+    "b200_expert_combine_bf16": (I32, [P, P, P, P, I64, I64, I64, P]),
+    "b200_experts_f8_workspace_bytes": (I64, [I64, I64, I64, I64, I64]),
+    "b200_experts_f8_bf16": (I32, [P, P, P, P, C.POINTER(F8Desc), C.POINTER(F8Desc), I64, I64, P, P]),
     "b200_w4_workspace_bytes": (I64, [I64, I64, I64]),
     "b200_w4_linear_bf16": (I32, [P, P, C.POINTER(W4Desc), P, I64, P, P]),
     "b200_w4_dequant_bf16": (I32, [P, C.POINTER(W4Desc), P]),

@@ -114,6 +114,25 @@ int make_tmap_sw128(CUtensorMap* out, int rank, const void* base, int64_t batch,
   return B200_OK;
 }
 
+int make_tmap_sw128_u8(CUtensorMap* out, const void* base, int64_t rows, int64_t cols, int64_t row_stride, int box_rows) {
+  EncodeTiledFn enc = get_encode();
+  if (!enc) {
+    set_error("cuTensorMapEncodeTiled is not available (no CUDA driver / device?)");
+    return B200_ERR_NO_DEVICE;
+  }
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)row_stride};
+  cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled(8 bits, swizzle 128B) failed with CUresult %d (rows=%lld cols=%lld)", (int)r, (long long)rows, (long long)cols);
+    return B200_ERR_CUDA;
+  }
+  return B200_OK;
+}
+
 // Words come from pages of 1 024 that stay with the process: pinning memory takes a millisecond, an engine comes and goes more often.
 static std::mutex word_mutex;
 static std::vector<unsigned*> free_words;

@@ -272,6 +272,8 @@ struct WaitScope {                           // launches of this thread write to
 // 128-byte swizzle; what lies outside is zero
 int make_tmap_sw128(CUtensorMap* out, int rank, const void* base, int64_t batch, int64_t rows, int64_t cols, int64_t batch_stride,
                     int64_t row_stride, int box_rows);
+// [rows, cols] of 8 bits, boxes of 128 columns × box_rows rows, 128-byte swizzle; row_stride in bytes, a multiple of 16
+int make_tmap_sw128_u8(CUtensorMap* out, const void* base, int64_t rows, int64_t cols, int64_t row_stride, int box_rows);
 // 2-D bf16 row-major [rows, cols] tensor map with box {box_cols, box_rows}, no swizzle (host).
 int make_tmap_2d_bf16(CUtensorMap* out, const void* base, int64_t rows, int64_t cols, int box_rows, int box_cols);
 

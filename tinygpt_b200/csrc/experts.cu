@@ -1,0 +1,225 @@
+// experts.cu — a layer of routed experts around its products (group_gemm.cu): the pairs (row, chosen expert) in the order of their experts, and the weighted sum of
+// the experts' rows back into the rows that they came from.
+#include "f8.cuh"
+
+#include <algorithm>
+
+namespace b200 {
+
+namespace {
+
+// A stable counting sort in one CTA: every warp takes a run of the pairs, 32 at a time in their order.  Lanes that hold the same expert find each other
+// (match), so a warp's count of an expert is its own and no atomics decide an order.
+//   1. counts[warp][e];  2. the sum in front of each: experts first, then warps;  3. the runs again, each pair to its place
+constexpr int kOrderWarps = 32;
+
+__global__ void __launch_bounds__(32 * kOrderWarps) expert_order_kernel(int32_t* __restrict__ starts, int32_t* __restrict__ source, int32_t* __restrict__ place,
+                                                                        const int32_t* __restrict__ chosen, int pairs, int top, int experts) {
+  extern __shared__ int counts[];                    // [warps][experts]
+  int* const total = counts + kOrderWarps * experts;   // [experts]: rows of all experts up to and with e
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  pdl_wait();
+  pdl_trigger();
+  for (int i = threadIdx.x; i < kOrderWarps * experts; i += 32 * kOrderWarps) counts[i] = 0;
+  __syncthreads();
+  const int run = (pairs + 32 * kOrderWarps - 1) / (32 * kOrderWarps) * 32, from = min(warp * run, pairs), to = min(from + run, pairs);
+  int* const own = counts + warp * experts;
+  auto walk = [&](auto at) {
+    for (int i = from; i < to; i += 32) {
+      const bool is = i + lane < to;
+      const int e = is ? chosen[i + lane] : -1;
+      const bool valid = e >= 0 && e < experts;
+      const unsigned same = __match_any_sync(0xffffffffu, valid ? e : -1);
+      int before = 0;
+      if (valid) before = own[e];
+      __syncwarp();
+      if (valid && lane == __ffs(same) - 1) own[e] = before + __popc(same);
+      __syncwarp();
+      if (is) at(i + lane, valid, before + __popc(same & ((1u << lane) - 1)));
+    }
+  };
+  walk([](int, bool, int) {});
+  __syncthreads();
+  for (int e = threadIdx.x; e < experts; e += 32 * kOrderWarps) {
+    int sum = 0;
+#pragma unroll 8
+    for (int w = 0; w < kOrderWarps; ++w) {
+      const int c = counts[w * experts + e];
+      counts[w * experts + e] = sum;
+      sum += c;
+    }
+    total[e] = sum;
+  }
+  __syncthreads();
+  if (warp == 0) {   // every lane a run of experts
+    const int each = (experts + 31) / 32, e0 = min(lane * each, experts), e1 = min(e0 + each, experts);
+    int mine = 0;
+    for (int e = e0; e < e1; ++e) mine += total[e];
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    upto -= mine;
+    for (int e = e0; e < e1; ++e) {
+      const int c = total[e];
+      total[e] = upto;
+      starts[e] = upto;
+      upto += c;
+    }
+    const int all = __shfl_sync(0xffffffffu, upto, 31);
+    if (lane == 0) starts[experts] = all;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kOrderWarps * experts; i += 32 * kOrderWarps) counts[i] += total[i % experts];
+  const int all_rows = starts[experts];
+  for (int i = all_rows + threadIdx.x; i < pairs; i += 32 * kOrderWarps) source[i] = -1;
+  __syncthreads();
+  walk([&](int i, bool valid, int to_place) {
+    place[i] = valid ? to_place : -1;
+    if (valid) source[to_place] = i / top;
+  });
+}
+
+// out[r] = bf16( Σ_t weights[r, t]·y[place[r, t]] ), t in order, fp32.  Eight channels a thread (WIDE) or one.
+template <bool WIDE>
+__global__ void __launch_bounds__(256) expert_combine_kernel(__nv_bfloat16* __restrict__ out, const __nv_bfloat16* __restrict__ y, const int32_t* __restrict__ place,
+                                                             const float* __restrict__ weights, int64_t rows, int top, int n) {
+  pdl_wait();
+  pdl_trigger();
+  constexpr int EACH = WIDE ? 8 : 1;
+  const int pieces = n / EACH;
+  const int64_t all = rows * pieces, y_rows = rows * top;
+  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < all; at += (int64_t)gridDim.x * 256) {
+    const int64_t row = at / pieces;
+    const int i = (int)(at % pieces) * EACH;
+    float acc[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) acc[e] = 0.f;
+#pragma unroll 4
+    for (int t = 0; t < top; ++t) {
+      const int64_t from = place[row * top + t];
+      if (from < 0 || from >= y_rows) continue;
+      const float w = weights[row * top + t];
+      if constexpr (WIDE) {
+        float v[8];
+        unpack8(*reinterpret_cast<const uint4*>(y + from * n + i), v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] = fmaf(w, v[e], acc[e]);
+      } else {
+        acc[0] = fmaf(w, bf16_to_f(y[from * n + i]), acc[0]);
+      }
+    }
+    if constexpr (WIDE) *reinterpret_cast<uint4*>(out + row * n + i) = make_uint4(pack2(acc[0], acc[1]), pack2(acc[2], acc[3]), pack2(acc[4], acc[5]), pack2(acc[6], acc[7]));
+    else out[row * n + i] = f_to_bf16(acc[0]);
+  }
+}
+
+constexpr int64_t up256(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+
+// where the parts of a layer's workspace lie
+struct ExpertsSpace {
+  int64_t starts, source, place, q, scale, gate_up, a, a_scale, y, bytes;
+};
+ExpertsSpace experts_space(int64_t rows, int64_t top, int64_t experts, int64_t width, int64_t ff) {
+  ExpertsSpace s{};
+  const int64_t pairs = rows * top;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t from = at;
+    at += up256(bytes);
+    return from;
+  };
+  s.starts = take((experts + 1) * 4);
+  s.source = take(pairs * 4);
+  s.place = take(pairs * 4);
+  s.q = take(pairs * f8_ld(width));
+  s.scale = take(pairs * f8_blocks(width) * 4);
+  s.gate_up = take(pairs * 2 * ff * 2);
+  s.a = take(pairs * f8_ld(ff));
+  s.a_scale = take(pairs * f8_blocks(ff) * 4);
+  s.y = take(pairs * width * 2);
+  s.bytes = at;
+  return s;
+}
+
+int check_pairs(const char* what, int64_t rows, int64_t top, int64_t experts) {
+  B200_CHECK_ARG(rows >= 1 && top >= 1 && experts >= 1 && experts <= kMaxExperts && rows < 1 << 24 && top <= experts && rows * top < 1 << 24,
+                 "%s: %lld rows with %lld of %lld experts out of range", what, (long long)rows, (long long)top, (long long)experts);
+  return B200_OK;
+}
+
+}  // namespace
+
+int launch_expert_order(int32_t* starts, int32_t* source, int32_t* place, const int32_t* chosen, int64_t rows, int64_t top, int64_t experts, cudaStream_t st) {
+  static PerDevice attrs;
+  B200_CUDA(attrs([] { return cudaFuncSetAttribute(expert_order_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kOrderWarps + 1) * kMaxExperts * 4); }));
+  B200_CUDA(launch_pdl(expert_order_kernel, dim3(1), dim3(32 * kOrderWarps), (size_t)(kOrderWarps + 1) * experts * 4, st, op_pdl(st), starts, source, place, chosen,
+                       (int)(rows * top), (int)top, (int)experts));
+  return B200_OK;
+}
+
+int launch_expert_combine(void* out, const void* y, const int32_t* place, const float* weights, int64_t rows, int64_t top, int64_t n, cudaStream_t st) {
+  const bool wide = n % 8 == 0 && aligned16(out, y);
+  const int64_t threads = rows * (wide ? n / 8 : n);
+  B200_CUDA(launch_pdl(wide ? expert_combine_kernel<true> : expert_combine_kernel<false>, dim3((unsigned)std::min<int64_t>((threads + 255) / 256, 148 * 8)), dim3(256),
+                       0, st, op_pdl(st), (__nv_bfloat16*)out, (const __nv_bfloat16*)y, place, weights, rows, (int)top, (int)n));
+  return B200_OK;
+}
+
+}  // namespace b200
+
+extern "C" {
+
+int b200_expert_order(int32_t* starts, int32_t* source, int32_t* place, const int32_t* chosen, int64_t rows, int64_t top, int64_t experts, void* stream) {
+  using namespace b200;
+  int rc = op_check();
+  if (rc != B200_OK || (rc = check_pairs("expert_order", rows, top, experts)) != B200_OK) return rc;
+  B200_CHECK_ARG(starts && source && place && chosen, "expert_order: null pointer");
+  return launch_expert_order(starts, source, place, chosen, rows, top, experts, (cudaStream_t)stream);
+}
+
+int b200_expert_combine_bf16(void* out, const void* y, const int32_t* place, const float* weights, int64_t rows, int64_t top, int64_t n, void* stream) {
+  using namespace b200;
+  int rc = op_check();
+  if (rc != B200_OK || (rc = check_pairs("expert_combine", rows, top, kMaxExperts)) != B200_OK) return rc;
+  B200_CHECK_ARG(out && y && place && weights && n >= 1 && n <= 1 << 24, "expert_combine: rows of %lld out of range, or a null pointer", (long long)n);
+  return launch_expert_combine(out, y, place, weights, rows, top, n, (cudaStream_t)stream);
+}
+
+int64_t b200_experts_f8_workspace_bytes(int64_t rows, int64_t top, int64_t experts, int64_t width, int64_t ff) {
+  using namespace b200;
+  if (rows < 1 || top < 1 || experts < 1 || width < 1 || ff < 1 || rows >= 1 << 24 || experts > kMaxExperts || top > experts || width > 1 << 20 || ff > 1 << 20) return -1;
+  return experts_space(rows, top, experts, width, ff).bytes;
+}
+
+int b200_experts_f8_bf16(void* out, const void* x, const int32_t* chosen, const float* weights, const b200_f8_weight* w_in, const b200_f8_weight* w_out, int64_t rows,
+                         int64_t top, void* workspace, void* stream) {
+  using namespace b200;
+  int rc = op_check();
+  if (rc != B200_OK) return rc;
+  B200_CHECK_ARG(out && x && chosen && weights && w_in && w_out && w_in->q && w_in->scale && w_out->q && w_out->scale, "experts_f8: null pointer");
+  const int64_t experts = w_in->experts, width = w_in->k, ff = w_out->k;
+  if ((rc = check_pairs("experts_f8", rows, top, experts)) != B200_OK) return rc;
+  B200_CHECK_ARG(w_out->experts == experts && w_in->n == 2 * ff && w_out->n == width && width >= 1 && ff >= 1 && width <= 1 << 20 && ff <= 1 << 19 &&
+                     experts * std::max(2 * ff, width) < 1ll << 31,
+                 "experts_f8: %d matrices [%d, %d] and %d [%d, %d]", (int)w_in->experts, (int)w_in->n, (int)w_in->k, (int)w_out->experts, (int)w_out->n, (int)w_out->k);
+  B200_CHECK_ARG(workspace && aligned16(workspace, w_in->q, w_out->q), "experts_f8: workspace and weights must be 16-byte aligned");
+  const ExpertsSpace s = experts_space(rows, top, experts, width, ff);
+  const int64_t pairs = rows * top;
+  uint8_t* const ws = (uint8_t*)workspace;
+  const cudaStream_t st = (cudaStream_t)stream;
+  auto ints = [&](int64_t at) { return (int32_t*)(ws + at); };
+  auto floats = [&](int64_t at) { return (float*)(ws + at); };
+  if ((rc = launch_expert_order(ints(s.starts), ints(s.source), ints(s.place), chosen, rows, top, experts, st)) != B200_OK) return rc;
+  if ((rc = launch_f8_rows(ws + s.q, floats(s.scale), x, width, rows, ints(s.source), pairs, width, st)) != B200_OK) return rc;
+  if ((rc = launch_group_product({ws + s.gate_up, ws + s.q, floats(s.scale), w_in->q, w_in->scale, ints(s.starts), nullptr, pairs, experts, 2 * ff, width}, st)) != B200_OK)
+    return rc;
+  if ((rc = launch_silu_mul_f8(ws + s.a, floats(s.a_scale), ws + s.gate_up, pairs, ff, st)) != B200_OK) return rc;
+  if ((rc = launch_group_product({ws + s.y, ws + s.a, floats(s.a_scale), w_out->q, w_out->scale, ints(s.starts), nullptr, pairs, experts, width, ff}, st)) != B200_OK)
+    return rc;
+  return launch_expert_combine(out, ws + s.y, ints(s.place), weights, rows, top, width, st);
+}
+
+}  // extern "C"

@@ -1,0 +1,288 @@
+// f8_rows.cu — rows of numbers → rows in 8 bits with a scale for every 128 entries, from bf16 rows (which may be picked by a list), from an RMS norm with or
+// without the residual's sum in front, from a SiLU product; and back to fp32.
+//
+//   t: the row's numbers in fp32;  of every block of 128:  s = max(fp32(max|t| / 448), 2^-126),  value = e4m3(fp32(t / s))
+//
+// A norm needs no second look at its row: with z the row, t = z·w and inv = rsqrt(mean(z²) + eps) the normed row is inv·t, its blocks' largest entries
+// are inv·max|t|, and in value = inv·t / (inv·s) the inv cancels.  So values come from t alone (a product of two bf16 numbers: exact) and
+// inv only meets the scale.  All of it is bound by HBM: a row is read once, 16 bytes a lane, and sixteen lanes that hold a block find its largest entry by
+// four shuffles.
+#include "f8.cuh"
+
+#include <algorithm>
+
+namespace b200 {
+
+namespace {
+
+// eight entries i … i + 7 of a row of k bf16; zero behind its end.  WIDE: rows are whole 16-byte pieces.
+template <bool WIDE>
+__device__ __forceinline__ void load8(const __nv_bfloat16* row, int i, int k, float (&v)[8]) {
+  if constexpr (WIDE) {
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if (i < k) u = *reinterpret_cast<const uint4*>(row + i);
+    unpack8(u, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = i + e < k ? bf16_to_f(row[i + e]) : 0.f;
+  }
+}
+
+// value and scale of eight entries of a block; a row's last piece may reach past its ld bytes
+__device__ __forceinline__ void store8(uint8_t* q, float* scale, int64_t row, int64_t rows, int i, int64_t ld, int blocks, const float (&t)[8], float s, float factor) {
+  if (i < ld) *reinterpret_cast<uint2*>(q + row * ld + i) = f8_pack8(t, s);
+  if (i % kF8Block == 0 && i / kF8Block < blocks) scale[(int64_t)(i / kF8Block) * rows + row] = s * factor;
+}
+
+// Sixteen lanes to a block.  SILU: x rows are [gate | up], k entries each.
+template <bool WIDE, bool SILU>
+__global__ void __launch_bounds__(256) f8_rows_kernel(uint8_t* __restrict__ q, float* __restrict__ scale, const __nv_bfloat16* __restrict__ x, int64_t ld_x,
+                                                      int64_t x_rows, const int32_t* __restrict__ index, int64_t rows, int k, int blocks) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t ld = f8_ld(k), all = rows * blocks;
+  const int part = threadIdx.x % 16;
+  for (int64_t first = (int64_t)blockIdx.x * 16; first < all; first += (int64_t)gridDim.x * 16) {   // (lanes of a warp stay together)
+    const int64_t at = first + threadIdx.x / 16;
+    const int64_t row = at / blocks;
+    const int i = (int)(at % blocks) * kF8Block + part * 8;
+    float t[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t[e] = 0.f;
+    if (at < all) {
+      const int64_t from = index == nullptr ? row : index[row];
+      if (from >= 0 && from < x_rows) {
+        load8<WIDE>(x + from * ld_x, i, k, t);
+        if constexpr (SILU) {
+          float u[8];
+          load8<WIDE>(x + from * ld_x + k, i, k, u);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) t[e] = silu_f(t[e]) * u[e];
+        }
+      }
+    }
+    const float s = f8_scale(block_max(magnitude8(t)));
+    if (at < all) store8(q, scale, row, rows, i, ld, blocks, t, s, 1.f);
+  }
+}
+
+// One CTA to a row, V pieces of 8 entries a thread.  The sum may lie where the row or the residual does: an entry is read and written by one thread.
+template <bool WIDE, int THREADS, int V>
+__global__ void __launch_bounds__(THREADS) norm_f8_kernel(uint8_t* __restrict__ q, float* __restrict__ scale, __nv_bfloat16* sum,
+                                                          const __nv_bfloat16* x, const __nv_bfloat16* residual,
+                                                          const __nv_bfloat16* __restrict__ w, int64_t rows, int dim, int blocks, float eps) {
+  __shared__ float red[THREADS / 32];
+  pdl_wait();
+  pdl_trigger();
+  const int64_t row = blockIdx.x, base = row * dim, ld = f8_ld(dim);
+  float t[V][8];
+  float ss = 0.f;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int i = (threadIdx.x + j * THREADS) * 8;
+    load8<WIDE>(x + base, i, dim, t[j]);
+    if (residual != nullptr) {
+      float r[8];
+      load8<WIDE>(residual + base, i, dim, r);
+      uint32_t z[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        z[e] = pack2(t[j][2 * e] + r[2 * e], t[j][2 * e + 1] + r[2 * e + 1]);
+        t[j][2 * e] = bf16_lo(z[e]);
+        t[j][2 * e + 1] = bf16_hi(z[e]);
+      }
+      if constexpr (WIDE) {
+        if (i < dim) *reinterpret_cast<uint4*>(sum + base + i) = make_uint4(z[0], z[1], z[2], z[3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (i + e < dim) sum[base + i + e] = f_to_bf16(t[j][e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss = fmaf(t[j][e], t[j][e], ss);
+    if (w != nullptr) {
+      float g[8];
+      load8<WIDE>(w, i, dim, g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) t[j][e] *= g[e];
+    }
+  }
+  ss = warp_sum(ss);
+  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = ss;
+  __syncthreads();
+  float tot = 0.f;
+#pragma unroll
+  for (int i = 0; i < THREADS / 32; ++i) tot += red[i];
+  const float inv = __frsqrt_rn(tot / (float)dim + eps);
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const float s = f8_scale(block_max(magnitude8(t[j])));
+    store8(q, scale, row, rows, (threadIdx.x + j * THREADS) * 8, ld, blocks, t[j], s, inv);
+  }
+}
+
+// Rows that no CTA holds in registers: once over them for the sum, a second time (from L2) for the values.
+template <bool WIDE>
+__global__ void __launch_bounds__(1024) norm_f8_long_kernel(uint8_t* __restrict__ q, float* __restrict__ scale, __nv_bfloat16* sum,
+                                                            const __nv_bfloat16* x, const __nv_bfloat16* residual,
+                                                            const __nv_bfloat16* __restrict__ w, int64_t rows, int dim, int blocks, float eps) {
+  __shared__ float red[32];
+  pdl_wait();
+  pdl_trigger();
+  const int64_t row = blockIdx.x, base = row * dim, ld = f8_ld(dim);
+  float ss = 0.f;
+  auto entry = [&](int i, float (&t)[8]) {
+    load8<WIDE>(x + base, i, dim, t);
+    if (residual != nullptr) {
+      float r[8];
+      load8<WIDE>(residual + base, i, dim, r);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) t[e] = round_bf16(t[e] + r[e]);
+    }
+  };
+  for (int i = threadIdx.x * 8; i < dim; i += 8192) {
+    float t[8];
+    entry(i, t);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss = fmaf(t[e], t[e], ss);
+  }
+  ss = warp_sum(ss);
+  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = ss;
+  __syncthreads();
+  const float inv = __frsqrt_rn(warp_sum(red[threadIdx.x % 32]) / (float)dim + eps);
+  for (int first = 0; first < blocks * kF8Block; first += 8192) {   // (all lanes take every turn)
+    const int i = first + threadIdx.x * 8;
+    float t[8], g[8];
+    entry(i, t);
+    if (residual != nullptr) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (i + e < dim) sum[base + i + e] = f_to_bf16(t[e]);
+    }
+    if (w != nullptr) {
+      load8<WIDE>(w, i, dim, g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) t[e] *= g[e];
+    }
+    const float s = f8_scale(block_max(magnitude8(t)));
+    store8(q, scale, row, rows, i, ld, blocks, t, s, inv);
+  }
+}
+
+template <bool WIDE>
+__global__ void __launch_bounds__(256) f8_dequant_kernel(float* __restrict__ out, const uint8_t* __restrict__ q, const float* __restrict__ scale, int64_t rows, int k,
+                                                         int pieces) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t ld = f8_ld(k), all = rows * pieces;
+  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < all; at += (int64_t)gridDim.x * 256) {
+    const int64_t row = at / pieces;
+    const int i = (int)(at % pieces) * 8;
+    const uint2 w = *reinterpret_cast<const uint2*>(q + row * ld + i);
+    const float s = scale[(int64_t)(i / kF8Block) * rows + row];
+    const float4 a = f8_unpack4(w.x), b = f8_unpack4(w.y);
+    float* const o = out + row * k + i;
+    if constexpr (WIDE) {
+      *reinterpret_cast<float4*>(o) = make_float4(a.x * s, a.y * s, a.z * s, a.w * s);
+      if (i + 4 < k) *reinterpret_cast<float4*>(o + 4) = make_float4(b.x * s, b.y * s, b.z * s, b.w * s);
+    } else {
+      const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (i + e < k) o[e] = v[e] * s;
+    }
+  }
+}
+
+unsigned ctas_for(int64_t work, int64_t each, int64_t most) { return (unsigned)std::max<int64_t>(1, std::min((work + each - 1) / each, most)); }
+
+template <bool SILU>
+int launch_rows(void* q, float* scale, const void* x, int64_t ld_x, int64_t x_rows, const int32_t* index, int64_t rows, int64_t k, cudaStream_t st) {
+  const int blocks = (int)f8_blocks(k);
+  const bool wide = k % 8 == 0 && ld_x % 8 == 0 && aligned16(x);
+  const auto f = wide ? f8_rows_kernel<true, SILU> : f8_rows_kernel<false, SILU>;
+  B200_CUDA(launch_pdl(f, dim3(ctas_for(rows * blocks, 16, 148 * 8)), dim3(256), 0, st, op_pdl(st), (uint8_t*)q, scale, (const __nv_bfloat16*)x, ld_x, x_rows, index,
+                       rows, (int)k, blocks));
+  return B200_OK;
+}
+
+template <bool WIDE>
+auto norm_kernel(int64_t dim, int* threads) {
+  const int64_t pieces = f8_blocks(dim) * 16;   // whole blocks: their lanes stay together
+  struct Form { int threads, v; decltype(&norm_f8_kernel<WIDE, 64, 1>) f; };
+  const Form forms[] = {{64, 1, norm_f8_kernel<WIDE, 64, 1>}, {128, 1, norm_f8_kernel<WIDE, 128, 1>}, {256, 1, norm_f8_kernel<WIDE, 256, 1>},
+                        {256, 2, norm_f8_kernel<WIDE, 256, 2>}, {512, 2, norm_f8_kernel<WIDE, 512, 2>}, {512, 4, norm_f8_kernel<WIDE, 512, 4>}};
+  for (const Form& f : forms)
+    if (pieces <= f.threads * f.v) {
+      *threads = f.threads;
+      return f.f;
+    }
+  *threads = 1024;
+  return decltype(&norm_f8_kernel<WIDE, 64, 1>)(norm_f8_long_kernel<WIDE>);
+}
+
+int check_rows(const char* what, const void* q, const void* scale, int64_t rows, int64_t k) {
+  B200_CHECK_ARG(q && scale && rows >= 1 && k >= 1 && rows < 1ll << 31 && k <= 1 << 24, "%s: %lld rows of %lld out of range, or a null pointer", what, (long long)rows,
+                 (long long)k);
+  B200_CHECK_ARG(aligned16(q), "%s: rows of 8 bits must be 16-byte aligned", what);
+  return B200_OK;
+}
+
+}  // namespace
+
+int launch_f8_rows(void* q, float* scale, const void* x, int64_t ld_x, int64_t x_rows, const int32_t* index, int64_t rows, int64_t k, cudaStream_t st) {
+  return launch_rows<false>(q, scale, x, ld_x, x_rows, index, rows, k, st);
+}
+int launch_silu_mul_f8(void* q, float* scale, const void* gate_up, int64_t rows, int64_t n, cudaStream_t st) {
+  return launch_rows<true>(q, scale, gate_up, 2 * n, rows, nullptr, rows, n, st);
+}
+
+}  // namespace b200
+
+extern "C" {
+
+int b200_f8_rows_bf16(void* q, float* scale, const void* x, int64_t ld_x, int64_t x_rows, const int32_t* index, int64_t rows, int64_t k, void* stream) {
+  using namespace b200;
+  int rc = op_check();
+  if (rc != B200_OK || (rc = check_rows("f8_rows", q, scale, rows, k)) != B200_OK) return rc;
+  B200_CHECK_ARG(x && ld_x >= k && ld_x < 1ll << 40 && x_rows >= (index ? 1 : rows) && x_rows < 1ll << 31, "f8_rows: %lld rows %lld apart, or a null pointer",
+                 (long long)x_rows, (long long)ld_x);
+  return launch_f8_rows(q, scale, x, ld_x, x_rows, index, rows, k, (cudaStream_t)stream);
+}
+
+int b200_silu_mul_f8(void* q, float* scale, const void* gate_up, int64_t rows, int64_t n, void* stream) {
+  using namespace b200;
+  int rc = op_check();
+  if (rc != B200_OK || (rc = check_rows("silu_mul_f8", q, scale, rows, n)) != B200_OK) return rc;
+  B200_CHECK_ARG(gate_up, "silu_mul_f8: null pointer");
+  return launch_silu_mul_f8(q, scale, gate_up, rows, n, (cudaStream_t)stream);
+}
+
+int b200_rmsnorm_f8(void* q, float* scale, void* sum, const void* x, const void* residual, const void* w, int64_t rows, int64_t dim, float eps, void* stream) {
+  using namespace b200;
+  int rc = op_check();
+  if (rc != B200_OK || (rc = check_rows("rmsnorm_f8", q, scale, rows, dim)) != B200_OK) return rc;
+  B200_CHECK_ARG(x && (residual == nullptr) == (sum == nullptr), "rmsnorm_f8: null pointer, or a sum without a residual");
+  int threads = 0;
+  const bool wide = dim % 8 == 0 && aligned16(x, residual, sum, w);
+  const auto f = wide ? norm_kernel<true>(dim, &threads) : norm_kernel<false>(dim, &threads);
+  const cudaStream_t st = (cudaStream_t)stream;
+  B200_CUDA(launch_pdl(f, dim3((unsigned)rows), dim3(threads), 0, st, op_pdl(st), (uint8_t*)q, scale, (__nv_bfloat16*)sum, (const __nv_bfloat16*)x,
+                       (const __nv_bfloat16*)residual, (const __nv_bfloat16*)w, rows, (int)dim, (int)f8_blocks(dim), eps));
+  return B200_OK;
+}
+
+int b200_f8_rows_dequant(float* out, const void* q, const float* scale, int64_t rows, int64_t k, void* stream) {
+  using namespace b200;
+  int rc = op_check();
+  if (rc != B200_OK || (rc = check_rows("f8_rows_dequant", q, scale, rows, k)) != B200_OK) return rc;
+  B200_CHECK_ARG(out, "f8_rows_dequant: null pointer");
+  const int pieces = (int)((k + 7) / 8);
+  const cudaStream_t st = (cudaStream_t)stream;
+  const auto f = k % 4 == 0 && aligned16(out) ? f8_dequant_kernel<true> : f8_dequant_kernel<false>;
+  B200_CUDA(launch_pdl(f, dim3(ctas_for(rows * pieces, 256, 148 * 16)), dim3(256), 0, st, op_pdl(st), out, (const uint8_t*)q, scale, rows, (int)k, pieces));
+  return B200_OK;
+}
+
+}  // extern "C"

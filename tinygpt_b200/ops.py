@@ -382,6 +382,333 @@ def w4_dequantize(weight: W4Weight) -> torch.Tensor:
     return out
 
 
+# ---- rows and weights of 8 bits, products grouped by expert (csrc/f8_rows.cu, group_gemm.cu, experts.cu)
+F8_BLOCK, MAX_EXPERTS = 128, 1024
+_F8 = torch.float8_e4m3fn
+
+
+class F8Rows(NamedTuple):
+    """Rows [..., k] in 8 bits: x[..., j] = q[..., j]·scale[j // 128, row].  Made by f8_rows, rms_norm_f8, add_rms_norm_f8 and silu_mul_f8."""
+    q: torch.Tensor        # float8_e4m3fn [..., k rounded up to 16], zeros behind k
+    scale: torch.Tensor    # fp32 [ceil(k / 128), rows]
+    k: int
+
+
+class F8Weight(NamedTuple):
+    """A Linear's weight in 8 bits, or those of many experts, laid out by f8_pack or f8_quantize: W[.., i, j] = value·scale[.., i // 128, j // 128]."""
+    q: torch.Tensor        # float8_e4m3fn [n, k rounded up to 16] or [experts, n, ..]
+    scale: torch.Tensor    # fp32 [ceil(n / 128), ceil(k / 128)] or [experts, ..]
+    n: int
+    k: int
+
+
+def _up(a: int, b: int) -> int:
+    return -(-a // b)
+
+
+def f8_pack(values: torch.Tensor, scale: torch.Tensor) -> F8Weight:
+    """The layout linear_f8 takes, made once per weight: values float8_e4m3fn [n, k] or [experts, n, k], scale fp32, one for every block of 128 × 128."""
+    if values.dim() not in (2, 3) or values.dtype != _F8:
+        raise B200Error(f"f8_pack: values must be float8_e4m3fn [n, k] or [experts, n, k], got {values.dtype} {tuple(values.shape)}")
+    *lead, n, k = values.shape
+    if n < 1 or k < 1 or (lead and not 1 <= lead[0] <= MAX_EXPERTS):
+        raise B200Error(f"f8_pack: W {tuple(values.shape)}: up to {MAX_EXPERTS} matrices, none of them empty")
+    want = (*lead, _up(n, F8_BLOCK), _up(k, F8_BLOCK))
+    if scale.dtype != torch.float32 or tuple(scale.shape) != want or scale.device != values.device:
+        raise B200Error(f"f8_pack: scale must be fp32 {list(want)} beside the values, got {scale.dtype} {tuple(scale.shape)}")
+    q = values.contiguous()
+    if k % 16:
+        q = torch.zeros(*lead, n, _up(k, 16) * 16, dtype=torch.uint8, device=values.device)
+        q[..., :k] = values.view(torch.uint8)
+        q = q.view(_F8)
+    elif q.data_ptr() % 16:
+        q = q.clone()
+    return F8Weight(q, scale.contiguous(), n, k)
+
+
+def f8_quantize(weight: torch.Tensor) -> F8Weight:
+    """The nearest 8-bit weight of a matrix [n, k] or of matrices [experts, n, k] (bf16 or fp32): a block's largest entry becomes 448."""
+    if weight.dim() not in (2, 3) or not weight.dtype.is_floating_point or weight.numel() == 0:
+        raise B200Error(f"f8_quantize: expected matrices, got {weight.dtype} {tuple(weight.shape)}")
+    if not bool(torch.isfinite(weight).all()):
+        raise B200Error("f8_quantize: the weight is not finite")
+    *lead, n, k = weight.shape
+    w = torch.nn.functional.pad(weight.float(), (0, -k % F8_BLOCK, 0, -n % F8_BLOCK))
+    w = w.view(*lead, _up(n, F8_BLOCK), F8_BLOCK, _up(k, F8_BLOCK), F8_BLOCK)
+    top = w.abs().amax((-3, -1))
+    scale = (top / torch.full_like(top, 448.0)).clamp(min=2.0 ** -126)
+    q = (w / scale[..., :, None, :, None]).clamp(-448, 448).to(_F8).view(torch.uint8)
+    q = q.view(*lead, w.shape[-4] * F8_BLOCK, w.shape[-2] * F8_BLOCK)[..., :n, :k].contiguous()
+    return f8_pack(q.view(_F8), scale)
+
+
+def f8_dequantize(weight: F8Weight) -> torch.Tensor:
+    """W as fp32 [n, k] or [experts, n, k]."""
+    _f8_fits(weight, "f8_dequantize")
+    s = weight.scale.repeat_interleave(F8_BLOCK, -2)[..., : weight.n, :].repeat_interleave(F8_BLOCK, -1)[..., : weight.k]
+    return weight.q[..., : weight.k].float() * s
+
+
+def _f8_fits(w: F8Weight, what: str) -> int:
+    """How many matrices the weight has, if its parts fit each other."""
+    if w.__class__ is not F8Weight:
+        raise B200Error(f"{what}: the weight must come from f8_pack or f8_quantize")
+    lead, n, k = tuple(w.q.shape[:-2]), w.n, w.k
+    if w.q.dim() not in (2, 3) or w.q.dtype != _F8 or w.scale.dtype != torch.float32 or not (1 <= n <= 1 << 20 and 1 <= k <= 1 << 24):
+        raise B200Error(f"{what}: W [{n}, {k}] out of range, or parts of other types than f8_pack's")
+    if tuple(w.q.shape) != (*lead, n, _up(k, 16) * 16) or tuple(w.scale.shape) != (*lead, _up(n, F8_BLOCK), _up(k, F8_BLOCK)):
+        raise B200Error(f"{what}: the weight's parts do not fit W [{n}, {k}]")
+    experts = lead[0] if lead else 1
+    if not 1 <= experts <= MAX_EXPERTS or experts * n >= 1 << 31:
+        raise B200Error(f"{what}: {experts} matrices of {n} rows out of range")
+    return experts
+
+
+def _f8_desc(w: F8Weight, what: str, dims: int):
+    """The weight's descriptor, and the tensors that it points into."""
+    from ._lib import F8Desc
+    experts = _f8_fits(w, what)
+    if w.q.dim() != dims:
+        raise B200Error(f"{what}: takes {'one matrix' if dims == 2 else 'the matrices of experts'}, got values {tuple(w.q.shape)}")
+    q, scale = _chk(w.q, f"{what}.q", _F8), _chk(w.scale, f"{what}.scale", torch.float32)
+    return F8Desc(q.data_ptr(), scale.data_ptr(), w.n, w.k, experts), (q, scale)
+
+
+def _f8_empty(shape, k: int, device) -> F8Rows:
+    rows = 1
+    for s in shape:
+        rows *= s
+    return F8Rows(torch.empty(*shape, _up(k, 16) * 16, dtype=_F8, device=device), torch.empty(_up(k, F8_BLOCK), rows, dtype=torch.float32, device=device), k)
+
+
+def _f8_take(x: F8Rows, what: str):
+    """Rows in 8 bits, checked: (q, scale, shape without the last, rows)."""
+    q, scale = _chk(x.q, f"{what}.q", _F8), _chk(x.scale, f"{what}.scale", torch.float32)
+    if q.dim() < 1 or not 1 <= x.k <= 1 << 24 or q.shape[-1] != _up(x.k, 16) * 16:
+        raise B200Error(f"{what}: values {tuple(q.shape)} are no rows of {x.k} in 8 bits")
+    rows = q.numel() // q.shape[-1]
+    if tuple(scale.shape) != (_up(x.k, F8_BLOCK), rows):
+        raise B200Error(f"{what}: scale must be [{_up(x.k, F8_BLOCK)}, {rows}], got {tuple(scale.shape)}")
+    if q.data_ptr() % 16:
+        q = q.clone()
+    return q, scale, tuple(q.shape[:-1]), rows
+
+
+def _f8_width(x: torch.Tensor, what: str) -> int:
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= 1 << 24:
+        raise B200Error(f"{what}: rows of {tuple(x.shape)}")
+    return x.shape[-1]
+
+
+def f8_rows(x: torch.Tensor, index: Optional[torch.Tensor] = None) -> F8Rows:
+    """Rows of x bf16 [..., k] in 8 bits, block by block of 128: s = max(fp32(max|x| / 448), 2^-126), value = e4m3(fp32(x / s)).  index int32 [rows]: row i of the
+    result is row index[i] of x [rows of x, k], zeros where that is none of them (as expert_order's source has it)."""
+    if not x.is_cuda or x.dtype != torch.bfloat16:
+        _chk(x, "f8_rows.x")
+    k = _f8_width(x, "f8_rows")
+    if x.dim() != 2 or x.stride(1) != 1 or x.stride(0) < k:   # (rows of a matrix may lie apart)
+        x = x.contiguous()
+    x_rows = x.numel() // k
+    if index is None:
+        out = _f8_empty(x.shape[:-1], k, x.device)
+    else:
+        index = _chk(index, "f8_rows.index", torch.int32)
+        if index.dim() != 1 or x.dim() != 2:
+            raise B200Error(f"f8_rows: a list picks rows of a matrix, got {tuple(index.shape)} and {tuple(x.shape)}")
+        out = _f8_empty((index.shape[0],), k, x.device)
+    _same_device("f8_rows", x, index)
+    rows = out.scale.shape[1]
+    if rows and x_rows:
+        check(lib().b200_f8_rows_bf16(out.q.data_ptr(), out.scale.data_ptr(), x.data_ptr(), x.stride(0) if x.dim() == 2 and x_rows > 1 else k, x_rows, _ptr(index),
+                                      rows, k, _stream()), "b200_f8_rows_bf16")
+    elif rows:
+        out.q.view(torch.uint8).zero_()
+        out.scale.fill_(2.0 ** -126)
+    return out
+
+
+def f8_rows_dequantize(x: F8Rows) -> torch.Tensor:
+    """fp32 [..., k]: what the 8 bits stand for."""
+    q, scale, shape, rows = _f8_take(x, "f8_rows_dequantize")
+    _same_device("f8_rows_dequantize", q, scale)
+    out = torch.empty(*shape, x.k, dtype=torch.float32, device=q.device)
+    if rows:
+        check(lib().b200_f8_rows_dequant(out.data_ptr(), q.data_ptr(), scale.data_ptr(), rows, x.k, _stream()), "b200_f8_rows_dequant")
+    return out
+
+
+def _norm_f8(x, residual, weight, eps, what):
+    x = _chk(x, f"{what}.x")
+    dim = _f8_width(x, what)
+    if residual is not None:
+        residual = _chk(residual, f"{what}.residual")
+        if residual.shape != x.shape:
+            raise B200Error(f"{what}: x {tuple(x.shape)} and the residual {tuple(residual.shape)} differ")
+    if weight is not None:
+        weight = _chk(weight, f"{what}.weight")
+        if weight.numel() != dim:
+            raise B200Error(f"{what}: a weight of {weight.numel()} for rows of {dim}")
+    _same_device(what, x, residual, weight)
+    out, total = _f8_empty(x.shape[:-1], dim, x.device), None if residual is None else torch.empty_like(x)
+    rows = out.scale.shape[1]
+    if rows:
+        check(lib().b200_rmsnorm_f8(out.q.data_ptr(), out.scale.data_ptr(), _ptr(total), x.data_ptr(), _ptr(residual), _ptr(weight), rows, dim, float(eps), _stream()),
+              "b200_rmsnorm_f8")
+    return out, total
+
+
+def rms_norm_f8(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float) -> F8Rows:
+    """rms_norm whose result leaves in 8 bits: t = x·weight in blocks of 128 as f8_rows has them, their scales times rsqrt(mean(x²) + eps)."""
+    return _norm_f8(x, None, weight, eps, "rms_norm_f8")[0]
+
+
+def add_rms_norm_f8(x: torch.Tensor, residual: torch.Tensor, weight: Optional[torch.Tensor], eps: float):
+    """The norm between two blocks in one pass: z = bf16(x + residual) → (rms_norm_f8 of z, z)."""
+    if residual is None:
+        raise B200Error("add_rms_norm_f8: no residual")
+    return _norm_f8(x, residual, weight, eps, "add_rms_norm_f8")
+
+
+def silu_mul_f8(x: torch.Tensor) -> F8Rows:
+    """silu_mul in 8 bits: last dim = [gate | up], t = silu(gate)·up in fp32, blocks of 128 as f8_rows has them."""
+    x = _chk(x, "silu_mul_f8.x")
+    if x.dim() < 1 or x.shape[-1] % 2 or x.shape[-1] < 2:
+        raise B200Error(f"silu_mul_f8: last dimension must be even, got {tuple(x.shape)}")
+    n = x.shape[-1] // 2
+    _same_device("silu_mul_f8", x)
+    out = _f8_empty(x.shape[:-1], n, x.device)
+    rows = out.scale.shape[1]
+    if rows:
+        check(lib().b200_silu_mul_f8(out.q.data_ptr(), out.scale.data_ptr(), x.data_ptr(), rows, n, _stream()), "b200_silu_mul_f8")
+    return out
+
+
+def linear_f8(x, weight: F8Weight, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """linear over a weight of 8 bits: x F8Rows, or bf16 [..., k] (which f8_rows makes 8-bit rows of first) → bf16(x·Wᵀ + bias) [..., n], sums of 128 products scaled
+    and added in fp32, rounded once."""
+    import ctypes as C
+    d, parts = _f8_desc(weight, "linear_f8", 2)
+    if x.__class__ is not F8Rows:
+        x = f8_rows(_chk(x, "linear_f8.x"))
+    q, scale, shape, rows = _f8_take(x, "linear_f8.x")
+    n, k = weight.n, weight.k
+    if x.k != k:
+        raise B200Error(f"linear_f8: rows of {x.k} do not match W[{n}, {k}]")
+    if bias is not None:
+        bias = _chk(bias, "linear_f8.bias")
+        if bias.numel() != n:
+            raise B200Error(f"linear_f8: a bias of {bias.numel()} for W[{n}, {k}]")
+    _same_device("linear_f8", q, scale, bias, *parts)
+    y = torch.empty(*shape, n, dtype=torch.bfloat16, device=q.device)
+    if rows:
+        check(lib().b200_f8_linear_bf16(y.data_ptr(), q.data_ptr(), scale.data_ptr(), C.byref(d), _ptr(bias), rows, _stream()), "b200_f8_linear_bf16")
+    return y
+
+
+def _starts(starts, experts: int, what: str) -> torch.Tensor:
+    starts = _chk(starts, f"{what}.starts", torch.int32)
+    if tuple(starts.shape) != (experts + 1,):
+        raise B200Error(f"{what}: {experts} experts take {experts + 1} starts, got {tuple(starts.shape)}")
+    return starts
+
+
+def grouped_linear(x: torch.Tensor, weight: torch.Tensor, starts: torch.Tensor) -> torch.Tensor:
+    """Products grouped by expert: rows starts[e] … starts[e + 1] − 1 of x bf16 [rows, k] meet weight[e] of bf16 [experts, n, k] → bf16 [rows, n], fp32 sums, rounded
+    once.  starts int32 [experts + 1] on the device, not falling; a group may be empty, rows of no group come out as zeros."""
+    x, weight = _chk(x, "grouped_linear.x"), _chk(weight, "grouped_linear.weight")
+    if x.dim() != 2 or weight.dim() != 3 or x.shape[1] != weight.shape[2]:
+        raise B200Error(f"grouped_linear: x {tuple(x.shape)} does not match weights {tuple(weight.shape)}")
+    experts, n, k = weight.shape
+    if not 1 <= experts <= MAX_EXPERTS or n < 1 or k < 8 or k % 8:
+        raise B200Error(f"grouped_linear: {experts} matrices [{n}, {k}]: up to {MAX_EXPERTS}, k a multiple of 8")
+    starts = _starts(starts, experts, "grouped_linear")
+    _same_device("grouped_linear", x, weight, starts)
+    x, weight = (t.clone() if t.data_ptr() % 16 else t for t in (x, weight))
+    y = torch.empty(x.shape[0], n, dtype=torch.bfloat16, device=x.device)
+    if x.shape[0]:
+        check(lib().b200_grouped_bf16(y.data_ptr(), x.data_ptr(), weight.data_ptr(), starts.data_ptr(), x.shape[0], experts, n, k, _stream()), "b200_grouped_bf16")
+    return y
+
+
+def grouped_linear_f8(x, weight: F8Weight, starts: torch.Tensor) -> torch.Tensor:
+    """grouped_linear over rows and weights of 8 bits: x F8Rows [rows, k], or bf16 (which f8_rows makes 8-bit rows of first), weight of experts."""
+    import ctypes as C
+    d, parts = _f8_desc(weight, "grouped_linear_f8", 3)
+    if x.__class__ is not F8Rows:
+        x = f8_rows(_chk(x, "grouped_linear_f8.x"))
+    q, scale, shape, rows = _f8_take(x, "grouped_linear_f8.x")
+    if len(shape) != 1 or x.k != weight.k:
+        raise B200Error(f"grouped_linear_f8: rows [{', '.join(map(str, shape))}, {x.k}] do not match weights [{d.experts}, {weight.n}, {weight.k}]")
+    starts = _starts(starts, d.experts, "grouped_linear_f8")
+    _same_device("grouped_linear_f8", q, scale, starts, *parts)
+    y = torch.empty(rows, weight.n, dtype=torch.bfloat16, device=q.device)
+    if rows:
+        check(lib().b200_f8_grouped_bf16(y.data_ptr(), q.data_ptr(), scale.data_ptr(), C.byref(d), starts.data_ptr(), rows, _stream()), "b200_f8_grouped_bf16")
+    return y
+
+
+def _pairs(chosen, experts: int, what: str):
+    chosen = _chk(chosen, f"{what}.chosen", torch.int32)
+    if chosen.dim() != 2 or not 1 <= int(experts) <= MAX_EXPERTS or not 1 <= chosen.shape[1] <= experts:
+        raise B200Error(f"{what}: choices {tuple(chosen.shape)} among {experts} experts (rows × up to as many, at most {MAX_EXPERTS})")
+    return chosen
+
+
+def expert_order(chosen: torch.Tensor, experts: int):
+    """The pairs (row, chosen expert) in the order of their experts, an expert's in the order of the rows: chosen int32 [rows, top] → (starts [experts + 1], source
+    [rows·top]: the row of every pair, −1 behind the last; place [rows, top]: where a pair went), all int32.  A choice outside 0 … experts − 1 is no pair: place −1."""
+    chosen = _pairs(chosen, experts, "expert_order")
+    _same_device("expert_order", chosen)
+    rows, top = chosen.shape
+    starts = torch.empty(experts + 1, dtype=torch.int32, device=chosen.device)
+    source, place = torch.empty(rows * top, dtype=torch.int32, device=chosen.device), torch.empty_like(chosen)
+    if rows:
+        check(lib().b200_expert_order(starts.data_ptr(), source.data_ptr(), place.data_ptr(), chosen.data_ptr(), rows, top, int(experts), _stream()), "b200_expert_order")
+    else:
+        starts.zero_()
+    return starts, source, place
+
+
+def expert_combine(y: torch.Tensor, place: torch.Tensor, weights: torch.Tensor) -> torch.Tensor:
+    """out[r] = bf16( Σ_t weights[r, t]·y[place[r, t]] ), fp32 in the order of t: y bf16 [rows·top, n], place int32 and weights fp32 [rows, top].  A place outside y
+    (expert_order's −1) adds nothing."""
+    y, place, weights = _chk(y, "expert_combine.y"), _chk(place, "expert_combine.place", torch.int32), _chk(weights, "expert_combine.weights", torch.float32)
+    if place.dim() != 2 or weights.shape != place.shape or y.dim() != 2 or y.shape[0] != place.numel() or y.shape[1] < 1 or not 1 <= place.shape[1] <= MAX_EXPERTS:
+        raise B200Error(f"expert_combine: rows {tuple(y.shape)}, places {tuple(place.shape)}, weights {tuple(weights.shape)} do not match")
+    _same_device("expert_combine", y, place, weights)
+    rows, top = place.shape
+    out = torch.empty(rows, y.shape[1], dtype=torch.bfloat16, device=y.device)
+    if rows:
+        check(lib().b200_expert_combine_bf16(out.data_ptr(), y.data_ptr(), place.data_ptr(), weights.data_ptr(), rows, top, y.shape[1], _stream()),
+              "b200_expert_combine_bf16")
+    return out
+
+
+def experts_f8(x: torch.Tensor, chosen: torch.Tensor, weights: torch.Tensor, w_in: F8Weight, w_out: F8Weight) -> torch.Tensor:
+    """A layer of routed experts in 8 bits: x bf16 [rows, width], chosen int32 and weights fp32 [rows, top], w_in [experts, 2·ff, width] (gate | up) and w_out
+    [experts, width, ff] of 8 bits → bf16 [rows, width].  What expert_order, f8_rows, grouped_linear_f8, silu_mul_f8, grouped_linear_f8 and expert_combine give one
+    behind the other.  A choice outside the experts adds nothing."""
+    import ctypes as C
+    d_in, parts_in = _f8_desc(w_in, "experts_f8", 3)
+    d_out, parts_out = _f8_desc(w_out, "experts_f8", 3)
+    x, chosen, weights = _chk(x, "experts_f8.x"), _pairs(chosen, d_in.experts, "experts_f8"), _chk(weights, "experts_f8.weights", torch.float32)
+    if d_out.experts != d_in.experts or w_in.n != 2 * w_out.k or w_out.n != w_in.k:
+        raise B200Error(f"experts_f8: {d_in.experts} matrices [{w_in.n}, {w_in.k}] and {d_out.experts} [{w_out.n}, {w_out.k}] are no experts' gate | up and down")
+    if x.dim() != 2 or x.shape[1] != w_in.k or chosen.shape[0] != x.shape[0] or weights.shape != chosen.shape:
+        raise B200Error(f"experts_f8: rows {tuple(x.shape)}, choices {tuple(chosen.shape)}, weights {tuple(weights.shape)} do not match width {w_in.k}")
+    _same_device("experts_f8", x, chosen, weights, *parts_in, *parts_out)
+    rows, top = chosen.shape
+    out = torch.empty_like(x)
+    if rows:
+        bytes_ = lib().b200_experts_f8_workspace_bytes(rows, top, d_in.experts, w_in.k, w_out.k)
+        if bytes_ < 0:
+            raise B200Error(f"experts_f8: {rows} rows with {top} of {d_in.experts} experts [{w_in.k}, {w_out.k}] out of range")
+        ws = torch.empty(bytes_, dtype=torch.uint8, device=x.device)
+        check(lib().b200_experts_f8_bf16(out.data_ptr(), x.data_ptr(), chosen.data_ptr(), weights.data_ptr(), C.byref(d_in), C.byref(d_out), rows, top, ws.data_ptr(),
+                                         _stream()), "b200_experts_f8_bf16")
+    return out
+
+
 # ---- the paged cache of 4-bit keys and values (csrc/kv4.cu, kv4_attn.cu, kv4_pages.cu)
 KV4_PAGE, KV4_GROUP, KV4_MAX_SEQS = 64, 64, 1024
 
