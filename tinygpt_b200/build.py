@@ -23,7 +23,7 @@ OBJ_DIR = LIB_DIR / "obj"
 LIB_PATH = LIB_DIR / "libb200decode.so"
 NATIVE_PATH = LIB_DIR / "b200ops.so"
 
-SOURCES = ["common.cu", "gemv.cu", "gemv_batch.cu", "gemm.cu", "prefill.cu", "prefill_attn.cu", "prefill_attn_tc.cu", "sampling.cu", "ops.cu", "attn.cu", "w4.cu", "w4_gemm.cu", "kv4.cu", "kv4_attn.cu", "kv4_pages.cu", "f8_rows.cu", "group_gemm.cu", "experts.cu", "engine.cu", "api.cu", "tp.cu", "stack_ops.cu",
+SOURCES = ["common.cu", "gemv.cu", "gemv_batch.cu", "gemm.cu", "prefill.cu", "prefill_attn.cu", "prefill_attn_tc.cu", "sampling.cu", "ops.cu", "attn.cu", "w4.cu", "w4_gemm.cu", "kv4.cu", "kv4_attn.cu", "kv4_pages.cu", "f8_rows.cu", "group_gemm.cu", "group_gemm_wide.cu", "experts.cu", "engine.cu", "api.cu", "tp.cu", "stack_ops.cu",
            "stack_mix.cu", "stack_rec.cu", "stack_hyper.cu", "stack_pool.cu", "stack_pool_mma.cu", "engine_stack.cu"]
 
 NVCC_FLAGS = [

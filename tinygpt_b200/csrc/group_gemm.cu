@@ -1,6 +1,6 @@
 // group_gemm.cu — products of rows with the matrix of their group, on the 5th-generation tensor cores:  y[r] = W[e]·x[r] for the rows r of group e.
 //
-// One kernel for bf16 and for 8 bits with scales, for one matrix (a Linear) and for many (experts, rows sorted by expert).  W is the A operand: a tile is
+// This kernel takes groups of up to 128 rows, on average, for bf16 and for 8 bits with scales, for one matrix (a Linear) and for many (experts, rows sorted by expert).  W is the A operand: a tile is
 // 128 of its rows (channels) × up to NT rows of x, and the product's N is what the tile really holds, rounded up to 16.  So a group of three rows costs a stream of its
 // matrix and little else, and a group that ends inside a tile costs no idle rows.
 //
@@ -8,15 +8,14 @@
 //   warp 0   TMA: of every 128 bytes of k 128 rows of W and the tile's rows of x, into a ring of shared memory
 //   warp 1   one thread issues four products (K = 32 bytes) per 128 bytes
 //   warp 2   8 bits: the products of x's and W's scales, NT of them for each block of 128 entries, fetched some blocks ahead
-//   warp 3   rows of no group are zeroed
+//   warp 3   takes finished tiles from shared memory to y, row by row in bulk copies, beside the next tile's products; rows of no group are zeroed
 //   warps 4 … 11   the sums: a warp has a quarter of the channels and half of the rows, as fragments of 8 × 8 (lane 4r + c: channel r, rows 2c and 2c + 1), so
 //            that a lane needs a quarter of the factors and a transposing store to shared memory makes rows of y of them
 // 8 bits: W has a scale for 128 × 128 entries and x one for 128 entries of a row, so that 128 entries of k meet one factor per row of x, and the sums of 128
 // entries — a slot of tensor memory each — are scaled and added in fp32 registers; two to four slots keep the tensor cores running meanwhile.
 // bf16: a slot holds the sums over all of k.
-// Tiles of up to 256 rows belong to pairs of CTAs (cta_group::2): 256 channels, each CTA brings its 128 of them and half of the rows, and sums its own channels.
-#include "f8.cuh"
-#include "tc.cuh"
+// More rows go to tiles of 256 × 256 on pairs of CTAs (group_gemm_wide.cu).
+#include "group_gemm.cuh"
 
 #include <algorithm>
 
@@ -26,65 +25,29 @@ namespace {
 
 constexpr int kCh = 128, kWBytes = kCh * 128, kThreads = 384, kEpiWarps = 8;
 constexpr int kMaxSplits = 8;
-constexpr int kPatch = 16 * 64;            // 16 rows of y, 32 channels of a warp
+constexpr int kOutLd = kCh * 2 + 16;       // bytes from row to row of a finished tile: eight rows meet all banks
 constexpr int kPartLd = kCh + 4;            // floats from row to row of a partial tile: a fragment's lanes meet 32 banks
-constexpr int kRegsFew = 72, kRegsMany = 216, kRegsLaunch = 168;   // where they are shared out unevenly
-static_assert(128 * kRegsFew + 256 * kRegsMany <= kThreads * kRegsLaunch, "no warp waits for registers that the launch does not have");
 constexpr unsigned kWaitCode = 0x67000000u;
-
-struct Args {
-  __nv_bfloat16* y;
-  const float *sx, *sw;
-  const int32_t* starts;
-  const __nv_bfloat16* bias;
-  unsigned* err;
-  int64_t rows;
-  int n, k_blocks, experts, ch_tiles, ch_blocks, splits;   // ch_tiles: of 128 channels, a pair's of 256
-  bool wide;    // y takes stores of 16 bytes
-};
 
 template <int NT>
 struct Form {
-  static constexpr int group = NT == 256 ? 2 : 1;      // CTAs to a tile
   static constexpr int per_sm = NT <= 64 ? 2 : 1;
-  static constexpr int x_rows = NT / group, x_bytes = x_rows * 128, stage = kWBytes + x_bytes;   // of a CTA
-  static constexpr int stages = NT <= 32 ? 5 : NT == 64 ? 4 : 6;
-  static constexpr int box = x_rows < 32 ? x_rows : 32;  // rows of x in a TMA box
-  static constexpr int slots8 = NT == 256 ? 2 : 4;     // of tensor memory, 8 bits
+  static constexpr int x_bytes = NT * 128, stage = kWBytes + x_bytes;
+  static constexpr int stages = NT <= 32 ? 5 : NT == 64 ? 3 : 5;
+  static constexpr int box = NT < 64 ? NT : 64;  // rows of x in a TMA box
+  static constexpr int slots8 = 4;                     // of tensor memory, 8 bits
   static constexpr int lag = 3;                        // blocks that factors are asked for ahead
   static constexpr int ahead = 2 * slots8 + 1 + lag;   // blocks of factors in shared memory: see where they are written
   static constexpr int f_slot = NT < 32 ? 32 : NT;
   static constexpr int cols = NT / 2;                  // rows of x of a summing warp
   static constexpr int ring = stages * stage;
-  static constexpr int tables = 1024 + ring + kEpiWarps * kPatch + ahead * f_slot * 4 + 512;
-  static constexpr int smem(int experts) { return tables + experts * 12; }
-  // 8 bits, 256 rows: a thread that sums holds 128 of them.  The four warps that do not give registers up: 128·72 + 256·216 of the launch's 384·168.
-  static constexpr bool uneven = NT == 256;
+  static constexpr int tables = 1024 + ring + NT * kOutLd + ahead * f_slot * 4 + 512;
+  static constexpr int smem(int experts) { return tables + Groups::bytes(experts); }
   static constexpr int tmem(int slots) { return slots * NT < 32 ? 32 : slots * NT; }
 };
 static_assert(Form<16>::smem(64) <= 113 * 1024 && Form<32>::smem(64) <= 114 * 1024 && Form<64>::smem(64) <= 114 * 1024, "two CTAs to an SM");
-static_assert(Form<128>::smem(kMaxExperts) <= 227 * 1024 && Form<256>::smem(kMaxExperts) <= 227 * 1024, "room");
+static_assert(Form<128>::smem(kMaxExperts) <= 227 * 1024, "room");
 static_assert(Form<128>::ring >= 128 * kPartLd * 4 && Form<64>::ring >= 64 * kPartLd * 4 && Form<16>::ring >= 16 * kPartLd * 4, "a partial tile fits in the drained ring");
-
-// D[tmem] (+)= A·B over 32 entries of 8 bits
-template <int GROUP>
-__device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
-  if constexpr (GROUP == 2)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a, b, %4, p;\n\t}" ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(kDescHi), "r"(idesc), "r"(accumulate)
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %4, p;\n\t}" ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(kDescHi), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-// kind::f8f6f4: D = F32 (bits 4-5 = 1), A = B = e4m3 (0), both K-major, N >> 3 at bits 17-22, M >> 4 at bits 24-28
-__device__ __forceinline__ uint32_t idesc_of(bool eight, int m, int n) {
-  const uint32_t shape = ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24) | (1u << 4);
-  return eight ? shape : shape | (1u << 7) | (1u << 10);
-}
 
 // 16 lanes of tensor memory × 8·N columns as N fragments: lane 4r + c takes {(r, 2c), (r, 2c + 1), (r + 8, 2c), (r + 8, 2c + 1)} of each.  What was loaded is held by the
 // wait (tmem_ready), so that nothing that uses it moves in front of that.
@@ -118,49 +81,8 @@ __device__ __forceinline__ void tmem_ready(uint32_t (&r)[16]) {
 __device__ __forceinline__ void store_transposed(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-__device__ __forceinline__ void cp_async4(void* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-// a wait of a whole warp that mostly finds what it waits for
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsigned* err, unsigned code) {
-  return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || __all_sync(0xffffffffu, mbar_wait_limited(bar, parity, err, code));
-}
 // where the factor of row j of a tile lies: a lane that holds rows 8i + 2c, + 1 finds those of four i side by side
 __device__ __forceinline__ int factor_at(int j) { return (j & ~31) + (j % 8 / 2) * 8 + (j % 32 / 8) * 2 + j % 2; }
-// Arrives in another CTA.  What it tells is that tensor memory was read (the fence in front); no memory is handed over, so that no release at the cluster's
-// scope is needed, which takes some 700 cycles.
-__device__ __forceinline__ void arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
-// two fp32 numbers in a 64-bit register: one instruction multiplies and adds both
-template <bool B>
-struct Is {
-  static constexpr bool value = B;
-};
-__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
-  return v;
-}
-__device__ __forceinline__ uint64_t pair_of(uint32_t lo, uint32_t hi) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
-  return v;
-}
-__device__ __forceinline__ float2 halves(uint64_t v) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-  return f;
-}
-__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-
 // Which rows and channels a tile has.  Tiles run over the row tiles of a group first (its matrix's rows stay in L2), then over channels, then over groups.
 struct Tile {
   int64_t row0;
@@ -169,27 +91,27 @@ struct Tile {
 
 template <bool F8, int NT>
 __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
-                                                                               const Args p) {
+                                                                               const GemmArgs p) {
   using F = Form<NT>;
-  constexpr int GROUP = F::group, ST = F::stages, SLOTS = F8 ? F::slots8 : 2, COLS = F::cols, TMEM = F::tmem(SLOTS), AHEAD = F::ahead, LAG = F::lag;
+  constexpr int ST = F::stages, SLOTS = F8 ? F::slots8 : 2, COLS = F::cols, TMEM = F::tmem(SLOTS), AHEAD = F::ahead, LAG = F::lag;
   constexpr int PIECE = COLS < 32 ? COLS : 32;      // rows of 16 channels that are loaded at once
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* const sx = smem + ST * kWBytes;
-  uint8_t* const patches = smem + F::ring;                                         // [summing warps][16 rows][32 channels], bf16
-  float* const factors = reinterpret_cast<float*>(patches + kEpiWarps * kPatch);   // [AHEAD][NT]
+  uint8_t* const done_tile = smem + F::ring;                                       // [NT][kOutLd]: bf16
+  float* const factors = reinterpret_cast<float*>(done_tile + NT * kOutLd);        // [AHEAD][NT]
   uint64_t* const full = reinterpret_cast<uint64_t*>(factors + AHEAD * F::f_slot);   // [stages], a pair's first CTA's
   uint64_t* const empty = full + ST;
   uint64_t* const sums_full = empty + ST;                                          // [slots]
   uint64_t* const sums_empty = sums_full + 4;                                      // a pair's first CTA's
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(sums_empty + 4);
+  uint64_t* const out_full = sums_empty + 4;                                       // of the finished tile
+  uint64_t* const out_empty = out_full + 1;
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(out_empty + 1);
   int* const gave_up = reinterpret_cast<int*>(tmem_slot + 1);
   float* const w_scale = reinterpret_cast<float*>(gave_up + 1);                       // [AHEAD]
-  int* const ends = reinterpret_cast<int*>(smem + F::tables - 1024);   // [experts] row tiles up to and with e
-  int* const froms = ends + p.experts;                                               // first row, rows
-  int* const counts = froms + p.experts;
+  Groups groups(reinterpret_cast<int*>(smem + F::tables - 1024), p.experts);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int rank = GROUP == 2 || p.splits > 1 ? (int)cluster_rank() : 0;
+  const int split = p.splits > 1 ? (int)cluster_rank() : 0;
   bool ok = true;
 
   if (threadIdx.x == 0) {
@@ -201,84 +123,48 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
     }
     for (int a = 0; a < SLOTS; ++a) {
       mbar_init(&sums_full[a], F8 ? 2 : 1);   // products done, factors there
-      mbar_init(&sums_empty[a], GROUP * kEpiWarps);
+      mbar_init(&sums_empty[a], kEpiWarps);
     }
+    mbar_init(out_full, kEpiWarps);
+    mbar_init(out_empty, 1);
     fence_mbar_init();
     *gave_up = 0;
   }
-  if (warp == 1) tmem_alloc<GROUP>(tmem_slot, TMEM);
+  if (warp == 1) tmem_alloc<1>(tmem_slot, TMEM);
   pdl_wait();
   pdl_trigger();
-  if (warp == 3) {   // every lane a run of groups; their rows lie inside the call's, whatever the starts say
-    const int each = (p.experts + 31) / 32, e0 = min(lane * each, p.experts), e1 = min(e0 + each, p.experts);
-    int mine = 0;
-    for (int e = e0; e < e1; ++e) {
-      const int64_t from = p.starts == nullptr ? 0 : min(max((int64_t)p.starts[e], (int64_t)0), p.rows);
-      const int64_t count = p.starts == nullptr ? p.rows : max(min((int64_t)p.starts[e + 1], p.rows) - from, (int64_t)0);
-      froms[e] = (int)from;
-      counts[e] = (int)count;
-      mine += (int)((count + NT - 1) / NT);
-    }
-    int upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o *= 2) {
-      const int v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += v;
-    }
-    upto -= mine;
-    for (int e = e0; e < e1; ++e) {
-      upto += (counts[e] + NT - 1) / NT;
-      ends[e] = upto;
-    }
-  }
+  if (warp == 3) groups.make<NT>(p.starts, p.rows, lane);
   tc_fence_before();
   __syncthreads();
-  if constexpr (GROUP == 2) cluster_sync_all();   // the pair's barriers exist
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int split = GROUP == 1 ? rank : 0;
-  const int64_t tiles = (int64_t)ends[p.experts - 1] * p.ch_tiles;
-  const int64_t first = blockIdx.x / (GROUP * p.splits), step = p.splits > 1 ? tiles : gridDim.x / GROUP;   // a cluster that splits k takes one tile
+  const int64_t tiles = (int64_t)groups.ends[p.experts - 1] * p.ch_tiles;
+  const int64_t first = blockIdx.x / p.splits, step = p.splits > 1 ? tiles : gridDim.x;   // a cluster that splits k takes one tile
   const int kb0 = (int)((int64_t)p.k_blocks * split / p.splits), kb1 = (int)((int64_t)p.k_blocks * (split + 1) / p.splits);
   auto tile_at = [&](int64_t t) {
-    const int at = (int)(t / p.ch_tiles);   // this group's: ends[e − 1] ≤ at < ends[e]
-    int lo = 0, hi = p.experts - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (ends[mid] > at) hi = mid;
-      else lo = mid + 1;
-    }
-    const int before = lo > 0 ? ends[lo - 1] : 0, row_tiles = ends[lo] - before, count = counts[lo];
-    const int local = (int)(t - (int64_t)before * p.ch_tiles);
+    int local, row_tiles;
+    const int e = groups.find(t, p.ch_tiles, local, row_tiles), count = groups.counts[e];
     const int i = local % row_tiles, each = ((count + row_tiles - 1) / row_tiles + 15) / 16 * 16;   // alike, and none is empty
-    return Tile{froms[lo] + (int64_t)i * each, min(each, count - i * each), (local / row_tiles * GROUP + (GROUP == 2 ? rank : 0)) * kCh, lo};
+    return Tile{groups.froms[e] + (int64_t)i * each, min(each, count - i * each), local / row_tiles * kCh, e};
   };
   auto up16 = [](int v) { return (v + 15) / 16 * 16; };
 
   if (warp < 4) {
-    if constexpr (F8 && F::uneven) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
     if (warp == 0) {
       if (lane == 0) {
         int s = 0;
         uint32_t ph = 1;
         for (int64_t t = first; t < tiles && ok; t += step) {
           const Tile tile = tile_at(t);
-          const int mine = up16(tile.rows) / GROUP, row0 = (int)tile.row0 + (GROUP == 2 ? rank * mine : 0);
-          const int boxes = (mine + F::box - 1) / F::box, w_row = tile.expert * p.n + tile.ch0;
+          const int row0 = (int)tile.row0;
+          const int boxes = (tile.rows + F::box - 1) / F::box, w_row = tile.expert * p.n + tile.ch0;
           for (int kb = kb0; kb < kb1; ++kb) {
             if (!(ok = mbar_wait_limited(&empty[s], ph, p.err, kWaitCode | 1))) break;
             uint8_t *const w_to = smem + s * kWBytes, *const x_to = sx + s * F::x_bytes;
             const int k0 = kb * (F8 ? 128 : 64);
-            if constexpr (GROUP == 2) {
-              const uint32_t bar = mapa_u32(smem_u32(&full[s]), 0);
-              if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * (kWBytes + boxes * F::box * 128));
-              tma_load_2d_pair(w_to, &tmap_w, k0, w_row, bar);
-              for (int b = 0; b < boxes; ++b) tma_load_2d_pair(x_to + b * F::box * 128, &tmap_x, k0, row0 + b * F::box, bar);
-            } else {
-              mbar_arrive_expect_tx(&full[s], kWBytes + boxes * F::box * 128);
-              tma_load_2d(w_to, &tmap_w, k0, w_row, &full[s]);
-              for (int b = 0; b < boxes; ++b) tma_load_2d(x_to + b * F::box * 128, &tmap_x, k0, row0 + b * F::box, &full[s]);
-            }
+            mbar_arrive_expect_tx(&full[s], kWBytes + boxes * F::box * 128);
+            tma_load_2d(w_to, &tmap_w, k0, w_row, &full[s]);
+            for (int b = 0; b < boxes; ++b) tma_load_2d(x_to + b * F::box * 128, &tmap_x, k0, row0 + b * F::box, &full[s]);
             if (++s == ST) {
               s = 0;
               ph ^= 1;
@@ -288,14 +174,14 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
         if (!ok) drain_async();
       }
     } else if (warp == 1) {
-      if ((GROUP == 1 || rank == 0) && elect_one()) {
+      if (elect_one()) {
         const uint32_t w0 = desc_lo(smem_u32(smem)), x0 = desc_lo(smem_u32(sx));
         int s = 0, slot = 0;
         uint32_t ph = 0, slot_ph = 1;
         bool ready = false;   // of the next stage, looked at before the products of this one go out
         for (int64_t t = first; t < tiles && ok; t += step) {
           const Tile tile = tile_at(t);
-          const uint32_t idesc = idesc_of(F8, kCh * GROUP, up16(tile.rows));
+          const uint32_t idesc = idesc_of(F8, kCh, up16(tile.rows));
           for (int kb = kb0; kb < kb1; ++kb) {
             if (F8 || kb == kb0) {
               if (!(ok = mbar_wait_limited(&sums_empty[slot], slot_ph, p.err, kWaitCode | 2))) break;
@@ -311,14 +197,12 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
             ready = mbar_test(&full[s], ph);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              if constexpr (F8) umma_f8<GROUP>(d, w + 2 * k, x + 2 * k, idesc, k > 0 ? 1u : 0u);
-              else umma_lo<GROUP>(d, w + 2 * k, x + 2 * k, idesc, kb > kb0 || k > 0 ? 1u : 0u);
+              if constexpr (F8) umma_f8<1>(d, w + 2 * k, x + 2 * k, idesc, k > 0 ? 1u : 0u);
+              else umma_lo<1>(d, w + 2 * k, x + 2 * k, idesc, kb > kb0 || k > 0 ? 1u : 0u);
             }
-            if constexpr (GROUP == 2) umma_commit_pair(done);
-            else umma_commit(done);
+            umma_commit(done);
             if (F8 || kb == kb1 - 1) {
-              if constexpr (GROUP == 2) umma_commit_pair(&sums_full[slot]);
-              else umma_commit(&sums_full[slot]);
+              umma_commit(&sums_full[slot]);
               if (++slot == SLOTS) {
                 slot = 0;
                 slot_ph ^= 1;
@@ -376,69 +260,56 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
         cp_async_wait<0>();
       }
     } else if (warp == 3) {
-      if (p.starts != nullptr) {   // rows in front of the first group and behind the last
-        const int64_t from = min(max((int64_t)p.starts[0], (int64_t)0), p.rows), to = min(max((int64_t)p.starts[p.experts], from), p.rows);
-        for (int64_t r = blockIdx.x; r < p.rows - (to - from); r += gridDim.x) {
-          __nv_bfloat16* const out = p.y + (r < from ? r : r - from + to) * p.n;
-          for (int i = lane; i < p.n; i += 32) out[i] = f_to_bf16(0.f);
+      if (p.splits == 1) {
+        uint32_t ph = 0;
+        for (int64_t t = first; t < tiles; t += step, ph ^= 1) {
+          const Tile tile = tile_at(t);
+          if (!(ok = warp_wait(out_full, ph, p.err, kWaitCode | 6))) break;
+          store_tile(p.y + tile.row0 * p.n + tile.ch0, done_tile, kOutLd, tile.rows, min(kCh, p.n - tile.ch0), p, lane);
+          if (lane == 0) mbar_arrive(out_empty);
         }
+        bulk_wait();   // (shared memory and what was stored outlive the CTA only so)
       }
+      zero_other_rows(p, lane);
     }
   } else {
-    if constexpr (F8 && F::uneven) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsMany));
     const int quad = warp & 3, half = (warp - 4) >> 2, r = lane / 4, c = lane % 4;
     const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + half * COLS;
-    uint8_t* const patch = patches + (warp - 4) * kPatch;
-    // lane 8m + i of a transposing store: row i, channels 8m … of 32, at a place that lets eight rows meet all banks; and row 8 + i
-    const uint32_t put_at = smem_u32(patch) + lane % 8 * 64 + (((lane / 8) ^ (lane % 8 / 2)) << 4);
-    const uint8_t* const get_at = patch + lane / 4 * 64 + (((lane % 4) ^ (lane / 4 / 2)) << 4);
+    // lane 8m + i of a transposing store: row i, channels 8m … 8m + 7 of 32
+    const uint32_t put_at = smem_u32(done_tile) + (half * COLS + lane % 8) * kOutLd + quad * 64 + lane / 8 * 16;
     int slot = 0, fslot = 0;
-    uint32_t slot_ph = 0;
-    for (int64_t t = first; t < tiles; t += step) {
+    uint32_t slot_ph = 0, out_ph = 1;
+    for (int64_t t = first; t < tiles; t += step, out_ph ^= 1) {
       const Tile tile = tile_at(t);
       const int mine = tile.rows - half * COLS;   // rows of this half
       const int ch0 = tile.ch0 + quad * 32;
       float bias[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) bias[e] = p.bias != nullptr && ch0 + r + 8 * e < p.n ? bf16_to_f(p.bias[ch0 + r + 8 * e]) : 0.f;
-      __nv_bfloat16* const out = p.y + (tile.row0 + half * COLS) * p.n + ch0;
-      // Rows j … j + 7 of this half, 32 channels: v[e][i] is channel r + 8e, row j + 2c + i.  Every second call stores sixteen rows.
+      // Rows j … j + 7 of this half, 32 channels: v[e][i] is channel r + 8e, row j + 2c + i.
       auto put8 = [&](int j, float2 (&v)[4]) {
-        if (GROUP == 1 && p.splits > 1) {   // [row][channel] where the operands were: every product has read them
+        if (p.splits > 1) {   // [row][channel] where the operands were: every product has read them
           float* const part = reinterpret_cast<float*>(smem) + (half * COLS + j + 2 * c) * kPartLd + quad * 32 + r;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             part[8 * e] = v[e].x;
             part[8 * e + kPartLd] = v[e].y;
           }
-          return;
+        } else {
+          store_transposed(put_at + j * kOutLd, pack2(v[0].x + bias[0], v[0].y + bias[0]), pack2(v[1].x + bias[1], v[1].y + bias[1]),
+                           pack2(v[2].x + bias[2], v[2].y + bias[2]), pack2(v[3].x + bias[3], v[3].y + bias[3]));
         }
-        store_transposed(put_at + j % 16 * 64, pack2(v[0].x + bias[0], v[0].y + bias[0]), pack2(v[1].x + bias[1], v[1].y + bias[1]),
-                         pack2(v[2].x + bias[2], v[2].y + bias[2]), pack2(v[3].x + bias[3], v[3].y + bias[3]));
-        if (j % 16 == 0 && j + 8 < COLS && j + 8 < mine) return;
+      };
+      auto finished = [&]() {   // this warp's part of the tile lies in shared memory
+        if (p.splits > 1) return;
+        fence_proxy_async();
         __syncwarp();
-        const int j0 = j / 16 * 16;
-        if (p.wide) {   // n is a multiple of 8: sixteen bytes lie inside a row or outside it
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int row = j0 + 8 * i + lane / 4;
-            if (row < mine && row < COLS && ch0 + lane % 4 * 8 < p.n)
-              *reinterpret_cast<uint4*>(out + (int64_t)row * p.n + lane % 4 * 8) = *reinterpret_cast<const uint4*>(get_at + i * 512);
-          }
-        } else if (ch0 + lane < p.n) {
-          for (int i = 0; i < 16 && j0 + i < min(mine, COLS); ++i)
-            out[(int64_t)(j0 + i) * p.n + lane] =
-                *reinterpret_cast<const __nv_bfloat16*>(patch + i * 64 + (((lane / 8) ^ (i % 8 / 2)) << 4) + lane % 8 * 2);
-        }
-        __syncwarp();
+        if (lane == 0) mbar_arrive(out_full);
       };
       auto release = [&]() {   // the slot may be filled again
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          if constexpr (GROUP == 2) arrive_at(mapa_u32(smem_u32(&sums_empty[slot]), 0));
-          else mbar_arrive(&sums_empty[slot]);
-        }
+        if (lane == 0) mbar_arrive(&sums_empty[slot]);
         if (++slot == SLOTS) {
           slot = 0;
           slot_ph ^= 1;
@@ -455,38 +326,39 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
           constexpr bool ALL = decltype(all_rows)::value;
           const float* const factor = factors + fslot * F::f_slot + (half * COLS & ~31) + c * 8 + half * COLS % 32 / 4;
           const uint32_t at = from + slot * NT;
-          constexpr int PIECES = 2 * (COLS / PIECE);   // in turn channels 0 … 15 and 16 … 31
-          const int pieces = ALL ? PIECES : 2 * ((mine + PIECE - 1) / PIECE);
-          uint32_t d[2][PIECE / 2];
+          constexpr int PIECES = COLS / PIECE;
+          const int pieces = ALL ? PIECES : (mine + PIECE - 1) / PIECE;
+          uint32_t d[2][2][PIECE / 2];   // channels 0 … 15, 16 … 31
           float2 f[PIECE / 8];
-          tmem_frag(at, d[0]);
+          tmem_frag(at, d[0][0]);
+          tmem_frag(at + (16u << 16), d[0][1]);
 #pragma unroll
           for (int i = 0; i < PIECES; ++i) {
             if (!ALL && i >= pieces) break;
-            uint32_t(&v)[PIECE / 2] = d[i % 2];
-            if (i % 2 == 0) {
+            if constexpr (PIECE >= 16) {
 #pragma unroll
-              for (int g = 0; g < PIECE / 8; ++g) {
-                if constexpr (PIECE >= 16) {
-                  if (g % 2 == 0) {
-                    const float4 both = *reinterpret_cast<const float4*>(factor + i / 2 * PIECE + 2 * g);
-                    f[g] = make_float2(both.x, both.y);
-                    f[g + 1] = make_float2(both.z, both.w);
-                  }
-                } else {
-                  f[g] = *reinterpret_cast<const float2*>(factor);
-                }
+              for (int g = 0; g < PIECE / 8; g += 2) {
+                const float4 both = *reinterpret_cast<const float4*>(factor + i * PIECE + 2 * g);
+                f[g] = make_float2(both.x, both.y);
+                f[g + 1] = make_float2(both.z, both.w);
               }
+            } else {
+              f[0] = *reinterpret_cast<const float2*>(factor);
             }
-            tmem_ready(v);
-            if (i + 1 < PIECES && (ALL || i + 1 < pieces)) tmem_frag(at + (i + 1) / 2 * PIECE + ((uint32_t)((i + 1) % 2 * 16) << 16), d[(i + 1) % 2]);
-            else release();
+            tmem_ready(d[i % 2][0]);
+            tmem_ready(d[i % 2][1]);
+            if (i + 1 < PIECES && (ALL || i + 1 < pieces)) {
+              tmem_frag(at + (i + 1) * PIECE, d[(i + 1) % 2][0]);
+              tmem_frag(at + (i + 1) * PIECE + (16u << 16), d[(i + 1) % 2][1]);
+            } else {
+              release();
+            }
 #pragma unroll
             for (int g = 0; g < PIECE / 8; ++g) {
               const uint64_t fg = pair_of(f[g].x, f[g].y);
-              uint64_t(&sum)[4] = acc[i / 2 * (PIECE / 8) + g];
-              sum[i % 2 * 2] = fma_pair(pair_of(v[4 * g], v[4 * g + 1]), fg, sum[i % 2 * 2]);
-              sum[i % 2 * 2 + 1] = fma_pair(pair_of(v[4 * g + 2], v[4 * g + 3]), fg, sum[i % 2 * 2 + 1]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                acc[i * (PIECE / 8) + g][e] = fma_pair(pair_of(d[i % 2][e / 2][4 * g + e % 2 * 2], d[i % 2][e / 2][4 * g + e % 2 * 2 + 1]), fg, acc[i * (PIECE / 8) + g][e]);
             }
           }
         };
@@ -499,15 +371,18 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
           if (++fslot == AHEAD) fslot = 0;
         }
         if (!ok) break;
+        if (p.splits == 1 && !(ok = warp_wait(out_empty, out_ph, p.err, kWaitCode | 7))) break;
 #pragma unroll
         for (int g = 0; g < COLS / 8; ++g)
           if (8 * g < mine) {
             float2 v[4] = {halves(acc[g][0]), halves(acc[g][1]), halves(acc[g][2]), halves(acc[g][3])};
             put8(8 * g, v);
           }
+        finished();
       } else {
         if (!(ok = warp_wait(&sums_full[slot], slot_ph, p.err, kWaitCode | 5))) break;
         tc_fence_after();
+        if (p.splits == 1 && !(ok = warp_wait(out_empty, out_ph, p.err, kWaitCode | 7))) break;
 #pragma unroll 1
         for (int j = 0; j < COLS && j < mine; j += PIECE) {
           uint32_t a[PIECE / 2], b[PIECE / 2];
@@ -529,6 +404,7 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
             }
         }
         if (mine <= 0) release();
+        finished();
       }
     }
   }
@@ -536,9 +412,7 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
   tc_fence_before();
   __syncwarp();
   __syncthreads();
-  if constexpr (GROUP == 2) {
-    cluster_sync_all();   // neither CTA still reads the pair's operands, barriers or sums
-  } else if (p.splits > 1) {
+  if (p.splits > 1) {
     cluster_sync_all();
     // a warp takes a row of x, a lane four channels; the CTAs' sums in order
     const bool lost = __any_sync(0xffffffffu, lane < p.splits && ld_cluster_i32(mapa_u32(smem_u32(gave_up), min(lane, p.splits - 1))) != 0);
@@ -572,20 +446,15 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
   }
   if (warp == 1) {
     tc_fence_after();
-    tmem_free<GROUP>(tmem, TMEM);
+    tmem_free<1>(tmem, TMEM);
   }
-  if constexpr (GROUP == 2) cluster_sync_all();
 }
 
 template <bool F8, int NT>
-int launch(const GroupProduct& g, Args& p, cudaStream_t st) {
+int launch(const GroupProduct& g, GemmArgs& p, cudaStream_t st) {
   using F = Form<NT>;
   static PerDevice attrs;
   B200_CUDA(attrs([] {
-    cudaFuncAttributes a{};
-    const cudaError_t e = cudaFuncGetAttributes(&a, group_gemm_kernel<F8, NT>);
-    if (e != cudaSuccess) return e;
-    if (F8 && F::uneven && a.numRegs != kRegsLaunch) return cudaErrorInvalidDeviceFunction;   // (the shares would not add up)
     return cudaFuncSetAttribute(group_gemm_kernel<F8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::smem(kMaxExperts));
   }));
   CUtensorMap tw, tx;
@@ -598,45 +467,45 @@ int launch(const GroupProduct& g, Args& p, cudaStream_t st) {
     if ((rc = make_tmap_sw128(&tx, 2, g.x, 1, g.rows, g.k, 0, g.k, F::box)) != B200_OK) return rc;
   }
   p.ch_blocks = (int)((g.n + kCh - 1) / kCh);
-  p.ch_tiles = (p.ch_blocks + F::group - 1) / F::group;
+  p.ch_tiles = p.ch_blocks;
   // tiles that there can be: every group's last one may be short
   const int64_t row_tiles = g.starts ? g.rows / NT + std::min<int64_t>(g.experts, g.rows) : (g.rows + NT - 1) / NT, most = row_tiles * p.ch_tiles;
-  const int64_t room = 148 / F::group * F::per_sm;
+  const int64_t room = 148 * F::per_sm;
   p.splits = 1;
-  while (F::group == 1 && p.splits < kMaxSplits && most * p.splits * 2 <= room && p.k_blocks >= 4 * p.splits) p.splits *= 2;
+  while (p.splits < kMaxSplits && most * p.splits * 2 <= room && p.k_blocks >= 4 * p.splits) p.splits *= 2;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(p.splits > 1 ? most * p.splits : std::min(most, room) * F::group));
+  cfg.gridDim = dim3((unsigned)(p.splits > 1 ? most * p.splits : std::min(most, room)));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = F::smem((int)g.experts);
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)(p.splits * F::group);
+  attr[0].val.clusterDim.x = (unsigned)p.splits;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = op_pdl(st) ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   g_launches.fetch_add(1, std::memory_order_relaxed);
-  B200_CUDA(cudaLaunchKernelEx(&cfg, group_gemm_kernel<F8, NT>, tw, tx, (const Args)p));
+  B200_CUDA(cudaLaunchKernelEx(&cfg, group_gemm_kernel<F8, NT>, tw, tx, (const GemmArgs)p));
   return B200_OK;
 }
 
 template <bool F8>
-int launch_for(const GroupProduct& g, Args& p, cudaStream_t st) {
+int launch_for(const GroupProduct& g, GemmArgs& p, cudaStream_t st) {
   // rows of a tile: a group's, or twice its share of them (groups are unlike)
   const int64_t want = g.starts == nullptr ? g.rows : 2 * g.rows / std::min<int64_t>(g.experts, g.rows);
   if (want <= 16) return launch<F8, 16>(g, p, st);
   if (want <= 32) return launch<F8, 32>(g, p, st);
   if (want <= 64) return launch<F8, 64>(g, p, st);
   if (want <= 128) return launch<F8, 128>(g, p, st);
-  return launch<F8, 256>(g, p, st);
+  return launch_group_wide(g, p, st);
 }
 
 }  // namespace
 
 int launch_group_product(const GroupProduct& g, cudaStream_t st) {
-  Args p{};
+  GemmArgs p{};
   const int rc = wait_word(&p.err);
   if (rc != B200_OK) return rc;
   p.y = (__nv_bfloat16*)g.y;

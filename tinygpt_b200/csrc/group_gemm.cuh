@@ -1,0 +1,159 @@
+// group_gemm.cuh — what the two kernels of grouped products share: arguments, 8-bit products, the groups' tiles, waits of a warp, stores of finished tiles.
+#pragma once
+#include "f8.cuh"
+#include "tc.cuh"
+
+namespace b200 {
+
+struct GemmArgs {
+  __nv_bfloat16* y;
+  const float *sx, *sw;
+  const int32_t* starts;
+  const __nv_bfloat16* bias;
+  unsigned* err;
+  int64_t rows;
+  int n, k_blocks, experts, ch_tiles, ch_blocks, splits;   // ch_tiles: of a tile's channels; ch_blocks: of 128 channels
+  bool wide;    // y takes stores of 16 bytes
+};
+// tiles of 256 rows × 256 channels on pairs of CTAs (group_gemm_wide.cu)
+int launch_group_wide(const GroupProduct& g, GemmArgs& p, cudaStream_t st);
+
+#ifdef __CUDACC__
+// D[tmem] (+)= A·B over 32 entries of 8 bits
+template <int GROUP>
+__device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (GROUP == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a, b, %4, p;\n\t}" ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(kDescHi), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %4, p;\n\t}" ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(kDescHi), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// kind::f8f6f4: D = F32 (bits 4-5 = 1), A = B = e4m3 (0), both K-major, N >> 3 at bits 17-22, M >> 4 at bits 24-28
+__device__ __forceinline__ uint32_t idesc_of(bool eight, int m, int n) {
+  const uint32_t shape = ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24) | (1u << 4);
+  return eight ? shape : shape | (1u << 7) | (1u << 10);
+}
+
+__device__ __forceinline__ void cp_async4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// bytes of shared memory → global memory, 16-byte pieces; what a lane has asked for is complete behind its bulk_wait, and read behind bulk_wait_read
+__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+// a wait of a whole warp that mostly finds what it waits for
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsigned* err, unsigned code) {
+  return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || __all_sync(0xffffffffu, mbar_wait_limited(bar, parity, err, code));
+}
+// Arrives in another CTA.  What it tells is that tensor memory was read (the fence in front); no memory is handed over, so that no release at the cluster's
+// scope is needed, which takes some 700 cycles.
+__device__ __forceinline__ void arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// two fp32 numbers in a 64-bit register: one instruction multiplies and adds both
+template <bool B>
+struct Is {
+  static constexpr bool value = B;
+};
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ uint64_t pair_of(uint32_t lo, uint32_t hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+  return v;
+}
+__device__ __forceinline__ float2 halves(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+
+// The row tiles of all groups, made by one warp: a group's rows (inside the call's, whatever the starts say) and the tiles of ROWS rows up to and with it.
+struct Groups {
+  int *ends, *froms, *counts;   // shared memory
+  int experts;
+  static constexpr int bytes(int experts) { return experts * 12; }
+  __device__ __forceinline__ Groups(int* at, int n) : ends(at), froms(at + n), counts(at + 2 * n), experts(n) {}
+  template <int ROWS>
+  __device__ __forceinline__ void make(const int32_t* starts, int64_t rows, int lane) {
+    const int each = (experts + 31) / 32, e0 = min(lane * each, experts), e1 = min(e0 + each, experts);
+    int mine = 0;
+    for (int e = e0; e < e1; ++e) {
+      const int64_t from = starts == nullptr ? 0 : min(max((int64_t)starts[e], (int64_t)0), rows);
+      const int64_t count = starts == nullptr ? rows : max(min((int64_t)starts[e + 1], rows) - from, (int64_t)0);
+      froms[e] = (int)from;
+      counts[e] = (int)count;
+      mine += (int)((count + ROWS - 1) / ROWS);
+    }
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    upto -= mine;
+    for (int e = e0; e < e1; ++e) {
+      upto += (counts[e] + ROWS - 1) / ROWS;
+      ends[e] = upto;
+    }
+  }
+  // the group whose row tiles times ch_tiles tile t is one of; local: its number there, row_tiles: how many row tiles the group has
+  __device__ __forceinline__ int find(int64_t t, int ch_tiles, int& local, int& row_tiles) const {
+    const int at = (int)(t / ch_tiles);   // ends[e − 1] ≤ at < ends[e]
+    int lo = 0, hi = experts - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      if (ends[mid] > at) hi = mid;
+      else lo = mid + 1;
+    }
+    const int before = lo > 0 ? ends[lo - 1] : 0;
+    row_tiles = ends[lo] - before;
+    local = (int)(t - (int64_t)before * ch_tiles);
+    return lo;
+  }
+};
+// rows in front of the first group and behind the last, by one warp of every CTA
+__device__ __forceinline__ void zero_other_rows(const GemmArgs& p, int lane) {
+  if (p.starts == nullptr) return;
+  const int64_t from = min(max((int64_t)p.starts[0], (int64_t)0), p.rows), to = min(max((int64_t)p.starts[p.experts], from), p.rows);
+  for (int64_t r = blockIdx.x; r < p.rows - (to - from); r += gridDim.x) {
+    __nv_bfloat16* const out = p.y + (r < from ? r : r - from + to) * p.n;
+    for (int i = lane; i < p.n; i += 32) out[i] = f_to_bf16(0.f);
+  }
+}
+// A finished tile in shared memory, rows `ld` bytes apart → y, by one warp: a bulk copy to a row where rows of y take 16-byte pieces.  Shared memory may be written
+// again afterwards; bulk_wait before the CTA ends.
+__device__ __forceinline__ void store_tile(__nv_bfloat16* out, const uint8_t* tile, int ld, int rows, int width, const GemmArgs& p, int lane) {
+  if (p.wide) {
+    if (width > 0)
+      for (int row = lane; row < rows; row += 32) bulk_store(out + (int64_t)row * p.n, tile + row * ld, width * 2);
+    bulk_commit();
+    bulk_wait_read();
+  } else {
+    for (int row = 0; row < rows; ++row)
+      for (int i = lane; i < width; i += 32) out[(int64_t)row * p.n + i] = reinterpret_cast<const __nv_bfloat16*>(tile + row * ld)[i];
+  }
+  __syncwarp();
+}
+#endif
+
+}  // namespace b200

@@ -1,0 +1,342 @@
+// group_gemm_wide.cu — grouped products for groups of many rows: tiles of 256 rows of x × 256 channels on pairs of CTAs (cta_group::2), bf16 and 8 bits with scales.
+//
+// x is the A operand here: a CTA brings 128 rows of x and 128 of W for every 128 bytes of k (32 KB where a CTA by itself would need 48) and sums its rows over
+// all 256 channels.  A lane of tensor memory is a row of x, so that in 8 bits a summing thread — a row, one block of 128 channels — needs one factor for 128 sums: it
+// scales and adds them in 313 cycles for eight warps, where the products of a block of k take 512.  With W as A (group_gemm.cu) factors differ from sum to sum:
+// 620 to 660 cycles alone, 900 beside the products' own traffic to shared memory, and 4 096 × 28 672 × 4 096 took 754 µs.
+// The roles of the warps are those of group_gemm.cu; two slots of 256 columns of tensor memory.
+#include "group_gemm.cuh"
+
+#include <algorithm>
+
+namespace b200 {
+
+namespace {
+
+constexpr int kTile = 256, kHalf = 128;           // rows and channels of a pair, of a CTA's operands
+constexpr int kOperand = kHalf * 128;             // bytes of a stage
+constexpr int kStages = 4, kSlots = 2, kThreads = 384, kEpiWarps = 8;
+constexpr int kLag = 3, kAhead = 2 * kSlots + 1 + kLag;   // blocks of factors, asked for and kept: see group_gemm.cu
+constexpr int kOutLd = kTile * 2 + 16;            // bytes from row to row of a finished tile: eight rows meet all banks
+constexpr int kRing = kStages * 2 * kOperand;
+constexpr int kTables = 1024 + kRing + kHalf * kOutLd + kAhead * kTile * 4 + 512;
+constexpr int kTmem = kSlots * kTile;
+constexpr unsigned kWaitCode = 0x68000000u;
+// A thread that sums 8-bit products holds 128 sums: the four warps that hold none give registers up.
+constexpr int kRegsFew = 56, kRegsMany = 224, kRegsLaunch = 168;
+static_assert(128 * kRegsFew + 256 * kRegsMany <= kThreads * kRegsLaunch, "no warp waits for registers that the launch does not have");
+static_assert(kTables + Groups::bytes(kMaxExperts) <= 227 * 1024, "room");
+
+#define B200_R8(b) "+r"(r[b]), "+r"(r[b + 1]), "+r"(r[b + 2]), "+r"(r[b + 3]), "+r"(r[b + 4]), "+r"(r[b + 5]), "+r"(r[b + 6]), "+r"(r[b + 7])
+// the wait holds what was loaded: nothing that uses it moves in front of it
+__device__ __forceinline__ void load32(uint32_t taddr, uint32_t (&r)[32]) {
+  tmem_ld32(taddr, r);
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : B200_R8(0), B200_R8(8));
+  asm volatile("" : B200_R8(16), B200_R8(24));
+}
+
+template <bool F8>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const GemmArgs p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* const sx = smem;                                                        // [stages][128 rows × 128 bytes]
+  uint8_t* const sw = smem + kStages * kOperand;                                   // the same of W
+  uint8_t* const done_tile = smem + kRing;                                         // [128][kOutLd]: bf16
+  float* const factors = reinterpret_cast<float*>(done_tile + kHalf * kOutLd);     // [kAhead][2][128]: of a block of channels, of a row
+  uint64_t* const full = reinterpret_cast<uint64_t*>(factors + kAhead * kTile);    // [stages], CTA 0's count the pair's bytes
+  uint64_t* const empty = full + kStages;
+  uint64_t* const sums_full = empty + kStages;                                     // [slots]
+  uint64_t* const sums_empty = sums_full + kSlots;                                 // CTA 0's
+  uint64_t* const out_full = sums_empty + kSlots;
+  uint64_t* const out_empty = out_full + 1;
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(out_empty + 1);
+  float* const w_scale = reinterpret_cast<float*>(tmem_slot + 1);                  // [kAhead][2]
+  Groups groups(reinterpret_cast<int*>(smem + kTables - 1024), p.experts);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int rank = (int)cluster_rank();
+  bool ok = true;
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmap_w);
+    tma_prefetch_desc(&tmap_x);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < kSlots; ++a) {
+      mbar_init(&sums_full[a], F8 ? 2 : 1);   // products done, factors there
+      mbar_init(&sums_empty[a], 2 * kEpiWarps);
+    }
+    mbar_init(out_full, kEpiWarps);
+    mbar_init(out_empty, 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc<2>(tmem_slot, kTmem);
+  pdl_wait();
+  pdl_trigger();
+  if (warp == 3) groups.make<kTile>(p.starts, p.rows, lane);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();   // the pair's barriers exist
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int64_t tiles = (int64_t)groups.ends[p.experts - 1] * p.ch_tiles;
+  const int64_t first = blockIdx.x / 2, step = gridDim.x / 2;
+  const int k_blocks = p.k_blocks;
+  struct Tile {
+    int64_t row0;             // of this CTA
+    int rows, ch0, expert;    // rows of this CTA: none where the tile ends in the pair's first half
+  };
+  auto tile_at = [&](int64_t t) {   // a group's row tiles first: its rows of W stay in L2
+    int local, row_tiles;
+    const int e = groups.find(t, p.ch_tiles, local, row_tiles);
+    const int row = local % row_tiles * kTile + rank * kHalf;
+    return Tile{(int64_t)groups.froms[e] + row, max(0, min(kHalf, groups.counts[e] - row)), local / row_tiles * kTile, e};
+  };
+
+  if (warp < 4) {
+    if constexpr (F8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
+    if (warp == 0) {
+      if (lane == 0) {
+        int s = 0;
+        uint32_t ph = 1;
+        for (int64_t t = first; t < tiles && ok; t += step) {
+          const Tile tile = tile_at(t);
+          const int x_row = (int)tile.row0, w_row = tile.expert * p.n + tile.ch0 + rank * kHalf;   // (what lies past the operands is zero)
+          for (int kb = 0; kb < k_blocks; ++kb) {
+            if (!(ok = mbar_wait_limited(&empty[s], ph, p.err, kWaitCode | 1))) break;
+            const int k0 = kb * (F8 ? 128 : 64);
+            const uint32_t bar = mapa_u32(smem_u32(&full[s]), 0);
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], 4 * kOperand);
+            tma_load_2d_pair(sx + s * kOperand, &tmap_x, k0, x_row, bar);
+            tma_load_2d_pair(sw + s * kOperand, &tmap_w, k0, w_row, bar);
+            if (++s == kStages) {
+              s = 0;
+              ph ^= 1;
+            }
+          }
+        }
+        if (!ok) drain_async();
+      }
+    } else if (warp == 1) {
+      if (rank == 0 && elect_one()) {
+        const uint32_t x0 = desc_lo(smem_u32(sx)), w0 = desc_lo(smem_u32(sw)), idesc = idesc_of(F8, kTile, kTile);
+        int s = 0, slot = 0;
+        uint32_t ph = 0, slot_ph = 1;
+        bool ready = false;   // of the next stage, looked at before the products of this one go out
+        for (int64_t t = first; t < tiles && ok; t += step) {
+          for (int kb = 0; kb < k_blocks; ++kb) {
+            if (F8 || kb == 0) {
+              if (!(ok = mbar_wait_limited(&sums_empty[slot], slot_ph, p.err, kWaitCode | 2))) break;
+            }
+            if (!ready && !(ok = mbar_wait_limited(&full[s], ph, p.err, kWaitCode | 3))) break;
+            tc_fence_after();
+            const uint32_t x = x0 + s * (kOperand >> 4), w = w0 + s * (kOperand >> 4), d = tmem + slot * kTile;
+            uint64_t* const done = &empty[s];
+            if (++s == kStages) {
+              s = 0;
+              ph ^= 1;
+            }
+            ready = mbar_test(&full[s], ph);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if constexpr (F8) umma_f8<2>(d, x + 2 * k, w + 2 * k, idesc, k > 0 ? 1u : 0u);
+              else umma_lo<2>(d, x + 2 * k, w + 2 * k, idesc, kb > 0 || k > 0 ? 1u : 0u);
+            }
+            umma_commit_pair(done);
+            if (F8 || kb == k_blocks - 1) {
+              umma_commit_pair(&sums_full[slot]);
+              if (++slot == kSlots) {
+                slot = 0;
+                slot_ph ^= 1;
+              }
+            }
+          }
+        }
+        if (!ok) drain_async();
+      }
+    } else if (warp == 2) {
+      if constexpr (F8) {   // as in group_gemm.cu, which says why the ring is never written where it is read
+        const int64_t units = first < tiles ? ((tiles - first + step - 1) / step) * k_blocks : 0;
+        int64_t t = first;
+        int kb = 0, into = 0, from_slot = 0, slot = 0;
+        uint32_t ph = 1;
+        Tile tile{};
+        auto ask = [&]() {
+          if (kb == 0) tile = tile_at(t);
+          const float* const from = p.sx + (int64_t)kb * p.rows + tile.row0 + lane;
+          float* const to = factors + into * kTile + lane;
+#pragma unroll
+          for (int i = 0; i < kHalf / 32; ++i)
+            if (lane + 32 * i < tile.rows) cp_async4(to + 32 * i, from + 32 * i);
+          if (lane < 2)
+            cp_async4(&w_scale[2 * into + lane], p.sw + ((int64_t)tile.expert * p.ch_blocks + min(tile.ch0 / kHalf + lane, p.ch_blocks - 1)) * k_blocks + kb);
+          if (++kb == k_blocks) {
+            kb = 0;
+            t += step;
+          }
+          if (++into == kAhead) into = 0;
+        };
+        for (int64_t u = -kLag; u < units; ++u) {
+          if (u >= 0 && !(ok = warp_wait(&sums_full[slot], ph, p.err, kWaitCode | 4))) break;
+          if (u + kLag < units) ask();
+          cp_async_commit();
+          if (u >= 0) {
+            cp_async_wait<kLag>();
+            __syncwarp();
+            const float w_lo = w_scale[2 * from_slot], w_hi = w_scale[2 * from_slot + 1];
+            float* const at = factors + from_slot * kTile + lane;
+#pragma unroll
+            for (int i = 0; i < kHalf / 32; ++i) {   // (places behind the tile's rows hold anything: nobody stores what they scale)
+              const float v = at[32 * i];
+              at[32 * i] = v * w_lo;
+              at[kHalf + 32 * i] = v * w_hi;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sums_full[slot]);
+            if (++from_slot == kAhead) from_slot = 0;
+            if (++slot == kSlots) {
+              slot = 0;
+              ph ^= 1;
+            }
+          }
+        }
+        cp_async_wait<0>();
+      }
+    } else {
+      uint32_t ph = 0;
+      for (int64_t t = first; t < tiles; t += step, ph ^= 1) {
+        const Tile tile = tile_at(t);
+        if (!(ok = warp_wait(out_full, ph, p.err, kWaitCode | 6))) break;
+        store_tile(p.y + tile.row0 * p.n + tile.ch0, done_tile, kOutLd, tile.rows, min(kTile, p.n - tile.ch0), p, lane);
+        if (lane == 0) mbar_arrive(out_empty);
+      }
+      bulk_wait();
+      zero_other_rows(p, lane);
+    }
+  } else {
+    if constexpr (F8) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsMany));
+    const int quad = warp & 3, half = (warp - 4) >> 2, row = quad * 32 + lane;
+    const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + half * kHalf, free_bar = mapa_u32(smem_u32(sums_empty), 0);
+    uint8_t* const put_at = done_tile + row * kOutLd + half * kHalf * 2;
+    int slot = 0, fslot = 0;
+    uint32_t slot_ph = 0, out_ph = 1;
+    for (int64_t t = first; t < tiles; t += step, out_ph ^= 1) {
+      const Tile tile = tile_at(t);
+      const bool mine = quad * 32 < tile.rows;   // some row of this warp is one
+      auto release = [&]() {   // the slot may be filled again
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_at(free_bar + slot * 8);
+        if (++slot == kSlots) {
+          slot = 0;
+          slot_ph ^= 1;
+        }
+      };
+      // channels 8j … 8j + 7 of this half
+      auto put8 = [&](int j, float2 a, float2 b, float2 c, float2 d) {
+        if (p.bias != nullptr) {
+          const int ch = tile.ch0 + half * kHalf + 8 * j;
+          float* const v[8] = {&a.x, &a.y, &b.x, &b.y, &c.x, &c.y, &d.x, &d.y};
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (ch + e < p.n) *v[e] += bf16_to_f(p.bias[ch + e]);
+        }
+        *reinterpret_cast<uint4*>(put_at + 16 * j) = make_uint4(pack2(a.x, a.y), pack2(b.x, b.y), pack2(c.x, c.y), pack2(d.x, d.y));
+      };
+      if constexpr (F8) {
+        uint64_t acc[kHalf / 2];
+#pragma unroll
+        for (int j = 0; j < kHalf / 2; ++j) acc[j] = 0;
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if (!(ok = warp_wait(&sums_full[slot], slot_ph, p.err, kWaitCode | 5))) break;
+          tc_fence_after();
+          if (mine) {
+            const float f = factors[fslot * kTile + half * kHalf + row];
+            const uint64_t ff = pair_of(f, f);
+            const uint32_t at = from + slot * kTile;
+#pragma unroll
+            for (int i = 0; i < kHalf / 32; ++i) {
+              uint32_t d[32];
+              load32(at + 32 * i, d);
+              if (i == kHalf / 32 - 1) release();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) acc[16 * i + j] = fma_pair(pair_of(d[2 * j], d[2 * j + 1]), ff, acc[16 * i + j]);
+            }
+          } else {
+            release();
+          }
+          if (++fslot == kAhead) fslot = 0;
+        }
+        if (!ok || !(ok = warp_wait(out_empty, out_ph, p.err, kWaitCode | 7))) break;
+        if (mine) {
+#pragma unroll
+          for (int j = 0; j < kHalf / 8; ++j) put8(j, halves(acc[4 * j]), halves(acc[4 * j + 1]), halves(acc[4 * j + 2]), halves(acc[4 * j + 3]));
+        }
+      } else {
+        if (!(ok = warp_wait(&sums_full[slot], slot_ph, p.err, kWaitCode | 5))) break;
+        tc_fence_after();
+        if (!(ok = warp_wait(out_empty, out_ph, p.err, kWaitCode | 7))) break;
+        if (mine) {
+#pragma unroll 1
+          for (int i = 0; i < kHalf / 32; ++i) {
+            uint32_t d[32];
+            load32(from + slot * kTile + 32 * i, d);
+            auto two = [&](int j) { return make_float2(__uint_as_float(d[j]), __uint_as_float(d[j + 1])); };
+#pragma unroll
+            for (int j = 0; j < 4; ++j) put8(4 * i + j, two(8 * j), two(8 * j + 2), two(8 * j + 4), two(8 * j + 6));
+          }
+        }
+        release();
+      }
+      fence_proxy_async();   // this warp's part of the tile lies in shared memory
+      __syncwarp();
+      if (lane == 0) mbar_arrive(out_full);
+    }
+  }
+  tc_fence_before();
+  __syncwarp();
+  __syncthreads();
+  cluster_sync_all();   // neither CTA still reads the pair's operands, barriers or sums
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_free<2>(tmem, kTmem);
+  }
+  cluster_sync_all();
+}
+
+template <bool F8>
+int launch(const GroupProduct& g, GemmArgs& p, cudaStream_t st) {
+  static PerDevice attrs;
+  B200_CUDA(attrs([] {
+    cudaFuncAttributes a{};
+    const cudaError_t e = cudaFuncGetAttributes(&a, group_wide_kernel<F8>);
+    if (e != cudaSuccess) return e;
+    if (F8 && a.numRegs != kRegsLaunch) return cudaErrorInvalidDeviceFunction;   // (the shares would not add up)
+    return cudaFuncSetAttribute(group_wide_kernel<F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTables + Groups::bytes(kMaxExperts));
+  }));
+  CUtensorMap tw, tx;
+  int rc;
+  if constexpr (F8) {
+    if ((rc = make_tmap_sw128_u8(&tw, g.w, g.experts * g.n, g.k, f8_ld(g.k), kHalf)) != B200_OK) return rc;
+    if ((rc = make_tmap_sw128_u8(&tx, g.x, g.rows, g.k, f8_ld(g.k), kHalf)) != B200_OK) return rc;
+  } else {
+    if ((rc = make_tmap_sw128(&tw, 2, g.w, 1, g.experts * g.n, g.k, 0, g.k, kHalf)) != B200_OK) return rc;
+    if ((rc = make_tmap_sw128(&tx, 2, g.x, 1, g.rows, g.k, 0, g.k, kHalf)) != B200_OK) return rc;
+  }
+  p.ch_blocks = (int)((g.n + kHalf - 1) / kHalf);
+  p.ch_tiles = (p.ch_blocks + 1) / 2;
+  p.splits = 1;
+  // tiles that there can be: every group's last one may be short
+  const int64_t row_tiles = g.starts ? g.rows / kTile + std::min<int64_t>(g.experts, g.rows) : (g.rows + kTile - 1) / kTile;
+  const int64_t pairs = std::min<int64_t>(row_tiles * p.ch_tiles, 74);
+  B200_CUDA(launch_pdl(group_wide_kernel<F8>, dim3((unsigned)(2 * pairs)), dim3(kThreads), (size_t)(kTables + Groups::bytes((int)g.experts)), st, op_pdl(st), tw, tx, p));
+  return B200_OK;
+}
+
+}  // namespace
+
+int launch_group_wide(const GroupProduct& g, GemmArgs& p, cudaStream_t st) { return g.x_scale != nullptr ? launch<true>(g, p, st) : launch<false>(g, p, st); }
+
+}  // namespace b200
