@@ -28,9 +28,8 @@ static_assert(128 * kRegsFew + 256 * kRegsMany <= kThreads * kRegsLaunch, "no wa
 static_assert(kTables + Groups::bytes(kMaxExperts) <= 227 * 1024, "room");
 
 #define B200_R8(b) "+r"(r[b]), "+r"(r[b + 1]), "+r"(r[b + 2]), "+r"(r[b + 3]), "+r"(r[b + 4]), "+r"(r[b + 5]), "+r"(r[b + 6]), "+r"(r[b + 7])
-// the wait holds what was loaded: nothing that uses it moves in front of it
-__device__ __forceinline__ void load32(uint32_t taddr, uint32_t (&r)[32]) {
-  tmem_ld32(taddr, r);
+// the wait for what tmem_ld32 has loaded holds it: nothing that uses it moves in front of the wait
+__device__ __forceinline__ void loaded(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" : B200_R8(0), B200_R8(8));
   asm volatile("" : B200_R8(16), B200_R8(24));
 }
@@ -236,41 +235,67 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
       };
       // channels 8j … 8j + 7 of this half
       auto put8 = [&](int j, float2 a, float2 b, float2 c, float2 d) {
-        if (p.bias != nullptr) {
-          const int ch = tile.ch0 + half * kHalf + 8 * j;
-          float* const v[8] = {&a.x, &a.y, &b.x, &b.y, &c.x, &c.y, &d.x, &d.y};
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (ch + e < p.n) *v[e] += bf16_to_f(p.bias[ch + e]);
-        }
         *reinterpret_cast<uint4*>(put_at + 16 * j) = make_uint4(pack2(a.x, a.y), pack2(b.x, b.y), pack2(c.x, c.y), pack2(d.x, d.y));
       };
+      auto bias_of = [&](int j) {   // of channels 2j, 2j + 1
+        const int ch = tile.ch0 + half * kHalf + 2 * j;
+        return make_float2(ch < p.n ? bf16_to_f(p.bias[ch]) : 0.f, ch + 1 < p.n ? bf16_to_f(p.bias[ch + 1]) : 0.f);
+      };
       if constexpr (F8) {
+        constexpr int PIECES = kHalf / 32;
         uint64_t acc[kHalf / 2];
 #pragma unroll
         for (int j = 0; j < kHalf / 2; ++j) acc[j] = 0;
-        for (int kb = 0; kb < k_blocks; ++kb) {
-          if (!(ok = warp_wait(&sums_full[slot], slot_ph, p.err, kWaitCode | 5))) break;
-          tc_fence_after();
-          if (mine) {
+        uint32_t d[2][32];
+        if (!(ok = warp_wait(&sums_full[slot], slot_ph, p.err, kWaitCode | 5))) break;
+        tc_fence_after();
+        if (mine) {
+          // One load is always on its way while another's sums are added, the next unit's first one too where its products are done by then.
+          tmem_ld32(from + slot * kTile, d[0]);
+          for (int kb = 0; kb < k_blocks; ++kb) {
             const float f = factors[fslot * kTile + half * kHalf + row];
             const uint64_t ff = pair_of(f, f);
             const uint32_t at = from + slot * kTile;
+            bool next = false;
 #pragma unroll
-            for (int i = 0; i < kHalf / 32; ++i) {
-              uint32_t d[32];
-              load32(at + 32 * i, d);
-              if (i == kHalf / 32 - 1) release();
+            for (int i = 0; i < PIECES; ++i) {
+              loaded(d[i % 2]);
+              if (i + 1 < PIECES) {
+                tmem_ld32(at + 32 * (i + 1), d[(i + 1) % 2]);
+              } else {
+                release();
+                next = kb + 1 < k_blocks && __all_sync(0xffffffffu, mbar_test(&sums_full[slot], slot_ph));
+                if (next) {
+                  tc_fence_after();
+                  tmem_ld32(from + slot * kTile, d[0]);
+                }
+              }
 #pragma unroll
-              for (int j = 0; j < 16; ++j) acc[16 * i + j] = fma_pair(pair_of(d[2 * j], d[2 * j + 1]), ff, acc[16 * i + j]);
+              for (int j = 0; j < 16; ++j) acc[16 * i + j] = fma_pair(pair_of(d[i % 2][2 * j], d[i % 2][2 * j + 1]), ff, acc[16 * i + j]);
             }
-          } else {
-            release();
+            if (++fslot == kAhead) fslot = 0;
+            if (!next && kb + 1 < k_blocks) {
+              if (!(ok = warp_wait(&sums_full[slot], slot_ph, p.err, kWaitCode | 5))) break;
+              tc_fence_after();
+              tmem_ld32(from + slot * kTile, d[0]);
+            }
           }
-          if (++fslot == kAhead) fslot = 0;
+        } else {
+          for (int kb = 0; kb < k_blocks; ++kb) {
+            release();
+            if (++fslot == kAhead) fslot = 0;
+            if (kb + 1 < k_blocks && !(ok = warp_wait(&sums_full[slot], slot_ph, p.err, kWaitCode | 5))) break;
+          }
         }
         if (!ok || !(ok = warp_wait(out_empty, out_ph, p.err, kWaitCode | 7))) break;
         if (mine) {
+          if (p.bias != nullptr) {
+#pragma unroll
+            for (int j = 0; j < kHalf / 2; ++j) {
+              const float2 v = halves(acc[j]), b = bias_of(j);
+              acc[j] = pair_of(v.x + b.x, v.y + b.y);
+            }
+          }
 #pragma unroll
           for (int j = 0; j < kHalf / 8; ++j) put8(j, halves(acc[4 * j]), halves(acc[4 * j + 1]), halves(acc[4 * j + 2]), halves(acc[4 * j + 3]));
         }
@@ -282,10 +307,18 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
 #pragma unroll 1
           for (int i = 0; i < kHalf / 32; ++i) {
             uint32_t d[32];
-            load32(from + slot * kTile + 32 * i, d);
-            auto two = [&](int j) { return make_float2(__uint_as_float(d[j]), __uint_as_float(d[j + 1])); };
+            tmem_ld32(from + slot * kTile + 32 * i, d);
+            loaded(d);
+            auto two = [&](int j) {
+              float2 v = make_float2(__uint_as_float(d[2 * j]), __uint_as_float(d[2 * j + 1]));
+              if (p.bias != nullptr) {
+                const float2 b = bias_of(16 * i + j);
+                v = make_float2(v.x + b.x, v.y + b.y);
+              }
+              return v;
+            };
 #pragma unroll
-            for (int j = 0; j < 4; ++j) put8(4 * i + j, two(8 * j), two(8 * j + 2), two(8 * j + 4), two(8 * j + 6));
+            for (int j = 0; j < 4; ++j) put8(4 * i + j, two(4 * j), two(4 * j + 1), two(4 * j + 2), two(4 * j + 3));
           }
         }
         release();
