@@ -27,7 +27,9 @@ namespace {
 // The C ABI of the library that _lib.py has loaded, whatever its file is called: this module is linked to none.
 #define B200_FUNCTIONS(F) \
   F(gemv_bf16) F(gemm_bf16) F(rmsnorm_bf16) F(silu_mul_bf16) F(add_bf16) F(attn_bf16) F(gemv_fused_bf16) F(attn_decode_workspace_bytes) F(attn_decode_bf16) F(w4_workspace_bytes) F(w4_linear_bf16) \
-  F(kv4_store) F(kv4_load) F(kv4_attention_workspace_bytes) F(kv4_attention) F(kv4_extend) F(kv4_fork) F(kv4_free) F(kv4_compact) F(kv4_workspace_bytes)
+  F(kv4_store) F(kv4_load) F(kv4_attention_workspace_bytes) F(kv4_attention) F(kv4_extend) F(kv4_fork) F(kv4_free) F(kv4_compact) F(kv4_workspace_bytes) \
+  F(f8_rows_bf16) F(rmsnorm_f8) F(silu_mul_f8) F(f8_rows_dequant) F(f8_linear_bf16) F(f8_grouped_bf16) F(grouped_bf16) \
+  F(experts_f8_workspace_bytes) F(experts_f8_bf16)
 struct {
 #define B200_FIELD(f) decltype(&b200_##f) f;
   B200_FUNCTIONS(B200_FIELD)
@@ -382,12 +384,222 @@ PyObject* kv4_compact(PyObject*, PyObject* const* a, Py_ssize_t n_args) {   // c
   END_HANDLE_TH_ERRORS
 }
 
+// ---- rows and weights of 8 bits, products grouped by expert
+constexpr at::ScalarType kF8 = at::kFloat8_e4m3fn;
+constexpr int64_t kMaxExperts = 1024;
+int64_t f8_ld(int64_t k) { return (k + 15) / 16 * 16; }
+int64_t f8_blocks(int64_t k) { return (k + 127) / 128; }
+bool on16(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+
+// rows of a result in 8 bits beside x, of the shape `lead` … k
+struct F8Out {
+  at::Tensor q, scale;
+  F8Out(const at::Tensor& x, at::IntArrayRef lead, int64_t rows, int64_t k) {
+    c10::SmallVector<int64_t, 6> s(lead.begin(), lead.end());
+    s.push_back(f8_ld(k));
+    q = at::empty(s, at::TensorOptions().dtype(kF8).device(x.device()));
+    scale = at::empty({f8_blocks(k), rows}, at::TensorOptions().dtype(at::kFloat).device(x.device()));
+  }
+  float* scales() const { return static_cast<float*>(scale.data_ptr()); }
+};
+PyObject* both(const at::Tensor& a, const at::Tensor& b, const at::Tensor* c = nullptr) {
+  PyObject *pa = THPVariable_Wrap(a), *pb = THPVariable_Wrap(b), *pc = c == nullptr ? nullptr : THPVariable_Wrap(*c);
+  PyObject* out = !pa || !pb || (c != nullptr && !pc) ? nullptr : pc == nullptr ? PyTuple_Pack(2, pa, pb) : PyTuple_Pack(3, pa, pb, pc);
+  Py_XDECREF(pa);
+  Py_XDECREF(pb);
+  Py_XDECREF(pc);
+  return out;
+}
+template <typename F>
+int launch(F call) {
+  return call((void*)c10::cuda::getCurrentCUDAStream().stream());
+}
+
+PyObject* f8_rows(PyObject*, PyObject* const* a, Py_ssize_t n_args) {   // x
+  HANDLE_TH_ERRORS
+  const at::Tensor* x;
+  if (n_args != 1 || modes() || !(x = plain(a[0])) || x->dim() < 1 || x->numel() < 1 || x->size(-1) > 1 << 24 || !here(*x)) Py_RETURN_NONE;
+  const int64_t k = x->size(-1), rows = x->numel() / k;
+  int rc;
+  c10::optional<F8Out> out;
+  {
+    pybind11::gil_scoped_release free;
+    out.emplace(*x, x->sizes().slice(0, x->dim() - 1), rows, k);
+    rc = launch([&](void* st) { return abi.f8_rows_bf16(out->q.data_ptr(), out->scales(), x->data_ptr(), k, rows, nullptr, rows, k, st); });
+  }
+  return rc != 0 ? PyLong_FromLong(rc) : both(out->q, out->scale);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* norm_f8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {   // x, residual or None, weight or None, eps
+  HANDLE_TH_ERRORS
+  const at::Tensor *x, *r, *w;
+  if (n_args != 4 || modes() || !(x = plain(a[0])) || !plain_or_none(a[1], r) || !plain_or_none(a[2], w) || !PyFloat_Check(a[3]) || x->dim() < 1 || x->numel() < 1 ||
+      x->size(-1) > 1 << 24 || (r && r->sizes() != x->sizes()) || (w && w->numel() != x->size(-1)) || !here(*x) || (r && r->device() != x->device()) ||
+      (w && w->device() != x->device()))
+    Py_RETURN_NONE;
+  const int64_t dim = x->size(-1), rows = x->numel() / dim;
+  const float eps = (float)PyFloat_AS_DOUBLE(a[3]);
+  int rc;
+  c10::optional<F8Out> out;
+  at::Tensor sum;
+  {
+    pybind11::gil_scoped_release free;
+    out.emplace(*x, x->sizes().slice(0, x->dim() - 1), rows, dim);
+    if (r) sum = at::empty(x->sizes(), at::TensorOptions().dtype(at::kBFloat16).device(x->device()));
+    rc = launch([&](void* st) {
+      return abi.rmsnorm_f8(out->q.data_ptr(), out->scales(), r ? sum.data_ptr() : nullptr, x->data_ptr(), ptr(r), ptr(w), rows, dim, eps, st);
+    });
+  }
+  return rc != 0 ? PyLong_FromLong(rc) : both(out->q, out->scale, r ? &sum : nullptr);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* silu_mul_f8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {   // x
+  HANDLE_TH_ERRORS
+  const at::Tensor* x;
+  if (n_args != 1 || modes() || !(x = plain(a[0])) || x->dim() < 1 || x->numel() < 1 || x->size(-1) % 2 != 0 || x->size(-1) > 1 << 24 || !here(*x)) Py_RETURN_NONE;
+  const int64_t n = x->size(-1) / 2, rows = x->numel() / (2 * n);
+  int rc;
+  c10::optional<F8Out> out;
+  {
+    pybind11::gil_scoped_release free;
+    out.emplace(*x, x->sizes().slice(0, x->dim() - 1), rows, n);
+    rc = launch([&](void* st) { return abi.silu_mul_f8(out->q.data_ptr(), out->scales(), x->data_ptr(), rows, n, st); });
+  }
+  return rc != 0 ? PyLong_FromLong(rc) : both(out->q, out->scale);
+  END_HANDLE_TH_ERRORS
+}
+
+// rows in 8 bits that a caller brings: q, scale, k — or a bf16 tensor in the place of q with None behind it, which becomes such rows first
+struct F8In {
+  const at::Tensor *q = nullptr, *scale = nullptr;
+  int64_t k, rows;
+  bool take(PyObject* const* a) {
+    if (a[1] == Py_None) {
+      if (!(q = plain(a[0])) || q->dim() < 1 || q->numel() < 1 || q->size(-1) > 1 << 24) return false;
+      k = q->size(-1);
+    } else {
+      if (!(q = plain(a[0], kF8)) || !(scale = plain(a[1], at::kFloat)) || !PyLong_Check(a[2]) || q->dim() < 1 || q->numel() < 1 || !on16(*q)) return false;
+      k = whole_number(a[2]);
+      if (k < 1 || k > 1 << 24 || q->size(-1) != f8_ld(k) || scale->dim() != 2 || scale->device() != q->device()) return false;
+    }
+    rows = q->numel() / q->size(-1);
+    return here(*q) && (scale == nullptr || (scale->size(0) == f8_blocks(k) && scale->size(1) == rows));
+  }
+  // calls with 8-bit rows: the caller's, or made in scratch memory
+  template <typename F>
+  int with(void* st, F call) const {
+    if (scale != nullptr) return call(q->data_ptr(), static_cast<const float*>(scale->data_ptr()));
+    const int64_t bytes = (rows * f8_ld(k) + 255) / 256 * 256;
+    const at::DataPtr ws = scratch(bytes + rows * f8_blocks(k) * 4);
+    float* const s = reinterpret_cast<float*>(static_cast<char*>(ws.get()) + bytes);
+    const int rc = abi.f8_rows_bf16(ws.get(), s, q->data_ptr(), k, rows, nullptr, rows, k, st);
+    return rc != 0 ? rc : call(ws.get(), s);
+  }
+};
+// q, scale, n, k of a weight of 8 bits, one matrix (experts 0) or many
+bool f8_weight(PyObject* const* a, const at::Tensor& beside, bool many, b200_f8_weight& w) {
+  const at::Tensor *q, *scale;
+  if (!(q = plain(a[0], kF8)) || !(scale = plain(a[1], at::kFloat)) || !PyLong_Check(a[2]) || !PyLong_Check(a[3]) || q->dim() != (many ? 3 : 2) || scale->dim() != q->dim())
+    return false;
+  const int64_t n = whole_number(a[2]), k = whole_number(a[3]), experts = many ? q->size(0) : 1;
+  if (n < 1 || k < 1 || n > 1 << 20 || k > 1 << 24 || experts < 1 || experts > kMaxExperts || experts * n >= int64_t(1) << 31 || q->size(-2) != n || q->size(-1) != f8_ld(k) ||
+      scale->size(-2) != f8_blocks(n) || scale->size(-1) != f8_blocks(k) || (many && scale->size(0) != experts) || q->device() != beside.device() ||
+      scale->device() != beside.device() || !on16(*q))
+    return false;
+  w = b200_f8_weight{q->data_ptr(), static_cast<const float*>(scale->data_ptr()), (int32_t)n, (int32_t)k, (int32_t)experts};
+  return true;
+}
+const at::Tensor* starts_of(PyObject* o, const at::Tensor& beside, int64_t experts) {
+  const at::Tensor* t = plain(o, at::kInt);
+  return t != nullptr && t->dim() == 1 && t->size(0) == experts + 1 && t->device() == beside.device() ? t : nullptr;
+}
+
+PyObject* f8_rows_dequantize(PyObject*, PyObject* const* a, Py_ssize_t n_args) {   // q, scale, k
+  HANDLE_TH_ERRORS
+  F8In x;
+  if (n_args != 3 || modes() || a[1] == Py_None || !x.take(a)) Py_RETURN_NONE;
+  at::Tensor y;
+  int rc;
+  {
+    pybind11::gil_scoped_release free;
+    y = at::empty(with_last(*x.q, x.k), at::TensorOptions().dtype(at::kFloat).device(x.q->device()));
+    rc = launch([&](void* st) {
+      return abi.f8_rows_dequant(static_cast<float*>(y.data_ptr()), x.q->data_ptr(), static_cast<const float*>(x.scale->data_ptr()), x.rows, x.k, st);
+    });
+  }
+  return rc == 0 ? THPVariable_Wrap(y) : PyLong_FromLong(rc);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* linear_f8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {   // x: q, scale, k or tensor, None, None; weight: q, scale, n, k; bias or None
+  HANDLE_TH_ERRORS
+  F8In x;
+  b200_f8_weight w;
+  const at::Tensor* b;
+  if (n_args != 8 || modes() || !x.take(a) || !f8_weight(a + 3, *x.q, false, w) || !plain_or_none(a[7], b) || w.k != x.k ||
+      (b && (b->numel() != w.n || b->device() != x.q->device())))
+    Py_RETURN_NONE;
+  return run(*x.q, with_last(*x.q, w.n), [&](void* y, void* st) {
+    return x.with(st, [&](const void* q, const float* scale) { return abi.f8_linear_bf16(y, q, scale, &w, ptr(b), x.rows, st); });
+  });
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* grouped_linear_f8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {   // x as above; weight of experts; starts
+  HANDLE_TH_ERRORS
+  F8In x;
+  b200_f8_weight w;
+  const at::Tensor* starts;
+  if (n_args != 8 || modes() || !x.take(a) || x.q->dim() != 2 || !f8_weight(a + 3, *x.q, true, w) || !(starts = starts_of(a[7], *x.q, w.experts)) || w.k != x.k)
+    Py_RETURN_NONE;
+  return run(*x.q, {x.rows, w.n}, [&](void* y, void* st) {
+    return x.with(st, [&](const void* q, const float* scale) { return abi.f8_grouped_bf16(y, q, scale, &w, static_cast<const int32_t*>(starts->data_ptr()), x.rows, st); });
+  });
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* grouped_linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {   // x, weight, starts
+  HANDLE_TH_ERRORS
+  const at::Tensor *x, *w, *starts;
+  if (n_args != 3 || modes() || !(x = plain(a[0])) || !(w = plain(a[1])) || x->dim() != 2 || w->dim() != 3 || x->numel() < 1 || w->numel() < 1 || !here(*x) ||
+      w->device() != x->device() || x->size(1) != w->size(2) || w->size(0) > kMaxExperts || w->size(2) % 8 != 0 || !on16(*x) || !on16(*w) ||
+      !(starts = starts_of(a[2], *x, w->size(0))))
+    Py_RETURN_NONE;
+  const int64_t rows = x->size(0), experts = w->size(0), n = w->size(1), k = w->size(2);
+  return run(*x, {rows, n}, [&](void* y, void* st) {
+    return abi.grouped_bf16(y, x->data_ptr(), w->data_ptr(), static_cast<const int32_t*>(starts->data_ptr()), rows, experts, n, k, st);
+  });
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* experts_f8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {   // x, chosen, weights, two weights of experts: q, scale, n, k
+  HANDLE_TH_ERRORS
+  const at::Tensor *x, *chosen, *weights;
+  b200_f8_weight w_in, w_out;
+  if (n_args != 11 || modes() || !(x = plain(a[0])) || !(chosen = plain(a[1], at::kInt)) || !(weights = plain(a[2], at::kFloat)) || x->dim() != 2 || x->numel() < 1 ||
+      chosen->dim() != 2 || chosen->numel() < 1 || weights->sizes() != chosen->sizes() || chosen->size(0) != x->size(0) || !here(*x) ||
+      chosen->device() != x->device() || weights->device() != x->device() || !f8_weight(a + 3, *x, true, w_in) || !f8_weight(a + 7, *x, true, w_out) ||
+      w_in.experts != w_out.experts || w_in.n != 2 * w_out.k || w_in.k != w_out.n || x->size(1) != w_in.k || chosen->size(1) > w_in.experts)
+    Py_RETURN_NONE;
+  const int64_t rows = x->size(0), top = chosen->size(1), bytes = abi.experts_f8_workspace_bytes(rows, top, w_in.experts, w_in.k, w_out.k);
+  if (bytes < 0) Py_RETURN_NONE;
+  return run(*x, x->sizes(), [&](void* y, void* st) {
+    const at::DataPtr ws = scratch(bytes);
+    return abi.experts_f8_bf16(y, x->data_ptr(), static_cast<const int32_t*>(chosen->data_ptr()), static_cast<const float*>(weights->data_ptr()), &w_in, &w_out, rows,
+                               top, ws.get(), st);
+  });
+  END_HANDLE_TH_ERRORS
+}
+
 #define B200_OP(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {{"_bind", bind, METH_O, nullptr}, B200_OP(linear),     B200_OP(gemm),        B200_OP(rms_norm),
                          B200_OP(silu_mul),                B200_OP(add),        B200_OP(flash_attention),
                          B200_OP(gemv_fused),              B200_OP(attn_decode), B200_OP(linear_w4),
                          B200_OP(kv4_store), B200_OP(kv4_load), B200_OP(kv4_attention), B200_OP(kv4_extend), B200_OP(kv4_fork), B200_OP(kv4_free),
-                         B200_OP(kv4_compact), {nullptr, nullptr, 0, nullptr}};
+                         B200_OP(kv4_compact), B200_OP(f8_rows), B200_OP(norm_f8), B200_OP(silu_mul_f8), B200_OP(f8_rows_dequantize), B200_OP(linear_f8),
+                         B200_OP(grouped_linear_f8), B200_OP(grouped_linear), B200_OP(experts_f8), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "b200ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -503,6 +503,12 @@ def _f8_width(x: torch.Tensor, what: str) -> int:
 def f8_rows(x: torch.Tensor, index: Optional[torch.Tensor] = None) -> F8Rows:
     """Rows of x bf16 [..., k] in 8 bits, block by block of 128: s = max(fp32(max|x| / 448), 2^-126), value = e4m3(fp32(x / s)).  index int32 [rows]: row i of the
     result is row index[i] of x [rows of x, k], zeros where that is none of them (as expert_order's source has it)."""
+    if index is None:
+        y = _fast.f8_rows(x)
+        if y.__class__ is tuple:
+            return F8Rows(*y, x.shape[-1])
+        if y is not None:
+            check(y, "b200_f8_rows_bf16")
     if not x.is_cuda or x.dtype != torch.bfloat16:
         _chk(x, "f8_rows.x")
     k = _f8_width(x, "f8_rows")
@@ -529,6 +535,11 @@ def f8_rows(x: torch.Tensor, index: Optional[torch.Tensor] = None) -> F8Rows:
 
 def f8_rows_dequantize(x: F8Rows) -> torch.Tensor:
     """fp32 [..., k]: what the 8 bits stand for."""
+    y = _fast.f8_rows_dequantize(x.q, x.scale, x.k) if x.__class__ is F8Rows else None
+    if y.__class__ is _Tensor:
+        return y
+    if y is not None:
+        check(y, "b200_f8_rows_dequant")
     q, scale, shape, rows = _f8_take(x, "f8_rows_dequantize")
     _same_device("f8_rows_dequantize", q, scale)
     out = torch.empty(*shape, x.k, dtype=torch.float32, device=q.device)
@@ -538,6 +549,11 @@ def f8_rows_dequantize(x: F8Rows) -> torch.Tensor:
 
 
 def _norm_f8(x, residual, weight, eps, what):
+    y = _fast.norm_f8(x, residual, weight, eps)
+    if y.__class__ is tuple:
+        return F8Rows(y[0], y[1], x.shape[-1]), (None if residual is None else y[2])
+    if y is not None:
+        check(y, "b200_rmsnorm_f8")
     x = _chk(x, f"{what}.x")
     dim = _f8_width(x, what)
     if residual is not None:
@@ -571,6 +587,11 @@ def add_rms_norm_f8(x: torch.Tensor, residual: torch.Tensor, weight: Optional[to
 
 def silu_mul_f8(x: torch.Tensor) -> F8Rows:
     """silu_mul in 8 bits: last dim = [gate | up], t = silu(gate)·up in fp32, blocks of 128 as f8_rows has them."""
+    y = _fast.silu_mul_f8(x)
+    if y.__class__ is tuple:
+        return F8Rows(*y, x.shape[-1] // 2)
+    if y is not None:
+        check(y, "b200_silu_mul_f8")
     x = _chk(x, "silu_mul_f8.x")
     if x.dim() < 1 or x.shape[-1] % 2 or x.shape[-1] < 2:
         raise B200Error(f"silu_mul_f8: last dimension must be even, got {tuple(x.shape)}")
@@ -586,6 +607,12 @@ def silu_mul_f8(x: torch.Tensor) -> F8Rows:
 def linear_f8(x, weight: F8Weight, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """linear over a weight of 8 bits: x F8Rows, or bf16 [..., k] (which f8_rows makes 8-bit rows of first) → bf16(x·Wᵀ + bias) [..., n], sums of 128 products scaled
     and added in fp32, rounded once."""
+    if weight.__class__ is F8Weight:
+        y = (_fast.linear_f8(x.q, x.scale, x.k, *weight, bias) if x.__class__ is F8Rows else _fast.linear_f8(x, None, None, *weight, bias))
+        if y.__class__ is _Tensor:
+            return y
+        if y is not None:
+            check(y, "b200_f8_linear_bf16")
     import ctypes as C
     d, parts = _f8_desc(weight, "linear_f8", 2)
     if x.__class__ is not F8Rows:
@@ -615,6 +642,11 @@ def _starts(starts, experts: int, what: str) -> torch.Tensor:
 def grouped_linear(x: torch.Tensor, weight: torch.Tensor, starts: torch.Tensor) -> torch.Tensor:
     """Products grouped by expert: rows starts[e] … starts[e + 1] − 1 of x bf16 [rows, k] meet weight[e] of bf16 [experts, n, k] → bf16 [rows, n], fp32 sums, rounded
     once.  starts int32 [experts + 1] on the device, not falling; a group may be empty, rows of no group come out as zeros."""
+    y = _fast.grouped_linear(x, weight, starts)
+    if y.__class__ is _Tensor:
+        return y
+    if y is not None:
+        check(y, "b200_grouped_bf16")
     x, weight = _chk(x, "grouped_linear.x"), _chk(weight, "grouped_linear.weight")
     if x.dim() != 2 or weight.dim() != 3 or x.shape[1] != weight.shape[2]:
         raise B200Error(f"grouped_linear: x {tuple(x.shape)} does not match weights {tuple(weight.shape)}")
@@ -632,6 +664,12 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, starts: torch.Tensor) 
 
 def grouped_linear_f8(x, weight: F8Weight, starts: torch.Tensor) -> torch.Tensor:
     """grouped_linear over rows and weights of 8 bits: x F8Rows [rows, k], or bf16 (which f8_rows makes 8-bit rows of first), weight of experts."""
+    if weight.__class__ is F8Weight:
+        y = (_fast.grouped_linear_f8(x.q, x.scale, x.k, *weight, starts) if x.__class__ is F8Rows else _fast.grouped_linear_f8(x, None, None, *weight, starts))
+        if y.__class__ is _Tensor:
+            return y
+        if y is not None:
+            check(y, "b200_f8_grouped_bf16")
     import ctypes as C
     d, parts = _f8_desc(weight, "grouped_linear_f8", 3)
     if x.__class__ is not F8Rows:
@@ -688,6 +726,12 @@ def experts_f8(x: torch.Tensor, chosen: torch.Tensor, weights: torch.Tensor, w_i
     """A layer of routed experts in 8 bits: x bf16 [rows, width], chosen int32 and weights fp32 [rows, top], w_in [experts, 2·ff, width] (gate | up) and w_out
     [experts, width, ff] of 8 bits → bf16 [rows, width].  What expert_order, f8_rows, grouped_linear_f8, silu_mul_f8, grouped_linear_f8 and expert_combine give one
     behind the other.  A choice outside the experts adds nothing."""
+    if w_in.__class__ is F8Weight and w_out.__class__ is F8Weight:
+        y = _fast.experts_f8(x, chosen, weights, *w_in, *w_out)
+        if y.__class__ is _Tensor:
+            return y
+        if y is not None:
+            check(y, "b200_experts_f8_bf16")
     import ctypes as C
     d_in, parts_in = _f8_desc(w_in, "experts_f8", 3)
     d_out, parts_out = _f8_desc(w_out, "experts_f8", 3)
