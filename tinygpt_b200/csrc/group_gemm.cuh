@@ -148,9 +148,29 @@ __device__ __forceinline__ void store_tile(__nv_bfloat16* out, const uint8_t* ti
       for (int row = lane; row < rows; row += 32) bulk_store(out + (int64_t)row * p.n, tile + row * ld, width * 2);
     bulk_commit();
     bulk_wait_read();
-  } else {
-    for (int row = 0; row < rows; ++row)
-      for (int i = lane; i < width; i += 32) out[(int64_t)row * p.n + i] = reinterpret_cast<const __nv_bfloat16*>(tile + row * ld)[i];
+  } else {   // a lane takes four channels, eight rows at a time, in pieces that n allows
+    const int piece = p.n % 4 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 7) == 0 ? 4 : p.n % 2 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 3) == 0 ? 2 : 1;
+    for (int i = lane * 4; i < width; i += 128)
+      for (int row0 = 0; row0 < rows; row0 += 8) {
+        uint2 v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const uint2*>(tile + min(row0 + j, rows - 1) * ld + i * 2);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          __nv_bfloat16* const to = out + (int64_t)(row0 + j) * p.n + i;
+          if (row0 + j >= rows) continue;
+          if (piece == 4) {   // (n ends on such a piece)
+            *reinterpret_cast<uint2*>(to) = v[j];
+          } else if (piece == 2) {
+            *reinterpret_cast<uint32_t*>(to) = v[j].x;
+            if (i + 2 < width) *reinterpret_cast<uint32_t*>(to + 2) = v[j].y;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (i + e < width) reinterpret_cast<uint16_t*>(to)[e] = (uint16_t)((e < 2 ? v[j].x : v[j].y) >> (e % 2 * 16));
+          }
+        }
+      }
   }
   __syncwarp();
 }
