@@ -11,7 +11,7 @@ namespace {
 // A stable counting sort in one CTA: every warp takes a run of the pairs, 32 at a time in their order.  Lanes that hold the same expert find each other
 // (match), so a warp's count of an expert is its own and no atomics decide an order.
 //   1. counts[warp][e];  2. the sum in front of each: experts first, then warps;  3. the runs again, each pair to its place
-constexpr int kOrderWarps = 32;
+constexpr int kOrderWarps = 32, kOrderAhead = 8;
 
 __global__ void __launch_bounds__(32 * kOrderWarps) expert_order_kernel(int32_t* __restrict__ starts, int32_t* __restrict__ source, int32_t* __restrict__ place,
                                                                         const int32_t* __restrict__ chosen, int pairs, int top, int experts) {
@@ -24,10 +24,12 @@ __global__ void __launch_bounds__(32 * kOrderWarps) expert_order_kernel(int32_t*
   __syncthreads();
   const int run = (pairs + 32 * kOrderWarps - 1) / (32 * kOrderWarps) * 32, from = min(warp * run, pairs), to = min(from + run, pairs);
   int* const own = counts + warp * experts;
+  int ahead[kOrderAhead];   // the run's first choices, asked for together
+#pragma unroll
+  for (int j = 0; j < kOrderAhead; ++j) ahead[j] = from + 32 * j + lane < to ? chosen[from + 32 * j + lane] : -1;
   auto walk = [&](auto at) {
-    for (int i = from; i < to; i += 32) {
+    auto step = [&](int i, int e) {
       const bool is = i + lane < to;
-      const int e = is ? chosen[i + lane] : -1;
       const bool valid = e >= 0 && e < experts;
       const unsigned same = __match_any_sync(0xffffffffu, valid ? e : -1);
       int before = 0;
@@ -36,7 +38,11 @@ __global__ void __launch_bounds__(32 * kOrderWarps) expert_order_kernel(int32_t*
       if (valid && lane == __ffs(same) - 1) own[e] = before + __popc(same);
       __syncwarp();
       if (is) at(i + lane, valid, before + __popc(same & ((1u << lane) - 1)));
-    }
+    };
+#pragma unroll
+    for (int j = 0; j < kOrderAhead; ++j)
+      if (from + 32 * j < to) step(from + 32 * j, ahead[j]);
+    for (int i = from + 32 * kOrderAhead; i < to; i += 32) step(i, i + lane < to ? chosen[i + lane] : -1);
   };
   walk([](int, bool, int) {});
   __syncthreads();
@@ -213,7 +219,7 @@ int b200_experts_f8_bf16(void* out, const void* x, const int32_t* chosen, const 
   auto ints = [&](int64_t at) { return (int32_t*)(ws + at); };
   auto floats = [&](int64_t at) { return (float*)(ws + at); };
   if ((rc = launch_expert_order(ints(s.starts), ints(s.source), ints(s.place), chosen, rows, top, experts, st)) != B200_OK) return rc;
-  if ((rc = launch_f8_rows(ws + s.q, floats(s.scale), x, width, rows, ints(s.source), pairs, width, st)) != B200_OK) return rc;
+  if ((rc = launch_f8_rows_to(ws + s.q, floats(s.scale), x, ints(s.place), rows, top, pairs, width, st)) != B200_OK) return rc;
   if ((rc = launch_group_product({ws + s.gate_up, ws + s.q, floats(s.scale), w_in->q, w_in->scale, ints(s.starts), nullptr, pairs, experts, 2 * ff, width}, st)) != B200_OK)
     return rc;
   if ((rc = launch_silu_mul_f8(ws + s.a, floats(s.a_scale), ws + s.gate_up, pairs, ff, st)) != B200_OK) return rc;

@@ -29,40 +29,58 @@ __device__ __forceinline__ void load8(const __nv_bfloat16* row, int i, int k, fl
 }
 
 // value and scale of eight entries of a block; a row's last piece may reach past its ld bytes
-__device__ __forceinline__ void store8(uint8_t* q, float* scale, int64_t row, int64_t rows, int i, int64_t ld, int blocks, const float (&t)[8], float s, float factor) {
-  if (i < ld) *reinterpret_cast<uint2*>(q + row * ld + i) = f8_pack8(t, s);
-  if (i % kF8Block == 0 && i / kF8Block < blocks) scale[(int64_t)(i / kF8Block) * rows + row] = s * factor;
+__device__ __forceinline__ void store8(uint8_t* q, float* scale, int64_t row, int64_t rows, int i, int64_t ld, int blocks, uint2 w, float s) {
+  if (i < ld) *reinterpret_cast<uint2*>(q + row * ld + i) = w;
+  if (i % kF8Block == 0 && i / kF8Block < blocks) scale[(int64_t)(i / kF8Block) * rows + row] = s;
 }
 
-// Sixteen lanes to a block.  SILU: x rows are [gate | up], k entries each.
-template <bool WIDE, bool SILU>
+// Sixteen lanes to a block, blocks in a row's order.  kList: row i of the result is row list[i] of x (list null: i).  kSilu: rows
+// of x are [gate | up], k entries each.  kTo: row i of x goes to the rows list[i][0 … top − 1] of the result, whose `rows` there are.
+enum RowsKind { kList, kSilu, kTo };
+template <bool WIDE, RowsKind KIND>
 __global__ void __launch_bounds__(256) f8_rows_kernel(uint8_t* __restrict__ q, float* __restrict__ scale, const __nv_bfloat16* __restrict__ x, int64_t ld_x,
-                                                      int64_t x_rows, const int32_t* __restrict__ index, int64_t rows, int k, int blocks) {
+                                                      int64_t x_rows, const int32_t* __restrict__ list, int top, int64_t rows, int k, int blocks) {
   pdl_wait();
   pdl_trigger();
-  const int64_t ld = f8_ld(k), all = rows * blocks;
-  const int part = threadIdx.x % 16;
+  const int64_t ld = f8_ld(k), all = (KIND == kTo ? x_rows : rows) * blocks;
   for (int64_t first = (int64_t)blockIdx.x * 16; first < all; first += (int64_t)gridDim.x * 16) {   // (lanes of a warp stay together)
     const int64_t at = first + threadIdx.x / 16;
-    const int64_t row = at / blocks;
-    const int i = (int)(at % blocks) * kF8Block + part * 8;
-    float t[8];
+    const int64_t row = all < 1ll << 31 ? (int64_t)((uint32_t)at / (uint32_t)blocks) : at / blocks;   // (64 bits: a hundred instructions)
+    const bool is = at < all;
+    int64_t from = row;
+    if (KIND == kList && list != nullptr && is) from = list[row];
+    const int i = (int)(at - row * blocks) * kF8Block + threadIdx.x % 16 * 8;
+    const bool in = is && from >= 0 && from < x_rows && i < k;
+    float t[8], s;
+    uint32_t m = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) t[e] = 0.f;
-    if (at < all) {
-      const int64_t from = index == nullptr ? row : index[row];
-      if (from >= 0 && from < x_rows) {
+    if (in) {
+      if (WIDE && KIND != kSilu) {
+        const uint4 u = *reinterpret_cast<const uint4*>(x + from * ld_x + i);
+        m = magnitude8(u);
+        unpack8(u, t);
+      } else {
         load8<WIDE>(x + from * ld_x, i, k, t);
-        if constexpr (SILU) {
+        if constexpr (KIND == kSilu) {
           float u[8];
           load8<WIDE>(x + from * ld_x + k, i, k, u);
 #pragma unroll
           for (int e = 0; e < 8; ++e) t[e] = silu_f(t[e]) * u[e];
         }
+        m = magnitude8(t);
       }
     }
-    const float s = f8_scale(block_max(magnitude8(t)));
-    if (at < all) store8(q, scale, row, rows, i, ld, blocks, t, s, 1.f);
+    const uint2 w = f8_block(t, block_max(m), s);
+    if constexpr (KIND == kTo) {
+      if (is)
+        for (int j = 0; j < top; ++j) {
+          const int64_t to = list[row * top + j];
+          if (to >= 0 && to < rows) store8(q, scale, to, rows, i, ld, blocks, w, s);
+        }
+    } else {
+      if (is) store8(q, scale, row, rows, i, ld, blocks, w, s);
+    }
   }
 }
 
@@ -117,8 +135,9 @@ __global__ void __launch_bounds__(THREADS) norm_f8_kernel(uint8_t* __restrict__ 
   const float inv = __frsqrt_rn(tot / (float)dim + eps);
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const float s = f8_scale(block_max(magnitude8(t[j])));
-    store8(q, scale, row, rows, (threadIdx.x + j * THREADS) * 8, ld, blocks, t[j], s, inv);
+    float s;
+    const uint2 v = f8_block(t[j], block_max(magnitude8(t[j])), s);
+    store8(q, scale, row, rows, (threadIdx.x + j * THREADS) * 8, ld, blocks, v, s * inv);
   }
 }
 
@@ -165,45 +184,47 @@ __global__ void __launch_bounds__(1024) norm_f8_long_kernel(uint8_t* __restrict_
 #pragma unroll
       for (int e = 0; e < 8; ++e) t[e] *= g[e];
     }
-    const float s = f8_scale(block_max(magnitude8(t)));
-    store8(q, scale, row, rows, i, ld, blocks, t, s, inv);
+    float s;
+    const uint2 v = f8_block(t, block_max(magnitude8(t)), s);
+    store8(q, scale, row, rows, i, ld, blocks, v, s * inv);
   }
 }
 
+// a CTA to a row, or to as many as its threads hold, eight entries a thread
 template <bool WIDE>
 __global__ void __launch_bounds__(256) f8_dequant_kernel(float* __restrict__ out, const uint8_t* __restrict__ q, const float* __restrict__ scale, int64_t rows, int k,
                                                          int pieces) {
   pdl_wait();
   pdl_trigger();
-  const int64_t ld = f8_ld(k), all = rows * pieces;
-  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < all; at += (int64_t)gridDim.x * 256) {
-    const int64_t row = at / pieces;
-    const int i = (int)(at % pieces) * 8;
-    const uint2 w = *reinterpret_cast<const uint2*>(q + row * ld + i);
-    const float s = scale[(int64_t)(i / kF8Block) * rows + row];
-    const float4 a = f8_unpack4(w.x), b = f8_unpack4(w.y);
-    float* const o = out + row * k + i;
-    if constexpr (WIDE) {
-      *reinterpret_cast<float4*>(o) = make_float4(a.x * s, a.y * s, a.z * s, a.w * s);
-      if (i + 4 < k) *reinterpret_cast<float4*>(o + 4) = make_float4(b.x * s, b.y * s, b.z * s, b.w * s);
-    } else {
-      const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  const int64_t ld = f8_ld(k);
+  const int side_by_side = max(256 / pieces, 1), mine = (int)threadIdx.x / pieces, first = (int)threadIdx.x - mine * pieces;
+  for (int64_t row = (int64_t)blockIdx.x * side_by_side + mine; row < rows && mine < side_by_side; row += (int64_t)gridDim.x * side_by_side)
+    for (int i = first * 8; i < k; i += 2048) {
+      const uint2 w = *reinterpret_cast<const uint2*>(q + row * ld + i);
+      const float s = scale[(int64_t)(i / kF8Block) * rows + row];
+      const float4 a = f8_unpack4(w.x), b = f8_unpack4(w.y);
+      float* const o = out + row * k + i;
+      if constexpr (WIDE) {
+        *reinterpret_cast<float4*>(o) = make_float4(a.x * s, a.y * s, a.z * s, a.w * s);
+        if (i + 4 < k) *reinterpret_cast<float4*>(o + 4) = make_float4(b.x * s, b.y * s, b.z * s, b.w * s);
+      } else {
+        const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (i + e < k) o[e] = v[e] * s;
+        for (int e = 0; e < 8; ++e)
+          if (i + e < k) o[e] = v[e] * s;
+      }
     }
-  }
 }
 
 unsigned ctas_for(int64_t work, int64_t each, int64_t most) { return (unsigned)std::max<int64_t>(1, std::min((work + each - 1) / each, most)); }
 
-template <bool SILU>
-int launch_rows(void* q, float* scale, const void* x, int64_t ld_x, int64_t x_rows, const int32_t* index, int64_t rows, int64_t k, cudaStream_t st) {
-  const int blocks = (int)f8_blocks(k);
+template <RowsKind KIND>
+int launch_rows(void* q, float* scale, const void* x, int64_t ld_x, int64_t x_rows, const int32_t* list, int64_t top, int64_t rows, int64_t k, cudaStream_t st) {
+  const int64_t blocks = f8_blocks(k), all = KIND == kTo ? x_rows : rows;
   const bool wide = k % 8 == 0 && ld_x % 8 == 0 && aligned16(x);
-  const auto f = wide ? f8_rows_kernel<true, SILU> : f8_rows_kernel<false, SILU>;
-  B200_CUDA(launch_pdl(f, dim3(ctas_for(rows * blocks, 16, 148 * 8)), dim3(256), 0, st, op_pdl(st), (uint8_t*)q, scale, (const __nv_bfloat16*)x, ld_x, x_rows, index,
-                       rows, (int)k, blocks));
+  const auto f = wide ? f8_rows_kernel<true, KIND> : f8_rows_kernel<false, KIND>;
+  B200_CUDA(launch_pdl(f, dim3(ctas_for(all * blocks, 16, 148 * 64)), dim3(256), 0, st, op_pdl(st), (uint8_t*)q, scale,
+                       (const __nv_bfloat16*)x, ld_x, x_rows, list, (int)top, rows, (int)k, (int)blocks));
   return B200_OK;
 }
 
@@ -232,10 +253,13 @@ int check_rows(const char* what, const void* q, const void* scale, int64_t rows,
 }  // namespace
 
 int launch_f8_rows(void* q, float* scale, const void* x, int64_t ld_x, int64_t x_rows, const int32_t* index, int64_t rows, int64_t k, cudaStream_t st) {
-  return launch_rows<false>(q, scale, x, ld_x, x_rows, index, rows, k, st);
+  return launch_rows<kList>(q, scale, x, ld_x, x_rows, index, 0, rows, k, st);
+}
+int launch_f8_rows_to(void* q, float* scale, const void* x, const int32_t* place, int64_t rows, int64_t top, int64_t dest_rows, int64_t k, cudaStream_t st) {
+  return launch_rows<kTo>(q, scale, x, k, rows, place, top, dest_rows, k, st);
 }
 int launch_silu_mul_f8(void* q, float* scale, const void* gate_up, int64_t rows, int64_t n, cudaStream_t st) {
-  return launch_rows<true>(q, scale, gate_up, 2 * n, rows, nullptr, rows, n, st);
+  return launch_rows<kSilu>(q, scale, gate_up, 2 * n, rows, nullptr, 0, rows, n, st);
 }
 
 }  // namespace b200
@@ -281,7 +305,7 @@ int b200_f8_rows_dequant(float* out, const void* q, const float* scale, int64_t 
   const int pieces = (int)((k + 7) / 8);
   const cudaStream_t st = (cudaStream_t)stream;
   const auto f = k % 4 == 0 && aligned16(out) ? f8_dequant_kernel<true> : f8_dequant_kernel<false>;
-  B200_CUDA(launch_pdl(f, dim3(ctas_for(rows * pieces, 256, 148 * 16)), dim3(256), 0, st, op_pdl(st), out, (const uint8_t*)q, scale, rows, (int)k, pieces));
+  B200_CUDA(launch_pdl(f, dim3(ctas_for(rows, std::max(256 / pieces, 1), 148 * 32)), dim3(256), 0, st, op_pdl(st), out, (const uint8_t*)q, scale, rows, (int)k, pieces));
   return B200_OK;
 }
 

@@ -33,7 +33,7 @@ template <int NT>
 struct Form {
   static constexpr int per_sm = NT <= 64 ? 2 : 1;
   static constexpr int x_bytes = NT * 128, stage = kWBytes + x_bytes;
-  static constexpr int stages = NT <= 32 ? 5 : NT == 64 ? 3 : 5;
+  static constexpr int stages = NT == 16 ? 5 : NT == 64 ? 3 : 4;
   static constexpr int box = NT < 64 ? NT : 64;  // rows of x in a TMA box
   static constexpr int slots8 = 4;                     // of tensor memory, 8 bits
   static constexpr int lag = 3;                        // blocks that factors are asked for ahead
@@ -41,7 +41,8 @@ struct Form {
   static constexpr int f_slot = NT < 32 ? 32 : NT;
   static constexpr int cols = NT / 2;                  // rows of x of a summing warp
   static constexpr int ring = stages * stage;
-  static constexpr int tables = 1024 + ring + NT * kOutLd + ahead * f_slot * 4 + 512;
+  static constexpr int out_bytes = NT * kPartLd * 4;   // a finished tile in bf16, or what the CTAs of a cluster send of theirs in fp32
+  static constexpr int tables = 1024 + ring + out_bytes + ahead * f_slot * 4 + 512;
   static constexpr int smem(int experts) { return tables + Groups::bytes(experts); }
   static constexpr int tmem(int slots) { return slots * NT < 32 ? 32 : slots * NT; }
 };
@@ -99,7 +100,7 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* const sx = smem + ST * kWBytes;
   uint8_t* const done_tile = smem + F::ring;                                       // [NT][kOutLd]: bf16
-  float* const factors = reinterpret_cast<float*>(done_tile + NT * kOutLd);        // [AHEAD][NT]
+  float* const factors = reinterpret_cast<float*>(done_tile + F::out_bytes);       // [AHEAD][NT]
   uint64_t* const full = reinterpret_cast<uint64_t*>(factors + AHEAD * F::f_slot);   // [stages], a pair's first CTA's
   uint64_t* const empty = full + ST;
   uint64_t* const sums_full = empty + ST;                                          // [slots]
@@ -108,9 +109,10 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
   uint64_t* const out_empty = out_full + 1;
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(out_empty + 1);
   int* const gave_up = reinterpret_cast<int*>(tmem_slot + 1);
-  float* const w_scale = reinterpret_cast<float*>(gave_up + 1);                       // [AHEAD]
+  int* const gave_up_of = gave_up + 1;                                                // [splits]
+  float* const w_scale = reinterpret_cast<float*>(gave_up_of + kMaxSplits);                       // [AHEAD]
   Groups groups(reinterpret_cast<int*>(smem + F::tables - 1024), p.experts);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = uniform((int)threadIdx.x / 32), lane = threadIdx.x % 32;
   const int split = p.splits > 1 ? (int)cluster_rank() : 0;
   bool ok = true;
 
@@ -130,6 +132,7 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
     fence_mbar_init();
     *gave_up = 0;
   }
+  if (p.splits > 1) cluster_arrive_relaxed();
   if (warp == 1) tmem_alloc<1>(tmem_slot, TMEM);
   pdl_wait();
   pdl_trigger();
@@ -137,13 +140,15 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  const int64_t tiles = (int64_t)groups.ends[p.experts - 1] * p.ch_tiles;
-  const int64_t first = blockIdx.x / p.splits, step = p.splits > 1 ? tiles : gridDim.x;   // a cluster that splits k takes one tile
+  const uint32_t tmem = uniform(*tmem_slot);
+  const int tiles = groups.ends[p.experts - 1] * p.ch_tiles;
+  const int first = blockIdx.x / p.splits, step = p.splits > 1 ? max(tiles, 1) : (int)gridDim.x;   // a cluster that splits k takes one tile
   const int kb0 = (int)((int64_t)p.k_blocks * split / p.splits), kb1 = (int)((int64_t)p.k_blocks * (split + 1) / p.splits);
-  auto tile_at = [&](int64_t t) {
+  int group = 0;   // of this warp's last tile
+  auto tile_at = [&](int t) {
     int local, row_tiles;
-    const int e = groups.find(t, p.ch_tiles, local, row_tiles), count = groups.counts[e];
+    groups.walk(t, p.ch_tiles, group, local, row_tiles);
+    const int e = group, count = groups.counts[e];
     const int i = local % row_tiles, each = ((count + row_tiles - 1) / row_tiles + 15) / 16 * 16;   // alike, and none is empty
     return Tile{groups.froms[e] + (int64_t)i * each, min(each, count - i * each), local / row_tiles * kCh, e};
   };
@@ -154,12 +159,12 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
       if (lane == 0) {
         int s = 0;
         uint32_t ph = 1;
-        for (int64_t t = first; t < tiles && ok; t += step) {
+        for (int t = first; t < tiles && ok; t += step) {
           const Tile tile = tile_at(t);
           const int row0 = (int)tile.row0;
           const int boxes = (tile.rows + F::box - 1) / F::box, w_row = tile.expert * p.n + tile.ch0;
           for (int kb = kb0; kb < kb1; ++kb) {
-            if (!(ok = mbar_wait_limited(&empty[s], ph, p.err, kWaitCode | 1))) break;
+            if (!(ok = wait_asleep(&empty[s], ph, p.err, kWaitCode | 1))) break;
             uint8_t *const w_to = smem + s * kWBytes, *const x_to = sx + s * F::x_bytes;
             const int k0 = kb * (F8 ? 128 : 64);
             mbar_arrive_expect_tx(&full[s], kWBytes + boxes * F::box * 128);
@@ -174,52 +179,47 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
         if (!ok) drain_async();
       }
     } else if (warp == 1) {
-      if (elect_one()) {
-        const uint32_t w0 = desc_lo(smem_u32(smem)), x0 = desc_lo(smem_u32(sx));
-        int s = 0, slot = 0;
-        uint32_t ph = 0, slot_ph = 1;
-        bool ready = false;   // of the next stage, looked at before the products of this one go out
-        for (int64_t t = first; t < tiles && ok; t += step) {
-          const Tile tile = tile_at(t);
-          const uint32_t idesc = idesc_of(F8, kCh, up16(tile.rows));
-          for (int kb = kb0; kb < kb1; ++kb) {
-            if (F8 || kb == kb0) {
-              if (!(ok = mbar_wait_limited(&sums_empty[slot], slot_ph, p.err, kWaitCode | 2))) break;
-            }
-            if (!ready && !(ok = mbar_wait_limited(&full[s], ph, p.err, kWaitCode | 3))) break;
-            tc_fence_after();
-            const uint32_t w = w0 + s * (kWBytes >> 4), x = x0 + s * (F::x_bytes >> 4), d = tmem + slot * NT;
-            uint64_t* const done = &empty[s];
-            if (++s == ST) {
-              s = 0;
-              ph ^= 1;
-            }
-            ready = mbar_test(&full[s], ph);
+      const uint32_t w0 = desc_lo(smem_u32(smem)), x0 = desc_lo(smem_u32(sx)), lead = elect_one();
+      int s = 0, slot = 0;
+      uint32_t ph = 0, slot_ph = 1;
+      bool ready = false;   // the next stage and slot, looked at behind the products of this one
+      for (int t = first; t < tiles && ok; t += step) {
+        const uint32_t idesc = uniform(idesc_of(F8, kCh, up16(tile_at(t).rows)));
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!ready) {
+            if (!(ok = warp_wait(&sums_empty[slot], slot_ph, p.err, kWaitCode | 2))) break;
+            if (!(ok = warp_wait(&full[s], ph, p.err, kWaitCode | 3))) break;
+          }
+          tc_fence_after();
+          const uint32_t w = w0 + s * (kWBytes >> 4), x = x0 + s * (F::x_bytes >> 4), d = tmem + slot * NT;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              if constexpr (F8) umma_f8<1>(d, w + 2 * k, x + 2 * k, idesc, k > 0 ? 1u : 0u);
-              else umma_lo<1>(d, w + 2 * k, x + 2 * k, idesc, kb > kb0 || k > 0 ? 1u : 0u);
-            }
-            umma_commit(done);
-            if (F8 || kb == kb1 - 1) {
-              umma_commit(&sums_full[slot]);
-              if (++slot == SLOTS) {
-                slot = 0;
-                slot_ph ^= 1;
-              }
+          for (int k = 0; k < 4; ++k) umma_by<F8, 1>(lead, d, w + 2 * k, x + 2 * k, idesc, k > 0 || (!F8 && kb > kb0) ? 1u : 0u);
+          commit_by<1>(lead, &empty[s]);
+          if (F8 || kb == kb1 - 1) {
+            commit_by<1>(lead, &sums_full[slot]);
+            if (++slot == SLOTS) {
+              slot = 0;
+              slot_ph ^= 1;
             }
           }
+          if (++s == ST) {
+            s = 0;
+            ph ^= 1;
+          }
+          ready = mbar_test(&full[s], ph);
+          if (F8 || kb == kb1 - 1) ready = mbar_test(&sums_empty[slot], slot_ph) && ready;
+          ready = __all_sync(0xffffffffu, ready);
         }
-        if (!ok) drain_async();
       }
+      if (!ok) drain_async();
     } else if (warp == 2) {
       if constexpr (F8) {
         // Of unit u — a block of a tile — x's scales and W's are asked for LAG units before they are multiplied.  A slot's barrier takes unit u's arrival when its
         // phase before, unit u − SLOTS, is complete.  Then the products of that unit are done, so every warp has released unit u − 2·SLOTS and needs nothing of the units in
         // front of that one any more: a ring of 2·SLOTS + 1 + LAG units is never written where it is read.
         constexpr int PER = (NT + 31) / 32;
-        const int64_t units = first < tiles ? ((tiles - first + step - 1) / step) * (kb1 - kb0) : 0;
-        int64_t t = first;
+        const int64_t units = first < tiles ? (int64_t)((tiles - first + step - 1) / step) * (kb1 - kb0) : 0;
+        int t = first;
         int kb = kb0, into = 0, from_slot = 0, slot = 0;
         uint32_t ph = 1;
         Tile tile{};
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
     } else if (warp == 3) {
       if (p.splits == 1) {
         uint32_t ph = 0;
-        for (int64_t t = first; t < tiles; t += step, ph ^= 1) {
+        for (int t = first; t < tiles; t += step, ph ^= 1) {
           const Tile tile = tile_at(t);
           if (!(ok = warp_wait(out_full, ph, p.err, kWaitCode | 6))) break;
           store_tile(p.y + tile.row0 * p.n + tile.ch0, done_tile, kOutLd, tile.rows, min(kCh, p.n - tile.ch0), p, lane);
@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
     const uint32_t put_at = smem_u32(done_tile) + (half * COLS + lane % 8) * kOutLd + quad * 64 + lane / 8 * 16;
     int slot = 0, fslot = 0;
     uint32_t slot_ph = 0, out_ph = 1;
-    for (int64_t t = first; t < tiles; t += step, out_ph ^= 1) {
+    for (int t = first; t < tiles; t += step, out_ph ^= 1) {
       const Tile tile = tile_at(t);
       const int mine = tile.rows - half * COLS;   // rows of this half
       const int ch0 = tile.ch0 + quad * 32;
@@ -413,36 +413,42 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
   __syncwarp();
   __syncthreads();
   if (p.splits > 1) {
+    // Every row has an owner among the CTAs, which get their rows of everybody's partial tile (a warp a row, a lane four channels) and sum them in order.
+    // Reading them from the others instead took a round trip and a second meeting, 1.4 µs of 17.
+    const int owned = NT / p.splits;
+    group = 0;
+    const Tile tile = first < tiles ? tile_at(first) : Tile{0, 0, 0, 0};
+    cluster_wait();   // all CTAs have started
+    for (int row = warp; row < tile.rows; row += kThreads / 32) {
+      const int owner = row / owned;
+      const float4 v = *reinterpret_cast<const float4*>(smem + (row * kPartLd + 4 * lane) * 4);
+      st_cluster_f4(mapa_u32(smem_u32(done_tile), owner) + ((split * owned + row - owner * owned) * kPartLd + 4 * lane) * 4, v);
+    }
+    if (lane == 0) st_cluster_i32(mapa_u32(smem_u32(gave_up_of), warp % p.splits) + split * 4, *gave_up);
     cluster_sync_all();
-    // a warp takes a row of x, a lane four channels; the CTAs' sums in order
-    const bool lost = __any_sync(0xffffffffu, lane < p.splits && ld_cluster_i32(mapa_u32(smem_u32(gave_up), min(lane, p.splits - 1))) != 0);
-    if (first < tiles && !lost) {
-      const Tile tile = tile_at(first);
-      const int ch = tile.ch0 + 4 * lane;
-      float bias[4];
+    const bool lost = __any_sync(0xffffffffu, lane < p.splits && gave_up_of[lane] != 0);
+    const int ch = tile.ch0 + 4 * lane;
+    float bias[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) bias[j] = p.bias != nullptr && ch + j < p.n ? bf16_to_f(p.bias[ch + j]) : 0.f;
-      for (int row = split + p.splits * warp; row < tile.rows; row += p.splits * (kThreads / 32)) {
-        const uint32_t at = smem_u32(smem) + (row * kPartLd + 4 * lane) * 4;
-        float4 of[kMaxSplits];
+    for (int j = 0; j < 4; ++j) bias[j] = p.bias != nullptr && ch + j < p.n ? bf16_to_f(p.bias[ch + j]) : 0.f;
+    for (int i = warp; i < owned && !lost; i += kThreads / 32) {
+      const int row = split * owned + i;
+      if (row >= tile.rows) break;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int e = 0; e < p.splits; ++e) {
+        const float4 u = *reinterpret_cast<const float4*>(done_tile + ((e * owned + i) * kPartLd + 4 * lane) * 4);
+        v = e == 0 ? u : make_float4(v.x + u.x, v.y + u.y, v.z + u.z, v.w + u.w);
+      }
+      const float r[4] = {v.x + bias[0], v.y + bias[1], v.z + bias[2], v.w + bias[3]};
+      __nv_bfloat16* const out = p.y + (tile.row0 + row) * p.n + ch;
+      if (p.wide) {
+        if (ch < p.n) *reinterpret_cast<uint2*>(out) = make_uint2(pack2(r[0], r[1]), pack2(r[2], r[3]));
+      } else {
 #pragma unroll
-        for (int e = 0; e < kMaxSplits; ++e) of[e] = e < p.splits ? ld_cluster_f4(mapa_u32(at, e)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        float4 v = of[0];
-#pragma unroll
-        for (int e = 1; e < kMaxSplits; ++e) v = make_float4(v.x + of[e].x, v.y + of[e].y, v.z + of[e].z, v.w + of[e].w);
-        __nv_bfloat16* const out = p.y + (tile.row0 + row) * p.n + ch;
-        const float r[4] = {v.x + bias[0], v.y + bias[1], v.z + bias[2], v.w + bias[3]};
-        if (p.wide) {
-          if (ch < p.n) *reinterpret_cast<uint2*>(out) = make_uint2(pack2(r[0], r[1]), pack2(r[2], r[3]));
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (ch + j < p.n) out[j] = f_to_bf16(r[j]);
-        }
+        for (int j = 0; j < 4; ++j)
+          if (ch + j < p.n) out[j] = f_to_bf16(r[j]);
       }
     }
-    __syncthreads();
-    cluster_sync_all();   // nobody reads this CTA's sums any more
   }
   if (warp == 1) {
     tc_fence_after();

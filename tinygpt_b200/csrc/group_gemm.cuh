@@ -19,20 +19,44 @@ struct GemmArgs {
 int launch_group_wide(const GroupProduct& g, GemmArgs& p, cudaStream_t st);
 
 #ifdef __CUDACC__
-// D[tmem] (+)= A·B over 32 entries of 8 bits
+// D[tmem] (+)= A·B over 32 bytes of k, of 8-bit entries or bf16, where `lead`.  A whole warp comes here with the same operands and one of its lanes is the leading
+// one: they stay in uniform registers.  Issued by a lane in a branch of its own four products and their commit take 445 cycles, however few columns they
+// have, so 249 — a tile of 128 × 128 needs 256 — and the products of 128 × 256 are there 646 cycles after the first one's issue, for 801.
+template <bool F8, int GROUP>
+__device__ __forceinline__ void umma_by(uint32_t lead, uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+#define B200_UMMA(group, kind)                                                                                                                              \
+  asm volatile(                                                                                                                                             \
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"     \
+      "@q tcgen05.mma.cta_group::" group ".kind::" kind " [%0], a, b, %4, p;\n\t}" ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(kDescHi), "r"(idesc),          \
+      "r"(accumulate), "r"(lead)                                                                                                                            \
+      : "memory")
+  if constexpr (GROUP == 2) {
+    if constexpr (F8) B200_UMMA("2", "f8f6f4");
+    else B200_UMMA("2", "f16");
+  } else {
+    if constexpr (F8) B200_UMMA("1", "f8f6f4");
+    else B200_UMMA("1", "f16");
+  }
+#undef B200_UMMA
+}
+// the barrier at this offset — in both CTAs of a pair — hears when what the leading lane has issued is done
 template <int GROUP>
-__device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void commit_by(uint32_t lead, uint64_t* bar) {
   if constexpr (GROUP == 2)
     asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a, b, %4, p;\n\t}" ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(kDescHi), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(smem_u32(bar)),
+        "h"((uint16_t)3), "r"(lead)
         : "memory");
   else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %4, p;\n\t}" ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(kDescHi), "r"(idesc), "r"(accumulate)
-        : "memory");
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+                 "r"(lead)
+                 : "memory");
 }
+__device__ __forceinline__ void st_cluster_i32(uint32_t addr, int v) { asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+// what is the same in all lanes of a warp, where the compiler sees that it is
+template <typename T>
+__device__ __forceinline__ T uniform(T v) { return __shfl_sync(0xffffffffu, v, 0); }
 // kind::f8f6f4: D = F32 (bits 4-5 = 1), A = B = e4m3 (0), both K-major, N >> 3 at bits 17-22, M >> 4 at bits 24-28
 __device__ __forceinline__ uint32_t idesc_of(bool eight, int m, int n) {
   const uint32_t shape = ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24) | (1u << 4);
@@ -54,9 +78,28 @@ __device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t 
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-// a wait of a whole warp that mostly finds what it waits for
+// Waits as mbar_wait_limited does, but asleep: a thread that polls takes issue slots from the warps that sum.  False after about two seconds.
+__device__ __forceinline__ bool try_wait_asleep(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u) : "memory");   // ns, at most
+  return ok != 0;
+}
+__device__ __forceinline__ bool wait_asleep(uint64_t* bar, uint32_t parity, unsigned* err, unsigned code) {
+  if (try_wait_asleep(bar, parity)) return true;
+  const unsigned long long t0 = global_timer_ns();
+  while (!try_wait_asleep(bar, parity)) {
+    if (global_timer_ns() - t0 > 2000000000ull) {
+      *reinterpret_cast<volatile unsigned*>(err) = code;
+      __threadfence_system();
+      return false;
+    }
+  }
+  return true;
+}
+// of a whole warp
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsigned* err, unsigned code) {
-  return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || __all_sync(0xffffffffu, mbar_wait_limited(bar, parity, err, code));
+  return __all_sync(0xffffffffu, wait_asleep(bar, parity, err, code));
 }
 // Arrives in another CTA.  What it tells is that tensor memory was read (the fence in front); no memory is handed over, so that no release at the cluster's
 // scope is needed, which takes some 700 cycles.
@@ -116,19 +159,22 @@ struct Groups {
       ends[e] = upto;
     }
   }
-  // the group whose row tiles times ch_tiles tile t is one of; local: its number there, row_tiles: how many row tiles the group has
-  __device__ __forceinline__ int find(int64_t t, int ch_tiles, int& local, int& row_tiles) const {
-    const int at = (int)(t / ch_tiles);   // ends[e − 1] ≤ at < ends[e]
-    int lo = 0, hi = experts - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (ends[mid] > at) hi = mid;
-      else lo = mid + 1;
+  // The group e that tile t is one of — its row tiles times ch_tiles tiles — from the group of a tile in front of it; local: its number there, row_tiles: how many
+  // row tiles the group has.  (A call has fewer than 2^31 tiles.)
+  __device__ __forceinline__ void walk(int t, int ch_tiles, int& e, int& local, int& row_tiles) const {
+    const int at = t / ch_tiles;
+    if (ends[e] <= at) {   // ends[e − 1] ≤ at < ends[e]
+      int lo = min(e + 1, experts - 1), hi = experts - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (ends[mid] > at) hi = mid;
+        else lo = mid + 1;
+      }
+      e = lo;
     }
-    const int before = lo > 0 ? ends[lo - 1] : 0;
-    row_tiles = ends[lo] - before;
-    local = (int)(t - (int64_t)before * ch_tiles);
-    return lo;
+    const int before = e > 0 ? ends[e - 1] : 0;
+    row_tiles = ends[e] - before;
+    local = t - before * ch_tiles;
   }
 };
 // rows in front of the first group and behind the last, by one warp of every CTA

@@ -13,19 +13,28 @@ namespace b200 {
 
 namespace {
 
-constexpr int kTile = 256, kHalf = 128;           // rows and channels of a pair, of a CTA's operands
-constexpr int kOperand = kHalf * 128;             // bytes of a stage
-constexpr int kStages = 4, kSlots = 2, kThreads = 384, kEpiWarps = 8;
-constexpr int kLag = 3, kAhead = 2 * kSlots + 1 + kLag;   // blocks of factors, asked for and kept: see group_gemm.cu
-constexpr int kOutLd = kTile * 2 + 16;            // bytes from row to row of a finished tile: eight rows meet all banks
-constexpr int kRing = kStages * 2 * kOperand;
-constexpr int kTables = 1024 + kRing + kHalf * kOutLd + kAhead * kTile * 4 + 512;
-constexpr int kTmem = kSlots * kTile;
+constexpr int kRows = 128;                        // of a CTA
+constexpr int kXBytes = kRows * 128;              // of a stage
+constexpr int kThreads = 384, kEpiWarps = 8;
 constexpr unsigned kWaitCode = 0x68000000u;
+constexpr int CH = 256, COLS = CH / 2, BLOCKS = CH / 128;   // channels of a tile, of a summing warp; blocks that share a scale of W
+constexpr int SLOTS = 512 / CH;
+constexpr int kOutLd = CH * 2 + 16;               // bytes from row to row of a finished tile: eight rows meet all banks
+// GROUP CTAs to a tile of GROUP·128 rows × 256 channels
+template <int GROUP>
+struct Wide {
+  static constexpr int w_rows = CH / GROUP, w_bytes = w_rows * 128, stage = kXBytes + w_bytes;
+  static constexpr int stages = GROUP == 2 ? 4 : 3;
+  static constexpr int lag = 4, ahead = 2 * SLOTS + 1 + lag;   // blocks of factors that are asked for ahead, and kept: see group_gemm.cu
+  static constexpr int ring = stages * stage;
+  static constexpr int tables = 1024 + ring + kRows * kOutLd + ahead * BLOCKS * kRows * 4 + 512;
+  static constexpr int smem(int experts) { return tables + Groups::bytes(experts); }
+  static constexpr int fit = (227 * 1024 - tables) / Groups::bytes(1), most_experts = fit < kMaxExperts ? fit : kMaxExperts;
+};
 // A thread that sums 8-bit products holds 128 sums: the four warps that hold none give registers up.
-constexpr int kRegsFew = 56, kRegsMany = 224, kRegsLaunch = 168;
+constexpr int kRegsFew = 72, kRegsMany = 216, kRegsLaunch = 168;
 static_assert(128 * kRegsFew + 256 * kRegsMany <= kThreads * kRegsLaunch, "no warp waits for registers that the launch does not have");
-static_assert(kTables + Groups::bytes(kMaxExperts) <= 227 * 1024, "room");
+static_assert(Wide<2>::most_experts == kMaxExperts && Wide<1>::most_experts >= 128, "room");
 
 #define B200_R8(b) "+r"(r[b]), "+r"(r[b + 1]), "+r"(r[b + 2]), "+r"(r[b + 3]), "+r"(r[b + 4]), "+r"(r[b + 5]), "+r"(r[b + 6]), "+r"(r[b + 7])
 // the wait for what tmem_ld32 has loaded holds it: nothing that uses it moves in front of the wait
@@ -34,64 +43,66 @@ __device__ __forceinline__ void loaded(uint32_t (&r)[32]) {
   asm volatile("" : B200_R8(16), B200_R8(24));
 }
 
-template <bool F8>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+template <bool F8, int GROUP>
+__global__ void __launch_bounds__(kThreads, 1)
 group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const GemmArgs p) {
+  using F = Wide<GROUP>;
+  constexpr int ST = F::stages, AHEAD = F::ahead, F_SLOT = BLOCKS * kRows;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* const sx = smem;                                                        // [stages][128 rows × 128 bytes]
-  uint8_t* const sw = smem + kStages * kOperand;                                   // the same of W
-  uint8_t* const done_tile = smem + kRing;                                         // [128][kOutLd]: bf16
-  float* const factors = reinterpret_cast<float*>(done_tile + kHalf * kOutLd);     // [kAhead][2][128]: of a block of channels, of a row
-  uint64_t* const full = reinterpret_cast<uint64_t*>(factors + kAhead * kTile);    // [stages], CTA 0's count the pair's bytes
-  uint64_t* const empty = full + kStages;
-  uint64_t* const sums_full = empty + kStages;                                     // [slots]
-  uint64_t* const sums_empty = sums_full + kSlots;                                 // CTA 0's
-  uint64_t* const out_full = sums_empty + kSlots;
+  uint8_t* const sw = smem + ST * kXBytes;                                         // this CTA's rows of W alike
+  uint8_t* const done_tile = smem + F::ring;                                       // [128][out_ld]: bf16
+  float* const factors = reinterpret_cast<float*>(done_tile + kRows * kOutLd);  // [AHEAD][blocks][128]: of a block of channels, of a row
+  uint64_t* const full = reinterpret_cast<uint64_t*>(factors + AHEAD * F_SLOT);    // [stages], CTA 0's count the pair's bytes
+  uint64_t* const empty = full + ST;
+  uint64_t* const sums_full = empty + ST;                                          // [slots]
+  uint64_t* const sums_empty = sums_full + SLOTS;                                  // CTA 0's
+  uint64_t* const out_full = sums_empty + SLOTS;
   uint64_t* const out_empty = out_full + 1;
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(out_empty + 1);
-  float* const w_scale = reinterpret_cast<float*>(tmem_slot + 1);                  // [kAhead][2]
-  Groups groups(reinterpret_cast<int*>(smem + kTables - 1024), p.experts);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int rank = (int)cluster_rank();
+  float* const w_scale = reinterpret_cast<float*>(tmem_slot + 1);                  // [AHEAD][blocks]
+  Groups groups(reinterpret_cast<int*>(smem + F::tables - 1024), p.experts);
+  const int warp = uniform((int)threadIdx.x / 32), lane = threadIdx.x % 32;
+  const int rank = GROUP == 2 ? (int)cluster_rank() : 0;
   bool ok = true;
 
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tmap_w);
     tma_prefetch_desc(&tmap_x);
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < ST; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int a = 0; a < kSlots; ++a) {
+    for (int a = 0; a < SLOTS; ++a) {
       mbar_init(&sums_full[a], F8 ? 2 : 1);   // products done, factors there
-      mbar_init(&sums_empty[a], 2 * kEpiWarps);
+      mbar_init(&sums_empty[a], GROUP * kEpiWarps);
     }
     mbar_init(out_full, kEpiWarps);
     mbar_init(out_empty, 1);
     fence_mbar_init();
   }
-  if (warp == 1) tmem_alloc<2>(tmem_slot, kTmem);
+  if (warp == 1) tmem_alloc<GROUP>(tmem_slot, 512);
   pdl_wait();
   pdl_trigger();
-  if (warp == 3) groups.make<kTile>(p.starts, p.rows, lane);
+  if (warp == 3) groups.make<GROUP * kRows>(p.starts, p.rows, lane);
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();   // the pair's barriers exist
+  if constexpr (GROUP == 2) cluster_sync_all();   // the pair's barriers exist
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  const int64_t tiles = (int64_t)groups.ends[p.experts - 1] * p.ch_tiles;
-  const int64_t first = blockIdx.x / 2, step = gridDim.x / 2;
+  const uint32_t tmem = uniform(*tmem_slot);
+  const int tiles = groups.ends[p.experts - 1] * p.ch_tiles, first = blockIdx.x / GROUP, step = gridDim.x / GROUP;
   const int k_blocks = p.k_blocks;
   struct Tile {
     int64_t row0;             // of this CTA
     int rows, ch0, expert;    // rows of this CTA: none where the tile ends in the pair's first half
   };
-  auto tile_at = [&](int64_t t) {   // a group's row tiles first: its rows of W stay in L2
+  int e = 0;                  // the group of this warp's last tile
+  auto tile_at = [&](int t) {   // a group's row tiles first: its rows of W stay in L2
     int local, row_tiles;
-    const int e = groups.find(t, p.ch_tiles, local, row_tiles);
-    const int row = local % row_tiles * kTile + rank * kHalf;
-    return Tile{(int64_t)groups.froms[e] + row, max(0, min(kHalf, groups.counts[e] - row)), local / row_tiles * kTile, e};
+    groups.walk(t, p.ch_tiles, e, local, row_tiles);
+    const int row = local % row_tiles * (GROUP * kRows) + rank * kRows;
+    return Tile{(int64_t)groups.froms[e] + row, max(0, min(kRows, groups.counts[e] - row)), local / row_tiles * CH, e};
   };
 
   if (warp < 4) {
@@ -100,17 +111,23 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
       if (lane == 0) {
         int s = 0;
         uint32_t ph = 1;
-        for (int64_t t = first; t < tiles && ok; t += step) {
+        for (int t = first; t < tiles && ok; t += step) {
           const Tile tile = tile_at(t);
-          const int x_row = (int)tile.row0, w_row = tile.expert * p.n + tile.ch0 + rank * kHalf;   // (what lies past the operands is zero)
+          const int x_row = (int)tile.row0, w_row = tile.expert * p.n + tile.ch0 + rank * F::w_rows;   // (what lies past the operands is zero)
           for (int kb = 0; kb < k_blocks; ++kb) {
-            if (!(ok = mbar_wait_limited(&empty[s], ph, p.err, kWaitCode | 1))) break;
+            if (!(ok = wait_asleep(&empty[s], ph, p.err, kWaitCode | 1))) break;
             const int k0 = kb * (F8 ? 128 : 64);
-            const uint32_t bar = mapa_u32(smem_u32(&full[s]), 0);
-            if (rank == 0) mbar_arrive_expect_tx(&full[s], 4 * kOperand);
-            tma_load_2d_pair(sx + s * kOperand, &tmap_x, k0, x_row, bar);
-            tma_load_2d_pair(sw + s * kOperand, &tmap_w, k0, w_row, bar);
-            if (++s == kStages) {
+            if constexpr (GROUP == 2) {
+              const uint32_t bar = mapa_u32(smem_u32(&full[s]), 0);
+              if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * F::stage);
+              tma_load_2d_pair(sx + s * kXBytes, &tmap_x, k0, x_row, bar);
+              tma_load_2d_pair(sw + s * F::w_bytes, &tmap_w, k0, w_row, bar);
+            } else {
+              mbar_arrive_expect_tx(&full[s], F::stage);
+              tma_load_2d(sx + s * kXBytes, &tmap_x, k0, x_row, &full[s]);
+              tma_load_2d(sw + s * F::w_bytes, &tmap_w, k0, w_row, &full[s]);
+            }
+            if (++s == ST) {
               s = 0;
               ph ^= 1;
             }
@@ -119,83 +136,77 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         if (!ok) drain_async();
       }
     } else if (warp == 1) {
-      if (rank == 0 && elect_one()) {
-        const uint32_t x0 = desc_lo(smem_u32(sx)), w0 = desc_lo(smem_u32(sw)), idesc = idesc_of(F8, kTile, kTile);
+      if (GROUP == 1 || rank == 0) {
+        const uint32_t x0 = desc_lo(smem_u32(sx)), w0 = desc_lo(smem_u32(sw)), idesc = idesc_of(F8, GROUP * kRows, CH), lead = elect_one();
         int s = 0, slot = 0;
         uint32_t ph = 0, slot_ph = 1;
-        bool ready = false;   // of the next stage, looked at before the products of this one go out
-        for (int64_t t = first; t < tiles && ok; t += step) {
+        bool ready = false;   // the next stage, looked at behind the products of this one
+        for (int t = first; t < tiles && ok; t += step) {
           for (int kb = 0; kb < k_blocks; ++kb) {
-            if (F8 || kb == 0) {
-              if (!(ok = mbar_wait_limited(&sums_empty[slot], slot_ph, p.err, kWaitCode | 2))) break;
-            }
-            if (!ready && !(ok = mbar_wait_limited(&full[s], ph, p.err, kWaitCode | 3))) break;
+            if ((F8 || kb == 0) && !(ok = warp_wait(&sums_empty[slot], slot_ph, p.err, kWaitCode | 2))) break;
+            if (!ready && !(ok = warp_wait(&full[s], ph, p.err, kWaitCode | 3))) break;
             tc_fence_after();
-            const uint32_t x = x0 + s * (kOperand >> 4), w = w0 + s * (kOperand >> 4), d = tmem + slot * kTile;
-            uint64_t* const done = &empty[s];
-            if (++s == kStages) {
-              s = 0;
-              ph ^= 1;
-            }
-            ready = mbar_test(&full[s], ph);
+            const uint32_t x = x0 + s * (kXBytes >> 4), w = w0 + s * (F::w_bytes >> 4), d = tmem + slot * CH;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              if constexpr (F8) umma_f8<2>(d, x + 2 * k, w + 2 * k, idesc, k > 0 ? 1u : 0u);
-              else umma_lo<2>(d, x + 2 * k, w + 2 * k, idesc, kb > 0 || k > 0 ? 1u : 0u);
-            }
-            umma_commit_pair(done);
+            for (int k = 0; k < 4; ++k) umma_by<F8, GROUP>(lead, d, x + 2 * k, w + 2 * k, idesc, k > 0 || (!F8 && kb > 0) ? 1u : 0u);
+            commit_by<GROUP>(lead, &empty[s]);
             if (F8 || kb == k_blocks - 1) {
-              umma_commit_pair(&sums_full[slot]);
-              if (++slot == kSlots) {
+              commit_by<GROUP>(lead, &sums_full[slot]);
+              if (++slot == SLOTS) {
                 slot = 0;
                 slot_ph ^= 1;
               }
             }
+            if (++s == ST) {
+              s = 0;
+              ph ^= 1;
+            }
+            ready = __all_sync(0xffffffffu, mbar_test(&full[s], ph));
           }
         }
         if (!ok) drain_async();
       }
     } else if (warp == 2) {
       if constexpr (F8) {   // as in group_gemm.cu, which says why the ring is never written where it is read
-        const int64_t units = first < tiles ? ((tiles - first + step - 1) / step) * k_blocks : 0;
-        int64_t t = first;
+        const int64_t units = first < tiles ? (int64_t)((tiles - first + step - 1) / step) * k_blocks : 0;
+        int t = first;
         int kb = 0, into = 0, from_slot = 0, slot = 0;
         uint32_t ph = 1;
         Tile tile{};
         auto ask = [&]() {
           if (kb == 0) tile = tile_at(t);
           const float* const from = p.sx + (int64_t)kb * p.rows + tile.row0 + lane;
-          float* const to = factors + into * kTile + lane;
+          float* const to = factors + into * F_SLOT + lane;
 #pragma unroll
-          for (int i = 0; i < kHalf / 32; ++i)
+          for (int i = 0; i < kRows / 32; ++i)
             if (lane + 32 * i < tile.rows) cp_async4(to + 32 * i, from + 32 * i);
-          if (lane < 2)
-            cp_async4(&w_scale[2 * into + lane], p.sw + ((int64_t)tile.expert * p.ch_blocks + min(tile.ch0 / kHalf + lane, p.ch_blocks - 1)) * k_blocks + kb);
+          if (lane < BLOCKS)
+            cp_async4(&w_scale[BLOCKS * into + lane], p.sw + ((int64_t)tile.expert * p.ch_blocks + min(tile.ch0 / 128 + lane, p.ch_blocks - 1)) * k_blocks + kb);
           if (++kb == k_blocks) {
             kb = 0;
             t += step;
           }
-          if (++into == kAhead) into = 0;
+          if (++into == AHEAD) into = 0;
         };
-        for (int64_t u = -kLag; u < units; ++u) {
+        for (int64_t u = -F::lag; u < units; ++u) {
           if (u >= 0 && !(ok = warp_wait(&sums_full[slot], ph, p.err, kWaitCode | 4))) break;
-          if (u + kLag < units) ask();
+          if (u + F::lag < units) ask();
           cp_async_commit();
           if (u >= 0) {
-            cp_async_wait<kLag>();
+            cp_async_wait<F::lag>();
             __syncwarp();
-            const float w_lo = w_scale[2 * from_slot], w_hi = w_scale[2 * from_slot + 1];
-            float* const at = factors + from_slot * kTile + lane;
+            const float w_lo = w_scale[BLOCKS * from_slot], w_hi = w_scale[BLOCKS * from_slot + 1];
+            float* const at = factors + from_slot * F_SLOT + lane;
 #pragma unroll
-            for (int i = 0; i < kHalf / 32; ++i) {   // (places behind the tile's rows hold anything: nobody stores what they scale)
+            for (int i = 0; i < kRows / 32; ++i) {   // (places behind the tile's rows hold anything: nobody stores what they scale)
               const float v = at[32 * i];
               at[32 * i] = v * w_lo;
-              at[kHalf + 32 * i] = v * w_hi;
+              at[kRows + 32 * i] = v * w_hi;
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&sums_full[slot]);
-            if (++from_slot == kAhead) from_slot = 0;
-            if (++slot == kSlots) {
+            if (++from_slot == AHEAD) from_slot = 0;
+            if (++slot == SLOTS) {
               slot = 0;
               ph ^= 1;
             }
@@ -205,10 +216,10 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
       }
     } else {
       uint32_t ph = 0;
-      for (int64_t t = first; t < tiles; t += step, ph ^= 1) {
+      for (int t = first; t < tiles; t += step, ph ^= 1) {
         const Tile tile = tile_at(t);
         if (!(ok = warp_wait(out_full, ph, p.err, kWaitCode | 6))) break;
-        store_tile(p.y + tile.row0 * p.n + tile.ch0, done_tile, kOutLd, tile.rows, min(kTile, p.n - tile.ch0), p, lane);
+        store_tile(p.y + tile.row0 * p.n + tile.ch0, done_tile, kOutLd, tile.rows, min(CH, p.n - tile.ch0), p, lane);
         if (lane == 0) mbar_arrive(out_empty);
       }
       bulk_wait();
@@ -217,18 +228,22 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
   } else {
     if constexpr (F8) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsMany));
     const int quad = warp & 3, half = (warp - 4) >> 2, row = quad * 32 + lane;
-    const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + half * kHalf, free_bar = mapa_u32(smem_u32(sums_empty), 0);
-    uint8_t* const put_at = done_tile + row * kOutLd + half * kHalf * 2;
+    const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + half * COLS, free_bar = GROUP == 2 ? mapa_u32(smem_u32(sums_empty), 0) : 0;
+    uint8_t* const put_at = done_tile + row * kOutLd + half * COLS * 2;
+    const float* const my_factors = factors + half * kRows + row;
     int slot = 0, fslot = 0;
     uint32_t slot_ph = 0, out_ph = 1;
-    for (int64_t t = first; t < tiles; t += step, out_ph ^= 1) {
+    for (int t = first; t < tiles; t += step, out_ph ^= 1) {
       const Tile tile = tile_at(t);
       const bool mine = quad * 32 < tile.rows;   // some row of this warp is one
       auto release = [&]() {   // the slot may be filled again
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) arrive_at(free_bar + slot * 8);
-        if (++slot == kSlots) {
+        if (lane == 0) {
+          if (GROUP == 1 || rank == 0) mbar_arrive(&sums_empty[slot]);
+          else arrive_at(free_bar + slot * 8);
+        }
+        if (++slot == SLOTS) {
           slot = 0;
           slot_ph ^= 1;
         }
@@ -238,24 +253,24 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         *reinterpret_cast<uint4*>(put_at + 16 * j) = make_uint4(pack2(a.x, a.y), pack2(b.x, b.y), pack2(c.x, c.y), pack2(d.x, d.y));
       };
       auto bias_of = [&](int j) {   // of channels 2j, 2j + 1
-        const int ch = tile.ch0 + half * kHalf + 2 * j;
+        const int ch = tile.ch0 + half * COLS + 2 * j;
         return make_float2(ch < p.n ? bf16_to_f(p.bias[ch]) : 0.f, ch + 1 < p.n ? bf16_to_f(p.bias[ch + 1]) : 0.f);
       };
       if constexpr (F8) {
-        constexpr int PIECES = kHalf / 32;
-        uint64_t acc[kHalf / 2];
+        constexpr int PIECES = COLS / 32;
+        uint64_t acc[COLS / 2];
 #pragma unroll
-        for (int j = 0; j < kHalf / 2; ++j) acc[j] = 0;
-        uint32_t d[2][32];
-        if (!(ok = warp_wait(&sums_full[slot], slot_ph, p.err, kWaitCode | 5))) break;
-        tc_fence_after();
+        for (int j = 0; j < COLS / 2; ++j) acc[j] = 0;
         if (mine) {
           // One load is always on its way while another's sums are added, the next unit's first one too where its products are done by then.
-          tmem_ld32(from + slot * kTile, d[0]);
+          uint32_t d[2][32];
+          if (!(ok = warp_wait(&sums_full[slot], slot_ph, p.err, kWaitCode | 5))) break;
+          tc_fence_after();
+          tmem_ld32(from + slot * CH, d[0]);
           for (int kb = 0; kb < k_blocks; ++kb) {
-            const float f = factors[fslot * kTile + half * kHalf + row];
+            const float f = my_factors[fslot * F_SLOT];
             const uint64_t ff = pair_of(f, f);
-            const uint32_t at = from + slot * kTile;
+            const uint32_t at = from + slot * CH;
             bool next = false;
 #pragma unroll
             for (int i = 0; i < PIECES; ++i) {
@@ -267,37 +282,37 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
                 next = kb + 1 < k_blocks && __all_sync(0xffffffffu, mbar_test(&sums_full[slot], slot_ph));
                 if (next) {
                   tc_fence_after();
-                  tmem_ld32(from + slot * kTile, d[0]);
+                  tmem_ld32(from + slot * CH, d[0]);
                 }
               }
 #pragma unroll
               for (int j = 0; j < 16; ++j) acc[16 * i + j] = fma_pair(pair_of(d[i % 2][2 * j], d[i % 2][2 * j + 1]), ff, acc[16 * i + j]);
             }
-            if (++fslot == kAhead) fslot = 0;
+            if (++fslot == AHEAD) fslot = 0;
             if (!next && kb + 1 < k_blocks) {
               if (!(ok = warp_wait(&sums_full[slot], slot_ph, p.err, kWaitCode | 5))) break;
               tc_fence_after();
-              tmem_ld32(from + slot * kTile, d[0]);
+              tmem_ld32(from + slot * CH, d[0]);
             }
           }
         } else {
           for (int kb = 0; kb < k_blocks; ++kb) {
+            if (!(ok = warp_wait(&sums_full[slot], slot_ph, p.err, kWaitCode | 5))) break;
             release();
-            if (++fslot == kAhead) fslot = 0;
-            if (kb + 1 < k_blocks && !(ok = warp_wait(&sums_full[slot], slot_ph, p.err, kWaitCode | 5))) break;
+            if (++fslot == AHEAD) fslot = 0;
           }
         }
         if (!ok || !(ok = warp_wait(out_empty, out_ph, p.err, kWaitCode | 7))) break;
         if (mine) {
           if (p.bias != nullptr) {
 #pragma unroll
-            for (int j = 0; j < kHalf / 2; ++j) {
+            for (int j = 0; j < COLS / 2; ++j) {
               const float2 v = halves(acc[j]), b = bias_of(j);
               acc[j] = pair_of(v.x + b.x, v.y + b.y);
             }
           }
 #pragma unroll
-          for (int j = 0; j < kHalf / 8; ++j) put8(j, halves(acc[4 * j]), halves(acc[4 * j + 1]), halves(acc[4 * j + 2]), halves(acc[4 * j + 3]));
+          for (int j = 0; j < COLS / 8; ++j) put8(j, halves(acc[4 * j]), halves(acc[4 * j + 1]), halves(acc[4 * j + 2]), halves(acc[4 * j + 3]));
         }
       } else {
         if (!(ok = warp_wait(&sums_full[slot], slot_ph, p.err, kWaitCode | 5))) break;
@@ -305,9 +320,9 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         if (!(ok = warp_wait(out_empty, out_ph, p.err, kWaitCode | 7))) break;
         if (mine) {
 #pragma unroll 1
-          for (int i = 0; i < kHalf / 32; ++i) {
+          for (int i = 0; i < COLS / 32; ++i) {
             uint32_t d[32];
-            tmem_ld32(from + slot * kTile + 32 * i, d);
+            tmem_ld32(from + slot * CH + 32 * i, d);
             loaded(d);
             auto two = [&](int j) {
               float2 v = make_float2(__uint_as_float(d[2 * j]), __uint_as_float(d[2 * j + 1]));
@@ -331,45 +346,62 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
   tc_fence_before();
   __syncwarp();
   __syncthreads();
-  cluster_sync_all();   // neither CTA still reads the pair's operands, barriers or sums
+  if constexpr (GROUP == 2) cluster_sync_all();   // neither CTA still reads the pair's operands, barriers or sums
   if (warp == 1) {
     tc_fence_after();
-    tmem_free<2>(tmem, kTmem);
+    tmem_free<GROUP>(tmem, 512);
   }
-  cluster_sync_all();
+  if constexpr (GROUP == 2) cluster_sync_all();
 }
 
-template <bool F8>
+template <bool F8, int GROUP>
 int launch(const GroupProduct& g, GemmArgs& p, cudaStream_t st) {
+  using F = Wide<GROUP>;
   static PerDevice attrs;
   B200_CUDA(attrs([] {
     cudaFuncAttributes a{};
-    const cudaError_t e = cudaFuncGetAttributes(&a, group_wide_kernel<F8>);
+    const cudaError_t e = cudaFuncGetAttributes(&a, group_wide_kernel<F8, GROUP>);
     if (e != cudaSuccess) return e;
     if (F8 && a.numRegs != kRegsLaunch) return cudaErrorInvalidDeviceFunction;   // (the shares would not add up)
-    return cudaFuncSetAttribute(group_wide_kernel<F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTables + Groups::bytes(kMaxExperts));
+    return cudaFuncSetAttribute(group_wide_kernel<F8, GROUP>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::smem(F::most_experts));
   }));
   CUtensorMap tw, tx;
   int rc;
   if constexpr (F8) {
-    if ((rc = make_tmap_sw128_u8(&tw, g.w, g.experts * g.n, g.k, f8_ld(g.k), kHalf)) != B200_OK) return rc;
-    if ((rc = make_tmap_sw128_u8(&tx, g.x, g.rows, g.k, f8_ld(g.k), kHalf)) != B200_OK) return rc;
+    if ((rc = make_tmap_sw128_u8(&tw, g.w, g.experts * g.n, g.k, f8_ld(g.k), F::w_rows)) != B200_OK) return rc;
+    if ((rc = make_tmap_sw128_u8(&tx, g.x, g.rows, g.k, f8_ld(g.k), kRows)) != B200_OK) return rc;
   } else {
-    if ((rc = make_tmap_sw128(&tw, 2, g.w, 1, g.experts * g.n, g.k, 0, g.k, kHalf)) != B200_OK) return rc;
-    if ((rc = make_tmap_sw128(&tx, 2, g.x, 1, g.rows, g.k, 0, g.k, kHalf)) != B200_OK) return rc;
+    if ((rc = make_tmap_sw128(&tw, 2, g.w, 1, g.experts * g.n, g.k, 0, g.k, F::w_rows)) != B200_OK) return rc;
+    if ((rc = make_tmap_sw128(&tx, 2, g.x, 1, g.rows, g.k, 0, g.k, kRows)) != B200_OK) return rc;
   }
-  p.ch_blocks = (int)((g.n + kHalf - 1) / kHalf);
-  p.ch_tiles = (p.ch_blocks + 1) / 2;
+  p.ch_blocks = (int)((g.n + 127) / 128);
+  p.ch_tiles = (int)((g.n + CH - 1) / CH);
   p.splits = 1;
   // tiles that there can be: every group's last one may be short
-  const int64_t row_tiles = g.starts ? g.rows / kTile + std::min<int64_t>(g.experts, g.rows) : (g.rows + kTile - 1) / kTile;
-  const int64_t pairs = std::min<int64_t>(row_tiles * p.ch_tiles, 74);
-  B200_CUDA(launch_pdl(group_wide_kernel<F8>, dim3((unsigned)(2 * pairs)), dim3(kThreads), (size_t)(kTables + Groups::bytes((int)g.experts)), st, op_pdl(st), tw, tx, p));
+  constexpr int kTileRows = GROUP * kRows;
+  const int64_t row_tiles = g.starts ? g.rows / kTileRows + std::min<int64_t>(g.experts, g.rows) : (g.rows + kTileRows - 1) / kTileRows;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(GROUP * std::min<int64_t>(row_tiles * p.ch_tiles, 148 / GROUP)));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = F::smem((int)g.experts);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = GROUP;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = op_pdl(st) ? 1 : 0;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  B200_CUDA(cudaLaunchKernelEx(&cfg, group_wide_kernel<F8, GROUP>, tw, tx, (const GemmArgs)p));
   return B200_OK;
 }
 
 }  // namespace
 
-int launch_group_wide(const GroupProduct& g, GemmArgs& p, cudaStream_t st) { return g.x_scale != nullptr ? launch<true>(g, p, st) : launch<false>(g, p, st); }
+int launch_group_wide(const GroupProduct& g, GemmArgs& p, cudaStream_t st) {
+  return g.x_scale == nullptr ? launch<false, 2>(g, p, st) : g.experts <= Wide<1>::most_experts ? launch<true, 1>(g, p, st) : launch<true, 2>(g, p, st);
+}
 
 }  // namespace b200
