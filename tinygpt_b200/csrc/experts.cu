@@ -9,52 +9,60 @@ namespace b200 {
 namespace {
 
 // A stable counting sort in one CTA: every warp takes a run of the pairs, 32 at a time in their order.  Lanes that hold the same expert find each other
-// (match), so a warp's count of an expert is its own and no atomics decide an order.
+// (ballots of its bits), so a warp's count of an expert is its own and no atomics decide an order.
 //   1. counts[warp][e];  2. the sum in front of each: experts first, then warps;  3. the runs again, each pair to its place
-constexpr int kOrderWarps = 32, kOrderAhead = 8;
+// Bound by latencies, all of one SM.
+constexpr int kOrderWarps = 32, kOrderThreads = 32 * kOrderWarps;
+constexpr int kOrderKept = 16384;   // choices that are kept in shared memory, the others are read twice
 
-__global__ void __launch_bounds__(32 * kOrderWarps) expert_order_kernel(int32_t* __restrict__ starts, int32_t* __restrict__ source, int32_t* __restrict__ place,
-                                                                        const int32_t* __restrict__ chosen, int pairs, int top, int experts) {
-  extern __shared__ int counts[];                    // [warps][experts]
-  int* const total = counts + kOrderWarps * experts;   // [experts]: rows of all experts up to and with e
+__global__ void __launch_bounds__(kOrderThreads) expert_order_kernel(int32_t* __restrict__ starts, int32_t* __restrict__ source, int32_t* __restrict__ place,
+                                                                     const int32_t* __restrict__ chosen, int pairs, int top, int experts) {
+  extern __shared__ int counts[];   // [warps][ld]
+  const int ld = experts | 1;       // (a warp that takes one expert of all warps meets all banks)
+  int* const total = counts + kOrderWarps * ld;   // [experts]: rows of all experts in front of e
+  int* const kept = total + experts;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   pdl_wait();
   pdl_trigger();
-  for (int i = threadIdx.x; i < kOrderWarps * experts; i += 32 * kOrderWarps) counts[i] = 0;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < min(pairs, kOrderKept); i += kOrderThreads) kept[i] = chosen[i];
+  for (int i = threadIdx.x; i < kOrderWarps * ld; i += kOrderThreads) counts[i] = 0;
   __syncthreads();
-  const int run = (pairs + 32 * kOrderWarps - 1) / (32 * kOrderWarps) * 32, from = min(warp * run, pairs), to = min(from + run, pairs);
-  int* const own = counts + warp * experts;
-  int ahead[kOrderAhead];   // the run's first choices, asked for together
-#pragma unroll
-  for (int j = 0; j < kOrderAhead; ++j) ahead[j] = from + 32 * j + lane < to ? chosen[from + 32 * j + lane] : -1;
+  const int run = (pairs + kOrderThreads - 1) / kOrderThreads * 32, from = min(warp * run, pairs), to = min(from + run, pairs);
+  const int bits = 32 - __clz(experts - 1);   // of an expert's number
+  int* const own = counts + warp * ld;
+  // the pairs of this warp's run: where they lie, if they are ones, and the count of their expert in front of them
   auto walk = [&](auto at) {
-    auto step = [&](int i, int e) {
-      const bool is = i + lane < to;
+#pragma unroll 1
+    for (int i = from + lane; i - lane < to; i += 32) {
+      const bool is = i < to;
+      const int e = !is ? -1 : i < kOrderKept ? kept[i] : chosen[i];
       const bool valid = e >= 0 && e < experts;
-      const unsigned same = __match_any_sync(0xffffffffu, valid ? e : -1);
+      unsigned same = __ballot_sync(0xffffffffu, valid);
+      for (int b = 0; b < bits; ++b) {
+        const unsigned ones = __ballot_sync(0xffffffffu, e >> b & 1);
+        same &= e >> b & 1 ? ones : ~ones;
+      }
       int before = 0;
       if (valid) before = own[e];
       __syncwarp();
       if (valid && lane == __ffs(same) - 1) own[e] = before + __popc(same);
       __syncwarp();
-      if (is) at(i + lane, valid, before + __popc(same & ((1u << lane) - 1)));
-    };
-#pragma unroll
-    for (int j = 0; j < kOrderAhead; ++j)
-      if (from + 32 * j < to) step(from + 32 * j, ahead[j]);
-    for (int i = from + 32 * kOrderAhead; i < to; i += 32) step(i, i + lane < to ? chosen[i + lane] : -1);
+      if (is) at(i, valid, before + __popc(same & ((1u << lane) - 1)));
+    }
   };
   walk([](int, bool, int) {});
   __syncthreads();
-  for (int e = threadIdx.x; e < experts; e += 32 * kOrderWarps) {
-    int sum = 0;
-#pragma unroll 8
-    for (int w = 0; w < kOrderWarps; ++w) {
-      const int c = counts[w * experts + e];
-      counts[w * experts + e] = sum;
-      sum += c;
+  for (int e = warp; e < experts; e += kOrderWarps) {   // a lane has a warp's count
+    const int c = counts[lane * ld + e];
+    int upto = c;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
     }
-    total[e] = sum;
+    counts[lane * ld + e] = upto - c;
+    if (lane == 31) total[e] = upto;
   }
   __syncthreads();
   if (warp == 0) {   // every lane a run of experts
@@ -76,15 +84,16 @@ __global__ void __launch_bounds__(32 * kOrderWarps) expert_order_kernel(int32_t*
     }
     const int all = __shfl_sync(0xffffffffu, upto, 31);
     if (lane == 0) starts[experts] = all;
+    for (int i = all + lane; i < pairs; i += 32) source[i] = -1;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < kOrderWarps * experts; i += 32 * kOrderWarps) counts[i] += total[i % experts];
-  const int all_rows = starts[experts];
-  for (int i = all_rows + threadIdx.x; i < pairs; i += 32 * kOrderWarps) source[i] = -1;
-  __syncthreads();
-  walk([&](int i, bool valid, int to_place) {
-    place[i] = valid ? to_place : -1;
-    if (valid) source[to_place] = i / top;
+  walk([&](int i, bool valid, int number) {
+    int to_place = -1;
+    if (valid) {
+      to_place = number + total[i < kOrderKept ? kept[i] : chosen[i]];
+      source[to_place] = i / top;
+    }
+    place[i] = to_place;
   });
 }
 
@@ -97,24 +106,38 @@ __global__ void __launch_bounds__(256) expert_combine_kernel(__nv_bfloat16* __re
   constexpr int EACH = WIDE ? 8 : 1;
   const int pieces = n / EACH;
   const int64_t all = rows * pieces, y_rows = rows * top;
+  const bool small = all < 1ll << 31;   // (a division of 64 bits: a hundred instructions)
   for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < all; at += (int64_t)gridDim.x * 256) {
-    const int64_t row = at / pieces;
-    const int i = (int)(at % pieces) * EACH;
+    const int64_t row = small ? (int64_t)((uint32_t)at / (uint32_t)pieces) : at / pieces;
+    const int i = (int)(at - row * pieces) * EACH;
     float acc[EACH];
 #pragma unroll
     for (int e = 0; e < EACH; ++e) acc[e] = 0.f;
-#pragma unroll 4
-    for (int t = 0; t < top; ++t) {
-      const int64_t from = place[row * top + t];
-      if (from < 0 || from >= y_rows) continue;
-      const float w = weights[row * top + t];
-      if constexpr (WIDE) {
-        float v[8];
-        unpack8(*reinterpret_cast<const uint4*>(y + from * n + i), v);
+    for (int t0 = 0; t0 < top; t0 += 4) {   // four rows on their way together
+      float w[4];
+      uint4 v[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] = fmaf(w, v[e], acc[e]);
-      } else {
-        acc[0] = fmaf(w, bf16_to_f(y[from * n + i]), acc[0]);
+      for (int j = 0; j < 4; ++j) {
+        const int64_t from = t0 + j < top ? (int64_t)place[row * top + t0 + j] : -1;
+        const bool is = from >= 0 && from < y_rows;
+        w[j] = is ? weights[row * top + t0 + j] : 0.f;
+        v[j] = make_uint4(0, 0, 0, 0);
+        if constexpr (WIDE) {
+          if (is) v[j] = *reinterpret_cast<const uint4*>(y + from * n + i);
+        } else {
+          if (is) v[j].x = *reinterpret_cast<const uint16_t*>(y + from * n + i);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (WIDE) {
+          float u[8];
+          unpack8(v[j], u);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[e] = fmaf(w[j], u[e], acc[e]);
+        } else {
+          acc[0] = fmaf(w[j], bf16_lo(v[j].x), acc[0]);
+        }
       }
     }
     if constexpr (WIDE) *reinterpret_cast<uint4*>(out + row * n + i) = make_uint4(pack2(acc[0], acc[1]), pack2(acc[2], acc[3]), pack2(acc[4], acc[5]), pack2(acc[6], acc[7]));
@@ -160,8 +183,9 @@ int check_pairs(const char* what, int64_t rows, int64_t top, int64_t experts) {
 
 int launch_expert_order(int32_t* starts, int32_t* source, int32_t* place, const int32_t* chosen, int64_t rows, int64_t top, int64_t experts, cudaStream_t st) {
   static PerDevice attrs;
-  B200_CUDA(attrs([] { return cudaFuncSetAttribute(expert_order_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kOrderWarps + 1) * kMaxExperts * 4); }));
-  B200_CUDA(launch_pdl(expert_order_kernel, dim3(1), dim3(32 * kOrderWarps), (size_t)(kOrderWarps + 1) * experts * 4, st, op_pdl(st), starts, source, place, chosen,
+  auto bytes = [](int64_t e, int64_t n) { return (kOrderWarps * (e | 1) + e + std::min<int64_t>(n, kOrderKept)) * 4; };
+  B200_CUDA(attrs([&] { return cudaFuncSetAttribute(expert_order_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes(kMaxExperts, kOrderKept)); }));
+  B200_CUDA(launch_pdl(expert_order_kernel, dim3(1), dim3(kOrderThreads), (size_t)bytes(experts, rows * top), st, op_pdl(st), starts, source, place, chosen,
                        (int)(rows * top), (int)top, (int)experts));
   return B200_OK;
 }
@@ -169,7 +193,7 @@ int launch_expert_order(int32_t* starts, int32_t* source, int32_t* place, const 
 int launch_expert_combine(void* out, const void* y, const int32_t* place, const float* weights, int64_t rows, int64_t top, int64_t n, cudaStream_t st) {
   const bool wide = n % 8 == 0 && aligned16(out, y);
   const int64_t threads = rows * (wide ? n / 8 : n);
-  B200_CUDA(launch_pdl(wide ? expert_combine_kernel<true> : expert_combine_kernel<false>, dim3((unsigned)std::min<int64_t>((threads + 255) / 256, 148 * 8)), dim3(256),
+  B200_CUDA(launch_pdl(wide ? expert_combine_kernel<true> : expert_combine_kernel<false>, dim3((unsigned)std::min<int64_t>((threads + 255) / 256, 148 * 32)), dim3(256),
                        0, st, op_pdl(st), (__nv_bfloat16*)out, (const __nv_bfloat16*)y, place, weights, rows, (int)top, (int)n));
   return B200_OK;
 }
