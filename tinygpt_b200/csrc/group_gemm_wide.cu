@@ -143,8 +143,8 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         bool ready = false;   // the next stage, looked at behind the products of this one
         for (int t = first; t < tiles && ok; t += step) {
           for (int kb = 0; kb < k_blocks; ++kb) {
-            if ((F8 || kb == 0) && !(ok = warp_wait(&sums_empty[slot], slot_ph, p.err, kWaitCode | 2))) break;
-            if (!ready && !(ok = warp_wait(&full[s], ph, p.err, kWaitCode | 3))) break;
+            if (!ready && !(ok = warp_wait(&full[s], ph, p.err, kWaitCode | 2))) break;
+            if ((F8 || kb == 0) && !(ok = warp_wait(&sums_empty[slot], slot_ph, p.err, kWaitCode | 3))) break;
             tc_fence_after();
             const uint32_t x = x0 + s * (kXBytes >> 4), w = w0 + s * (F::w_bytes >> 4), d = tmem + slot * CH;
 #pragma unroll
