@@ -19,22 +19,23 @@ constexpr int kThreads = 384, kEpiWarps = 8;
 constexpr unsigned kWaitCode = 0x68000000u;
 constexpr int CH = 256, COLS = CH / 2, BLOCKS = CH / 128;   // channels of a tile, of a summing warp; blocks that share a scale of W
 constexpr int SLOTS = 512 / CH;
-constexpr int kOutLd = CH * 2 + 16;               // bytes from row to row of a finished tile: eight rows meet all banks
-// GROUP CTAs to a tile of GROUP·128 rows × 256 channels
-template <int GROUP>
+// GROUP CTAs to a tile of GROUP·128 rows × 256 channels.  8 bits: a finished tile lies in shared memory as a whole, so that no summing thread waits for the
+// store of another's part.  bf16: its two halves one behind the other, for a fifth stage.
+template <bool F8, int GROUP>
 struct Wide {
   static constexpr int w_rows = CH / GROUP, w_bytes = w_rows * 128, stage = kXBytes + w_bytes;
-  static constexpr int stages = GROUP == 2 ? 4 : 3;
-  static constexpr int lag = 4, ahead = 2 * SLOTS + 1 + lag;   // blocks of factors that are asked for ahead, and kept: see group_gemm.cu
+  static constexpr int stages = GROUP == 1 ? 3 : F8 ? 4 : 5;
+  static constexpr int lag = 4, ahead = F8 ? 2 * SLOTS + 1 + lag : 0;   // blocks of factors that are asked for ahead, and kept: see group_gemm.cu
+  static constexpr int out_parts = F8 ? 1 : 2, out_ch = CH / out_parts, out_ld = out_ch * 2 + 16;   // bytes from row to row: eight rows meet all banks
   static constexpr int ring = stages * stage;
-  static constexpr int tables = 1024 + ring + kRows * kOutLd + ahead * BLOCKS * kRows * 4 + 512;
+  static constexpr int tables = 1024 + ring + kRows * out_ld + ahead * BLOCKS * kRows * 4 + 512;
   static constexpr int smem(int experts) { return tables + Groups::bytes(experts); }
   static constexpr int fit = (227 * 1024 - tables) / Groups::bytes(1), most_experts = fit < kMaxExperts ? fit : kMaxExperts;
 };
 // A thread that sums 8-bit products holds 128 sums: the four warps that hold none give registers up.
 constexpr int kRegsFew = 72, kRegsMany = 216, kRegsLaunch = 168;
 static_assert(128 * kRegsFew + 256 * kRegsMany <= kThreads * kRegsLaunch, "no warp waits for registers that the launch does not have");
-static_assert(Wide<2>::most_experts == kMaxExperts && Wide<1>::most_experts >= 128, "room");
+static_assert(Wide<true, 2>::most_experts == kMaxExperts && Wide<false, 2>::most_experts == kMaxExperts && Wide<true, 1>::most_experts >= 128, "room");
 
 #define B200_R8(b) "+r"(r[b]), "+r"(r[b + 1]), "+r"(r[b + 2]), "+r"(r[b + 3]), "+r"(r[b + 4]), "+r"(r[b + 5]), "+r"(r[b + 6]), "+r"(r[b + 7])
 // the wait for what tmem_ld32 has loaded holds it: nothing that uses it moves in front of the wait
@@ -46,21 +47,21 @@ __device__ __forceinline__ void loaded(uint32_t (&r)[32]) {
 template <bool F8, int GROUP>
 __global__ void __launch_bounds__(kThreads, 1)
 group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const GemmArgs p) {
-  using F = Wide<GROUP>;
+  using F = Wide<F8, GROUP>;
   constexpr int ST = F::stages, AHEAD = F::ahead, F_SLOT = BLOCKS * kRows;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* const sx = smem;                                                        // [stages][128 rows × 128 bytes]
   uint8_t* const sw = smem + ST * kXBytes;                                         // this CTA's rows of W alike
   uint8_t* const done_tile = smem + F::ring;                                       // [128][out_ld]: bf16
-  float* const factors = reinterpret_cast<float*>(done_tile + kRows * kOutLd);  // [AHEAD][blocks][128]: of a block of channels, of a row
+  float* const factors = reinterpret_cast<float*>(done_tile + kRows * F::out_ld);  // [AHEAD][blocks][128]: of a block of channels, of a row
   uint64_t* const full = reinterpret_cast<uint64_t*>(factors + AHEAD * F_SLOT);    // [stages], CTA 0's count the pair's bytes
   uint64_t* const empty = full + ST;
   uint64_t* const sums_full = empty + ST;                                          // [slots]
   uint64_t* const sums_empty = sums_full + SLOTS;                                  // CTA 0's
   uint64_t* const out_full = sums_empty + SLOTS;
-  uint64_t* const out_empty = out_full + 1;
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(out_empty + 1);
+  uint64_t* const out_empty = out_full + 1;                                        // [parts]
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(out_empty + F::out_parts);
   float* const w_scale = reinterpret_cast<float*>(tmem_slot + 1);                  // [AHEAD][blocks]
   Groups groups(reinterpret_cast<int*>(smem + F::tables - 1024), p.experts);
   const int warp = uniform((int)threadIdx.x / 32), lane = threadIdx.x % 32;
@@ -78,8 +79,8 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
       mbar_init(&sums_full[a], F8 ? 2 : 1);   // products done, factors there
       mbar_init(&sums_empty[a], GROUP * kEpiWarps);
     }
-    mbar_init(out_full, kEpiWarps);
-    mbar_init(out_empty, 1);
+    mbar_init(out_full, kEpiWarps / F::out_parts);
+    for (int part = 0; part < F::out_parts; ++part) mbar_init(&out_empty[part], 1);
     fence_mbar_init();
   }
   if (warp == 1) tmem_alloc<GROUP>(tmem_slot, 512);
@@ -218,9 +219,15 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
       uint32_t ph = 0;
       for (int t = first; t < tiles; t += step, ph ^= 1) {
         const Tile tile = tile_at(t);
-        if (!(ok = warp_wait(out_full, ph, p.err, kWaitCode | 6))) break;
-        store_tile(p.y + tile.row0 * p.n + tile.ch0, done_tile, kOutLd, tile.rows, min(CH, p.n - tile.ch0), p, lane);
-        if (lane == 0) mbar_arrive(out_empty);
+#pragma unroll
+        for (int part = 0; part < F::out_parts && ok; ++part) {
+          if (!(ok = warp_wait(out_full, ph, p.err, kWaitCode | 6))) break;
+          const int ch = tile.ch0 + part * F::out_ch;
+          store_tile(p.y + tile.row0 * p.n + ch, done_tile, F::out_ld, tile.rows, min(F::out_ch, p.n - ch), p, lane);
+          if (lane == 0) mbar_arrive(&out_empty[part]);
+          if (part + 1 < F::out_parts) ph ^= 1;
+        }
+        if (!ok) break;
       }
       bulk_wait();
       zero_other_rows(p, lane);
@@ -229,7 +236,7 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
     if constexpr (F8) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsMany));
     const int quad = warp & 3, half = (warp - 4) >> 2, row = quad * 32 + lane;
     const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + half * COLS, free_bar = GROUP == 2 ? mapa_u32(smem_u32(sums_empty), 0) : 0;
-    uint8_t* const put_at = done_tile + row * kOutLd + half * COLS * 2;
+    uint8_t* const put_at = done_tile + row * F::out_ld + (F8 ? half * COLS * 2 : 0);
     const float* const my_factors = factors + half * kRows + row;
     int slot = 0, fslot = 0;
     uint32_t slot_ph = 0, out_ph = 1;
@@ -317,7 +324,8 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
       } else {
         if (!(ok = warp_wait(&sums_full[slot], slot_ph, p.err, kWaitCode | 5))) break;
         tc_fence_after();
-        if (!(ok = warp_wait(out_empty, out_ph, p.err, kWaitCode | 7))) break;
+        // the first half waits for the store of the last tile's second half, the second half for that of the first
+        if (!(ok = warp_wait(&out_empty[1 - half], half == 0 ? out_ph : out_ph ^ 1, p.err, kWaitCode | 7))) break;
         if (mine) {
 #pragma unroll 1
           for (int i = 0; i < COLS / 32; ++i) {
@@ -356,7 +364,7 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
 
 template <bool F8, int GROUP>
 int launch(const GroupProduct& g, GemmArgs& p, cudaStream_t st) {
-  using F = Wide<GROUP>;
+  using F = Wide<F8, GROUP>;
   static PerDevice attrs;
   B200_CUDA(attrs([] {
     cudaFuncAttributes a{};
@@ -401,7 +409,7 @@ int launch(const GroupProduct& g, GemmArgs& p, cudaStream_t st) {
 }  // namespace
 
 int launch_group_wide(const GroupProduct& g, GemmArgs& p, cudaStream_t st) {
-  return g.x_scale == nullptr ? launch<false, 2>(g, p, st) : g.experts <= Wide<1>::most_experts ? launch<true, 1>(g, p, st) : launch<true, 2>(g, p, st);
+  return g.x_scale == nullptr ? launch<false, 2>(g, p, st) : g.experts <= Wide<true, 1>::most_experts ? launch<true, 1>(g, p, st) : launch<true, 2>(g, p, st);
 }
 
 }  // namespace b200
