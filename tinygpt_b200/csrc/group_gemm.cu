@@ -8,7 +8,7 @@
 //   warp 0   TMA: of every 128 bytes of k 128 rows of W and the tile's rows of x, into a ring of shared memory
 //   warp 1   one thread issues four products (K = 32 bytes) per 128 bytes
 //   warp 2   8 bits: the products of x's and W's scales, NT of them for each block of 128 entries, fetched some blocks ahead
-//   warp 3   takes finished tiles from shared memory to y, row by row in bulk copies, beside the next tile's products; rows of no group are zeroed
+//   warp 3   takes finished tiles from shared memory to y, beside the next tile's products; rows of no group are zeroed
 //   warps 4 … 11   the sums: a warp has a quarter of the channels and half of the rows, as fragments of 8 × 8 (lane 4r + c: channel r, rows 2c and 2c + 1), so
 //            that a lane needs a quarter of the factors and a transposing store to shared memory makes rows of y of them
 // 8 bits: W has a scale for 128 × 128 entries and x one for 128 entries of a row, so that 128 entries of k meet one factor per row of x, and the sums of 128
@@ -18,6 +18,7 @@
 #include "group_gemm.cuh"
 
 #include <algorithm>
+#include <cmath>
 
 namespace b200 {
 
@@ -265,10 +266,9 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
         for (int t = first; t < tiles; t += step, ph ^= 1) {
           const Tile tile = tile_at(t);
           if (!(ok = warp_wait(out_full, ph, p.err, kWaitCode | 6))) break;
-          store_tile(p.y + tile.row0 * p.n + tile.ch0, done_tile, kOutLd, tile.rows, min(kCh, p.n - tile.ch0), p, lane);
+          store_tile<kCh / 8>(p.y + tile.row0 * p.n + tile.ch0, done_tile, kOutLd, tile.rows, min(kCh, p.n - tile.ch0), p, lane);
           if (lane == 0) mbar_arrive(out_empty);
         }
-        bulk_wait();   // (shared memory and what was stored outlive the CTA only so)
       }
       zero_other_rows(p, lane);
     }
@@ -302,7 +302,6 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
       };
       auto finished = [&]() {   // this warp's part of the tile lies in shared memory
         if (p.splits > 1) return;
-        fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(out_full);
       };
@@ -457,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
 }
 
 template <bool F8, int NT>
-int launch(const GroupProduct& g, GemmArgs& p, cudaStream_t st) {
+int launch(const GroupProduct& g, GemmArgs& p, int splits, cudaStream_t st) {
   using F = Form<NT>;
   static PerDevice attrs;
   B200_CUDA(attrs([] {
@@ -476,11 +475,9 @@ int launch(const GroupProduct& g, GemmArgs& p, cudaStream_t st) {
   p.ch_tiles = p.ch_blocks;
   // tiles that there can be: every group's last one may be short
   const int64_t row_tiles = g.starts ? g.rows / NT + std::min<int64_t>(g.experts, g.rows) : (g.rows + NT - 1) / NT, most = row_tiles * p.ch_tiles;
-  const int64_t room = 148 * F::per_sm;
-  p.splits = 1;
-  while (p.splits < kMaxSplits && most * p.splits * 2 <= room && p.k_blocks >= 4 * p.splits) p.splits *= 2;
+  p.splits = splits;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(p.splits > 1 ? most * p.splits : std::min(most, room)));
+  cfg.gridDim = dim3((unsigned)(p.splits > 1 ? most * p.splits : std::min<int64_t>(most, 148 * F::per_sm)));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = F::smem((int)g.experts);
   cfg.stream = st;
@@ -497,15 +494,51 @@ int launch(const GroupProduct& g, GemmArgs& p, cudaStream_t st) {
   return B200_OK;
 }
 
+// Rows of a tile (16 to 128 here, or a tile of group_gemm_wide.cu) and CTAs to a tile: what the whole call is estimated to take, in µs.  A CTA needs 0.25 (16 rows) to
+// 0.5 µs (128) for 128 bytes of k, a wide one 0.53 (bf16 0.38 a pair); two CTAs on an SM 1.45 times that each; partial tiles that meet cost 1 µs and more.  Measured:
+// one of each in the way that is taken and, in brackets, the next best: 200 × 4 096 × 14 336 33 µs in tiles of 128 rows and two CTAs to each (64, wide), 512 × 4 096 × 14 336
+// 56 in tiles of 128 (64, wide), 768 rows 66 wide (101, 128), 100 × 28 672 × 4 096 30 wide (39, 128), 48 × 4 096 × 4 096 10.7 with 32 (11.6, 64), 512 × 1 152 × 896 8.3 with 32 (12.8,
+// wide), 1 × 4 096 × 4 096 9.1 with four CTAs to a tile (13.9, one; 9.2, eight).
+struct Way {
+  int rows, splits;   // rows 0: wide
+};
+Way choose(const GroupProduct& g, bool f8) {
+  auto up = [](double a, double b) { return std::ceil(a / b); };
+  const double groups = g.starts ? (double)std::min<int64_t>(g.experts, g.rows) : 1, average = (double)g.rows / groups;
+  const double k_blocks = up((double)g.k, f8 ? 128 : 64);
+  // groups are unlike: half of a last tile is empty on average, and no group has less than a tile
+  auto row_tiles = [&](int rows) { return g.starts ? groups * std::max(1.0, average / rows + 0.5) : up(average, rows); };
+  Way best{0, 1};
+  // wide: a CTA of 128 rows in 8 bits, a pair of 256 in bf16
+  double least = 7.5 + up(row_tiles(f8 ? 128 : 256) * up((double)g.n, 256), f8 ? 148 : 74) * (k_blocks * (f8 ? 0.53 : 0.38) + 1.2);
+  for (int rows = 16; rows <= 128; rows *= 2) {
+    const double tiles = row_tiles(rows) * up((double)g.n, kCh), each = (f8 ? 0.22 : 0.19) + (f8 ? 0.0021 : 0.0012) * std::min<double>(rows, average);
+    for (int splits = 1; splits <= kMaxSplits && (splits == 1 || k_blocks >= 2 * splits); splits *= 2) {
+      constexpr int kOne[4] = {148, 74, 33, 15}, kTwo[4] = {296, 148, 70, 32};   // clusters that the SMs hold at once
+      const int i = splits == 1 ? 0 : splits == 2 ? 1 : splits == 4 ? 2 : 3;
+      const double share = rows <= 64 && tiles * splits > 148 ? 1.45 : 1.0;
+      const int hold = rows <= 64 ? kTwo[i] : kOne[i];
+      if (splits > 1 && (g.starts ? (g.rows / rows + groups) * up((double)g.n, kCh) : tiles) > hold) break;   // (a cluster that comes later starts from nothing)
+      const double us = 5.5 + (splits > 1 ? 1.0 + 0.35 * splits : 0.0) + up(tiles, hold) * up(k_blocks, splits) * each * share;
+      if (us < least) {
+        least = us;
+        best = Way{rows, splits};
+      }
+    }
+  }
+  return best;
+}
+
 template <bool F8>
 int launch_for(const GroupProduct& g, GemmArgs& p, cudaStream_t st) {
-  // rows of a tile: a group's, or twice its share of them (groups are unlike)
-  const int64_t want = g.starts == nullptr ? g.rows : 2 * g.rows / std::min<int64_t>(g.experts, g.rows);
-  if (want <= 16) return launch<F8, 16>(g, p, st);
-  if (want <= 32) return launch<F8, 32>(g, p, st);
-  if (want <= 64) return launch<F8, 64>(g, p, st);
-  if (want <= 128) return launch<F8, 128>(g, p, st);
-  return launch_group_wide(g, p, st);
+  const Way way = choose(g, F8);
+  switch (way.rows) {
+    case 16: return launch<F8, 16>(g, p, way.splits, st);
+    case 32: return launch<F8, 32>(g, p, way.splits, st);
+    case 64: return launch<F8, 64>(g, p, way.splits, st);
+    case 128: return launch<F8, 128>(g, p, way.splits, st);
+    default: return launch_group_wide(g, p, st);
+  }
 }
 
 }  // namespace

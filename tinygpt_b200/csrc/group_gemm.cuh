@@ -71,13 +71,6 @@ template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-// bytes of shared memory → global memory, 16-byte pieces; what a lane has asked for is complete behind its bulk_wait, and read behind bulk_wait_read
-__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 // Waits as mbar_wait_limited does, but asleep: a thread that polls takes issue slots from the warps that sum.  False after about two seconds.
 __device__ __forceinline__ bool try_wait_asleep(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
@@ -186,14 +179,21 @@ __device__ __forceinline__ void zero_other_rows(const GemmArgs& p, int lane) {
     for (int i = lane; i < p.n; i += 32) out[i] = f_to_bf16(0.f);
   }
 }
-// A finished tile in shared memory, rows `ld` bytes apart → y, by one warp: a bulk copy to a row where rows of y take 16-byte pieces.  Shared memory may be written
-// again afterwards; bulk_wait before the CTA ends.
+// A finished tile of LANES·8 channels in shared memory, rows `ld` bytes apart → y, by one warp, sixteen bytes a lane where rows of y take them.  Shared memory may
+// be written again afterwards.  (A bulk copy to a row took the copy engine 3 µs for 128 rows of 256 bytes.)
+template <int LANES>
 __device__ __forceinline__ void store_tile(__nv_bfloat16* out, const uint8_t* tile, int ld, int rows, int width, const GemmArgs& p, int lane) {
   if (p.wide) {
-    if (width > 0)
-      for (int row = lane; row < rows; row += 32) bulk_store(out + (int64_t)row * p.n, tile + row * ld, width * 2);
-    bulk_commit();
-    bulk_wait_read();
+    constexpr int U = 8, SIDE = 32 / LANES;   // rows side by side
+    const int i = lane % LANES * 8;
+    for (int row0 = lane / LANES; row0 - lane / LANES < rows; row0 += U * SIDE) {
+      uint4 v[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) v[j] = *reinterpret_cast<const uint4*>(tile + min(row0 + j * SIDE, rows - 1) * ld + i * 2);
+#pragma unroll
+      for (int j = 0; j < U; ++j)
+        if (row0 + j * SIDE < rows && i < width) *reinterpret_cast<uint4*>(out + (int64_t)(row0 + j * SIDE) * p.n + i) = v[j];
+    }
   } else {   // a lane takes four channels, eight rows at a time, in pieces that n allows
     const int piece = p.n % 4 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 7) == 0 ? 4 : p.n % 2 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 3) == 0 ? 2 : 1;
     for (int i = lane * 4; i < width; i += 128)

@@ -223,13 +223,12 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         for (int part = 0; part < F::out_parts && ok; ++part) {
           if (!(ok = warp_wait(out_full, ph, p.err, kWaitCode | 6))) break;
           const int ch = tile.ch0 + part * F::out_ch;
-          store_tile(p.y + tile.row0 * p.n + ch, done_tile, F::out_ld, tile.rows, min(F::out_ch, p.n - ch), p, lane);
+          store_tile<F::out_ch / 8>(p.y + tile.row0 * p.n + ch, done_tile, F::out_ld, tile.rows, min(F::out_ch, p.n - ch), p, lane);
           if (lane == 0) mbar_arrive(&out_empty[part]);
           if (part + 1 < F::out_parts) ph ^= 1;
         }
         if (!ok) break;
       }
-      bulk_wait();
       zero_other_rows(p, lane);
     }
   } else {
@@ -346,8 +345,7 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         }
         release();
       }
-      fence_proxy_async();   // this warp's part of the tile lies in shared memory
-      __syncwarp();
+      __syncwarp();   // this warp's part of the tile lies in shared memory
       if (lane == 0) mbar_arrive(out_full);
     }
   }
