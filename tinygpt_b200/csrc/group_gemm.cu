@@ -1,8 +1,9 @@
 // group_gemm.cu — products of rows with the matrix of their group, on the 5th-generation tensor cores:  y[r] = W[e]·x[r] for the rows r of group e.
 //
-// This kernel takes groups of up to 128 rows, on average, for bf16 and for 8 bits with scales, for one matrix (a Linear) and for many (experts, rows sorted by expert).  W is the A operand: a tile is
-// 128 of its rows (channels) × up to NT rows of x, and the product's N is what the tile really holds, rounded up to 16.  So a group of three rows costs a stream of its
-// matrix and little else, and a group that ends inside a tile costs no idle rows.
+// For bf16 and for 8 bits with scales, for one matrix (a Linear) and for many (experts, rows sorted by expert).  W is the A operand: a tile is 128 of its rows (channels) ×
+// up to NT rows of x, and the product's N is what the tile really holds, rounded up to 16.  So a group of three rows costs a stream of its matrix and little else, and a
+// group that ends inside a tile costs no idle rows.  Few rows are bound by that stream: one row × 28 672 × 4 096 in 8 bits 22.8 µs, 5.2 TB/s; launch, the first loads' way
+// (1.6 µs) and the end are 5 µs of any call.
 //
 // Warp-specialised, persistent over the tiles:
 //   warp 0   TMA: of every 128 bytes of k 128 rows of W and the tile's rows of x, into a ring of shared memory
@@ -14,7 +15,8 @@
 // 8 bits: W has a scale for 128 × 128 entries and x one for 128 entries of a row, so that 128 entries of k meet one factor per row of x, and the sums of 128
 // entries — a slot of tensor memory each — are scaled and added in fp32 registers; two to four slots keep the tensor cores running meanwhile.
 // bf16: a slot holds the sums over all of k.
-// More rows go to tiles of 256 × 256 on pairs of CTAs (group_gemm_wide.cu).
+// Where there are few tiles, a cluster of CTAs shares a tile's k and each sums its rows of the partial tiles, sent through distributed shared memory.
+// Many rows go to tiles of 256 channels with x as the A operand (group_gemm_wide.cu); choose() says when.
 #include "group_gemm.cuh"
 
 #include <algorithm>
@@ -510,7 +512,7 @@ Way choose(const GroupProduct& g, bool f8) {
   auto row_tiles = [&](int rows) { return g.starts ? groups * std::max(1.0, average / rows + 0.5) : up(average, rows); };
   Way best{0, 1};
   // wide: a CTA of 128 rows in 8 bits, a pair of 256 in bf16
-  double least = 7.5 + up(row_tiles(f8 ? 128 : 256) * up((double)g.n, 256), f8 ? 148 : 74) * (k_blocks * (f8 ? 0.53 : 0.38) + 1.2);
+  double least = f8 && g.experts > kWideExperts8 ? 1e30 : 7.5 + up(row_tiles(f8 ? 128 : 256) * up((double)g.n, 256), f8 ? 148 : 74) * (k_blocks * (f8 ? 0.53 : 0.38) + 1.2);
   for (int rows = 16; rows <= 128; rows *= 2) {
     const double tiles = row_tiles(rows) * up((double)g.n, kCh), each = (f8 ? 0.22 : 0.19) + (f8 ? 0.0021 : 0.0012) * std::min<double>(rows, average);
     for (int splits = 1; splits <= kMaxSplits && (splits == 1 || k_blocks >= 2 * splits); splits *= 2) {

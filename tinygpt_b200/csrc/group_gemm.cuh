@@ -15,7 +15,8 @@ struct GemmArgs {
   int n, k_blocks, experts, ch_tiles, ch_blocks, splits;   // ch_tiles: of a tile's channels; ch_blocks: of 128 channels
   bool wide;    // y takes stores of 16 bytes
 };
-// tiles of 256 rows × 256 channels on pairs of CTAs (group_gemm_wide.cu)
+// tiles of 256 channels (group_gemm_wide.cu); in 8 bits for so many matrices
+constexpr int kWideExperts8 = 512;
 int launch_group_wide(const GroupProduct& g, GemmArgs& p, cudaStream_t st);
 
 #ifdef __CUDACC__
@@ -176,7 +177,10 @@ __device__ __forceinline__ void zero_other_rows(const GemmArgs& p, int lane) {
   const int64_t from = min(max((int64_t)p.starts[0], (int64_t)0), p.rows), to = min(max((int64_t)p.starts[p.experts], from), p.rows);
   for (int64_t r = blockIdx.x; r < p.rows - (to - from); r += gridDim.x) {
     __nv_bfloat16* const out = p.y + (r < from ? r : r - from + to) * p.n;
-    for (int i = lane; i < p.n; i += 32) out[i] = f_to_bf16(0.f);
+    if (p.wide)
+      for (int i = lane * 8; i < p.n; i += 256) *reinterpret_cast<uint4*>(out + i) = make_uint4(0, 0, 0, 0);
+    else
+      for (int i = lane; i < p.n; i += 32) out[i] = f_to_bf16(0.f);
   }
 }
 // A finished tile of LANES·8 channels in shared memory, rows `ld` bytes apart → y, by one warp, sixteen bytes a lane where rows of y take them.  Shared memory may

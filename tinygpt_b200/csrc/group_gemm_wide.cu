@@ -1,10 +1,15 @@
-// group_gemm_wide.cu — grouped products for groups of many rows: tiles of 256 rows of x × 256 channels on pairs of CTAs (cta_group::2), bf16 and 8 bits with scales.
+// group_gemm_wide.cu — grouped products for groups of many rows: 256 channels and, in 8 bits, 128 rows of x to a CTA, in bf16 256 rows to a pair of them (cta_group::2).
 //
-// x is the A operand here: a CTA brings 128 rows of x and 128 of W for every 128 bytes of k (32 KB where a CTA by itself would need 48) and sums its rows over
-// all 256 channels.  A lane of tensor memory is a row of x, so that in 8 bits a summing thread — a row, one block of 128 channels — needs one factor for 128 sums: it
-// scales and adds them in 313 cycles for eight warps, where the products of a block of k take 512.  With W as A (group_gemm.cu) factors differ from sum to sum:
-// 620 to 660 cycles alone, 900 beside the products' own traffic to shared memory, and 4 096 × 28 672 × 4 096 took 754 µs.
-// The roles of the warps are those of group_gemm.cu; two slots of 256 columns of tensor memory.
+// x is the A operand here: a lane of tensor memory is a row of x, so that in 8 bits a summing thread — a row, one block of 128 channels — needs one factor for 128
+// sums.  With W as A (group_gemm.cu) factors differ from sum to sum: adding 128 entries of k for 128 × 256 sums took 620 to 660 cycles alone for 313 here, and
+// 4 096 × 28 672 × 4 096 took 754 µs for 465 (2.07 PFLOP/s; 530 in a run of them, under the power cap).  The roles of the warps are those of group_gemm.cu; two slots of 256
+// columns of tensor memory.
+// 8 bits: a block of k takes some 950 cycles where its products need 512.  A slot goes around — products, 646 cycles until they are seen; factors, loads and sums, 450; back to
+// the issuing warp — and there is room for two; reading sums also holds the products up (a block's loads by 124 cycles), and x and W of 48 KB a block are
+// written to and read from shared memory in 768.  Tried and as slow or slower: pairs with 256 rows (32 KB a block; longer ways from CTA to CTA), four slots of 128
+// columns (the issue of four products alone takes 249 cycles), halves of a slot by themselves, sums in pairs or one by one, an earlier look at the next slot.
+// A pair in 8 bits ends groups in tiles of 256 rows: 2 048 rows with four of 32 experts each 159 µs for 143.
+// bf16: tensor memory sums over all of k; 4 096 × 4 096 × 4 096 96.6 µs (1.42 PFLOP/s), a CTA by itself 127.
 #include "group_gemm.cuh"
 
 #include <algorithm>
@@ -19,23 +24,23 @@ constexpr int kThreads = 384, kEpiWarps = 8;
 constexpr unsigned kWaitCode = 0x68000000u;
 constexpr int CH = 256, COLS = CH / 2, BLOCKS = CH / 128;   // channels of a tile, of a summing warp; blocks that share a scale of W
 constexpr int SLOTS = 512 / CH;
-// GROUP CTAs to a tile of GROUP·128 rows × 256 channels.  8 bits: a finished tile lies in shared memory as a whole, so that no summing thread waits for the
-// store of another's part.  bf16: its two halves one behind the other, for a fifth stage.
-template <bool F8, int GROUP>
+// 8 bits: a finished tile lies in shared memory as a whole, so that no summing thread waits for the store of another's part.  bf16: its two halves one behind the other,
+// for a fifth stage (4 096 × 4 096 × 4 096 107 → 101 µs).
+template <bool F8>
 struct Wide {
-  static constexpr int w_rows = CH / GROUP, w_bytes = w_rows * 128, stage = kXBytes + w_bytes;
-  static constexpr int stages = GROUP == 1 ? 3 : F8 ? 4 : 5;
+  static constexpr int group = F8 ? 1 : 2;        // CTAs to a tile
+  static constexpr int w_rows = CH / group, w_bytes = w_rows * 128, stage = kXBytes + w_bytes;
+  static constexpr int stages = F8 ? 3 : 5;
   static constexpr int lag = 4, ahead = F8 ? 2 * SLOTS + 1 + lag : 0;   // blocks of factors that are asked for ahead, and kept: see group_gemm.cu
   static constexpr int out_parts = F8 ? 1 : 2, out_ch = CH / out_parts, out_ld = out_ch * 2 + 16;   // bytes from row to row: eight rows meet all banks
   static constexpr int ring = stages * stage;
   static constexpr int tables = 1024 + ring + kRows * out_ld + ahead * BLOCKS * kRows * 4 + 512;
   static constexpr int smem(int experts) { return tables + Groups::bytes(experts); }
-  static constexpr int fit = (227 * 1024 - tables) / Groups::bytes(1), most_experts = fit < kMaxExperts ? fit : kMaxExperts;
 };
 // A thread that sums 8-bit products holds 128 sums: the four warps that hold none give registers up.
 constexpr int kRegsFew = 72, kRegsMany = 216, kRegsLaunch = 168;
 static_assert(128 * kRegsFew + 256 * kRegsMany <= kThreads * kRegsLaunch, "no warp waits for registers that the launch does not have");
-static_assert(Wide<true, 2>::most_experts == kMaxExperts && Wide<false, 2>::most_experts == kMaxExperts && Wide<true, 1>::most_experts >= 128, "room");
+static_assert(Wide<true>::smem(kWideExperts8) <= 227 * 1024 && Wide<false>::smem(kMaxExperts) <= 227 * 1024, "room");
 
 #define B200_R8(b) "+r"(r[b]), "+r"(r[b + 1]), "+r"(r[b + 2]), "+r"(r[b + 3]), "+r"(r[b + 4]), "+r"(r[b + 5]), "+r"(r[b + 6]), "+r"(r[b + 7])
 // the wait for what tmem_ld32 has loaded holds it: nothing that uses it moves in front of the wait
@@ -44,11 +49,11 @@ __device__ __forceinline__ void loaded(uint32_t (&r)[32]) {
   asm volatile("" : B200_R8(16), B200_R8(24));
 }
 
-template <bool F8, int GROUP>
+template <bool F8>
 __global__ void __launch_bounds__(kThreads, 1)
 group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const GemmArgs p) {
-  using F = Wide<F8, GROUP>;
-  constexpr int ST = F::stages, AHEAD = F::ahead, F_SLOT = BLOCKS * kRows;
+  using F = Wide<F8>;
+  constexpr int GROUP = F::group, ST = F::stages, AHEAD = F::ahead, F_SLOT = BLOCKS * kRows;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* const sx = smem;                                                        // [stages][128 rows × 128 bytes]
@@ -360,16 +365,16 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
   if constexpr (GROUP == 2) cluster_sync_all();
 }
 
-template <bool F8, int GROUP>
+template <bool F8>
 int launch(const GroupProduct& g, GemmArgs& p, cudaStream_t st) {
-  using F = Wide<F8, GROUP>;
+  using F = Wide<F8>;
   static PerDevice attrs;
   B200_CUDA(attrs([] {
     cudaFuncAttributes a{};
-    const cudaError_t e = cudaFuncGetAttributes(&a, group_wide_kernel<F8, GROUP>);
+    const cudaError_t e = cudaFuncGetAttributes(&a, group_wide_kernel<F8>);
     if (e != cudaSuccess) return e;
     if (F8 && a.numRegs != kRegsLaunch) return cudaErrorInvalidDeviceFunction;   // (the shares would not add up)
-    return cudaFuncSetAttribute(group_wide_kernel<F8, GROUP>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::smem(F::most_experts));
+    return cudaFuncSetAttribute(group_wide_kernel<F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::smem(F8 ? kWideExperts8 : kMaxExperts));
   }));
   CUtensorMap tw, tx;
   int rc;
@@ -384,7 +389,7 @@ int launch(const GroupProduct& g, GemmArgs& p, cudaStream_t st) {
   p.ch_tiles = (int)((g.n + CH - 1) / CH);
   p.splits = 1;
   // tiles that there can be: every group's last one may be short
-  constexpr int kTileRows = GROUP * kRows;
+  constexpr int GROUP = F::group, kTileRows = GROUP * kRows;
   const int64_t row_tiles = g.starts ? g.rows / kTileRows + std::min<int64_t>(g.experts, g.rows) : (g.rows + kTileRows - 1) / kTileRows;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(GROUP * std::min<int64_t>(row_tiles * p.ch_tiles, 148 / GROUP)));
@@ -400,14 +405,12 @@ int launch(const GroupProduct& g, GemmArgs& p, cudaStream_t st) {
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   g_launches.fetch_add(1, std::memory_order_relaxed);
-  B200_CUDA(cudaLaunchKernelEx(&cfg, group_wide_kernel<F8, GROUP>, tw, tx, (const GemmArgs)p));
+  B200_CUDA(cudaLaunchKernelEx(&cfg, group_wide_kernel<F8>, tw, tx, (const GemmArgs)p));
   return B200_OK;
 }
 
 }  // namespace
 
-int launch_group_wide(const GroupProduct& g, GemmArgs& p, cudaStream_t st) {
-  return g.x_scale == nullptr ? launch<false, 2>(g, p, st) : g.experts <= Wide<true, 1>::most_experts ? launch<true, 1>(g, p, st) : launch<true, 2>(g, p, st);
-}
+int launch_group_wide(const GroupProduct& g, GemmArgs& p, cudaStream_t st) { return g.x_scale == nullptr ? launch<false>(g, p, st) : launch<true>(g, p, st); }
 
 }  // namespace b200
