@@ -2,14 +2,17 @@
 //
 // x is the A operand here: a lane of tensor memory is a row of x, so that in 8 bits a summing thread — a row, one block of 128 channels — needs one factor for 128
 // sums.  With W as A (group_gemm.cu) factors differ from sum to sum: adding 128 entries of k for 128 × 256 sums took 620 to 660 cycles alone for 313 here, and
-// 4 096 × 28 672 × 4 096 took 754 µs for 465 (2.07 PFLOP/s; 530 in a run of them, under the power cap).  The roles of the warps are those of group_gemm.cu; two slots of 256
-// columns of tensor memory.
+// 4 096 × 28 672 × 4 096 took 754 µs for 465 (2.07 PFLOP/s; 530 in a run of them, under the power cap).  The roles of the warps are those of group_gemm.cu but for warp 3, which
+// finds the CTA's tiles; two slots of 256 columns of tensor memory.
 // 8 bits: a block of k takes some 950 cycles where its products need 512.  A slot goes around — products, 646 cycles until they are seen; factors, loads and sums, 450; back to
 // the issuing warp — and there is room for two; reading sums also holds the products up (a block's loads by 124 cycles), and x and W of 48 KB a block are
 // written to and read from shared memory in 768.  Tried and as slow or slower: pairs with 256 rows (32 KB a block; longer ways from CTA to CTA), four slots of 128
 // columns (the issue of four products alone takes 249 cycles), halves of a slot by themselves, sums in pairs or one by one, an earlier look at the next slot.
 // A pair in 8 bits ends groups in tiles of 256 rows: 2 048 rows with four of 32 experts each 159 µs for 143.
-// bf16: tensor memory sums over all of k; 4 096 × 4 096 × 4 096 96.6 µs (1.42 PFLOP/s), a CTA by itself 127.
+// bf16: tensor memory sums over all of k; 4 096 × 4 096 × 4 096 93.5 µs (1.47 PFLOP/s).  A CTA by itself took 127 where a pair took 97.
+// A summing warp stores what it summed itself, 32 channels at a time through two kilobytes: with whole tiles handed to a storing warp the last one of a CTA came 5 µs
+// behind its sums, and their room is a stage of operands now.  With the tiles found by warp 3, ahead, that took 8 192 rows over 32 experts, 2 048 × 2 048, from 52.2 to
+// 48.1 µs in 8 bits and 72 to 65.6 in bf16.
 #include "group_gemm.cuh"
 
 #include <algorithm>
@@ -24,17 +27,16 @@ constexpr int kThreads = 384, kEpiWarps = 8;
 constexpr unsigned kWaitCode = 0x68000000u;
 constexpr int CH = 256, COLS = CH / 2, BLOCKS = CH / 128;   // channels of a tile, of a summing warp; blocks that share a scale of W
 constexpr int SLOTS = 512 / CH;
-// 8 bits: a finished tile lies in shared memory as a whole, so that no summing thread waits for the store of another's part.  bf16: its two halves one behind the other,
-// for a fifth stage (4 096 × 4 096 × 4 096 107 → 101 µs).
+constexpr int kTileRing = 4;                      // tiles that are known ahead
+constexpr int kPiece = 32 * 64;                   // of a summing warp: 32 rows of 32 finished channels
 template <bool F8>
 struct Wide {
   static constexpr int group = F8 ? 1 : 2;        // CTAs to a tile
   static constexpr int w_rows = CH / group, w_bytes = w_rows * 128, stage = kXBytes + w_bytes;
-  static constexpr int stages = F8 ? 3 : 5;
+  static constexpr int stages = F8 ? 4 : 6;
   static constexpr int lag = 4, ahead = F8 ? 2 * SLOTS + 1 + lag : 0;   // blocks of factors that are asked for ahead, and kept: see group_gemm.cu
-  static constexpr int out_parts = F8 ? 1 : 2, out_ch = CH / out_parts, out_ld = out_ch * 2 + 16;   // bytes from row to row: eight rows meet all banks
   static constexpr int ring = stages * stage;
-  static constexpr int tables = 1024 + ring + kRows * out_ld + ahead * BLOCKS * kRows * 4 + 512;
+  static constexpr int tables = 1024 + ring + kEpiWarps * kPiece + ahead * BLOCKS * kRows * 4 + 512;
   static constexpr int smem(int experts) { return tables + Groups::bytes(experts); }
 };
 // A thread that sums 8-bit products holds 128 sums: the four warps that hold none give registers up.
@@ -49,6 +51,24 @@ __device__ __forceinline__ void loaded(uint32_t (&r)[32]) {
   asm volatile("" : B200_R8(16), B200_R8(24));
 }
 
+// 32 channels of `rows` rows — as many as there are of 32 —, from a warp's piece → y
+__device__ __forceinline__ void store_piece(__nv_bfloat16* out, const uint8_t* piece, int rows, int width, const GemmArgs& p, int lane) {
+  if (p.wide) {
+    const int c = lane & 3, row0 = lane >> 2;
+    uint4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint4*>(piece + (row0 + 8 * j) * 64 + (c ^ (row0 >> 1 & 3)) * 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (row0 + 8 * j < rows && 8 * c < width) *reinterpret_cast<uint4*>(out + (int64_t)(row0 + 8 * j) * p.n + 8 * c) = v[j];
+  } else {   // a lane's channel of every row
+    if (lane >= width) return;
+#pragma unroll 8
+    for (int r = 0; r < min(rows, 32); ++r)
+      out[(int64_t)r * p.n + lane] = *reinterpret_cast<const __nv_bfloat16*>(piece + r * 64 + ((lane >> 3 ^ (r >> 1 & 3)) * 16) + (lane & 7) * 2);
+  }
+}
+
 template <bool F8>
 __global__ void __launch_bounds__(kThreads, 1)
 group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const GemmArgs p) {
@@ -58,15 +78,16 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* const sx = smem;                                                        // [stages][128 rows × 128 bytes]
   uint8_t* const sw = smem + ST * kXBytes;                                         // this CTA's rows of W alike
-  uint8_t* const done_tile = smem + F::ring;                                       // [128][out_ld]: bf16
-  float* const factors = reinterpret_cast<float*>(done_tile + kRows * F::out_ld);  // [AHEAD][blocks][128]: of a block of channels, of a row
+  uint8_t* const pieces = smem + F::ring;                                          // [summing warps][32][32]: bf16
+  float* const factors = reinterpret_cast<float*>(pieces + kEpiWarps * kPiece);    // [AHEAD][blocks][128]: of a block of channels, of a row
   uint64_t* const full = reinterpret_cast<uint64_t*>(factors + AHEAD * F_SLOT);    // [stages], CTA 0's count the pair's bytes
   uint64_t* const empty = full + ST;
   uint64_t* const sums_full = empty + ST;                                          // [slots]
   uint64_t* const sums_empty = sums_full + SLOTS;                                  // CTA 0's
-  uint64_t* const out_full = sums_empty + SLOTS;
-  uint64_t* const out_empty = out_full + 1;                                        // [parts]
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(out_empty + F::out_parts);
+  uint64_t* const tile_full = sums_empty + SLOTS;                                  // [tile ring]
+  uint64_t* const tile_empty = tile_full + kTileRing;
+  int4* const tile_ring = reinterpret_cast<int4*>(tile_empty + kTileRing);
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(tile_ring + kTileRing);
   float* const w_scale = reinterpret_cast<float*>(tmem_slot + 1);                  // [AHEAD][blocks]
   Groups groups(reinterpret_cast<int*>(smem + F::tables - 1024), p.experts);
   const int warp = uniform((int)threadIdx.x / 32), lane = threadIdx.x % 32;
@@ -84,8 +105,10 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
       mbar_init(&sums_full[a], F8 ? 2 : 1);   // products done, factors there
       mbar_init(&sums_empty[a], GROUP * kEpiWarps);
     }
-    mbar_init(out_full, kEpiWarps / F::out_parts);
-    for (int part = 0; part < F::out_parts; ++part) mbar_init(&out_empty[part], 1);
+    for (int i = 0; i < kTileRing; ++i) {
+      mbar_init(&tile_full[i], 1);
+      mbar_init(&tile_empty[i], kEpiWarps + (F8 ? 2 : 1));
+    }
     fence_mbar_init();
   }
   if (warp == 1) tmem_alloc<GROUP>(tmem_slot, 512);
@@ -103,22 +126,31 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
     int64_t row0;             // of this CTA
     int rows, ch0, expert;    // rows of this CTA: none where the tile ends in the pair's first half
   };
-  int e = 0;                  // the group of this warp's last tile
-  auto tile_at = [&](int t) {   // a group's row tiles first: its rows of W stay in L2
-    int local, row_tiles;
-    groups.walk(t, p.ch_tiles, e, local, row_tiles);
-    const int row = local % row_tiles * (GROUP * kRows) + rank * kRows;
-    return Tile{(int64_t)groups.froms[e] + row, max(0, min(kRows, groups.counts[e] - row)), local / row_tiles * CH, e};
+  // This CTA's tiles, as warp 3 finds them: a search and three divisions take some 1 500 cycles, in which a summing warp would let both slots fill.
+  int at_ring = 0;
+  uint32_t ring_ph = 0;
+  Tile tile{};
+  auto next_tile = [&]() {   // of a whole warp
+    if (!(ok = warp_wait(&tile_full[at_ring], ring_ph, p.err, kWaitCode | 6))) return false;
+    const int4 v = tile_ring[at_ring];
+    tile = Tile{v.x, v.y, v.z, v.w};
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&tile_empty[at_ring]);
+    if (++at_ring == kTileRing) {
+      at_ring = 0;
+      ring_ph ^= 1;
+    }
+    return true;
   };
 
   if (warp < 4) {
     if constexpr (F8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
     if (warp == 0) {
-      if (lane == 0) {
-        int s = 0;
-        uint32_t ph = 1;
-        for (int t = first; t < tiles && ok; t += step) {
-          const Tile tile = tile_at(t);
+      int s = 0;
+      uint32_t ph = 1;
+      for (int t = first; t < tiles && ok; t += step) {
+        if (!next_tile()) break;
+        if (lane == 0) {
           const int x_row = (int)tile.row0, w_row = tile.expert * p.n + tile.ch0 + rank * F::w_rows;   // (what lies past the operands is zero)
           for (int kb = 0; kb < k_blocks; ++kb) {
             if (!(ok = wait_asleep(&empty[s], ph, p.err, kWaitCode | 1))) break;
@@ -139,8 +171,10 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
             }
           }
         }
-        if (!ok) drain_async();
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+        __syncwarp();
       }
+      if (lane == 0 && !ok) drain_async();
     } else if (warp == 1) {
       if (GROUP == 1 || rank == 0) {
         const uint32_t x0 = desc_lo(smem_u32(sx)), w0 = desc_lo(smem_u32(sw)), idesc = idesc_of(F8, GROUP * kRows, CH), lead = elect_one();
@@ -175,12 +209,10 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
     } else if (warp == 2) {
       if constexpr (F8) {   // as in group_gemm.cu, which says why the ring is never written where it is read
         const int64_t units = first < tiles ? (int64_t)((tiles - first + step - 1) / step) * k_blocks : 0;
-        int t = first;
         int kb = 0, into = 0, from_slot = 0, slot = 0;
         uint32_t ph = 1;
-        Tile tile{};
         auto ask = [&]() {
-          if (kb == 0) tile = tile_at(t);
+          if (kb == 0 && !next_tile()) return false;
           const float* const from = p.sx + (int64_t)kb * p.rows + tile.row0 + lane;
           float* const to = factors + into * F_SLOT + lane;
 #pragma unroll
@@ -188,15 +220,13 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
             if (lane + 32 * i < tile.rows) cp_async4(to + 32 * i, from + 32 * i);
           if (lane < BLOCKS)
             cp_async4(&w_scale[BLOCKS * into + lane], p.sw + ((int64_t)tile.expert * p.ch_blocks + min(tile.ch0 / 128 + lane, p.ch_blocks - 1)) * k_blocks + kb);
-          if (++kb == k_blocks) {
-            kb = 0;
-            t += step;
-          }
+          if (++kb == k_blocks) kb = 0;
           if (++into == AHEAD) into = 0;
+          return true;
         };
         for (int64_t u = -F::lag; u < units; ++u) {
           if (u >= 0 && !(ok = warp_wait(&sums_full[slot], ph, p.err, kWaitCode | 4))) break;
-          if (u + F::lag < units) ask();
+          if (u + F::lag < units && !ask()) break;
           cp_async_commit();
           if (u >= 0) {
             cp_async_wait<F::lag>();
@@ -221,18 +251,22 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         cp_async_wait<0>();
       }
     } else {
-      uint32_t ph = 0;
-      for (int t = first; t < tiles; t += step, ph ^= 1) {
-        const Tile tile = tile_at(t);
-#pragma unroll
-        for (int part = 0; part < F::out_parts && ok; ++part) {
-          if (!(ok = warp_wait(out_full, ph, p.err, kWaitCode | 6))) break;
-          const int ch = tile.ch0 + part * F::out_ch;
-          store_tile<F::out_ch / 8>(p.y + tile.row0 * p.n + ch, done_tile, F::out_ld, tile.rows, min(F::out_ch, p.n - ch), p, lane);
-          if (lane == 0) mbar_arrive(&out_empty[part]);
-          if (part + 1 < F::out_parts) ph ^= 1;
+      uint32_t ph = 1;
+      int e = 0;   // the group of the last tile
+      for (int t = first; t < tiles; t += step) {
+        int local, row_tiles;
+        groups.walk(t, p.ch_tiles, e, local, row_tiles);   // a group's row tiles first: its rows of W stay in L2
+        const int row = local % row_tiles * (GROUP * kRows) + rank * kRows;
+        const int4 v = make_int4(groups.froms[e] + row, max(0, min(kRows, groups.counts[e] - row)), local / row_tiles * CH, e);
+        if (!(ok = warp_wait(&tile_empty[at_ring], ph, p.err, kWaitCode | 7))) break;
+        if (lane == 0) {
+          tile_ring[at_ring] = v;
+          mbar_arrive(&tile_full[at_ring]);
         }
-        if (!ok) break;
+        if (++at_ring == kTileRing) {
+          at_ring = 0;
+          ph ^= 1;
+        }
       }
       zero_other_rows(p, lane);
     }
@@ -240,12 +274,13 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
     if constexpr (F8) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsMany));
     const int quad = warp & 3, half = (warp - 4) >> 2, row = quad * 32 + lane;
     const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + half * COLS, free_bar = GROUP == 2 ? mapa_u32(smem_u32(sums_empty), 0) : 0;
-    uint8_t* const put_at = done_tile + row * F::out_ld + (F8 ? half * COLS * 2 : 0);
+    uint8_t* const piece = pieces + (warp - 4) * kPiece;
+    const int swizzle = lane >> 1 & 3;   // rows' sixteen bytes change places: eight lanes meet all banks, writing and reading
     const float* const my_factors = factors + half * kRows + row;
     int slot = 0, fslot = 0;
-    uint32_t slot_ph = 0, out_ph = 1;
-    for (int t = first; t < tiles; t += step, out_ph ^= 1) {
-      const Tile tile = tile_at(t);
+    uint32_t slot_ph = 0;
+    for (int t = first; t < tiles; t += step) {
+      if (!next_tile()) break;
       const bool mine = quad * 32 < tile.rows;   // some row of this warp is one
       auto release = [&]() {   // the slot may be filled again
         tc_fence_before();
@@ -259,13 +294,26 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
           slot_ph ^= 1;
         }
       };
-      // channels 8j … 8j + 7 of this half
-      auto put8 = [&](int j, float2 a, float2 b, float2 c, float2 d) {
-        *reinterpret_cast<uint4*>(put_at + 16 * j) = make_uint4(pack2(a.x, a.y), pack2(b.x, b.y), pack2(c.x, c.y), pack2(d.x, d.y));
-      };
-      auto bias_of = [&](int j) {   // of channels 2j, 2j + 1
-        const int ch = tile.ch0 + half * COLS + 2 * j;
-        return make_float2(ch < p.n ? bf16_to_f(p.bias[ch]) : 0.f, ch + 1 < p.n ? bf16_to_f(p.bias[ch + 1]) : 0.f);
+      // A row's next 32 channels, from those of this half that `i` counts by 32, as pairs → y: through shared memory, for stores of 64 bytes.
+      auto put = [&](int i, auto pair_at) {
+        const int ch0 = tile.ch0 + half * COLS + 32 * i;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t v[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            float2 f = pair_at(4 * j + c);
+            if (p.bias != nullptr) {
+              const int ch = ch0 + 8 * j + 2 * c;
+              f = make_float2(f.x + (ch < p.n ? bf16_to_f(p.bias[ch]) : 0.f), f.y + (ch + 1 < p.n ? bf16_to_f(p.bias[ch + 1]) : 0.f));
+            }
+            v[c] = pack2(f.x, f.y);
+          }
+          *reinterpret_cast<uint4*>(piece + lane * 64 + (j ^ swizzle) * 16) = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+        __syncwarp();
+        store_piece(p.y + (tile.row0 + quad * 32) * p.n + ch0, piece, tile.rows - quad * 32, p.n - ch0, p, lane);
+        __syncwarp();
       };
       if constexpr (F8) {
         constexpr int PIECES = COLS / 32;
@@ -313,45 +361,27 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
             if (++fslot == AHEAD) fslot = 0;
           }
         }
-        if (!ok || !(ok = warp_wait(out_empty, out_ph, p.err, kWaitCode | 7))) break;
+        if (!ok) break;
         if (mine) {
-          if (p.bias != nullptr) {
 #pragma unroll
-            for (int j = 0; j < COLS / 2; ++j) {
-              const float2 v = halves(acc[j]), b = bias_of(j);
-              acc[j] = pair_of(v.x + b.x, v.y + b.y);
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < COLS / 8; ++j) put8(j, halves(acc[4 * j]), halves(acc[4 * j + 1]), halves(acc[4 * j + 2]), halves(acc[4 * j + 3]));
+          for (int i = 0; i < PIECES; ++i) put(i, [&](int j) { return halves(acc[16 * i + j]); });
         }
       } else {
         if (!(ok = warp_wait(&sums_full[slot], slot_ph, p.err, kWaitCode | 5))) break;
         tc_fence_after();
-        // the first half waits for the store of the last tile's second half, the second half for that of the first
-        if (!(ok = warp_wait(&out_empty[1 - half], half == 0 ? out_ph : out_ph ^ 1, p.err, kWaitCode | 7))) break;
         if (mine) {
 #pragma unroll 1
           for (int i = 0; i < COLS / 32; ++i) {
             uint32_t d[32];
             tmem_ld32(from + slot * CH + 32 * i, d);
             loaded(d);
-            auto two = [&](int j) {
-              float2 v = make_float2(__uint_as_float(d[2 * j]), __uint_as_float(d[2 * j + 1]));
-              if (p.bias != nullptr) {
-                const float2 b = bias_of(16 * i + j);
-                v = make_float2(v.x + b.x, v.y + b.y);
-              }
-              return v;
-            };
-#pragma unroll
-            for (int j = 0; j < 4; ++j) put8(4 * i + j, two(4 * j), two(4 * j + 1), two(4 * j + 2), two(4 * j + 3));
+            if (i + 1 == COLS / 32) release();
+            put(i, [&](int j) { return make_float2(__uint_as_float(d[2 * j]), __uint_as_float(d[2 * j + 1])); });
           }
+        } else {
+          release();
         }
-        release();
       }
-      __syncwarp();   // this warp's part of the tile lies in shared memory
-      if (lane == 0) mbar_arrive(out_full);
     }
   }
   tc_fence_before();
