@@ -9,9 +9,9 @@
 //   warp 0   TMA: of every 128 bytes of k 128 rows of W and the tile's rows of x, into a ring of shared memory
 //   warp 1   one thread issues four products (K = 32 bytes) per 128 bytes
 //   warp 2   8 bits: the products of x's and W's scales, NT of them for each block of 128 entries, fetched some blocks ahead
-//   warp 3   takes finished tiles from shared memory to y, beside the next tile's products; rows of no group are zeroed
+//   warp 3   finds the CTA's tiles; rows of no group are zeroed
 //   warps 4 … 11   the sums: a warp has a quarter of the channels and half of the rows, as fragments of 8 × 8 (lane 4r + c: channel r, rows 2c and 2c + 1), so
-//            that a lane needs a quarter of the factors and a transposing store to shared memory makes rows of y of them
+//            that a lane needs a quarter of the factors and a transposing store to shared memory makes rows of y of them, which the warp stores
 // 8 bits: W has a scale for 128 × 128 entries and x one for 128 entries of a row, so that 128 entries of k meet one factor per row of x, and the sums of 128
 // entries — a slot of tensor memory each — are scaled and added in fp32 registers; two to four slots keep the tensor cores running meanwhile.
 // bf16: a slot holds the sums over all of k.
@@ -28,7 +28,6 @@ namespace {
 
 constexpr int kCh = 128, kWBytes = kCh * 128, kThreads = 384, kEpiWarps = 8;
 constexpr int kMaxSplits = 8;
-constexpr int kOutLd = kCh * 2 + 16;       // bytes from row to row of a finished tile: eight rows meet all banks
 constexpr int kPartLd = kCh + 4;            // floats from row to row of a partial tile: a fragment's lanes meet 32 banks
 constexpr unsigned kWaitCode = 0x67000000u;
 
@@ -44,7 +43,7 @@ struct Form {
   static constexpr int f_slot = NT < 32 ? 32 : NT;
   static constexpr int cols = NT / 2;                  // rows of x of a summing warp
   static constexpr int ring = stages * stage;
-  static constexpr int out_bytes = NT * kPartLd * 4;   // a finished tile in bf16, or what the CTAs of a cluster send of theirs in fp32
+  static constexpr int out_bytes = NT * kPartLd * 4;   // a finished tile in bf16, the warps' pieces one behind the other, or what the CTAs of a cluster send of theirs in fp32
   static constexpr int tables = 1024 + ring + out_bytes + ahead * f_slot * 4 + 512;
   static constexpr int smem(int experts) { return tables + Groups::bytes(experts); }
   static constexpr int tmem(int slots) { return slots * NT < 32 ? 32 : slots * NT; }
@@ -87,12 +86,6 @@ __device__ __forceinline__ void store_transposed(uint32_t addr, uint32_t a, uint
 }
 // where the factor of row j of a tile lies: a lane that holds rows 8i + 2c, + 1 finds those of four i side by side
 __device__ __forceinline__ int factor_at(int j) { return (j & ~31) + (j % 8 / 2) * 8 + (j % 32 / 8) * 2 + j % 2; }
-// Which rows and channels a tile has.  Tiles run over the row tiles of a group first (its matrix's rows stay in L2), then over channels, then over groups.
-struct Tile {
-  int64_t row0;
-  int rows, ch0, expert;
-};
-
 template <bool F8, int NT>
 __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
                                                                                const GemmArgs p) {
@@ -102,15 +95,14 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* const sx = smem + ST * kWBytes;
-  uint8_t* const done_tile = smem + F::ring;                                       // [NT][kOutLd]: bf16
+  uint8_t* const done_tile = smem + F::ring;
   float* const factors = reinterpret_cast<float*>(done_tile + F::out_bytes);       // [AHEAD][NT]
   uint64_t* const full = reinterpret_cast<uint64_t*>(factors + AHEAD * F::f_slot);   // [stages], a pair's first CTA's
   uint64_t* const empty = full + ST;
   uint64_t* const sums_full = empty + ST;                                          // [slots]
   uint64_t* const sums_empty = sums_full + 4;                                      // a pair's first CTA's
-  uint64_t* const out_full = sums_empty + 4;                                       // of the finished tile
-  uint64_t* const out_empty = out_full + 1;
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(out_empty + 1);
+  TileRing ring(sums_empty + 4);
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(sums_empty + 4) + TileRing::bytes / 4;
   int* const gave_up = reinterpret_cast<int*>(tmem_slot + 1);
   int* const gave_up_of = gave_up + 1;                                                // [splits]
   float* const w_scale = reinterpret_cast<float*>(gave_up_of + kMaxSplits);                       // [AHEAD]
@@ -130,8 +122,7 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
       mbar_init(&sums_full[a], F8 ? 2 : 1);   // products done, factors there
       mbar_init(&sums_empty[a], kEpiWarps);
     }
-    mbar_init(out_full, kEpiWarps);
-    mbar_init(out_empty, 1);
+    ring.init(kEpiWarps + (F8 ? 3 : 2));
     fence_mbar_init();
     *gave_up = 0;
   }
@@ -147,23 +138,17 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
   const int tiles = groups.ends[p.experts - 1] * p.ch_tiles;
   const int first = blockIdx.x / p.splits, step = p.splits > 1 ? max(tiles, 1) : (int)gridDim.x;   // a cluster that splits k takes one tile
   const int kb0 = (int)((int64_t)p.k_blocks * split / p.splits), kb1 = (int)((int64_t)p.k_blocks * (split + 1) / p.splits);
-  int group = 0;   // of this warp's last tile
-  auto tile_at = [&](int t) {
-    int local, row_tiles;
-    groups.walk(t, p.ch_tiles, group, local, row_tiles);
-    const int e = group, count = groups.counts[e];
-    const int i = local % row_tiles, each = ((count + row_tiles - 1) / row_tiles + 15) / 16 * 16;   // alike, and none is empty
-    return Tile{groups.froms[e] + (int64_t)i * each, min(each, count - i * each), local / row_tiles * kCh, e};
-  };
+  Tile tile{};
+  auto next_tile = [&]() { return ok = ring.take(tile, lane, p.err, kWaitCode | 6); };
   auto up16 = [](int v) { return (v + 15) / 16 * 16; };
 
   if (warp < 4) {
     if (warp == 0) {
-      if (lane == 0) {
-        int s = 0;
-        uint32_t ph = 1;
-        for (int t = first; t < tiles && ok; t += step) {
-          const Tile tile = tile_at(t);
+      int s = 0;
+      uint32_t ph = 1;
+      for (int t = first; t < tiles && ok; t += step) {
+        if (!next_tile()) break;
+        if (lane == 0) {
           const int row0 = (int)tile.row0;
           const int boxes = (tile.rows + F::box - 1) / F::box, w_row = tile.expert * p.n + tile.ch0;
           for (int kb = kb0; kb < kb1; ++kb) {
@@ -179,15 +164,17 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
             }
           }
         }
-        if (!ok) drain_async();
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0);
       }
+      if (lane == 0 && !ok) drain_async();
     } else if (warp == 1) {
       const uint32_t w0 = desc_lo(smem_u32(smem)), x0 = desc_lo(smem_u32(sx)), lead = elect_one();
       int s = 0, slot = 0;
       uint32_t ph = 0, slot_ph = 1;
       bool ready = false;   // the next stage and slot, looked at behind the products of this one
       for (int t = first; t < tiles && ok; t += step) {
-        const uint32_t idesc = uniform(idesc_of(F8, kCh, up16(tile_at(t).rows)));
+        if (!next_tile()) break;
+        const uint32_t idesc = uniform(idesc_of(F8, kCh, up16(tile.rows)));
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!ready) {
             if (!(ok = warp_wait(&sums_empty[slot], slot_ph, p.err, kWaitCode | 2))) break;
@@ -222,27 +209,23 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
         // front of that one any more: a ring of 2·SLOTS + 1 + LAG units is never written where it is read.
         constexpr int PER = (NT + 31) / 32;
         const int64_t units = first < tiles ? (int64_t)((tiles - first + step - 1) / step) * (kb1 - kb0) : 0;
-        int t = first;
         int kb = kb0, into = 0, from_slot = 0, slot = 0;
         uint32_t ph = 1;
-        Tile tile{};
         auto ask = [&]() {
-          if (kb == kb0) tile = tile_at(t);
+          if (kb == kb0 && !next_tile()) return false;
           const float* const from = p.sx + (int64_t)kb * p.rows + tile.row0 + lane;
           float* const to = factors + into * F::f_slot + factor_at(lane);
 #pragma unroll
           for (int i = 0; i < PER; ++i)
             if (lane + 32 * i < tile.rows) cp_async4(to + 32 * i, from + 32 * i);
           if (lane == 0) cp_async4(&w_scale[into], p.sw + ((int64_t)tile.expert * p.ch_blocks + min(tile.ch0 / kCh, p.ch_blocks - 1)) * p.k_blocks + kb);
-          if (++kb == kb1) {
-            kb = kb0;
-            t += step;
-          }
+          if (++kb == kb1) kb = kb0;
           if (++into == AHEAD) into = 0;
+          return true;
         };
         for (int64_t u = -LAG; u < units; ++u) {
           if (u >= 0 && !(ok = warp_wait(&sums_full[slot], ph, p.err, kWaitCode | 4))) break;
-          if (u + LAG < units) ask();
+          if (u + LAG < units && !ask()) break;
           cp_async_commit();
           if (u >= 0) {
             cp_async_wait<LAG>();
@@ -263,26 +246,25 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
         cp_async_wait<0>();
       }
     } else if (warp == 3) {
-      if (p.splits == 1) {
-        uint32_t ph = 0;
-        for (int t = first; t < tiles; t += step, ph ^= 1) {
-          const Tile tile = tile_at(t);
-          if (!(ok = warp_wait(out_full, ph, p.err, kWaitCode | 6))) break;
-          store_tile<kCh / 8>(p.y + tile.row0 * p.n + tile.ch0, done_tile, kOutLd, tile.rows, min(kCh, p.n - tile.ch0), p, lane);
-          if (lane == 0) mbar_arrive(out_empty);
-        }
+      int e = 0;   // the group of the last tile
+      for (int t = first; t < tiles && ok; t += step) {
+        int local, row_tiles;
+        groups.walk(t, p.ch_tiles, lane, e, local, row_tiles);   // a group's row tiles first: its rows of W stay in L2
+        const int count = groups.counts[e], channels = row_tiles == 1 ? local : local / row_tiles, i = local - channels * row_tiles;
+        const int each = row_tiles == 1 ? count : ((count + row_tiles - 1) / row_tiles + 15) / 16 * 16;   // alike, and none is empty
+        ok = ring.give(groups.froms[e] + i * each, min(each, count - i * each), channels * kCh, e, lane, p.err, kWaitCode | 7);
       }
       zero_other_rows(p, lane);
     }
   } else {
     const int quad = warp & 3, half = (warp - 4) >> 2, r = lane / 4, c = lane % 4;
     const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + half * COLS;
-    // lane 8m + i of a transposing store: row i, channels 8m … 8m + 7 of 32
-    const uint32_t put_at = smem_u32(done_tile) + (half * COLS + lane % 8) * kOutLd + quad * 64 + lane / 8 * 16;
+    uint8_t* const piece = done_tile + (warp - 4) * (COLS * 64);
+    const uint32_t put_at = smem_u32(piece) + piece_at(lane % 8, lane / 8);   // lane 8m + i of a transposing store: row i, channels 8m … 8m + 7 of 32
     int slot = 0, fslot = 0;
-    uint32_t slot_ph = 0, out_ph = 1;
-    for (int t = first; t < tiles; t += step, out_ph ^= 1) {
-      const Tile tile = tile_at(t);
+    uint32_t slot_ph = 0;
+    for (int t = first; t < tiles; t += step) {
+      if (!next_tile()) break;
       const int mine = tile.rows - half * COLS;   // rows of this half
       const int ch0 = tile.ch0 + quad * 32;
       float bias[4];
@@ -298,14 +280,15 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
             part[8 * e + kPartLd] = v[e].y;
           }
         } else {
-          store_transposed(put_at + j * kOutLd, pack2(v[0].x + bias[0], v[0].y + bias[0]), pack2(v[1].x + bias[1], v[1].y + bias[1]),
+          store_transposed(put_at + j * 64, pack2(v[0].x + bias[0], v[0].y + bias[0]), pack2(v[1].x + bias[1], v[1].y + bias[1]),
                            pack2(v[2].x + bias[2], v[2].y + bias[2]), pack2(v[3].x + bias[3], v[3].y + bias[3]));
         }
       };
-      auto finished = [&]() {   // this warp's part of the tile lies in shared memory
+      auto store = [&]() {
         if (p.splits > 1) return;
         __syncwarp();
-        if (lane == 0) mbar_arrive(out_full);
+        store_piece(p.y + (tile.row0 + half * COLS) * p.n + ch0, piece, min(mine, COLS), p.n - ch0, p, lane);
+        __syncwarp();
       };
       auto release = [&]() {   // the slot may be filled again
         tc_fence_before();
@@ -372,18 +355,16 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
           if (++fslot == AHEAD) fslot = 0;
         }
         if (!ok) break;
-        if (p.splits == 1 && !(ok = warp_wait(out_empty, out_ph, p.err, kWaitCode | 7))) break;
 #pragma unroll
         for (int g = 0; g < COLS / 8; ++g)
           if (8 * g < mine) {
             float2 v[4] = {halves(acc[g][0]), halves(acc[g][1]), halves(acc[g][2]), halves(acc[g][3])};
             put8(8 * g, v);
           }
-        finished();
+        store();
       } else {
         if (!(ok = warp_wait(&sums_full[slot], slot_ph, p.err, kWaitCode | 5))) break;
         tc_fence_after();
-        if (p.splits == 1 && !(ok = warp_wait(out_empty, out_ph, p.err, kWaitCode | 7))) break;
 #pragma unroll 1
         for (int j = 0; j < COLS && j < mine; j += PIECE) {
           uint32_t a[PIECE / 2], b[PIECE / 2];
@@ -405,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
             }
         }
         if (mine <= 0) release();
-        finished();
+        store();
       }
     }
   }
@@ -417,8 +398,8 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
     // Every row has an owner among the CTAs, which get their rows of everybody's partial tile (a warp a row, a lane four channels) and sum them in order.
     // Reading them from the others instead took a round trip and a second meeting, 1.4 µs of 17.
     const int owned = NT / p.splits;
-    group = 0;
-    const Tile tile = first < tiles ? tile_at(first) : Tile{0, 0, 0, 0};
+    const int4 only = first < tiles ? ring.tiles[0] : make_int4(0, 0, 0, 0);
+    tile = Tile{only.x, only.y, only.z, only.w};
     cluster_wait();   // all CTAs have started
     for (int row = warp; row < tile.rows; row += kThreads / 32) {
       const int owner = row / owned;

@@ -154,21 +154,66 @@ struct Groups {
     }
   }
   // The group e that tile t is one of — its row tiles times ch_tiles tiles — from the group of a tile in front of it; local: its number there, row_tiles: how many
-  // row tiles the group has.  (A call has fewer than 2^31 tiles.)
-  __device__ __forceinline__ void walk(int t, int ch_tiles, int& e, int& local, int& row_tiles) const {
-    const int at = t / ch_tiles;
-    if (ends[e] <= at) {   // ends[e − 1] ≤ at < ends[e]
-      int lo = min(e + 1, experts - 1), hi = experts - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (ends[mid] > at) hi = mid;
-        else lo = mid + 1;
+  // row tiles the group has.  Of a whole warp.  (A call has fewer than 2^31 tiles.)
+  __device__ __forceinline__ void walk(int t, int ch_tiles, int lane, int& e, int& local, int& row_tiles) const {
+    int before = 0;
+    if (experts > 1) {
+      const int at = t / ch_tiles;
+      for (int from = e; from < experts; from += 32) {   // ends[e − 1] ≤ at < ends[e]
+        const unsigned past = __ballot_sync(0xffffffffu, from + lane < experts && ends[from + lane] > at);
+        if (past != 0) {
+          e = from + __ffs(past) - 1;
+          break;
+        }
       }
-      e = lo;
+      before = e > 0 ? ends[e - 1] : 0;
     }
-    const int before = e > 0 ? ends[e - 1] : 0;
     row_tiles = ends[e] - before;
     local = t - before * ch_tiles;
+  }
+};
+// A CTA's tiles, which one warp finds ahead of those that work on them: a search and divisions take 1 000 cycles and more, in which a summing warp would let its slots fill.
+struct Tile {
+  int64_t row0;
+  int rows, ch0, expert;
+};
+struct TileRing {
+  static constexpr int places = 4, bytes = places * 32;
+  uint64_t *full, *empty;
+  int4* tiles;
+  int at = 0;
+  uint32_t ph = 0;
+  __device__ __forceinline__ TileRing(void* room) : full((uint64_t*)room), empty(full + places), tiles((int4*)(empty + places)) {}
+  __device__ __forceinline__ void init(int takers) {
+    for (int i = 0; i < places; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], takers);
+    }
+  }
+  __device__ __forceinline__ void step() {
+    if (++at == places) {
+      at = 0;
+      ph ^= 1;
+    }
+  }
+  // both of a whole warp
+  __device__ __forceinline__ bool give(int row0, int rows, int ch0, int expert, int lane, unsigned* err, unsigned code) {
+    if (!warp_wait(&empty[at], ph ^ 1, err, code)) return false;
+    if (lane == 0) {
+      tiles[at] = make_int4(row0, rows, ch0, expert);
+      mbar_arrive(&full[at]);
+    }
+    step();
+    return true;
+  }
+  __device__ __forceinline__ bool take(Tile& tile, int lane, unsigned* err, unsigned code) {
+    if (!warp_wait(&full[at], ph, err, code)) return false;
+    const int4 v = tiles[at];
+    tile = Tile{v.x, v.y, v.z, v.w};
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[at]);
+    step();
+    return true;
   }
 };
 // rows in front of the first group and behind the last, by one warp of every CTA
@@ -183,46 +228,24 @@ __device__ __forceinline__ void zero_other_rows(const GemmArgs& p, int lane) {
       for (int i = lane; i < p.n; i += 32) out[i] = f_to_bf16(0.f);
   }
 }
-// A finished tile of LANES·8 channels in shared memory, rows `ld` bytes apart → y, by one warp, sixteen bytes a lane where rows of y take them.  Shared memory may
-// be written again afterwards.  (A bulk copy to a row took the copy engine 3 µs for 128 rows of 256 bytes.)
-template <int LANES>
-__device__ __forceinline__ void store_tile(__nv_bfloat16* out, const uint8_t* tile, int ld, int rows, int width, const GemmArgs& p, int lane) {
+// A summing warp stores what it summed itself, through a piece of shared memory of rows × 32 channels in bf16, for stores of 64 bytes.  A row's sixteen bytes c lie at
+// piece_at: eight lanes meet all banks, writing and reading.
+__device__ __forceinline__ int piece_at(int row, int c) { return row * 64 + (c ^ (row >> 1 & 3)) * 16; }
+__device__ __forceinline__ void store_piece(__nv_bfloat16* out, const uint8_t* piece, int rows, int width, const GemmArgs& p, int lane) {
   if (p.wide) {
-    constexpr int U = 8, SIDE = 32 / LANES;   // rows side by side
-    const int i = lane % LANES * 8;
-    for (int row0 = lane / LANES; row0 - lane / LANES < rows; row0 += U * SIDE) {
-      uint4 v[U];
+    const int c = lane & 3;
+    for (int row0 = lane >> 2; row0 < rows; row0 += 32) {
+      uint4 v[4];
 #pragma unroll
-      for (int j = 0; j < U; ++j) v[j] = *reinterpret_cast<const uint4*>(tile + min(row0 + j * SIDE, rows - 1) * ld + i * 2);
+      for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint4*>(piece + piece_at(min(row0 + 8 * j, rows - 1), c));
 #pragma unroll
-      for (int j = 0; j < U; ++j)
-        if (row0 + j * SIDE < rows && i < width) *reinterpret_cast<uint4*>(out + (int64_t)(row0 + j * SIDE) * p.n + i) = v[j];
+      for (int j = 0; j < 4; ++j)
+        if (row0 + 8 * j < rows && 8 * c < width) *reinterpret_cast<uint4*>(out + (int64_t)(row0 + 8 * j) * p.n + 8 * c) = v[j];
     }
-  } else {   // a lane takes four channels, eight rows at a time, in pieces that n allows
-    const int piece = p.n % 4 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 7) == 0 ? 4 : p.n % 2 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 3) == 0 ? 2 : 1;
-    for (int i = lane * 4; i < width; i += 128)
-      for (int row0 = 0; row0 < rows; row0 += 8) {
-        uint2 v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const uint2*>(tile + min(row0 + j, rows - 1) * ld + i * 2);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          __nv_bfloat16* const to = out + (int64_t)(row0 + j) * p.n + i;
-          if (row0 + j >= rows) continue;
-          if (piece == 4) {   // (n ends on such a piece)
-            *reinterpret_cast<uint2*>(to) = v[j];
-          } else if (piece == 2) {
-            *reinterpret_cast<uint32_t*>(to) = v[j].x;
-            if (i + 2 < width) *reinterpret_cast<uint32_t*>(to + 2) = v[j].y;
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (i + e < width) reinterpret_cast<uint16_t*>(to)[e] = (uint16_t)((e < 2 ? v[j].x : v[j].y) >> (e % 2 * 16));
-          }
-        }
-      }
+  } else if (lane < width) {   // a lane has a channel of every row
+#pragma unroll 8
+    for (int r = 0; r < rows; ++r) out[(int64_t)r * p.n + lane] = *reinterpret_cast<const __nv_bfloat16*>(piece + piece_at(r, lane >> 3) + (lane & 7) * 2);
   }
-  __syncwarp();
 }
 #endif
 

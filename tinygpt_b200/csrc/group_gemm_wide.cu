@@ -27,7 +27,6 @@ constexpr int kThreads = 384, kEpiWarps = 8;
 constexpr unsigned kWaitCode = 0x68000000u;
 constexpr int CH = 256, COLS = CH / 2, BLOCKS = CH / 128;   // channels of a tile, of a summing warp; blocks that share a scale of W
 constexpr int SLOTS = 512 / CH;
-constexpr int kTileRing = 4;                      // tiles that are known ahead
 constexpr int kPiece = 32 * 64;                   // of a summing warp: 32 rows of 32 finished channels
 template <bool F8>
 struct Wide {
@@ -51,24 +50,6 @@ __device__ __forceinline__ void loaded(uint32_t (&r)[32]) {
   asm volatile("" : B200_R8(16), B200_R8(24));
 }
 
-// 32 channels of `rows` rows — as many as there are of 32 —, from a warp's piece → y
-__device__ __forceinline__ void store_piece(__nv_bfloat16* out, const uint8_t* piece, int rows, int width, const GemmArgs& p, int lane) {
-  if (p.wide) {
-    const int c = lane & 3, row0 = lane >> 2;
-    uint4 v[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const uint4*>(piece + (row0 + 8 * j) * 64 + (c ^ (row0 >> 1 & 3)) * 16);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (row0 + 8 * j < rows && 8 * c < width) *reinterpret_cast<uint4*>(out + (int64_t)(row0 + 8 * j) * p.n + 8 * c) = v[j];
-  } else {   // a lane's channel of every row
-    if (lane >= width) return;
-#pragma unroll 8
-    for (int r = 0; r < min(rows, 32); ++r)
-      out[(int64_t)r * p.n + lane] = *reinterpret_cast<const __nv_bfloat16*>(piece + r * 64 + ((lane >> 3 ^ (r >> 1 & 3)) * 16) + (lane & 7) * 2);
-  }
-}
-
 template <bool F8>
 __global__ void __launch_bounds__(kThreads, 1)
 group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const GemmArgs p) {
@@ -84,10 +65,8 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
   uint64_t* const empty = full + ST;
   uint64_t* const sums_full = empty + ST;                                          // [slots]
   uint64_t* const sums_empty = sums_full + SLOTS;                                  // CTA 0's
-  uint64_t* const tile_full = sums_empty + SLOTS;                                  // [tile ring]
-  uint64_t* const tile_empty = tile_full + kTileRing;
-  int4* const tile_ring = reinterpret_cast<int4*>(tile_empty + kTileRing);
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(tile_ring + kTileRing);
+  TileRing ring(sums_empty + SLOTS);
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(sums_empty + SLOTS) + TileRing::bytes / 4;
   float* const w_scale = reinterpret_cast<float*>(tmem_slot + 1);                  // [AHEAD][blocks]
   Groups groups(reinterpret_cast<int*>(smem + F::tables - 1024), p.experts);
   const int warp = uniform((int)threadIdx.x / 32), lane = threadIdx.x % 32;
@@ -105,10 +84,7 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
       mbar_init(&sums_full[a], F8 ? 2 : 1);   // products done, factors there
       mbar_init(&sums_empty[a], GROUP * kEpiWarps);
     }
-    for (int i = 0; i < kTileRing; ++i) {
-      mbar_init(&tile_full[i], 1);
-      mbar_init(&tile_empty[i], kEpiWarps + (F8 ? 2 : 1));
-    }
+    ring.init(kEpiWarps + (F8 ? 2 : 1));
     fence_mbar_init();
   }
   if (warp == 1) tmem_alloc<GROUP>(tmem_slot, 512);
@@ -122,26 +98,8 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
   const uint32_t tmem = uniform(*tmem_slot);
   const int tiles = groups.ends[p.experts - 1] * p.ch_tiles, first = blockIdx.x / GROUP, step = gridDim.x / GROUP;
   const int k_blocks = p.k_blocks;
-  struct Tile {
-    int64_t row0;             // of this CTA
-    int rows, ch0, expert;    // rows of this CTA: none where the tile ends in the pair's first half
-  };
-  // This CTA's tiles, as warp 3 finds them: a search and three divisions take some 1 500 cycles, in which a summing warp would let both slots fill.
-  int at_ring = 0;
-  uint32_t ring_ph = 0;
-  Tile tile{};
-  auto next_tile = [&]() {   // of a whole warp
-    if (!(ok = warp_wait(&tile_full[at_ring], ring_ph, p.err, kWaitCode | 6))) return false;
-    const int4 v = tile_ring[at_ring];
-    tile = Tile{v.x, v.y, v.z, v.w};
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&tile_empty[at_ring]);
-    if (++at_ring == kTileRing) {
-      at_ring = 0;
-      ring_ph ^= 1;
-    }
-    return true;
-  };
+  Tile tile{};   // row0 and rows of this CTA: none where the tile ends in the pair's first half
+  auto next_tile = [&]() { return ok = ring.take(tile, lane, p.err, kWaitCode | 6); };
 
   if (warp < 4) {
     if constexpr (F8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
@@ -251,22 +209,12 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         cp_async_wait<0>();
       }
     } else {
-      uint32_t ph = 1;
       int e = 0;   // the group of the last tile
-      for (int t = first; t < tiles; t += step) {
+      for (int t = first; t < tiles && ok; t += step) {
         int local, row_tiles;
-        groups.walk(t, p.ch_tiles, e, local, row_tiles);   // a group's row tiles first: its rows of W stay in L2
-        const int row = local % row_tiles * (GROUP * kRows) + rank * kRows;
-        const int4 v = make_int4(groups.froms[e] + row, max(0, min(kRows, groups.counts[e] - row)), local / row_tiles * CH, e);
-        if (!(ok = warp_wait(&tile_empty[at_ring], ph, p.err, kWaitCode | 7))) break;
-        if (lane == 0) {
-          tile_ring[at_ring] = v;
-          mbar_arrive(&tile_full[at_ring]);
-        }
-        if (++at_ring == kTileRing) {
-          at_ring = 0;
-          ph ^= 1;
-        }
+        groups.walk(t, p.ch_tiles, lane, e, local, row_tiles);   // a group's row tiles first: its rows of W stay in L2
+        const int channels = row_tiles == 1 ? local : local / row_tiles, row = (local - channels * row_tiles) * (GROUP * kRows) + rank * kRows;
+        ok = ring.give(groups.froms[e] + row, max(0, min(kRows, groups.counts[e] - row)), channels * CH, e, lane, p.err, kWaitCode | 7);
       }
       zero_other_rows(p, lane);
     }
@@ -275,7 +223,6 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
     const int quad = warp & 3, half = (warp - 4) >> 2, row = quad * 32 + lane;
     const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + half * COLS, free_bar = GROUP == 2 ? mapa_u32(smem_u32(sums_empty), 0) : 0;
     uint8_t* const piece = pieces + (warp - 4) * kPiece;
-    const int swizzle = lane >> 1 & 3;   // rows' sixteen bytes change places: eight lanes meet all banks, writing and reading
     const float* const my_factors = factors + half * kRows + row;
     int slot = 0, fslot = 0;
     uint32_t slot_ph = 0;
@@ -294,7 +241,7 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
           slot_ph ^= 1;
         }
       };
-      // A row's next 32 channels, from those of this half that `i` counts by 32, as pairs → y: through shared memory, for stores of 64 bytes.
+      // channels 32i … 32i + 31 of this half, as pairs, → y
       auto put = [&](int i, auto pair_at) {
         const int ch0 = tile.ch0 + half * COLS + 32 * i;
 #pragma unroll
@@ -309,10 +256,10 @@ group_wide_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
             }
             v[c] = pack2(f.x, f.y);
           }
-          *reinterpret_cast<uint4*>(piece + lane * 64 + (j ^ swizzle) * 16) = make_uint4(v[0], v[1], v[2], v[3]);
+          *reinterpret_cast<uint4*>(piece + piece_at(lane, j)) = make_uint4(v[0], v[1], v[2], v[3]);
         }
         __syncwarp();
-        store_piece(p.y + (tile.row0 + quad * 32) * p.n + ch0, piece, tile.rows - quad * 32, p.n - ch0, p, lane);
+        store_piece(p.y + (tile.row0 + quad * 32) * p.n + ch0, piece, min(32, tile.rows - quad * 32), p.n - ch0, p, lane);
         __syncwarp();
       };
       if constexpr (F8) {
