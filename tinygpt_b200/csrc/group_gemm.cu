@@ -477,32 +477,36 @@ int launch(const GroupProduct& g, GemmArgs& p, int splits, cudaStream_t st) {
   return B200_OK;
 }
 
-// Rows of a tile (16 to 128 here, or a tile of group_gemm_wide.cu) and CTAs to a tile: what the whole call is estimated to take, in µs.  A CTA needs 0.25 (16 rows) to
-// 0.5 µs (128) for 128 bytes of k, a wide one 0.53 (bf16 0.38 a pair); two CTAs on an SM 1.45 times that each; partial tiles that meet cost 1 µs and more.  Measured:
-// one of each in the way that is taken and, in brackets, the next best: 200 × 4 096 × 14 336 33 µs in tiles of 128 rows and two CTAs to each (64, wide), 512 × 4 096 × 14 336
-// 56 in tiles of 128 (64, wide), 768 rows 66 wide (101, 128), 100 × 28 672 × 4 096 30 wide (39, 128), 48 × 4 096 × 4 096 10.7 with 32 (11.6, 64), 512 × 1 152 × 896 8.3 with 32 (12.8,
-// wide), 1 × 4 096 × 4 096 9.1 with four CTAs to a tile (13.9, one; 9.2, eight).
+// Rows of a tile (16 to 128 here, or a tile of group_gemm_wide.cu) and CTAs to a tile: what the whole call is estimated to take, in µs.  W cannot come faster than
+// memory gives it; a CTA needs 0.25 (16 rows) to 0.5 µs (128) for 128 bytes of k, a wide one 0.49 (bf16 0.38 a pair), and something for a tile's end; two CTAs on an SM 1.45
+// times that each; partial tiles that meet cost 2 to 4.5 µs.  The rates are fitted to 189 calls — 1 to 4 096 rows, up to 20 000 over 8 to 64 experts, seven and five
+// matrices — in all the forms that can run: 13 of those calls take more than 5 % longer than in the best form, the worst 12 %.  For one of each, the way that is taken and,
+// in brackets, others: 200 × 4 096 × 14 336 33 µs in tiles of 128 rows and two CTAs to each (37, 64 and two; 42, 64 and four), 512 × 4 096 × 14 336 53 with 128 (55, wide), 768 × 4 096 × 4 096 22 wide
+// (34, 128), 512 × 2 048 × 2 048 11.1 with 64 (12.0, 32; 12.3, 128), 1 × 896 × 4 864 7.0 with eight CTAs to a tile (8.0, four).
 struct Way {
   int rows, splits;   // rows 0: wide
 };
 Way choose(const GroupProduct& g, bool f8) {
   auto up = [](double a, double b) { return std::ceil(a / b); };
   const double groups = g.starts ? (double)std::min<int64_t>(g.experts, g.rows) : 1, average = (double)g.rows / groups;
-  const double k_blocks = up((double)g.k, f8 ? 128 : 64);
-  // groups are unlike: half of a last tile is empty on average, and no group has less than a tile
-  auto row_tiles = [&](int rows) { return g.starts ? groups * std::max(1.0, average / rows + 0.5) : up(average, rows); };
+  const double k_blocks = up((double)g.k, f8 ? 128 : 64), stream = groups * (double)g.n * (double)g.k * (f8 ? 1 : 2) / 6.8e6;
+  // groups are unlike: four tenths of a last tile are empty on average, and no group has less than a tile
+  auto row_tiles = [&](int rows) { return g.starts ? groups * std::max(1.0, average / rows + 0.4) : up(average, rows); };
   Way best{0, 1};
   // wide: a CTA of 128 rows in 8 bits, a pair of 256 in bf16
-  double least = f8 && g.experts > kWideExperts8 ? 1e30 : 7.5 + up(row_tiles(f8 ? 128 : 256) * up((double)g.n, 256), f8 ? 148 : 74) * (k_blocks * (f8 ? 0.53 : 0.38) + 1.2);
+  double least = f8 && g.experts > kWideExperts8
+                     ? 1e30
+                     : 5.0 + std::max(stream, up(row_tiles(f8 ? 128 : 256) * up((double)g.n, 256), f8 ? 148 : 74) * (k_blocks * (f8 ? 0.49 : 0.38) + 1.35));
   for (int rows = 16; rows <= 128; rows *= 2) {
-    const double tiles = row_tiles(rows) * up((double)g.n, kCh), each = (f8 ? 0.22 : 0.19) + (f8 ? 0.0021 : 0.0012) * std::min<double>(rows, average);
+    const double tiles = row_tiles(rows) * up((double)g.n, kCh), each = (f8 ? 0.24 : 0.25) + (f8 ? 0.0021 : 0.0009) * std::min<double>(rows, average);
     for (int splits = 1; splits <= kMaxSplits && (splits == 1 || k_blocks >= 2 * splits); splits *= 2) {
       constexpr int kOne[4] = {148, 74, 33, 15}, kTwo[4] = {296, 148, 70, 32};   // clusters that the SMs hold at once
       const int i = splits == 1 ? 0 : splits == 2 ? 1 : splits == 4 ? 2 : 3;
       const double share = rows <= 64 && tiles * splits > 148 ? 1.45 : 1.0;
       const int hold = rows <= 64 ? kTwo[i] : kOne[i];
       if (splits > 1 && (g.starts ? (g.rows / rows + groups) * up((double)g.n, kCh) : tiles) > hold) break;   // (a cluster that comes later starts from nothing)
-      const double us = 5.5 + (splits > 1 ? 1.0 + 0.35 * splits : 0.0) + up(tiles, hold) * up(k_blocks, splits) * each * share;
+      const double us =
+          4.9 + (splits > 1 ? 1.2 + 0.3 * splits + 0.008 * rows : 0.0) + std::max(stream, up(tiles, hold) * (up(k_blocks, splits) * each * share + 0.6));
       if (us < least) {
         least = us;
         best = Way{rows, splits};
