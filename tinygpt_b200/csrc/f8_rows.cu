@@ -40,7 +40,7 @@ __device__ __forceinline__ void store8(uint8_t* q, float* scale, int64_t row, in
 enum RowsKind { kList, kSilu, kTo };
 // g / (1 + exp(−g)) within 2^-22 of it: exp2 of the product's rounded part, and what was rounded off it to first order; below 2^-119 it may be 0
 // (a power past 2^126 is that, and what is then rounded off it is positive: no infinity meets a negative factor).  The quotient and
-// expf of silu_f cost twice the instructions, and a product of 8 192 × 1 024 17 µs.
+// expf of silu_f take a product of 8 192 × 1 024 from 12.5 to 16.5 µs.
 __device__ __forceinline__ float silu_fast(float g) {
   const float p = fminf(g * -1.44269504f, 126.f), rest = fmaf(g, -1.44269504f, -p) + g * -1.92596303e-8f;   // −log2 e in two parts
   float e, r;
