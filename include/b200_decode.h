@@ -207,7 +207,7 @@ int b200_f8_rows_bf16(void* q, float* scale, const void* x, int64_t ld_x, int64_
 /* z = x, or bf16(x + residual), which goes to `sum` (it may lie where x or the residual does); t = z·w (fp32; w NULL: 1); scale = s·rsqrt(mean(z²) + eps). */
 int b200_rmsnorm_f8(void* q, float* scale, void* sum_or_null, const void* x, const void* residual_or_null, const void* w_or_null, int64_t rows, int64_t dim,
                     float eps, void* stream);
-/* gate_up rows are [gate(n) | up(n)], bf16; t = silu(gate)·up in fp32; scale = s. */
+/* gate_up rows are [gate(n) | up(n)], bf16; t = silu(gate)·up in fp32 (a silu below 2^-119 may be 0); scale = s. */
 int b200_silu_mul_f8(void* q, float* scale, const void* gate_up, int64_t rows, int64_t n, void* stream);
 /* out[rows, k] = value·scale, fp32. */
 int b200_f8_rows_dequant(float* out, const void* q, const float* scale, int64_t rows, int64_t k, void* stream);

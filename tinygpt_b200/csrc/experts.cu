@@ -12,7 +12,7 @@ namespace {
 // A stable counting sort by one CTA, or by a cluster of eight where there are many pairs: every warp takes a run of the pairs, 32 at a time in their order.
 // Lanes that hold the same expert find each other (ballots of its bits), so a warp's count of an expert is its own and no atomics decide an order.
 //   1. counts[warp][e];  2. the sum in front of each: experts first, then CTAs, then warps;  3. the runs again, each pair to its place
-// Bound by latencies and by the instructions of the SMs that it has: 8 192 pairs on one took 10 µs.
+// Bound by latencies and by the instructions of the SMs that it has: 8 192 pairs take 5.4 µs with eight, 12.6 with one.
 constexpr int kOrderWarps = 32, kOrderThreads = 32 * kOrderWarps, kOrderCtas = 8;
 constexpr int kOrderKept = 16384;   // choices of a CTA that are kept in shared memory, the others are read twice
 
