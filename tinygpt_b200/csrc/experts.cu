@@ -203,16 +203,17 @@ int check_pairs(const char* what, int64_t rows, int64_t top, int64_t experts) {
 
 }  // namespace
 
+static int order_bytes(int64_t experts, int64_t kept) { return (int)(kOrderWarps * (experts | 1) + 2 * experts + std::min<int64_t>(kept, kOrderKept)) * 4; }
+
 int launch_expert_order(int32_t* starts, int32_t* source, int32_t* place, const int32_t* chosen, int64_t rows, int64_t top, int64_t experts, cudaStream_t st) {
   const int64_t pairs = rows * top, ctas = pairs > 2 * kOrderThreads ? kOrderCtas : 1;
   const int64_t run = (pairs + ctas * kOrderThreads - 1) / (ctas * kOrderThreads) * 32;
   static PerDevice attrs;
-  auto bytes = [](int64_t e, int64_t n) { return (kOrderWarps * (e | 1) + 2 * e + std::min<int64_t>(n, kOrderKept)) * 4; };
-  B200_CUDA(attrs([&] { return cudaFuncSetAttribute(expert_order_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes(kMaxExperts, kOrderKept)); }));
+  B200_CUDA(attrs([] { return cudaFuncSetAttribute(expert_order_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, order_bytes(kMaxExperts, kOrderKept)); }));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)ctas);
   cfg.blockDim = dim3(kOrderThreads);
-  cfg.dynamicSmemBytes = (size_t)bytes(experts, run * kOrderWarps);
+  cfg.dynamicSmemBytes = (size_t)order_bytes(experts, run * kOrderWarps);
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
