@@ -226,6 +226,9 @@ int b200_f8_linear_bf16(void* y, const void* q, const float* scale, const b200_f
 /* Rows starts[e] … starts[e + 1] − 1 meet W[e] (starts int32 [experts + 1] on the device, not falling; none, or any number of rows to an expert); rows in front of the first
  * group and behind the last are zeros in y.  Up to 1 024 experts. */
 int b200_f8_grouped_bf16(void* y, const void* q, const float* scale, const b200_f8_weight* w, const int32_t* starts, int64_t rows, void* stream);
+/* b200_f8_rows_bf16 of x bf16 [rows, k] into q and scale, and one of these two over them; W begins to be read while the rows are made. */
+int b200_f8_linear_of_bf16(void* y, void* q, float* scale, const void* x, const b200_f8_weight* w, const void* bias_or_null, int64_t rows, void* stream);
+int b200_f8_grouped_of_bf16(void* y, void* q, float* scale, const void* x, const b200_f8_weight* w, const int32_t* starts, int64_t rows, void* stream);
 /* The same over x bf16 [rows, k] and w bf16 [experts, n, k], k % 8 == 0, 16-byte aligned. */
 int b200_grouped_bf16(void* y, const void* x, const void* w, const int32_t* starts, int64_t rows, int64_t experts, int64_t n, int64_t k, void* stream);
 

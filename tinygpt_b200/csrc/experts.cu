@@ -282,10 +282,10 @@ int b200_experts_f8_bf16(void* out, const void* x, const int32_t* chosen, const 
   auto floats = [&](int64_t at) { return (float*)(ws + at); };
   if ((rc = launch_expert_order(ints(s.starts), ints(s.source), ints(s.place), chosen, rows, top, experts, st)) != B200_OK) return rc;
   if ((rc = launch_f8_rows_to(ws + s.q, floats(s.scale), x, ints(s.place), rows, top, pairs, width, st)) != B200_OK) return rc;
-  if ((rc = launch_group_product({ws + s.gate_up, ws + s.q, floats(s.scale), w_in->q, w_in->scale, ints(s.starts), nullptr, pairs, experts, 2 * ff, width}, st)) != B200_OK)
+  if ((rc = launch_group_product({ws + s.gate_up, ws + s.q, floats(s.scale), w_in->q, w_in->scale, ints(s.starts), nullptr, pairs, experts, 2 * ff, width, true}, st)) != B200_OK)
     return rc;
   if ((rc = launch_silu_mul_f8(ws + s.a, floats(s.a_scale), ws + s.gate_up, pairs, ff, st)) != B200_OK) return rc;
-  if ((rc = launch_group_product({ws + s.y, ws + s.a, floats(s.a_scale), w_out->q, w_out->scale, ints(s.starts), nullptr, pairs, experts, width, ff}, st)) != B200_OK)
+  if ((rc = launch_group_product({ws + s.y, ws + s.a, floats(s.a_scale), w_out->q, w_out->scale, ints(s.starts), nullptr, pairs, experts, width, ff, true}, st)) != B200_OK)
     return rc;
   return launch_expert_combine(out, ws + s.y, ints(s.place), weights, rows, top, width, st);
 }

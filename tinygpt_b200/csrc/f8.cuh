@@ -92,6 +92,9 @@ struct GroupProduct {
   const int32_t* starts;    // [experts + 1], or null: one group of all rows
   const void* bias;         // bf16 [n] or null
   int64_t rows, experts, n, k;
+  // In front in the stream is the kernel that makes x, launched by the same call, and it lets this one start when all that came before it is done: nothing but
+  // x and its scales has to be waited for.
+  bool x_in_front = false;
 };
 int launch_group_product(const GroupProduct& p, cudaStream_t st);
 

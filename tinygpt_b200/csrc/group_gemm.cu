@@ -128,8 +128,13 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
   }
   if (p.splits > 1) cluster_arrive_relaxed();
   if (warp == 1) tmem_alloc<1>(tmem_slot, TMEM);
-  pdl_wait();
-  pdl_trigger();
+  // Where the kernel in front only makes x: the groups and, of the first tile, as many blocks of W as there are stages come beside it.  48 × 4 096 × 14 336
+  // from bf16 rows 18.8 µs for 20.3, a layer of 32 experts over 8 rows 33.1 for 35.1.
+  const bool ahead = F8 && p.ahead;
+  if (!ahead) {
+    pdl_wait();
+    pdl_trigger();
+  }
   if (warp == 3) groups.make<NT>(p.starts, p.rows, lane);
   tc_fence_before();
   __syncthreads();
@@ -151,12 +156,22 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
         if (lane == 0) {
           const int row0 = (int)tile.row0;
           const int boxes = (tile.rows + F::box - 1) / F::box, w_row = tile.expert * p.n + tile.ch0;
-          for (int kb = kb0; kb < kb1; ++kb) {
-            if (!(ok = wait_asleep(&empty[s], ph, p.err, kWaitCode | 1))) break;
-            uint8_t *const w_to = smem + s * kWBytes, *const x_to = sx + s * F::x_bytes;
-            const int k0 = kb * (F8 ? 128 : 64);
+          auto ask_w = [&](int kb, int s) {
             mbar_arrive_expect_tx(&full[s], kWBytes + boxes * F::box * 128);
-            tma_load_2d(w_to, &tmap_w, k0, w_row, &full[s]);
+            tma_load_2d(smem + s * kWBytes, &tmap_w, kb * (F8 ? 128 : 64), w_row, &full[s]);
+          };
+          int asked = kb0;   // blocks of W in front of this one are on their way
+          if (ahead && t == first) {
+            for (; asked < kb1 && asked - kb0 < ST; ++asked) ask_w(asked, asked - kb0);
+            pdl_wait();
+          }
+          for (int kb = kb0; kb < kb1; ++kb) {
+            if (kb >= asked) {
+              if (!(ok = wait_asleep(&empty[s], ph, p.err, kWaitCode | 1))) break;
+              ask_w(kb, s);
+            }
+            uint8_t* const x_to = sx + s * F::x_bytes;
+            const int k0 = kb * (F8 ? 128 : 64);
             for (int b = 0; b < boxes; ++b) tma_load_2d(x_to + b * F::box * 128, &tmap_x, k0, row0 + b * F::box, &full[s]);
             if (++s == ST) {
               s = 0;
@@ -208,6 +223,10 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
         // phase before, unit u − SLOTS, is complete.  Then the products of that unit are done, so every warp has released unit u − 2·SLOTS and needs nothing of the units in
         // front of that one any more: a ring of 2·SLOTS + 1 + LAG units is never written where it is read.
         constexpr int PER = (NT + 31) / 32;
+        if (ahead) {
+          pdl_wait();
+          pdl_trigger();
+        }
         const int64_t units = first < tiles ? (int64_t)((tiles - first + step - 1) / step) * (kb1 - kb0) : 0;
         int kb = kb0, into = 0, from_slot = 0, slot = 0;
         uint32_t ph = 1;
@@ -254,6 +273,7 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
         const int each = row_tiles == 1 ? count : ((count + row_tiles - 1) / row_tiles + 15) / 16 * 16;   // alike, and none is empty
         ok = ring.give(groups.froms[e] + i * each, min(each, count - i * each), channels * kCh, e, lane, p.err, kWaitCode | 7);
       }
+      if (ahead) pdl_wait();
       zero_other_rows(p, lane);
     }
   } else {
@@ -396,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
   __syncthreads();
   if (p.splits > 1) {
     // Every row has an owner among the CTAs, which get their rows of everybody's partial tile (a warp a row, a lane four channels) and sum them in order.
-    // Reading them from the others instead takes a round trip and a second meeting: 48 × 4 096 × 14 336 21.1 µs where this took 20.6, its rows included.
+    // Reading them from the others instead takes a round trip and a second meeting: 48 × 4 096 × 14 336 from bf16 rows 0.5 µs more.
     const int owned = NT / p.splits;
     const int4 only = first < tiles ? ring.tiles[0] : make_int4(0, 0, 0, 0);
     tile = Tile{only.x, only.y, only.z, only.w};
@@ -544,6 +564,7 @@ int launch_group_product(const GroupProduct& g, cudaStream_t st) {
   p.experts = (int)g.experts;
   p.k_blocks = (int)(g.x_scale != nullptr ? f8_blocks(g.k) : (g.k + 63) / 64);
   p.wide = g.n % 8 == 0 && aligned16(g.y);
+  p.ahead = g.x_in_front;
   return g.x_scale != nullptr ? launch_for<true>(g, p, st) : launch_for<false>(g, p, st);
 }
 
@@ -576,6 +597,26 @@ int b200_f8_grouped_bf16(void* y, const void* q, const float* scale, const b200_
   B200_CHECK_ARG(w && scale && w->scale && starts, "f8_grouped: null pointer");
   if ((rc = check_product("f8_grouped", y, q, w->q, rows, w->experts, w->n, w->k)) != B200_OK) return rc;
   return launch_group_product({y, q, scale, w->q, w->scale, starts, nullptr, rows, w->experts, w->n, w->k}, (cudaStream_t)stream);
+}
+
+int b200_f8_linear_of_bf16(void* y, void* q, float* scale, const void* x, const b200_f8_weight* w, const void* bias, int64_t rows, void* stream) {
+  using namespace b200;
+  int rc = op_check();
+  if (rc != B200_OK) return rc;
+  B200_CHECK_ARG(x && w && scale && w->scale && w->experts == 1, "f8_linear_of: null pointer, or a weight of experts");
+  if ((rc = check_product("f8_linear_of", y, q, w->q, rows, 1, w->n, w->k)) != B200_OK) return rc;
+  if ((rc = launch_f8_rows(q, scale, x, w->k, rows, nullptr, rows, w->k, (cudaStream_t)stream)) != B200_OK) return rc;
+  return launch_group_product({y, q, scale, w->q, w->scale, nullptr, bias, rows, 1, w->n, w->k, true}, (cudaStream_t)stream);
+}
+
+int b200_f8_grouped_of_bf16(void* y, void* q, float* scale, const void* x, const b200_f8_weight* w, const int32_t* starts, int64_t rows, void* stream) {
+  using namespace b200;
+  int rc = op_check();
+  if (rc != B200_OK) return rc;
+  B200_CHECK_ARG(x && w && scale && w->scale && starts, "f8_grouped_of: null pointer");
+  if ((rc = check_product("f8_grouped_of", y, q, w->q, rows, w->experts, w->n, w->k)) != B200_OK) return rc;
+  if ((rc = launch_f8_rows(q, scale, x, w->k, rows, nullptr, rows, w->k, (cudaStream_t)stream)) != B200_OK) return rc;
+  return launch_group_product({y, q, scale, w->q, w->scale, starts, nullptr, rows, w->experts, w->n, w->k, true}, (cudaStream_t)stream);
 }
 
 int b200_grouped_bf16(void* y, const void* x, const void* w, const int32_t* starts, int64_t rows, int64_t experts, int64_t n, int64_t k, void* stream) {

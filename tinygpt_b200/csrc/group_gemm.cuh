@@ -14,6 +14,7 @@ struct GemmArgs {
   int64_t rows;
   int n, k_blocks, experts, ch_tiles, ch_blocks, splits;   // ch_tiles: of a tile's channels; ch_blocks: of 128 channels
   bool wide;    // y takes stores of 16 bytes
+  bool ahead;   // W, groups and bias may be read before the kernel in front is done
 };
 // tiles of 256 channels (group_gemm_wide.cu); in 8 bits for so many matrices
 constexpr int kWideExperts8 = 512;

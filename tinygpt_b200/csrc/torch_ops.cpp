@@ -28,7 +28,7 @@ namespace {
 #define B200_FUNCTIONS(F) \
   F(gemv_bf16) F(gemm_bf16) F(rmsnorm_bf16) F(silu_mul_bf16) F(add_bf16) F(attn_bf16) F(gemv_fused_bf16) F(attn_decode_workspace_bytes) F(attn_decode_bf16) F(w4_workspace_bytes) F(w4_linear_bf16) \
   F(kv4_store) F(kv4_load) F(kv4_attention_workspace_bytes) F(kv4_attention) F(kv4_extend) F(kv4_fork) F(kv4_free) F(kv4_compact) F(kv4_workspace_bytes) \
-  F(f8_rows_bf16) F(rmsnorm_f8) F(silu_mul_f8) F(f8_rows_dequant) F(f8_linear_bf16) F(f8_grouped_bf16) F(grouped_bf16) \
+  F(f8_rows_bf16) F(rmsnorm_f8) F(silu_mul_f8) F(f8_rows_dequant) F(f8_linear_bf16) F(f8_grouped_bf16) F(f8_linear_of_bf16) F(f8_grouped_of_bf16) F(grouped_bf16) \
   F(experts_f8_workspace_bytes) F(experts_f8_bf16)
 struct {
 #define B200_FIELD(f) decltype(&b200_##f) f;
@@ -487,15 +487,13 @@ struct F8In {
     rows = q->numel() / q->size(-1);
     return here(*q) && (scale == nullptr || (scale->size(0) == f8_blocks(k) && scale->size(1) == rows));
   }
-  // calls with 8-bit rows: the caller's, or made in scratch memory
-  template <typename F>
-  int with(void* st, F call) const {
-    if (scale != nullptr) return call(q->data_ptr(), static_cast<const float*>(scale->data_ptr()));
+  // calls `given` with the caller's 8-bit rows, or `of` with scratch memory for those of bf16 rows
+  template <typename F, typename G>
+  int with(F given, G of) const {
+    if (scale != nullptr) return given(q->data_ptr(), static_cast<const float*>(scale->data_ptr()));
     const int64_t bytes = (rows * f8_ld(k) + 255) / 256 * 256;
     const at::DataPtr ws = scratch(bytes + rows * f8_blocks(k) * 4);
-    float* const s = reinterpret_cast<float*>(static_cast<char*>(ws.get()) + bytes);
-    const int rc = abi.f8_rows_bf16(ws.get(), s, q->data_ptr(), k, rows, nullptr, rows, k, st);
-    return rc != 0 ? rc : call(ws.get(), s);
+    return of(ws.get(), reinterpret_cast<float*>(static_cast<char*>(ws.get()) + bytes), q->data_ptr());
   }
 };
 // q, scale, n, k of a weight of 8 bits, one matrix (experts 0) or many
@@ -542,7 +540,8 @@ PyObject* linear_f8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {   // x: 
       (b && (b->numel() != w.n || b->device() != x.q->device())))
     Py_RETURN_NONE;
   return run(*x.q, with_last(*x.q, w.n), [&](void* y, void* st) {
-    return x.with(st, [&](const void* q, const float* scale) { return abi.f8_linear_bf16(y, q, scale, &w, ptr(b), x.rows, st); });
+    return x.with([&](const void* q, const float* scale) { return abi.f8_linear_bf16(y, q, scale, &w, ptr(b), x.rows, st); },
+                  [&](void* q, float* scale, const void* from) { return abi.f8_linear_of_bf16(y, q, scale, from, &w, ptr(b), x.rows, st); });
   });
   END_HANDLE_TH_ERRORS
 }
@@ -555,7 +554,9 @@ PyObject* grouped_linear_f8(PyObject*, PyObject* const* a, Py_ssize_t n_args) { 
   if (n_args != 8 || modes() || !x.take(a) || x.q->dim() != 2 || !f8_weight(a + 3, *x.q, true, w) || !(starts = starts_of(a[7], *x.q, w.experts)) || w.k != x.k)
     Py_RETURN_NONE;
   return run(*x.q, {x.rows, w.n}, [&](void* y, void* st) {
-    return x.with(st, [&](const void* q, const float* scale) { return abi.f8_grouped_bf16(y, q, scale, &w, static_cast<const int32_t*>(starts->data_ptr()), x.rows, st); });
+    const auto* const s = static_cast<const int32_t*>(starts->data_ptr());
+    return x.with([&](const void* q, const float* scale) { return abi.f8_grouped_bf16(y, q, scale, &w, s, x.rows, st); },
+                  [&](void* q, float* scale, const void* from) { return abi.f8_grouped_of_bf16(y, q, scale, from, &w, s, x.rows, st); });
   });
   END_HANDLE_TH_ERRORS
 }

@@ -430,10 +430,11 @@ def f8_quantize(weight: torch.Tensor) -> F8Weight:
     """The nearest 8-bit weight of a matrix [n, k] or of matrices [experts, n, k] (bf16 or fp32): a block's largest entry becomes 448."""
     if weight.dim() not in (2, 3) or not weight.dtype.is_floating_point or weight.numel() == 0:
         raise B200Error(f"f8_quantize: expected matrices, got {weight.dtype} {tuple(weight.shape)}")
+    weight = weight.float()
     if not bool(torch.isfinite(weight).all()):
         raise B200Error("f8_quantize: the weight is not finite")
     *lead, n, k = weight.shape
-    w = torch.nn.functional.pad(weight.float(), (0, -k % F8_BLOCK, 0, -n % F8_BLOCK))
+    w = torch.nn.functional.pad(weight, (0, -k % F8_BLOCK, 0, -n % F8_BLOCK))
     w = w.view(*lead, _up(n, F8_BLOCK), F8_BLOCK, _up(k, F8_BLOCK), F8_BLOCK)
     top = w.abs().amax((-3, -1))
     scale = (top / torch.full_like(top, 448.0)).clamp(min=2.0 ** -126)
