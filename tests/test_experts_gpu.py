@@ -139,3 +139,24 @@ def test_layer_refusals_and_captures(built_lib):
     got = ops.experts_f8(x2, chosen, weights, w_in, w_out)
     keep = torch.tensor([0, 1, 2, 4, 5], device="cuda")
     assert bool(got[3].isnan().all()) and torch.equal(got[keep], ops.experts_f8(x, chosen, weights, w_in, w_out)[keep])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,top,experts,width,ff", [(700, 2, 4, 264, 256), (3000, 1, 3, 520, 128), (1500, 4, 32, 1000, 640), (2048, 4, 32, 512, 1024), (900, 2, 2, 136, 200)],
+                         ids=lambda v: str(v))
+def test_many_rows_are_the_steps(built_lib, rows, top, experts, width, ff):
+    """Layers over many rows: the bits of the calls one behind the other, with choices that are none, an expert without rows, and rows that are not finite."""
+    w_in, w_out = weight(2 * ff, width, experts, seed=1), weight(width, ff, experts, seed=2)
+    x = randn(rows, width, seed=3)
+    x[5, 7], x[rows - 1, 0], x[17] = float("inf"), float("nan"), 0.0
+    chosen = torch.randint(-1, experts, (rows, top), generator=gen(4), device="cuda", dtype=I32)
+    chosen[chosen == experts - 2] = experts - 1
+    weights = torch.rand(rows, top, generator=gen(5), device="cuda")
+    starts, source, place = ops.expert_order(chosen, experts)
+    a = ops.silu_mul_f8(ops.grouped_linear_f8(ops.f8_rows(x, source), w_in, starts))
+    want = ops.expert_combine(ops.grouped_linear_f8(a, w_out, starts), place, weights)
+    for _ in range(2):
+        got = ops.experts_f8(x, chosen, weights, w_in, w_out)
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
+    fine = got[6 : rows - 1]
+    assert bool(torch.isfinite(fine).all()) and bool((got[5].isnan() | (chosen[5] < 0).all()).all())
