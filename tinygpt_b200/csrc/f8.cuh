@@ -10,11 +10,38 @@ constexpr int64_t f8_blocks(int64_t k) { return (k + kF8Block - 1) / kF8Block; }
 constexpr int kMaxExperts = 1024;
 
 #ifdef __CUDACC__
+// two fp32 numbers in a 64-bit register: one instruction multiplies and adds both
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ uint64_t pair_of(uint32_t lo, uint32_t hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+  return v;
+}
+__device__ __forceinline__ float2 halves(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 // A block of 128 numbers t, eight a lane, in 8 bits.  `top`: the bits of their largest magnitude (as integers magnitudes order like numbers, and NaN comes out on top of
 // them all).  s = max(fp32(top / 448), 2^-126): never below the least normal number, so that its reciprocal is finite.  value = e4m3(fp32(t / s)), nearest with
 // ties to even, at most ±448; NaN stays.  With r = 1 / s, rounded, one correction of t·r is the quotient as a division rounds it (Markstein), as
 // long as nothing is infinite and no remainder falls below the normal numbers: blocks of tiny and of huge numbers divide.  Eight divisions a lane in all blocks
-// take the rows of 8 192 × 2 048 from 14.8 µs to 17.6.
+// take the rows of 8 192 × 2 048 from 14.3 µs to 17.6; corrections one by one instead of in pairs to 14.8.
 __device__ __forceinline__ uint2 f8_block(const float (&t)[8], uint32_t top, float& s) {
   constexpr float kR = 1.f / 448.f;
   const float m = __uint_as_float(top), a = m * kR;
@@ -27,10 +54,13 @@ __device__ __forceinline__ uint2 f8_block(const float (&t)[8], uint32_t top, flo
   float q[8];
   if (plain) {
     const float r = __frcp_rn(s);
+    const uint64_t rr = pair_of(r, r), minus_s = pair_of(-s, -s);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float v = t[e] * r;
-      q[e] = fmaf(fmaf(-v, s, t[e]), r, v);
+    for (int e = 0; e < 8; e += 2) {
+      const uint64_t tt = pair_of(t[e], t[e + 1]), v = mul_pair(tt, rr);
+      const float2 both = halves(fma_pair(fma_pair(v, minus_s, tt), rr, v));
+      q[e] = both.x;
+      q[e + 1] = both.y;
     }
   } else {
 #pragma unroll
