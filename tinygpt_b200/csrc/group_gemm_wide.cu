@@ -8,7 +8,7 @@
 // the issuing warp — and there is room for two; reading sums also holds the products up (a block's loads by 124 cycles), and x and W of 48 KB a block are
 // written to and read from shared memory in 768.  Tried and as slow or slower: pairs with 256 rows (32 KB a block; longer ways from CTA to CTA), four slots of 128
 // columns (the issue of four products alone takes 249 cycles), halves of a slot by themselves, sums in pairs or one by one, an earlier look at the next slot.
-// A pair in 8 bits ends groups in tiles of 256 rows: 2 048 rows with four of 32 experts each 159 µs for 143.
+// A pair in 8 bits ends groups in tiles of 256 rows: 2 048 rows with four of 32 experts each 146 µs for 125, and 4 096 × 4 096 × 4 096 82 for 75.
 // bf16: tensor memory sums over all of k; 4 096 × 4 096 × 4 096 93.5 µs (1.47 PFLOP/s).  A CTA by itself took 127 where a pair took 97.
 // A summing warp stores what it summed itself, 32 channels at a time through two kilobytes: with whole tiles handed to a storing warp the last one of a CTA came 5 µs
 // behind its sums, and their room is a stage of operands now.  With the tiles found by warp 3, ahead, that took 8 192 rows over 32 experts, 2 048 × 2 048, from 52.2 to
