@@ -2,7 +2,7 @@
 //
 // For bf16 and for 8 bits with scales, for one matrix (a Linear) and for many (experts, rows sorted by expert).  W is the A operand: a tile is 128 of its rows (channels) ×
 // up to NT rows of x, and the product's N is what the tile really holds, rounded up to 16.  So a group of three rows costs a stream of its matrix and little else, and a
-// group that ends inside a tile costs no idle rows.  Few rows are bound by that stream: one row × 28 672 × 4 096 in 8 bits 22.3 µs, 5.3 TB/s; launch, the first loads' way
+// group that ends inside a tile costs no idle rows.  Few rows are bound by that stream: one row × 28 672 × 4 096 in 8 bits 21.3 µs, 5.5 TB/s; launch, the first loads' way
 // and the end are 5 µs of any call.
 //
 // Warp-specialised, persistent over the tiles:
@@ -30,6 +30,10 @@ constexpr int kCh = 128, kWBytes = kCh * 128, kThreads = 384, kEpiWarps = 8;
 constexpr int kMaxSplits = 8;
 constexpr int kPartLd = kCh + 4;            // floats from row to row of a partial tile: a fragment's lanes meet 32 banks
 constexpr unsigned kWaitCode = 0x67000000u;
+// Blocks of W that are asked into L2 beside the kernel in front.  Behind a norm 16 × 6 144 × 4 096 take 12.1 µs for 12.5 without, 48 × 4 096 × 4 096 13.0 for 13.4, in a run of
+// its own 128 × 4 096 × 4 096 11.8 for 12.3 and 1 × 28 672 × 4 096 21.3 for 21.6 (1 × 4 096 × 14 336 15.2 for 14.9); more blocks compete with the running kernel's: with 16 and
+// 32 1 × 28 672 × 4 096 takes 22.6 and 25.1.
+constexpr int kWToL2 = 4;
 
 template <int NT>
 struct Form {
@@ -84,6 +88,10 @@ __device__ __forceinline__ void tmem_ready(uint32_t (&r)[16]) {
 __device__ __forceinline__ void store_transposed(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+// what a load at these coordinates would read, to L2
+__device__ __forceinline__ void tma_to_l2(const CUtensorMap* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
+}
 // where the factor of row j of a tile lies: a lane that holds rows 8i + 2c, + 1 finds those of four i side by side
 __device__ __forceinline__ int factor_at(int j) { return (j & ~31) + (j % 8 / 2) * 8 + (j % 32 / 8) * 2 + j % 2; }
 template <bool F8, int NT>
@@ -131,7 +139,13 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
   // Where the kernel in front only makes x: the groups and, of the first tile, as many blocks of W as there are stages come beside it.  48 × 4 096 × 14 336
   // from bf16 rows 18.8 µs for 20.3, a layer of 32 experts over 8 rows 33.1 for 35.1.
   const bool ahead = F8 && p.ahead;
+  const int first = blockIdx.x / p.splits;
+  const int kb0 = (int)((int64_t)p.k_blocks * split / p.splits), kb1 = (int)((int64_t)p.k_blocks * (split + 1) / p.splits);
   if (!ahead) {
+    if (p.starts == nullptr && threadIdx.x == 0) {   // rows that are given: W may be written by the kernel in front, but L2 has what is written
+      const int ch0 = first / (int)((p.rows + NT - 1) / NT) * kCh;
+      for (int kb = kb0; kb < kb1 && kb - kb0 < kWToL2 && ch0 < p.n; ++kb) tma_to_l2(&tmap_w, kb * 128, ch0);
+    }
     pdl_wait();
     pdl_trigger();
   }
@@ -141,8 +155,7 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
   tc_fence_after();
   const uint32_t tmem = uniform(*tmem_slot);
   const int tiles = groups.ends[p.experts - 1] * p.ch_tiles;
-  const int first = blockIdx.x / p.splits, step = p.splits > 1 ? max(tiles, 1) : (int)gridDim.x;   // a cluster that splits k takes one tile
-  const int kb0 = (int)((int64_t)p.k_blocks * split / p.splits), kb1 = (int)((int64_t)p.k_blocks * (split + 1) / p.splits);
+  const int step = p.splits > 1 ? max(tiles, 1) : (int)gridDim.x;   // a cluster that splits k takes one tile
   Tile tile{};
   auto next_tile = [&]() { return ok = ring.take(tile, lane, p.err, kWaitCode | 6); };
   auto up16 = [](int v) { return (v + 15) / 16 * 16; };
