@@ -101,3 +101,27 @@ def test_the_c_calls_over_bf16_rows(built_lib):
 def test_a_weight_too_large_for_fp32_is_refused():
     with pytest.raises(B200Error):
         ops.f8_quantize(torch.full((4, 4), 1e300, dtype=torch.float64))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(1, 1152, 896), (48, 4096, 1440), (100, 520, 304)], ids=lambda v: str(v))
+def test_given_rows_and_a_weight_written_in_front(built_lib, m, n, k):
+    """Rows that are given: the first blocks of W are asked into L2 while the kernel in front, which may write W, still runs."""
+    from tinygpt_b200._lib import check, lib
+    raw, rows = [randn(n, k, seed=20 + i) for i in range(6)], [ops.f8_rows(randn(m, k, seed=50 + i)) for i in range(6)]
+    now = ops.F8Weight(torch.empty(n, k, device="cuda", dtype=torch.uint8).view(rows[0].q.dtype), weight(n, k, seed=1).scale, n, k)
+    junk = torch.empty(-(-k // 128), n, device="cuda")
+    want = []
+    for r, x in zip(raw, rows):
+        w = now._replace(q=ops.f8_rows(r).q)
+        torch.cuda.synchronize()
+        want.append(ops.linear_f8(x, w))
+        torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for r, x in zip(raw, rows):
+            check(lib().b200_f8_rows_bf16(now.q.data_ptr(), junk.data_ptr(), r.data_ptr(), k, n, None, n, k, _stream()))
+            got.append(ops.linear_f8(x, now))
+    torch.cuda.synchronize()
+    for i, y in enumerate(got):
+        assert torch.equal(y, want[i % len(want)]), i
