@@ -410,6 +410,7 @@ def f8_pack(values: torch.Tensor, scale: torch.Tensor) -> F8Weight:
     """The layout linear_f8 takes, made once per weight: values float8_e4m3fn [n, k] or [experts, n, k], scale fp32, one for every block of 128 × 128."""
     if values.dim() not in (2, 3) or values.dtype != _F8:
         raise B200Error(f"f8_pack: values must be float8_e4m3fn [n, k] or [experts, n, k], got {values.dtype} {tuple(values.shape)}")
+    values, scale = values.detach(), scale.detach()
     *lead, n, k = values.shape
     if n < 1 or k < 1 or (lead and not 1 <= lead[0] <= MAX_EXPERTS):
         raise B200Error(f"f8_pack: W {tuple(values.shape)}: up to {MAX_EXPERTS} matrices, none of them empty")
@@ -430,7 +431,7 @@ def f8_quantize(weight: torch.Tensor) -> F8Weight:
     """The nearest 8-bit weight of a matrix [n, k] or of matrices [experts, n, k] (bf16 or fp32): a block's largest entry becomes 448."""
     if weight.dim() not in (2, 3) or not weight.dtype.is_floating_point or weight.numel() == 0:
         raise B200Error(f"f8_quantize: expected matrices, got {weight.dtype} {tuple(weight.shape)}")
-    weight = weight.float()
+    weight = weight.detach().float()   # (of a parameter: else its scales would keep the 32-bit copies below)
     if not bool(torch.isfinite(weight).all()):
         raise B200Error("f8_quantize: the weight is not finite")
     *lead, n, k = weight.shape
