@@ -473,6 +473,8 @@ def _f8_desc(w: F8Weight, what: str, dims: int):
     if w.q.dim() != dims:
         raise B200Error(f"{what}: takes {'one matrix' if dims == 2 else 'the matrices of experts'}, got values {tuple(w.q.shape)}")
     q, scale = _chk(w.q, f"{what}.q", _F8), _chk(w.scale, f"{what}.scale", torch.float32)
+    if q.data_ptr() % 16:
+        q = q.clone()
     return F8Desc(q.data_ptr(), scale.data_ptr(), w.n, w.k, experts), (q, scale)
 
 
