@@ -123,7 +123,7 @@ struct GroupProduct {
   const void* bias;         // bf16 [n] or null
   int64_t rows, experts, n, k;
   // In front in the stream is the kernel that makes x, launched by the same call, and it lets this one start when all that came before it is done: nothing but
-  // x and its scales has to be waited for.
+  // x and its scales has to be waited for.  What is read before that wait comes from L2 (W by TMA, groups and bias past L1).
   bool x_in_front = false;
 };
 int launch_group_product(const GroupProduct& p, cudaStream_t st);

@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
       const int ch0 = tile.ch0 + quad * 32;
       float bias[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) bias[e] = p.bias != nullptr && ch0 + r + 8 * e < p.n ? bf16_to_f(p.bias[ch0 + r + 8 * e]) : 0.f;
+      for (int e = 0; e < 4; ++e) bias[e] = p.bias != nullptr && ch0 + r + 8 * e < p.n ? bias_at(p.bias + ch0 + r + 8 * e) : 0.f;
       // Rows j … j + 7 of this half, 32 channels: v[e][i] is channel r + 8e, row j + 2c + i.
       auto put8 = [&](int j, float2 (&v)[4]) {
         if (p.splits > 1) {   // [row][channel] where the operands were: every product has read them
@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
     const int ch = tile.ch0 + 4 * lane;
     float bias[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) bias[j] = p.bias != nullptr && ch + j < p.n ? bf16_to_f(p.bias[ch + j]) : 0.f;
+    for (int j = 0; j < 4; ++j) bias[j] = p.bias != nullptr && ch + j < p.n ? bias_at(p.bias + ch + j) : 0.f;
     for (int i = warp; i < owned && !lost; i += kThreads / 32) {
       const int row = split * owned + i;
       if (row >= tile.rows) break;

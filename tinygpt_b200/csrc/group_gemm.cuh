@@ -99,6 +99,10 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsign
 // Arrives in another CTA.  What it tells is that tensor memory was read (the fence in front); no memory is handed over, so that no release at the cluster's
 // scope is needed, which takes some 700 cycles.
 __device__ __forceinline__ void arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// Groups and bias where the warp that reads them may not have waited for the kernel in front (`ahead`): whoever wrote them is done and L2 has what was written, so
+// they are read from there, past an L1 of which nothing is promised before the wait.
+__device__ __forceinline__ int start_at(const int32_t* p) { return __ldcg(p); }
+__device__ __forceinline__ float bias_at(const __nv_bfloat16* p) { return bf16_lo(__ldcg(reinterpret_cast<const unsigned short*>(p))); }
 template <bool B>
 struct Is {
   static constexpr bool value = B;
@@ -115,8 +119,8 @@ struct Groups {
     const int each = (experts + 31) / 32, e0 = min(lane * each, experts), e1 = min(e0 + each, experts);
     int mine = 0;
     for (int e = e0; e < e1; ++e) {
-      const int64_t from = starts == nullptr ? 0 : min(max((int64_t)starts[e], (int64_t)0), rows);
-      const int64_t count = starts == nullptr ? rows : max(min((int64_t)starts[e + 1], rows) - from, (int64_t)0);
+      const int64_t from = starts == nullptr ? 0 : min(max((int64_t)start_at(starts + e), (int64_t)0), rows);
+      const int64_t count = starts == nullptr ? rows : max(min((int64_t)start_at(starts + e + 1), rows) - from, (int64_t)0);
       froms[e] = (int)from;
       counts[e] = (int)count;
       mine += (int)((count + ROWS - 1) / ROWS);
