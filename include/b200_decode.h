@@ -41,8 +41,8 @@ extern "C" {
  * convolutions and per-head norms in front of any attention (fields appended to b200_attn_prep_desc and b200_pool_attn_desc),
  * gated feed-forwards in sandwich blocks;  10: + weights of 4 bits (b200_w4_*) and the paged cache of 4 bits (b200_kv4_*);
  * 11: + rows and weights of 8 bits (b200_f8_*, b200_rmsnorm_f8, b200_silu_mul_f8), products grouped by expert (b200_grouped_bf16) and routed experts
- * (b200_expert_*, b200_experts_f8_*).  All additive: callers of an older version keep working once they are compiled against this header. */
-#define B200_ABI_VERSION 11
+ * (b200_expert_*, b200_experts_f8_*);  12: + b200_product_way.  All additive: callers of an older version keep working once they are compiled against this header. */
+#define B200_ABI_VERSION 12
 
 typedef enum b200_status {
   B200_OK = 0,
@@ -231,6 +231,9 @@ int b200_f8_linear_of_bf16(void* y, void* q, float* scale, const void* x, const 
 int b200_f8_grouped_of_bf16(void* y, void* q, float* scale, const void* x, const b200_f8_weight* w, const int32_t* starts, int64_t rows, void* stream);
 /* The same over x bf16 [rows, k] and w bf16 [experts, n, k], k % 8 == 0, 16-byte aligned. */
 int b200_grouped_bf16(void* y, const void* x, const void* w, const int32_t* starts, int64_t rows, int64_t experts, int64_t n, int64_t k, void* stream);
+/* How such a product of these sizes is cut, by arithmetic on the host alone: rows of a tile of 128 channels (16, 32, 64 or 128; 0: tiles of 256 channels) and the CTAs that share a
+ * tile's k.  experts 0: one matrix, in 8 bits. */
+int b200_product_way(int64_t rows, int64_t experts, int64_t n, int64_t k, int32_t eight_bits, int32_t* tile_rows, int32_t* ctas);
 
 /* chosen int32 [rows, top] → the pairs in the order of their experts, an expert's in the order of the rows: starts [experts + 1], source [rows·top] (the row of every
  * pair; −1 behind the last), place [rows, top] (where a pair went).  A choice outside 0 … experts − 1 is no pair: place −1. */

@@ -186,6 +186,7 @@ PROTOTYPES = {
     "b200_f8_linear_of_bf16": (I32, [P, P, P, P, C.POINTER(F8Desc), P, I64, P]),
     "b200_f8_grouped_of_bf16": (I32, [P, P, P, P, C.POINTER(F8Desc), P, I64, P]),
     "b200_grouped_bf16": (I32, [P, P, P, P, I64, I64, I64, I64, P]),
+    "b200_product_way": (I32, [I64, I64, I64, I64, I32, C.POINTER(I32), C.POINTER(I32)]),
     "b200_expert_order": (I32, [P, P, P, P, I64, I64, I64, P]),
     "b200_expert_combine_bf16": (I32, [P, P, P, P, I64, I64, I64, P]),
     "b200_experts_f8_workspace_bytes": (I64, [I64, I64, I64, I64, I64]),

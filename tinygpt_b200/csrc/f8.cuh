@@ -127,6 +127,8 @@ struct GroupProduct {
   bool x_in_front = false;
 };
 int launch_group_product(const GroupProduct& p, cudaStream_t st);
+// rows of a tile (0: group_gemm_wide.cu's) and CTAs to a tile that such a call takes
+void group_way(const GroupProduct& g, bool f8, int32_t* rows, int32_t* splits);
 
 // ---- rows by expert and back (experts.cu)
 int launch_expert_order(int32_t* starts, int32_t* source, int32_t* place, const int32_t* chosen, int64_t rows, int64_t top, int64_t experts, cudaStream_t st);

@@ -563,6 +563,12 @@ int launch_for(const GroupProduct& g, GemmArgs& p, cudaStream_t st) {
 
 }  // namespace
 
+void group_way(const GroupProduct& g, bool f8, int32_t* rows, int32_t* splits) {
+  const Way way = choose(g, f8);
+  *rows = way.rows;
+  *splits = way.splits;
+}
+
 int launch_group_product(const GroupProduct& g, cudaStream_t st) {
   GemmArgs p{};
   const int rc = wait_word(&p.err);
@@ -585,12 +591,34 @@ int launch_group_product(const GroupProduct& g, cudaStream_t st) {
 
 extern "C" {
 
-static int check_product(const char* what, const void* y, const void* x, const void* w, int64_t rows, int64_t experts, int64_t n, int64_t k) {
+static int check_sizes(const char* what, int64_t rows, int64_t experts, int64_t n, int64_t k) {
   using namespace b200;
-  B200_CHECK_ARG(y && x && w && rows >= 1 && rows < 1 << 24, "%s: %lld rows out of range, or a null pointer", what, (long long)rows);
+  B200_CHECK_ARG(rows >= 1 && rows < 1 << 24, "%s: %lld rows out of range", what, (long long)rows);
   B200_CHECK_ARG(experts >= 1 && experts <= kMaxExperts && n >= 1 && n <= 1 << 20 && k >= 1 && k <= 1 << 24 && experts * n < 1ll << 31,
                  "%s: %lld matrices [%lld, %lld] out of range", what, (long long)experts, (long long)n, (long long)k);
+  return B200_OK;
+}
+static int check_product(const char* what, const void* y, const void* x, const void* w, int64_t rows, int64_t experts, int64_t n, int64_t k) {
+  using namespace b200;
+  const int rc = check_sizes(what, rows, experts, n, k);
+  if (rc != B200_OK) return rc;
+  B200_CHECK_ARG(y && x && w, "%s: null pointer", what);
   B200_CHECK_ARG(aligned16(x, w), "%s: x and the weight must be 16-byte aligned", what);
+  return B200_OK;
+}
+
+int b200_product_way(int64_t rows, int64_t experts, int64_t n, int64_t k, int32_t eight_bits, int32_t* tile_rows, int32_t* ctas) {
+  using namespace b200;
+  B200_CHECK_ARG(tile_rows && ctas && (experts != 0 || eight_bits), "product_way: null pointer, or one matrix in bf16");
+  const int rc = check_sizes("product_way", rows, experts == 0 ? 1 : experts, n, k);
+  if (rc != B200_OK) return rc;
+  GroupProduct g{};
+  g.rows = rows;
+  g.experts = experts == 0 ? 1 : experts;
+  g.n = n;
+  g.k = k;
+  g.starts = experts == 0 ? nullptr : tile_rows;   // (whether there are groups: no estimate reads them)
+  group_way(g, eight_bits != 0, tile_rows, ctas);
   return B200_OK;
 }
 
