@@ -204,10 +204,11 @@ int b200_w4_dequant_bf16(void* out, const b200_w4_weight* w, void* stream);
  * ---------------------------------------------------------------------------------------------------------------- */
 /* t = row index[i] of x (bf16 [x_rows], ld_x entries apart; index NULL: row i), zeros where the index is none of x_rows; scale = s. */
 int b200_f8_rows_bf16(void* q, float* scale, const void* x, int64_t ld_x, int64_t x_rows, const int32_t* index_or_null, int64_t rows, int64_t k, void* stream);
-/* z = x, or bf16(x + residual), which goes to `sum` (it may lie where x or the residual does); t = z·w (fp32; w NULL: 1); scale = s·rsqrt(mean(z²) + eps). */
+/* z = x, or bf16(x + residual), which goes to `sum` (it may lie where x or the residual does); t = z·w (fp32; w NULL: 1); scale = s·rsqrt(mean(z²) + eps),
+ * the sum of z² in fp32, as b200_rmsnorm_bf16 has it: a row whose sum passes the largest fp32 number reads as zeros. */
 int b200_rmsnorm_f8(void* q, float* scale, void* sum_or_null, const void* x, const void* residual_or_null, const void* w_or_null, int64_t rows, int64_t dim,
                     float eps, void* stream);
-/* gate_up rows are [gate(n) | up(n)], bf16; t = silu(gate)·up in fp32 (a silu below 2^-119 may be 0); scale = s. */
+/* gate_up rows are [gate(n) | up(n)], bf16; t = silu(gate)·up in fp32, silu within 2^-20 of its value for every gate (below 2^-119 it may be 0); scale = s. */
 int b200_silu_mul_f8(void* q, float* scale, const void* gate_up, int64_t rows, int64_t n, void* stream);
 /* out[rows, k] = value·scale, fp32. */
 int b200_f8_rows_dequant(float* out, const void* q, const float* scale, int64_t rows, int64_t k, void* stream);
@@ -221,7 +222,7 @@ typedef struct b200_f8_weight {
 } b200_f8_weight;
 
 /* y[rows, n] = bf16( x·Wᵀ + bias ) of rows in 8 bits: the products of 128 entries are summed in the tensor cores, scaled and added in fp32, rounded once.  The
- * magnitude of value sums · scales stays below 2^127.  How a sum is cut over CTAs depends on the number of rows. */
+ * magnitude of value sums · scales stays below 2^127; where a product of scales is below 2^-126, a block's sum may be off by 2^-125.  How a sum is cut over CTAs depends on the number of rows. */
 int b200_f8_linear_bf16(void* y, const void* q, const float* scale, const b200_f8_weight* w, const void* bias_or_null, int64_t rows, void* stream);
 /* Rows starts[e] … starts[e + 1] − 1 meet W[e] (starts int32 [experts + 1] on the device, not falling; none, or any number of rows to an expert); rows in front of the first
  * group and behind the last are zeros in y.  Up to 1 024 experts. */

@@ -7,7 +7,7 @@
 //
 // Warp-specialised, persistent over the tiles:
 //   warp 0   TMA: of every 128 bytes of k 128 rows of W and the tile's rows of x, into a ring of shared memory
-//   warp 1   one thread issues four products (K = 32 bytes) per 128 bytes
+//   warp 1   issues four products (K = 32 bytes) per 128 bytes, as a whole warp with one leading lane (umma_by)
 //   warp 2   8 bits: the products of x's and W's scales, NT of them for each block of 128 entries, fetched some blocks ahead
 //   warp 3   finds the CTA's tiles; rows of no group are zeroed
 //   warps 4 … 11   the sums: a warp has a quarter of the channels and half of the rows, as fragments of 8 × 8 (lane 4r + c: channel r, rows 2c and 2c + 1), so
@@ -105,10 +105,10 @@ __global__ void __launch_bounds__(kThreads, Form<NT>::per_sm) group_gemm_kernel(
   uint8_t* const sx = smem + ST * kWBytes;
   uint8_t* const done_tile = smem + F::ring;
   float* const factors = reinterpret_cast<float*>(done_tile + F::out_bytes);       // [AHEAD][NT]
-  uint64_t* const full = reinterpret_cast<uint64_t*>(factors + AHEAD * F::f_slot);   // [stages], a pair's first CTA's
+  uint64_t* const full = reinterpret_cast<uint64_t*>(factors + AHEAD * F::f_slot);   // [stages]
   uint64_t* const empty = full + ST;
   uint64_t* const sums_full = empty + ST;                                          // [slots]
-  uint64_t* const sums_empty = sums_full + 4;                                      // a pair's first CTA's
+  uint64_t* const sums_empty = sums_full + 4;
   TileRing ring(sums_empty + 4);
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(sums_empty + 4) + TileRing::bytes / 4;
   int* const gave_up = reinterpret_cast<int*>(tmem_slot + 1);
@@ -514,8 +514,9 @@ int launch(const GroupProduct& g, GemmArgs& p, int splits, cudaStream_t st) {
 // memory gives it; a CTA needs 0.25 (16 rows) to 0.5 µs (128) for 128 bytes of k, a wide one 0.49 (bf16 0.38 a pair), and something for a tile's end; two CTAs on an SM 1.45
 // times that each; partial tiles that meet cost 2 to 4.5 µs.  The rates are fitted to 189 calls — 1 to 4 096 rows, up to 20 000 over 8 to 64 experts, seven and five
 // matrices — in all the forms that can run: 13 of those calls take more than 5 % longer than in the best form, the worst 12 %.  For one of each, the way that is taken and,
-// in brackets, others: 200 × 4 096 × 14 336 33 µs in tiles of 128 rows and two CTAs to each (37, 64 and two; 42, 64 and four), 512 × 4 096 × 14 336 53 with 128 (55, wide), 768 × 4 096 × 4 096 22 wide
-// (34, 128), 512 × 2 048 × 2 048 11.1 with 64 (12.0, 32; 12.3, 128), 1 × 896 × 4 864 7.0 with eight CTAs to a tile (8.0, four).
+// in brackets, others: 200 × 4 096 × 14 336 33 µs in tiles of 128 rows and two CTAs to each (37, 64 and two; 42, 64 and four), 512 × 4 096 × 14 336 55 wide (53, 128: one of those that
+// are not cut best), 768 × 4 096 × 4 096 22 wide (34, 128), 512 × 2 048 × 2 048 11.1 with 64 (12.0, 32; 12.3, 128), 1 × 896 × 4 864 7.0 with eight CTAs to a tile (8.0, four).
+// b200_product_way tells the way that any call takes.
 struct Way {
   int rows, splits;   // rows 0: wide
 };

@@ -2,16 +2,16 @@
 //
 // x is the A operand here: a lane of tensor memory is a row of x, so that in 8 bits a summing thread — a row, one block of 128 channels — needs one factor for 128
 // sums.  With W as A (group_gemm.cu) factors differ from sum to sum: adding 128 entries of k for 128 × 256 sums took 620 to 660 cycles alone for 313 here, and
-// 4 096 × 28 672 × 4 096 took 754 µs for 465 (2.07 PFLOP/s; 530 in a run of them, under the power cap).  The roles of the warps are those of group_gemm.cu but for warp 3, which
-// finds the CTA's tiles; two slots of 256 columns of tensor memory.
-// 8 bits: a block of k takes some 950 cycles where its products need 512.  A slot goes around — products, 646 cycles until they are seen; factors, loads and sums, 450; back to
-// the issuing warp — and there is room for two; reading sums also holds the products up (a block's loads by 124 cycles), and x and W of 48 KB a block are
-// written to and read from shared memory in 768.  Tried and as slow or slower: pairs with 256 rows (32 KB a block; longer ways from CTA to CTA), four slots of 128
-// columns (the issue of four products alone takes 249 cycles), halves of a slot by themselves, sums in pairs or one by one, an earlier look at the next slot.
+// 4 096 × 28 672 × 4 096 took 754 µs for 465 (2.07 PFLOP/s; 530 in a run of them, under the power cap).  The roles of the warps are those of group_gemm.cu; two slots of 256
+// columns of tensor memory.
+// 8 bits: a block of k takes some 950 cycles where its products need 512.  What is known of them: a slot goes around — products, 646 cycles until they are seen; factors, loads
+// and sums, 450; back to the issuing warp — and there is room for two, so a block every 550 to 575; reading sums holds the products up (a block's loads by 124 cycles); x and W of
+// 48 KB a block are written to and read from shared memory in 768.  None of these is 950: the last 180 cycles are not accounted for.  Tried and
+// as slow or slower: pairs with 256 rows (32 KB a block; longer ways from CTA to CTA), four slots of 128 columns (the issue of four products alone takes 249 cycles), halves of a slot by themselves, sums in pairs or one by one, an earlier look at the next slot.
 // A pair in 8 bits ends groups in tiles of 256 rows: 2 048 rows with four of 32 experts each 146 µs for 125, and 4 096 × 4 096 × 4 096 82 for 75.
 // bf16: tensor memory sums over all of k; 4 096 × 4 096 × 4 096 93.5 µs (1.47 PFLOP/s).  A CTA by itself took 127 where a pair took 97.
 // A summing warp stores what it summed itself, 32 channels at a time through two kilobytes: with whole tiles handed to a storing warp the last one of a CTA came 5 µs
-// behind its sums, and their room is a stage of operands now.  With the tiles found by warp 3, ahead, that took 8 192 rows over 32 experts, 2 048 × 2 048, from 52.2 to
+// behind its sums, and their room is a stage of operands now.  With the tiles found by warp 3, ahead, that took 8 192 rows over 32 experts, as many for each, 2 048 × 2 048, from 52.2 to
 // 48.1 µs in 8 bits and 72 to 65.6 in bf16.
 #include "group_gemm.cuh"
 
